@@ -716,6 +716,99 @@ KOEMI_API int koemi_ep_collect(const int64_t *sorted_experts, const int64_t *seg
                      const uint64_t *peers, void *own, int64_t pairs, int64_t width, int64_t rank,
                      int64_t ranks, int64_t local_experts, int64_t capacity, int dtype, void *stream);
 
+/* ------------------------------------------------ operators of a training step
+ * Equal inputs give equal bits: no floating-point atomics. */
+
+/* Gated linear recurrence from raw projections ([batch, length, 2 F]: p | c,
+ * F = features):
+ *   s = sigmoid(p), a = lo + (hi - lo) s, k = tanh(c),
+ *   h_t = a_t h' + (1 - a_t) k_t, h' = 0 where restart, else h_{t-1};
+ * a position that is not valid keeps the state. projections and states
+ * ([batch, length, F]) are dtype (f32, f16, bf16); initial ([batch, F], NULL:
+ * zeros), final_state and all arithmetic are fp32. valid and restart are
+ * [batch, length] bytes or NULL. carries (NULL for inference) receives the
+ * state before every 64th position, [batch, ceil(length / 64), F], which the
+ * backward needs. Nothing is written when a size is 0. The gates are those of
+ * BoundedRecurrentState (model/memory.py:22-26). */
+KOEMI_API int koemi_dense_gated_recurrence_forward(const void *projections, const float *initial,
+                                                   const uint8_t *valid, const uint8_t *restart, void *states,
+                                                   float *final_state, float *carries, int64_t batch, int64_t length,
+                                                   int64_t features, float minimum_retention,
+                                                   float maximum_retention, int dtype, void *stream);
+/* Its gradient: grad_states (dtype) and grad_final (fp32) may be NULL (zero);
+ * grad_projections is dtype, grad_initial fp32 or NULL. */
+KOEMI_API int koemi_dense_gated_recurrence_backward(const void *projections, const uint8_t *valid,
+                                                    const uint8_t *restart, const float *carries,
+                                                    const void *grad_states, const float *grad_final,
+                                                    void *grad_projections, float *grad_initial, int64_t batch,
+                                                    int64_t length, int64_t features, float minimum_retention,
+                                                    float maximum_retention, int dtype, void *stream);
+
+/* Learned route of a training step over gate logits [tokens, expert_count]
+ * (f32, f16, bf16): expert_ids [tokens, top_k] (int64) are the top_k largest
+ * logits of a row, ties to the lowest id; weights (fp32) their softmax
+ * probabilities, divided by their sum under renormalize; counts
+ * [expert_count] (int64) the pairs per expert; balance (one float)
+ *   E sum_e (mean probability of e over the rows)(counts_e / sum counts),
+ * as RouterStatistics.balance_loss; slope [expert_count] is d balance /
+ * d probability of any row, kept for the backward. Rows with valid == 0, and
+ * rows whose logits are all -inf, take no part (ids -1, weights 0).
+ * expert_count <= 4096, top_k <= min(expert_count, 256). */
+KOEMI_API size_t koemi_moe_route_learned_workspace(int64_t tokens, int64_t expert_count);
+KOEMI_API int koemi_moe_route_learned_forward(const void *logits, const uint8_t *valid, int64_t *expert_ids,
+                                              float *weights, int64_t *counts, float *balance, float *slope,
+                                              int64_t tokens, int64_t expert_count, int64_t top_k, int renormalize,
+                                              int dtype, void *workspace, size_t workspace_bytes, void *stream);
+/* Gradient with respect to the logits: grad_weights [tokens, top_k] and
+ * grad_balance (one float) may be NULL (zero). */
+KOEMI_API int koemi_moe_route_learned_backward(const void *logits, const int64_t *expert_ids, const float *weights,
+                                               const float *grad_weights, const float *grad_balance,
+                                               const float *slope, void *grad_logits, int64_t tokens,
+                                               int64_t expert_count, int64_t top_k, int renormalize, int dtype,
+                                               void *stream);
+
+/* Clipped policy loss with a KL term over vocabulary logits (f32, f16, bf16).
+ * Row r of the logits starts at (r / inner_rows) * outer_stride +
+ * (r % inner_rows) * inner_stride elements; its entries are contiguous.
+ *   lp = l[target] - lse(l), q = exp(lp - old), d = reference - lp,
+ *   loss = mean over valid rows of -min(q A, clip(q, 1 - clip_low,
+ *          1 + clip_high) A) + kl_weight (exp(d) - d - 1),
+ *   kl = mean of exp(d) - d - 1 (0 with reference_log_probs NULL).
+ * log_probs [rows] is 0 on rows that are not valid and NaN where a target is
+ * outside [0, vocab). lse and slopes [rows] are kept for the backward.
+ * grad_logits ([rows, vocab], dtype, contiguous, 16-byte aligned; NULL: not
+ * wanted) receives d loss / d logits in the same pass. */
+KOEMI_API size_t koemi_think_policy_loss_workspace(void);
+KOEMI_API int koemi_think_policy_loss_forward(const void *logits, int64_t rows, int64_t vocab, int64_t inner_rows,
+                                              int64_t outer_stride, int64_t inner_stride, const int64_t *targets,
+                                              const float *old_log_probs, const float *advantages,
+                                              const float *reference_log_probs, const uint8_t *valid, float clip_low,
+                                              float clip_high, float kl_weight, float *loss, float *kl,
+                                              float *log_probs, float *lse, float *slopes, void *grad_logits,
+                                              int dtype, void *workspace, size_t workspace_bytes, void *stream);
+/* d loss / d logits times *grad_loss from the logits, lse and slopes (where
+ * the forward did not write it, and for f16, whose gradients underflow before
+ * the factor of a scaled loss). */
+KOEMI_API int koemi_think_policy_loss_backward(const void *logits, int64_t rows, int64_t vocab, int64_t inner_rows,
+                                               int64_t outer_stride, int64_t inner_stride, const int64_t *targets,
+                                               const uint8_t *valid, const float *lse, const float *slopes,
+                                               const float *grad_loss, void *grad_logits, int dtype, void *stream);
+/* grad_logits *= *factor in place; a factor of one reads and writes nothing. */
+KOEMI_API int koemi_think_policy_loss_scale(void *grad_logits, int64_t count, const float *factor, int dtype,
+                                            void *stream);
+
+/* Global 2-norm of `count` tensors and clipping: norm = sqrt(sum g^2) (one
+ * float), outputs[i] = gradients[i] * min(1, max_norm / (norm + 1e-6)).
+ * gradients and outputs are HOST arrays of device addresses (outputs NULL:
+ * norm only; outputs[i] may equal gradients[i], else they must not overlap),
+ * elements and dtypes (f32, f16, bf16) host arrays too; all are read before
+ * the call returns. Squares are summed in fp32 per 16384 elements and in fp64
+ * beyond. */
+KOEMI_API size_t koemi_core_clip_gradients_workspace(const int64_t *elements, int64_t count);
+KOEMI_API int koemi_core_clip_gradients(const uint64_t *gradients, const uint64_t *outputs, const int64_t *elements,
+                                        const int32_t *dtypes, int64_t count, float max_norm, float *norm,
+                                        void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

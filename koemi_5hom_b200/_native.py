@@ -129,6 +129,20 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "koemi_ep_collect": (_int, (_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p)),
     "koemi_moe_combine_residual_rmsnorm": (
         _int, (_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _f, _int, _p)),
+    "koemi_dense_gated_recurrence_forward": (_int, (_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _f, _f, _int, _p)),
+    "koemi_dense_gated_recurrence_backward": (_int, (_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _f, _f, _int, _p)),
+    "koemi_moe_route_learned_workspace": (_sz, (_i64, _i64)),
+    "koemi_moe_route_learned_forward": (
+        _int, (_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _int, _p, _sz, _p)),
+    "koemi_moe_route_learned_backward": (_int, (_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _int, _p)),
+    "koemi_think_policy_loss_workspace": (_sz, ()),
+    "koemi_think_policy_loss_forward": (
+        _int, (_p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _f, _f, _f, _p, _p, _p, _p, _p, _p, _int, _p, _sz, _p)),
+    "koemi_think_policy_loss_backward": (
+        _int, (_p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _int, _p)),
+    "koemi_think_policy_loss_scale": (_int, (_p, _i64, _p, _int, _p)),
+    "koemi_core_clip_gradients_workspace": (_sz, (_p, _i64)),
+    "koemi_core_clip_gradients": (_int, (_p, _p, _p, _p, _i64, _f, _p, _p, _sz, _p)),
 }
 
 

@@ -1,0 +1,214 @@
+// Core front: global 2-norm of many gradient tensors, and clipping.
+//
+//   norm = sqrt(sum over all tensors of g^2)
+//   out = g min(1, max_norm / (norm + 1e-6))
+//
+// The tensors travel in the kernel's parameters (up to kMaxTensors per
+// launch), cut into chunks of kChunkElements; a chunk's sum of squares is one
+// partial, and every CTA of the second kernel adds all partials in the same
+// fixed order, so equal inputs give equal bits. In place, a factor of one
+// writes nothing.
+#include <cstring>
+
+#include "vec.cuh"
+
+namespace koemi {
+namespace {
+
+constexpr int kMaxTensors = 1000;          // 24 bytes each: the parameters stay below 32 KB
+constexpr int64_t kChunkElements = 16384;  // elements of one partial sum
+constexpr int kClipThreads = 256;
+constexpr int kClipBlocks = 592;
+
+struct ClipTable {
+    const void *in[kMaxTensors];
+    void *out[kMaxTensors];
+    uint32_t first_chunk[kMaxTensors + 1];
+    uint32_t tail_type[kMaxTensors];  // elements of the last chunk (1..kChunkElements) * 4 + type code
+    int count;
+};
+
+struct Chunk {
+    int tensor;
+    int64_t first;
+    int elements;
+    int type;
+};
+
+__device__ __forceinline__ Chunk chunk_of(const ClipTable &table, uint32_t chunk) {
+    int lo = 0, hi = table.count;  // first_chunk[lo] <= chunk < first_chunk[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (table.first_chunk[mid] <= chunk) {
+            lo = mid;
+        } else {
+            hi = mid;
+        }
+    }
+    Chunk c;
+    c.tensor = lo;
+    c.first = int64_t(chunk - table.first_chunk[lo]) * kChunkElements;
+    c.type = table.tail_type[lo] & 3;
+    c.elements = chunk + 1 == table.first_chunk[lo + 1] ? int(table.tail_type[lo] >> 2) : int(kChunkElements);
+    return c;
+}
+
+template <typename T>
+__device__ float chunk_squares(const T *in, int elements) {
+    float sum = 0.0f;
+    for (int i = threadIdx.x; i < elements; i += kClipThreads) {
+        const float v = to_acc(in[i]);
+        sum = fmaf(v, v, sum);
+    }
+    return sum;
+}
+
+template <typename T>
+__device__ void chunk_scale(const T *in, T *out, int elements, float factor) {
+    for (int i = threadIdx.x; i < elements; i += kClipThreads) out[i] = from_acc<T>(to_acc(in[i]) * factor);
+}
+
+__global__ __launch_bounds__(kClipThreads) void clip_squares_kernel(const __grid_constant__ ClipTable table,
+                                                                    uint32_t chunks, float *__restrict__ partials) {
+    __shared__ float sums[kClipThreads / 32];
+    for (uint32_t index = blockIdx.x; index < chunks; index += gridDim.x) {
+        const Chunk c = chunk_of(table, index);
+        float sum;
+        if (c.type == KOEMI_F32) {
+            sum = chunk_squares(static_cast<const float *>(table.in[c.tensor]) + c.first, c.elements);
+        } else if (c.type == KOEMI_F16) {
+            sum = chunk_squares(static_cast<const __half *>(table.in[c.tensor]) + c.first, c.elements);
+        } else {
+            sum = chunk_squares(static_cast<const __nv_bfloat16 *>(table.in[c.tensor]) + c.first, c.elements);
+        }
+        sum = warp_sum(sum);
+        if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float all = 0.0f;
+            for (int w = 0; w < kClipThreads / 32; ++w) all += sums[w];
+            partials[index] = all;
+        }
+        __syncthreads();
+    }
+}
+
+// The sum of all partials, the same bits in every CTA.
+__device__ double sum_partials(const float *partials, int64_t count) {
+    __shared__ double sums[kClipThreads / 32];
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < count; i += kClipThreads) sum += partials[i];
+#pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < kClipThreads / 32; ++w) sum += sums[w];
+    return sum;
+}
+
+__global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const __grid_constant__ ClipTable table,
+                                                                  uint32_t chunks, const float *__restrict__ partials,
+                                                                  int64_t partial_count, float max_norm,
+                                                                  float *__restrict__ norm_out) {
+    const float norm = static_cast<float>(sqrt(sum_partials(partials, partial_count)));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+    float factor = max_norm / (norm + 1e-6f);
+    if (factor > 1.0f) factor = 1.0f;  // a NaN stays
+    for (uint32_t index = blockIdx.x; index < chunks; index += gridDim.x) {
+        const Chunk c = chunk_of(table, index);
+        const void *in = table.in[c.tensor];
+        void *out = table.out[c.tensor];
+        if (out == nullptr || (factor == 1.0f && in == out)) continue;
+        if (c.type == KOEMI_F32) {
+            chunk_scale(static_cast<const float *>(in) + c.first, static_cast<float *>(out) + c.first, c.elements, factor);
+        } else if (c.type == KOEMI_F16) {
+            chunk_scale(static_cast<const __half *>(in) + c.first, static_cast<__half *>(out) + c.first, c.elements, factor);
+        } else {
+            chunk_scale(static_cast<const __nv_bfloat16 *>(in) + c.first, static_cast<__nv_bfloat16 *>(out) + c.first,
+                        c.elements, factor);
+        }
+    }
+}
+
+int64_t chunk_count(int64_t elements) { return ceil_div(elements, kChunkElements); }
+
+// Fills `table` with tensors from `first` on; returns one past the last.
+int64_t fill_table(ClipTable &table, const uint64_t *in, const uint64_t *out, const int64_t *elements,
+                   const int32_t *dtypes, int64_t first, int64_t count) {
+    uint32_t chunk = 0;
+    int n = 0;
+    int64_t i = first;
+    for (; i < count && n < kMaxTensors; ++i) {
+        if (elements[i] == 0) continue;
+        const int64_t chunks = chunk_count(elements[i]);
+        if (chunk + chunks > int64_t(1) << 31) break;
+        table.in[n] = reinterpret_cast<const void *>(in[i]);
+        table.out[n] = out == nullptr ? nullptr : reinterpret_cast<void *>(out[i]);
+        table.first_chunk[n] = chunk;
+        table.tail_type[n] = static_cast<uint32_t>(elements[i] - (chunks - 1) * kChunkElements) * 4 + dtypes[i];
+        chunk += static_cast<uint32_t>(chunks);
+        ++n;
+    }
+    table.first_chunk[n] = chunk;
+    table.count = n;
+    return i;
+}
+
+}  // namespace
+}  // namespace koemi
+
+using namespace koemi;
+
+extern "C" size_t koemi_core_clip_gradients_workspace(const int64_t *elements, int64_t count) {
+    if (elements == nullptr || count < 0) return 0;
+    int64_t chunks = 0;
+    for (int64_t i = 0; i < count; ++i) chunks += elements[i] > 0 ? chunk_count(elements[i]) : 0;
+    return static_cast<size_t>(chunks) * sizeof(float);
+}
+
+extern "C" int koemi_core_clip_gradients(const uint64_t *gradients, const uint64_t *outputs, const int64_t *elements,
+                                         const int32_t *dtypes, int64_t count, float max_norm, float *norm,
+                                         void *workspace, size_t workspace_bytes, void *stream) {
+    clear_error();
+    if (count < 0) return fail(KOEMI_ERR_INVALID, "count must be non-negative");
+    if (!(max_norm >= 0.0f)) return fail(KOEMI_ERR_INVALID, "max_norm must be non-negative");
+    if (norm == nullptr || (count > 0 && (gradients == nullptr || elements == nullptr || dtypes == nullptr))) {
+        return fail(KOEMI_ERR_INVALID, "norm, gradients, elements and dtypes must be non-NULL");
+    }
+    int64_t chunks = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (elements[i] < 0 || elements[i] > int64_t(1) << 44) return fail(KOEMI_ERR_INVALID, "tensor %lld has a bad size", static_cast<long long>(i));
+        if (dtypes[i] != KOEMI_F32 && dtypes[i] != KOEMI_F16 && dtypes[i] != KOEMI_BF16) {
+            return fail(KOEMI_ERR_INVALID, "tensor %lld has an unsupported dtype %d", static_cast<long long>(i), dtypes[i]);
+        }
+        if (elements[i] > 0 && (gradients[i] == 0 || (outputs != nullptr && outputs[i] == 0))) {
+            return fail(KOEMI_ERR_INVALID, "tensor %lld has no data", static_cast<long long>(i));
+        }
+        chunks += chunk_count(elements[i]);
+    }
+    if (workspace_bytes < chunks * sizeof(float) || (chunks > 0 && workspace == nullptr)) {
+        return fail(KOEMI_ERR_WORKSPACE, "the clipping workspace is smaller than koemi_core_clip_gradients_workspace()");
+    }
+    cudaStream_t s = as_stream(stream);
+    float *partials = static_cast<float *>(workspace);
+    ClipTable table;
+    int64_t done = 0;
+    for (int64_t i = 0; i < count;) {
+        i = fill_table(table, gradients, outputs, elements, dtypes, i, count);
+        const uint32_t n = table.first_chunk[table.count];
+        if (n == 0) continue;
+        clip_squares_kernel<<<n < kClipBlocks ? n : kClipBlocks, kClipThreads, 0, s>>>(table, n, partials + done);
+        KOEMI_LAUNCH_CHECK();
+        done += n;
+    }
+    int64_t i = 0;
+    do {
+        i = fill_table(table, gradients, outputs, elements, dtypes, i, outputs == nullptr ? 0 : count);
+        const uint32_t n = table.first_chunk[table.count];
+        const uint32_t blocks = n < 1 ? 1 : n < kClipBlocks ? n : kClipBlocks;
+        clip_scale_kernel<<<blocks, kClipThreads, 0, s>>>(table, n, partials, done, max_norm, norm);
+        KOEMI_LAUNCH_CHECK();
+    } while (outputs != nullptr && i < count);
+    return KOEMI_OK;
+}

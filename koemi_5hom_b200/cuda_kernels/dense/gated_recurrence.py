@@ -1,0 +1,95 @@
+"""Dense front: the gated linear recurrence of a HERM block from raw projections.
+
+``gated_recurrence`` takes the gate GEMM's output (retention | candidate, the
+packed layout of ``gates_weight``) and runs the bounded gates
+(src/koemi/model/memory.py:22-26), the padding masks, the restarts of packed
+documents and the affine scan (model/scan.py:17-30) in one kernel, forward and
+backward. There is no CPU fallback.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from koemi_5hom_b200.cuda_kernels import _training
+from koemi_5hom_b200.cuda_kernels.dense.affine_scan import (DenseCudaUnavailableError, DenseCudaValidationError,
+                                                            _load_library, native_cuda_available)
+
+__all__ = ["gated_recurrence"]
+
+_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def gated_recurrence(projections: Tensor, initial: Tensor | None = None, *, valid: Tensor | None = None,
+                     restart: Tensor | None = None, minimum_retention: float = 2.0 ** -8,
+                     maximum_retention: float = 1.0 - 2.0 ** -8) -> tuple[Tensor, Tensor]:
+    """Run ``h_t = a_t h' + (1 - a_t) tanh(c_t)`` and return (states, final state).
+
+    ``projections`` is ``[batch, length, 2 F]`` (p | c; f32, bf16 or f16) and
+    ``a = minimum + (maximum - minimum) sigmoid(p)``; ``h'`` is ``h_{t-1}``, or
+    zero where ``restart`` (bool ``[batch, length]``: the first position of a
+    packed document). A position where ``valid`` (same shape) is false keeps
+    the state, whatever its projections hold. ``initial`` is fp32 ``[batch, F]``
+    (zeros when omitted). States have the projections' dtype; the running state
+    and the returned final state are fp32. Differentiable to first order in
+    ``projections`` and ``initial``; a single token is ``length == 1``.
+    """
+    _validate(projections, initial, valid, restart, minimum_retention, maximum_retention)
+    _load_library(projections.device)
+    projections = projections.contiguous()
+    initial, valid, restart = (None if t is None else t.contiguous() for t in (initial, valid, restart))
+    if projections.shape[1] == 0:
+        features = projections.shape[2] // 2
+        start = projections.new_zeros((projections.shape[0], features), dtype=torch.float32) if initial is None else initial.clone()
+        return projections[..., :features].contiguous(), start
+    if torch.is_grad_enabled() and (projections.requires_grad or (initial is not None and initial.requires_grad)):
+        return _GatedRecurrence.apply(projections, initial, valid, restart, minimum_retention, maximum_retention)
+    return _training.gated_recurrence(projections, initial, valid, restart, minimum_retention, maximum_retention, False)[:2]
+
+
+class _GatedRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(context, projections, initial, valid, restart, low, high):
+        states, final, carries = _training.gated_recurrence(projections, initial, valid, restart, low, high, True)
+        context.save_for_backward(projections, valid, restart, carries)
+        context.bounds = low, high
+        context.set_materialize_grads(False)
+        return states, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(context, grad_states, grad_final):
+        if grad_states is None and grad_final is None:
+            return None, None, None, None, None, None
+        projections, valid, restart, carries = context.saved_tensors
+        grad_states, grad_final = (None if g is None else g.contiguous() for g in (grad_states, grad_final))
+        grad_projections, grad_initial = _training.gated_recurrence_backward(
+            projections, valid, restart, carries, grad_states, grad_final, *context.bounds)
+        return grad_projections, grad_initial if context.needs_input_grad[1] else None, None, None, None, None
+
+
+def _validate(projections, initial, valid, restart, low, high) -> None:
+    def fail(message: str) -> None:
+        raise DenseCudaValidationError(message)
+
+    for name, value in (("projections", projections), ("initial", initial), ("valid", valid), ("restart", restart)):
+        if not isinstance(value, Tensor) and (value is not None or name == "projections"):
+            raise TypeError(f"{name} must be a torch.Tensor")
+    if projections.ndim != 3 or projections.shape[2] % 2:
+        fail("projections must have shape [batch, length, 2 * features]")
+    if projections.dtype not in _DTYPES:
+        fail(f"unsupported CUDA dtype(s): {projections.dtype}")
+    batch, length, double = projections.shape
+    if initial is not None and (initial.shape != (batch, double // 2) or initial.dtype != torch.float32):
+        fail(f"initial must be float32 with shape {(batch, double // 2)}, got {initial.dtype} {tuple(initial.shape)}")
+    for name, mask in (("valid", valid), ("restart", restart)):
+        if mask is not None and (mask.shape != (batch, length) or mask.dtype != torch.bool):
+            fail(f"{name} must be bool with shape {(batch, length)}, got {mask.dtype} {tuple(mask.shape)}")
+    if not 0.0 < low <= high < 1.0:
+        fail("retention bounds must satisfy 0 < minimum <= maximum < 1")
+    if not projections.is_cuda and not native_cuda_available():
+        raise DenseCudaUnavailableError("native gated recurrence requires torch CUDA support, a CUDA device, and the built kernel library")
+    for value in (projections, initial, valid, restart):
+        if value is not None and (not value.is_cuda or value.device != projections.device):
+            fail(f"all recurrence tensors must use one CUDA device; found {projections.device} and {value.device}")

@@ -28,6 +28,7 @@ from torch import Tensor
 
 from koemi_5hom_b200 import _native
 from koemi_5hom_b200.cuda_kernels import _ops
+from koemi_5hom_b200.cuda_kernels.moe.learned_route import LearnedRoute, route_learned_topk
 
 
 class CudaMoeUnavailableError(RuntimeError):
@@ -252,9 +253,11 @@ def combine_topk(expert_outputs: Tensor, sorted_rows: Tensor, segment_offsets: T
 __all__ = [
     "CudaMoeUnavailableError",
     "CudaMoeValidationError",
+    "LearnedRoute",
     "combine_topk",
     "grouped_expert_mlp_inference",
     "load_native_extension",
     "permute_topk",
+    "route_learned_topk",
     "route_topk_valid",
 ]
