@@ -79,13 +79,22 @@ int encode_tensor_map(CUtensorMap *map, CUtensorMapDataType type, uint32_t rank,
         return fail(KOEMI_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
     }
     cuuint32_t element_strides[5] = {1, 1, 1, 1, 1};
-    CUresult result = g_encode_tiled(map, type, rank, const_cast<void *>(base),
-                                     reinterpret_cast<const cuuint64_t *>(dims),
-                                     reinterpret_cast<const cuuint64_t *>(strides_bytes),
-                                     reinterpret_cast<const cuuint32_t *>(box), element_strides,
-                                     CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&] {
+        return g_encode_tiled(map, type, rank, const_cast<void *>(base), reinterpret_cast<const cuuint64_t *>(dims),
+                              reinterpret_cast<const cuuint64_t *>(strides_bytes),
+                              reinterpret_cast<const cuuint32_t *>(box), element_strides,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult result = encode();
+    if (result == CUDA_ERROR_INVALID_CONTEXT) {
+        // A thread whose first CUDA call this is (an autograd thread, say) has
+        // no current context yet: binding its device makes the primary one current.
+        int device = 0;
+        KOEMI_CUDA_TRY(cudaGetDevice(&device));
+        KOEMI_CUDA_TRY(cudaSetDevice(device));
+        result = encode();
+    }
     if (result != CUDA_SUCCESS) {
         return fail(KOEMI_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", int(result));
     }

@@ -8,6 +8,7 @@ test derives its count where it uses it.
 from __future__ import annotations
 
 import math
+import threading
 
 import pytest
 import torch
@@ -225,6 +226,16 @@ def test_recurrence_bits_repeat_also_on_another_stream(shape, cuda):
     torch.cuda.synchronize()
     for other in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+def test_recurrence_as_a_threads_first_cuda_call(cuda):
+    """A thread without a current context (an autograd thread is one) can encode tensor maps."""
+    x, h0, *_ = recurrence_case(2, 100, 64, torch.bfloat16, 16, False, cuda)
+    expected, got = gated_recurrence(x, h0), []
+    thread = threading.Thread(target=lambda: got.extend(gated_recurrence(x, h0)))
+    thread.start()
+    thread.join()
+    assert len(got) == 2 and all(torch.equal(a, b) for a, b in zip(got, expected))
 
 
 def test_recurrence_offsets_past_32_bits(cuda):
