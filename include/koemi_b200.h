@@ -727,7 +727,7 @@ KOEMI_API int koemi_ep_collect(const int64_t *sorted_experts, const int64_t *seg
  * ([batch, length, F]) are dtype (f32, f16, bf16); initial ([batch, F], NULL:
  * zeros), final_state and all arithmetic are fp32. valid and restart are
  * [batch, length] bytes or NULL. carries (NULL for inference) receives the
- * state before every 64th position, [batch, ceil(length / 64), F], which the
+ * state before every 128th position, [batch, ceil(length / 128), F], which the
  * backward needs. Nothing is written when a size is 0. The gates are those of
  * BoundedRecurrentState (model/memory.py:22-26). */
 KOEMI_API int koemi_dense_gated_recurrence_forward(const void *projections, const float *initial,

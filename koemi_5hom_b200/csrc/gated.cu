@@ -7,7 +7,7 @@
 //
 // projections are [batch, length, 2 F] (p | c), states [batch, length, F];
 // the running state is fp32. The forward can leave the state before every
-// 64th position in `carries`, from which the backward recomputes the states
+// 128th position in `carries`, from which the backward recomputes the states
 // it needs on chip instead of reading them:
 //
 //   adj_t = g_t + x_t,  x_{t-1} = a_t adj_t (0 at a restart)
@@ -15,26 +15,31 @@
 //   dc_t = adj_t (1 - a_t) (1 - k_t^2),  d_initial = x_{-1}
 //
 // Every step is an affine map of the state (forward) or of x (backward), so a
-// tile of 64 positions x 64 features composes into one map per feature. A CTA
-// of 8 warps takes a tile: warp w holds rows [8 w, 8 w + 8) in registers, a
-// lane two features; the warps' maps meet in shared memory. A chain (one
-// batch row, 64 features) is walked by a cluster of 1 to 8 CTAs, a wave of as
-// many neighbouring tiles at a time: every CTA stores its tile's map into the
-// other CTAs' shared memory, and one cluster barrier later each folds the
-// maps in front of its tile onto the carry and replays its rows. Nothing is
-// exchanged through global memory, no CTA waits for one outside its cluster,
-// and the order of every sum is fixed, so equal inputs give equal bits.
+// tile of 128 positions x 32 features composes into one map per feature. A
+// CTA takes a tile: each half warp holds 8 neighbouring rows in registers, a
+// lane two features, and leaves its rows' map in shared memory; one warp, a
+// thread per feature, then walks these maps from the carry and leaves each
+// half warp the value its rows start from. A chain (one batch row, 32
+// features) is walked by a cluster of 1 to 8 CTAs, a wave of as many
+// neighbouring tiles at a time: the walking warps store their tiles' maps
+// into each other's shared memory and fold the maps of the tiles in front of
+// theirs onto the carry. Nothing is exchanged through global memory, no CTA
+// waits for one outside its cluster, and the order of every sum is fixed, so
+// equal inputs give equal bits.
 #include "common.cuh"
 
 namespace koemi {
 namespace {
 
-constexpr int kSegment = 64;  // positions of a tile, and between two carries
-constexpr int kTileFeatures = 64;
-constexpr int kTileWarps = 8;
-constexpr int kTileThreads = kTileWarps * 32;
-constexpr int kTileRows = kSegment / kTileWarps;
+constexpr int kSegment = 128;  // positions of a tile, and between two carries
+constexpr int kTileFeatures = 32;
+constexpr int kWarps = 8;
+constexpr int kTileThreads = kWarps * 32;
+constexpr int kBlocks = 2 * kWarps;             // half warps of a CTA
+constexpr int kRows = kSegment / kBlocks;       // rows of a half warp
 constexpr int kMaxCluster = 8;
+constexpr int kForwardResident = 4;  // CTAs per SM (registers, and shared memory of the 16-bit types)
+constexpr int kBackwardResident = 2;
 constexpr int kShortLength = 16;  // up to here one thread walks a lane
 
 struct GatedShape {
@@ -46,6 +51,11 @@ struct GatedShape {
 __device__ __forceinline__ float min_nan(float a, float b) {
     float r;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 __device__ __forceinline__ float ex2_approx(float x) {
@@ -161,27 +171,91 @@ __global__ void gated_backward_lane_kernel(GatedShape shape, const T *__restrict
 
 // ------------------------------------------------------------------ tiles
 
+// Two features at once: Blackwell's packed fp32 instructions issue once for
+// both, and the tile kernels are bound by issue slots next to HBM.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, c, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 r, a, b, c;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 r, a, b;\n\t"
+        "mov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 r, a, b;\n\t"
+        "mov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, both(-1.0f), a); }
+
+// s and k of gate_of for two features; p and c are already clamped (p >= -40,
+// c <= 20).
+template <typename T>
+__device__ __forceinline__ void gates_of(float2 p, float2 c, float2 &s, float2 &k) {
+    constexpr float kLog2e = 1.4426950408889634f;
+    const float2 ep = mul2(p, both(-kLog2e)), ec = mul2(c, both(2.0f * kLog2e));
+    const float2 yp = add2(make_float2(ex2_approx(ep.x), ex2_approx(ep.y)), both(1.0f));
+    const float2 yc = add2(make_float2(ex2_approx(ec.x), ex2_approx(ec.y)), both(1.0f));
+    const float2 product = mul2(yp, yc);
+    const float2 r = make_float2(rcp_approx(product.x), rcp_approx(product.y));
+    s = mul2(r, yc);
+    k = fma2(mul2(r, yp), both(-2.0f), both(1.0f));
+    if constexpr (sizeof(T) == 4) {
+        const float2 z = mul2(c, c);
+        float2 series = fma2(z, both(62.0f / 2835.0f), both(-17.0f / 315.0f));
+        series = fma2(z, series, both(2.0f / 15.0f));
+        series = fma2(z, series, both(-1.0f / 3.0f));
+        series = fma2(mul2(c, z), series, c);
+        if (z.x < 0.0625f) k.x = series.x;
+        if (z.y < 0.0625f) k.y = series.y;
+    }
+}
+
+// Two features of a projection row in shared memory, clamped from below (p)
+// or above (c); a NaN stays.
+template <bool kBelow>
+__device__ __forceinline__ float2 load_clamped(const __nv_bfloat16 *at) {
+    const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(at);
+    return __bfloat1622float2(kBelow ? __hmax2_nan(v, __float2bfloat162_rn(-40.0f)) : __hmin2_nan(v, __float2bfloat162_rn(20.0f)));
+}
+template <bool kBelow>
+__device__ __forceinline__ float2 load_clamped(const __half *at) {
+    const __half2 v = *reinterpret_cast<const __half2 *>(at);
+    return __half22float2(kBelow ? __hmax2_nan(v, __float2half2_rn(-40.0f)) : __hmin2_nan(v, __float2half2_rn(20.0f)));
+}
+template <bool kBelow>
+__device__ __forceinline__ float2 clamped(float2 v) {
+    return kBelow ? make_float2(max_nan(v.x, -40.0f), max_nan(v.y, -40.0f)) : make_float2(min_nan(v.x, 20.0f), min_nan(v.y, 20.0f));
+}
+template <bool kBelow>
+__device__ __forceinline__ float2 load_clamped(const float *at) {
+    return clamped<kBelow>(*reinterpret_cast<const float2 *>(at));
+}
+
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void store_remote(void *local, uint32_t rank, float4 v) {
-    uint32_t address;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(address) : "r"(smem_addr(local)), "r"(rank));
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(address), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-                 : "memory");
-}
-
-// A map v -> m v + n of two features, {m.x, m.y, n.x, n.y}. m is exactly 0
-// only where a restart drops v, and then v is not multiplied (it may be a
-// NaN); a product that underflows stays at the smallest positive number.
-__device__ __forceinline__ float apply(float m, float n, float v) { return m == 0.0f ? n : fmaf(m, v, n); }
-__device__ __forceinline__ float chain(float m, float n) {
-    return m == 0.0f || n == 0.0f ? 0.0f : fmaxf(m * n, 1.4e-45f);
-}
-// first, then second
-__device__ __forceinline__ float4 compose(float4 first, float4 second) {
-    return make_float4(chain(second.x, first.x), chain(second.y, first.y), apply(second.x, second.z, first.z),
-                       apply(second.y, second.w, first.w));
+// Stores 8 bytes into CTA `rank`'s copy of `local` and counts them on its copy
+// of `bar`. Unlike a plain remote store and a barrier it needs no release,
+// which would wait for the warp's global stores.
+__device__ __forceinline__ void store_to_rank(float2 *local, uint64_t *bar, int rank, float2 v) {
+    asm volatile(
+        "{\n\t.reg .b32 a, b;\n\tmapa.shared::cluster.u32 a, %0, %2;\n\tmapa.shared::cluster.u32 b, %1, %2;\n\t"
+        "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [a], {%3, %4}, [b];\n\t}" ::"r"(smem_addr(local)),
+        "r"(smem_addr(bar)), "r"(rank), "f"(v.x), "f"(v.y)
+        : "memory");
 }
 
 template <typename T>
@@ -214,472 +288,518 @@ __device__ __forceinline__ void store_two(__half *p, float2 v) {
 }
 __device__ __forceinline__ void store_two(float *p, float2 v) { *reinterpret_cast<float2 *>(p) = v; }
 
-// Where a lane's two features are. TMA tiles: features 2 l and 2 l + 1 (one
-// 4- or 8-byte access, the width is a multiple of 8 bytes at least). Without
-// TMA: l and l + 32, single elements, so that a warp's accesses stay
-// contiguous at any alignment.
+// Where a lane's two features are; lanes 16 to 31 hold the same features of
+// other rows. TMA tiles: features 2 l and 2 l + 1 (one 4- or 8-byte access;
+// the width is a multiple of 4 features at least). Without TMA: l and l + 16,
+// single elements, so that accesses stay contiguous at any alignment.
 template <bool kTma>
 struct LaneFeatures {
-    int64_t x, y;
+    int64_t x;
     bool x_in, y_in;
     __device__ LaneFeatures(int64_t first, int lane, int64_t features) {
-        x = first + (kTma ? 2 * lane : lane);
-        y = kTma ? x + 1 : x + 32;
+        x = first + (kTma ? 2 * (lane & 15) : lane & 15);
         x_in = x < features;
-        y_in = y < features;
+        y_in = x + (kTma ? 1 : 16) < features;
     }
+    // `row` points at feature x of a row
     template <typename T>
     __device__ __forceinline__ float2 load(const T *row) const {
-        if (kTma) return x_in ? load_two(row + x) : make_float2(0.0f, 0.0f);
-        return make_float2(x_in ? to_acc(row[x]) : 0.0f, y_in ? to_acc(row[y]) : 0.0f);
+        return make_float2(x_in ? to_acc(row[0]) : 0.0f, y_in ? to_acc(row[kTma ? 1 : 16]) : 0.0f);
     }
     template <typename T>
     __device__ __forceinline__ void store(T *row, float2 v) const {
         if (kTma) {
-            if (x_in) store_two(row + x, v);
+            if (x_in) store_two(row, v);
         } else {
-            if (x_in) row[x] = from_acc<T>(v.x);
-            if (y_in) row[y] = from_acc<T>(v.y);
+            if (x_in) row[0] = from_acc<T>(v.x);
+            if (y_in) row[16] = from_acc<T>(v.y);
         }
-    }
-    // fp32 side arrays, whose base has its own alignment
-    __device__ __forceinline__ float2 load_side(const float *row) const {
-        return make_float2(x_in ? row[x] : 0.0f, y_in ? row[y] : 0.0f);
-    }
-    __device__ __forceinline__ void store_side(float *row, float2 v) const {
-        if (x_in) row[x] = v.x;
-        if (y_in) row[y] = v.y;
     }
 };
 
-// Which of a warp's rows are inside the sequence and valid, and which restart.
+// The tile feature at place i of a row of the shared maps (places 2 l and 2 l + 1
+// are lane l's).
+template <bool kTma>
+__device__ __forceinline__ int walked_feature(int i) {
+    return kTma ? i : (i >> 1) + 16 * (i & 1);
+}
+
+// Which of a half warp's rows are inside the sequence, which of those are
+// valid, and which restart (bits); plain: all of the warp's rows are ordinary.
 struct RowFlags {
     uint32_t live, cut;
+    int rows_in;
+    bool plain;
 };
 template <bool kMasks>
-__device__ __forceinline__ RowFlags row_flags(const GatedShape &shape, int64_t batch, int64_t t0, int lane) {
+__device__ __forceinline__ RowFlags row_flags(const GatedShape &shape, int64_t batch, int segment, int warp, int lane) {
+    constexpr uint32_t kAll = (1u << kRows) - 1;
     RowFlags f;
+    const int t0 = segment * kSegment + warp * 2 * kRows, half = lane >> 4;
+    const int left = static_cast<int>(shape.length) - t0;
+    const int mine = left - half * kRows;
+    f.rows_in = mine >= kRows ? kRows : mine > 0 ? mine : 0;
     if (kMasks) {
-        const int64_t t = t0 + lane;
-        const bool in = lane < kTileRows && t < shape.length;
-        const int64_t row = batch * shape.length + t;
-        f.live = __ballot_sync(0xffffffffu, in && (shape.valid == nullptr || shape.valid[row] != 0));
-        f.cut = __ballot_sync(0xffffffffu, in && shape.restart != nullptr && shape.restart[row] != 0);
+        const bool in = lane < 2 * kRows && lane < left;
+        const int64_t row = batch * shape.length + t0 + lane;
+        const uint32_t live = __ballot_sync(0xffffffffu, in && (shape.valid == nullptr || shape.valid[row] != 0));
+        const uint32_t cut = __ballot_sync(0xffffffffu, in && shape.restart != nullptr && shape.restart[row] != 0);
+        f.plain = live == (kAll << kRows | kAll) && cut == 0;
+        f.live = live >> half * kRows & kAll;
+        f.cut = cut >> half * kRows & kAll;
     } else {
-        const int64_t left = shape.length - t0;
-        f.live = left >= kTileRows ? (1u << kTileRows) - 1 : left <= 0 ? 0u : (1u << left) - 1;
+        f.plain = left >= 2 * kRows;
+        f.live = (1u << f.rows_in) - 1;
         f.cut = 0;
     }
     return f;
 }
 
-// Shared memory of a tile kernel: kStages stages of kArrays boxes, then the
-// warps' maps of two waves, the cluster's maps of two waves, the barriers.
-template <typename T, int kArrays, int kStages>
-struct TileMemory {
-    static constexpr int kBox = kSegment * kTileFeatures;
-    static constexpr uint32_t kStageBytes = kArrays * kBox * sizeof(T);
-    T *stages;
-    float4 *warps;    // [2][kTileWarps][32]
-    float2 *extra;    // [2][kTileWarps][32], the backward's third value
-    float4 *cluster;  // [2][kMaxCluster][32]
-    uint64_t *full;   // [kStages]
-    __device__ explicit TileMemory(unsigned char *raw) {
-        stages = reinterpret_cast<T *>(raw);
-        warps = reinterpret_cast<float4 *>(raw + size_t(kStages) * kStageBytes);
-        cluster = warps + 2 * kTileWarps * 32;
-        extra = reinterpret_cast<float2 *>(cluster + 2 * kMaxCluster * 32);
-        full = reinterpret_cast<uint64_t *>(extra + 2 * kTileWarps * 32);
-    }
-    static size_t bytes(bool tma) {
-        return (tma ? size_t(kStages) * kStageBytes : 0) + 2 * (kTileWarps + kMaxCluster) * 32 * sizeof(float4) +
-               2 * kTileWarps * 32 * sizeof(float2) + kStages * sizeof(uint64_t);
-    }
-};
+constexpr float kSmallest = 1.4e-45f;  // keeps a product of positive factors positive: 0 would undo an infinity
 
+// A map v -> m v + n. A restart among its rows makes n the result, whatever v
+// holds (a NaN, say): m is then 0, and only there.
+template <bool kMasks>
+__device__ __forceinline__ float apply(float m, float n, float v) {
+    const float r = fmaf(m, v, n);
+    return kMasks && m == 0.0f ? n : r;
+}
+// m of a map put in front of one with m of `next`
+template <bool kMasks>
+__device__ __forceinline__ float chain(float m, float next) {
+    return kMasks && (m == 0.0f || next == 0.0f) ? 0.0f : fmaxf(m * next, kSmallest);
+}
+
+constexpr int kLoader = kTileThreads - 32;  // the thread that issues the loads: not in the walking warp
 template <typename T>
-constexpr int forward_stages() {
+constexpr int backward_stages() {
     return sizeof(T) == 2 ? 3 : 2;
 }
 
+// The chains of a cluster: `count` neighbouring ones from `first` on, each
+// `waves` waves long; item i of a CTA is wave i % waves of chain first + i /
+// waves.
+struct Walk {
+    int64_t first, feature_tiles;
+    int count, waves, cluster, rank;
+    __device__ Walk(const GatedShape &shape, int64_t tiles, int cluster_, int per) : feature_tiles(tiles), cluster(cluster_) {
+        rank = static_cast<int>(blockIdx.x % cluster);
+        first = int64_t(blockIdx.x / cluster) * per;
+        const int64_t left = shape.batch * feature_tiles - first;
+        count = left < per ? static_cast<int>(left) : per;
+        waves = (static_cast<int>(shape.segments) + cluster - 1) / cluster;
+    }
+    __device__ __forceinline__ int64_t batch(int chain) const { return (first + chain) / feature_tiles; }
+    __device__ __forceinline__ int64_t feature(int chain) const { return (first + chain) % feature_tiles * kTileFeatures; }
+};
+
+// Shared memory of a tile kernel: kStages stages of kArrays boxes; per half
+// warp and feature the rows' map (kMaps values) and the start values
+// (kStarts); the cluster's maps of two waves; the barriers.
+template <typename T, int kArrays, int kStages, int kMaps, int kStarts>
+struct TileMemory {
+    static constexpr int kBox = kSegment * kTileFeatures;
+    static constexpr uint32_t kStageBytes = kArrays * kBox * sizeof(T);
+    static constexpr int kPlane = kBlocks * kTileFeatures;
+    T *stages;
+    uint64_t *full;  // [kStages]
+    uint64_t *met;   // [2]
+    float *maps;     // [kMaps][kBlocks][32]
+    float *starts;   // [kStarts][kBlocks][32]
+    float2 *tiles;   // [2][CTAs of the cluster][32]
+    __device__ explicit TileMemory(unsigned char *raw) {
+        stages = reinterpret_cast<T *>(raw);
+        full = reinterpret_cast<uint64_t *>(raw + size_t(kStages) * kStageBytes);
+        met = full + 4;
+        maps = reinterpret_cast<float *>(met + 4);
+        starts = maps + kMaps * kPlane;
+        tiles = reinterpret_cast<float2 *>(starts + kStarts * kPlane);
+    }
+    static size_t bytes(int cluster_size) {
+        return size_t(kStages) * kStageBytes + 64 + (kMaps + kStarts) * kPlane * sizeof(float) +
+               (cluster_size > 1 ? 2 * size_t(cluster_size) * kTileFeatures * sizeof(float2) : 0);
+    }
+};
+
+// The map of a whole tile, by the walking warp (a thread per feature), in row
+// order or from the last row.
+template <bool kMasks, bool kBackward>
+__device__ __forceinline__ float2 tile_map_of(const float *mm, const float *nn) {
+    float tm = 1.0f, tn = 0.0f;
+#pragma unroll 8
+    for (int i = 0; i < kBlocks; ++i) {
+        const int block = kBackward ? kBlocks - 1 - i : i;
+        const float m = mm[block * kTileFeatures], n = nn[block * kTileFeatures];
+        tm = chain<kMasks>(tm, m);
+        tn = apply<kMasks>(m, n, tn);
+    }
+    return make_float2(tm, tn);
+}
+
+// The walking warp of a cluster's CTA gives its tile's map to every CTA, waits
+// for everyone's and folds them onto `carry` in tile order (or from the last
+// tile). Returns the value its own tile starts from. The maps of two items
+// have places of their own: a CTA has received every map of item i + 1 only
+// when all have left item i.
+template <bool kMasks, bool kBackward, typename Memory>
+__device__ __forceinline__ float meet(Memory &memory, int item, int cluster, int rank, float2 mine, float &carry,
+                                      bool &dead, int *status) {
+    const int lane = threadIdx.x, parity = item & 1;
+    uint64_t *bar = &memory.met[parity];
+    float2 *tiles = memory.tiles + parity * cluster * kTileFeatures + lane;
+    if (lane == 0) mbar_arrive_expect_tx(bar, cluster * kTileFeatures * sizeof(float2));
+    for (int r = 0; r < cluster; ++r) store_to_rank(tiles + rank * kTileFeatures, bar, r, mine);
+    if (!dead) dead = !mbar_wait_bounded(bar, static_cast<uint32_t>(item >> 1) & 1, status);
+    float start = carry;
+    for (int i = 0; i < cluster; ++i) {
+        const int r = kBackward ? cluster - 1 - i : i;
+        if (r == rank) start = carry;
+        const float2 v = tiles[r * kTileFeatures];
+        carry = apply<kMasks>(v.x, v.y, carry);
+    }
+    return start;
+}
+
 template <typename T, bool kTma, bool kMasks>
-__global__ __launch_bounds__(kTileThreads, 3) void gated_forward_tile_kernel(
-    const __grid_constant__ CUtensorMap map, GatedShape shape, int64_t feature_tiles, int cluster,
+__global__ __launch_bounds__(kTileThreads, sizeof(T) == 2 ? kForwardResident : 3) void gated_forward_tile_kernel(
+    const __grid_constant__ CUtensorMap map, GatedShape shape, int64_t feature_tiles, int cluster, int per,
     const T *__restrict__ projections, const float *__restrict__ initial, T *__restrict__ states,
     float *__restrict__ final_state, float *__restrict__ carries, int *status) {
-    constexpr int kStages = kTma ? forward_stages<T>() : 0;
-    using Memory = TileMemory<T, 2, kStages>;
+    constexpr int kStages = kTma ? 2 : 0;
+    using Memory = TileMemory<T, 2, kStages, 2, 1>;
     extern __shared__ __align__(128) unsigned char smem_raw[];
     Memory memory(smem_raw);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int rank = static_cast<int>(blockIdx.x % cluster);
-    const int64_t chain_index = blockIdx.x / cluster;
-    const int64_t batch = chain_index / feature_tiles;
-    const int64_t f0 = (chain_index - batch * feature_tiles) * kTileFeatures;
-    const int64_t waves = (shape.segments + cluster - 1) / cluster;
-    const LaneFeatures<kTma> features(f0, lane, shape.features);
-    const float span = shape.hi - shape.lo;
-    const T *in = projections + batch * shape.length * 2 * shape.features;
-    T *out = states + batch * shape.length * shape.features;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, block = 2 * warp + (lane >> 4);
+    const Walk walk(shape, feature_tiles, cluster, per);
+    const int rank = walk.rank, segments = static_cast<int>(shape.segments), items = walk.count * walk.waves;
+    const float2 span = both(shape.hi - shape.lo), lo = both(shape.lo);
+    const float2 fall = both(shape.lo - shape.hi), top = both(1.0f - shape.lo);  // 1 - a = top + fall s
 
-    auto issue = [&](int64_t wave) {
-        const int64_t segment = wave * cluster + rank;
-        if (segment >= shape.segments) return;
-        const int stage = static_cast<int>(wave % (kStages > 0 ? kStages : 1));
-        T *box = memory.stages + size_t(stage) * 2 * Memory::kBox;
-        mbar_arrive_expect_tx(&memory.full[stage], Memory::kStageBytes);
-        const int32_t t = static_cast<int32_t>(segment * kSegment), f = static_cast<int32_t>(f0);
-        tma_load_3d(box, &map, &memory.full[stage], f, t, static_cast<int32_t>(batch));
-        tma_load_3d(box + Memory::kBox, &map, &memory.full[stage], static_cast<int32_t>(shape.features) + f, t,
-                    static_cast<int32_t>(batch));
+    auto issue = [&](int item) {
+        const int chain = item / walk.waves, segment = (item - chain * walk.waves) * cluster + rank;
+        uint64_t *bar = &memory.full[item & 1];
+        if (segment >= segments) {  // no tile in the chain's last wave: an empty phase
+            mbar_arrive(bar);
+            return;
+        }
+        T *box = memory.stages + (item & 1) * 2 * Memory::kBox;
+        mbar_arrive_expect_tx(bar, Memory::kStageBytes);
+        const int32_t f = static_cast<int32_t>(walk.feature(chain)), batch = static_cast<int32_t>(walk.batch(chain));
+        tma_load_3d(box, &map, bar, f, segment * kSegment, batch);
+        tma_load_3d(box + Memory::kBox, &map, bar, static_cast<int32_t>(shape.features) + f, segment * kSegment, batch);
     };
-    bool dead = false;  // a load never arrived: go on without waiting or loading
-    if (kTma) {
-        if (threadIdx.x == 0) {
-            for (int s = 0; s < kStages; ++s) mbar_init(&memory.full[s], 1);
-            fence_barrier_init();
-            prefetch_tensor_map(&map);
+    bool dead = false;  // a wait gave up: go on without waiting or loading
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&memory.full[s], 1);
+            mbar_init(&memory.met[s], 1);
         }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int64_t w = 0; w < waves && w < kStages; ++w) issue(w);
-        }
+        fence_barrier_init();
+        if (kTma) prefetch_tensor_map(&map);
     }
-    if (cluster > 1) cluster_sync();  // every CTA of the cluster runs before one stores into another
+    __syncthreads();
+    if (kTma && threadIdx.x == kLoader) {
+        for (int i = 0; i < items && i < kStages; ++i) issue(i);
+    }
+    if (cluster > 1) cluster_sync();  // every CTA's barriers are ready before one stores into another
 
-    float2 carry = initial != nullptr ? features.load_side(initial + batch * shape.features) : make_float2(0.0f, 0.0f);
-    RowFlags next_flags = row_flags<kMasks>(shape, batch, int64_t(rank) * kSegment + warp * kTileRows, lane);
-    for (int64_t wave = 0; wave < waves; ++wave) {
-        const int64_t segment = wave * cluster + rank;
-        const int64_t t0 = segment * kSegment + warp * kTileRows;
-        const int parity = static_cast<int>(wave & 1);
-        const RowFlags flags = next_flags;
-        next_flags = row_flags<kMasks>(shape, batch, t0 + int64_t(cluster) * kSegment, lane);
-        const bool plain = flags.live == (1u << kTileRows) - 1 && flags.cut == 0;
+    int item = 0;
+    for (int chain = 0; chain < walk.count; ++chain) {
+        const int64_t batch = walk.batch(chain), f0 = walk.feature(chain);
+        const LaneFeatures<kTma> features(f0, lane, shape.features);
+        const int64_t first_row = batch * shape.length + int64_t(rank) * kSegment + block * kRows;
+        const T *in = projections + first_row * 2 * shape.features + features.x;
+        T *out = states + first_row * shape.features + features.x;
+        // the walking warp's feature and state
+        const int64_t walked = f0 + walked_feature<kTma>(lane);
+        const bool walks = warp == 0, walks_in = walks && walked < shape.features;
+        float carry = walks_in && initial != nullptr ? initial[batch * shape.features + walked] : 0.0f;
+        RowFlags next_flags = row_flags<kMasks>(shape, batch, rank, warp, lane);
+        for (int segment = rank; segment - rank < segments; segment += cluster, ++item) {
+            const RowFlags flags = next_flags;
+            next_flags = row_flags<kMasks>(shape, batch, segment + cluster, warp, lane);
 
-        float2 a[kTileRows], b[kTileRows];
-        if (kTma && segment < shape.segments && !dead) {
-            const int stage = static_cast<int>(wave % (kStages > 0 ? kStages : 1));
-            dead = !mbar_wait_bounded(&memory.full[stage], static_cast<uint32_t>(wave / (kStages > 0 ? kStages : 1)) & 1, status);
-        }
-        {
-            const int stage = static_cast<int>(wave % (kStages > 0 ? kStages : 1));
-            const T *box = memory.stages + size_t(stage) * 2 * Memory::kBox + warp * kTileRows * kTileFeatures + 2 * lane;
-#pragma unroll
-            for (int j = 0; j < kTileRows; ++j) {
-                float2 p, c;
+            if (kTma && !dead) dead = !mbar_wait_bounded(&memory.full[item & 1], static_cast<uint32_t>(item >> 1) & 1, status);
+            float2 a[kRows], b[kRows];
+            float2 m = both(1.0f), n = both(0.0f);
+            const T *box = memory.stages + (item & 1) * 2 * Memory::kBox + block * kRows * kTileFeatures + 2 * (lane & 15);
+            auto gates = [&](int j) {
+                float2 p, c, s, k;
                 if (kTma) {
-                    p = load_two(box + j * kTileFeatures);
-                    c = load_two(box + Memory::kBox + j * kTileFeatures);
+                    p = load_clamped<true>(box + j * kTileFeatures);
+                    c = load_clamped<false>(box + Memory::kBox + j * kTileFeatures);
                 } else {
-                    p = c = make_float2(0.0f, 0.0f);
-                    if (t0 + j < shape.length) {
-                        p = features.load(in + (t0 + j) * 2 * shape.features);
-                        c = features.load(in + (t0 + j) * 2 * shape.features + shape.features);
+                    p = clamped<true>(features.load(in + j * 2 * shape.features));
+                    c = clamped<false>(features.load(in + j * 2 * shape.features + shape.features));
+                }
+                gates_of<T>(p, c, s, k);
+                a[j] = fma2(span, s, lo);
+                b[j] = mul2(fma2(fall, s, top), k);
+            };
+            if (flags.plain) {
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) {
+                    gates(j);
+                    m = mul2(m, a[j]);
+                    n = fma2(a[j], n, b[j]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) {
+                    a[j] = both(1.0f);
+                    b[j] = both(0.0f);
+                    if (flags.cut >> j & 1u) n = both(0.0f);
+                    if (flags.live >> j & 1u) gates(j);
+                    m = mul2(m, a[j]);
+                    n = fma2(a[j], n, b[j]);
+                }
+            }
+            m = flags.cut != 0 ? both(0.0f) : make_float2(fmaxf(m.x, kSmallest), fmaxf(m.y, kSmallest));
+            const int at = block * kTileFeatures + 2 * (lane & 15);
+            *reinterpret_cast<float2 *>(memory.maps + at) = m;
+            *reinterpret_cast<float2 *>(memory.maps + Memory::kPlane + at) = n;
+            __syncthreads();
+            if (kTma && threadIdx.x == kLoader && !dead && item + kStages < items) issue(item + kStages);
+
+            if (walks) {
+                const float *mm = memory.maps + lane, *nn = mm + Memory::kPlane;
+                float start = carry;
+                if (cluster > 1) {
+                    start = meet<kMasks, false>(memory, item, cluster, rank, tile_map_of<kMasks, false>(mm, nn), carry, dead, status);
+                }
+                if (carries != nullptr && walks_in && segment < segments) {
+                    carries[(batch * shape.segments + segment) * shape.features + walked] = start;
+                }
+                float mr[kBlocks / 2], nr[kBlocks / 2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int i = 0; i < kBlocks / 2; ++i) {
+                        mr[i] = mm[(half * (kBlocks / 2) + i) * kTileFeatures];
+                        nr[i] = nn[(half * (kBlocks / 2) + i) * kTileFeatures];
+                    }
+#pragma unroll
+                    for (int i = 0; i < kBlocks / 2; ++i) {
+                        memory.starts[(half * (kBlocks / 2) + i) * kTileFeatures + lane] = start;
+                        start = apply<kMasks>(mr[i], nr[i], start);
                     }
                 }
-                float kx, ky;
-                gate_of<T>(p.x, c.x, shape.lo, span, a[j].x, kx);
-                gate_of<T>(p.y, c.y, shape.lo, span, a[j].y, ky);
-                b[j] = make_float2(fmaf(-a[j].x, kx, kx), fmaf(-a[j].y, ky, ky));
+                if (cluster == 1) carry = start;
             }
-        }
-        float4 rows = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
-        if (plain) {
-#pragma unroll
-            for (int j = 0; j < kTileRows; ++j) {
-                rows.x *= a[j].x;
-                rows.y *= a[j].y;
-                rows.z = fmaf(a[j].x, rows.z, b[j].x);
-                rows.w = fmaf(a[j].y, rows.w, b[j].y);
-            }
-            rows.x = fmaxf(rows.x, 1.4e-45f);
-            rows.y = fmaxf(rows.y, 1.4e-45f);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kTileRows; ++j) {
-                if (!(flags.live >> j & 1u)) {
-                    a[j] = make_float2(1.0f, 1.0f);
-                    b[j] = make_float2(0.0f, 0.0f);
-                }
-                if (flags.cut >> j & 1u) a[j] = make_float2(0.0f, 0.0f);
-                rows = compose(rows, make_float4(a[j].x, a[j].y, b[j].x, b[j].y));
-            }
-        }
-        float4 *warps = memory.warps + parity * kTileWarps * 32 + lane;
-        warps[warp * 32] = rows;
-        __syncthreads();
-        if (kTma && threadIdx.x == 0 && !dead && wave + kStages < waves) issue(wave + kStages);
+            __syncthreads();
 
-        if (cluster > 1) {
-            float4 *tiles = memory.cluster + parity * kMaxCluster * 32 + lane;
-            if (warp < cluster) {
-                float4 total = warps[0];
+            float2 h = *reinterpret_cast<const float2 *>(memory.starts + at);
+            T *row = out;
+            if (flags.plain) {
 #pragma unroll
-                for (int w = 1; w < kTileWarps; ++w) total = compose(total, warps[w * 32]);
-                store_remote(tiles + rank * 32, static_cast<uint32_t>(warp), total);
-            }
-            cluster_sync();
-            float2 h = carry;
-            for (int r = 0; r < cluster; ++r) {
-                if (r == rank) carry = h;  // from here on: the state before this tile
-                const float4 m = tiles[r * 32];
-                h = make_float2(apply(m.x, m.z, h.x), apply(m.y, m.w, h.y));
-            }
-            // h: the state after the wave; carry: before this tile
-            const float2 after = h;
-            h = carry;
-            if (carries != nullptr && warp == 0 && segment < shape.segments) {
-                features.store_side(carries + (batch * shape.segments + segment) * shape.features, h);
-            }
-            for (int w = 0; w < warp; ++w) {
-                const float4 m = warps[w * 32];
-                h = make_float2(apply(m.x, m.z, h.x), apply(m.y, m.w, h.y));
-            }
-            carry = h;
-#pragma unroll
-            for (int j = 0; j < kTileRows; ++j) {
-                if (plain) {
-                    carry = make_float2(fmaf(a[j].x, carry.x, b[j].x), fmaf(a[j].y, carry.y, b[j].y));
-                } else {
-                    carry = make_float2(apply(a[j].x, b[j].x, carry.x), apply(a[j].y, b[j].y, carry.y));
+                for (int j = 0; j < kRows; ++j) {
+                    h = fma2(a[j], h, b[j]);
+                    features.store(row, h);
+                    row += shape.features;
                 }
-                if (t0 + j < shape.length) features.store(out + (t0 + j) * shape.features, carry);
-            }
-            carry = after;
-        } else {
-            if (carries != nullptr && warp == 0) {
-                features.store_side(carries + (batch * shape.segments + segment) * shape.features, carry);
-            }
-            float2 h = carry;
+            } else {
 #pragma unroll
-            for (int w = 0; w < kTileWarps; ++w) {
-                if (w == warp) h = carry;
-                const float4 m = warps[w * 32];
-                carry = make_float2(apply(m.x, m.z, carry.x), apply(m.y, m.w, carry.y));
-            }
-#pragma unroll
-            for (int j = 0; j < kTileRows; ++j) {
-                if (plain) {
-                    h = make_float2(fmaf(a[j].x, h.x, b[j].x), fmaf(a[j].y, h.y, b[j].y));
-                } else {
-                    h = make_float2(apply(a[j].x, b[j].x, h.x), apply(a[j].y, b[j].y, h.y));
+                for (int j = 0; j < kRows; ++j) {
+                    if (flags.cut >> j & 1u) h = both(0.0f);
+                    h = fma2(a[j], h, b[j]);
+                    if (j < flags.rows_in) features.store(row, h);
+                    row += shape.features;
                 }
-                if (t0 + j < shape.length) features.store(out + (t0 + j) * shape.features, h);
             }
+            in += int64_t(cluster) * kSegment * 2 * shape.features;
+            out += int64_t(cluster) * kSegment * shape.features;
         }
+        if (rank == 0 && walks_in) final_state[batch * shape.features + walked] = carry;
     }
-    if (rank == 0 && warp == 0) features.store_side(final_state + batch * shape.features, carry);
 }
 
-template <typename T>
-constexpr int backward_stages() {
-    return 2;
-}
-
-// The waves run from the end. A row's rolling values: a, k (registers), the
-// state before it (recomputed from the segment's carry and the warps' maps)
-// and g; x comes from the right.
+// The waves run from the end. Per row a lane keeps a, k and u = (h' - k)(hi -
+// lo) s (1 - s) in registers, h' recomputed from the tile's carry; g stays in
+// its stage until the row's gradients are stored.
 template <typename T, bool kTma, bool kMasks>
-__global__ __launch_bounds__(kTileThreads, 2) void gated_backward_tile_kernel(
+__global__ __launch_bounds__(kTileThreads, kBackwardResident) void gated_backward_tile_kernel(
     const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap grad_map, GatedShape shape,
-    int64_t feature_tiles, int cluster, const T *__restrict__ projections, const float *__restrict__ carries,
+    int64_t feature_tiles, int cluster, int per, const T *__restrict__ projections, const float *__restrict__ carries,
     const T *__restrict__ grad_states, const float *__restrict__ grad_final, T *__restrict__ grad_projections,
     float *__restrict__ grad_initial, int *status) {
     constexpr int kStages = kTma ? backward_stages<T>() : 0;
-    using Memory = TileMemory<T, 3, kStages>;
+    using Memory = TileMemory<T, 3, kStages, 3, 2>;
     extern __shared__ __align__(128) unsigned char smem_raw[];
     Memory memory(smem_raw);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int rank = static_cast<int>(blockIdx.x % cluster);
-    const int64_t chain_index = blockIdx.x / cluster;
-    const int64_t batch = chain_index / feature_tiles;
-    const int64_t f0 = (chain_index - batch * feature_tiles) * kTileFeatures;
-    const int64_t waves = (shape.segments + cluster - 1) / cluster;
-    const LaneFeatures<kTma> features(f0, lane, shape.features);
-    const float span = shape.hi - shape.lo, inverse_span = 1.0f / span;
-    const T *in = projections + batch * shape.length * 2 * shape.features;
-    const T *grad_in = grad_states == nullptr ? nullptr : grad_states + batch * shape.length * shape.features;
-    T *grad_out = grad_projections + batch * shape.length * 2 * shape.features;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, block = 2 * warp + (lane >> 4);
+    const Walk walk(shape, feature_tiles, cluster, per);
+    const int rank = walk.rank, segments = static_cast<int>(shape.segments), items = walk.count * walk.waves;
+    const float2 span = both(shape.hi - shape.lo), lo = both(shape.lo);
+    const bool have_grad = grad_states != nullptr;
 
-    // step i is wave waves - 1 - i
-    auto issue = [&](int64_t step) {
-        const int64_t segment = (waves - 1 - step) * cluster + rank;
-        if (segment >= shape.segments) return;
-        const int stage = static_cast<int>(step % (kStages > 0 ? kStages : 1));
-        T *box = memory.stages + size_t(stage) * 3 * Memory::kBox;
-        const uint32_t bytes = grad_in == nullptr ? Memory::kStageBytes / 3 * 2 : Memory::kStageBytes;
-        mbar_arrive_expect_tx(&memory.full[stage], bytes);
-        const int32_t t = static_cast<int32_t>(segment * kSegment), f = static_cast<int32_t>(f0);
-        tma_load_3d(box, &map, &memory.full[stage], f, t, static_cast<int32_t>(batch));
-        tma_load_3d(box + Memory::kBox, &map, &memory.full[stage], static_cast<int32_t>(shape.features) + f, t,
-                    static_cast<int32_t>(batch));
-        if (grad_in != nullptr) {
-            tma_load_3d(box + 2 * Memory::kBox, &grad_map, &memory.full[stage], f, t, static_cast<int32_t>(batch));
+    auto issue = [&](int item) {
+        const int chain = item / walk.waves, segment = (walk.waves - 1 - (item - chain * walk.waves)) * cluster + rank;
+        const int stage = item % (kStages > 0 ? kStages : 1);
+        uint64_t *bar = &memory.full[stage];
+        if (segment >= segments) {  // no tile in the chain's last wave: an empty phase
+            mbar_arrive(bar);
+            return;
         }
+        T *box = memory.stages + stage * 3 * Memory::kBox;
+        mbar_arrive_expect_tx(bar, have_grad ? Memory::kStageBytes : Memory::kStageBytes / 3 * 2);
+        const int32_t t = segment * kSegment, f = static_cast<int32_t>(walk.feature(chain));
+        const int32_t batch = static_cast<int32_t>(walk.batch(chain));
+        tma_load_3d(box, &map, bar, f, t, batch);
+        tma_load_3d(box + Memory::kBox, &map, bar, static_cast<int32_t>(shape.features) + f, t, batch);
+        if (have_grad) tma_load_3d(box + 2 * Memory::kBox, &grad_map, bar, f, t, batch);
     };
-    // A stage's phase counts the loads it has had: a rank without a tile in
-    // the last wave skips that one.
-    const int64_t skipped = (waves - 1) * cluster + rank >= shape.segments ? 1 : 0;
     bool dead = false;
-    if (kTma) {
-        if (threadIdx.x == 0) {
-            for (int s = 0; s < kStages; ++s) mbar_init(&memory.full[s], 1);
-            fence_barrier_init();
-            prefetch_tensor_map(&map);
-            if (grad_in != nullptr) prefetch_tensor_map(&grad_map);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int64_t i = 0; i < waves && i < kStages; ++i) issue(i);
-        }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) mbar_init(&memory.full[s], 1);
+        for (int s = 0; s < 2; ++s) mbar_init(&memory.met[s], 1);
+        fence_barrier_init();
+        if (kTma) prefetch_tensor_map(&map);
+        if (kTma && have_grad) prefetch_tensor_map(&grad_map);
+    }
+    __syncthreads();
+    if (kTma && threadIdx.x == kLoader) {
+        for (int i = 0; i < items && i < kStages; ++i) issue(i);
     }
     if (cluster > 1) cluster_sync();
 
-    float2 x = grad_final != nullptr ? features.load_side(grad_final + batch * shape.features) : make_float2(0.0f, 0.0f);
-    for (int64_t step = 0; step < waves; ++step) {
-        const int64_t segment = (waves - 1 - step) * cluster + rank;
-        const int64_t t0 = segment * kSegment + warp * kTileRows;
-        const int parity = static_cast<int>(step & 1);
-        const bool have = segment < shape.segments;
-        const float2 carry = have ? features.load_side(carries + (batch * shape.segments + segment) * shape.features)
-                                  : make_float2(0.0f, 0.0f);
-        const RowFlags flags = row_flags<kMasks>(shape, batch, t0, lane);
-        const bool plain = flags.live == (1u << kTileRows) - 1 && flags.cut == 0;
-        const int stage = static_cast<int>(step % (kStages > 0 ? kStages : 1));
-        if (kTma && have && !dead) {
-            const int64_t use = step / (kStages > 0 ? kStages : 1) - (stage == 0 ? skipped : 0);
-            dead = !mbar_wait_bounded(&memory.full[stage], static_cast<uint32_t>(use) & 1, status);
-        }
-        const T *box = memory.stages + size_t(stage) * 3 * Memory::kBox + warp * kTileRows * kTileFeatures + 2 * lane;
+    int item = 0;
+    for (int chain = 0; chain < walk.count; ++chain) {
+        const int64_t batch = walk.batch(chain), f0 = walk.feature(chain);
+        const LaneFeatures<kTma> features(f0, lane, shape.features);
+        const int last = (walk.waves - 1) * cluster + rank;
+        const int64_t first_row = batch * shape.length + int64_t(last) * kSegment + block * kRows;
+        const T *in = projections + first_row * 2 * shape.features + features.x;
+        const T *grad_in = grad_states + first_row * shape.features + features.x;
+        T *grad_out = grad_projections + first_row * 2 * shape.features + features.x;
+        const int64_t walked = f0 + walked_feature<kTma>(lane);
+        const bool walks = warp == 0, walks_in = walks && walked < shape.features;
+        float x = walks_in && grad_final != nullptr ? grad_final[batch * shape.features + walked] : 0.0f;
+        RowFlags next_flags = row_flags<kMasks>(shape, batch, last, warp, lane);
+        for (int segment = last; segment >= 0; segment -= cluster, ++item) {
+            float before = 0.0f;  // the state before this tile
+            if (walks_in && segment < segments) before = carries[(batch * shape.segments + segment) * shape.features + walked];
+            const RowFlags flags = next_flags;
+            if (segment >= cluster) next_flags = row_flags<kMasks>(shape, batch, segment - cluster, warp, lane);
+            const int stage = item % (kStages > 0 ? kStages : 1);
+            if (kTma && !dead) {
+                dead = !mbar_wait_bounded(&memory.full[stage], static_cast<uint32_t>(item / (kStages > 0 ? kStages : 1)) & 1, status);
+            }
+            const T *box = memory.stages + stage * 3 * Memory::kBox + block * kRows * kTileFeatures + 2 * (lane & 15);
+            auto load_grad = [&](int j) {
+                if (!have_grad) return both(0.0f);
+                return kTma ? load_two(box + 2 * Memory::kBox + j * kTileFeatures) : features.load(grad_in + j * shape.features);
+            };
 
-        float2 a[kTileRows], k[kTileRows], g[kTileRows];
-        float4 rows = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
-        float2 back = make_float2(0.0f, 0.0f);
+            float2 a[kRows], k[kRows], u[kRows];  // u: (hi - lo) s (1 - s), then times h' - k
+            float2 m = both(1.0f), n = both(0.0f), back = both(0.0f);
+            auto gates = [&](int j) {
+                float2 p, c, s;
+                if (kTma) {
+                    p = load_clamped<true>(box + j * kTileFeatures);
+                    c = load_clamped<false>(box + Memory::kBox + j * kTileFeatures);
+                } else {
+                    p = clamped<true>(features.load(in + j * 2 * shape.features));
+                    c = clamped<false>(features.load(in + j * 2 * shape.features + shape.features));
+                }
+                gates_of<T>(p, c, s, k[j]);
+                a[j] = fma2(span, s, lo);
+                u[j] = mul2(mul2(span, s), sub2(both(1.0f), s));
+            };
+            if (flags.plain) {
 #pragma unroll
-        for (int j = 0; j < kTileRows; ++j) {
-            float2 p, c;
-            if (kTma) {
-                p = load_two(box + j * kTileFeatures);
-                c = load_two(box + Memory::kBox + j * kTileFeatures);
-                g[j] = grad_in != nullptr ? load_two(box + 2 * Memory::kBox + j * kTileFeatures) : make_float2(0.0f, 0.0f);
+                for (int j = 0; j < kRows; ++j) {
+                    gates(j);
+                    m = mul2(m, a[j]);
+                    n = fma2(a[j], sub2(n, k[j]), k[j]);
+                }
+#pragma unroll
+                for (int j = kRows - 1; j >= 0; --j) back = mul2(a[j], add2(back, load_grad(j)));
             } else {
-                p = c = g[j] = make_float2(0.0f, 0.0f);
-                if (t0 + j < shape.length) {
-                    p = features.load(in + (t0 + j) * 2 * shape.features);
-                    c = features.load(in + (t0 + j) * 2 * shape.features + shape.features);
-                    if (grad_in != nullptr) g[j] = features.load(grad_in + (t0 + j) * shape.features);
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) {
+                    a[j] = both(1.0f);
+                    k[j] = u[j] = both(0.0f);
+                    if (flags.cut >> j & 1u) n = both(0.0f);
+                    if (flags.live >> j & 1u) {
+                        gates(j);
+                        m = mul2(m, a[j]);
+                        n = fma2(a[j], sub2(n, k[j]), k[j]);
+                    }
+                }
+#pragma unroll
+                for (int j = kRows - 1; j >= 0; --j) {
+                    if (j < flags.rows_in) back = mul2(a[j], add2(back, load_grad(j)));
+                    if (flags.cut >> j & 1u) back = both(0.0f);
                 }
             }
-            gate_of<T>(p.x, c.x, shape.lo, span, a[j].x, k[j].x);
-            gate_of<T>(p.y, c.y, shape.lo, span, a[j].y, k[j].y);
-        }
-        if (plain) {
-#pragma unroll
-            for (int j = 0; j < kTileRows; ++j) {
-                rows.x *= a[j].x;
-                rows.y *= a[j].y;
-                rows.z = fmaf(a[j].x, rows.z, fmaf(-a[j].x, k[j].x, k[j].x));
-                rows.w = fmaf(a[j].y, rows.w, fmaf(-a[j].y, k[j].y, k[j].y));
-            }
-#pragma unroll
-            for (int j = kTileRows - 1; j >= 0; --j) back = make_float2(a[j].x * (back.x + g[j].x), a[j].y * (back.y + g[j].y));
-            rows.x = fmaxf(rows.x, 1.4e-45f);
-            rows.y = fmaxf(rows.y, 1.4e-45f);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kTileRows; ++j) {
-                if (!(flags.live >> j & 1u)) {
-                    a[j] = make_float2(1.0f, 1.0f);
-                    k[j] = make_float2(0.0f, 0.0f);
-                    if (t0 + j >= shape.length) g[j] = make_float2(0.0f, 0.0f);
-                }
-                const bool cut = flags.cut >> j & 1u;
-                rows = compose(rows, make_float4(cut ? 0.0f : a[j].x, cut ? 0.0f : a[j].y, fmaf(-a[j].x, k[j].x, k[j].x),
-                                                 fmaf(-a[j].y, k[j].y, k[j].y)));
-            }
-#pragma unroll
-            for (int j = kTileRows - 1; j >= 0; --j) {
-                back = flags.cut >> j & 1u ? make_float2(0.0f, 0.0f)
-                                           : make_float2(a[j].x * (back.x + g[j].x), a[j].y * (back.y + g[j].y));
-            }
-        }
-        float4 *warps = memory.warps + parity * kTileWarps * 32 + lane;
-        float2 *backs = memory.extra + parity * kTileWarps * 32 + lane;
-        warps[warp * 32] = rows;
-        backs[warp * 32] = back;
-        __syncthreads();
-        if (kTma && threadIdx.x == 0 && !dead && step + kStages < waves) issue(step + kStages);
+            m = flags.cut != 0 ? both(0.0f) : make_float2(fmaxf(m.x, kSmallest), fmaxf(m.y, kSmallest));
+            const int at = block * kTileFeatures + 2 * (lane & 15);
+            *reinterpret_cast<float2 *>(memory.maps + at) = m;
+            *reinterpret_cast<float2 *>(memory.maps + Memory::kPlane + at) = n;
+            *reinterpret_cast<float2 *>(memory.maps + 2 * Memory::kPlane + at) = back;
+            __syncthreads();
+            // every warp is done with the previous item's stage
+            if (kTma && threadIdx.x == kLoader && !dead && item > 0 && item - 1 + kStages < items) issue(item - 1 + kStages);
 
-        // the state before this warp's rows
-        float2 h = carry;
-        for (int w = 0; w < warp; ++w) {
-            const float4 m = warps[w * 32];
-            h = make_float2(apply(m.x, m.z, h.x), apply(m.y, m.w, h.y));
-        }
-        // x after this warp's rows, and x before the whole wave
-        float2 from = x;
-        if (cluster > 1) {
-            float4 *tiles = memory.cluster + parity * kMaxCluster * 32 + lane;
-            if (warp < cluster) {
-                float4 total = make_float4(1.0f, 1.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int w = kTileWarps - 1; w >= 0; --w) {
-                    const float4 m = warps[w * 32];
-                    const float2 n = backs[w * 32];
-                    total = compose(total, make_float4(m.x, m.y, n.x, n.y));
+            if (walks) {
+                const float *mm = memory.maps + lane, *nn = mm + Memory::kPlane, *gg = nn + Memory::kPlane;
+                float *h_at = memory.starts + lane, *x_at = h_at + Memory::kPlane;
+                float start = x;
+                if (cluster > 1) {
+                    start = meet<kMasks, true>(memory, item, cluster, rank, tile_map_of<kMasks, true>(mm, gg), x, dead, status);
                 }
-                store_remote(tiles + rank * 32, static_cast<uint32_t>(warp), total);
-            }
-            cluster_sync();
-            for (int r = cluster - 1; r >= 0; --r) {
-                if (r == rank) from = x;
-                const float4 m = tiles[r * 32];
-                x = make_float2(apply(m.x, m.z, x.x), apply(m.y, m.w, x.y));
-            }
-            for (int w = kTileWarps - 1; w > warp; --w) {
-                const float4 m = warps[w * 32];
-                const float2 n = backs[w * 32];
-                from = make_float2(apply(m.x, n.x, from.x), apply(m.y, n.y, from.y));
-            }
-        } else {
+                float mr[kBlocks], vr[kBlocks];
 #pragma unroll
-            for (int w = kTileWarps - 1; w >= 0; --w) {
-                if (w == warp) from = x;
-                const float4 m = warps[w * 32];
-                const float2 n = backs[w * 32];
-                x = make_float2(apply(m.x, n.x, x.x), apply(m.y, n.y, x.y));
-            }
-        }
-        // Replay: u = (h' - k)(hi - lo) s (1 - s), with (hi - lo) s (1 - s) =
-        // (a - lo)(hi - a) / (hi - lo).
-        float2 u[kTileRows];
+                for (int i = 0; i < kBlocks; ++i) {
+                    mr[i] = mm[i * kTileFeatures];
+                    vr[i] = nn[i * kTileFeatures];
+                }
 #pragma unroll
-        for (int j = 0; j < kTileRows; ++j) {
-            if (!plain && (flags.cut >> j & 1u)) h = make_float2(0.0f, 0.0f);
-            const float wx = (a[j].x - shape.lo) * (shape.hi - a[j].x) * inverse_span;
-            const float wy = (a[j].y - shape.lo) * (shape.hi - a[j].y) * inverse_span;
-            u[j] = make_float2((h.x - k[j].x) * wx, (h.y - k[j].y) * wy);
-            h = make_float2(fmaf(a[j].x, h.x - k[j].x, k[j].x), fmaf(a[j].y, h.y - k[j].y, k[j].y));
-        }
+                for (int i = 0; i < kBlocks; ++i) {
+                    h_at[i * kTileFeatures] = before;
+                    before = apply<kMasks>(mr[i], vr[i], before);
+                }
 #pragma unroll
-        for (int j = kTileRows - 1; j >= 0; --j) {
-            const float2 adjoint = make_float2(from.x + g[j].x, from.y + g[j].y);
-            float2 dp = make_float2(adjoint.x * u[j].x, adjoint.y * u[j].y);
-            float2 dc = make_float2(adjoint.x * ((1.0f - a[j].x) * fmaf(-k[j].x, k[j].x, 1.0f)),
-                                    adjoint.y * ((1.0f - a[j].y) * fmaf(-k[j].y, k[j].y, 1.0f)));
-            from = make_float2(a[j].x * adjoint.x, a[j].y * adjoint.y);
-            if (!plain) {
-                if (!(flags.live >> j & 1u)) dp = dc = make_float2(0.0f, 0.0f);
-                if (flags.cut >> j & 1u) from = make_float2(0.0f, 0.0f);
+                for (int i = 0; i < kBlocks; ++i) vr[i] = gg[i * kTileFeatures];
+#pragma unroll
+                for (int i = kBlocks - 1; i >= 0; --i) {
+                    x_at[i * kTileFeatures] = start;
+                    start = apply<kMasks>(mr[i], vr[i], start);
+                }
+                if (cluster == 1) x = start;
             }
-            if (t0 + j < shape.length) {
-                features.store(grad_out + (t0 + j) * 2 * shape.features, dp);
-                features.store(grad_out + (t0 + j) * 2 * shape.features + shape.features, dc);
+            __syncthreads();
+
+            float2 h = *reinterpret_cast<const float2 *>(memory.starts + at);
+            float2 from = *reinterpret_cast<const float2 *>(memory.starts + Memory::kPlane + at);
+#pragma unroll
+            for (int j = 0; j < kRows; ++j) {
+                if (!flags.plain && (flags.cut >> j & 1u)) h = both(0.0f);
+                const float2 gap = sub2(h, k[j]);
+                u[j] = mul2(gap, u[j]);
+                h = fma2(a[j], gap, k[j]);
             }
+            T *row = grad_out + int64_t(kRows - 1) * 2 * shape.features;
+#pragma unroll
+            for (int j = kRows - 1; j >= 0; --j, row -= 2 * shape.features) {
+                if (!flags.plain && j >= flags.rows_in) continue;
+                const float2 adjoint = add2(from, load_grad(j));
+                float2 dp = mul2(adjoint, u[j]);
+                float2 dc = mul2(adjoint, mul2(sub2(both(1.0f), a[j]), sub2(both(1.0f), mul2(k[j], k[j]))));
+                from = mul2(a[j], adjoint);
+                if (!flags.plain) {
+                    if (!(flags.live >> j & 1u)) dp = dc = both(0.0f);
+                    if (flags.cut >> j & 1u) from = both(0.0f);
+                }
+                features.store(row, dp);
+                features.store(row + shape.features, dc);
+            }
+            in -= int64_t(cluster) * kSegment * 2 * shape.features;
+            grad_in -= int64_t(cluster) * kSegment * shape.features;
+            grad_out -= int64_t(cluster) * kSegment * 2 * shape.features;
         }
+        if (grad_initial != nullptr && rank == 0 && walks_in) grad_initial[batch * shape.features + walked] = x;
     }
-    if (grad_initial != nullptr && rank == 0 && warp == 0) features.store_side(grad_initial + batch * shape.features, x);
 }
 
 // A tensor map over [batch, length, width] in boxes of one tile.
@@ -699,19 +819,31 @@ bool tma_rows(const GatedShape &shape, const void *projections, const void *grad
     return (shape.features * sizeof(T)) % 16 == 0 && aligned(projections, 16) && aligned(grad, 16) && aligned(out, 16);
 }
 
-// CTAs per chain: as many as fill the GPU (`resident` CTAs per SM), up to 8
-// and to the number of tiles.
-int cluster_size(const GatedShape &shape, int64_t chains, int resident) {
+// CTAs per chain: as many as the GPU holds at once (`resident` CTAs per SM),
+// up to `most` and to the number of tiles.
+int cluster_size(const GatedShape &shape, int64_t chains, int resident, int most) {
     int cluster = 1;
-    while (cluster < kMaxCluster && chains * cluster < int64_t(resident) * sm_count() && 2 * cluster <= shape.segments) cluster *= 2;
+    while (cluster < most && 2 * chains * cluster <= int64_t(resident) * sm_count() && 2 * cluster <= shape.segments) cluster *= 2;
     return cluster;
 }
 
+// Neighbouring chains a cluster walks one after the other: up to kItems tiles
+// per CTA, as long as the GPU's places are taken kRounds times over (with
+// fewer rounds the last, partly filled one costs more than a CTA's first load
+// and setup do).
+int chains_per_cluster(const GatedShape &shape, int64_t chains, int cluster, int resident) {
+    constexpr int64_t kItems = 8, kRounds = 4;
+    const int64_t waves = ceil_div(shape.segments, cluster), places = ceil_div(int64_t(resident) * sm_count(), cluster);
+    int64_t per = kItems / waves;
+    if (per > chains / (kRounds * places)) per = chains / (kRounds * places);
+    return per < 1 ? 1 : static_cast<int>(per);
+}
+
 template <typename... KernelArgs, typename... Args>
-int launch_tiles(void (*kernel)(KernelArgs...), int64_t chains, int cluster, size_t smem, cudaStream_t stream, Args &&...args) {
-    if (chains * cluster >= (int64_t(1) << 31)) return fail(KOEMI_ERR_UNSUPPORTED, "the recurrence has too many lanes");
+int launch_tiles(void (*kernel)(KernelArgs...), int64_t clusters, int cluster, size_t smem, cudaStream_t stream, Args &&...args) {
+    if (clusters * cluster >= (int64_t(1) << 31)) return fail(KOEMI_ERR_UNSUPPORTED, "the recurrence has too many lanes");
     KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    KOEMI_CUDA_TRY(launch_programmatic(false, kernel, dim3(static_cast<unsigned>(chains * cluster)), dim3(kTileThreads), smem,
+    KOEMI_CUDA_TRY(launch_programmatic(false, kernel, dim3(static_cast<unsigned>(clusters * cluster)), dim3(kTileThreads), smem,
                                        stream, dim3(cluster, 1, 1), std::forward<Args>(args)...));
     return KOEMI_OK;
 }
@@ -729,13 +861,16 @@ int gated_forward(const GatedShape &shape, const void *projections, const float 
     }
     const int64_t feature_tiles = ceil_div(shape.features, kTileFeatures);
     const int64_t chains = shape.batch * feature_tiles;
-    const int cluster = cluster_size(shape, chains, 3);
+    constexpr int kResident = sizeof(T) == 2 ? kForwardResident : 2;
+    const int cluster = cluster_size(shape, chains, kResident, kMaxCluster);
+    const int per = chains_per_cluster(shape, chains, cluster, kResident);
     const bool masks = shape.valid != nullptr || shape.restart != nullptr;
     int *status = device_status_word();
     CUtensorMap map{};
     auto go = [&](auto kernel, bool tma) {
-        return launch_tiles(kernel, chains, cluster, TileMemory<T, 2, forward_stages<T>()>::bytes(tma), stream, map, shape,
-                            feature_tiles, cluster, in, initial, out, final_state, carries, status);
+        const size_t smem = tma ? TileMemory<T, 2, 2, 2, 1>::bytes(cluster) : TileMemory<T, 2, 0, 2, 1>::bytes(cluster);
+        return launch_tiles(kernel, ceil_div(chains, per), cluster, smem, stream, map, shape,
+                            feature_tiles, cluster, per, in, initial, out, final_state, carries, status);
     };
     if (tma_rows<T>(shape, projections, nullptr, states)) {
         const int rc = tile_map<T>(&map, projections, shape.batch, shape.length, 2 * shape.features);
@@ -759,13 +894,15 @@ int gated_backward(const GatedShape &shape, const void *projections, const float
     }
     const int64_t feature_tiles = ceil_div(shape.features, kTileFeatures);
     const int64_t chains = shape.batch * feature_tiles;
-    const int cluster = cluster_size(shape, chains, 2);
+    const int cluster = cluster_size(shape, chains, kBackwardResident, kMaxCluster);
+    const int per = chains_per_cluster(shape, chains, cluster, kBackwardResident);
     const bool masks = shape.valid != nullptr || shape.restart != nullptr;
     int *status = device_status_word();
     CUtensorMap map{}, grad_map{};
     auto go = [&](auto kernel, bool tma) {
-        return launch_tiles(kernel, chains, cluster, TileMemory<T, 3, backward_stages<T>()>::bytes(tma), stream, map, grad_map,
-                            shape, feature_tiles, cluster, in, carries, grad, grad_final, out, grad_initial, status);
+        const size_t smem = tma ? TileMemory<T, 3, backward_stages<T>(), 3, 2>::bytes(cluster) : TileMemory<T, 3, 0, 3, 2>::bytes(cluster);
+        return launch_tiles(kernel, ceil_div(chains, per), cluster, smem, stream, map, grad_map,
+                            shape, feature_tiles, cluster, per, in, carries, grad, grad_final, out, grad_initial, status);
     };
     if (tma_rows<T>(shape, projections, grad_states, grad_projections)) {
         int rc = tile_map<T>(&map, projections, shape.batch, shape.length, 2 * shape.features);

@@ -21,7 +21,7 @@ from koemi_5hom_b200._native import DTYPE_CODES, ptr
 
 _LIBRARY = torch.library.Library("koemi_b200", "FRAGMENT")
 _HERE = nullcontext()
-SEGMENT = 64  # positions between two carries of the gated recurrence
+SEGMENT = 128  # positions between two carries of the gated recurrence
 
 
 def _define(schema: str, implementation, fake):
