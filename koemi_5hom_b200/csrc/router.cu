@@ -10,9 +10,16 @@
 //
 // Rows that are not valid, or whose logits are all -inf, take no part: ids
 // -1, weights 0, gradient 0. A NaN logit is never preferred, and its row's
-// probabilities are NaN. One warp works on one row at a time; a CTA adds its
-// rows' probabilities up in a fixed order and leaves one partial row, and a
-// second kernel adds the partial rows, so equal inputs give equal bits.
+// probabilities are NaN. A CTA adds its rows' probabilities up in a fixed order
+// and leaves one partial row, and a second kernel adds the partial rows, so
+// equal inputs give equal bits.
+//
+// Up to 256 experts a row is held in registers by a group of 8, 16 or 32
+// lanes, element e in lane e % lanes: every logit is loaded once, and a warp
+// works on 1 to 4 rows. Wider rows are walked from memory by one warp
+// (route_*_wide_kernel).
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace koemi {
@@ -53,7 +60,7 @@ __device__ RowSoftmax row_softmax(const T *row, int64_t experts, bool valid) {
 }
 
 template <typename T>
-__global__ void route_forward_kernel(RouteShape shape, const T *__restrict__ logits, int64_t *__restrict__ ids,
+__global__ void route_forward_wide_kernel(RouteShape shape, const T *__restrict__ logits, int64_t *__restrict__ ids,
                                      float *__restrict__ weights, float *__restrict__ partial_mass,
                                      int32_t *__restrict__ partial_counts, int32_t *__restrict__ partial_live) {
     extern __shared__ float mass[];  // [warps][experts], then counts [experts]
@@ -119,40 +126,261 @@ __global__ void route_forward_kernel(RouteShape shape, const T *__restrict__ log
     if (threadIdx.x == 0) partial_live[blockIdx.x] = live_rows;
 }
 
-__global__ void route_finish_kernel(const float *__restrict__ partial_mass, const int32_t *__restrict__ partial_counts,
-                                    const int32_t *__restrict__ partial_live, int64_t blocks, int64_t experts,
-                                    int64_t top_k, int64_t *__restrict__ counts, float *__restrict__ balance,
-                                    float *__restrict__ slope) {
-    __shared__ float sums[32];
+// Adds the partial rows: `parts` threads per expert take every parts-th block,
+// then one adds the parts, always in the same order.
+constexpr int kFinishThreads = 1024;
+__global__ __launch_bounds__(kFinishThreads) void route_finish_kernel(
+    const float *__restrict__ partial_mass, const int32_t *__restrict__ partial_counts,
+    const int32_t *__restrict__ partial_live, int blocks, int experts, int64_t top_k, int64_t *__restrict__ counts,
+    float *__restrict__ balance, float *__restrict__ slope) {
+    __shared__ double masses[kFinishThreads];
+    __shared__ int64_t pairs[kFinishThreads];
+    __shared__ int64_t live_sums[kFinishThreads / 32];
+    __shared__ float sums[kFinishThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t live = 0;
-    for (int64_t b = 0; b < blocks; ++b) live += partial_live[b];
-    const float n = static_cast<float>(live > 0 ? live : 1);
-    const float scale = static_cast<float>(experts) / n / (n * static_cast<float>(top_k));
+    int live = 0;
+    for (int b = threadIdx.x; b < blocks; b += kFinishThreads) live += partial_live[b];
+    live = __reduce_add_sync(0xffffffffu, live);
+    if (lane == 0) live_sums[warp] = live;
+    const int width = experts < kFinishThreads ? experts : kFinishThreads, parts = kFinishThreads / width;
+    const int part = threadIdx.x / width, column = threadIdx.x - part * width;
     float total = 0.0f;
-    for (int64_t e = threadIdx.x; e < experts; e += blockDim.x) {
+    for (int first = 0; first < experts; first += width) {
+        const int e = first + column;
         double mass = 0.0;
         int64_t count = 0;
-        for (int64_t b = 0; b < blocks; ++b) {
-            mass += partial_mass[b * experts + e];
-            count += partial_counts[b * experts + e];
+        if (part < parts && e < experts) {
+#pragma unroll 4
+            for (int b = part; b < blocks; b += parts) {
+                mass += partial_mass[int64_t(b) * experts + e];
+                count += partial_counts[int64_t(b) * experts + e];
+            }
         }
-        counts[e] = count;
-        slope[e] = scale * static_cast<float>(count);
-        total += static_cast<float>(mass) * slope[e];
+        masses[threadIdx.x] = mass;
+        pairs[threadIdx.x] = count;
+        __syncthreads();
+        if (part == 0 && e < experts) {
+            int64_t all = 0;
+            for (int w = 0; w < kFinishThreads / 32; ++w) all += live_sums[w];
+            for (int i = 1; i < parts; ++i) {
+                mass += masses[i * width + column];
+                count += pairs[i * width + column];
+            }
+            const float n = static_cast<float>(all > 0 ? all : 1);
+            const float s = static_cast<float>(experts) / n / (n * static_cast<float>(top_k)) * static_cast<float>(count);
+            counts[e] = count;
+            slope[e] = s;
+            total += static_cast<float>(mass) * s;
+        }
+        __syncthreads();
     }
     total = warp_sum(total);
     if (lane == 0) sums[warp] = total;
     __syncthreads();
     if (threadIdx.x == 0) {
         float all = 0.0f;
-        for (unsigned w = 0; w < blockDim.x / 32; ++w) all += sums[w];
+        for (int w = 0; w < kFinishThreads / 32; ++w) all += sums[w];
         *balance = all;
     }
 }
 
+// ------------------------------------------------------- rows in registers
+
+// e^(v - max): the difference is exact to half a unit, ex2.approx to 2 units.
+__device__ __forceinline__ float exp_from(float v, float max) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((v - max) * 1.4426950408889634f));
+    return r;
+}
+template <int kLanes>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+    for (int offset = kLanes / 2; offset > 0; offset >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, offset));
+    return v;
+}
+template <int kLanes>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int offset = kLanes / 2; offset > 0; offset >>= 1) v += __shfl_xor_sync(0xffffffffu, v, offset);
+    return v;
+}
+// Larger for what is chosen first: the value's order in the upper word (a NaN
+// ranks with -inf), the lower expert id first in the lower. 0: no candidate.
+__device__ __forceinline__ uint64_t rank_key(float v, int e) {
+    uint32_t bits = __float_as_uint(selectable(v) + 0.0f);  // -0 becomes +0
+    bits = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+    return static_cast<uint64_t>(bits) << 32 | static_cast<uint32_t>(~e);
+}
+
+// One row of a group: the lane's logits become exponentials; -inf beyond the row.
+template <typename T, int kLanes, int kPer>
+__device__ __forceinline__ RowSoftmax load_row(const T *row, int experts, int at, bool take, float (&logit)[kPer],
+                                               float (&e)[kPer]) {
+    float m = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int id = at + j * kLanes;
+        logit[j] = take && id < experts ? to_acc(row[id]) : -INFINITY;
+        nan |= isnan(logit[j]);
+        m = fmaxf(m, logit[j]);
+    }
+    m = group_max<kLanes>(m);
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        e[j] = exp_from(logit[j], m);
+        sum += at + j * kLanes < experts ? e[j] : 0.0f;
+    }
+    sum = group_sum<kLanes>(sum);
+    const bool any_nan = group_max<kLanes>(nan ? 1.0f : 0.0f) != 0.0f;  // the maximum passes NaNs over
+    return RowSoftmax{m, sum, take && (m != -INFINITY || any_nan)};
+}
+
+template <typename T, int kLanes, int kPer>
+__global__ __launch_bounds__(kRouteWarps * 32) void route_forward_kernel(
+    RouteShape shape, const T *__restrict__ logits, int64_t *__restrict__ ids, float *__restrict__ weights,
+    float *__restrict__ partial_mass, int32_t *__restrict__ partial_counts, int32_t *__restrict__ partial_live) {
+    constexpr int kGroups = kRouteWarps * 32 / kLanes, kWidth = kLanes * kPer;
+    __shared__ float mass[kRouteWarps][kWidth];
+    __shared__ int32_t counts[kWidth];
+    __shared__ int32_t live_rows;
+    const int at = threadIdx.x % kLanes, group = threadIdx.x / kLanes, warp = threadIdx.x >> 5;
+    const int experts = static_cast<int>(shape.experts), top_k = static_cast<int>(shape.top_k);
+    for (int i = threadIdx.x; i < kWidth; i += blockDim.x) counts[i] = 0;
+    if (threadIdx.x == 0) live_rows = 0;
+    __syncthreads();
+    float summed[kPer] = {};
+    int live = 0;
+    // every group of a warp takes the same number of turns: the shuffles are the warp's
+    for (int64_t first = int64_t(blockIdx.x) * kGroups; first < shape.tokens; first += int64_t(gridDim.x) * kGroups) {
+        const int64_t t = first + group;
+        const bool take = t < shape.tokens && (shape.valid == nullptr || shape.valid[t] != 0);
+        float logit[kPer], e[kPer];
+        const RowSoftmax soft = load_row<T, kLanes, kPer>(logits + t * shape.experts, experts, at, take, logit, e);
+        const float inverse = 1.0f / soft.sum;
+        uint64_t keys[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int id = at + j * kLanes;
+            keys[j] = id < experts ? rank_key(logit[j], id) : 0;
+            if (soft.live && id < experts) summed[j] += e[j] * inverse;
+        }
+        live += soft.live && at == 0;
+        float chosen = 0.0f, first_weight = 0.0f;
+        for (int k = 0; k < top_k; ++k) {
+            uint64_t best = keys[0];
+#pragma unroll
+            for (int j = 1; j < kPer; ++j) best = keys[j] > best ? keys[j] : best;
+#pragma unroll
+            for (int offset = kLanes / 2; offset > 0; offset >>= 1) {
+                const uint64_t other = __shfl_xor_sync(0xffffffffu, best, offset);
+                best = other > best ? other : best;
+            }
+            const int id = static_cast<int>(~static_cast<uint32_t>(best));
+            float p = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                if (keys[j] == best) {
+                    p = e[j] * inverse;
+                    keys[j] = 0;
+                }
+            }
+            p = __shfl_sync(0xffffffffu, p, id % kLanes, kLanes);
+            chosen += p;
+            if (k % kLanes == at) first_weight = p;
+            if (t < shape.tokens && at == 0) {
+                ids[t * top_k + k] = soft.live ? id : -1;
+                if (soft.live) atomicAdd(&counts[id], 1);
+            }
+            // a lane keeps every kLanes-th weight; they are written kLanes at a time
+            if (t < shape.tokens && !shape.renormalize && (k % kLanes == kLanes - 1 || k == top_k - 1)) {
+                const int slot = k / kLanes * kLanes + at;
+                if (slot <= k) weights[t * top_k + slot] = soft.live ? first_weight : 0.0f;
+            }
+            if (shape.renormalize && t < shape.tokens && at == 0) weights[t * top_k + k] = soft.live ? p : 0.0f;
+        }
+        if (shape.renormalize && t < shape.tokens && at == 0 && soft.live) {
+            for (int k = 0; k < top_k; ++k) weights[t * top_k + k] /= chosen;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        // the warp's groups, then the CTA's warps
+#pragma unroll
+        for (int offset = kLanes; offset < 32; offset <<= 1) summed[j] += __shfl_xor_sync(0xffffffffu, summed[j], offset);
+        if ((threadIdx.x & 31) < kLanes) mass[warp][at + j * kLanes] = summed[j];
+    }
+    if (live > 0) atomicAdd(&live_rows, live);
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRouteWarps; ++w) sum += mass[w][e];
+        partial_mass[int64_t(blockIdx.x) * experts + e] = sum;
+        partial_counts[int64_t(blockIdx.x) * experts + e] = counts[e];
+    }
+    if (threadIdx.x == 0) partial_live[blockIdx.x] = live_rows;
+}
+
+template <typename T, int kLanes, int kPer>
+__global__ __launch_bounds__(kRouteWarps * 32) void route_backward_kernel(
+    RouteShape shape, const T *__restrict__ logits, const int64_t *__restrict__ ids, const float *__restrict__ weights,
+    const float *__restrict__ grad_weights, const float *__restrict__ grad_balance, const float *__restrict__ slope,
+    T *__restrict__ grad_logits) {
+    constexpr int kGroups = kRouteWarps * 32 / kLanes;
+    const int at = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    const int experts = static_cast<int>(shape.experts), top_k = static_cast<int>(shape.top_k);
+    const float db = grad_balance != nullptr ? *grad_balance : 0.0f;
+    float base[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) base[j] = at + j * kLanes < experts ? db * slope[at + j * kLanes] : 0.0f;
+    for (int64_t first = int64_t(blockIdx.x) * kGroups; first < shape.tokens; first += int64_t(gridDim.x) * kGroups) {
+        const int64_t t = first + group;
+        const int64_t *chosen = ids + t * top_k;
+        const bool live = t < shape.tokens && chosen[0] >= 0;
+        float logit[kPer], e[kPer];
+        const RowSoftmax soft = load_row<T, kLanes, kPer>(logits + t * shape.experts, experts, at, live, logit, e);
+        const float inverse = 1.0f / soft.sum;
+        float dp[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            e[j] *= inverse;
+            dp[j] = base[j];
+        }
+        if (live && grad_weights != nullptr) {
+            const float *gw = grad_weights + t * top_k;
+            float mean = 0.0f, scale = 1.0f;
+            if (shape.renormalize) {
+                // a weight is its probability over their sum; the largest weight's probability gives the sum
+                for (int k = 0; k < top_k; ++k) mean = fmaf(gw[k], weights[t * top_k + k], mean);
+                scale = weights[t * top_k] / (exp_from(to_acc(logits[t * shape.experts + chosen[0]]), soft.max) * inverse);
+            }
+            for (int k = 0; k < top_k; ++k) {
+                const int id = static_cast<int>(chosen[k]);
+                const float g = (gw[k] - mean) * scale;
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) dp[j] += id == at + j * kLanes ? g : 0.0f;
+            }
+        }
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) dot += at + j * kLanes < experts ? e[j] * dp[j] : 0.0f;
+        dot = group_sum<kLanes>(dot);
+        if (t < shape.tokens) {
+            T *out = grad_logits + t * shape.experts;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                if (at + j * kLanes < experts) out[at + j * kLanes] = from_acc<T>(live ? e[j] * (dp[j] - dot) : 0.0f);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------ wider rows
+
 template <typename T>
-__global__ void route_backward_kernel(RouteShape shape, const T *__restrict__ logits, const int64_t *__restrict__ ids,
+__global__ void route_backward_wide_kernel(RouteShape shape, const T *__restrict__ logits, const int64_t *__restrict__ ids,
                                       const float *__restrict__ weights, const float *__restrict__ grad_weights,
                                       const float *__restrict__ grad_balance, const float *__restrict__ slope,
                                       T *__restrict__ grad_logits) {
@@ -198,9 +426,23 @@ __global__ void route_backward_kernel(RouteShape shape, const T *__restrict__ lo
     }
 }
 
-int64_t route_blocks(int64_t tokens) {
-    const int64_t blocks = ceil_div(tokens, kRouteWarps);
+// Rows a CTA takes in one turn: a warp each, or a group of lanes each.
+int rows_per_turn(int64_t experts) {
+    return experts <= 32 ? kRouteWarps * 4 : experts <= 64 ? kRouteWarps * 2 : kRouteWarps;
+}
+int64_t route_blocks(int64_t tokens, int64_t experts) {
+    const int64_t blocks = ceil_div(tokens, rows_per_turn(experts));
     return blocks < kRouteBlocks ? (blocks > 0 ? blocks : 1) : kRouteBlocks;
+}
+
+// Calls go(lanes, per) with the register layout of `experts`, or returns false.
+template <typename F>
+bool with_layout(int64_t experts, F &&go) {
+    if (experts <= 32) return go(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{}), true;
+    if (experts <= 64) return go(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{}), true;
+    if (experts <= 128) return go(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{}), true;
+    if (experts <= 256) return go(std::integral_constant<int, 32>{}, std::integral_constant<int, 8>{}), true;
+    return false;
 }
 
 int check_route(const RouteShape &shape) {
@@ -215,18 +457,26 @@ int check_route(const RouteShape &shape) {
 template <typename T>
 int route_forward(const RouteShape &shape, const void *logits, int64_t *ids, float *weights, int64_t *counts,
                   float *balance, float *slope, void *workspace, cudaStream_t stream) {
-    const int64_t blocks = route_blocks(shape.tokens);
+    const int64_t blocks = route_blocks(shape.tokens, shape.experts);
     float *mass = static_cast<float *>(workspace);
     int32_t *partial_counts = reinterpret_cast<int32_t *>(mass + blocks * shape.experts);
     int32_t *live = partial_counts + blocks * shape.experts;
-    const size_t smem = (kRouteWarps + 1) * shape.experts * sizeof(float);
-    auto kernel = route_forward_kernel<T>;
-    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    kernel<<<static_cast<unsigned>(blocks), kRouteWarps * 32, smem, stream>>>(
-        shape, static_cast<const T *>(logits), ids, weights, mass, partial_counts, live);
+    const T *in = static_cast<const T *>(logits);
+    const unsigned grid = static_cast<unsigned>(blocks);
+    const bool narrow = with_layout(shape.experts, [&](auto lanes, auto per) {
+        route_forward_kernel<T, lanes.value, per.value><<<grid, kRouteWarps * 32, 0, stream>>>(
+            shape, in, ids, weights, mass, partial_counts, live);
+    });
+    if (!narrow) {
+        const size_t smem = (kRouteWarps + 1) * shape.experts * sizeof(float);
+        auto kernel = route_forward_wide_kernel<T>;
+        KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+        kernel<<<grid, kRouteWarps * 32, smem, stream>>>(shape, in, ids, weights, mass, partial_counts, live);
+    }
     KOEMI_LAUNCH_CHECK();
-    route_finish_kernel<<<1, 512, 0, stream>>>(mass, partial_counts, live, blocks, shape.experts, shape.top_k, counts,
-                                               balance, slope);
+    route_finish_kernel<<<1, kFinishThreads, 0, stream>>>(mass, partial_counts, live, static_cast<int>(blocks),
+                                                          static_cast<int>(shape.experts), shape.top_k, counts, balance,
+                                                          slope);
     KOEMI_LAUNCH_CHECK();
     return KOEMI_OK;
 }
@@ -235,9 +485,17 @@ template <typename T>
 int route_backward(const RouteShape &shape, const void *logits, const int64_t *ids, const float *weights,
                    const float *grad_weights, const float *grad_balance, const float *slope, void *grad_logits,
                    cudaStream_t stream) {
-    route_backward_kernel<T><<<static_cast<unsigned>(route_blocks(shape.tokens)), kRouteWarps * 32, 0, stream>>>(
-        shape, static_cast<const T *>(logits), ids, weights, grad_weights, grad_balance, slope,
-        static_cast<T *>(grad_logits));
+    const T *in = static_cast<const T *>(logits);
+    T *out = static_cast<T *>(grad_logits);
+    const unsigned grid = static_cast<unsigned>(route_blocks(shape.tokens, shape.experts));
+    const bool narrow = with_layout(shape.experts, [&](auto lanes, auto per) {
+        route_backward_kernel<T, lanes.value, per.value><<<grid, kRouteWarps * 32, 0, stream>>>(
+            shape, in, ids, weights, grad_weights, grad_balance, slope, out);
+    });
+    if (!narrow) {
+        route_backward_wide_kernel<T><<<grid, kRouteWarps * 32, 0, stream>>>(shape, in, ids, weights, grad_weights,
+                                                                             grad_balance, slope, out);
+    }
     KOEMI_LAUNCH_CHECK();
     return KOEMI_OK;
 }
@@ -249,7 +507,7 @@ using namespace koemi;
 
 extern "C" size_t koemi_moe_route_learned_workspace(int64_t tokens, int64_t expert_count) {
     if (tokens < 0 || expert_count < 1) return 0;
-    const int64_t blocks = route_blocks(tokens);
+    const int64_t blocks = route_blocks(tokens, expert_count);
     return static_cast<size_t>(blocks * (2 * expert_count + 1)) * 4;
 }
 
