@@ -9,21 +9,34 @@
 //
 // Rows that are not valid read nothing of their logits, give log-prob 0 and
 // gradient 0. A target outside [0, vocab) makes its row's log-prob NaN.
-// A CTA takes whole rows; per-CTA sums are added in a fixed order by a second
-// kernel, so equal inputs give equal bits.
+//
+// The logits are read once and their gradient is written once, in one pass
+// over the rows, bound by HBM. Up to 1024 entries a warp holds a row in
+// registers. Up to 32768 a CTA of 256, 512 or 1024 threads does: a bulk copy
+// brings the row into shared memory (the next rows' copies run meanwhile), a
+// thread turns 32 entries into exponentials relative to its warp's maximum,
+// the warps' (maximum, sum) pairs meet at the row's only barrier, and the
+// gradient is the kept exponential times one factor per warp: one exponential
+// per entry, one read of shared memory. Longer rows are walked twice from
+// memory in blocks of 32768, the second time mostly from L2.
+// Every row belongs to one CTA and per-CTA sums are added in a fixed order by
+// a second kernel, so equal inputs give equal bits.
 #include "vec.cuh"
 
 namespace koemi {
 namespace {
 
-constexpr int kPolicyThreads = 256;
-constexpr int kPolicyBlocks = 592;
+constexpr int kPolicyBlocks = 1184;     // most CTAs of a launch: eight per SM
+constexpr int kWarpRow = 1024;          // entries a warp holds
+constexpr int kPerThread = 32;          // entries a thread holds
+constexpr int64_t kCountedRows = 16384; // up to here every CTA counts the valid rows itself
+constexpr float kLog2e = 1.4426950408889634f;
 
 // Row r of the logits starts at (r / inner) * outer_stride + (r % inner) *
 // inner_stride elements.
 struct PolicyRows {
     int64_t rows, vocab, inner, outer_stride, inner_stride;
-    __device__ int64_t start(int64_t row) const {
+    __device__ __forceinline__ int64_t start(int64_t row) const {
         return (row / inner) * outer_stride + (row % inner) * inner_stride;
     }
 };
@@ -34,25 +47,6 @@ struct PolicyTerms {
     const uint8_t *valid;                       // may be NULL: every row
     float clip_low, clip_high, beta;
 };
-
-__device__ __forceinline__ float block_max(float v, float *scratch) {
-    v = warp_max(v);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = scratch[0];
-    for (unsigned w = 1; w < blockDim.x / 32; ++w) v = fmaxf(v, scratch[w]);
-    __syncthreads();
-    return v;
-}
-__device__ __forceinline__ float block_sum(float v, float *scratch) {
-    v = warp_sum(v);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0f;
-    for (unsigned w = 0; w < blockDim.x / 32; ++w) v += scratch[w];
-    __syncthreads();
-    return v;
-}
 
 // Loss, KL and d loss / d log-prob of one row.
 __device__ __forceinline__ void policy_terms(const PolicyTerms &terms, int64_t row, float lp, float &loss, float &kl,
@@ -75,116 +69,516 @@ __device__ __forceinline__ void policy_terms(const PolicyTerms &terms, int64_t r
     if (isnan(free) || isnan(clipped)) loss = slope = NAN;
 }
 
-__global__ void policy_count_kernel(const uint8_t *__restrict__ valid, int64_t rows, float *__restrict__ inverse) {
+__device__ __forceinline__ bool aligned_to(const void *p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// 1 / (valid rows), by one CTA. 16 flags at a time where they are aligned.
+__device__ float inverse_count(const uint8_t *valid, int64_t rows) {
     __shared__ int32_t sums[32];
+    if (valid == nullptr) return 1.0f / static_cast<float>(rows > 0 ? rows : 1);
     int32_t count = 0;
-    for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) count += valid == nullptr || valid[i] != 0;
+    const int64_t packets = aligned_to(valid, 16) ? rows / 16 : 0;
+    for (int64_t i = threadIdx.x; i < packets; i += blockDim.x) {
+        const uint4 raw = load_cached(valid + 16 * i);
+        // a bool is one byte of value 0 or 1
+        count += __popc(__vcmpne4(raw.x, 0) & 0x01010101u) + __popc(__vcmpne4(raw.y, 0) & 0x01010101u) +
+                 __popc(__vcmpne4(raw.z, 0) & 0x01010101u) + __popc(__vcmpne4(raw.w, 0) & 0x01010101u);
+    }
+    for (int64_t i = 16 * packets + threadIdx.x; i < rows; i += blockDim.x) count += valid[i] != 0;
     count = __reduce_add_sync(0xffffffffu, count);
     if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = count;
     __syncthreads();
+    int64_t all = 0;
+    for (unsigned w = 0; w < blockDim.x / 32; ++w) all += sums[w];
+    __syncthreads();
+    return 1.0f / static_cast<float>(all > 0 ? all : 1);
+}
+
+__global__ void policy_count_kernel(const uint8_t *__restrict__ valid, int64_t rows, float *__restrict__ inverse) {
+    const float v = inverse_count(valid, rows);
+    if (threadIdx.x == 0) *inverse = v;
+}
+
+__device__ __forceinline__ float ex2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// e^(v - m), m a maximum: the difference is exact to half a unit in its last
+// place whatever the logits' magnitude (the type's lowest value in every entry
+// gives a uniform row); ex2.approx adds 2 units. A maximum of nothing but -inf
+// counts as 0, so that its entries give 0.
+__device__ __forceinline__ float origin(float max) { return max == -INFINITY ? 0.0f : max; }
+__device__ __forceinline__ float exp_from(float v, float from) { return ex2_approx((v - from) * kLog2e); }
+
+// A maximum and the sum of e^(entry - it) over a thread's, a warp's, a row's entries.
+struct Partial {
+    float max, sum;
+};
+__device__ __forceinline__ Partial warp_merge(Partial p) {
+    const float m = warp_max(p.max);
+    return Partial{m, warp_sum(p.sum * exp_from(p.max, origin(m)))};
+}
+__device__ __forceinline__ float lse_of(Partial p) { return p.max + logf(p.sum); }
+
+// What a forward kernel writes beside the gradient.
+struct PolicyOut {
+    const float *inverse;  // NULL: the CTA counts the valid rows
+    float *log_probs, *lse, *slopes;
+    float2 *partials;
+};
+
+// A row's scalars, loaded ahead of its logits.
+template <typename T>
+struct RowScalars {
+    int64_t target;
+    float chosen;
+    __device__ RowScalars(const T *row, const PolicyTerms &terms, int64_t index, int64_t vocab) {
+        target = terms.targets[index];
+        chosen = target >= 0 && target < vocab ? to_acc(row[target]) : NAN;
+    }
+};
+
+// Up to 1024 entries: a warp per row, entry v in lane v % 32.
+template <typename T, int kPer>
+__global__ __launch_bounds__(256) void policy_warp_kernel(PolicyRows shape, PolicyTerms terms,
+                                                          const T *__restrict__ logits, PolicyOut result,
+                                                          T *__restrict__ grad_logits) {
+    __shared__ float2 sums[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, vocab = static_cast<int>(shape.vocab);
+    const float scale = result.inverse != nullptr ? *result.inverse : inverse_count(terms.valid, shape.rows);
+    float loss_sum = 0.0f, kl_sum = 0.0f;
+    for (int64_t row = int64_t(blockIdx.x) * 8 + warp; row < shape.rows; row += int64_t(gridDim.x) * 8) {
+        T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
+        if (terms.valid != nullptr && terms.valid[row] == 0) {
+            if (out != nullptr) {
+                for (int v = lane; v < vocab; v += 32) out[v] = from_acc<T>(0.0f);
+            }
+            if (lane == 0) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
+            continue;
+        }
+        const T *in = logits + shape.start(row);
+        const RowScalars<T> scalars(in, terms, row, vocab);
+        float e[kPer];
+        Partial p{-INFINITY, 0.0f};
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            e[j] = lane + 32 * j < vocab ? to_acc(in[lane + 32 * j]) : -INFINITY;
+            p.max = fmaxf(p.max, e[j]);
+        }
+        p.max = warp_max(p.max);
+        const float from = origin(p.max);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            e[j] = exp_from(e[j], from);
+            p.sum += e[j];
+        }
+        p.sum = warp_sum(p.sum);
+        const float lse = lse_of(p), lp = scalars.chosen - lse;
+        float loss, kl, slope;
+        policy_terms(terms, row, lp, loss, kl, slope);
+        loss_sum += loss;
+        kl_sum += kl;
+        slope *= scale;
+        if (lane == 0) {
+            result.log_probs[row] = lp;
+            result.lse[row] = lse;
+            result.slopes[row] = slope;
+        }
+        if (out != nullptr) {
+            const float factor = -slope / p.sum;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const int v = lane + 32 * j;
+                if (v < vocab) out[v] = from_acc<T>(fmaf(e[j], factor, v == scalars.target ? slope : 0.0f));
+            }
+        }
+    }
+    if (lane == 0) sums[warp] = make_float2(loss_sum, kl_sum);
+    __syncthreads();
     if (threadIdx.x == 0) {
-        int64_t all = 0;
-        for (unsigned w = 0; w < blockDim.x / 32; ++w) all += sums[w];
-        *inverse = 1.0f / static_cast<float>(all > 0 ? all : 1);
+        for (int w = 1; w < 8; ++w) {
+            loss_sum += sums[w].x;
+            kl_sum += sums[w].y;
+        }
+        result.partials[blockIdx.x] = make_float2(loss_sum, kl_sum);
     }
 }
 
+// A row in packets of 16 bytes at 16-byte boundaries: packet c holds entries
+// c width - skip and following; the first and the last may be partly outside.
 template <typename T>
-__global__ __launch_bounds__(kPolicyThreads) void policy_forward_kernel(
-    PolicyRows shape, PolicyTerms terms, const T *__restrict__ logits, const float *__restrict__ inverse,
-    float *__restrict__ log_probs, float *__restrict__ lse_out, float *__restrict__ slope_out,
-    T *__restrict__ grad_logits, float2 *__restrict__ partials) {
-    __shared__ float scratch[kPolicyThreads / 32];
-    const float scale = *inverse;
+struct Packets {
+    static constexpr int kWidth = Pack<T>::kWidth;
+    const T *base;  // the boundary at or before the row's start
+    int skip;
+    int64_t vocab, count;
+    __device__ Packets(const T *row, int64_t vocab_) : vocab(vocab_) {
+        skip = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
+        base = row - skip;
+        count = (skip + vocab + kWidth - 1) / kWidth;
+    }
+    __device__ __forceinline__ bool whole(int64_t c) const { return c * kWidth >= skip && (c + 1) * kWidth <= skip + vocab; }
+    __device__ __forceinline__ int64_t first_whole() const { return skip > 0 ? 1 : 0; }
+    __device__ __forceinline__ int64_t end_whole() const { return (skip + vocab) / kWidth; }
+    __device__ __forceinline__ bool in_row(int64_t c, int i) const {
+        const int64_t at = c * kWidth + i;
+        return at >= skip && at < skip + vocab;
+    }
+    // entries of a packet that is partly outside, one by one
+    __device__ __forceinline__ void load_partly(int64_t c, float (&v)[kWidth]) const {
+#pragma unroll
+        for (int i = 0; i < kWidth; ++i) v[i] = in_row(c, i) ? to_acc(base[c * kWidth + i]) : -INFINITY;
+    }
+    // v into packet c of the row at `out`, whose packets lie as this row's
+    // where `fits`, else one by one
+    __device__ __forceinline__ void store(T *out, bool fits, int64_t c, const float (&v)[kWidth]) const {
+        T *to = out - skip + c * kWidth;
+        if (fits && whole(c)) {
+            *reinterpret_cast<uint4 *>(to) = pack(v, T());
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kWidth; ++i) {
+            if (in_row(c, i)) to[i] = from_acc<T>(v[i]);
+        }
+    }
+    __device__ __forceinline__ bool fits(const T *out) const {
+        return reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T) == static_cast<unsigned>(skip);
+    }
+};
+
+// Zeros into a row of the gradient, by a CTA.
+template <typename T>
+__device__ void clear_row(T *out, int64_t vocab) {
+    const Packets<T> packets(out, vocab);
+    float zeros[Packets<T>::kWidth] = {};
+    for (int64_t c = threadIdx.x; c < packets.count; c += blockDim.x) packets.store(out, true, c, zeros);
+}
+
+// The warps' partials of a row, merged by every warp alike: the row's partial
+// from one barrier. `place` alternates between two rows.
+template <int kThreads>
+__device__ __forceinline__ Partial block_merge(Partial p, Partial (*place)[32], int parity) {
+    constexpr int kWarps = kThreads / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (lane == 0) place[parity][warp] = p;
+    __syncthreads();
+    p = lane < kWarps ? place[parity][lane] : Partial{-INFINITY, 0.0f};
+    return warp_merge(p);
+}
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_addr(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+// Up to 32 entries a thread: a CTA per row at a time.
+template <typename T, int kThreads>
+__global__ __launch_bounds__(kThreads, 1024 / kThreads) void policy_row_kernel(
+    PolicyRows shape, PolicyTerms terms, const T *__restrict__ logits, PolicyOut result, T *__restrict__ grad_logits,
+    int buffers, uint32_t buffer_bytes, int *status) {
+    constexpr int kWidth = Pack<T>::kWidth, kPackets = kPerThread / kWidth;
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    __shared__ uint64_t full[4];
+    __shared__ Partial merged[2][32];
+    auto live = [&](int64_t row) { return terms.valid == nullptr || terms.valid[row] != 0; };
+    int64_t next = blockIdx.x;  // thread 0: the next row to load
+    int loaded = 0;
+    auto load_next = [&] {
+        while (next < shape.rows && !live(next)) next += gridDim.x;
+        if (next >= shape.rows) return;
+        const Packets<T> packets(logits + shape.start(next), shape.vocab);
+        const int64_t first = packets.first_whole(), end = packets.end_whole();
+        uint64_t *bar = &full[loaded % buffers];
+        if (end > first) {
+            const uint32_t bytes = static_cast<uint32_t>(end - first) * 16;
+            mbar_arrive_expect_tx(bar, bytes);
+            bulk_load(smem_raw + loaded % buffers * buffer_bytes + first * 16, packets.base + first * kWidth, bytes, bar);
+        } else {
+            mbar_arrive(bar);
+        }
+        ++loaded;
+        next += gridDim.x;
+    };
+    if (threadIdx.x == 0) {
+        for (int b = 0; b < buffers; ++b) mbar_init(&full[b], 1);
+        fence_barrier_init();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int b = 0; b < buffers; ++b) load_next();
+    }
+    const float scale = result.inverse != nullptr ? *result.inverse : inverse_count(terms.valid, shape.rows);
     float loss_sum = 0.0f, kl_sum = 0.0f;
+    bool dead = false;  // a copy never arrived: go on without waiting or loading
+    int taken = 0;
     for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
-        const T *in = logits + shape.start(row);
         T *out = grad_logits == nullptr ? nullptr : grad_logits + row * shape.vocab;
-        if (terms.valid != nullptr && terms.valid[row] == 0) {
-            if (out != nullptr) {
-                for (int64_t v = threadIdx.x; v < shape.vocab; v += blockDim.x) out[v] = from_acc<T>(0.0f);
-            }
-            if (threadIdx.x == 0) log_probs[row] = lse_out[row] = slope_out[row] = 0.0f;
+        if (!live(row)) {
+            if (out != nullptr) clear_row(out, shape.vocab);
+            if (threadIdx.x == 0) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
             continue;
         }
-        float m = -INFINITY;
-        for (int64_t v = threadIdx.x; v < shape.vocab; v += blockDim.x) m = fmaxf(m, to_acc(in[v]));
-        m = block_max(m, scratch);
-        float sum = 0.0f;
-        for (int64_t v = threadIdx.x; v < shape.vocab; v += blockDim.x) sum += expf(to_acc(in[v]) - m);
-        sum = block_sum(sum, scratch);
-        const float lse = m + logf(sum);
-        const int64_t target = terms.targets[row];
-        const float lp = target >= 0 && target < shape.vocab ? to_acc(in[target]) - lse : NAN;
+        const T *in = logits + shape.start(row);
+        const RowScalars<T> scalars(in, terms, row, shape.vocab);
+        const Packets<T> packets(in, shape.vocab);
+        const uint4 *staged = reinterpret_cast<const uint4 *>(smem_raw + taken % buffers * buffer_bytes);
+        if (!dead) dead = !mbar_wait_bounded(&full[taken % buffers], static_cast<uint32_t>(taken / buffers) & 1, status);
+
+        float e[kPackets][kWidth];
+        Partial p{-INFINITY, 0.0f};
+#pragma unroll
+        for (int j = 0; j < kPackets; ++j) {
+            const int c = threadIdx.x + j * kThreads;
+            if (c < packets.count && packets.whole(c)) {
+                unpack(staged[c], e[j], T());
+            } else {
+                packets.load_partly(c, e[j]);  // -inf throughout where c is behind the row
+            }
+#pragma unroll
+            for (int i = 0; i < kWidth; ++i) p.max = fmaxf(p.max, e[j][i]);
+        }
+        p.max = warp_max(p.max);
+        const float from = origin(p.max);
+#pragma unroll
+        for (int j = 0; j < kPackets; ++j) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kWidth; ++i) {
+                e[j][i] = exp_from(e[j][i], from);
+                sum += e[j][i];
+            }
+            p.sum += sum;
+        }
+        p.sum = warp_sum(p.sum);
+        const Partial all = block_merge<kThreads>(p, merged, taken & 1);
+        // every thread is done with the row's buffer
+        if (threadIdx.x == 0 && !dead) load_next();
+        ++taken;
+
+        const float lse = lse_of(all), lp = scalars.chosen - lse;
         float loss, kl, slope;
         policy_terms(terms, row, lp, loss, kl, slope);
         loss_sum += loss;
         kl_sum += kl;
         slope *= scale;
         if (threadIdx.x == 0) {
-            log_probs[row] = lp;
-            lse_out[row] = lse;
-            slope_out[row] = slope;
+            result.log_probs[row] = lp;
+            result.lse[row] = lse;
+            result.slopes[row] = slope;
         }
         if (out != nullptr) {
-            for (int64_t v = threadIdx.x; v < shape.vocab; v += blockDim.x) {
-                out[v] = from_acc<T>(slope * ((v == target ? 1.0f : 0.0f) - expf(to_acc(in[v]) - lse)));
+            const float factor = -slope / all.sum * exp_from(from, all.max);
+            const bool fits = packets.fits(out);
+            const int64_t at = scalars.target + packets.skip;  // the target's place among the packets' entries
+#pragma unroll
+            for (int j = 0; j < kPackets; ++j) {
+                const int c = threadIdx.x + j * kThreads;
+                if (c >= packets.count) continue;
+#pragma unroll
+                for (int i = 0; i < kWidth; ++i) e[j][i] *= factor;
+                if (at / kWidth == c) {
+#pragma unroll
+                    for (int i = 0; i < kWidth; ++i) e[j][i] += at % kWidth == i ? slope : 0.0f;
+                }
+                packets.store(out, fits, c, e[j]);
             }
         }
     }
-    if (threadIdx.x == 0) partials[blockIdx.x] = make_float2(loss_sum, kl_sum);
+    if (threadIdx.x == 0) result.partials[blockIdx.x] = make_float2(loss_sum, kl_sum);
 }
 
-__global__ void policy_finish_kernel(const float2 *__restrict__ partials, int64_t count,
-                                     const float *__restrict__ inverse, float *__restrict__ loss,
-                                     float *__restrict__ kl) {
+// Longer rows, in blocks of 1024 threads x 32 entries, walked twice.
+constexpr int kWalkThreads = 1024;
+template <typename T>
+__global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows shape, PolicyTerms terms,
+                                                                   const T *__restrict__ logits, PolicyOut result,
+                                                                   T *__restrict__ grad_logits) {
+    constexpr int kWidth = Pack<T>::kWidth, kPackets = kPerThread / kWidth / 2;  // in flight per thread
+    __shared__ Partial merged[2][32];
+    const float scale = result.inverse != nullptr ? *result.inverse : inverse_count(terms.valid, shape.rows);
+    float loss_sum = 0.0f, kl_sum = 0.0f;
+    int taken = 0;
+    for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
+        T *out = grad_logits == nullptr ? nullptr : grad_logits + row * shape.vocab;
+        if (terms.valid != nullptr && terms.valid[row] == 0) {
+            if (out != nullptr) clear_row(out, shape.vocab);
+            if (threadIdx.x == 0) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
+            continue;
+        }
+        const T *in = logits + shape.start(row);
+        const RowScalars<T> scalars(in, terms, row, shape.vocab);
+        const Packets<T> packets(in, shape.vocab);
+        auto walk = [&](auto &&each) {
+            for (int64_t first = threadIdx.x; first < packets.count; first += kPackets * kWalkThreads) {
+                uint4 raw[kPackets];
+#pragma unroll
+                for (int j = 0; j < kPackets; ++j) {
+                    const int64_t c = first + j * kWalkThreads;
+                    raw[j] = c < packets.count && packets.whole(c) ? load_cached(packets.base + c * kWidth) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < kPackets; ++j) {
+                    const int64_t c = first + j * kWalkThreads;
+                    if (c >= packets.count) continue;
+                    float v[kWidth];
+                    if (packets.whole(c)) {
+                        unpack(raw[j], v, T());
+                    } else {
+                        packets.load_partly(c, v);
+                    }
+                    each(c, v);
+                }
+            }
+        };
+        Partial p{-INFINITY, 0.0f};
+        walk([&](int64_t, const float (&v)[kWidth]) {
+            float m = v[0];
+#pragma unroll
+            for (int i = 1; i < kWidth; ++i) m = fmaxf(m, v[i]);
+            if (m > p.max) {
+                p.sum *= exp_from(p.max, m);
+                p.max = m;
+            }
+            const float from = origin(p.max);
+#pragma unroll
+            for (int i = 0; i < kWidth; ++i) p.sum += exp_from(v[i], from);
+        });
+        const Partial all = block_merge<kWalkThreads>(warp_merge(p), merged, taken++ & 1);
+        const float lse = lse_of(all), lp = scalars.chosen - lse;
+        float loss, kl, slope;
+        policy_terms(terms, row, lp, loss, kl, slope);
+        loss_sum += loss;
+        kl_sum += kl;
+        slope *= scale;
+        if (threadIdx.x == 0) {
+            result.log_probs[row] = lp;
+            result.lse[row] = lse;
+            result.slopes[row] = slope;
+        }
+        if (out != nullptr) {
+            const float factor = -slope / all.sum;
+            const bool fits = packets.fits(out);
+            const int64_t at = scalars.target + packets.skip;
+            walk([&](int64_t c, float (&v)[kWidth]) {
+#pragma unroll
+                for (int i = 0; i < kWidth; ++i) v[i] = exp_from(v[i], all.max) * factor;
+                if (at / kWidth == c) {
+#pragma unroll
+                    for (int i = 0; i < kWidth; ++i) v[i] += at % kWidth == i ? slope : 0.0f;
+                }
+                packets.store(out, fits, c, v);
+            });
+        }
+    }
+    if (threadIdx.x == 0) result.partials[blockIdx.x] = make_float2(loss_sum, kl_sum);
+}
+
+constexpr int kFinishThreads = 256;
+__global__ __launch_bounds__(kFinishThreads) void policy_finish_kernel(const float2 *__restrict__ partials, int count,
+                                                                       const float *__restrict__ inverse,
+                                                                       const uint8_t *__restrict__ valid, int64_t rows,
+                                                                       float *__restrict__ loss, float *__restrict__ kl) {
+    __shared__ double sums[2][kFinishThreads / 32];
     double l = 0.0, k = 0.0;
-    for (int64_t i = threadIdx.x; i < count; i += 32) {
+    for (int i = threadIdx.x; i < count; i += kFinishThreads) {
         l += partials[i].x;
         k += partials[i].y;
     }
+    const float scale = inverse != nullptr ? *inverse : inverse_count(valid, rows);
 #pragma unroll
     for (int offset = 16; offset > 0; offset >>= 1) {
         l += __shfl_xor_sync(0xffffffffu, l, offset);
         k += __shfl_xor_sync(0xffffffffu, k, offset);
     }
+    if ((threadIdx.x & 31) == 0) {
+        sums[0][threadIdx.x >> 5] = l;
+        sums[1][threadIdx.x >> 5] = k;
+    }
+    __syncthreads();
     if (threadIdx.x == 0) {
-        *loss = static_cast<float>(l * *inverse);
-        *kl = static_cast<float>(k * *inverse);
+        for (int w = 1; w < kFinishThreads / 32; ++w) {
+            l += sums[0][w];
+            k += sums[1][w];
+        }
+        *loss = static_cast<float>(l * scale);
+        *kl = static_cast<float>(k * scale);
     }
 }
 
+// The gradient from the kept log-sum-exps: a CTA takes a row's packets (or,
+// grid.y > 1, every grid.y-th run of them).
+constexpr int kBackwardThreads = 256;
 template <typename T>
-__global__ __launch_bounds__(kPolicyThreads) void policy_backward_kernel(
+__global__ __launch_bounds__(kBackwardThreads) void policy_backward_kernel(
     PolicyRows shape, const T *__restrict__ logits, const int64_t *__restrict__ targets,
     const uint8_t *__restrict__ valid, const float *__restrict__ lse, const float *__restrict__ slopes,
     const float *__restrict__ grad_loss, T *__restrict__ grad_logits) {
+    constexpr int kWidth = Pack<T>::kWidth, kPackets = 4;
     const float scale = *grad_loss;
+    const int64_t step = int64_t(gridDim.y) * kBackwardThreads * kPackets;
     for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
         const T *in = logits + shape.start(row);
         T *out = grad_logits + row * shape.vocab;
-        const bool live = valid == nullptr || valid[row] != 0;
-        const float slope = slopes[row] * scale, z = lse[row];
-        const int64_t target = targets[row];
-        for (int64_t v = threadIdx.x; v < shape.vocab; v += blockDim.x) {
-            const float g = live ? slope * ((v == target ? 1.0f : 0.0f) - expf(to_acc(in[v]) - z)) : 0.0f;
-            out[v] = from_acc<T>(g);
+        if (valid != nullptr && valid[row] == 0) {
+            if (blockIdx.y == 0) clear_row(out, shape.vocab);
+            continue;
+        }
+        const Packets<T> packets(in, shape.vocab);
+        const bool fits = packets.fits(out);
+        const float slope = slopes[row] * scale, from = lse[row];
+        const int64_t at = targets[row] + packets.skip;
+        for (int64_t first = int64_t(blockIdx.y) * kBackwardThreads * kPackets + threadIdx.x; first < packets.count; first += step) {
+            uint4 raw[kPackets];
+#pragma unroll
+            for (int j = 0; j < kPackets; ++j) {
+                const int64_t c = first + j * kBackwardThreads;
+                raw[j] = c < packets.count && packets.whole(c) ? load_cached(packets.base + c * kWidth) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < kPackets; ++j) {
+                const int64_t c = first + j * kBackwardThreads;
+                if (c >= packets.count) continue;
+                float v[kWidth];
+                if (packets.whole(c)) {
+                    unpack(raw[j], v, T());
+                } else {
+                    packets.load_partly(c, v);
+                }
+#pragma unroll
+                for (int i = 0; i < kWidth; ++i) v[i] = -slope * exp_from(v[i], from);
+                if (at / kWidth == c) {
+#pragma unroll
+                    for (int i = 0; i < kWidth; ++i) v[i] += at % kWidth == i ? slope : 0.0f;
+                }
+                packets.store(out, fits, c, v);
+            }
         }
     }
 }
 
-// grad *= *factor, unless the factor is one.
+// grad *= *factor, unless the factor is one. grad is 16-byte aligned.
 template <typename T>
-__global__ void policy_scale_kernel(T *__restrict__ grad, int64_t count, const float *__restrict__ factor) {
+__global__ __launch_bounds__(256) void policy_scale_kernel(T *__restrict__ grad, int64_t count,
+                                                           const float *__restrict__ factor) {
+    constexpr int kWidth = Pack<T>::kWidth;
     const float f = *factor;
     if (f == 1.0f) return;
-    for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < count; i += int64_t(gridDim.x) * blockDim.x) {
-        grad[i] = from_acc<T>(to_acc(grad[i]) * f);
+    const int64_t packets = count / kWidth, thread = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    for (int64_t i = thread; i < packets; i += int64_t(gridDim.x) * blockDim.x) {
+        float v[kWidth];
+        unpack(reinterpret_cast<const uint4 *>(grad)[i], v, T());
+#pragma unroll
+        for (int j = 0; j < kWidth; ++j) v[j] *= f;
+        reinterpret_cast<uint4 *>(grad)[i] = pack(v, T());
     }
-}
-
-unsigned policy_blocks(int64_t rows) {
-    return static_cast<unsigned>(rows < kPolicyBlocks ? (rows > 0 ? rows : 1) : kPolicyBlocks);
+    if (thread < count - packets * kWidth) {
+        T *tail = grad + packets * kWidth + thread;
+        *tail = from_acc<T>(to_acc(*tail) * f);
+    }
 }
 
 int check_policy(const PolicyRows &shape) {
@@ -194,20 +588,76 @@ int check_policy(const PolicyRows &shape) {
     return KOEMI_OK;
 }
 
+template <typename T, int kThreads>
+int launch_rows(const PolicyRows &shape, const PolicyTerms &terms, const T *logits, const PolicyOut &result, T *grad,
+                unsigned &blocks, cudaStream_t stream) {
+    // a row's packets, and one more where it starts inside a packet; as many
+    // buffers as fit beside the other CTAs of the SM (1024 threads in all)
+    const uint32_t bytes = static_cast<uint32_t>(ceil_div(shape.vocab * sizeof(T), 128) * 128 + 128);
+    const uint32_t room = 222 * 1024 / (1024 / kThreads) - 1024;
+    const int buffers = static_cast<int>(room / bytes > 3 ? 3 : room / bytes);
+    const int64_t places = int64_t(sm_count()) * (1024 / kThreads);
+    blocks = static_cast<unsigned>(shape.rows < places ? shape.rows : places);
+    auto kernel = policy_row_kernel<T, kThreads>;
+    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(buffers * bytes)));
+    kernel<<<blocks, kThreads, buffers * bytes, stream>>>(shape, terms, logits, result, grad, buffers, bytes,
+                                                          device_status_word());
+    KOEMI_LAUNCH_CHECK();
+    return KOEMI_OK;
+}
+
+template <typename T, int kPer>
+int launch_warps(const PolicyRows &shape, const PolicyTerms &terms, const T *logits, const PolicyOut &result, T *grad,
+                 unsigned &blocks, cudaStream_t stream) {
+    const int64_t wanted = ceil_div(shape.rows, 8);
+    blocks = static_cast<unsigned>(wanted < kPolicyBlocks ? wanted : kPolicyBlocks);
+    policy_warp_kernel<T, kPer><<<blocks, 256, 0, stream>>>(shape, terms, logits, result, grad);
+    KOEMI_LAUNCH_CHECK();
+    return KOEMI_OK;
+}
+
 template <typename T>
 int policy_forward(const PolicyRows &shape, const PolicyTerms &terms, const void *logits, float *loss, float *kl,
                    float *log_probs, float *lse, float *slopes, void *grad_logits, void *workspace,
                    cudaStream_t stream) {
     float *inverse = static_cast<float *>(workspace);
-    float2 *partials = reinterpret_cast<float2 *>(static_cast<unsigned char *>(workspace) + 256);
-    policy_count_kernel<<<1, 1024, 0, stream>>>(terms.valid, shape.rows, inverse);
-    KOEMI_LAUNCH_CHECK();
-    const unsigned blocks = policy_blocks(shape.rows);
-    policy_forward_kernel<T><<<blocks, kPolicyThreads, 0, stream>>>(shape, terms, static_cast<const T *>(logits), inverse,
-                                                                    log_probs, lse, slopes,
-                                                                    static_cast<T *>(grad_logits), partials);
-    KOEMI_LAUNCH_CHECK();
-    policy_finish_kernel<<<1, 32, 0, stream>>>(partials, blocks, inverse, loss, kl);
+    PolicyOut result{nullptr, log_probs, lse, slopes, reinterpret_cast<float2 *>(static_cast<unsigned char *>(workspace) + 256)};
+    const T *in = static_cast<const T *>(logits);
+    T *grad = static_cast<T *>(grad_logits);
+    unsigned blocks = 0;
+    if (terms.valid != nullptr && shape.rows > kCountedRows) {
+        policy_count_kernel<<<1, 1024, 0, stream>>>(terms.valid, shape.rows, inverse);
+        KOEMI_LAUNCH_CHECK();
+        result.inverse = inverse;
+    }
+    if (shape.rows > 0) {
+        // rows that can start inside a packet may touch one packet more
+        const bool inside = !aligned(logits, 16) || shape.outer_stride * sizeof(T) % 16 != 0 || shape.inner_stride * sizeof(T) % 16 != 0;
+        const int64_t entries = shape.vocab + (inside ? Pack<T>::kWidth - 1 : 0);
+        int rc;
+        if (shape.vocab <= 256) {
+            rc = launch_warps<T, 8>(shape, terms, in, result, grad, blocks, stream);
+        } else if (shape.vocab <= 512) {
+            rc = launch_warps<T, 16>(shape, terms, in, result, grad, blocks, stream);
+        } else if (shape.vocab <= kWarpRow) {
+            rc = launch_warps<T, 32>(shape, terms, in, result, grad, blocks, stream);
+        } else if (entries <= 256 * kPerThread) {
+            rc = launch_rows<T, 256>(shape, terms, in, result, grad, blocks, stream);
+        } else if (entries <= 512 * kPerThread) {
+            rc = launch_rows<T, 512>(shape, terms, in, result, grad, blocks, stream);
+        } else if (entries <= 1024 * kPerThread) {
+            rc = launch_rows<T, 1024>(shape, terms, in, result, grad, blocks, stream);
+        } else {
+            const int64_t places = 2 * int64_t(sm_count());
+            blocks = static_cast<unsigned>(shape.rows < places ? shape.rows : places);
+            policy_walk_kernel<T><<<blocks, kWalkThreads, 0, stream>>>(shape, terms, in, result, grad);
+            KOEMI_LAUNCH_CHECK();
+            rc = KOEMI_OK;
+        }
+        if (rc != KOEMI_OK) return rc;
+    }
+    policy_finish_kernel<<<1, kFinishThreads, 0, stream>>>(result.partials, static_cast<int>(blocks), result.inverse,
+                                                           terms.valid, shape.rows, loss, kl);
     KOEMI_LAUNCH_CHECK();
     return KOEMI_OK;
 }
@@ -216,7 +666,12 @@ template <typename T>
 int policy_backward(const PolicyRows &shape, const void *logits, const int64_t *targets, const uint8_t *valid,
                     const float *lse, const float *slopes, const float *grad_loss, void *grad_logits,
                     cudaStream_t stream) {
-    policy_backward_kernel<T><<<policy_blocks(shape.rows), kPolicyThreads, 0, stream>>>(
+    // few long rows: several CTAs a row
+    const int64_t runs = ceil_div(shape.vocab, kBackwardThreads * 4 * Pack<T>::kWidth), places = 8 * int64_t(sm_count());
+    const unsigned x = static_cast<unsigned>(shape.rows < places ? shape.rows : places);
+    int64_t y = ceil_div(places, x);
+    if (y > runs) y = runs;
+    policy_backward_kernel<T><<<dim3(x, static_cast<unsigned>(y)), kBackwardThreads, 0, stream>>>(
         shape, static_cast<const T *>(logits), targets, valid, lse, slopes, grad_loss, static_cast<T *>(grad_logits));
     KOEMI_LAUNCH_CHECK();
     return KOEMI_OK;
@@ -224,7 +679,7 @@ int policy_backward(const PolicyRows &shape, const void *logits, const int64_t *
 
 template <typename T>
 int policy_scale(void *grad, int64_t count, const float *factor, cudaStream_t stream) {
-    const int64_t blocks = ceil_div(count, 256);
+    const int64_t blocks = ceil_div(count, 256 * Pack<T>::kWidth);
     policy_scale_kernel<T><<<static_cast<unsigned>(blocks < 1184 ? blocks : 1184), 256, 0, stream>>>(
         static_cast<T *>(grad), count, factor);
     KOEMI_LAUNCH_CHECK();
