@@ -4,10 +4,10 @@
 //   out = g min(1, max_norm / (norm + 1e-6))
 //
 // The tensors travel in the kernel's parameters (up to kMaxTensors per
-// launch), cut into chunks of kChunkElements; a chunk's sum of squares is one
-// partial, and every CTA of the second kernel adds all partials in the same
-// fixed order, so equal inputs give equal bits. In place, a factor of one
-// writes nothing.
+// launch), cut into chunks of kChunkElements; a CTA adds its chunks' sums of
+// squares up into one partial, and every CTA of the second kernel adds all
+// partials in the same fixed order, so equal inputs give equal bits. In place,
+// a factor of one writes nothing.
 #include <cstring>
 
 #include "vec.cuh"
@@ -16,9 +16,9 @@ namespace koemi {
 namespace {
 
 constexpr int kMaxTensors = 1000;          // 24 bytes each: the parameters stay below 32 KB
-constexpr int64_t kChunkElements = 16384;  // elements of one partial sum
+constexpr int64_t kChunkElements = 16384;  // elements summed in fp32; beyond, sums are fp64
 constexpr int kClipThreads = 256;
-constexpr int kClipBlocks = 592;
+constexpr int kClipBlocks = 888;  // six CTAs per SM
 
 struct ClipTable {
     const void *in[kMaxTensors];
@@ -53,24 +53,89 @@ __device__ __forceinline__ Chunk chunk_of(const ClipTable &table, uint32_t chunk
     return c;
 }
 
+// A chunk is a few single elements up to the first 16-byte boundary, packets of
+// 16 bytes, and the rest; kUnroll packets per thread are in flight at once.
+constexpr int kUnroll = 8;
+
 template <typename T>
-__device__ float chunk_squares(const T *in, int elements) {
-    float sum = 0.0f;
-    for (int i = threadIdx.x; i < elements; i += kClipThreads) {
-        const float v = to_acc(in[i]);
-        sum = fmaf(v, v, sum);
-    }
+__device__ __forceinline__ int elements_to_boundary(const T *p, int elements) {
+    const int ahead = static_cast<int>((16 - reinterpret_cast<uintptr_t>(p) % 16) % 16 / sizeof(T));
+    return ahead < elements ? ahead : elements;
+}
+template <typename T>
+__device__ __forceinline__ float packet_squares(const uint4 &raw, float sum) {
+    float v[Pack<T>::kWidth];
+    unpack(raw, v, T());
+#pragma unroll
+    for (int i = 0; i < Pack<T>::kWidth; ++i) sum = fmaf(v[i], v[i], sum);
     return sum;
 }
 
 template <typename T>
+__device__ float chunk_squares(const T *in, int elements) {
+    constexpr int kWidth = Pack<T>::kWidth;
+    const int head = elements_to_boundary(in, elements), packets = (elements - head) / kWidth;
+    const uint4 *body = reinterpret_cast<const uint4 *>(in + head);
+    float sums[2] = {0.0f, 0.0f};
+    int i = threadIdx.x;
+    for (; i + (kUnroll - 1) * kClipThreads < packets; i += kUnroll * kClipThreads) {
+        uint4 raw[kUnroll];
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j) raw[j] = load_cached(body + i + j * kClipThreads);
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j) sums[j & 1] = packet_squares<T>(raw[j], sums[j & 1]);
+    }
+    for (; i < packets; i += kClipThreads) sums[0] = packet_squares<T>(load_cached(body + i), sums[0]);
+    // the single elements: the first `head`, and those behind the packets
+    const int tail = head + packets * kWidth;
+    for (int k = threadIdx.x; k < head + elements - tail; k += kClipThreads) {
+        const float v = to_acc(in[k < head ? k : tail + k - head]);
+        sums[1] = fmaf(v, v, sums[1]);
+    }
+    return sums[0] + sums[1];
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 scaled_packet(const uint4 &raw, float factor) {
+    float v[Pack<T>::kWidth];
+    unpack(raw, v, T());
+#pragma unroll
+    for (int i = 0; i < Pack<T>::kWidth; ++i) v[i] *= factor;
+    return pack(v, T());
+}
+
+// in and out may be the same tensor, or tensors that do not overlap.
+template <typename T>
 __device__ void chunk_scale(const T *in, T *out, int elements, float factor) {
-    for (int i = threadIdx.x; i < elements; i += kClipThreads) out[i] = from_acc<T>(to_acc(in[i]) * factor);
+    constexpr int kWidth = Pack<T>::kWidth;
+    if ((reinterpret_cast<uintptr_t>(in) - reinterpret_cast<uintptr_t>(out)) % 16 != 0) {
+        // no boundary fits both: single elements, neighbouring threads next to each other
+        for (int i = threadIdx.x; i < elements; i += kClipThreads) out[i] = from_acc<T>(to_acc(in[i]) * factor);
+        return;
+    }
+    const int head = elements_to_boundary(in, elements), packets = (elements - head) / kWidth;
+    const uint4 *body = reinterpret_cast<const uint4 *>(in + head);
+    uint4 *target = reinterpret_cast<uint4 *>(out + head);
+    int i = threadIdx.x;
+    for (; i + (kUnroll - 1) * kClipThreads < packets; i += kUnroll * kClipThreads) {
+        uint4 raw[kUnroll];
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j) raw[j] = __ldcs(body + i + j * kClipThreads);
+#pragma unroll
+        for (int j = 0; j < kUnroll; ++j) __stcs(target + i + j * kClipThreads, scaled_packet<T>(raw[j], factor));
+    }
+    for (; i < packets; i += kClipThreads) __stcs(target + i, scaled_packet<T>(__ldcs(body + i), factor));
+    const int tail = head + packets * kWidth;
+    for (int k = threadIdx.x; k < head + elements - tail; k += kClipThreads) {
+        const int at = k < head ? k : tail + k - head;
+        out[at] = from_acc<T>(to_acc(in[at]) * factor);
+    }
 }
 
 __global__ __launch_bounds__(kClipThreads) void clip_squares_kernel(const __grid_constant__ ClipTable table,
-                                                                    uint32_t chunks, float *__restrict__ partials) {
+                                                                    uint32_t chunks, double *__restrict__ partials) {
     __shared__ float sums[kClipThreads / 32];
+    double total = 0.0;  // thread 0's
     for (uint32_t index = blockIdx.x; index < chunks; index += gridDim.x) {
         const Chunk c = chunk_of(table, index);
         float sum;
@@ -87,14 +152,15 @@ __global__ __launch_bounds__(kClipThreads) void clip_squares_kernel(const __grid
         if (threadIdx.x == 0) {
             float all = 0.0f;
             for (int w = 0; w < kClipThreads / 32; ++w) all += sums[w];
-            partials[index] = all;
+            total += all;
         }
         __syncthreads();
     }
+    if (threadIdx.x == 0) partials[blockIdx.x] = total;
 }
 
 // The sum of all partials, the same bits in every CTA.
-__device__ double sum_partials(const float *partials, int64_t count) {
+__device__ double sum_partials(const double *partials, int64_t count) {
     __shared__ double sums[kClipThreads / 32];
     double sum = 0.0;
     for (int64_t i = threadIdx.x; i < count; i += kClipThreads) sum += partials[i];
@@ -108,15 +174,16 @@ __device__ double sum_partials(const float *partials, int64_t count) {
 }
 
 __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const __grid_constant__ ClipTable table,
-                                                                  uint32_t chunks, const float *__restrict__ partials,
+                                                                  uint32_t chunks, const double *__restrict__ partials,
                                                                   int64_t partial_count, float max_norm,
                                                                   float *__restrict__ norm_out) {
     const float norm = static_cast<float>(sqrt(sum_partials(partials, partial_count)));
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
     float factor = max_norm / (norm + 1e-6f);
     if (factor > 1.0f) factor = 1.0f;  // a NaN stays
-    for (uint32_t index = blockIdx.x; index < chunks; index += gridDim.x) {
-        const Chunk c = chunk_of(table, index);
+    // from the last chunk on: the tail of the first pass's reads is still in L2
+    for (int64_t index = int64_t(chunks) - 1 - blockIdx.x; index >= 0; index -= gridDim.x) {
+        const Chunk c = chunk_of(table, static_cast<uint32_t>(index));
         const void *in = table.in[c.tensor];
         void *out = table.out[c.tensor];
         if (out == nullptr || (factor == 1.0f && in == out)) continue;
@@ -164,7 +231,8 @@ extern "C" size_t koemi_core_clip_gradients_workspace(const int64_t *elements, i
     if (elements == nullptr || count < 0) return 0;
     int64_t chunks = 0;
     for (int64_t i = 0; i < count; ++i) chunks += elements[i] > 0 ? chunk_count(elements[i]) : 0;
-    return static_cast<size_t>(chunks) * sizeof(float);
+    const int64_t launches = ceil_div(count, kMaxTensors) + (chunks >> 30) + 1;
+    return static_cast<size_t>(launches) * kClipBlocks * sizeof(double);
 }
 
 extern "C" int koemi_core_clip_gradients(const uint64_t *gradients, const uint64_t *outputs, const int64_t *elements,
@@ -176,7 +244,6 @@ extern "C" int koemi_core_clip_gradients(const uint64_t *gradients, const uint64
     if (norm == nullptr || (count > 0 && (gradients == nullptr || elements == nullptr || dtypes == nullptr))) {
         return fail(KOEMI_ERR_INVALID, "norm, gradients, elements and dtypes must be non-NULL");
     }
-    int64_t chunks = 0;
     for (int64_t i = 0; i < count; ++i) {
         if (elements[i] < 0 || elements[i] > int64_t(1) << 44) return fail(KOEMI_ERR_INVALID, "tensor %lld has a bad size", static_cast<long long>(i));
         if (dtypes[i] != KOEMI_F32 && dtypes[i] != KOEMI_F16 && dtypes[i] != KOEMI_BF16) {
@@ -185,22 +252,22 @@ extern "C" int koemi_core_clip_gradients(const uint64_t *gradients, const uint64
         if (elements[i] > 0 && (gradients[i] == 0 || (outputs != nullptr && outputs[i] == 0))) {
             return fail(KOEMI_ERR_INVALID, "tensor %lld has no data", static_cast<long long>(i));
         }
-        chunks += chunk_count(elements[i]);
     }
-    if (workspace_bytes < chunks * sizeof(float) || (chunks > 0 && workspace == nullptr)) {
+    if (workspace == nullptr || workspace_bytes < koemi_core_clip_gradients_workspace(elements, count)) {
         return fail(KOEMI_ERR_WORKSPACE, "the clipping workspace is smaller than koemi_core_clip_gradients_workspace()");
     }
     cudaStream_t s = as_stream(stream);
-    float *partials = static_cast<float *>(workspace);
+    double *partials = static_cast<double *>(workspace);
     ClipTable table;
     int64_t done = 0;
     for (int64_t i = 0; i < count;) {
         i = fill_table(table, gradients, outputs, elements, dtypes, i, count);
         const uint32_t n = table.first_chunk[table.count];
         if (n == 0) continue;
-        clip_squares_kernel<<<n < kClipBlocks ? n : kClipBlocks, kClipThreads, 0, s>>>(table, n, partials + done);
+        const uint32_t blocks = n < kClipBlocks ? n : kClipBlocks;
+        clip_squares_kernel<<<blocks, kClipThreads, 0, s>>>(table, n, partials + done);
         KOEMI_LAUNCH_CHECK();
-        done += n;
+        done += blocks;
     }
     int64_t i = 0;
     do {
