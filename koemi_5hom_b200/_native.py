@@ -15,6 +15,7 @@ from pathlib import Path
 import torch
 
 LIBRARY_PATH = Path(__file__).resolve().parent / "lib" / "libkoemi_b200.so"
+BINDING_PATH = LIBRARY_PATH.with_name("libkoemi_b200_torch.so")
 ABI_VERSION = 1
 
 KOEMI_OK = 0
@@ -162,6 +163,7 @@ class KoemiNativeError(RuntimeError):
 _LOCK = threading.RLock()
 _LIBRARY: ctypes.CDLL | None = None
 _INITIALISED_DEVICES: set[int] = set()
+_BINDING: ctypes.CDLL | None = None
 
 
 def library() -> ctypes.CDLL:
@@ -196,6 +198,32 @@ def library() -> ctypes.CDLL:
             )
         _LIBRARY = handle
     return _LIBRARY
+
+
+def binding() -> ctypes.CDLL:
+    """Load (once) the torch binding, which registers the training ops, and open the kernel library in it."""
+    global _BINDING
+    if _BINDING is not None:
+        return _BINDING
+    handle = library()
+    with _LOCK:
+        if _BINDING is not None:
+            return _BINDING
+        if not BINDING_PATH.is_file():
+            raise KoemiNativeUnavailableError(
+                f"{BINDING_PATH} is missing; build it with `python -m koemi_5hom_b200.build`"
+            )
+        try:
+            ops = ctypes.CDLL(str(BINDING_PATH))
+        except OSError as error:
+            raise KoemiNativeUnavailableError(f"cannot load {BINDING_PATH}: {error}") from error
+        ops.koemi_torch_open.restype = ctypes.c_char_p
+        ops.koemi_torch_open.argtypes = [ctypes.c_char_p]
+        message = ops.koemi_torch_open(str(handle._name).encode())
+        if message is not None:
+            raise KoemiNativeUnavailableError(message.decode("utf-8", errors="replace"))
+        _BINDING = ops
+    return _BINDING
 
 
 def last_error() -> str:

@@ -6,6 +6,10 @@ Every ``csrc/*.cu`` translation unit is compiled by nvcc for
 linked into ``lib/libkoemi_b200.so`` with a static CUDA runtime, so the
 library depends on nothing but the driver. nvcc cross-compiles without a GPU.
 
+``csrc/binding/training_ops.cpp`` is compiled by g++ against the installed torch into
+``lib/libkoemi_b200_torch.so``: the dispatcher ops and autograd formulas of the
+training operators, which open the kernel library at run time.
+
 Run ``python -m koemi_5hom_b200.build`` (or call :func:`build`).
 """
 from __future__ import annotations
@@ -23,6 +27,8 @@ SOURCE_DIR = PACKAGE_DIR / "csrc"
 INCLUDE_DIR = PACKAGE_DIR.parent / "include"
 BUILD_DIR = PACKAGE_DIR.parent / "_build"
 LIBRARY_PATH = PACKAGE_DIR / "lib" / "libkoemi_b200.so"
+BINDING_SOURCE = SOURCE_DIR / "binding" / "training_ops.cpp"
+BINDING_PATH = PACKAGE_DIR / "lib" / "libkoemi_b200_torch.so"
 
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 NVCC_FLAGS = (
@@ -65,8 +71,38 @@ def _compile(nvcc: str, source: Path, verbose: bool) -> Path:
     return target
 
 
+def build_binding(verbose: bool = False) -> Path:
+    """Compile the torch binding (skipped when newer than its inputs and the torch it was built for)."""
+    import torch
+
+    compiler = os.environ.get("CXX") or shutil.which("g++")
+    if not compiler:
+        raise RuntimeError("g++ was not found; set CXX")
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(find_nvcc()).resolve().parent.parent
+    newest_input = max(p.stat().st_mtime for p in
+                       [BINDING_SOURCE, *INCLUDE_DIR.glob("*.h"), Path(__file__), root / "version.py"])
+    if BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= newest_input:
+        return BINDING_PATH
+    BINDING_PATH.parent.mkdir(parents=True, exist_ok=True)
+    temporary = BINDING_PATH.with_suffix(".so.tmp")
+    command = [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               "-I", str(INCLUDE_DIR), "-isystem", str(root / "include"),
+               "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+               "-isystem", str(cuda / "include"), str(BINDING_SOURCE), "-o", str(temporary),
+               "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl"]
+    if verbose:
+        print(" ".join(command), flush=True)
+    result = subprocess.run(command, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"compiling {BINDING_SOURCE.name} failed:\n{result.stdout}\n{result.stderr}")
+    os.replace(temporary, BINDING_PATH)
+    return BINDING_PATH
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compile every kernel translation unit and link the shared library."""
+    """Compile every kernel translation unit and link the shared library, and compile the torch binding."""
     nvcc = find_nvcc()
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
     LIBRARY_PATH.parent.mkdir(parents=True, exist_ok=True)
@@ -75,7 +111,9 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
         raise RuntimeError(f"no CUDA sources under {SOURCE_DIR}")
     workers = jobs or min(len(sources), os.cpu_count() or 4)
     with concurrent.futures.ThreadPoolExecutor(max_workers=workers) as pool:
+        binding = pool.submit(build_binding, verbose)
         objects = list(pool.map(lambda s: _compile(nvcc, s, verbose), sources))
+        binding.result()
     newest_object = max(o.stat().st_mtime for o in objects)
     if LIBRARY_PATH.exists() and LIBRARY_PATH.stat().st_mtime >= newest_object:
         return LIBRARY_PATH

@@ -1,0 +1,528 @@
+// PyTorch operators of a training step over the C ABI of libkoemi_b200.so:
+// dispatcher schemas, CUDA implementations and autograd formulas.
+//
+// They are C++ because their backward passes run on autograd's device thread,
+// where a Python function waits for the interpreter: a forward and backward of
+// an 8 x 257 policy loss took 142 us of host time with Python autograd functions
+// and ctypes calls (kernels: 10 us), of which 50 us are autograd's own.
+// Nothing here computes: every op checks what the kernels rely on, allocates
+// from the caching allocator and calls one entry point on the current stream.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <dlfcn.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <mutex>
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "koemi_b200.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptionalTensor = std::optional<Tensor>;
+
+// ------------------------------------------------------------ the library
+
+struct Library {
+    decltype(&koemi_last_error) last_error;
+    decltype(&koemi_device_init) device_init;
+    decltype(&koemi_dense_gated_recurrence_forward) gated_forward;
+    decltype(&koemi_dense_gated_recurrence_backward) gated_backward;
+    decltype(&koemi_moe_route_learned_workspace) route_workspace;
+    decltype(&koemi_moe_route_learned_forward) route_forward;
+    decltype(&koemi_moe_route_learned_backward) route_backward;
+    decltype(&koemi_think_policy_loss_workspace) policy_workspace;
+    decltype(&koemi_think_policy_loss_forward) policy_forward;
+    decltype(&koemi_think_policy_loss_backward) policy_backward;
+    decltype(&koemi_think_policy_loss_scale) policy_scale;
+    decltype(&koemi_core_clip_gradients_workspace) clip_workspace;
+    decltype(&koemi_core_clip_gradients) clip;
+};
+
+Library library;
+bool opened = false;
+
+const Library &lib() {
+    TORCH_CHECK(opened, "libkoemi_b200 is not open");
+    return library;
+}
+
+void check(const char *function, int status) {
+    if (status == KOEMI_OK) return;
+    char message[1024];
+    lib().last_error(message, sizeof(message));
+    TORCH_CHECK(false, function, " failed with status ", status, ": ", message);
+}
+
+// Makes a tensor's device current, its per-device state initialised, and
+// names its current stream.
+struct Launch {
+    c10::cuda::CUDAGuard guard;
+    void *stream;
+    explicit Launch(const Tensor &t) : guard(t.device()) {
+        static std::once_flag initialised[64];
+        const int device = t.device().index();
+        TORCH_CHECK(device >= 0 && device < 64, "device index ", device, " is out of range");
+        std::call_once(initialised[device], [device] { check("koemi_device_init", lib().device_init(device)); });
+        stream = c10::cuda::getCurrentCUDAStream(device).stream();
+    }
+};
+
+int code_of(const Tensor &t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return KOEMI_F32;
+        case at::kHalf: return KOEMI_F16;
+        case at::kBFloat16: return KOEMI_BF16;
+        default: TORCH_CHECK_VALUE(false, "unsupported dtype ", t.scalar_type());
+    }
+}
+
+template <typename T>
+T *address(const Tensor &t) {
+    return static_cast<T *>(t.data_ptr());
+}
+template <typename T>
+T *address(const OptionalTensor &t) {
+    return t.has_value() && t->defined() ? static_cast<T *>(t->data_ptr()) : nullptr;
+}
+Tensor f32(const Tensor &like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
+OptionalTensor given(const Tensor &t) { return t.defined() ? OptionalTensor(t) : OptionalTensor(); }
+OptionalTensor dense(const Tensor &t) { return t.defined() ? OptionalTensor(t.contiguous()) : OptionalTensor(); }
+
+bool differentiates(const Tensor &t) { return t.defined() && t.requires_grad(); }
+bool differentiates(const OptionalTensor &t) { return t.has_value() && differentiates(*t); }
+
+void first_order_only() {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the training operators are differentiable to first order only (create_graph=True)");
+}
+
+// ----------------------------------------------------- the gated recurrence
+
+constexpr int64_t kSegment = 128;  // positions between two carries
+
+std::tuple<Tensor, Tensor, Tensor> gated_forward(const Tensor &projections, const OptionalTensor &initial,
+                                                 const OptionalTensor &valid, const OptionalTensor &restart, double low,
+                                                 double high, bool keep) {
+    const Launch launch(projections);
+    const int64_t batch = projections.size(0), length = projections.size(1), features = projections.size(2) / 2;
+    Tensor states = at::empty({batch, length, features}, projections.options());
+    Tensor final_state = f32(projections, {batch, features});
+    Tensor carries;
+    if (keep) carries = f32(projections, {batch, (length + kSegment - 1) / kSegment, features});
+    check("koemi_dense_gated_recurrence_forward",
+          lib().gated_forward(address<void>(projections), address<float>(initial), address<uint8_t>(valid), address<uint8_t>(restart),
+                              address<void>(states), address<float>(final_state), keep ? address<float>(carries) : nullptr, batch,
+                              length, features, static_cast<float>(low), static_cast<float>(high), code_of(projections),
+                              launch.stream));
+    return {states, final_state, carries};
+}
+
+std::tuple<Tensor, Tensor> gated_recurrence_cuda(const Tensor &projections, const OptionalTensor &initial,
+                                                 const OptionalTensor &valid, const OptionalTensor &restart, double low,
+                                                 double high) {
+    auto [states, final_state, carries] = gated_forward(projections, initial, valid, restart, low, high, false);
+    return {states, final_state};
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_recurrence_keep_cuda(const Tensor &projections, const OptionalTensor &initial,
+                                                              const OptionalTensor &valid, const OptionalTensor &restart,
+                                                              double low, double high) {
+    return gated_forward(projections, initial, valid, restart, low, high, true);
+}
+
+std::tuple<Tensor, Tensor> gated_recurrence_backward_cuda(const Tensor &projections, const OptionalTensor &valid,
+                                                          const OptionalTensor &restart, const Tensor &carries,
+                                                          const OptionalTensor &grad_states,
+                                                          const OptionalTensor &grad_final, double low, double high) {
+    const Launch launch(projections);
+    const int64_t batch = projections.size(0), length = projections.size(1), features = projections.size(2) / 2;
+    Tensor grad_projections = at::empty_like(projections), grad_initial = f32(projections, {batch, features});
+    check("koemi_dense_gated_recurrence_backward",
+          lib().gated_backward(address<void>(projections), address<uint8_t>(valid), address<uint8_t>(restart), address<float>(carries),
+                               address<void>(grad_states), address<float>(grad_final), address<void>(grad_projections),
+                               address<float>(grad_initial), batch, length, features, static_cast<float>(low),
+                               static_cast<float>(high), code_of(projections), launch.stream));
+    return {grad_projections, grad_initial};
+}
+
+#define KOEMI_OP(name, signature) \
+    static auto name = c10::Dispatcher::singleton().findSchemaOrThrow("koemi_b200::" #name, "").typed<signature>()
+
+struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
+    static variable_list forward(AutogradContext *context, const Tensor &projections, const OptionalTensor &initial,
+                                 const OptionalTensor &valid, const OptionalTensor &restart, double low, double high) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        KOEMI_OP(gated_recurrence_keep, decltype(gated_recurrence_keep_cuda));
+        auto [states, final_state, carries] = gated_recurrence_keep.call(projections, initial, valid, restart, low, high);
+        context->save_for_backward({projections, valid.value_or(Tensor()), restart.value_or(Tensor()), carries});
+        context->saved_data["low"] = low;
+        context->saved_data["high"] = high;
+        context->saved_data["initial"] = differentiates(initial);
+        context->set_materialize_grads(false);
+        return {states, final_state};
+    }
+    static variable_list backward(AutogradContext *context, variable_list grads) {
+        first_order_only();
+        variable_list result(6);
+        if (!grads[0].defined() && !grads[1].defined()) return result;
+        const auto saved = context->get_saved_variables();
+        KOEMI_OP(gated_recurrence_backward, decltype(gated_recurrence_backward_cuda));
+        auto [grad_projections, grad_initial] = gated_recurrence_backward.call(
+            saved[0], given(saved[1]), given(saved[2]), saved[3], dense(grads[0]), dense(grads[1]),
+            context->saved_data["low"].toDouble(), context->saved_data["high"].toDouble());
+        result[0] = grad_projections;
+        if (context->saved_data["initial"].toBool()) result[1] = grad_initial;
+        return result;
+    }
+};
+
+std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor &projections, const OptionalTensor &initial,
+                                                     const OptionalTensor &valid, const OptionalTensor &restart,
+                                                     double low, double high) {
+    if (at::GradMode::is_enabled() && (differentiates(projections) || differentiates(initial))) {
+        auto out = GatedRecurrence::apply(projections, initial, valid, restart, low, high);
+        return {out[0], out[1]};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    KOEMI_OP(gated_recurrence, decltype(gated_recurrence_cuda));
+    return gated_recurrence.call(projections, initial, valid, restart, low, high);
+}
+
+// ---------------------------------------------------------- the learned route
+
+using Route = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
+
+// ids, weights, counts, balance loss, and the loss's slope per probability
+Route route_learned_keep_cuda(const Tensor &logits, const OptionalTensor &valid, int64_t top_k, bool renormalize) {
+    const Launch launch(logits);
+    const int64_t tokens = logits.size(0), experts = logits.size(1);
+    const auto ints = logits.options().dtype(at::kLong);
+    Tensor ids = at::empty({tokens, top_k}, ints), weights = f32(logits, {tokens, top_k});
+    Tensor counts = at::empty({experts}, ints), balance = f32(logits, {}), slope = f32(logits, {experts});
+    const int64_t size = static_cast<int64_t>(lib().route_workspace(tokens, experts));
+    Tensor workspace = at::empty({size}, logits.options().dtype(at::kByte));
+    check("koemi_moe_route_learned_forward",
+          lib().route_forward(address<void>(logits), address<uint8_t>(valid), address<int64_t>(ids), address<float>(weights),
+                              address<int64_t>(counts), address<float>(balance), address<float>(slope), tokens, experts, top_k,
+                              renormalize, code_of(logits), address<void>(workspace), size, launch.stream));
+    return {ids, weights, counts, balance, slope};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> route_learned_cuda(const Tensor &logits, const OptionalTensor &valid,
+                                                              int64_t top_k, bool renormalize) {
+    auto [ids, weights, counts, balance, slope] = route_learned_keep_cuda(logits, valid, top_k, renormalize);
+    return {ids, weights, counts, balance};
+}
+
+Tensor route_learned_backward_cuda(const Tensor &logits, const Tensor &ids, const Tensor &weights, const Tensor &slope,
+                                   const OptionalTensor &grad_weights, const OptionalTensor &grad_balance,
+                                   bool renormalize) {
+    const Launch launch(logits);
+    Tensor grad = at::empty_like(logits);
+    check("koemi_moe_route_learned_backward",
+          lib().route_backward(address<void>(logits), address<int64_t>(ids), address<float>(weights), address<float>(grad_weights),
+                               address<float>(grad_balance), address<float>(slope), address<void>(grad), logits.size(0),
+                               logits.size(1), ids.size(1), renormalize, code_of(logits), launch.stream));
+    return grad;
+}
+
+struct RouteLearned : torch::autograd::Function<RouteLearned> {
+    static variable_list forward(AutogradContext *context, const Tensor &logits, const OptionalTensor &valid,
+                                 int64_t top_k, bool renormalize) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        KOEMI_OP(route_learned_keep, decltype(route_learned_keep_cuda));
+        auto [ids, weights, counts, balance, slope] = route_learned_keep.call(logits, valid, top_k, renormalize);
+        context->save_for_backward({logits, ids, weights, slope});
+        context->saved_data["renormalize"] = renormalize;
+        context->mark_non_differentiable({ids, counts});
+        context->set_materialize_grads(false);
+        return {ids, weights, counts, balance};
+    }
+    static variable_list backward(AutogradContext *context, variable_list grads) {
+        first_order_only();
+        variable_list result(4);
+        if (!grads[1].defined() && !grads[3].defined()) return result;
+        const auto saved = context->get_saved_variables();
+        KOEMI_OP(route_learned_backward, decltype(route_learned_backward_cuda));
+        result[0] = route_learned_backward.call(saved[0], saved[1], saved[2], saved[3], dense(grads[1]), dense(grads[3]),
+                                                context->saved_data["renormalize"].toBool());
+        return result;
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> route_learned_autograd(const Tensor &logits, const OptionalTensor &valid,
+                                                                  int64_t top_k, bool renormalize) {
+    if (at::GradMode::is_enabled() && differentiates(logits)) {
+        auto out = RouteLearned::apply(logits, valid, top_k, renormalize);
+        return {out[0], out[1], out[2], out[3]};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    KOEMI_OP(route_learned, decltype(route_learned_cuda));
+    return route_learned.call(logits, valid, top_k, renormalize);
+}
+
+// ------------------------------------------------------------ the policy loss
+
+struct Rows {
+    int64_t rows, vocab, inner, outer_stride, inner_stride;
+    // [N, V] or [B, T, V] logits whose last dimension is contiguous
+    explicit Rows(const Tensor &logits) : vocab(logits.size(-1)) {
+        const bool batched = logits.dim() == 3;
+        rows = batched ? logits.size(0) * logits.size(1) : logits.size(0);
+        inner = std::max<int64_t>(batched ? logits.size(1) : rows, 1);
+        outer_stride = batched ? logits.stride(0) : 0;
+        inner_stride = batched ? logits.stride(1) : logits.stride(0);
+    }
+};
+
+// loss, kl, log-probs, (log-sum-exps | slopes), gradient (undefined unless wanted)
+Route policy_forward(const Tensor &logits, const Tensor &targets, const Tensor &old, const Tensor &advantages,
+                     const OptionalTensor &reference, const OptionalTensor &valid, double clip_low, double clip_high,
+                     double kl_weight, bool with_gradient) {
+    const Launch launch(logits);
+    const Rows shape(logits);
+    Tensor loss = f32(logits, {}), kl = f32(logits, {}), log_probs = f32(logits, targets.sizes());
+    Tensor kept = f32(logits, {2, shape.rows}), gradient;
+    if (with_gradient) gradient = at::empty(logits.sizes(), logits.options());
+    const int64_t size = static_cast<int64_t>(lib().policy_workspace());
+    Tensor workspace = at::empty({size}, logits.options().dtype(at::kByte));
+    check("koemi_think_policy_loss_forward",
+          lib().policy_forward(address<void>(logits), shape.rows, shape.vocab, shape.inner, shape.outer_stride,
+                               shape.inner_stride, address<int64_t>(targets), address<float>(old), address<float>(advantages),
+                               address<float>(reference), address<uint8_t>(valid), static_cast<float>(clip_low),
+                               static_cast<float>(clip_high), static_cast<float>(kl_weight), address<float>(loss),
+                               address<float>(kl), address<float>(log_probs), address<float>(kept), address<float>(kept) + shape.rows,
+                               with_gradient ? address<void>(gradient) : nullptr, code_of(logits), address<void>(workspace), size,
+                               launch.stream));
+    return {loss, kl, log_probs, kept, gradient};
+}
+
+std::tuple<Tensor, Tensor, Tensor> policy_loss_cuda(const Tensor &logits, const Tensor &targets, const Tensor &old,
+                                                    const Tensor &advantages, const OptionalTensor &reference,
+                                                    const OptionalTensor &valid, double clip_low, double clip_high,
+                                                    double kl_weight) {
+    auto [loss, kl, log_probs, kept, gradient] = policy_forward(logits, targets, old, advantages, reference, valid, clip_low,
+                                                                clip_high, kl_weight, false);
+    return {loss, kl, log_probs};
+}
+
+Route policy_loss_keep_cuda(const Tensor &logits, const Tensor &targets, const Tensor &old, const Tensor &advantages,
+                            const OptionalTensor &reference, const OptionalTensor &valid, double clip_low,
+                            double clip_high, double kl_weight) {
+    Route out = policy_forward(logits, targets, old, advantages, reference, valid, clip_low, clip_high, kl_weight,
+                               logits.scalar_type() != at::kHalf);
+    if (!std::get<4>(out).defined()) std::get<4>(out) = at::empty({0}, logits.options());
+    return out;
+}
+
+Tensor policy_loss_backward_cuda(const Tensor &logits, const Tensor &targets, const OptionalTensor &valid,
+                                 const Tensor &kept, const Tensor &grad_loss) {
+    const Launch launch(logits);
+    const Rows shape(logits);
+    Tensor grad = at::empty(logits.sizes(), logits.options());
+    check("koemi_think_policy_loss_backward",
+          lib().policy_backward(address<void>(logits), shape.rows, shape.vocab, shape.inner, shape.outer_stride,
+                                shape.inner_stride, address<int64_t>(targets), address<uint8_t>(valid), address<float>(kept),
+                                address<float>(kept) + shape.rows, address<float>(grad_loss), address<void>(grad), code_of(logits),
+                                launch.stream));
+    return grad;
+}
+
+void policy_loss_scale_cuda(const Tensor &gradient, const Tensor &factor) {
+    const Launch launch(gradient);
+    check("koemi_think_policy_loss_scale", lib().policy_scale(address<void>(gradient), gradient.numel(), address<float>(factor),
+                                                              code_of(gradient), launch.stream));
+}
+
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+    static variable_list forward(AutogradContext *context, const Tensor &logits, const Tensor &targets, const Tensor &old,
+                                 const Tensor &advantages, const OptionalTensor &reference, const OptionalTensor &valid,
+                                 double clip_low, double clip_high, double kl_weight) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        KOEMI_OP(policy_loss_keep, decltype(policy_loss_keep_cuda));
+        auto [loss, kl, log_probs, kept, gradient] = policy_loss_keep.call(logits, targets, old, advantages, reference, valid,
+                                                                           clip_low, clip_high, kl_weight);
+        context->save_for_backward({logits, targets, valid.value_or(Tensor()), kept});
+        if (logits.scalar_type() != at::kHalf) context->saved_data["gradient"] = gradient;
+        context->mark_non_differentiable({kl, log_probs});
+        context->set_materialize_grads(false);
+        return {loss, kl, log_probs};
+    }
+    static variable_list backward(AutogradContext *context, variable_list grads) {
+        first_order_only();
+        variable_list result(9);
+        if (!grads[0].defined()) return result;
+        const auto saved = context->get_saved_variables();
+        const Tensor factor = grads[0].contiguous();
+        // The gradient of the forward's pass is handed out once; f16, and
+        // another backward through a retained graph, form it from the logits.
+        auto kept = context->saved_data.find("gradient");
+        if (kept != context->saved_data.end()) {
+            result[0] = kept->second.toTensor();
+            context->saved_data.erase(kept);
+            KOEMI_OP(policy_loss_scale, decltype(policy_loss_scale_cuda));
+            policy_loss_scale.call(result[0], factor);
+        } else {
+            KOEMI_OP(policy_loss_backward, decltype(policy_loss_backward_cuda));
+            result[0] = policy_loss_backward.call(saved[0], saved[1], given(saved[2]), saved[3], factor);
+        }
+        return result;
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor> policy_loss_autograd(const Tensor &logits, const Tensor &targets, const Tensor &old,
+                                                        const Tensor &advantages, const OptionalTensor &reference,
+                                                        const OptionalTensor &valid, double clip_low, double clip_high,
+                                                        double kl_weight) {
+    if (at::GradMode::is_enabled() && differentiates(logits)) {
+        auto out = PolicyLoss::apply(logits, targets, old, advantages, reference, valid, clip_low, clip_high, kl_weight);
+        return {out[0], out[1], out[2]};
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    KOEMI_OP(policy_loss, decltype(policy_loss_cuda));
+    return policy_loss.call(logits, targets, old, advantages, reference, valid, clip_low, clip_high, kl_weight);
+}
+
+// ---------------------------------------------------- the clipping of gradients
+
+struct Table {
+    std::vector<uint64_t> addresses;
+    std::vector<int64_t> elements;
+    std::vector<int32_t> codes;
+    explicit Table(at::TensorList tensors, const char *name) {
+        TORCH_CHECK_VALUE(!tensors.empty(), name, " must not be empty");
+        addresses.reserve(tensors.size());
+        elements.reserve(tensors.size());
+        codes.reserve(tensors.size());
+        const auto device = tensors[0].device();
+        for (const Tensor &t : tensors) {
+            TORCH_CHECK_VALUE(t.is_contiguous() && t.layout() == at::kStrided, name, " must be contiguous");
+            TORCH_CHECK_VALUE(t.is_cuda() && t.device() == device, name, " must be on one CUDA device, got ", device, " and ", t.device());
+            const auto type = t.scalar_type();
+            TORCH_CHECK_VALUE(type == at::kFloat || type == at::kHalf || type == at::kBFloat16, name,
+                              " must use float32, float16 or bfloat16; found ", type);
+            addresses.push_back(reinterpret_cast<uint64_t>(t.data_ptr()));
+            elements.push_back(t.numel());
+            codes.push_back(code_of(t));
+        }
+    }
+};
+
+Tensor clip(const Tensor &like, const Table &gradients, const uint64_t *outputs, double max_norm) {
+    const Launch launch(like);
+    const int64_t count = static_cast<int64_t>(gradients.elements.size());
+    Tensor norm = f32(like, {});
+    const int64_t size = static_cast<int64_t>(lib().clip_workspace(gradients.elements.data(), count));
+    Tensor workspace = at::empty({size}, like.options().dtype(at::kByte));
+    check("koemi_core_clip_gradients",
+          lib().clip(gradients.addresses.data(), outputs, gradients.elements.data(), gradients.codes.data(), count,
+                     static_cast<float>(max_norm), address<float>(norm), address<void>(workspace), size, launch.stream));
+    return norm;
+}
+
+void written(at::TensorList tensors) {
+    for (const Tensor &t : tensors) {
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+}
+
+Tensor clip_gradients_inplace(at::TensorList gradients, double max_norm) {
+    const Table table(gradients, "gradients");
+    Tensor norm = clip(gradients[0], table, table.addresses.data(), max_norm);
+    written(gradients);
+    return norm;
+}
+
+Tensor clip_gradients_out(at::TensorList gradients, at::TensorList out, double max_norm) {
+    const Table table(gradients, "gradients"), target(out, "out");
+    TORCH_CHECK_VALUE(table.elements == target.elements && table.codes == target.codes && out[0].device() == gradients[0].device(),
+                      "out must match gradients in sizes, dtypes and device");
+    Tensor norm = clip(gradients[0], table, target.addresses.data(), max_norm);
+    written(out);
+    return norm;
+}
+
+Tensor gradient_norm(at::TensorList gradients) {
+    return clip(gradients[0], Table(gradients, "gradients"), nullptr, 0.0);
+}
+
+}  // namespace
+
+// Takes the entry points from the library at `path`; a message, or NULL.
+extern "C" __attribute__((visibility("default"))) const char *koemi_torch_open(const char *path) {
+    static std::string message;
+    void *handle = dlopen(path, RTLD_NOW | RTLD_LOCAL);
+    if (handle == nullptr) {
+        message = dlerror();
+        return message.c_str();
+    }
+    auto take = [&](auto &function, const char *name) {
+        function = reinterpret_cast<std::decay_t<decltype(function)>>(dlsym(handle, name));
+        if (function == nullptr && message.empty()) message = std::string(path) + " does not export " + name;
+    };
+    message.clear();
+    take(library.last_error, "koemi_last_error");
+    take(library.device_init, "koemi_device_init");
+    take(library.gated_forward, "koemi_dense_gated_recurrence_forward");
+    take(library.gated_backward, "koemi_dense_gated_recurrence_backward");
+    take(library.route_workspace, "koemi_moe_route_learned_workspace");
+    take(library.route_forward, "koemi_moe_route_learned_forward");
+    take(library.route_backward, "koemi_moe_route_learned_backward");
+    take(library.policy_workspace, "koemi_think_policy_loss_workspace");
+    take(library.policy_forward, "koemi_think_policy_loss_forward");
+    take(library.policy_backward, "koemi_think_policy_loss_backward");
+    take(library.policy_scale, "koemi_think_policy_loss_scale");
+    take(library.clip_workspace, "koemi_core_clip_gradients_workspace");
+    take(library.clip, "koemi_core_clip_gradients");
+    opened = message.empty();
+    return opened ? nullptr : message.c_str();
+}
+
+TORCH_LIBRARY_FRAGMENT(koemi_b200, m) {
+    m.def("gated_recurrence(Tensor projections, Tensor? initial, Tensor? valid, Tensor? restart, float low, float high) -> (Tensor, Tensor)");
+    m.def("gated_recurrence_keep(Tensor projections, Tensor? initial, Tensor? valid, Tensor? restart, float low, float high) -> (Tensor, Tensor, Tensor)");
+    m.def("gated_recurrence_backward(Tensor projections, Tensor? valid, Tensor? restart, Tensor carries, Tensor? grad_states, Tensor? grad_final, float low, float high) -> (Tensor, Tensor)");
+    m.def("route_learned(Tensor logits, Tensor? valid, int top_k, bool renormalize) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("route_learned_keep(Tensor logits, Tensor? valid, int top_k, bool renormalize) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("route_learned_backward(Tensor logits, Tensor ids, Tensor weights, Tensor slope, Tensor? grad_weights, Tensor? grad_balance, bool renormalize) -> Tensor");
+    m.def("policy_loss(Tensor logits, Tensor targets, Tensor old, Tensor advantages, Tensor? reference, Tensor? valid, float clip_low, float clip_high, float kl_weight) -> (Tensor, Tensor, Tensor)");
+    m.def("policy_loss_keep(Tensor logits, Tensor targets, Tensor old, Tensor advantages, Tensor? reference, Tensor? valid, float clip_low, float clip_high, float kl_weight) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def("policy_loss_backward(Tensor logits, Tensor targets, Tensor? valid, Tensor kept, Tensor grad_loss) -> Tensor");
+    m.def("policy_loss_scale(Tensor(a!) gradient, Tensor factor) -> ()");
+    m.def("clip_gradients_(Tensor(a!)[] gradients, float max_norm) -> Tensor");
+    m.def("clip_gradients_out(Tensor[] gradients, Tensor(a!)[] out, float max_norm) -> Tensor");
+    m.def("gradient_norm(Tensor[] gradients) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(koemi_b200, CUDA, m) {
+    m.impl("gated_recurrence", gated_recurrence_cuda);
+    m.impl("gated_recurrence_keep", gated_recurrence_keep_cuda);
+    m.impl("gated_recurrence_backward", gated_recurrence_backward_cuda);
+    m.impl("route_learned", route_learned_cuda);
+    m.impl("route_learned_keep", route_learned_keep_cuda);
+    m.impl("route_learned_backward", route_learned_backward_cuda);
+    m.impl("policy_loss", policy_loss_cuda);
+    m.impl("policy_loss_keep", policy_loss_keep_cuda);
+    m.impl("policy_loss_backward", policy_loss_backward_cuda);
+    m.impl("policy_loss_scale", policy_loss_scale_cuda);
+}
+
+TORCH_LIBRARY_IMPL(koemi_b200, Autograd, m) {
+    m.impl("gated_recurrence", gated_recurrence_autograd);
+    m.impl("route_learned", route_learned_autograd);
+    m.impl("policy_loss", policy_loss_autograd);
+}
+
+// Gradients are data: no formula, whichever of them requires one.
+TORCH_LIBRARY_IMPL(koemi_b200, CompositeExplicitAutograd, m) {
+    m.impl("clip_gradients_", clip_gradients_inplace);
+    m.impl("clip_gradients_out", clip_gradients_out);
+    m.impl("gradient_norm", gradient_norm);
+}

@@ -6,7 +6,6 @@ and nothing synchronises.
 """
 from __future__ import annotations
 
-from array import array
 from typing import Iterable, Sequence
 
 import torch
@@ -17,7 +16,7 @@ from koemi_5hom_b200.cuda_kernels.loader import CudaExtensionValidationError, lo
 
 __all__ = ["clip_gradients", "gradient_norm"]
 
-_CODES = {dtype: _training.DTYPE_CODES[dtype] for dtype in (torch.float32, torch.float16, torch.bfloat16)}
+_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def clip_gradients(gradients: Iterable[Tensor], max_norm: float, *, out: Sequence[Tensor] | None = None) -> Tensor:
@@ -33,42 +32,46 @@ def clip_gradients(gradients: Iterable[Tensor], max_norm: float, *, out: Sequenc
     gradients = list(gradients)
     if isinstance(max_norm, bool) or not isinstance(max_norm, (int, float)) or not max_norm >= 0.0:
         raise CudaExtensionValidationError("max_norm must be a non-negative number")
-    elements, codes = _table(gradients, "gradients")
     if out is None:
-        out = gradients
-    else:
-        out = list(out)
-        if _table(out, "out") != (elements, codes) or (out and out[0].device != gradients[0].device):
-            raise CudaExtensionValidationError("out must match gradients in sizes, dtypes and device")
-    return _run(gradients, out, elements, codes, float(max_norm))
+        return _call("clip_gradients_", (gradients,), float(max_norm))
+    return _call("clip_gradients_out", (gradients, list(out)), float(max_norm))
 
 
 def gradient_norm(gradients: Iterable[Tensor]) -> Tensor:
     """The 2-norm over all tensors, an fp32 scalar on their device (see :func:`clip_gradients`)."""
-    gradients = list(gradients)
-    return _run(gradients, None, *_table(gradients, "gradients"), 0.0)
+    return _call("gradient_norm", (list(gradients),))
 
 
-def _run(gradients, out, elements, codes, max_norm: float) -> Tensor:
-    if not gradients:
-        raise CudaExtensionValidationError("gradients must not be empty")
-    load_cuda_extension(device=gradients[0].device)
-    with torch.no_grad():
-        return _training.clip_gradients(gradients, out, elements, codes, max_norm)
-
-
-def _table(tensors: list[Tensor], name: str) -> tuple[array, array]:
-    """Element counts and dtype codes; the checks run as whole-list passes,
-    which cost a third of a loop's statements per tensor."""
-    if not all(isinstance(t, Tensor) for t in tensors):
-        raise TypeError(f"{name} must be torch.Tensors")
+def _call(name: str, lists: tuple[list, ...], *options) -> Tensor:
+    """Run the op, which checks the tensors as it collects their addresses (a
+    list of hundreds costs microseconds there); what it refuses is explained here."""
+    first = lists[0][0] if lists[0] else None
+    if not isinstance(first, Tensor) or not first.is_cuda:
+        _explain(lists)
+    if not _training._loaded:
+        load_cuda_extension(device=first.device)
+    _training.load(first.device)
     try:
-        codes = array("i", map(_CODES.__getitem__, map(_training.attribute_dtype, tensors)))
-    except KeyError as error:
-        raise CudaExtensionValidationError(f"{name} must use float32, float16 or bfloat16; found {error.args[0]}") from None
-    if not all(map(Tensor.is_contiguous, tensors)):
-        raise CudaExtensionValidationError(f"{name} must be contiguous")
-    devices = set(map(_training.attribute_device, tensors))
-    if len(devices) > 1 or any(device.type != "cuda" for device in devices):
-        raise CudaExtensionValidationError(f"{name} must be on one CUDA device, got {', '.join(sorted(map(str, devices)))}")
-    return array("q", map(Tensor.numel, tensors)), codes
+        return getattr(torch.ops.koemi_b200, name).default(*lists, *options)
+    except (ValueError, TypeError, RuntimeError):
+        _explain(lists)
+        raise
+
+
+def _explain(lists: tuple[list, ...]) -> None:
+    """Raise the typed error for the first rule that the tensors break."""
+    for name, tensors in zip(("gradients", "out"), lists):
+        if not all(isinstance(t, Tensor) for t in tensors):
+            raise TypeError(f"{name} must be torch.Tensors")
+        if not tensors:
+            raise CudaExtensionValidationError(f"{name} must not be empty")
+        for t in tensors:
+            if t.dtype not in _DTYPES:
+                raise CudaExtensionValidationError(f"{name} must use float32, float16 or bfloat16; found {t.dtype}")
+            if not t.is_contiguous():
+                raise CudaExtensionValidationError(f"{name} must be contiguous")
+        devices = {t.device for t in tensors}
+        if len(devices) > 1 or next(iter(devices)).type != "cuda":
+            raise CudaExtensionValidationError(f"{name} must be on one CUDA device, got {', '.join(sorted(map(str, devices)))}")
+    if len(lists) == 2 and ([(t.numel(), t.dtype, t.device) for t in lists[0]] != [(t.numel(), t.dtype, t.device) for t in lists[1]]):
+        raise CudaExtensionValidationError("out must match gradients in sizes, dtypes and device")

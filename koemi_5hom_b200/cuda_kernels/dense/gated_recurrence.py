@@ -10,11 +10,11 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
+from koemi_5hom_b200 import _native
 from koemi_5hom_b200.cuda_kernels import _training
-from koemi_5hom_b200.cuda_kernels.dense.affine_scan import (DenseCudaUnavailableError, DenseCudaValidationError,
-                                                            _load_library, native_cuda_available)
+from koemi_5hom_b200.cuda_kernels.dense.affine_scan import (DenseCudaBuildError, DenseCudaUnavailableError,
+                                                            DenseCudaValidationError, native_cuda_available)
 
 __all__ = ["gated_recurrence"]
 
@@ -36,37 +36,18 @@ def gated_recurrence(projections: Tensor, initial: Tensor | None = None, *, vali
     ``projections`` and ``initial``; a single token is ``length == 1``.
     """
     _validate(projections, initial, valid, restart, minimum_retention, maximum_retention)
-    _load_library(projections.device)
+    try:
+        _training.load(projections.device)
+    except _native.KoemiNativeUnavailableError as error:
+        raise DenseCudaBuildError(f"failed to load the native dense CUDA library: {error}") from error
     projections = projections.contiguous()
     initial, valid, restart = (None if t is None else t.contiguous() for t in (initial, valid, restart))
     if projections.shape[1] == 0:
         features = projections.shape[2] // 2
         start = projections.new_zeros((projections.shape[0], features), dtype=torch.float32) if initial is None else initial.clone()
         return projections[..., :features].contiguous(), start
-    if torch.is_grad_enabled() and (projections.requires_grad or (initial is not None and initial.requires_grad)):
-        return _GatedRecurrence.apply(projections, initial, valid, restart, minimum_retention, maximum_retention)
-    return _training.gated_recurrence(projections, initial, valid, restart, minimum_retention, maximum_retention, False)[:2]
-
-
-class _GatedRecurrence(torch.autograd.Function):
-    @staticmethod
-    def forward(context, projections, initial, valid, restart, low, high):
-        states, final, carries = _training.gated_recurrence(projections, initial, valid, restart, low, high, True)
-        context.save_for_backward(projections, valid, restart, carries)
-        context.bounds = low, high
-        context.set_materialize_grads(False)
-        return states, final
-
-    @staticmethod
-    @once_differentiable
-    def backward(context, grad_states, grad_final):
-        if grad_states is None and grad_final is None:
-            return None, None, None, None, None, None
-        projections, valid, restart, carries = context.saved_tensors
-        grad_states, grad_final = (None if g is None else g.contiguous() for g in (grad_states, grad_final))
-        grad_projections, grad_initial = _training.gated_recurrence_backward(
-            projections, valid, restart, carries, grad_states, grad_final, *context.bounds)
-        return grad_projections, grad_initial if context.needs_input_grad[1] else None, None, None, None, None
+    return torch.ops.koemi_b200.gated_recurrence.default(projections, initial, valid, restart, minimum_retention,
+                                                         maximum_retention)
 
 
 def _validate(projections, initial, valid, restart, low, high) -> None:

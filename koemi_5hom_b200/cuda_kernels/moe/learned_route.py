@@ -11,8 +11,8 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
+from koemi_5hom_b200 import _native
 from koemi_5hom_b200.cuda_kernels import _training
 
 __all__ = ["LearnedRoute", "route_learned_topk"]
@@ -44,7 +44,7 @@ def route_learned_topk(gate_logits: Tensor, valid_mask: Tensor | None = None, *,
     ids -1, weights and gradient zero. A NaN logit is never preferred and makes
     its row's weights NaN. Differentiable to first order in the logits.
     """
-    from koemi_5hom_b200.cuda_kernels.moe import CudaMoeValidationError, load_native_extension
+    from koemi_5hom_b200.cuda_kernels.moe import CudaMoeUnavailableError, CudaMoeValidationError  # the package imports this module
 
     def fail(message: str) -> None:
         raise CudaMoeValidationError(message)
@@ -65,30 +65,9 @@ def route_learned_topk(gate_logits: Tensor, valid_mask: Tensor | None = None, *,
         fail("valid_mask must be boolean with shape [tokens]")
     if not gate_logits.is_cuda or (valid_mask is not None and valid_mask.device != gate_logits.device):
         fail("gate_logits and valid_mask must be CUDA tensors on one device")
-    load_native_extension()
-    logits = gate_logits.contiguous()
+    try:
+        _training.load(gate_logits.device)
+    except _native.KoemiNativeUnavailableError as error:
+        raise CudaMoeUnavailableError(f"Koemi MoE CUDA library failed to load: {error}") from error
     valid = None if valid_mask is None else valid_mask.contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
-        return LearnedRoute(*_LearnedRoute.apply(logits, valid, top_k, bool(renormalize)))
-    return LearnedRoute(*_training.route_learned(logits, valid, top_k, bool(renormalize))[:4])
-
-
-class _LearnedRoute(torch.autograd.Function):
-    @staticmethod
-    def forward(context, logits, valid, top_k, renormalize):
-        ids, weights, counts, balance, slope = _training.route_learned(logits, valid, top_k, renormalize)
-        context.save_for_backward(logits, ids, weights, slope)
-        context.renormalize = renormalize
-        context.mark_non_differentiable(ids, counts)
-        context.set_materialize_grads(False)
-        return ids, weights, counts, balance
-
-    @staticmethod
-    @once_differentiable
-    def backward(context, _ids, grad_weights, _counts, grad_balance):
-        if grad_weights is None and grad_balance is None:
-            return None, None, None, None
-        logits, ids, weights, slope = context.saved_tensors
-        grad_weights, grad_balance = (None if g is None else g.contiguous() for g in (grad_weights, grad_balance))
-        return _training.route_learned_backward(logits, ids, weights, slope, grad_weights, grad_balance,
-                                                context.renormalize), None, None, None
+    return LearnedRoute(*torch.ops.koemi_b200.route_learned.default(gate_logits.contiguous(), valid, top_k, bool(renormalize)))

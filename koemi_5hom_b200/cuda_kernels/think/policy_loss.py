@@ -13,10 +13,10 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
+from koemi_5hom_b200 import _native
 from koemi_5hom_b200.cuda_kernels import _training
-from koemi_5hom_b200.cuda_kernels.think.surprise import CudaThinkUnavailableError, CudaThinkValidationError, _load
+from koemi_5hom_b200.cuda_kernels.think.surprise import CudaThinkUnavailableError, CudaThinkValidationError
 
 __all__ = ["PolicyLoss", "policy_loss"]
 
@@ -49,42 +49,15 @@ def policy_loss(logits: Tensor, target_ids: Tensor, old_log_probs: Tensor, advan
     for f32 and bf16 logits the call allocates the logits' gradient.
     """
     _validate(logits, target_ids, old_log_probs, advantages, reference_log_probs, valid_mask, clip_low, clip_high, kl_weight)
-    _load(logits.device)
+    try:
+        _training.load(logits.device)
+    except _native.KoemiNativeUnavailableError as error:
+        raise CudaThinkUnavailableError(str(error)) from error
     if logits.shape[-1] > 1 and logits.stride(-1) != 1:
         logits = logits.contiguous()
-    others = tuple(None if t is None else t.contiguous() for t in
-                   (target_ids, old_log_probs, advantages, reference_log_probs, valid_mask))
-    options = float(clip_low), float(clip_high), float(kl_weight)
-    if logits.requires_grad and torch.is_grad_enabled():
-        return PolicyLoss(*_PolicyLoss.apply(logits, *others, *options))
-    return PolicyLoss(*_training.policy_loss(logits, *others, *options, False)[:3])
-
-
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(context, logits, targets, old, advantages, reference, valid, clip_low, clip_high, kl_weight):
-        at_once = logits.dtype != torch.float16
-        loss, kl, log_probs, kept, gradient = _training.policy_loss(
-            logits, targets, old, advantages, reference, valid, clip_low, clip_high, kl_weight, at_once)
-        context.save_for_backward(logits, targets, valid, kept)
-        context.gradient = gradient if at_once else None
-        context.mark_non_differentiable(kl, log_probs)
-        context.set_materialize_grads(False)
-        return loss, kl, log_probs
-
-    @staticmethod
-    @once_differentiable
-    def backward(context, grad_loss, _kl, _log_probs):
-        none = (None,) * 9
-        if grad_loss is None:
-            return none
-        logits, targets, valid, kept = context.saved_tensors
-        gradient, context.gradient = context.gradient, None
-        if gradient is None:  # f16, or another backward through a retained graph
-            gradient = _training.policy_loss_backward(logits, targets, valid, kept, grad_loss)
-        else:
-            _training.policy_loss_scale(gradient, grad_loss)
-        return (gradient, *none[1:])
+    others = (None if t is None else t.contiguous() for t in
+              (target_ids, old_log_probs, advantages, reference_log_probs, valid_mask))
+    return PolicyLoss(*torch.ops.koemi_b200.policy_loss.default(logits, *others, clip_low, clip_high, kl_weight))
 
 
 def _validate(logits, targets, old, advantages, reference, valid, clip_low, clip_high, kl_weight) -> None:
