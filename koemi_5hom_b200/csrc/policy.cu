@@ -12,13 +12,18 @@
 //
 // The logits are read once and their gradient is written once, in one pass
 // over the rows, bound by HBM. Up to 1024 entries a warp holds a row in
-// registers. Up to 32768 a CTA of 256, 512 or 1024 threads does: a bulk copy
-// brings the row into shared memory (the next rows' copies run meanwhile), a
-// thread turns 32 entries into exponentials relative to its warp's maximum,
-// the warps' (maximum, sum) pairs meet at the row's only barrier, and the
-// gradient is the kept exponential times one factor per warp: one exponential
-// per entry, one read of shared memory. Longer rows are walked twice from
-// memory in blocks of 32768, the second time mostly from L2.
+// registers. Up to 32768 (fp32) or 65536 a CTA of 64 to 1024 threads does: a bulk copy brings
+// the row into shared memory, a thread takes 128 bytes of it (32 fp32 or 64
+// 16-bit entries) into registers, which frees the buffer for the next row's
+// copy, adds its exponentials up relative to its warp's maximum, and the
+// warps' (maximum, sum) pairs meet at the row's only barrier; then it forms the
+// gradient from its registers. fp32 entries are kept as exponentials, 16-bit
+// ones as they came, with a second exponential: half the registers, so that
+// two CTAs share an SM at 32768 entries and hide each other's latency (8192 x
+// 32768 bf16: 178 us, 243 us with one CTA of 1024 threads that keeps
+// exponentials).
+// Longer rows are walked twice from memory in blocks of 32768, the second time
+// mostly from L2.
 // Every row belongs to one CTA and per-CTA sums are added in a fixed order by
 // a second kernel, so equal inputs give equal bits.
 #include "vec.cuh"
@@ -26,9 +31,13 @@
 namespace koemi {
 namespace {
 
-constexpr int kPolicyBlocks = 1184;     // most CTAs of a launch: eight per SM
+constexpr int kPolicyBlocks = 2368;     // most CTAs of a launch: 16 per SM
 constexpr int kWarpRow = 1024;          // entries a warp holds
-constexpr int kPerThread = 32;          // entries a thread holds
+constexpr int kThreadBytes = 128;       // bytes of a row that a thread holds
+template <typename T>
+constexpr int64_t longest_row() {       // entries a CTA of 1024 threads holds
+    return 1024 * kThreadBytes / sizeof(T);
+}
 constexpr int64_t kCountedRows = 16384; // up to here every CTA counts the valid rows itself
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -47,27 +56,6 @@ struct PolicyTerms {
     const uint8_t *valid;                       // may be NULL: every row
     float clip_low, clip_high, beta;
 };
-
-// Loss, KL and d loss / d log-prob of one row.
-__device__ __forceinline__ void policy_terms(const PolicyTerms &terms, int64_t row, float lp, float &loss, float &kl,
-                                             float &slope) {
-    const float a = terms.advantages[row];
-    const float r = expf(lp - terms.old[row]);
-    const float free = r * a;
-    const float clipped = fminf(fmaxf(r, 1.0f - terms.clip_low), 1.0f + terms.clip_high) * a;
-    const bool take = free <= clipped;
-    loss = -(take ? free : clipped);
-    slope = take ? -free : 0.0f;
-    kl = 0.0f;
-    if (terms.reference != nullptr) {
-        const float d = terms.reference[row] - lp;
-        const float e = expm1f(d);
-        kl = e - d;
-        loss += terms.beta * kl;
-        slope -= terms.beta * e;
-    }
-    if (isnan(free) || isnan(clipped)) loss = slope = NAN;
-}
 
 __device__ __forceinline__ bool aligned_to(const void *p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
@@ -104,6 +92,31 @@ __device__ __forceinline__ float ex2_approx(float x) {
     return r;
 }
 
+// Two fp32 operations in one issue slot.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 r, a, b;\n\t"
+        "mov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 r, a, b;\n\t"
+        "mov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+template <int kWidth>
+__device__ __forceinline__ float packet_max(const float (&v)[kWidth]) {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < kWidth; ++i) m = fmaxf(m, v[i]);
+    return m;
+}
+
 // e^(v - m), m a maximum: the difference is exact to half a unit in its last
 // place whatever the logits' magnitude (the type's lowest value in every entry
 // gives a uniform row); ex2.approx adds 2 units. A maximum of nothing but -inf
@@ -128,14 +141,46 @@ struct PolicyOut {
     float2 *partials;
 };
 
-// A row's scalars, loaded ahead of its logits.
+// A row's scalars, loaded ahead of its logits, and what follows from its
+// log-sum-exp: every thread takes the slope (two ex2.approx), one thread per
+// row the loss and the KL term (expf and expm1f: exp(d) - d - 1 cancels).
 template <typename T>
 struct RowScalars {
-    int64_t target;
-    float chosen;
-    __device__ RowScalars(const T *row, const PolicyTerms &terms, int64_t index, int64_t vocab) {
-        target = terms.targets[index];
-        chosen = target >= 0 && target < vocab ? to_acc(row[target]) : NAN;
+    int target;  // -1 outside the vocabulary
+    float chosen, old, advantage, reference;
+    __device__ __forceinline__ RowScalars(const T *row, const PolicyTerms &terms, int64_t index, int vocab) {
+        const int64_t id = terms.targets[index];
+        target = id >= 0 && id < vocab ? static_cast<int>(id) : -1;
+        chosen = target >= 0 ? to_acc(row[target]) : NAN;
+        old = terms.old[index];
+        advantage = terms.advantages[index];
+        reference = terms.reference != nullptr ? terms.reference[index] : 0.0f;
+    }
+    // d loss / d log-prob, of a row alone
+    __device__ __forceinline__ float slope(const PolicyTerms &terms, float lp) const {
+        const float r = exp_from(lp, old), free = r * advantage;
+        const float clipped = fminf(fmaxf(r, 1.0f - terms.clip_low), 1.0f + terms.clip_high) * advantage;
+        float s = free <= clipped ? -free : 0.0f;
+        if (terms.reference != nullptr) s += terms.beta * (1.0f - exp_from(reference, lp));
+        return isnan(free) || isnan(clipped) ? NAN : s;
+    }
+    __device__ void add_loss(const PolicyTerms &terms, float lp, float &loss, float &kl) const {
+        const float r = expf(lp - old), free = r * advantage;
+        const float clipped = fminf(fmaxf(r, 1.0f - terms.clip_low), 1.0f + terms.clip_high) * advantage;
+        loss -= isnan(free) || isnan(clipped) ? NAN : fminf(free, clipped);
+        if (terms.reference != nullptr) {
+            const float d = reference - lp, k = expm1f(d) - d;
+            kl += k;
+            loss = fmaf(terms.beta, k, loss);
+        }
+    }
+    // the row's results, by one thread
+    __device__ void finish(const PolicyTerms &terms, const PolicyOut &out, int64_t index, float lp, float lse,
+                           float scaled_slope, float &loss, float &kl) const {
+        add_loss(terms, lp, loss, kl);
+        out.log_probs[index] = lp;
+        out.lse[index] = lse;
+        out.slopes[index] = scaled_slope;
     }
 };
 
@@ -174,17 +219,8 @@ __global__ __launch_bounds__(256) void policy_warp_kernel(PolicyRows shape, Poli
             p.sum += e[j];
         }
         p.sum = warp_sum(p.sum);
-        const float lse = lse_of(p), lp = scalars.chosen - lse;
-        float loss, kl, slope;
-        policy_terms(terms, row, lp, loss, kl, slope);
-        loss_sum += loss;
-        kl_sum += kl;
-        slope *= scale;
-        if (lane == 0) {
-            result.log_probs[row] = lp;
-            result.lse[row] = lse;
-            result.slopes[row] = slope;
-        }
+        const float lse = lse_of(p), lp = scalars.chosen - lse, slope = scalars.slope(terms, lp) * scale;
+        if (lane == 0) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
         if (out != nullptr) {
             const float factor = -slope / p.sum;
 #pragma unroll
@@ -211,31 +247,33 @@ template <typename T>
 struct Packets {
     static constexpr int kWidth = Pack<T>::kWidth;
     const T *base;  // the boundary at or before the row's start
-    int skip;
-    int64_t vocab, count;
-    __device__ Packets(const T *row, int64_t vocab_) : vocab(vocab_) {
+    int skip, vocab, count;
+    int first, end;  // packets first .. end - 1 are whole
+    __device__ __forceinline__ Packets(const T *row, int vocab_) : vocab(vocab_) {
         skip = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
         base = row - skip;
         count = (skip + vocab + kWidth - 1) / kWidth;
+        first = skip > 0 ? 1 : 0;
+        end = (skip + vocab) / kWidth;
     }
-    __device__ __forceinline__ bool whole(int64_t c) const { return c * kWidth >= skip && (c + 1) * kWidth <= skip + vocab; }
-    __device__ __forceinline__ int64_t first_whole() const { return skip > 0 ? 1 : 0; }
-    __device__ __forceinline__ int64_t end_whole() const { return (skip + vocab) / kWidth; }
-    __device__ __forceinline__ bool in_row(int64_t c, int i) const {
-        const int64_t at = c * kWidth + i;
-        return at >= skip && at < skip + vocab;
+    __device__ __forceinline__ bool whole(int c) const { return c >= first && c < end; }
+    __device__ __forceinline__ bool in_row(int c, int i) const {
+        return static_cast<unsigned>(c * kWidth + i - skip) < static_cast<unsigned>(vocab);
     }
-    // entries of a packet that is partly outside, one by one
-    __device__ __forceinline__ void load_partly(int64_t c, float (&v)[kWidth]) const {
+    // entries of a packet that is partly (or all) outside, one by one
+    __device__ __forceinline__ void load_partly(int c, float (&v)[kWidth]) const {
 #pragma unroll
-        for (int i = 0; i < kWidth; ++i) v[i] = in_row(c, i) ? to_acc(base[c * kWidth + i]) : -INFINITY;
+        for (int i = 0; i < kWidth; ++i) v[i] = in_row(c, i) ? to_acc(base[int64_t(c) * kWidth + i]) : -INFINITY;
     }
-    // v into packet c of the row at `out`, whose packets lie as this row's
-    // where `fits`, else one by one
-    __device__ __forceinline__ void store(T *out, bool fits, int64_t c, const float (&v)[kWidth]) const {
-        T *to = out - skip + c * kWidth;
-        if (fits && whole(c)) {
-            *reinterpret_cast<uint4 *>(to) = pack(v, T());
+    // Whether the packets of the row at `out` lie as this row's.
+    __device__ __forceinline__ bool fits(const T *out) const {
+        return reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T) == static_cast<unsigned>(skip);
+    }
+    // v into packet c of the row at `out`: whole, or one by one
+    __device__ __forceinline__ void store(T *out, bool whole_packet, int c, const float (&v)[kWidth]) const {
+        T *to = out - skip + int64_t(c) * kWidth;
+        if (whole_packet) {
+            __stcs(reinterpret_cast<uint4 *>(to), pack(v, T()));
             return;
         }
 #pragma unroll
@@ -243,17 +281,14 @@ struct Packets {
             if (in_row(c, i)) to[i] = from_acc<T>(v[i]);
         }
     }
-    __device__ __forceinline__ bool fits(const T *out) const {
-        return reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T) == static_cast<unsigned>(skip);
-    }
 };
 
 // Zeros into a row of the gradient, by a CTA.
 template <typename T>
-__device__ void clear_row(T *out, int64_t vocab) {
+__device__ void clear_row(T *out, int vocab) {
     const Packets<T> packets(out, vocab);
-    float zeros[Packets<T>::kWidth] = {};
-    for (int64_t c = threadIdx.x; c < packets.count; c += blockDim.x) packets.store(out, true, c, zeros);
+    const float zeros[Packets<T>::kWidth] = {};
+    for (int c = threadIdx.x; c < packets.count; c += blockDim.x) packets.store(out, packets.whole(c), c, zeros);
 }
 
 // The warps' partials of a row, merged by every warp alike: the row's partial
@@ -275,31 +310,62 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
                  : "memory");
 }
 
-// Up to 32 entries a thread: a CTA per row at a time.
-template <typename T, int kThreads>
+// Two entries at a time of a packet's words.
+__device__ __forceinline__ float2 word_of(uint32_t w, __nv_bfloat16) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&w)); }
+__device__ __forceinline__ float2 word_of(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2 *>(&w)); }
+// The larger entries of two packets; a NaN is passed over (the sum shows it).
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b, __nv_bfloat16) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&m);
+}
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b, __half) {
+    const __half2 m = __hmax2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&m);
+}
+template <typename T>
+__device__ __forceinline__ float row_part_max(const uint4 &m, T type) {
+    const uint32_t w = word_max(word_max(m.x, m.y, type), word_max(m.z, m.w, type), type);
+    const float2 v = word_of(w, type);
+    return fmaxf(v.x, v.y);
+}
+__device__ __forceinline__ float row_part_max(const uint4 &m, float) {
+    return fmaxf(fmaxf(__uint_as_float(m.x), __uint_as_float(m.y)), fmaxf(__uint_as_float(m.z), __uint_as_float(m.w)));
+}
+template <typename T>
+__device__ __forceinline__ uint4 packet_larger(const uint4 &a, const uint4 &b, T type) {
+    return make_uint4(word_max(a.x, b.x, type), word_max(a.y, b.y, type), word_max(a.z, b.z, type), word_max(a.w, b.w, type));
+}
+__device__ __forceinline__ uint4 packet_larger(const uint4 &a, const uint4 &b, float) {
+    auto larger = [](uint32_t x, uint32_t y) { return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y))); };
+    return make_uint4(larger(a.x, b.x), larger(a.y, b.y), larger(a.z, b.z), larger(a.w, b.w));
+}
+__device__ __forceinline__ float2 exp_from(float2 v, float from) {
+    v = mul2(add2(v, make_float2(-from, -from)), make_float2(kLog2e, kLog2e));
+    return make_float2(ex2_approx(v.x), ex2_approx(v.y));
+}
+
+// A CTA per row at a time. kExact: every row is whole packets (16-byte aligned
+// rows, a vocabulary of whole packets).
+template <typename T, int kThreads, bool kExact>
 __global__ __launch_bounds__(kThreads, 1024 / kThreads) void policy_row_kernel(
     PolicyRows shape, PolicyTerms terms, const T *__restrict__ logits, PolicyOut result, T *__restrict__ grad_logits,
     int buffers, uint32_t buffer_bytes, int *status) {
-    constexpr int kWidth = Pack<T>::kWidth, kPackets = kPerThread / kWidth;
+    constexpr int kWidth = Pack<T>::kWidth, kPackets = kThreadBytes / 16;
     extern __shared__ __align__(128) unsigned char smem_raw[];
     __shared__ uint64_t full[4];
     __shared__ Partial merged[2][32];
+    const int vocab = static_cast<int>(shape.vocab);
     auto live = [&](int64_t row) { return terms.valid == nullptr || terms.valid[row] != 0; };
     int64_t next = blockIdx.x;  // thread 0: the next row to load
     int loaded = 0;
     auto load_next = [&] {
         while (next < shape.rows && !live(next)) next += gridDim.x;
         if (next >= shape.rows) return;
-        const Packets<T> packets(logits + shape.start(next), shape.vocab);
-        const int64_t first = packets.first_whole(), end = packets.end_whole();
+        const Packets<T> packets(logits + shape.start(next), vocab);  // more than 1024 entries: some packets are whole
         uint64_t *bar = &full[loaded % buffers];
-        if (end > first) {
-            const uint32_t bytes = static_cast<uint32_t>(end - first) * 16;
-            mbar_arrive_expect_tx(bar, bytes);
-            bulk_load(smem_raw + loaded % buffers * buffer_bytes + first * 16, packets.base + first * kWidth, bytes, bar);
-        } else {
-            mbar_arrive(bar);
-        }
+        const uint32_t bytes = static_cast<uint32_t>(packets.end - packets.first) * 16;
+        mbar_arrive_expect_tx(bar, bytes);
+        bulk_load(smem_raw + loaded % buffers * buffer_bytes + packets.first * 16, packets.base + packets.first * kWidth, bytes, bar);
         ++loaded;
         next += gridDim.x;
     };
@@ -316,79 +382,92 @@ __global__ __launch_bounds__(kThreads, 1024 / kThreads) void policy_row_kernel(
     bool dead = false;  // a copy never arrived: go on without waiting or loading
     int taken = 0;
     for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
-        T *out = grad_logits == nullptr ? nullptr : grad_logits + row * shape.vocab;
+        T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
         if (!live(row)) {
-            if (out != nullptr) clear_row(out, shape.vocab);
-            if (threadIdx.x == 0) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
+            if (out != nullptr) clear_row(out, vocab);
+            if (threadIdx.x == kThreads - 1) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
             continue;
         }
         const T *in = logits + shape.start(row);
-        const RowScalars<T> scalars(in, terms, row, shape.vocab);
-        const Packets<T> packets(in, shape.vocab);
-        const uint4 *staged = reinterpret_cast<const uint4 *>(smem_raw + taken % buffers * buffer_bytes);
+        const RowScalars<T> scalars(in, terms, row, vocab);
+        const Packets<T> packets(in, vocab);
+        const uint4 *staged = reinterpret_cast<const uint4 *>(smem_raw + taken % buffers * buffer_bytes) + threadIdx.x;
         if (!dead) dead = !mbar_wait_bounded(&full[taken % buffers], static_cast<uint32_t>(taken / buffers) & 1, status);
 
-        float e[kPackets][kWidth];
-        Partial p{-INFINITY, 0.0f};
+        uint4 kept[kPackets];
 #pragma unroll
         for (int j = 0; j < kPackets; ++j) {
             const int c = threadIdx.x + j * kThreads;
-            if (c < packets.count && packets.whole(c)) {
-                unpack(staged[c], e[j], T());
+            if (kExact ? c < packets.count : packets.whole(c)) {
+                kept[j] = staged[j * kThreads];
             } else {
-                packets.load_partly(c, e[j]);  // -inf throughout where c is behind the row
-            }
+                float v[kWidth];
 #pragma unroll
-            for (int i = 0; i < kWidth; ++i) p.max = fmaxf(p.max, e[j][i]);
+                for (int i = 0; i < kWidth; ++i) v[i] = -INFINITY;
+                if (!kExact) packets.load_partly(c, v);
+                kept[j] = pack(v, T());
+            }
         }
-        p.max = warp_max(p.max);
+        uint4 largest = kept[0];
+#pragma unroll
+        for (int j = 1; j < kPackets; ++j) largest = packet_larger(largest, kept[j], T());
+        Partial p{warp_max(row_part_max(largest, T())), 0.0f};
         const float from = origin(p.max);
+        float2 sums = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < kPackets; ++j) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kWidth; ++i) {
-                e[j][i] = exp_from(e[j][i], from);
-                sum += e[j][i];
+            if constexpr (sizeof(T) == 4) {
+                const float2 x = exp_from(make_float2(__uint_as_float(kept[j].x), __uint_as_float(kept[j].y)), from);
+                const float2 y = exp_from(make_float2(__uint_as_float(kept[j].z), __uint_as_float(kept[j].w)), from);
+                sums = add2(sums, add2(x, y));
+                kept[j] = make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
+            } else {
+                sums = add2(sums, exp_from(word_of(kept[j].x, T()), from));
+                sums = add2(sums, exp_from(word_of(kept[j].y, T()), from));
+                sums = add2(sums, exp_from(word_of(kept[j].z, T()), from));
+                sums = add2(sums, exp_from(word_of(kept[j].w, T()), from));
             }
-            p.sum += sum;
         }
-        p.sum = warp_sum(p.sum);
+        p.sum = warp_sum(sums.x + sums.y);
         const Partial all = block_merge<kThreads>(p, merged, taken & 1);
         // every thread is done with the row's buffer
         if (threadIdx.x == 0 && !dead) load_next();
         ++taken;
 
-        const float lse = lse_of(all), lp = scalars.chosen - lse;
-        float loss, kl, slope;
-        policy_terms(terms, row, lp, loss, kl, slope);
-        loss_sum += loss;
-        kl_sum += kl;
-        slope *= scale;
-        if (threadIdx.x == 0) {
-            result.log_probs[row] = lp;
-            result.lse[row] = lse;
-            result.slopes[row] = slope;
-        }
+        const float lse = lse_of(all), lp = scalars.chosen - lse, slope = scalars.slope(terms, lp) * scale;
+        if (threadIdx.x == kThreads - 1) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
         if (out != nullptr) {
-            const float factor = -slope / all.sum * exp_from(from, all.max);
-            const bool fits = packets.fits(out);
-            const int64_t at = scalars.target + packets.skip;  // the target's place among the packets' entries
+            // of an fp32 warp with nothing but -inf: 0
+            const float factor = -slope / all.sum * (sizeof(T) == 4 ? exp_from(p.max, all.max) : 1.0f);
+            const bool fits = kExact || packets.fits(out);
+            // the packet and the place in it of the target
+            const int at = scalars.target + packets.skip, packet = scalars.target >= 0 ? at / kWidth : -1;
 #pragma unroll
             for (int j = 0; j < kPackets; ++j) {
                 const int c = threadIdx.x + j * kThreads;
                 if (c >= packets.count) continue;
+                // from here a value of its own: else the first loop's fp32
+                // entries would be kept across the barrier, and spilled
+                asm("" : "+r"(kept[j].x), "+r"(kept[j].y), "+r"(kept[j].z), "+r"(kept[j].w));
+                float v[kWidth];
+                unpack(kept[j], v, T());
 #pragma unroll
-                for (int i = 0; i < kWidth; ++i) e[j][i] *= factor;
-                if (at / kWidth == c) {
-#pragma unroll
-                    for (int i = 0; i < kWidth; ++i) e[j][i] += at % kWidth == i ? slope : 0.0f;
+                for (int i = 0; i < kWidth; i += 2) {
+                    float2 e = make_float2(v[i], v[i + 1]);
+                    if constexpr (sizeof(T) == 2) e = exp_from(e, all.max);
+                    e = mul2(e, make_float2(factor, factor));
+                    v[i] = e.x;
+                    v[i + 1] = e.y;
                 }
-                packets.store(out, fits, c, e[j]);
+                if (packet == c) {
+#pragma unroll
+                    for (int i = 0; i < kWidth; ++i) v[i] += at % kWidth == i ? slope : 0.0f;
+                }
+                packets.store(out, kExact || (fits && packets.whole(c)), c, v);
             }
         }
     }
-    if (threadIdx.x == 0) result.partials[blockIdx.x] = make_float2(loss_sum, kl_sum);
+    if (threadIdx.x == kThreads - 1) result.partials[blockIdx.x] = make_float2(loss_sum, kl_sum);
 }
 
 // Longer rows, in blocks of 1024 threads x 32 entries, walked twice.
@@ -397,32 +476,33 @@ template <typename T>
 __global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows shape, PolicyTerms terms,
                                                                    const T *__restrict__ logits, PolicyOut result,
                                                                    T *__restrict__ grad_logits) {
-    constexpr int kWidth = Pack<T>::kWidth, kPackets = kPerThread / kWidth / 2;  // in flight per thread
+    constexpr int kWidth = Pack<T>::kWidth, kPackets = 32 / kWidth / 2;  // in flight per thread
     __shared__ Partial merged[2][32];
+    const int vocab = static_cast<int>(shape.vocab);
     const float scale = result.inverse != nullptr ? *result.inverse : inverse_count(terms.valid, shape.rows);
     float loss_sum = 0.0f, kl_sum = 0.0f;
     int taken = 0;
     for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
-        T *out = grad_logits == nullptr ? nullptr : grad_logits + row * shape.vocab;
+        T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
         if (terms.valid != nullptr && terms.valid[row] == 0) {
-            if (out != nullptr) clear_row(out, shape.vocab);
+            if (out != nullptr) clear_row(out, vocab);
             if (threadIdx.x == 0) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
             continue;
         }
         const T *in = logits + shape.start(row);
-        const RowScalars<T> scalars(in, terms, row, shape.vocab);
-        const Packets<T> packets(in, shape.vocab);
+        const RowScalars<T> scalars(in, terms, row, vocab);
+        const Packets<T> packets(in, vocab);
         auto walk = [&](auto &&each) {
-            for (int64_t first = threadIdx.x; first < packets.count; first += kPackets * kWalkThreads) {
+            for (int first = threadIdx.x; first < packets.count; first += kPackets * kWalkThreads) {
                 uint4 raw[kPackets];
 #pragma unroll
                 for (int j = 0; j < kPackets; ++j) {
-                    const int64_t c = first + j * kWalkThreads;
-                    raw[j] = c < packets.count && packets.whole(c) ? load_cached(packets.base + c * kWidth) : make_uint4(0, 0, 0, 0);
+                    const int c = first + j * kWalkThreads;
+                    raw[j] = packets.whole(c) ? load_cached(packets.base + int64_t(c) * kWidth) : make_uint4(0, 0, 0, 0);
                 }
 #pragma unroll
                 for (int j = 0; j < kPackets; ++j) {
-                    const int64_t c = first + j * kWalkThreads;
+                    const int c = first + j * kWalkThreads;
                     if (c >= packets.count) continue;
                     float v[kWidth];
                     if (packets.whole(c)) {
@@ -435,10 +515,8 @@ __global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows sh
             }
         };
         Partial p{-INFINITY, 0.0f};
-        walk([&](int64_t, const float (&v)[kWidth]) {
-            float m = v[0];
-#pragma unroll
-            for (int i = 1; i < kWidth; ++i) m = fmaxf(m, v[i]);
+        walk([&](int, const float (&v)[kWidth]) {
+            const float m = packet_max(v);
             if (m > p.max) {
                 p.sum *= exp_from(p.max, m);
                 p.max = m;
@@ -448,29 +526,20 @@ __global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows sh
             for (int i = 0; i < kWidth; ++i) p.sum += exp_from(v[i], from);
         });
         const Partial all = block_merge<kWalkThreads>(warp_merge(p), merged, taken++ & 1);
-        const float lse = lse_of(all), lp = scalars.chosen - lse;
-        float loss, kl, slope;
-        policy_terms(terms, row, lp, loss, kl, slope);
-        loss_sum += loss;
-        kl_sum += kl;
-        slope *= scale;
-        if (threadIdx.x == 0) {
-            result.log_probs[row] = lp;
-            result.lse[row] = lse;
-            result.slopes[row] = slope;
-        }
+        const float lse = lse_of(all), lp = scalars.chosen - lse, slope = scalars.slope(terms, lp) * scale;
+        if (threadIdx.x == 0) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
         if (out != nullptr) {
             const float factor = -slope / all.sum;
             const bool fits = packets.fits(out);
-            const int64_t at = scalars.target + packets.skip;
-            walk([&](int64_t c, float (&v)[kWidth]) {
+            const int at = scalars.target + packets.skip, packet = scalars.target >= 0 ? at / kWidth : -1;
+            walk([&](int c, float (&v)[kWidth]) {
 #pragma unroll
                 for (int i = 0; i < kWidth; ++i) v[i] = exp_from(v[i], all.max) * factor;
-                if (at / kWidth == c) {
+                if (packet == c) {
 #pragma unroll
                     for (int i = 0; i < kWidth; ++i) v[i] += at % kWidth == i ? slope : 0.0f;
                 }
-                packets.store(out, fits, c, v);
+                packets.store(out, fits && packets.whole(c), c, v);
             });
         }
     }
@@ -519,28 +588,29 @@ __global__ __launch_bounds__(kBackwardThreads) void policy_backward_kernel(
     const float *__restrict__ grad_loss, T *__restrict__ grad_logits) {
     constexpr int kWidth = Pack<T>::kWidth, kPackets = 4;
     const float scale = *grad_loss;
-    const int64_t step = int64_t(gridDim.y) * kBackwardThreads * kPackets;
+    const int vocab = static_cast<int>(shape.vocab), step = static_cast<int>(gridDim.y) * kBackwardThreads * kPackets;
     for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
         const T *in = logits + shape.start(row);
-        T *out = grad_logits + row * shape.vocab;
+        T *out = grad_logits + row * vocab;
         if (valid != nullptr && valid[row] == 0) {
-            if (blockIdx.y == 0) clear_row(out, shape.vocab);
+            if (blockIdx.y == 0) clear_row(out, vocab);
             continue;
         }
-        const Packets<T> packets(in, shape.vocab);
+        const Packets<T> packets(in, vocab);
         const bool fits = packets.fits(out);
         const float slope = slopes[row] * scale, from = lse[row];
-        const int64_t at = targets[row] + packets.skip;
-        for (int64_t first = int64_t(blockIdx.y) * kBackwardThreads * kPackets + threadIdx.x; first < packets.count; first += step) {
+        const int64_t target = targets[row];
+        const int at = static_cast<int>(target) + packets.skip, packet = target >= 0 && target < vocab ? at / kWidth : -1;
+        for (int first = blockIdx.y * kBackwardThreads * kPackets + threadIdx.x; first < packets.count; first += step) {
             uint4 raw[kPackets];
 #pragma unroll
             for (int j = 0; j < kPackets; ++j) {
-                const int64_t c = first + j * kBackwardThreads;
-                raw[j] = c < packets.count && packets.whole(c) ? load_cached(packets.base + c * kWidth) : make_uint4(0, 0, 0, 0);
+                const int c = first + j * kBackwardThreads;
+                raw[j] = packets.whole(c) ? load_cached(packets.base + int64_t(c) * kWidth) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int j = 0; j < kPackets; ++j) {
-                const int64_t c = first + j * kBackwardThreads;
+                const int c = first + j * kBackwardThreads;
                 if (c >= packets.count) continue;
                 float v[kWidth];
                 if (packets.whole(c)) {
@@ -550,11 +620,11 @@ __global__ __launch_bounds__(kBackwardThreads) void policy_backward_kernel(
                 }
 #pragma unroll
                 for (int i = 0; i < kWidth; ++i) v[i] = -slope * exp_from(v[i], from);
-                if (at / kWidth == c) {
+                if (packet == c) {
 #pragma unroll
                     for (int i = 0; i < kWidth; ++i) v[i] += at % kWidth == i ? slope : 0.0f;
                 }
-                packets.store(out, fits, c, v);
+                packets.store(out, fits && packets.whole(c), c, v);
             }
         }
     }
@@ -588,17 +658,21 @@ int check_policy(const PolicyRows &shape) {
     return KOEMI_OK;
 }
 
-template <typename T, int kThreads>
-int launch_rows(const PolicyRows &shape, const PolicyTerms &terms, const T *logits, const PolicyOut &result, T *grad,
-                unsigned &blocks, cudaStream_t stream) {
-    // a row's packets, and one more where it starts inside a packet; as many
-    // buffers as fit beside the other CTAs of the SM (1024 threads in all)
-    const uint32_t bytes = static_cast<uint32_t>(ceil_div(shape.vocab * sizeof(T), 128) * 128 + 128);
-    const uint32_t room = 222 * 1024 / (1024 / kThreads) - 1024;
+// The row kernel with the fewest threads that hold `entries`.
+template <typename T, int kThreads = 64>
+int launch_rows(int64_t entries, bool exact, const PolicyRows &shape, const PolicyTerms &terms, const T *logits,
+                const PolicyOut &result, T *grad, unsigned &blocks, cudaStream_t stream) {
+    constexpr int64_t kHeld = kThreads * (kThreadBytes / sizeof(T));
+    if constexpr (kHeld < longest_row<T>()) {
+        if (entries > kHeld) return launch_rows<T, 2 * kThreads>(entries, exact, shape, terms, logits, result, grad, blocks, stream);
+    }
+    // as many buffers as fit beside the other CTAs of the SM (1024 threads in all)
+    const uint32_t bytes = static_cast<uint32_t>(ceil_div(entries * sizeof(T), 128) * 128);
+    const uint32_t room = 222 * 1024 / (1024 / kThreads) - 2048;
     const int buffers = static_cast<int>(room / bytes > 3 ? 3 : room / bytes);
     const int64_t places = int64_t(sm_count()) * (1024 / kThreads);
     blocks = static_cast<unsigned>(shape.rows < places ? shape.rows : places);
-    auto kernel = policy_row_kernel<T, kThreads>;
+    auto kernel = exact ? policy_row_kernel<T, kThreads, true> : policy_row_kernel<T, kThreads, false>;
     KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(buffers * bytes)));
     kernel<<<blocks, kThreads, buffers * bytes, stream>>>(shape, terms, logits, result, grad, buffers, bytes,
                                                           device_status_word());
@@ -641,12 +715,9 @@ int policy_forward(const PolicyRows &shape, const PolicyTerms &terms, const void
             rc = launch_warps<T, 16>(shape, terms, in, result, grad, blocks, stream);
         } else if (shape.vocab <= kWarpRow) {
             rc = launch_warps<T, 32>(shape, terms, in, result, grad, blocks, stream);
-        } else if (entries <= 256 * kPerThread) {
-            rc = launch_rows<T, 256>(shape, terms, in, result, grad, blocks, stream);
-        } else if (entries <= 512 * kPerThread) {
-            rc = launch_rows<T, 512>(shape, terms, in, result, grad, blocks, stream);
-        } else if (entries <= 1024 * kPerThread) {
-            rc = launch_rows<T, 1024>(shape, terms, in, result, grad, blocks, stream);
+        } else if (entries <= longest_row<T>()) {
+            const bool exact = !inside && shape.vocab % Pack<T>::kWidth == 0;
+            rc = launch_rows<T>(entries, exact, shape, terms, in, result, grad, blocks, stream);
         } else {
             const int64_t places = 2 * int64_t(sm_count());
             blocks = static_cast<unsigned>(shape.rows < places ? shape.rows : places);

@@ -524,6 +524,30 @@ def test_policy_masked_vocabulary(vocab, low, cuda):
     assert not grad[forbidden].any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [900, 8000, 32768, 70000])
+def test_policy_masked_halves_beside_very_low_logits(vocab, dtype, cuda):
+    """A run of forbidden entries longer than any thread's or warp's share, beside logits near -200: e^200 must not
+    meet their zeros."""
+    case = policy_case(4, vocab, dtype, 16, cuda)
+    half = vocab // 2
+    case["targets"] %= half
+    case["logits"] = (case["logits"].float() - 200).to(dtype)
+    case["logits"][:, half:] = -math.inf
+    case["logits"][3] = torch.finfo(dtype).min  # a row of the type's lowest value: uniform
+    lp = torch.log_softmax(case["logits"].double(), -1).gather(-1, case["targets"][:, None])[:, 0]
+    case["old"], case["reference"] = (lp - 0.1).float(), (lp + 0.1).float()
+    scale = 64.0 if dtype == torch.float16 else None
+    result, grad = run_policy(case, scale=scale)
+    # a log-sum-exp near -200 rounds at 16 times the magnitude of the ones above; the uniform row's at the lowest value's
+    check(result.log_probs[:3], plain_policy(case)[2][:3], torch.float32, (32 + 40 + 2 * 256) * EPS)
+    assert grad.isfinite().all() and not grad[:3, half:].any()
+    size = 3 * max(1.0, case["advantages"].abs().max().item()) * (scale or 1.0)
+    rounds = (1 if scale is None else 2) * U[dtype]
+    want = plain_policy(case, scale=scale or 1.0)[3]
+    check(grad[:3], want[:3], dtype, 2 * (32 + 40 + 2 * 256) * EPS * size + rounds * want[:3].abs().max().item())
+
+
 def test_policy_bad_targets_are_loud_and_local(cuda):
     case = policy_case(6, 500, torch.float32, 7, cuda)
     case["valid"][:] = True
