@@ -25,7 +25,8 @@
 namespace koemi {
 namespace {
 
-constexpr int kRouteWarps = 8;
+constexpr int kRouteWarps = 16;  // 32 warps per SM: a row is a chain of reductions
+constexpr int kWideWarps = 8;    // each has a row of sums in shared memory
 constexpr int kRouteBlocks = 296;
 
 struct RouteShape {
@@ -64,13 +65,13 @@ __global__ void route_forward_wide_kernel(RouteShape shape, const T *__restrict_
                                      float *__restrict__ weights, float *__restrict__ partial_mass,
                                      int32_t *__restrict__ partial_counts, int32_t *__restrict__ partial_live) {
     extern __shared__ float mass[];  // [warps][experts], then counts [experts]
-    int32_t *counts = reinterpret_cast<int32_t *>(mass + kRouteWarps * shape.experts);
+    int32_t *counts = reinterpret_cast<int32_t *>(mass + kWideWarps * shape.experts);
     __shared__ int32_t live_rows;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int64_t i = threadIdx.x; i < (kRouteWarps + 1) * shape.experts; i += blockDim.x) mass[i] = 0.0f;
+    for (int64_t i = threadIdx.x; i < (kWideWarps + 1) * shape.experts; i += blockDim.x) mass[i] = 0.0f;
     if (threadIdx.x == 0) live_rows = 0;
     __syncthreads();
-    for (int64_t t = int64_t(blockIdx.x) * kRouteWarps + warp; t < shape.tokens; t += int64_t(gridDim.x) * kRouteWarps) {
+    for (int64_t t = int64_t(blockIdx.x) * kWideWarps + warp; t < shape.tokens; t += int64_t(gridDim.x) * kWideWarps) {
         const T *row = logits + t * shape.experts;
         const RowSoftmax soft = row_softmax(row, shape.experts, shape.valid == nullptr || shape.valid[t] != 0);
         if (!soft.live) {
@@ -119,7 +120,7 @@ __global__ void route_forward_wide_kernel(RouteShape shape, const T *__restrict_
     __syncthreads();
     for (int64_t e = threadIdx.x; e < shape.experts; e += blockDim.x) {
         float sum = 0.0f;
-        for (int w = 0; w < kRouteWarps; ++w) sum += mass[w * shape.experts + e];
+        for (int w = 0; w < kWideWarps; ++w) sum += mass[w * shape.experts + e];
         partial_mass[blockIdx.x * shape.experts + e] = sum;
         partial_counts[blockIdx.x * shape.experts + e] = counts[e];
     }
@@ -204,12 +205,14 @@ __device__ __forceinline__ float group_sum(float v) {
     for (int offset = kLanes / 2; offset > 0; offset >>= 1) v += __shfl_xor_sync(0xffffffffu, v, offset);
     return v;
 }
-// Larger for what is chosen first: the value's order in the upper word (a NaN
-// ranks with -inf), the lower expert id first in the lower. 0: no candidate.
-__device__ __forceinline__ uint64_t rank_key(float v, int e) {
-    uint32_t bits = __float_as_uint(selectable(v) + 0.0f);  // -0 becomes +0
-    bits = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-    return static_cast<uint64_t>(bits) << 32 | static_cast<uint32_t>(~e);
+// The value's order as an integer; a NaN ranks with -inf. 0: no candidate.
+__device__ __forceinline__ uint32_t rank_key(float v) {
+    const uint32_t bits = __float_as_uint(selectable(v) + 0.0f);  // -0 becomes +0
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
 // One row of a group: the lane's logits become exponentials; -inf beyond the row.
@@ -238,7 +241,7 @@ __device__ __forceinline__ RowSoftmax load_row(const T *row, int experts, int at
 }
 
 template <typename T, int kLanes, int kPer>
-__global__ __launch_bounds__(kRouteWarps * 32) void route_forward_kernel(
+__global__ __launch_bounds__(kRouteWarps * 32, 2) void route_forward_kernel(
     RouteShape shape, const T *__restrict__ logits, int64_t *__restrict__ ids, float *__restrict__ weights,
     float *__restrict__ partial_mass, int32_t *__restrict__ partial_counts, int32_t *__restrict__ partial_live) {
     constexpr int kGroups = kRouteWarps * 32 / kLanes, kWidth = kLanes * kPer;
@@ -246,6 +249,8 @@ __global__ __launch_bounds__(kRouteWarps * 32) void route_forward_kernel(
     __shared__ int32_t counts[kWidth];
     __shared__ int32_t live_rows;
     const int at = threadIdx.x % kLanes, group = threadIdx.x / kLanes, warp = threadIdx.x >> 5;
+    // the lanes of this group: the reductions of a warp's groups are apart
+    const uint32_t members = kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1) << (threadIdx.x % 32 / kLanes * kLanes);
     const int experts = static_cast<int>(shape.experts), top_k = static_cast<int>(shape.top_k);
     for (int i = threadIdx.x; i < kWidth; i += blockDim.x) counts[i] = 0;
     if (threadIdx.x == 0) live_rows = 0;
@@ -259,49 +264,51 @@ __global__ __launch_bounds__(kRouteWarps * 32) void route_forward_kernel(
         float logit[kPer], e[kPer];
         const RowSoftmax soft = load_row<T, kLanes, kPer>(logits + t * shape.experts, experts, at, take, logit, e);
         const float inverse = 1.0f / soft.sum;
-        uint64_t keys[kPer];
+        uint32_t keys[kPer];
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             const int id = at + j * kLanes;
-            keys[j] = id < experts ? rank_key(logit[j], id) : 0;
+            keys[j] = id < experts ? rank_key(logit[j]) : 0;
             if (soft.live && id < experts) summed[j] += e[j] * inverse;
         }
         live += soft.live && at == 0;
-        float chosen = 0.0f, first_weight = 0.0f;
+        // Choice k stays in lane k % lanes, slot k / lanes, until all are known.
+        float chosen = 0.0f, weight[kPer] = {};
+        int choice[kPer] = {};
         for (int k = 0; k < top_k; ++k) {
-            uint64_t best = keys[0];
+            uint32_t best = keys[0];
 #pragma unroll
             for (int j = 1; j < kPer; ++j) best = keys[j] > best ? keys[j] : best;
+            best = __reduce_max_sync(members, best);
+            uint32_t id = 0xffffffffu;  // the lowest that has it
 #pragma unroll
-            for (int offset = kLanes / 2; offset > 0; offset >>= 1) {
-                const uint64_t other = __shfl_xor_sync(0xffffffffu, best, offset);
-                best = other > best ? other : best;
-            }
-            const int id = static_cast<int>(~static_cast<uint32_t>(best));
-            float p = 0.0f;
+            for (int j = kPer - 1; j >= 0; --j) id = keys[j] == best ? at + j * kLanes : id;
+            id = __reduce_min_sync(members, id);
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                if (keys[j] == best) {
-                    p = e[j] * inverse;
-                    keys[j] = 0;
+            for (int j = 0; j < kPer; ++j) keys[j] = static_cast<uint32_t>(at + j * kLanes) == id ? 0 : keys[j];
+            const float p = exp_from(value_of(best), soft.max) * inverse;
+            chosen += p;
+            if (k < kLanes) {
+                weight[0] = k == at ? p : weight[0];
+                choice[0] = k == at ? static_cast<int>(id) : choice[0];
+            } else {
+#pragma unroll
+                for (int j = 1; j < kPer; ++j) {
+                    weight[j] = k == at + j * kLanes ? p : weight[j];
+                    choice[j] = k == at + j * kLanes ? static_cast<int>(id) : choice[j];
                 }
             }
-            p = __shfl_sync(0xffffffffu, p, id % kLanes, kLanes);
-            chosen += p;
-            if (k % kLanes == at) first_weight = p;
-            if (t < shape.tokens && at == 0) {
-                ids[t * top_k + k] = soft.live ? id : -1;
-                if (soft.live) atomicAdd(&counts[id], 1);
-            }
-            // a lane keeps every kLanes-th weight; they are written kLanes at a time
-            if (t < shape.tokens && !shape.renormalize && (k % kLanes == kLanes - 1 || k == top_k - 1)) {
-                const int slot = k / kLanes * kLanes + at;
-                if (slot <= k) weights[t * top_k + slot] = soft.live ? first_weight : 0.0f;
-            }
-            if (shape.renormalize && t < shape.tokens && at == 0) weights[t * top_k + k] = soft.live ? p : 0.0f;
         }
-        if (shape.renormalize && t < shape.tokens && at == 0 && soft.live) {
-            for (int k = 0; k < top_k; ++k) weights[t * top_k + k] /= chosen;
+        if (t < shape.tokens) {
+            const float share = shape.renormalize ? 1.0f / chosen : 1.0f;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const int k = at + j * kLanes;
+                if (k >= top_k) continue;
+                ids[t * top_k + k] = soft.live ? choice[j] : -1;
+                weights[t * top_k + k] = soft.live ? weight[j] * share : 0.0f;
+                if (soft.live) atomicAdd(&counts[choice[j]], 1);
+            }
         }
     }
 #pragma unroll
@@ -324,7 +331,7 @@ __global__ __launch_bounds__(kRouteWarps * 32) void route_forward_kernel(
 }
 
 template <typename T, int kLanes, int kPer>
-__global__ __launch_bounds__(kRouteWarps * 32) void route_backward_kernel(
+__global__ __launch_bounds__(kRouteWarps * 32, 2) void route_backward_kernel(
     RouteShape shape, const T *__restrict__ logits, const int64_t *__restrict__ ids, const float *__restrict__ weights,
     const float *__restrict__ grad_weights, const float *__restrict__ grad_balance, const float *__restrict__ slope,
     T *__restrict__ grad_logits) {
@@ -386,7 +393,7 @@ __global__ void route_backward_wide_kernel(RouteShape shape, const T *__restrict
                                       T *__restrict__ grad_logits) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float db = grad_balance != nullptr ? *grad_balance : 0.0f;
-    for (int64_t t = int64_t(blockIdx.x) * kRouteWarps + warp; t < shape.tokens; t += int64_t(gridDim.x) * kRouteWarps) {
+    for (int64_t t = int64_t(blockIdx.x) * kWideWarps + warp; t < shape.tokens; t += int64_t(gridDim.x) * kWideWarps) {
         const T *row = logits + t * shape.experts;
         T *out = grad_logits + t * shape.experts;
         const int64_t *chosen = ids + t * shape.top_k;
@@ -428,7 +435,7 @@ __global__ void route_backward_wide_kernel(RouteShape shape, const T *__restrict
 
 // Rows a CTA takes in one turn: a warp each, or a group of lanes each.
 int rows_per_turn(int64_t experts) {
-    return experts <= 32 ? kRouteWarps * 4 : experts <= 64 ? kRouteWarps * 2 : kRouteWarps;
+    return experts <= 32 ? kRouteWarps * 4 : experts <= 64 ? kRouteWarps * 2 : experts <= 256 ? kRouteWarps : kWideWarps;
 }
 int64_t route_blocks(int64_t tokens, int64_t experts) {
     const int64_t blocks = ceil_div(tokens, rows_per_turn(experts));
@@ -468,10 +475,10 @@ int route_forward(const RouteShape &shape, const void *logits, int64_t *ids, flo
             shape, in, ids, weights, mass, partial_counts, live);
     });
     if (!narrow) {
-        const size_t smem = (kRouteWarps + 1) * shape.experts * sizeof(float);
+        const size_t smem = (kWideWarps + 1) * shape.experts * sizeof(float);
         auto kernel = route_forward_wide_kernel<T>;
         KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-        kernel<<<grid, kRouteWarps * 32, smem, stream>>>(shape, in, ids, weights, mass, partial_counts, live);
+        kernel<<<grid, kWideWarps * 32, smem, stream>>>(shape, in, ids, weights, mass, partial_counts, live);
     }
     KOEMI_LAUNCH_CHECK();
     route_finish_kernel<<<1, kFinishThreads, 0, stream>>>(mass, partial_counts, live, static_cast<int>(blocks),
@@ -493,7 +500,7 @@ int route_backward(const RouteShape &shape, const void *logits, const int64_t *i
             shape, in, ids, weights, grad_weights, grad_balance, slope, out);
     });
     if (!narrow) {
-        route_backward_wide_kernel<T><<<grid, kRouteWarps * 32, 0, stream>>>(shape, in, ids, weights, grad_weights,
+        route_backward_wide_kernel<T><<<grid, kWideWarps * 32, 0, stream>>>(shape, in, ids, weights, grad_weights,
                                                                              grad_balance, slope, out);
     }
     KOEMI_LAUNCH_CHECK();
