@@ -3,8 +3,8 @@
 //   norm = sqrt(sum over all tensors of g^2)
 //   out = g min(1, max_norm / (norm + 1e-6))
 //
-// The tensors travel in the kernel's parameters (up to kMaxTensors per
-// launch), cut into chunks of kChunkElements; a CTA adds its chunks' sums of
+// The tensors travel in the kernel's parameters, in a table of 16, 160 or 1000
+// (a launch copies the whole table, 28 KB of the largest), cut into chunks of kChunkElements; a CTA adds its chunks' sums of
 // squares up into one partial, and every CTA of the second kernel adds all
 // partials in the same fixed order, so equal inputs give equal bits. In place,
 // a factor of one writes nothing.
@@ -16,15 +16,17 @@ namespace koemi {
 namespace {
 
 constexpr int kMaxTensors = 1000;          // 24 bytes each: the parameters stay below 32 KB
+constexpr int kFewTensors = 16, kSomeTensors = 160;
 constexpr int64_t kChunkElements = 16384;  // elements summed in fp32; beyond, sums are fp64
 constexpr int kClipThreads = 256;
 constexpr int kClipBlocks = 888;  // six CTAs per SM
 
+template <int kTensors>
 struct ClipTable {
-    const void *in[kMaxTensors];
-    void *out[kMaxTensors];
-    uint32_t first_chunk[kMaxTensors + 1];
-    uint32_t tail_type[kMaxTensors];  // elements of the last chunk (1..kChunkElements) * 4 + type code
+    const void *in[kTensors];
+    void *out[kTensors];
+    uint32_t first_chunk[kTensors + 1];
+    uint32_t tail_type[kTensors];  // elements of the last chunk (1..kChunkElements) * 4 + type code
     int count;
 };
 
@@ -35,7 +37,8 @@ struct Chunk {
     int type;
 };
 
-__device__ __forceinline__ Chunk chunk_of(const ClipTable &table, uint32_t chunk) {
+template <int kTensors>
+__device__ __forceinline__ Chunk chunk_of(const ClipTable<kTensors> &table, uint32_t chunk) {
     int lo = 0, hi = table.count;  // first_chunk[lo] <= chunk < first_chunk[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
@@ -132,7 +135,8 @@ __device__ void chunk_scale(const T *in, T *out, int elements, float factor) {
     }
 }
 
-__global__ __launch_bounds__(kClipThreads) void clip_squares_kernel(const __grid_constant__ ClipTable table,
+template <int kTensors>
+__global__ __launch_bounds__(kClipThreads) void clip_squares_kernel(const __grid_constant__ ClipTable<kTensors> table,
                                                                     uint32_t chunks, double *__restrict__ partials) {
     __shared__ float sums[kClipThreads / 32];
     double total = 0.0;  // thread 0's
@@ -173,7 +177,8 @@ __device__ double sum_partials(const double *partials, int64_t count) {
     return sum;
 }
 
-__global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const __grid_constant__ ClipTable table,
+template <int kTensors>
+__global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const __grid_constant__ ClipTable<kTensors> table,
                                                                   uint32_t chunks, const double *__restrict__ partials,
                                                                   int64_t partial_count, float max_norm,
                                                                   float *__restrict__ norm_out) {
@@ -201,12 +206,13 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const __grid_c
 int64_t chunk_count(int64_t elements) { return ceil_div(elements, kChunkElements); }
 
 // Fills `table` with tensors from `first` on; returns one past the last.
-int64_t fill_table(ClipTable &table, const uint64_t *in, const uint64_t *out, const int64_t *elements,
+template <int kTensors>
+int64_t fill_table(ClipTable<kTensors> &table, const uint64_t *in, const uint64_t *out, const int64_t *elements,
                    const int32_t *dtypes, int64_t first, int64_t count) {
     uint32_t chunk = 0;
     int n = 0;
     int64_t i = first;
-    for (; i < count && n < kMaxTensors; ++i) {
+    for (; i < count && n < kTensors; ++i) {
         if (elements[i] == 0) continue;
         const int64_t chunks = chunk_count(elements[i]);
         if (chunk + chunks > int64_t(1) << 31) break;
@@ -220,6 +226,31 @@ int64_t fill_table(ClipTable &table, const uint64_t *in, const uint64_t *out, co
     table.first_chunk[n] = chunk;
     table.count = n;
     return i;
+}
+
+template <int kTensors>
+int clip_all(const uint64_t *gradients, const uint64_t *outputs, const int64_t *elements, const int32_t *dtypes,
+             int64_t count, float max_norm, float *norm, double *partials, cudaStream_t s) {
+    ClipTable<kTensors> table;
+    int64_t done = 0;
+    for (int64_t i = 0; i < count;) {
+        i = fill_table(table, gradients, outputs, elements, dtypes, i, count);
+        const uint32_t n = table.first_chunk[table.count];
+        if (n == 0) continue;
+        const uint32_t blocks = n < kClipBlocks ? n : kClipBlocks;
+        clip_squares_kernel<<<blocks, kClipThreads, 0, s>>>(table, n, partials + done);
+        KOEMI_LAUNCH_CHECK();
+        done += blocks;
+    }
+    int64_t i = 0;
+    do {
+        i = fill_table(table, gradients, outputs, elements, dtypes, i, outputs == nullptr ? 0 : count);
+        const uint32_t n = table.first_chunk[table.count];
+        const uint32_t blocks = n < 1 ? 1 : n < kClipBlocks ? n : kClipBlocks;
+        clip_scale_kernel<<<blocks, kClipThreads, 0, s>>>(table, n, partials, done, max_norm, norm);
+        KOEMI_LAUNCH_CHECK();
+    } while (outputs != nullptr && i < count);
+    return KOEMI_OK;
 }
 
 }  // namespace
@@ -256,26 +287,7 @@ extern "C" int koemi_core_clip_gradients(const uint64_t *gradients, const uint64
     if (workspace == nullptr || workspace_bytes < koemi_core_clip_gradients_workspace(elements, count)) {
         return fail(KOEMI_ERR_WORKSPACE, "the clipping workspace is smaller than koemi_core_clip_gradients_workspace()");
     }
-    cudaStream_t s = as_stream(stream);
     double *partials = static_cast<double *>(workspace);
-    ClipTable table;
-    int64_t done = 0;
-    for (int64_t i = 0; i < count;) {
-        i = fill_table(table, gradients, outputs, elements, dtypes, i, count);
-        const uint32_t n = table.first_chunk[table.count];
-        if (n == 0) continue;
-        const uint32_t blocks = n < kClipBlocks ? n : kClipBlocks;
-        clip_squares_kernel<<<blocks, kClipThreads, 0, s>>>(table, n, partials + done);
-        KOEMI_LAUNCH_CHECK();
-        done += blocks;
-    }
-    int64_t i = 0;
-    do {
-        i = fill_table(table, gradients, outputs, elements, dtypes, i, outputs == nullptr ? 0 : count);
-        const uint32_t n = table.first_chunk[table.count];
-        const uint32_t blocks = n < 1 ? 1 : n < kClipBlocks ? n : kClipBlocks;
-        clip_scale_kernel<<<blocks, kClipThreads, 0, s>>>(table, n, partials, done, max_norm, norm);
-        KOEMI_LAUNCH_CHECK();
-    } while (outputs != nullptr && i < count);
-    return KOEMI_OK;
+    auto go = count <= kFewTensors ? clip_all<kFewTensors> : count <= kSomeTensors ? clip_all<kSomeTensors> : clip_all<kMaxTensors>;
+    return go(gradients, outputs, elements, dtypes, count, max_norm, norm, partials, as_stream(stream));
 }
