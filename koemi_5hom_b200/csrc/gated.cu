@@ -667,10 +667,13 @@ __global__ __launch_bounds__(kTileThreads, kBackwardResident) void gated_backwar
         const int64_t batch = walk.batch(chain), f0 = walk.feature(chain);
         const LaneFeatures<kTma> features(f0, lane, shape.features);
         const int last = (walk.waves - 1) * cluster + rank;
-        const int64_t first_row = batch * shape.length + int64_t(last) * kSegment + block * kRows;
-        const T *in = projections + first_row * 2 * shape.features + features.x;
-        const T *grad_in = grad_states + first_row * shape.features + features.x;
-        T *grad_out = grad_projections + first_row * 2 * shape.features + features.x;
+        const int64_t first_row = batch * shape.length + int64_t(last) * kSegment;
+        const T *in = projections + first_row * 2 * shape.features;
+        const T *grad_in = grad_states + first_row * shape.features;
+        T *grad_out = grad_projections + first_row * 2 * shape.features;
+        const uint32_t width = static_cast<uint32_t>(shape.features);
+        const uint32_t two_at = block * kRows * 2 * width + static_cast<uint32_t>(features.x);
+        const uint32_t one_at = block * kRows * width + static_cast<uint32_t>(features.x);
         const int64_t walked = f0 + walked_feature<kTma>(lane);
         const bool walks = warp == 0, walks_in = walks && walked < shape.features;
         float x = walks_in && grad_final != nullptr ? grad_final[batch * shape.features + walked] : 0.0f;
@@ -687,7 +690,7 @@ __global__ __launch_bounds__(kTileThreads, kBackwardResident) void gated_backwar
             const T *box = memory.stages + stage * 3 * Memory::kBox + block * kRows * kTileFeatures + 2 * (lane & 15);
             auto load_grad = [&](int j) {
                 if (!have_grad) return both(0.0f);
-                return kTma ? load_two(box + 2 * Memory::kBox + j * kTileFeatures) : features.load(grad_in + j * shape.features);
+                return kTma ? load_two(box + 2 * Memory::kBox + j * kTileFeatures) : features.load(grad_in + (one_at + j * width));
             };
 
             float2 a[kRows], k[kRows], u[kRows];  // u: (hi - lo) s (1 - s), then times h' - k
@@ -698,8 +701,8 @@ __global__ __launch_bounds__(kTileThreads, kBackwardResident) void gated_backwar
                     p = load_clamped<true>(box + j * kTileFeatures);
                     c = load_clamped<false>(box + Memory::kBox + j * kTileFeatures);
                 } else {
-                    p = clamped<true>(features.load(in + j * 2 * shape.features));
-                    c = clamped<false>(features.load(in + j * 2 * shape.features + shape.features));
+                    p = clamped<true>(features.load(in + (two_at + j * 2 * width)));
+                    c = clamped<false>(features.load(in + (two_at + j * 2 * width + width)));
                 }
                 gates_of<T>(p, c, s, k[j]);
                 a[j] = fma2(span, s, lo);
@@ -772,27 +775,45 @@ __global__ __launch_bounds__(kTileThreads, kBackwardResident) void gated_backwar
 
             float2 h = *reinterpret_cast<const float2 *>(memory.starts + at);
             float2 from = *reinterpret_cast<const float2 *>(memory.starts + Memory::kPlane + at);
-#pragma unroll
-            for (int j = 0; j < kRows; ++j) {
-                if (!flags.plain && (flags.cut >> j & 1u)) h = both(0.0f);
+            auto state_through = [&](int j) {  // u times h' - k, and the state behind row j
                 const float2 gap = sub2(h, k[j]);
                 u[j] = mul2(gap, u[j]);
                 h = fma2(a[j], gap, k[j]);
-            }
-            T *row = grad_out + int64_t(kRows - 1) * 2 * shape.features;
-#pragma unroll
-            for (int j = kRows - 1; j >= 0; --j, row -= 2 * shape.features) {
-                if (!flags.plain && j >= flags.rows_in) continue;
+            };
+            auto gradients = [&](int j, float2 &dp, float2 &dc) {  // of row j, and x in front of it
                 const float2 adjoint = add2(from, load_grad(j));
-                float2 dp = mul2(adjoint, u[j]);
-                float2 dc = mul2(adjoint, mul2(sub2(both(1.0f), a[j]), sub2(both(1.0f), mul2(k[j], k[j]))));
+                dp = mul2(adjoint, u[j]);
+                dc = mul2(adjoint, mul2(sub2(both(1.0f), a[j]), sub2(both(1.0f), mul2(k[j], k[j]))));
                 from = mul2(a[j], adjoint);
-                if (!flags.plain) {
+            };
+            if (flags.plain) {
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) state_through(j);
+                T *row = grad_out + (two_at + (kRows - 1) * 2 * width);
+#pragma unroll
+                for (int j = kRows - 1; j >= 0; --j) {
+                    float2 dp, dc;
+                    gradients(j, dp, dc);
+                    features.store(row + width, dc);
+                    features.store(row, dp);
+                    row -= 2 * shape.features;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) {
+                    if (flags.cut >> j & 1u) h = both(0.0f);
+                    state_through(j);
+                }
+#pragma unroll
+                for (int j = kRows - 1; j >= 0; --j) {
+                    if (j >= flags.rows_in) continue;
+                    float2 dp, dc;
+                    gradients(j, dp, dc);
                     if (!(flags.live >> j & 1u)) dp = dc = both(0.0f);
                     if (flags.cut >> j & 1u) from = both(0.0f);
+                    features.store(grad_out + (two_at + j * 2 * width), dp);
+                    features.store(grad_out + (two_at + j * 2 * width + width), dc);
                 }
-                features.store(row, dp);
-                features.store(row + shape.features, dc);
             }
             in -= int64_t(cluster) * kSegment * 2 * shape.features;
             grad_in -= int64_t(cluster) * kSegment * shape.features;
@@ -929,8 +950,9 @@ int check_gated(const GatedShape &shape) {
     if (!(shape.lo > 0.0f && shape.lo <= shape.hi && shape.hi < 1.0f)) {
         return fail(KOEMI_ERR_INVALID, "retention bounds must satisfy 0 < minimum <= maximum < 1");
     }
-    constexpr int64_t kMost = int64_t(1) << 30;
-    if (shape.batch > kMost || shape.length > kMost || shape.features > kMost ||
+    // a tile's places are counted in 32 bits: 128 rows of 2 F elements
+    constexpr int64_t kMost = int64_t(1) << 30, kWidest = int64_t(1) << 22;
+    if (shape.batch > kMost || shape.length > kMost || shape.features > kWidest ||
         (shape.features > 0 && shape.batch > (int64_t(1) << 36) / shape.features)) {
         return fail(KOEMI_ERR_INVALID, "recurrence tensor is too large");
     }
