@@ -163,7 +163,7 @@ class KoemiNativeError(RuntimeError):
 _LOCK = threading.RLock()
 _LIBRARY: ctypes.CDLL | None = None
 _INITIALISED_DEVICES: set[int] = set()
-_BINDING: ctypes.CDLL | None = None
+_BINDING: ctypes.PyDLL | None = None
 
 
 def library() -> ctypes.CDLL:
@@ -200,8 +200,9 @@ def library() -> ctypes.CDLL:
     return _LIBRARY
 
 
-def binding() -> ctypes.CDLL:
-    """Load (once) the torch binding, which registers the training ops, and open the kernel library in it."""
+def binding() -> ctypes.PyDLL:
+    """Load (once) the torch binding, which registers the training ops, and open the kernel library in it.
+    Its functions take and return Python objects, so they are called with the interpreter held."""
     global _BINDING
     if _BINDING is not None:
         return _BINDING
@@ -214,7 +215,7 @@ def binding() -> ctypes.CDLL:
                 f"{BINDING_PATH} is missing; build it with `python -m koemi_5hom_b200.build`"
             )
         try:
-            ops = ctypes.CDLL(str(BINDING_PATH))
+            ops = ctypes.PyDLL(str(BINDING_PATH))
         except OSError as error:
             raise KoemiNativeUnavailableError(f"cannot load {BINDING_PATH}: {error}") from error
         ops.koemi_torch_open.restype = ctypes.c_char_p
@@ -222,6 +223,8 @@ def binding() -> ctypes.CDLL:
         message = ops.koemi_torch_open(str(handle._name).encode())
         if message is not None:
             raise KoemiNativeUnavailableError(message.decode("utf-8", errors="replace"))
+        ops.koemi_torch_clip_gradients.restype = ctypes.py_object
+        ops.koemi_torch_clip_gradients.argtypes = [ctypes.py_object, ctypes.py_object, ctypes.c_double]
         _BINDING = ops
     return _BINDING
 

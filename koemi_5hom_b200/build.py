@@ -20,6 +20,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -90,8 +91,8 @@ def build_binding(verbose: bool = False) -> Path:
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                "-I", str(INCLUDE_DIR), "-isystem", str(root / "include"),
                "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
-               "-isystem", str(cuda / "include"), str(BINDING_SOURCE), "-o", str(temporary),
-               "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl"]
+               "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_path("include"), str(BINDING_SOURCE), "-o", str(temporary),
+               "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python", "-ldl"]
     if verbose:
         print(" ".join(command), flush=True)
     result = subprocess.run(command, capture_output=True, text=True)

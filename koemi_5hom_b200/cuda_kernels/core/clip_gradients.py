@@ -11,6 +11,7 @@ from typing import Iterable, Sequence
 import torch
 from torch import Tensor
 
+from koemi_5hom_b200 import _native
 from koemi_5hom_b200.cuda_kernels import _training
 from koemi_5hom_b200.cuda_kernels.loader import CudaExtensionValidationError, load_cuda_extension
 
@@ -32,27 +33,26 @@ def clip_gradients(gradients: Iterable[Tensor], max_norm: float, *, out: Sequenc
     gradients = list(gradients)
     if isinstance(max_norm, bool) or not isinstance(max_norm, (int, float)) or not max_norm >= 0.0:
         raise CudaExtensionValidationError("max_norm must be a non-negative number")
-    if out is None:
-        return _call("clip_gradients_", (gradients,), float(max_norm))
-    return _call("clip_gradients_out", (gradients, list(out)), float(max_norm))
+    return _call(gradients, gradients if out is None else list(out), float(max_norm))
 
 
 def gradient_norm(gradients: Iterable[Tensor]) -> Tensor:
     """The 2-norm over all tensors, an fp32 scalar on their device (see :func:`clip_gradients`)."""
-    return _call("gradient_norm", (list(gradients),))
+    return _call(list(gradients), None, 0.0)
 
 
-def _call(name: str, lists: tuple[list, ...], *options) -> Tensor:
-    """Run the op, which checks the tensors as it collects their addresses (a
-    list of hundreds costs microseconds there); what it refuses is explained here."""
-    first = lists[0][0] if lists[0] else None
+def _call(gradients: list, out: list | None, max_norm: float) -> Tensor:
+    """The binding checks the tensors as it collects their addresses (a list of
+    hundreds costs microseconds there); what it refuses is explained here."""
+    lists = (gradients,) if out is None else (gradients, out)
+    first = gradients[0] if gradients else None
     if not isinstance(first, Tensor) or not first.is_cuda:
         _explain(lists)
     if not _training._loaded:
         load_cuda_extension(device=first.device)
     _training.load(first.device)
     try:
-        return getattr(torch.ops.koemi_b200, name).default(*lists, *options)
+        return _native.binding().koemi_torch_clip_gradients(gradients, out, max_norm)
     except (ValueError, TypeError, RuntimeError):
         _explain(lists)
         raise
