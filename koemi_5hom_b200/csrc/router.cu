@@ -37,6 +37,18 @@ struct RouteShape {
 
 __device__ __forceinline__ float selectable(float v) { return isnan(v) ? -INFINITY : v; }
 
+// Where the results over all rows go.
+struct RouteTotals {
+    int64_t *counts;
+    float *balance, *slope;
+};
+// d balance / d probability of any row: E counts_e / (N sum counts), all rows
+// that take part having top_k pairs.
+__device__ __forceinline__ float balance_slope(int64_t experts, int64_t top_k, int64_t live, int64_t count) {
+    const float n = static_cast<float>(live > 0 ? live : 1);
+    return static_cast<float>(experts) / n / (n * static_cast<float>(top_k)) * static_cast<float>(count);
+}
+
 struct RowSoftmax {
     float max, sum;
     bool live;
@@ -167,8 +179,7 @@ __global__ __launch_bounds__(kFinishThreads) void route_finish_kernel(
                 mass += masses[i * width + column];
                 count += pairs[i * width + column];
             }
-            const float n = static_cast<float>(all > 0 ? all : 1);
-            const float s = static_cast<float>(experts) / n / (n * static_cast<float>(top_k)) * static_cast<float>(count);
+            const float s = balance_slope(experts, top_k, all, count);
             counts[e] = count;
             slope[e] = s;
             total += static_cast<float>(mass) * s;
@@ -243,7 +254,8 @@ __device__ __forceinline__ RowSoftmax load_row(const T *row, int experts, int at
 template <typename T, int kLanes, int kPer>
 __global__ __launch_bounds__(kRouteWarps * 32, 2) void route_forward_kernel(
     RouteShape shape, const T *__restrict__ logits, int64_t *__restrict__ ids, float *__restrict__ weights,
-    float *__restrict__ partial_mass, int32_t *__restrict__ partial_counts, int32_t *__restrict__ partial_live) {
+    float *__restrict__ partial_mass, int32_t *__restrict__ partial_counts, int32_t *__restrict__ partial_live,
+    RouteTotals totals) {
     constexpr int kGroups = kRouteWarps * 32 / kLanes, kWidth = kLanes * kPer;
     __shared__ float mass[kRouteWarps][kWidth];
     __shared__ int32_t counts[kWidth];
@@ -320,14 +332,33 @@ __global__ __launch_bounds__(kRouteWarps * 32, 2) void route_forward_kernel(
     }
     if (live > 0) atomicAdd(&live_rows, live);
     __syncthreads();
+    float total = 0.0f;
     for (int e = threadIdx.x; e < experts; e += blockDim.x) {
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kRouteWarps; ++w) sum += mass[w][e];
-        partial_mass[int64_t(blockIdx.x) * experts + e] = sum;
-        partial_counts[int64_t(blockIdx.x) * experts + e] = counts[e];
+        if (gridDim.x > 1) {
+            partial_mass[int64_t(blockIdx.x) * experts + e] = sum;
+            partial_counts[int64_t(blockIdx.x) * experts + e] = counts[e];
+        } else {  // all rows are this CTA's: no second kernel
+            const float slope = balance_slope(experts, top_k, live_rows, counts[e]);
+            totals.counts[e] = counts[e];
+            totals.slope[e] = slope;
+            total = fmaf(sum, slope, total);
+        }
     }
-    if (threadIdx.x == 0) partial_live[blockIdx.x] = live_rows;
+    if (gridDim.x > 1) {
+        if (threadIdx.x == 0) partial_live[blockIdx.x] = live_rows;
+        return;
+    }
+    __shared__ float sums[kRouteWarps];
+    total = warp_sum(total);
+    if (threadIdx.x % 32 == 0) sums[warp] = total;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kRouteWarps; ++w) total += sums[w];
+        *totals.balance = total;
+    }
 }
 
 template <typename T, int kLanes, int kPer>
@@ -437,8 +468,14 @@ __global__ void route_backward_wide_kernel(RouteShape shape, const T *__restrict
 int rows_per_turn(int64_t experts) {
     return experts <= 32 ? kRouteWarps * 4 : experts <= 64 ? kRouteWarps * 2 : experts <= 256 ? kRouteWarps : kWideWarps;
 }
+// Up to kSoloTurns turns one CTA takes all rows, and finishes: a launch less. A
+// turn takes 1.5 us, as much as the second launch; 8 turns (256 tokens of 64
+// experts) were faster for a host that launches one call after the other, 16.4
+// for 18.9 us, and slower on the device, 14.6 for 7.0 us, which counts in a graph.
+constexpr int64_t kSoloTurns = 2;
 int64_t route_blocks(int64_t tokens, int64_t experts) {
     const int64_t blocks = ceil_div(tokens, rows_per_turn(experts));
+    if (experts <= 256 && blocks <= kSoloTurns) return 1;
     return blocks < kRouteBlocks ? (blocks > 0 ? blocks : 1) : kRouteBlocks;
 }
 
@@ -472,7 +509,7 @@ int route_forward(const RouteShape &shape, const void *logits, int64_t *ids, flo
     const unsigned grid = static_cast<unsigned>(blocks);
     const bool narrow = with_layout(shape.experts, [&](auto lanes, auto per) {
         route_forward_kernel<T, lanes.value, per.value><<<grid, kRouteWarps * 32, 0, stream>>>(
-            shape, in, ids, weights, mass, partial_counts, live);
+            shape, in, ids, weights, mass, partial_counts, live, RouteTotals{counts, balance, slope});
     });
     if (!narrow) {
         const size_t smem = (kWideWarps + 1) * shape.experts * sizeof(float);
@@ -481,6 +518,7 @@ int route_forward(const RouteShape &shape, const void *logits, int64_t *ids, flo
         kernel<<<grid, kWideWarps * 32, smem, stream>>>(shape, in, ids, weights, mass, partial_counts, live);
     }
     KOEMI_LAUNCH_CHECK();
+    if (narrow && blocks == 1) return KOEMI_OK;
     route_finish_kernel<<<1, kFinishThreads, 0, stream>>>(mass, partial_counts, live, static_cast<int>(blocks),
                                                           static_cast<int>(shape.experts), shape.top_k, counts, balance,
                                                           slope);
@@ -494,7 +532,9 @@ int route_backward(const RouteShape &shape, const void *logits, const int64_t *i
                    cudaStream_t stream) {
     const T *in = static_cast<const T *>(logits);
     T *out = static_cast<T *>(grad_logits);
-    const unsigned grid = static_cast<unsigned>(route_blocks(shape.tokens, shape.experts));
+    // enough CTAs for a turn each, up to two per SM
+    const int64_t turns = ceil_div(shape.tokens, rows_per_turn(shape.experts));
+    const unsigned grid = static_cast<unsigned>(turns < kRouteBlocks ? turns : kRouteBlocks);
     const bool narrow = with_layout(shape.experts, [&](auto lanes, auto per) {
         route_backward_kernel<T, lanes.value, per.value><<<grid, kRouteWarps * 32, 0, stream>>>(
             shape, in, ids, weights, grad_weights, grad_balance, slope, out);
