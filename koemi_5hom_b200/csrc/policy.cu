@@ -138,7 +138,7 @@ __device__ __forceinline__ float lse_of(Partial p) { return p.max + logf(p.sum);
 struct PolicyOut {
     const float *inverse;  // NULL: the CTA counts the valid rows
     float *log_probs, *lse, *slopes;
-    float2 *partials;
+    double2 *partials;
 };
 
 // A row's scalars, loaded ahead of its logits, and what follows from its
@@ -156,6 +156,8 @@ struct RowScalars {
         advantage = terms.advantages[index];
         reference = terms.reference != nullptr ? terms.reference[index] : 0.0f;
     }
+    // from the maximum, not from the log-sum-exp, which rounds at its own magnitude
+    __device__ __forceinline__ float log_prob(Partial p) const { return (chosen - p.max) - logf(p.sum); }
     // d loss / d log-prob, of a row alone
     __device__ __forceinline__ float slope(const PolicyTerms &terms, float lp) const {
         const float r = exp_from(lp, old), free = r * advantage;
@@ -164,19 +166,19 @@ struct RowScalars {
         if (terms.reference != nullptr) s += terms.beta * (1.0f - exp_from(reference, lp));
         return isnan(free) || isnan(clipped) ? NAN : s;
     }
-    __device__ void add_loss(const PolicyTerms &terms, float lp, float &loss, float &kl) const {
+    __device__ void add_loss(const PolicyTerms &terms, float lp, double &loss, double &kl) const {
         const float r = expf(lp - old), free = r * advantage;
         const float clipped = fminf(fmaxf(r, 1.0f - terms.clip_low), 1.0f + terms.clip_high) * advantage;
         loss -= isnan(free) || isnan(clipped) ? NAN : fminf(free, clipped);
         if (terms.reference != nullptr) {
             const float d = reference - lp, k = expm1f(d) - d;
             kl += k;
-            loss = fmaf(terms.beta, k, loss);
+            loss += terms.beta * k;
         }
     }
     // the row's results, by one thread
     __device__ void finish(const PolicyTerms &terms, const PolicyOut &out, int64_t index, float lp, float lse,
-                           float scaled_slope, float &loss, float &kl) const {
+                           float scaled_slope, double &loss, double &kl) const {
         add_loss(terms, lp, loss, kl);
         out.log_probs[index] = lp;
         out.lse[index] = lse;
@@ -189,10 +191,10 @@ template <typename T, int kPer>
 __global__ __launch_bounds__(256) void policy_warp_kernel(PolicyRows shape, PolicyTerms terms,
                                                           const T *__restrict__ logits, PolicyOut result,
                                                           T *__restrict__ grad_logits) {
-    __shared__ float2 sums[8];
+    __shared__ double2 sums[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, vocab = static_cast<int>(shape.vocab);
     const float scale = result.inverse != nullptr ? *result.inverse : inverse_count(terms.valid, shape.rows);
-    float loss_sum = 0.0f, kl_sum = 0.0f;
+    double loss_sum = 0.0, kl_sum = 0.0;  // advantages cancel: fp32 sums would lose what is left
     for (int64_t row = int64_t(blockIdx.x) * 8 + warp; row < shape.rows; row += int64_t(gridDim.x) * 8) {
         T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
         if (terms.valid != nullptr && terms.valid[row] == 0) {
@@ -219,7 +221,7 @@ __global__ __launch_bounds__(256) void policy_warp_kernel(PolicyRows shape, Poli
             p.sum += e[j];
         }
         p.sum = warp_sum(p.sum);
-        const float lse = lse_of(p), lp = scalars.chosen - lse, slope = scalars.slope(terms, lp) * scale;
+        const float lse = lse_of(p), lp = scalars.log_prob(p), slope = scalars.slope(terms, lp) * scale;
         if (lane == 0) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
         if (out != nullptr) {
             const float factor = -slope / p.sum;
@@ -230,14 +232,14 @@ __global__ __launch_bounds__(256) void policy_warp_kernel(PolicyRows shape, Poli
             }
         }
     }
-    if (lane == 0) sums[warp] = make_float2(loss_sum, kl_sum);
+    if (lane == 0) sums[warp] = make_double2(loss_sum, kl_sum);
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 8; ++w) {
             loss_sum += sums[w].x;
             kl_sum += sums[w].y;
         }
-        result.partials[blockIdx.x] = make_float2(loss_sum, kl_sum);
+        result.partials[blockIdx.x] = make_double2(loss_sum, kl_sum);
     }
 }
 
@@ -378,7 +380,7 @@ __global__ __launch_bounds__(kThreads, 1024 / kThreads) void policy_row_kernel(
         for (int b = 0; b < buffers; ++b) load_next();
     }
     const float scale = result.inverse != nullptr ? *result.inverse : inverse_count(terms.valid, shape.rows);
-    float loss_sum = 0.0f, kl_sum = 0.0f;
+    double loss_sum = 0.0, kl_sum = 0.0;  // advantages cancel: fp32 sums would lose what is left
     bool dead = false;  // a copy never arrived: go on without waiting or loading
     int taken = 0;
     for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
@@ -434,7 +436,7 @@ __global__ __launch_bounds__(kThreads, 1024 / kThreads) void policy_row_kernel(
         if (threadIdx.x == 0 && !dead) load_next();
         ++taken;
 
-        const float lse = lse_of(all), lp = scalars.chosen - lse, slope = scalars.slope(terms, lp) * scale;
+        const float lse = lse_of(all), lp = scalars.log_prob(all), slope = scalars.slope(terms, lp) * scale;
         if (threadIdx.x == kThreads - 1) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
         if (out != nullptr) {
             // of an fp32 warp with nothing but -inf: 0
@@ -467,7 +469,7 @@ __global__ __launch_bounds__(kThreads, 1024 / kThreads) void policy_row_kernel(
             }
         }
     }
-    if (threadIdx.x == kThreads - 1) result.partials[blockIdx.x] = make_float2(loss_sum, kl_sum);
+    if (threadIdx.x == kThreads - 1) result.partials[blockIdx.x] = make_double2(loss_sum, kl_sum);
 }
 
 // Longer rows, in blocks of 1024 threads x 32 entries, walked twice.
@@ -480,7 +482,7 @@ __global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows sh
     __shared__ Partial merged[2][32];
     const int vocab = static_cast<int>(shape.vocab);
     const float scale = result.inverse != nullptr ? *result.inverse : inverse_count(terms.valid, shape.rows);
-    float loss_sum = 0.0f, kl_sum = 0.0f;
+    double loss_sum = 0.0, kl_sum = 0.0;  // advantages cancel: fp32 sums would lose what is left
     int taken = 0;
     for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
         T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
@@ -526,7 +528,7 @@ __global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows sh
             for (int i = 0; i < kWidth; ++i) p.sum += exp_from(v[i], from);
         });
         const Partial all = block_merge<kWalkThreads>(warp_merge(p), merged, taken++ & 1);
-        const float lse = lse_of(all), lp = scalars.chosen - lse, slope = scalars.slope(terms, lp) * scale;
+        const float lse = lse_of(all), lp = scalars.log_prob(all), slope = scalars.slope(terms, lp) * scale;
         if (threadIdx.x == 0) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
         if (out != nullptr) {
             const float factor = -slope / all.sum;
@@ -543,11 +545,11 @@ __global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows sh
             });
         }
     }
-    if (threadIdx.x == 0) result.partials[blockIdx.x] = make_float2(loss_sum, kl_sum);
+    if (threadIdx.x == 0) result.partials[blockIdx.x] = make_double2(loss_sum, kl_sum);
 }
 
 constexpr int kFinishThreads = 256;
-__global__ __launch_bounds__(kFinishThreads) void policy_finish_kernel(const float2 *__restrict__ partials, int count,
+__global__ __launch_bounds__(kFinishThreads) void policy_finish_kernel(const double2 *__restrict__ partials, int count,
                                                                        const float *__restrict__ inverse,
                                                                        const uint8_t *__restrict__ valid, int64_t rows,
                                                                        float *__restrict__ loss, float *__restrict__ kl) {
@@ -695,7 +697,7 @@ int policy_forward(const PolicyRows &shape, const PolicyTerms &terms, const void
                    float *log_probs, float *lse, float *slopes, void *grad_logits, void *workspace,
                    cudaStream_t stream) {
     float *inverse = static_cast<float *>(workspace);
-    PolicyOut result{nullptr, log_probs, lse, slopes, reinterpret_cast<float2 *>(static_cast<unsigned char *>(workspace) + 256)};
+    PolicyOut result{nullptr, log_probs, lse, slopes, reinterpret_cast<double2 *>(static_cast<unsigned char *>(workspace) + 256)};
     const T *in = static_cast<const T *>(logits);
     T *grad = static_cast<T *>(grad_logits);
     unsigned blocks = 0;
@@ -762,7 +764,7 @@ int policy_scale(void *grad, int64_t count, const float *factor, cudaStream_t st
 
 using namespace koemi;
 
-extern "C" size_t koemi_think_policy_loss_workspace(void) { return 256 + kPolicyBlocks * sizeof(float2); }
+extern "C" size_t koemi_think_policy_loss_workspace(void) { return 256 + kPolicyBlocks * sizeof(double2); }
 
 extern "C" int koemi_think_policy_loss_forward(const void *logits, int64_t rows, int64_t vocab, int64_t inner_rows,
                                                int64_t outer_stride, int64_t inner_stride, const int64_t *targets,
@@ -781,6 +783,7 @@ extern "C" int koemi_think_policy_loss_forward(const void *logits, int64_t rows,
                       log_probs == nullptr || lse == nullptr || slopes == nullptr))) {
         return fail(KOEMI_ERR_INVALID, "policy loss tensors and workspace must be non-NULL");
     }
+    if (!aligned(grad_logits, 16)) return fail(KOEMI_ERR_INVALID, "grad_logits must be 16-byte aligned");
     if (workspace_bytes < koemi_think_policy_loss_workspace()) {
         return fail(KOEMI_ERR_WORKSPACE, "the policy loss's workspace is smaller than koemi_think_policy_loss_workspace()");
     }
@@ -807,6 +810,7 @@ extern "C" int koemi_think_policy_loss_backward(const void *logits, int64_t rows
         grad_logits == nullptr) {
         return fail(KOEMI_ERR_INVALID, "policy loss backward tensors must be non-NULL");
     }
+    if (!aligned(grad_logits, 16)) return fail(KOEMI_ERR_INVALID, "grad_logits must be 16-byte aligned");
     cudaStream_t s = as_stream(stream);
     switch (dtype) {
         case KOEMI_F32: return policy_backward<float>(shape, logits, targets, valid, lse, slopes, grad_loss, grad_logits, s);
@@ -822,6 +826,7 @@ extern "C" int koemi_think_policy_loss_scale(void *grad_logits, int64_t count, c
     if (count < 0) return fail(KOEMI_ERR_INVALID, "count must be non-negative");
     if (count == 0) return KOEMI_OK;
     if (grad_logits == nullptr || factor == nullptr) return fail(KOEMI_ERR_INVALID, "grad_logits and factor must be non-NULL");
+    if (!aligned(grad_logits, 16)) return fail(KOEMI_ERR_INVALID, "grad_logits must be 16-byte aligned");
     cudaStream_t s = as_stream(stream);
     switch (dtype) {
         case KOEMI_F32: return policy_scale<float>(grad_logits, count, factor, s);

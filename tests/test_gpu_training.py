@@ -90,6 +90,26 @@ def test_recurrence_and_gradients_match_the_plain_form(shape, dtype, masks, cuda
     check(got_h, want_h, torch.float32, 16 * EPS * amplify * adjoint)
 
 
+@pytest.mark.parametrize("masks", [False, True])
+@pytest.mark.parametrize("shape", [(300, 130, 520), (320, 300, 264), (700, 20, 328)])
+def test_recurrence_of_more_chains_than_the_gpu_holds(shape, masks, cuda):
+    """Several chains walked by one CTA, one after the other."""
+    x, h0, valid, restart, gs, gf = recurrence_case(*shape, torch.bfloat16, 17, masks, cuda)
+    xg, hg = x.clone().requires_grad_(True), h0.clone().requires_grad_(True)
+    states, final = gated_recurrence(xg, hg, valid=valid, restart=restart)
+    got_x, got_h = torch.autograd.grad((states, final), (xg, hg), (gs, gf))
+    amplify, most = recurrence_bounds(x, h0)
+    adjoint = amplify * gs.abs().max().item() + gf.abs().max().item()
+    for rows in (slice(0, 8), slice(shape[0] // 2, shape[0] // 2 + 8), slice(shape[0] - 8, shape[0])):
+        x64, h64 = x[rows].double().requires_grad_(True), h0[rows].double().requires_grad_(True)
+        expected, expected_final = plain.gated_recurrence(x64, h64, *(None if m is None else m[rows] for m in (valid, restart)))
+        check(states[rows].detach(), expected.detach(), torch.bfloat16, 16 * EPS * amplify * most)
+        check(final[rows].detach(), expected_final.detach(), torch.float32, 16 * EPS * amplify * most)
+        want_x, want_h = torch.autograd.grad((expected, expected_final), (x64, h64), (gs[rows].double(), gf[rows].double()))
+        check(got_x[rows], want_x, torch.bfloat16, 32 * EPS * amplify * adjoint * most)
+        check(got_h[rows], want_h, torch.float32, 16 * EPS * amplify * adjoint)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_recurrence_carried_over_pieces_equals_one_call(dtype, cuda):
     x, h0, *_ = recurrence_case(2, 200, 48, dtype, 1, False, cuda)
