@@ -7,7 +7,8 @@
 // and ctypes calls (kernels: 10 us), of which 50 us are autograd's own.
 // The clipping of gradients is called directly with its Python lists: through
 // the dispatcher, which copies a list of tensors twice, 2 x 144 tensors took 48
-// us where the kernels take 10.
+// us where the kernels take 10. The autograd nodes are plain ones, as torch's
+// own ops have, with what the backward needs in fields.
 // Nothing here computes: every op checks what the kernels rely on, allocates
 // from the caching allocator and calls one entry point on the current stream.
 #include <Python.h>
@@ -16,8 +17,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include <mutex>
@@ -30,7 +33,7 @@
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 using OptionalTensor = std::optional<Tensor>;
 
@@ -105,6 +108,14 @@ OptionalTensor dense(const Tensor &t) { return t.defined() ? OptionalTensor(t.co
 bool differentiates(const Tensor &t) { return t.defined() && t.requires_grad(); }
 bool differentiates(const OptionalTensor &t) { return t.has_value() && differentiates(*t); }
 
+// A node whose gradients go to `inputs`, in their order.
+template <typename NodeType, typename... Inputs>
+std::shared_ptr<NodeType> node_of(const Inputs &...inputs) {
+    std::shared_ptr<NodeType> node(new NodeType(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+    return node;
+}
+
 void first_order_only() {
     TORCH_CHECK(!at::GradMode::is_enabled(), "the training operators are differentiable to first order only (create_graph=True)");
 }
@@ -161,40 +172,49 @@ std::tuple<Tensor, Tensor> gated_recurrence_backward_cuda(const Tensor &projecti
 #define KOEMI_OP(name, signature) \
     static auto name = c10::Dispatcher::singleton().findSchemaOrThrow("koemi_b200::" #name, "").typed<signature>()
 
-struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
-    static variable_list forward(AutogradContext *context, const Tensor &projections, const OptionalTensor &initial,
-                                 const OptionalTensor &valid, const OptionalTensor &restart, double low, double high) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        KOEMI_OP(gated_recurrence_keep, decltype(gated_recurrence_keep_cuda));
-        auto [states, final_state, carries] = gated_recurrence_keep.call(projections, initial, valid, restart, low, high);
-        context->save_for_backward({projections, valid.value_or(Tensor()), restart.value_or(Tensor()), carries});
-        context->saved_data["low"] = low;
-        context->saved_data["high"] = high;
-        context->saved_data["initial"] = differentiates(initial);
-        context->set_materialize_grads(false);
-        return {states, final_state};
-    }
-    static variable_list backward(AutogradContext *context, variable_list grads) {
+struct GatedRecurrenceBackward final : torch::autograd::Node {
+    SavedVariable projections, valid, restart, carries;
+    double low = 0, high = 0;
+    variable_list apply(variable_list &&grads) override {
         first_order_only();
-        variable_list result(6);
+        std::lock_guard<std::mutex> lock(mutex_);
+        at::AutoDispatchBelowADInplaceOrView below;
+        variable_list result(2);
         if (!grads[0].defined() && !grads[1].defined()) return result;
-        const auto saved = context->get_saved_variables();
         KOEMI_OP(gated_recurrence_backward, decltype(gated_recurrence_backward_cuda));
-        auto [grad_projections, grad_initial] = gated_recurrence_backward.call(
-            saved[0], given(saved[1]), given(saved[2]), saved[3], dense(grads[0]), dense(grads[1]),
-            context->saved_data["low"].toDouble(), context->saved_data["high"].toDouble());
-        result[0] = grad_projections;
-        if (context->saved_data["initial"].toBool()) result[1] = grad_initial;
+        auto [grad_projections, grad_initial] =
+            gated_recurrence_backward.call(projections.unpack(), given(valid.unpack()), given(restart.unpack()),
+                                           carries.unpack(), dense(grads[0]), dense(grads[1]), low, high);
+        if (task_should_compute_output(0)) result[0] = grad_projections;
+        if (task_should_compute_output(1)) result[1] = grad_initial;
         return result;
     }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *saved : {&projections, &valid, &restart, &carries}) saved->reset_data();
+    }
+    std::string name() const override { return "GatedRecurrenceBackward"; }
 };
 
 std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor &projections, const OptionalTensor &initial,
                                                      const OptionalTensor &valid, const OptionalTensor &restart,
                                                      double low, double high) {
     if (at::GradMode::is_enabled() && (differentiates(projections) || differentiates(initial))) {
-        auto out = GatedRecurrence::apply(projections, initial, valid, restart, low, high);
-        return {out[0], out[1]};
+        auto node = node_of<GatedRecurrenceBackward>(projections, initial);
+        Tensor states, final_state, carries;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            KOEMI_OP(gated_recurrence_keep, decltype(gated_recurrence_keep_cuda));
+            std::tie(states, final_state, carries) = gated_recurrence_keep.call(projections, initial, valid, restart, low, high);
+        }
+        node->projections = SavedVariable(projections, false);
+        node->valid = SavedVariable(valid, false);
+        node->restart = SavedVariable(restart, false);
+        node->carries = SavedVariable(carries, false);
+        node->low = low;
+        node->high = high;
+        torch::autograd::set_history({states, final_state}, node);
+        return {states, final_state};
     }
     at::AutoDispatchBelowADInplaceOrView below;
     KOEMI_OP(gated_recurrence, decltype(gated_recurrence_cuda));
@@ -239,35 +259,44 @@ Tensor route_learned_backward_cuda(const Tensor &logits, const Tensor &ids, cons
     return grad;
 }
 
-struct RouteLearned : torch::autograd::Function<RouteLearned> {
-    static variable_list forward(AutogradContext *context, const Tensor &logits, const OptionalTensor &valid,
-                                 int64_t top_k, bool renormalize) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        KOEMI_OP(route_learned_keep, decltype(route_learned_keep_cuda));
-        auto [ids, weights, counts, balance, slope] = route_learned_keep.call(logits, valid, top_k, renormalize);
-        context->save_for_backward({logits, ids, weights, slope});
-        context->saved_data["renormalize"] = renormalize;
-        context->mark_non_differentiable({ids, counts});
-        context->set_materialize_grads(false);
-        return {ids, weights, counts, balance};
-    }
-    static variable_list backward(AutogradContext *context, variable_list grads) {
+struct RouteLearnedBackward final : torch::autograd::Node {
+    SavedVariable logits, ids, weights, slope;
+    bool renormalize = false;
+    variable_list apply(variable_list &&grads) override {
         first_order_only();
-        variable_list result(4);
-        if (!grads[1].defined() && !grads[3].defined()) return result;
-        const auto saved = context->get_saved_variables();
+        std::lock_guard<std::mutex> lock(mutex_);
+        at::AutoDispatchBelowADInplaceOrView below;
+        variable_list result(1);
+        if (!grads[0].defined() && !grads[1].defined()) return result;
         KOEMI_OP(route_learned_backward, decltype(route_learned_backward_cuda));
-        result[0] = route_learned_backward.call(saved[0], saved[1], saved[2], saved[3], dense(grads[1]), dense(grads[3]),
-                                                context->saved_data["renormalize"].toBool());
+        result[0] = route_learned_backward.call(logits.unpack(), ids.unpack(), weights.unpack(shared_from_this()), slope.unpack(),
+                                                dense(grads[0]), dense(grads[1]), renormalize);
         return result;
     }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *saved : {&logits, &ids, &weights, &slope}) saved->reset_data();
+    }
+    std::string name() const override { return "RouteLearnedBackward"; }
 };
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> route_learned_autograd(const Tensor &logits, const OptionalTensor &valid,
                                                                   int64_t top_k, bool renormalize) {
     if (at::GradMode::is_enabled() && differentiates(logits)) {
-        auto out = RouteLearned::apply(logits, valid, top_k, renormalize);
-        return {out[0], out[1], out[2], out[3]};
+        auto node = node_of<RouteLearnedBackward>(logits);
+        Tensor ids, weights, counts, balance, slope;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            KOEMI_OP(route_learned_keep, decltype(route_learned_keep_cuda));
+            std::tie(ids, weights, counts, balance, slope) = route_learned_keep.call(logits, valid, top_k, renormalize);
+        }
+        node->logits = SavedVariable(logits, false);
+        node->ids = SavedVariable(ids, false);
+        node->slope = SavedVariable(slope, false);
+        node->renormalize = renormalize;
+        torch::autograd::set_history({weights, balance}, node);
+        node->weights = SavedVariable(weights, true);  // an output of the node itself
+        return {ids, weights, counts, balance};
     }
     at::AutoDispatchBelowADInplaceOrView below;
     KOEMI_OP(route_learned, decltype(route_learned_cuda));
@@ -347,40 +376,35 @@ void policy_loss_scale_cuda(const Tensor &gradient, const Tensor &factor) {
                                                               code_of(gradient), launch.stream));
 }
 
-struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
-    static variable_list forward(AutogradContext *context, const Tensor &logits, const Tensor &targets, const Tensor &old,
-                                 const Tensor &advantages, const OptionalTensor &reference, const OptionalTensor &valid,
-                                 double clip_low, double clip_high, double kl_weight) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        KOEMI_OP(policy_loss_keep, decltype(policy_loss_keep_cuda));
-        auto [loss, kl, log_probs, kept, gradient] = policy_loss_keep.call(logits, targets, old, advantages, reference, valid,
-                                                                           clip_low, clip_high, kl_weight);
-        context->save_for_backward({logits, targets, valid.value_or(Tensor()), kept});
-        if (logits.scalar_type() != at::kHalf) context->saved_data["gradient"] = gradient;
-        context->mark_non_differentiable({kl, log_probs});
-        context->set_materialize_grads(false);
-        return {loss, kl, log_probs};
-    }
-    static variable_list backward(AutogradContext *context, variable_list grads) {
+struct PolicyLossBackward final : torch::autograd::Node {
+    SavedVariable logits, targets, valid, kept;
+    Tensor gradient;  // of the forward's pass, until it is handed out
+    variable_list apply(variable_list &&grads) override {
         first_order_only();
-        variable_list result(9);
+        std::lock_guard<std::mutex> lock(mutex_);
+        at::AutoDispatchBelowADInplaceOrView below;
+        variable_list result(1);
         if (!grads[0].defined()) return result;
-        const auto saved = context->get_saved_variables();
         const Tensor factor = grads[0].contiguous();
-        // The gradient of the forward's pass is handed out once; f16, and
-        // another backward through a retained graph, form it from the logits.
-        auto kept = context->saved_data.find("gradient");
-        if (kept != context->saved_data.end()) {
-            result[0] = kept->second.toTensor();
-            context->saved_data.erase(kept);
+        // f16, and another backward through a retained graph, form the gradient from the logits
+        Tensor saved = logits.unpack();
+        if (gradient.defined()) {
+            result[0] = std::move(gradient);
+            gradient = Tensor();
             KOEMI_OP(policy_loss_scale, decltype(policy_loss_scale_cuda));
             policy_loss_scale.call(result[0], factor);
         } else {
             KOEMI_OP(policy_loss_backward, decltype(policy_loss_backward_cuda));
-            result[0] = policy_loss_backward.call(saved[0], saved[1], given(saved[2]), saved[3], factor);
+            result[0] = policy_loss_backward.call(saved, targets.unpack(), given(valid.unpack()), kept.unpack(), factor);
         }
         return result;
     }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *saved : {&logits, &targets, &valid, &kept}) saved->reset_data();
+        gradient = Tensor();
+    }
+    std::string name() const override { return "PolicyLossBackward"; }
 };
 
 std::tuple<Tensor, Tensor, Tensor> policy_loss_autograd(const Tensor &logits, const Tensor &targets, const Tensor &old,
@@ -388,8 +412,21 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_autograd(const Tensor &logits, co
                                                         const OptionalTensor &valid, double clip_low, double clip_high,
                                                         double kl_weight) {
     if (at::GradMode::is_enabled() && differentiates(logits)) {
-        auto out = PolicyLoss::apply(logits, targets, old, advantages, reference, valid, clip_low, clip_high, kl_weight);
-        return {out[0], out[1], out[2]};
+        auto node = node_of<PolicyLossBackward>(logits);
+        Tensor loss, kl, log_probs, kept, gradient;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            KOEMI_OP(policy_loss_keep, decltype(policy_loss_keep_cuda));
+            std::tie(loss, kl, log_probs, kept, gradient) = policy_loss_keep.call(
+                logits, targets, old, advantages, reference, valid, clip_low, clip_high, kl_weight);
+        }
+        node->logits = SavedVariable(logits, false);
+        node->targets = SavedVariable(targets, false);
+        node->valid = SavedVariable(valid, false);
+        node->kept = SavedVariable(kept, false);
+        if (logits.scalar_type() != at::kHalf) node->gradient = gradient;
+        torch::autograd::set_history(loss, node);
+        return {loss, kl, log_probs};
     }
     at::AutoDispatchBelowADInplaceOrView below;
     KOEMI_OP(policy_loss, decltype(policy_loss_cuda));

@@ -290,6 +290,34 @@ def test_recurrence_in_a_cuda_graph(cuda):
     assert all(torch.equal(a, b) for a, b in zip(captured, expected))
 
 
+def test_recurrence_saved_tensors_are_guarded(cuda):
+    """A changed input, a second backward of a freed graph and a second order are errors, not wrong gradients."""
+    x, h0, *_ = recurrence_case(2, 40, 16, torch.float32, 18, False, cuda)
+    y = x.clone().requires_grad_(True)
+    z = y * 1.0
+    states, _ = gated_recurrence(z, h0)
+    states.sum().backward(retain_graph=True)
+    first = y.grad.clone()
+    y.grad = None
+    states.sum().backward()
+    assert torch.equal(first, y.grad)
+    with pytest.raises(RuntimeError, match="second time"):
+        states.sum().backward()
+    z = y * 1.0
+    states, _ = gated_recurrence(z, h0)
+    with torch.no_grad():
+        z.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        states.sum().backward()
+    with pytest.raises(RuntimeError, match="first order"):
+        torch.autograd.grad(gated_recurrence(y, h0)[0].sum(), y, create_graph=True)
+    states, final = gated_recurrence(y, h0)
+    states *= 2  # an output may be changed in place: nothing of it is kept
+    got, = torch.autograd.grad(states.sum() + final.sum(), y)
+    want, = torch.autograd.grad(2 * gated_recurrence(y, h0)[0].sum() + gated_recurrence(y, h0)[1].sum(), y)
+    check(got, want.double(), torch.float32, 64 * EPS * 256)
+
+
 # ------------------------------------------------------------ the learned route
 
 def route_case(tokens, experts, top_k, dtype, seed, masks, cuda):
