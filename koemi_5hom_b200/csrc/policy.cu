@@ -33,20 +33,18 @@ namespace {
 
 constexpr int kPolicyBlocks = 2368;     // most CTAs of a launch: 16 per SM
 constexpr int kWarpRow = 1024;          // entries a warp holds
-constexpr int kThreadBytes = 128;       // bytes of a row that a thread holds
-template <typename T>
-constexpr int64_t longest_row() {       // entries a CTA of 1024 threads holds
-    return 1024 * kThreadBytes / sizeof(T);
-}
+constexpr int kSmBytes = 128 * 1024;    // of rows, in the registers of an SM
+constexpr int64_t kRowBytes = kSmBytes; // longest row that one CTA holds
 constexpr int64_t kCountedRows = 16384; // up to here every CTA counts the valid rows itself
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Row r of the logits starts at (r / inner) * outer_stride + (r % inner) *
 // inner_stride elements.
 struct PolicyRows {
-    int64_t rows, vocab, inner, outer_stride, inner_stride;
+    int64_t rows, vocab, inner, outer_stride, inner_stride;  // rows up to 2^31, inner up to rows
     __device__ __forceinline__ int64_t start(int64_t row) const {
-        return (row / inner) * outer_stride + (row % inner) * inner_stride;
+        const uint32_t r = static_cast<uint32_t>(row), n = static_cast<uint32_t>(inner), outer = r / n;
+        return outer * outer_stride + (r - outer * n) * inner_stride;
     }
 };
 
@@ -124,12 +122,17 @@ __device__ __forceinline__ float packet_max(const float (&v)[kWidth]) {
 __device__ __forceinline__ float origin(float max) { return max == -INFINITY ? 0.0f : max; }
 __device__ __forceinline__ float exp_from(float v, float from) { return ex2_approx((v - from) * kLog2e); }
 
+__device__ __forceinline__ float redux_max(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
 // A maximum and the sum of e^(entry - it) over a thread's, a warp's, a row's entries.
 struct Partial {
     float max, sum;
 };
 __device__ __forceinline__ Partial warp_merge(Partial p) {
-    const float m = warp_max(p.max);
+    const float m = redux_max(p.max);
     return Partial{m, warp_sum(p.sum * exp_from(p.max, origin(m)))};
 }
 __device__ __forceinline__ float lse_of(Partial p) { return p.max + logf(p.sum); }
@@ -141,21 +144,23 @@ struct PolicyOut {
     double2 *partials;
 };
 
-// A row's scalars, loaded ahead of its logits, and what follows from its
-// log-sum-exp: every thread takes the slope (two ex2.approx), one thread per
-// row the loss and the KL term (expf and expm1f: exp(d) - d - 1 cancels).
-template <typename T>
-struct RowScalars {
-    int target;  // -1 outside the vocabulary
-    float chosen, old, advantage, reference;
-    __device__ __forceinline__ RowScalars(const T *row, const PolicyTerms &terms, int64_t index, int vocab) {
-        const int64_t id = terms.targets[index];
-        target = id >= 0 && id < vocab ? static_cast<int>(id) : -1;
-        chosen = target >= 0 ? to_acc(row[target]) : NAN;
-        old = terms.old[index];
-        advantage = terms.advantages[index];
-        reference = terms.reference != nullptr ? terms.reference[index] : 0.0f;
-    }
+// A row's scalars, and what follows from its log-sum-exp: every thread takes
+// the slope (two ex2.approx), one thread per row the loss and the KL term
+// (expf and expm1f: exp(d) - d - 1 cancels).
+struct __align__(16) RowTerms {
+    int target;  // -1 outside the vocabulary, -2 in a row that is not valid
+    float old, advantage, reference;
+    __device__ __forceinline__ bool valid() const { return target != -2; }
+};
+__device__ __forceinline__ RowTerms load_terms(const PolicyTerms &terms, int64_t index, int vocab) {
+    if (terms.valid != nullptr && terms.valid[index] == 0) return RowTerms{-2, 0.0f, 0.0f, 0.0f};
+    const int64_t id = terms.targets[index];
+    return RowTerms{id >= 0 && id < vocab ? static_cast<int>(id) : -1, terms.old[index], terms.advantages[index],
+                    terms.reference != nullptr ? terms.reference[index] : 0.0f};
+}
+struct RowScalars : RowTerms {
+    float chosen;  // the target's logit
+    __device__ __forceinline__ RowScalars(const RowTerms &row, float logit) : RowTerms(row), chosen(target >= 0 ? logit : NAN) {}
     // from the maximum, not from the log-sum-exp, which rounds at its own magnitude
     __device__ __forceinline__ float log_prob(Partial p) const { return (chosen - p.max) - logf(p.sum); }
     // d loss / d log-prob, of a row alone
@@ -197,7 +202,8 @@ __global__ __launch_bounds__(256) void policy_warp_kernel(PolicyRows shape, Poli
     double loss_sum = 0.0, kl_sum = 0.0;  // advantages cancel: fp32 sums would lose what is left
     for (int64_t row = int64_t(blockIdx.x) * 8 + warp; row < shape.rows; row += int64_t(gridDim.x) * 8) {
         T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
-        if (terms.valid != nullptr && terms.valid[row] == 0) {
+        const RowTerms row_terms = load_terms(terms, row, vocab);
+        if (!row_terms.valid()) {
             if (out != nullptr) {
                 for (int v = lane; v < vocab; v += 32) out[v] = from_acc<T>(0.0f);
             }
@@ -205,7 +211,7 @@ __global__ __launch_bounds__(256) void policy_warp_kernel(PolicyRows shape, Poli
             continue;
         }
         const T *in = logits + shape.start(row);
-        const RowScalars<T> scalars(in, terms, row, vocab);
+        const RowScalars scalars(row_terms, row_terms.target >= 0 ? to_acc(in[row_terms.target]) : NAN);
         float e[kPer];
         Partial p{-INFINITY, 0.0f};
 #pragma unroll
@@ -259,6 +265,11 @@ struct Packets {
         end = (skip + vocab) / kWidth;
     }
     __device__ __forceinline__ bool whole(int c) const { return c >= first && c < end; }
+    // packet c lies inside the tensor that ends before `tensor_end`
+    __device__ __forceinline__ bool inside(int c, const T *tensor, const T *tensor_end) const {
+        const T *packet = base + int64_t(c) * kWidth;
+        return packet >= tensor && packet + kWidth <= tensor_end;
+    }
     __device__ __forceinline__ bool in_row(int c, int i) const {
         return static_cast<unsigned>(c * kWidth + i - skip) < static_cast<unsigned>(vocab);
     }
@@ -346,78 +357,154 @@ __device__ __forceinline__ float2 exp_from(float2 v, float from) {
     return make_float2(ex2_approx(v.x), ex2_approx(v.y));
 }
 
-// A CTA per row at a time. kExact: every row is whole packets (16-byte aligned
-// rows, a vocabulary of whole packets).
-template <typename T, int kThreads, bool kExact>
-__global__ __launch_bounds__(kThreads, 1024 / kThreads) void policy_row_kernel(
-    PolicyRows shape, PolicyTerms terms, const T *__restrict__ logits, PolicyOut result, T *__restrict__ grad_logits,
-    int buffers, uint32_t buffer_bytes, int *status) {
+// A CTA per row at a time, kThreadBytes of it in a thread's registers. kExact:
+// every row is whole packets (16-byte aligned rows, a vocabulary of whole
+// packets). [logits, logits_end) is the tensor, with whatever its strides skip.
+template <typename T, int kThreads, int kThreadBytes, bool kExact>
+__global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void policy_row_kernel(
+    PolicyRows shape, PolicyTerms terms, const T *__restrict__ logits, const T *logits_end, PolicyOut result,
+    T *__restrict__ grad_logits, int buffers, uint32_t buffer_bytes, int *status) {
     constexpr int kWidth = Pack<T>::kWidth, kPackets = kThreadBytes / 16;
+    constexpr int kGroup = kPackets / 4;  // packets whose exponentials are taken, or skipped, together
+    // whether the next row is loaded as soon as this one is in registers, at a
+    // barrier more, or after the row's only barrier: small rows have several
+    // buffers and many CTAs
+    constexpr bool kEarly = kThreads > 64;
     extern __shared__ __align__(128) unsigned char smem_raw[];
+    constexpr int kTable = 64;
     __shared__ uint64_t full[4];
     __shared__ Partial merged[2][32];
+    // the scalars of kTable of the CTA's rows, loaded at once: their latency is
+    // paid once per table and not in every row
+    __shared__ RowTerms table[kTable];
+    int64_t table_end = 0;  // rows of the CTA's that have been in the table
     const int vocab = static_cast<int>(shape.vocab);
-    auto live = [&](int64_t row) { return terms.valid == nullptr || terms.valid[row] != 0; };
-    int64_t next = blockIdx.x;  // thread 0: the next row to load
-    int loaded = 0;
+    auto live = [&](int64_t row, int64_t index) {
+        if (index < table_end) return table[index % kTable].valid();
+        return terms.valid == nullptr || terms.valid[row] != 0;
+    };
+    // thread 0's: the next row to load (nothing: bytes 0), found while there is time
+    __shared__ struct {
+        const T *from;
+        int64_t row, index;
+        uint32_t to, bytes;
+        int buffer, loads;
+    } next;
+    auto find_next = [&] {
+        for (; next.row < shape.rows && !live(next.row, next.index); next.row += gridDim.x) ++next.index;
+        next.bytes = 0;
+        if (next.row >= shape.rows) return;
+        const Packets<T> packets(logits + shape.start(next.row), vocab);
+        const int from = kExact || packets.inside(0, logits, logits_end) ? 0 : 1;
+        const int to = kExact || packets.inside(packets.count - 1, logits, logits_end) ? packets.count : packets.count - 1;
+        next.from = packets.base + from * kWidth;
+        next.to = next.buffer * buffer_bytes + from * 16;
+        next.bytes = static_cast<uint32_t>(to - from) * 16;
+        next.row += gridDim.x;
+        ++next.index;
+    };
     auto load_next = [&] {
-        while (next < shape.rows && !live(next)) next += gridDim.x;
-        if (next >= shape.rows) return;
-        const Packets<T> packets(logits + shape.start(next), vocab);  // more than 1024 entries: some packets are whole
-        uint64_t *bar = &full[loaded % buffers];
-        const uint32_t bytes = static_cast<uint32_t>(packets.end - packets.first) * 16;
+        const uint32_t bytes = next.bytes;
+        if (bytes == 0) return;
+        uint64_t *bar = &full[next.buffer];
         mbar_arrive_expect_tx(bar, bytes);
-        bulk_load(smem_raw + loaded % buffers * buffer_bytes + packets.first * 16, packets.base + packets.first * kWidth, bytes, bar);
-        ++loaded;
-        next += gridDim.x;
+        bulk_load(smem_raw + next.to, next.from, bytes, bar);
+        next.buffer = next.buffer + 1 == buffers ? 0 : next.buffer + 1;
+        ++next.loads;
     };
     if (threadIdx.x == 0) {
         for (int b = 0; b < buffers; ++b) mbar_init(&full[b], 1);
+        next.row = blockIdx.x;
+        next.index = next.buffer = next.loads = 0;
         fence_barrier_init();
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int b = 0; b < buffers; ++b) load_next();
     }
     const float scale = result.inverse != nullptr ? *result.inverse : inverse_count(terms.valid, shape.rows);
     double loss_sum = 0.0, kl_sum = 0.0;  // advantages cancel: fp32 sums would lose what is left
     bool dead = false;  // a copy never arrived: go on without waiting or loading
-    int taken = 0;
-    for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
+    int taken = 0, buffer = 0;
+    uint32_t parity = 0;
+    int64_t index = 0;
+    for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x, ++index) {
+        if (index == table_end) {
+            __syncthreads();
+            if (threadIdx.x < kTable) {
+                const int64_t r = row + int64_t(threadIdx.x) * gridDim.x;
+                if (r < shape.rows) table[threadIdx.x] = load_terms(terms, r, vocab);
+            }
+            table_end += kTable;
+            __syncthreads();
+            if (threadIdx.x == 0 && index == 0) {
+                for (int b = 0; b < buffers; ++b) {
+                    find_next();
+                    load_next();
+                }
+                find_next();
+            }
+        }
+        const RowTerms row_terms = table[index % kTable];
         T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
-        if (!live(row)) {
+        if (!row_terms.valid()) {
             if (out != nullptr) clear_row(out, vocab);
             if (threadIdx.x == kThreads - 1) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
             continue;
         }
-        const T *in = logits + shape.start(row);
-        const RowScalars<T> scalars(in, terms, row, vocab);
+        const T *in = logits + (kExact ? 0 : shape.start(row));
         const Packets<T> packets(in, vocab);
-        const uint4 *staged = reinterpret_cast<const uint4 *>(smem_raw + taken % buffers * buffer_bytes) + threadIdx.x;
-        if (!dead) dead = !mbar_wait_bounded(&full[taken % buffers], static_cast<uint32_t>(taken / buffers) & 1, status);
-
-        uint4 kept[kPackets];
-#pragma unroll
-        for (int j = 0; j < kPackets; ++j) {
-            const int c = threadIdx.x + j * kThreads;
-            if (kExact ? c < packets.count : packets.whole(c)) {
-                kept[j] = staged[j * kThreads];
-            } else {
-                float v[kWidth];
-#pragma unroll
-                for (int i = 0; i < kWidth; ++i) v[i] = -INFINITY;
-                if (!kExact) packets.load_partly(c, v);
-                kept[j] = pack(v, T());
+        unsigned char *place = smem_raw + buffer * buffer_bytes;
+        const uint4 *staged = reinterpret_cast<const uint4 *>(place) + threadIdx.x;
+        if (!dead) dead = !mbar_wait_bounded(&full[buffer], parity, status);
+        if (++buffer == buffers) {
+            buffer = 0;
+            parity ^= 1;
+        }
+        // the entries of the first and the last packet, a thread each: in
+        // shared memory those outside the row become -inf
+        const int edge_packet = threadIdx.x < kWidth ? 0 : packets.count - 1, edge_place = threadIdx.x % kWidth;
+        const bool on_edge = !kExact && threadIdx.x < 2 * kWidth && !packets.whole(edge_packet);
+        T edge = from_acc<T>(-INFINITY);
+        if (!kExact) {
+            if (on_edge) {
+                const int entry = edge_packet * kWidth + edge_place;
+                T *cell = reinterpret_cast<T *>(place) + entry;
+                if (packets.in_row(edge_packet, edge_place)) {
+                    edge = packets.inside(edge_packet, logits, logits_end) ? *cell : packets.base[entry];
+                }
+                *cell = edge;
+                fence_proxy_async();  // before a copy takes the place
             }
+            __syncthreads();
+        }
+
+        // the packet and the place in it of the target
+        const int at = row_terms.target + packets.skip, packet = row_terms.target >= 0 ? at / kWidth : -1;
+        const RowScalars scalars(row_terms, packet >= 0 ? to_acc(reinterpret_cast<const T *>(place)[at]) : NAN);
+        uint4 kept[kPackets];
+        if (kExact && packets.count == kPackets * kThreads) {
+#pragma unroll
+            for (int j = 0; j < kPackets; ++j) kept[j] = staged[j * kThreads];
+        } else {
+            float nothing[kWidth];
+#pragma unroll
+            for (int i = 0; i < kWidth; ++i) nothing[i] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < kPackets; ++j) {
+                kept[j] = pack(nothing, T());
+                if (static_cast<int>(threadIdx.x) + j * kThreads < packets.count) kept[j] = staged[j * kThreads];
+            }
+        }
+        if (kEarly) {
+            __syncthreads();
+            if (threadIdx.x == 0 && !dead) load_next();
         }
         uint4 largest = kept[0];
 #pragma unroll
         for (int j = 1; j < kPackets; ++j) largest = packet_larger(largest, kept[j], T());
-        Partial p{warp_max(row_part_max(largest, T())), 0.0f};
+        Partial p{redux_max(row_part_max(largest, T())), 0.0f};
         const float from = origin(p.max);
         float2 sums = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < kPackets; ++j) {
+            if (j / kGroup * kGroup * kThreads >= packets.count) continue;
             if constexpr (sizeof(T) == 4) {
                 const float2 x = exp_from(make_float2(__uint_as_float(kept[j].x), __uint_as_float(kept[j].y)), from);
                 const float2 y = exp_from(make_float2(__uint_as_float(kept[j].z), __uint_as_float(kept[j].w)), from);
@@ -432,18 +519,18 @@ __global__ __launch_bounds__(kThreads, 1024 / kThreads) void policy_row_kernel(
         }
         p.sum = warp_sum(sums.x + sums.y);
         const Partial all = block_merge<kThreads>(p, merged, taken & 1);
-        // every thread is done with the row's buffer
-        if (threadIdx.x == 0 && !dead) load_next();
+        if (threadIdx.x == 0) {
+            if (!kEarly && !dead) load_next();
+            find_next();
+        }
         ++taken;
 
         const float lse = lse_of(all), lp = scalars.log_prob(all), slope = scalars.slope(terms, lp) * scale;
         if (threadIdx.x == kThreads - 1) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
         if (out != nullptr) {
             // of an fp32 warp with nothing but -inf: 0
-            const float factor = -slope / all.sum * (sizeof(T) == 4 ? exp_from(p.max, all.max) : 1.0f);
+            const float factor = -__fdividef(slope, all.sum) * (sizeof(T) == 4 ? exp_from(p.max, all.max) : 1.0f);
             const bool fits = kExact || packets.fits(out);
-            // the packet and the place in it of the target
-            const int at = scalars.target + packets.skip, packet = scalars.target >= 0 ? at / kWidth : -1;
 #pragma unroll
             for (int j = 0; j < kPackets; ++j) {
                 const int c = threadIdx.x + j * kThreads;
@@ -461,12 +548,29 @@ __global__ __launch_bounds__(kThreads, 1024 / kThreads) void policy_row_kernel(
                     v[i] = e.x;
                     v[i + 1] = e.y;
                 }
-                if (packet == c) {
-#pragma unroll
-                    for (int i = 0; i < kWidth; ++i) v[i] += at % kWidth == i ? slope : 0.0f;
+                if (kExact || (fits && packets.whole(c))) {
+                    packets.store(out, true, c, v);
+                } else if (!fits) {
+                    packets.store(out, false, c, v);
                 }
-                packets.store(out, kExact || (fits && packets.whole(c)), c, v);
             }
+            // the entries of packets that are not whole, and the target's again
+            // by the thread that stored it
+            const float weight = -__fdividef(slope, all.sum);
+            const bool edges = !kExact && fits, target_on_edge = edges && !packets.whole(packet);
+            if (edges && on_edge && packets.in_row(edge_packet, edge_place)) {
+                const int v = edge_packet * kWidth + edge_place - packets.skip;
+                out[v] = from_acc<T>(fmaf(exp_from(to_acc(edge), all.max), weight, v == scalars.target ? slope : 0.0f));
+            }
+            if (packet >= 0 && packet % kThreads == threadIdx.x && !target_on_edge) {
+                out[scalars.target] = from_acc<T>(fmaf(exp_from(scalars.chosen, all.max), weight, slope));
+            }
+        }
+    }
+    if (threadIdx.x == 0 && dead) {  // no copy may land after the CTA's end
+        for (int b = 0; b < buffers; ++b) {
+            const int loads = (next.loads + buffers - 1 - b) / buffers;
+            if (loads > 0) mbar_wait_bounded(&full[b], (loads - 1) & 1, status);
         }
     }
     if (threadIdx.x == kThreads - 1) result.partials[blockIdx.x] = make_double2(loss_sum, kl_sum);
@@ -486,13 +590,14 @@ __global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows sh
     int taken = 0;
     for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
         T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
-        if (terms.valid != nullptr && terms.valid[row] == 0) {
+        const RowTerms row_terms = load_terms(terms, row, vocab);
+        if (!row_terms.valid()) {
             if (out != nullptr) clear_row(out, vocab);
             if (threadIdx.x == 0) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
             continue;
         }
         const T *in = logits + shape.start(row);
-        const RowScalars<T> scalars(in, terms, row, vocab);
+        const RowScalars scalars(row_terms, row_terms.target >= 0 ? to_acc(in[row_terms.target]) : NAN);
         const Packets<T> packets(in, vocab);
         auto walk = [&](auto &&each) {
             for (int first = threadIdx.x; first < packets.count; first += kPackets * kWalkThreads) {
@@ -653,6 +758,11 @@ __global__ __launch_bounds__(256) void policy_scale_kernel(T *__restrict__ grad,
     }
 }
 
+PolicyRows rows_of(int64_t rows, int64_t vocab, int64_t inner_rows, int64_t outer_stride, int64_t inner_stride) {
+    // one run of rows, however long, is a run of all of them
+    return PolicyRows{rows, vocab, inner_rows > rows && rows > 0 ? rows : inner_rows, outer_stride, inner_stride};
+}
+
 int check_policy(const PolicyRows &shape) {
     if (shape.rows < 0 || shape.rows > (int64_t(1) << 31)) return fail(KOEMI_ERR_INVALID, "rows must be in [0, 2^31]");
     if (shape.vocab < 1 || shape.vocab > (int64_t(1) << 30)) return fail(KOEMI_ERR_INVALID, "vocab must be in [1, 2^30]");
@@ -660,26 +770,37 @@ int check_policy(const PolicyRows &shape) {
     return KOEMI_OK;
 }
 
-// The row kernel with the fewest threads that hold `entries`.
-template <typename T, int kThreads = 64>
-int launch_rows(int64_t entries, bool exact, const PolicyRows &shape, const PolicyTerms &terms, const T *logits,
+template <typename T, int kThreads, int kThreadBytes>
+int launch_rows(int64_t bytes, bool exact, const PolicyRows &shape, const PolicyTerms &terms, const T *logits,
                 const PolicyOut &result, T *grad, unsigned &blocks, cudaStream_t stream) {
-    constexpr int64_t kHeld = kThreads * (kThreadBytes / sizeof(T));
-    if constexpr (kHeld < longest_row<T>()) {
-        if (entries > kHeld) return launch_rows<T, 2 * kThreads>(entries, exact, shape, terms, logits, result, grad, blocks, stream);
-    }
-    // as many buffers as fit beside the other CTAs of the SM (1024 threads in all)
-    const uint32_t bytes = static_cast<uint32_t>(ceil_div(entries * sizeof(T), 128) * 128);
-    const uint32_t room = 222 * 1024 / (1024 / kThreads) - 2048;
-    const int buffers = static_cast<int>(room / bytes > 3 ? 3 : room / bytes);
-    const int64_t places = int64_t(sm_count()) * (1024 / kThreads);
+    constexpr int kPerSm = kSmBytes / kThreadBytes / kThreads;
+    // as many buffers as fit beside the other CTAs of the SM
+    const uint32_t buffer_bytes = static_cast<uint32_t>(ceil_div(bytes, 128) * 128), room = 222 * 1024 / kPerSm - 2048;
+    const int buffers = static_cast<int>(room / buffer_bytes > 3 ? 3 : room / buffer_bytes);
+    const int64_t places = int64_t(sm_count()) * kPerSm;
     blocks = static_cast<unsigned>(shape.rows < places ? shape.rows : places);
-    auto kernel = exact ? policy_row_kernel<T, kThreads, true> : policy_row_kernel<T, kThreads, false>;
-    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(buffers * bytes)));
-    kernel<<<blocks, kThreads, buffers * bytes, stream>>>(shape, terms, logits, result, grad, buffers, bytes,
-                                                          device_status_word());
+    const int64_t outer = (shape.rows - 1) / shape.inner, inner = (shape.rows < shape.inner ? shape.rows : shape.inner) - 1;
+    const T *end = logits + outer * shape.outer_stride + inner * shape.inner_stride + shape.vocab;
+    auto kernel = exact ? policy_row_kernel<T, kThreads, kThreadBytes, true> : policy_row_kernel<T, kThreads, kThreadBytes, false>;
+    const int shared = buffers * static_cast<int>(buffer_bytes);
+    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
+    kernel<<<blocks, kThreads, shared, stream>>>(shape, terms, logits, end, result, grad, buffers, buffer_bytes,
+                                                 device_status_word());
     KOEMI_LAUNCH_CHECK();
     return KOEMI_OK;
+}
+
+// The row kernel with the fewest threads that hold the row.
+template <typename T, int kThreads = 64>
+int launch_held(int64_t bytes, bool exact, const PolicyRows &shape, const PolicyTerms &terms, const T *logits,
+                const PolicyOut &result, T *grad, unsigned &blocks, cudaStream_t stream) {
+    if (kThreads == 64 && bytes <= 64 * 128) {
+        return launch_rows<T, 64, 128>(bytes, exact, shape, terms, logits, result, grad, blocks, stream);
+    }
+    if constexpr (kThreads * 256 < kRowBytes) {
+        if (bytes > kThreads * 256) return launch_held<T, 2 * kThreads>(bytes, exact, shape, terms, logits, result, grad, blocks, stream);
+    }
+    return launch_rows<T, kThreads, 256>(bytes, exact, shape, terms, logits, result, grad, blocks, stream);
 }
 
 template <typename T, int kPer>
@@ -717,9 +838,9 @@ int policy_forward(const PolicyRows &shape, const PolicyTerms &terms, const void
             rc = launch_warps<T, 16>(shape, terms, in, result, grad, blocks, stream);
         } else if (shape.vocab <= kWarpRow) {
             rc = launch_warps<T, 32>(shape, terms, in, result, grad, blocks, stream);
-        } else if (entries <= longest_row<T>()) {
+        } else if (entries * int64_t(sizeof(T)) <= kRowBytes) {
             const bool exact = !inside && shape.vocab % Pack<T>::kWidth == 0;
-            rc = launch_rows<T>(entries, exact, shape, terms, in, result, grad, blocks, stream);
+            rc = launch_held<T>(entries * sizeof(T), exact, shape, terms, in, result, grad, blocks, stream);
         } else {
             const int64_t places = 2 * int64_t(sm_count());
             blocks = static_cast<unsigned>(shape.rows < places ? shape.rows : places);
@@ -774,7 +895,7 @@ extern "C" int koemi_think_policy_loss_forward(const void *logits, int64_t rows,
                                                float *log_probs, float *lse, float *slopes, void *grad_logits,
                                                int dtype, void *workspace, size_t workspace_bytes, void *stream) {
     clear_error();
-    const PolicyRows shape{rows, vocab, inner_rows, outer_stride, inner_stride};
+    const PolicyRows shape = rows_of(rows, vocab, inner_rows, outer_stride, inner_stride);
     const int rc = check_policy(shape);
     if (rc != KOEMI_OK) return rc;
     if (!(clip_low >= 0.0f && clip_high >= 0.0f)) return fail(KOEMI_ERR_INVALID, "clip widths must be non-negative");
@@ -802,7 +923,7 @@ extern "C" int koemi_think_policy_loss_backward(const void *logits, int64_t rows
                                                 const uint8_t *valid, const float *lse, const float *slopes,
                                                 const float *grad_loss, void *grad_logits, int dtype, void *stream) {
     clear_error();
-    const PolicyRows shape{rows, vocab, inner_rows, outer_stride, inner_stride};
+    const PolicyRows shape = rows_of(rows, vocab, inner_rows, outer_stride, inner_stride);
     const int rc = check_policy(shape);
     if (rc != KOEMI_OK) return rc;
     if (rows == 0) return KOEMI_OK;
