@@ -34,7 +34,8 @@ namespace {
 constexpr int kPolicyBlocks = 2368;     // most CTAs of a launch: 16 per SM
 constexpr int kWarpRow = 1024;          // entries a warp holds
 constexpr int kSmBytes = 128 * 1024;    // of rows, in the registers of an SM
-constexpr int64_t kRowBytes = kSmBytes; // longest row that one CTA holds
+constexpr int kSliceBytes = 64 * 1024;  // of a row, in one CTA: longer rows are split over a cluster
+constexpr int kMaxCluster = 8;
 constexpr int64_t kCountedRows = 16384; // up to here every CTA counts the valid rows itself
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -296,12 +297,14 @@ struct Packets {
     }
 };
 
-// Zeros into a row of the gradient, by a CTA.
+// Zeros into a row of the gradient, by a CTA: from packet `first` on, `count`
+// of them or, the last slice, to the row's end.
 template <typename T>
-__device__ void clear_row(T *out, int vocab) {
+__device__ void clear_row(T *out, int vocab, int first = 0, int count = 0) {
     const Packets<T> packets(out, vocab);
     const float zeros[Packets<T>::kWidth] = {};
-    for (int c = threadIdx.x; c < packets.count; c += blockDim.x) packets.store(out, packets.whole(c), c, zeros);
+    const int end = count > 0 ? first + count : packets.count;
+    for (int c = first + threadIdx.x; c < end; c += blockDim.x) packets.store(out, packets.whole(c), c, zeros);
 }
 
 // The warps' partials of a row, merged by every warp alike: the row's partial
@@ -357,13 +360,28 @@ __device__ __forceinline__ float2 exp_from(float2 v, float from) {
     return make_float2(ex2_approx(v.x), ex2_approx(v.y));
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Four floats into the same place of CTA `rank` of the cluster, counted on its
+// barrier in the same place as `bar`.
+__device__ __forceinline__ void store_to_rank(float4 *local, uint64_t *bar, int rank, float4 v) {
+    asm volatile(
+        "{\n\t.reg .b32 a, b;\n\tmapa.shared::cluster.u32 a, %0, %2;\n\tmapa.shared::cluster.u32 b, %1, %2;\n\t"
+        "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [a], {%3, %4, %5, %6}, [b];\n\t}" ::"r"(smem_addr(local)),
+        "r"(smem_addr(bar)), "r"(rank), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+        : "memory");
+}
+
 // A CTA per row at a time, kThreadBytes of it in a thread's registers. kExact:
 // every row is whole packets (16-byte aligned rows, a vocabulary of whole
 // packets). [logits, logits_end) is the tensor, with whatever its strides skip.
-template <typename T, int kThreads, int kThreadBytes, bool kExact>
+// kSplit: a cluster per row; each CTA takes `slice` packets of it, the last
+// one the rest, and they give each other their (maximum, sum, target's logit).
+template <typename T, int kThreads, int kThreadBytes, bool kExact, bool kSplit>
 __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void policy_row_kernel(
     PolicyRows shape, PolicyTerms terms, const T *__restrict__ logits, const T *logits_end, PolicyOut result,
-    T *__restrict__ grad_logits, int buffers, uint32_t buffer_bytes, int *status) {
+    T *__restrict__ grad_logits, int buffers, uint32_t buffer_bytes, int cluster, int slice, int *status) {
     constexpr int kWidth = Pack<T>::kWidth, kPackets = kThreadBytes / 16;
     constexpr int kGroup = kPackets / 4;  // packets whose exponentials are taken, or skipped, together
     // whether the next row is loaded as soon as this one is in registers, at a
@@ -377,6 +395,11 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
     // the scalars of kTable of the CTA's rows, loaded at once: their latency is
     // paid once per table and not in every row
     __shared__ RowTerms table[kTable];
+    __shared__ float4 met[2][kSplit ? kMaxCluster : 1];  // the CTAs' parts of two rows
+    __shared__ uint64_t meeting[2];
+    const int rank = kSplit ? static_cast<int>(blockIdx.x % cluster) : 0, first = rank * slice;  // the slice's first packet
+    const int64_t first_row = kSplit ? blockIdx.x / cluster : blockIdx.x, row_step = kSplit ? gridDim.x / cluster : gridDim.x;
+    const bool last_slice = !kSplit || rank == cluster - 1;
     int64_t table_end = 0;  // rows of the CTA's that have been in the table
     const int vocab = static_cast<int>(shape.vocab);
     auto live = [&](int64_t row, int64_t index) {
@@ -391,16 +414,17 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
         int buffer, loads;
     } next;
     auto find_next = [&] {
-        for (; next.row < shape.rows && !live(next.row, next.index); next.row += gridDim.x) ++next.index;
+        for (; next.row < shape.rows && !live(next.row, next.index); next.row += row_step) ++next.index;
         next.bytes = 0;
         if (next.row >= shape.rows) return;
         const Packets<T> packets(logits + shape.start(next.row), vocab);
-        const int from = kExact || packets.inside(0, logits, logits_end) ? 0 : 1;
-        const int to = kExact || packets.inside(packets.count - 1, logits, logits_end) ? packets.count : packets.count - 1;
-        next.from = packets.base + from * kWidth;
-        next.to = next.buffer * buffer_bytes + from * 16;
+        const int from = kExact || first > 0 || packets.inside(0, logits, logits_end) ? first : first + 1;
+        const int to = !last_slice ? first + slice
+                       : kExact || packets.inside(packets.count - 1, logits, logits_end) ? packets.count : packets.count - 1;
+        next.from = packets.base + int64_t(from) * kWidth;
+        next.to = next.buffer * buffer_bytes + (from - first) * 16;
         next.bytes = static_cast<uint32_t>(to - from) * 16;
-        next.row += gridDim.x;
+        next.row += row_step;
         ++next.index;
     };
     auto load_next = [&] {
@@ -414,21 +438,24 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
     };
     if (threadIdx.x == 0) {
         for (int b = 0; b < buffers; ++b) mbar_init(&full[b], 1);
-        next.row = blockIdx.x;
+        next.row = first_row;
         next.index = next.buffer = next.loads = 0;
+        mbar_init(&meeting[0], 1);
+        mbar_init(&meeting[1], 1);
         fence_barrier_init();
     }
+    if (kSplit) cluster_sync();  // every CTA's barriers are ready before one stores into another
     const float scale = result.inverse != nullptr ? *result.inverse : inverse_count(terms.valid, shape.rows);
     double loss_sum = 0.0, kl_sum = 0.0;  // advantages cancel: fp32 sums would lose what is left
     bool dead = false;  // a copy never arrived: go on without waiting or loading
     int taken = 0, buffer = 0;
     uint32_t parity = 0;
     int64_t index = 0;
-    for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x, ++index) {
+    for (int64_t row = first_row; row < shape.rows; row += row_step, ++index) {
         if (index == table_end) {
             __syncthreads();
             if (threadIdx.x < kTable) {
-                const int64_t r = row + int64_t(threadIdx.x) * gridDim.x;
+                const int64_t r = row + int64_t(threadIdx.x) * row_step;
                 if (r < shape.rows) table[threadIdx.x] = load_terms(terms, r, vocab);
             }
             table_end += kTable;
@@ -444,12 +471,13 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
         const RowTerms row_terms = table[index % kTable];
         T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
         if (!row_terms.valid()) {
-            if (out != nullptr) clear_row(out, vocab);
-            if (threadIdx.x == kThreads - 1) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
+            if (out != nullptr) clear_row(out, vocab, first, last_slice ? 0 : slice);
+            if (threadIdx.x == kThreads - 1 && rank == 0) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
             continue;
         }
         const T *in = logits + (kExact ? 0 : shape.start(row));
         const Packets<T> packets(in, vocab);
+        const int count = last_slice ? packets.count - first : slice;  // of the slice
         unsigned char *place = smem_raw + buffer * buffer_bytes;
         const uint4 *staged = reinterpret_cast<const uint4 *>(place) + threadIdx.x;
         if (!dead) dead = !mbar_wait_bounded(&full[buffer], parity, status);
@@ -460,12 +488,13 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
         // the entries of the first and the last packet, a thread each: in
         // shared memory those outside the row become -inf
         const int edge_packet = threadIdx.x < kWidth ? 0 : packets.count - 1, edge_place = threadIdx.x % kWidth;
-        const bool on_edge = !kExact && threadIdx.x < 2 * kWidth && !packets.whole(edge_packet);
+        const bool on_edge = !kExact && threadIdx.x < 2 * kWidth && !packets.whole(edge_packet) &&
+                             (threadIdx.x < kWidth ? rank == 0 : last_slice);
         T edge = from_acc<T>(-INFINITY);
         if (!kExact) {
             if (on_edge) {
                 const int entry = edge_packet * kWidth + edge_place;
-                T *cell = reinterpret_cast<T *>(place) + entry;
+                T *cell = reinterpret_cast<T *>(place) + (entry - first * kWidth);
                 if (packets.in_row(edge_packet, edge_place)) {
                     edge = packets.inside(edge_packet, logits, logits_end) ? *cell : packets.base[entry];
                 }
@@ -475,11 +504,12 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
             __syncthreads();
         }
 
-        // the packet and the place in it of the target
+        // the target's entry and packet, and the packet's place in the slice
         const int at = row_terms.target + packets.skip, packet = row_terms.target >= 0 ? at / kWidth : -1;
-        const RowScalars scalars(row_terms, packet >= 0 ? to_acc(reinterpret_cast<const T *>(place)[at]) : NAN);
+        const bool here = packet >= first && packet < first + count;
+        float chosen = here ? to_acc(reinterpret_cast<const T *>(place)[at - first * kWidth]) : NAN;
         uint4 kept[kPackets];
-        if (kExact && packets.count == kPackets * kThreads) {
+        if (kExact && count == kPackets * kThreads) {
 #pragma unroll
             for (int j = 0; j < kPackets; ++j) kept[j] = staged[j * kThreads];
         } else {
@@ -489,7 +519,7 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
 #pragma unroll
             for (int j = 0; j < kPackets; ++j) {
                 kept[j] = pack(nothing, T());
-                if (static_cast<int>(threadIdx.x) + j * kThreads < packets.count) kept[j] = staged[j * kThreads];
+                if (static_cast<int>(threadIdx.x) + j * kThreads < count) kept[j] = staged[j * kThreads];
             }
         }
         if (kEarly) {
@@ -504,7 +534,7 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
         float2 sums = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < kPackets; ++j) {
-            if (j / kGroup * kGroup * kThreads >= packets.count) continue;
+            if (j / kGroup * kGroup * kThreads >= count) continue;
             if constexpr (sizeof(T) == 4) {
                 const float2 x = exp_from(make_float2(__uint_as_float(kept[j].x), __uint_as_float(kept[j].y)), from);
                 const float2 y = exp_from(make_float2(__uint_as_float(kept[j].z), __uint_as_float(kept[j].w)), from);
@@ -518,23 +548,34 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
             }
         }
         p.sum = warp_sum(sums.x + sums.y);
-        const Partial all = block_merge<kThreads>(p, merged, taken & 1);
+        Partial all = block_merge<kThreads>(p, merged, taken & 1);
+        if (kSplit) {
+            float4 *parts = met[taken & 1];
+            uint64_t *bar = &meeting[taken & 1];
+            if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, cluster * sizeof(float4));
+            if (threadIdx.x < cluster) store_to_rank(parts + rank, bar, threadIdx.x, make_float4(all.max, all.sum, chosen, 0.0f));
+            if (!dead) dead = !mbar_wait_bounded(bar, static_cast<uint32_t>(taken >> 1) & 1, status);
+            const int lane = threadIdx.x & 31;
+            all = warp_merge(lane < cluster ? Partial{parts[lane].x, parts[lane].y} : Partial{-INFINITY, 0.0f});
+            if (packet >= 0) chosen = parts[packet / slice < cluster ? packet / slice : cluster - 1].z;
+        }
         if (threadIdx.x == 0) {
             if (!kEarly && !dead) load_next();
             find_next();
         }
         ++taken;
 
+        const RowScalars scalars(row_terms, chosen);
         const float lse = lse_of(all), lp = scalars.log_prob(all), slope = scalars.slope(terms, lp) * scale;
-        if (threadIdx.x == kThreads - 1) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
+        if (threadIdx.x == kThreads - 1 && rank == 0) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
         if (out != nullptr) {
             // of an fp32 warp with nothing but -inf: 0
             const float factor = -__fdividef(slope, all.sum) * (sizeof(T) == 4 ? exp_from(p.max, all.max) : 1.0f);
             const bool fits = kExact || packets.fits(out);
 #pragma unroll
             for (int j = 0; j < kPackets; ++j) {
-                const int c = threadIdx.x + j * kThreads;
-                if (c >= packets.count) continue;
+                const int c = first + threadIdx.x + j * kThreads;
+                if (c >= first + count) continue;
                 // from here a value of its own: else the first loop's fp32
                 // entries would be kept across the barrier, and spilled
                 asm("" : "+r"(kept[j].x), "+r"(kept[j].y), "+r"(kept[j].z), "+r"(kept[j].w));
@@ -562,7 +603,7 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
                 const int v = edge_packet * kWidth + edge_place - packets.skip;
                 out[v] = from_acc<T>(fmaf(exp_from(to_acc(edge), all.max), weight, v == scalars.target ? slope : 0.0f));
             }
-            if (packet >= 0 && packet % kThreads == threadIdx.x && !target_on_edge) {
+            if (here && (packet - first) % kThreads == threadIdx.x && !target_on_edge) {
                 out[scalars.target] = from_acc<T>(fmaf(exp_from(scalars.chosen, all.max), weight, slope));
             }
         }
@@ -573,7 +614,8 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
             if (loads > 0) mbar_wait_bounded(&full[b], (loads - 1) & 1, status);
         }
     }
-    if (threadIdx.x == kThreads - 1) result.partials[blockIdx.x] = make_double2(loss_sum, kl_sum);
+    if (kSplit) cluster_sync();  // no CTA ends while another may store into it
+    if (threadIdx.x == kThreads - 1 && rank == 0) result.partials[first_row] = make_double2(loss_sum, kl_sum);
 }
 
 // Longer rows, in blocks of 1024 threads x 32 entries, walked twice.
@@ -770,37 +812,61 @@ int check_policy(const PolicyRows &shape) {
     return KOEMI_OK;
 }
 
-template <typename T, int kThreads, int kThreadBytes>
+// The clusters of `size` CTAs that run at the same time, two CTAs on an SM.
+template <typename Kernel>
+int resident_clusters(Kernel kernel, int threads, int shared, int size) {
+    cudaLaunchConfig_t config{};
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = size;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.gridDim = dim3(size);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess || clusters < 1) {
+        cudaGetLastError();
+        clusters = 2 * sm_count() / size;
+    }
+    return clusters;
+}
+
+// `blocks`: the partial sums that the kernel leaves.
+template <typename T, int kThreads, int kThreadBytes, bool kSplit>
 int launch_rows(int64_t bytes, bool exact, const PolicyRows &shape, const PolicyTerms &terms, const T *logits,
                 const PolicyOut &result, T *grad, unsigned &blocks, cudaStream_t stream) {
     constexpr int kPerSm = kSmBytes / kThreadBytes / kThreads;
+    const int cluster = kSplit ? static_cast<int>(ceil_div(bytes, kSliceBytes)) : 1;
+    const int slice = static_cast<int>(ceil_div(ceil_div(bytes, 16), cluster));
     // as many buffers as fit beside the other CTAs of the SM
-    const uint32_t buffer_bytes = static_cast<uint32_t>(ceil_div(bytes, 128) * 128), room = 222 * 1024 / kPerSm - 2048;
+    const uint32_t buffer_bytes = static_cast<uint32_t>(ceil_div(slice * 16, 128) * 128), room = 222 * 1024 / kPerSm - 2048;
     const int buffers = static_cast<int>(room / buffer_bytes > 3 ? 3 : room / buffer_bytes);
-    const int64_t places = int64_t(sm_count()) * kPerSm;
-    blocks = static_cast<unsigned>(shape.rows < places ? shape.rows : places);
     const int64_t outer = (shape.rows - 1) / shape.inner, inner = (shape.rows < shape.inner ? shape.rows : shape.inner) - 1;
     const T *end = logits + outer * shape.outer_stride + inner * shape.inner_stride + shape.vocab;
-    auto kernel = exact ? policy_row_kernel<T, kThreads, kThreadBytes, true> : policy_row_kernel<T, kThreads, kThreadBytes, false>;
+    auto kernel = exact ? policy_row_kernel<T, kThreads, kThreadBytes, true, kSplit>
+                        : policy_row_kernel<T, kThreads, kThreadBytes, false, kSplit>;
     const int shared = buffers * static_cast<int>(buffer_bytes);
     KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
-    kernel<<<blocks, kThreads, shared, stream>>>(shape, terms, logits, end, result, grad, buffers, buffer_bytes,
-                                                 device_status_word());
-    KOEMI_LAUNCH_CHECK();
+    const int64_t places = kSplit ? resident_clusters(kernel, kThreads, shared, cluster) : int64_t(sm_count()) * kPerSm;
+    blocks = static_cast<unsigned>(shape.rows < places ? shape.rows : places);
+    KOEMI_CUDA_TRY(launch_programmatic(false, kernel, dim3(blocks * cluster), dim3(kThreads), static_cast<size_t>(shared), stream,
+                                       dim3(cluster), shape, terms, logits, end, result, grad, buffers, buffer_bytes, cluster,
+                                       slice, device_status_word()));
     return KOEMI_OK;
 }
 
 // The row kernel with the fewest threads that hold the row.
-template <typename T, int kThreads = 64>
+template <typename T>
 int launch_held(int64_t bytes, bool exact, const PolicyRows &shape, const PolicyTerms &terms, const T *logits,
                 const PolicyOut &result, T *grad, unsigned &blocks, cudaStream_t stream) {
-    if (kThreads == 64 && bytes <= 64 * 128) {
-        return launch_rows<T, 64, 128>(bytes, exact, shape, terms, logits, result, grad, blocks, stream);
-    }
-    if constexpr (kThreads * 256 < kRowBytes) {
-        if (bytes > kThreads * 256) return launch_held<T, 2 * kThreads>(bytes, exact, shape, terms, logits, result, grad, blocks, stream);
-    }
-    return launch_rows<T, kThreads, 256>(bytes, exact, shape, terms, logits, result, grad, blocks, stream);
+    auto go = [&](auto launch) { return launch(bytes, exact, shape, terms, logits, result, grad, blocks, stream); };
+    if (bytes <= 64 * 128) return go(launch_rows<T, 64, 128, false>);
+    if (bytes <= 64 * 256) return go(launch_rows<T, 64, 256, false>);
+    if (bytes <= 128 * 256) return go(launch_rows<T, 128, 256, false>);
+    if (bytes <= 256 * 256) return go(launch_rows<T, 256, 256, false>);
+    return go(launch_rows<T, 256, 256, true>);
 }
 
 template <typename T, int kPer>
@@ -838,7 +904,7 @@ int policy_forward(const PolicyRows &shape, const PolicyTerms &terms, const void
             rc = launch_warps<T, 16>(shape, terms, in, result, grad, blocks, stream);
         } else if (shape.vocab <= kWarpRow) {
             rc = launch_warps<T, 32>(shape, terms, in, result, grad, blocks, stream);
-        } else if (entries * int64_t(sizeof(T)) <= kRowBytes) {
+        } else if (entries * int64_t(sizeof(T)) <= kMaxCluster * kSliceBytes) {
             const bool exact = !inside && shape.vocab % Pack<T>::kWidth == 0;
             rc = launch_held<T>(entries * sizeof(T), exact, shape, terms, in, result, grad, blocks, stream);
         } else {
