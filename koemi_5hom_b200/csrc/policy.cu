@@ -12,20 +12,32 @@
 //
 // The logits are read once and their gradient is written once, in one pass
 // over the rows, bound by HBM. Up to 1024 entries a warp holds a row in
-// registers. Up to 32768 (fp32) or 65536 a CTA of 64 to 1024 threads does: a bulk copy brings
-// the row into shared memory, a thread takes 128 bytes of it (32 fp32 or 64
-// 16-bit entries) into registers, which frees the buffer for the next row's
-// copy, adds its exponentials up relative to its warp's maximum, and the
-// warps' (maximum, sum) pairs meet at the row's only barrier; then it forms the
-// gradient from its registers. fp32 entries are kept as exponentials, 16-bit
-// ones as they came, with a second exponential: half the registers, so that
-// two CTAs share an SM at 32768 entries and hide each other's latency (8192 x
-// 32768 bf16: 178 us, 243 us with one CTA of 1024 threads that keeps
-// exponentials).
-// Longer rows are walked twice from memory in blocks of 32768, the second time
-// mostly from L2.
-// Every row belongs to one CTA and per-CTA sums are added in a fixed order by
-// a second kernel, so equal inputs give equal bits.
+// registers. Up to 64 KB a CTA of 64 to 256 threads does: a bulk copy brings
+// the row into shared memory, a thread takes up to 256 bytes of it into
+// registers, which frees the buffer for the next row's copy, adds its
+// exponentials up relative to its warp's maximum, and the warps' (maximum,
+// sum) pairs meet at a barrier; then it forms the gradient from its registers.
+// fp32 entries are kept as exponentials, 16-bit ones as they came, with a
+// second exponential: half the registers, so that 512 threads hold two rows of
+// 64 KB and one row's arithmetic hides the other's latency. Up to 512 KB a
+// cluster of 2 to 8 CTAs holds a row so, 64 KB a CTA, and the CTAs exchange
+// their (maximum, sum) through distributed shared memory. Longer rows are
+// walked twice from memory, the second time mostly from L2.
+//
+// Read and written at the device's copy bandwidth, these take (time, fraction
+// of it): 8192 x 32768 bf16 182 us, 0.90; 8192 x 16384 fp32 189 us, 0.87; 1024
+// x 131072 fp32 185 us, 0.89; 2048 x 131072 bf16 221 us, 0.74, with the cluster's
+// exchange in every row; rows that are not whole packets pay a barrier more
+// and the edges' own stores, 4096 x 50257 bf16 201 us, 0.63; evaluation reads
+// only, and the exponentials' share shows: 8192 x 32768 bf16 105 us,
+// 0.78. What these replaced: 128 bytes of a row to each of twice as many
+// threads (half the work per row and warp that is not per entry) 8192 x 32768
+// bf16 196 us; the next row's copy after the row's reduction, 187 us and 123 in
+// evaluation; the row in chunks with a barrier each, 209 us and more; one CTA
+// for 128 KB 4096 x 50257 bf16 196 us and 4096 x 32768 fp32 196 us, as the
+// cluster, but 266 us for rows of 256 KB, walked.
+// Every row belongs to one CTA or cluster and their sums are added in a fixed
+// order by a second kernel, so equal inputs give equal bits.
 #include "vec.cuh"
 
 namespace koemi {
@@ -383,7 +395,6 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
     PolicyRows shape, PolicyTerms terms, const T *__restrict__ logits, const T *logits_end, PolicyOut result,
     T *__restrict__ grad_logits, int buffers, uint32_t buffer_bytes, int cluster, int slice, int *status) {
     constexpr int kWidth = Pack<T>::kWidth, kPackets = kThreadBytes / 16;
-    constexpr int kGroup = kPackets / 4;  // packets whose exponentials are taken, or skipped, together
     // whether the next row is loaded as soon as this one is in registers, at a
     // barrier more, or after the row's only barrier: small rows have several
     // buffers and many CTAs
@@ -534,7 +545,7 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
         float2 sums = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int j = 0; j < kPackets; ++j) {
-            if (j / kGroup * kGroup * kThreads >= count) continue;
+            if (j * kThreads >= count) continue;
             if constexpr (sizeof(T) == 4) {
                 const float2 x = exp_from(make_float2(__uint_as_float(kept[j].x), __uint_as_float(kept[j].y)), from);
                 const float2 y = exp_from(make_float2(__uint_as_float(kept[j].z), __uint_as_float(kept[j].w)), from);

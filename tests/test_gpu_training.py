@@ -645,6 +645,37 @@ def test_policy_bits_repeat(cuda):
         assert torch.equal(first.loss, again.loss) and torch.equal(first.kl, again.kl) and torch.equal(grad, grad2)
 
 
+@pytest.mark.parametrize("vocab,dtype", [(1030, torch.float32), (4097, torch.bfloat16), (16397, torch.float16),
+                                         (33001, torch.float32), (70003, torch.bfloat16)])
+def test_policy_ragged_rows_at_the_ends_of_their_storage(vocab, dtype, cuda):
+    """Rows of odd lengths that start one element into a storage and end with it, between NaN where it has room."""
+    rows = 7
+    case = policy_case(rows, vocab, dtype, vocab, cuda)
+    scale = 64.0 if dtype == torch.float16 else None
+    expected = plain_policy(case, scale=scale or 1.0)
+    for stride in (vocab, vocab + 3):
+        storage = torch.full((1 + (rows - 1) * stride + vocab,), math.nan, dtype=dtype, device=cuda)
+        logits = storage.as_strided((rows, vocab), (stride, 1), 1)
+        logits.copy_(case["logits"])
+        result, grad = run_policy(case, scale=scale, logits=logits.detach().requires_grad_(True))
+        check_policy(case, result, grad, expected, scale or 1.0)
+
+
+def test_policy_many_rows_of_a_cta(cuda):
+    """512 times the same 40 rows: more than a CTA's table of row scalars holds."""
+    case = policy_case(40, 16400, torch.bfloat16, 21, cuda)
+    loss, kl, lp, want = plain_policy(case)
+    many = {k: t.repeat(512, *[1] * (t.ndim - 1)) for k, t in case.items()}
+    result, grad = run_policy(many)
+    size = 136 * EPS * 3 * max(1.0, case["advantages"].abs().max().item())
+    check(result.loss.detach(), loss, torch.float32, size)
+    check(result.kl, kl, torch.float32, size)
+    check(result.log_probs, lp.repeat(512), torch.float32, 136 * EPS)
+    assert torch.equal(grad.view(512, 40, -1), grad[:40].expand(512, -1, -1))  # equal rows, equal bits
+    count = int(case["valid"].sum())
+    check(grad[:40] * 512, want, torch.bfloat16, size / count)
+
+
 def test_policy_offsets_past_32_bits(cuda):
     """70000 rows of 32768: only the last ones are valid."""
     rows, vocab = 70000, 32768
