@@ -18,6 +18,11 @@
 // lanes, element e in lane e % lanes: every logit is loaded once, and a warp
 // works on 1 to 4 rows. Wider rows are walked from memory by one warp
 // (route_*_wide_kernel).
+//
+// A row is a chain of reductions and its bytes are few: 32768 tokens of 64
+// fp32 logits, top-2, take 11.8 us (8.4 MB, 1.3 us of copy bandwidth), the
+// second kernel 6.5 us and the gradient 7.1 us (16.8 MB, 2.6 us); 256 tokens
+// 3.5 and 2.8 us, the latency of two launches.
 #include <type_traits>
 
 #include "common.cuh"
