@@ -225,14 +225,21 @@ __global__ __launch_bounds__(256) void policy_warp_kernel(PolicyRows shape, Poli
         }
         const T *in = logits + shape.start(row);
         const RowScalars scalars(row_terms, row_terms.target >= 0 ? to_acc(in[row_terms.target]) : NAN);
+        // loaded as they are and converted later: every load is on its way first
+        T raw[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            raw[j] = from_acc<T>(-INFINITY);
+            if (lane + 32 * j < vocab) raw[j] = in[lane + 32 * j];
+        }
         float e[kPer];
         Partial p{-INFINITY, 0.0f};
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            e[j] = lane + 32 * j < vocab ? to_acc(in[lane + 32 * j]) : -INFINITY;
+            e[j] = to_acc(raw[j]);
             p.max = fmaxf(p.max, e[j]);
         }
-        p.max = warp_max(p.max);
+        p.max = redux_max(p.max);
         const float from = origin(p.max);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
@@ -909,8 +916,11 @@ int policy_forward(const PolicyRows &shape, const PolicyTerms &terms, const void
         const bool inside = !aligned(logits, 16) || shape.outer_stride * sizeof(T) % 16 != 0 || shape.inner_stride * sizeof(T) % 16 != 0;
         const int64_t entries = shape.vocab + (inside ? Pack<T>::kWidth - 1 : 0);
         int rc;
+        // 65536 x 257 fp32: 45 us with 12 entries a lane, 48 us with 16
         if (shape.vocab <= 256) {
             rc = launch_warps<T, 8>(shape, terms, in, result, grad, blocks, stream);
+        } else if (shape.vocab <= 384) {
+            rc = launch_warps<T, 12>(shape, terms, in, result, grad, blocks, stream);
         } else if (shape.vocab <= 512) {
             rc = launch_warps<T, 16>(shape, terms, in, result, grad, blocks, stream);
         } else if (shape.vocab <= kWarpRow) {
