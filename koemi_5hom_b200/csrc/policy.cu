@@ -867,7 +867,8 @@ int launch_rows(int64_t bytes, bool exact, const PolicyRows &shape, const Policy
                         : policy_row_kernel<T, kThreads, kThreadBytes, false, kSplit>;
     const int shared = buffers * static_cast<int>(buffer_bytes);
     KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
-    const int64_t places = kSplit ? resident_clusters(kernel, kThreads, shared, cluster) : int64_t(sm_count()) * kPerSm;
+    int64_t places = kSplit ? resident_clusters(kernel, kThreads, shared, cluster) : int64_t(sm_count()) * kPerSm;
+    if (places > kPolicyBlocks) places = kPolicyBlocks;  // a partial sum each
     blocks = static_cast<unsigned>(shape.rows < places ? shape.rows : places);
     KOEMI_CUDA_TRY(launch_programmatic(false, kernel, dim3(blocks * cluster), dim3(kThreads), static_cast<size_t>(shared), stream,
                                        dim3(cluster), shape, terms, logits, end, result, grad, buffers, buffer_bytes, cluster,
