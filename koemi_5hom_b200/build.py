@@ -92,7 +92,9 @@ def build_binding(verbose: bool = False) -> Path:
                "-I", str(INCLUDE_DIR), "-isystem", str(root / "include"),
                "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
                "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_path("include"), str(BINDING_SOURCE), "-o", str(temporary),
-               "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python", "-ldl"]
+               # torch's own C++ library: one linked in statically, as some compilers do by
+               # themselves, crashes where both sides' streams meet
+               "-l:libstdc++.so.6", "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python", "-ldl"]
     if verbose:
         print(" ".join(command), flush=True)
     result = subprocess.run(command, capture_output=True, text=True)

@@ -169,3 +169,9 @@ def test_entries_refuse_bad_arguments_before_touching_the_device():
     address[0] = 0
     assert clip() == invalid and "no data" in _native.last_error()
     assert lib.koemi_core_clip_gradients_workspace(elements, 1) >= 4
+
+
+def test_binding_formats_its_refusals():
+    """Its messages are formatted with the process's C++ library, not with one of its own."""
+    with pytest.raises(ValueError, match="gradients must be on one CUDA device"):
+        _native.binding().koemi_torch_clip_gradients([torch.zeros(2)], None, 1.0)
