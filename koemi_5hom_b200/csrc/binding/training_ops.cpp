@@ -4,13 +4,14 @@
 // They are C++ because their backward passes run on autograd's device thread,
 // where a Python function waits for the interpreter: a forward and backward of
 // an 8 x 257 policy loss took 142 us of host time with Python autograd functions
-// and ctypes calls (kernels: 10 us), of which 50 us are autograd's own.
+// and ctypes calls (kernels: 10 us) and takes 67 us; a C++ op of torch takes 50.
 // The clipping of gradients is called directly with its Python lists: through
 // the dispatcher, which copies a list of tensors twice, 2 x 144 tensors took 48
 // us where the kernels take 10. The autograd nodes are plain ones, as torch's
 // own ops have, with what the backward needs in fields.
-// Nothing here computes: every op checks what the kernels rely on, allocates
-// from the caching allocator and calls one entry point on the current stream.
+// Nothing here computes: every op checks what the kernels rely on (3 to 5 us
+// less than in Python, where only a refusal is explained), allocates from the
+// caching allocator and calls one entry point on the current stream.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -23,6 +24,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
+#include <cmath>
 #include <mutex>
 #include <string>
 #include <tuple>
@@ -116,6 +118,22 @@ std::shared_ptr<NodeType> node_of(const Inputs &...inputs) {
     return node;
 }
 
+// The fronts explain a refusal in their own error types; these are what the
+// kernels rely on, whoever calls.
+bool one_of_ours(const Tensor &t) {
+    const auto type = t.scalar_type();
+    return t.is_cuda() && (type == at::kFloat || type == at::kHalf || type == at::kBFloat16);
+}
+void require(const char *name, const Tensor &t, at::IntArrayRef shape, at::ScalarType type, const Tensor &on) {
+    TORCH_CHECK_VALUE(t.scalar_type() == type && t.sizes() == shape && t.device() == on.device() && t.is_contiguous(), name,
+                      " must be contiguous ", type, " of shape ", shape, " on ", on.device(), ", got ", t.scalar_type(), " of ",
+                      t.sizes(), " on ", t.device());
+}
+void require(const char *name, const OptionalTensor &t, at::IntArrayRef shape, at::ScalarType type, const Tensor &on) {
+    if (t.has_value() && t->defined()) require(name, *t, shape, type, on);
+}
+OptionalTensor dense(const OptionalTensor &t) { return t.has_value() && t->defined() ? OptionalTensor(t->contiguous()) : OptionalTensor(); }
+
 void first_order_only() {
     TORCH_CHECK(!at::GradMode::is_enabled(), "the training operators are differentiable to first order only (create_graph=True)");
 }
@@ -124,9 +142,26 @@ void first_order_only() {
 
 constexpr int64_t kSegment = 128;  // positions between two carries
 
+void check_recurrence(const Tensor &projections, const OptionalTensor &valid, const OptionalTensor &restart) {
+    TORCH_CHECK_VALUE(one_of_ours(projections) && projections.dim() == 3 && projections.size(2) % 2 == 0 && projections.is_contiguous(),
+                      "projections must be contiguous [batch, length, 2 * features] in f32, bf16 or f16 on a CUDA device");
+    const int64_t shape[] = {projections.size(0), projections.size(1)};
+    require("valid", valid, shape, at::kBool, projections);
+    require("restart", restart, shape, at::kBool, projections);
+}
+
+void check_forward(const Tensor &projections, const OptionalTensor &initial, const OptionalTensor &valid,
+                   const OptionalTensor &restart, double low, double high) {
+    check_recurrence(projections, valid, restart);
+    require("initial", initial, {projections.size(0), projections.size(2) / 2}, at::kFloat, projections);
+    TORCH_CHECK_VALUE(0.0 < low && low <= high && high < 1.0, "retention bounds must satisfy 0 < minimum <= maximum < 1");
+}
+
 std::tuple<Tensor, Tensor, Tensor> gated_forward(const Tensor &projections, const OptionalTensor &initial,
                                                  const OptionalTensor &valid, const OptionalTensor &restart, double low,
                                                  double high, bool keep) {
+    check_forward(projections, initial, valid, restart, low, high);
+    TORCH_CHECK_VALUE(projections.size(1) > 0, "projections must hold a position");
     const Launch launch(projections);
     const int64_t batch = projections.size(0), length = projections.size(1), features = projections.size(2) / 2;
     Tensor states = at::empty({batch, length, features}, projections.options());
@@ -141,10 +176,22 @@ std::tuple<Tensor, Tensor, Tensor> gated_forward(const Tensor &projections, cons
     return {states, final_state, carries};
 }
 
+// No position: no states, and the state as it was (differentiably, above the CUDA key).
+std::tuple<Tensor, Tensor> no_positions(const Tensor &projections, const OptionalTensor &initial) {
+    const int64_t features = projections.size(2) / 2;
+    return {projections.slice(2, 0, features).contiguous(),
+            initial.has_value() && initial->defined() ? initial->clone() : at::zeros({projections.size(0), features}, projections.options().dtype(at::kFloat))};
+}
+
 std::tuple<Tensor, Tensor> gated_recurrence_cuda(const Tensor &projections, const OptionalTensor &initial,
                                                  const OptionalTensor &valid, const OptionalTensor &restart, double low,
                                                  double high) {
-    auto [states, final_state, carries] = gated_forward(projections, initial, valid, restart, low, high, false);
+    if (projections.dim() == 3 && projections.size(1) == 0) {
+        check_forward(projections.contiguous(), dense(initial), dense(valid), dense(restart), low, high);
+        return no_positions(projections, initial);
+    }
+    auto [states, final_state, carries] =
+        gated_forward(projections.contiguous(), dense(initial), dense(valid), dense(restart), low, high, false);
     return {states, final_state};
 }
 
@@ -158,8 +205,13 @@ std::tuple<Tensor, Tensor> gated_recurrence_backward_cuda(const Tensor &projecti
                                                           const OptionalTensor &restart, const Tensor &carries,
                                                           const OptionalTensor &grad_states,
                                                           const OptionalTensor &grad_final, double low, double high) {
+    check_recurrence(projections, valid, restart);
+    TORCH_CHECK_VALUE(projections.size(1) > 0, "projections must hold a position");
     const Launch launch(projections);
     const int64_t batch = projections.size(0), length = projections.size(1), features = projections.size(2) / 2;
+    require("carries", carries, {batch, (length + kSegment - 1) / kSegment, features}, at::kFloat, projections);
+    require("grad_states", grad_states, {batch, length, features}, projections.scalar_type(), projections);
+    require("grad_final", grad_final, {batch, features}, at::kFloat, projections);
     Tensor grad_projections = at::empty_like(projections), grad_initial = f32(projections, {batch, features});
     check("koemi_dense_gated_recurrence_backward",
           lib().gated_backward(address<void>(projections), address<uint8_t>(valid), address<uint8_t>(restart), address<float>(carries),
@@ -196,9 +248,15 @@ struct GatedRecurrenceBackward final : torch::autograd::Node {
     std::string name() const override { return "GatedRecurrenceBackward"; }
 };
 
-std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor &projections, const OptionalTensor &initial,
-                                                     const OptionalTensor &valid, const OptionalTensor &restart,
+std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor &projections_, const OptionalTensor &initial_,
+                                                     const OptionalTensor &valid_, const OptionalTensor &restart_,
                                                      double low, double high) {
+    const Tensor projections = projections_.contiguous();  // differentiably
+    const OptionalTensor initial = dense(initial_), valid = dense(valid_), restart = dense(restart_);
+    if (projections.dim() == 3 && projections.size(1) == 0) {
+        check_forward(projections, initial, valid, restart, low, high);
+        return no_positions(projections, initial);
+    }
     if (at::GradMode::is_enabled() && (differentiates(projections) || differentiates(initial))) {
         auto node = node_of<GatedRecurrenceBackward>(projections, initial);
         Tensor states, final_state, carries;
@@ -227,8 +285,12 @@ using Route = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
 
 // ids, weights, counts, balance loss, and the loss's slope per probability
 Route route_learned_keep_cuda(const Tensor &logits, const OptionalTensor &valid, int64_t top_k, bool renormalize) {
-    const Launch launch(logits);
+    TORCH_CHECK_VALUE(one_of_ours(logits) && logits.dim() == 2 && logits.is_contiguous(),
+                      "logits must be contiguous [tokens, experts] in f32, bf16 or f16 on a CUDA device");
     const int64_t tokens = logits.size(0), experts = logits.size(1);
+    require("valid", valid, {tokens}, at::kBool, logits);
+    TORCH_CHECK_VALUE(1 <= top_k && top_k <= experts, "top_k must be in [1, experts]");
+    const Launch launch(logits);
     const auto ints = logits.options().dtype(at::kLong);
     Tensor ids = at::empty({tokens, top_k}, ints), weights = f32(logits, {tokens, top_k});
     Tensor counts = at::empty({experts}, ints), balance = f32(logits, {}), slope = f32(logits, {experts});
@@ -243,13 +305,21 @@ Route route_learned_keep_cuda(const Tensor &logits, const OptionalTensor &valid,
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> route_learned_cuda(const Tensor &logits, const OptionalTensor &valid,
                                                               int64_t top_k, bool renormalize) {
-    auto [ids, weights, counts, balance, slope] = route_learned_keep_cuda(logits, valid, top_k, renormalize);
+    auto [ids, weights, counts, balance, slope] = route_learned_keep_cuda(logits.contiguous(), dense(valid), top_k, renormalize);
     return {ids, weights, counts, balance};
 }
 
 Tensor route_learned_backward_cuda(const Tensor &logits, const Tensor &ids, const Tensor &weights, const Tensor &slope,
                                    const OptionalTensor &grad_weights, const OptionalTensor &grad_balance,
                                    bool renormalize) {
+    TORCH_CHECK_VALUE(one_of_ours(logits) && logits.dim() == 2 && logits.is_contiguous() && ids.dim() == 2,
+                      "logits must be contiguous [tokens, experts] in f32, bf16 or f16 on a CUDA device");
+    const int64_t pairs[] = {logits.size(0), ids.size(1)};
+    require("ids", ids, pairs, at::kLong, logits);
+    require("weights", weights, pairs, at::kFloat, logits);
+    require("slope", slope, {logits.size(1)}, at::kFloat, logits);
+    require("grad_weights", grad_weights, pairs, at::kFloat, logits);
+    require("grad_balance", grad_balance, {}, at::kFloat, logits);
     const Launch launch(logits);
     Tensor grad = at::empty_like(logits);
     check("koemi_moe_route_learned_backward",
@@ -280,8 +350,10 @@ struct RouteLearnedBackward final : torch::autograd::Node {
     std::string name() const override { return "RouteLearnedBackward"; }
 };
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> route_learned_autograd(const Tensor &logits, const OptionalTensor &valid,
+std::tuple<Tensor, Tensor, Tensor, Tensor> route_learned_autograd(const Tensor &logits_, const OptionalTensor &valid_,
                                                                   int64_t top_k, bool renormalize) {
+    const Tensor logits = logits_.contiguous();
+    const OptionalTensor valid = dense(valid_);
     if (at::GradMode::is_enabled() && differentiates(logits)) {
         auto node = node_of<RouteLearnedBackward>(logits);
         Tensor ids, weights, counts, balance, slope;
@@ -317,10 +389,31 @@ struct Rows {
     }
 };
 
+// Logits with the last dimension contiguous, the others as they are.
+Tensor readable(const Tensor &logits) {
+    return logits.dim() > 0 && logits.size(-1) > 1 && logits.stride(-1) != 1 ? logits.contiguous() : logits;
+}
+
+void check_policy(const Tensor &logits, const Tensor &targets, const OptionalTensor &valid) {
+    TORCH_CHECK_VALUE(one_of_ours(logits) && (logits.dim() == 2 || logits.dim() == 3) && logits.size(-1) > 0 &&
+                          (logits.size(-1) == 1 || logits.stride(-1) == 1),
+                      "logits must be [rows, vocabulary] or [batch, length, vocabulary] in f32, bf16 or f16 on a CUDA device");
+    const auto shape = logits.sizes().slice(0, logits.dim() - 1);
+    require("targets", targets, shape, at::kLong, logits);
+    require("valid", valid, shape, at::kBool, logits);
+}
+
 // loss, kl, log-probs, (log-sum-exps | slopes), gradient (undefined unless wanted)
 Route policy_forward(const Tensor &logits, const Tensor &targets, const Tensor &old, const Tensor &advantages,
                      const OptionalTensor &reference, const OptionalTensor &valid, double clip_low, double clip_high,
                      double kl_weight, bool with_gradient) {
+    check_policy(logits, targets, valid);
+    require("old", old, targets.sizes(), at::kFloat, logits);
+    require("advantages", advantages, targets.sizes(), at::kFloat, logits);
+    require("reference", reference, targets.sizes(), at::kFloat, logits);
+    TORCH_CHECK_VALUE(clip_low >= 0.0 && clip_high >= 0.0 && std::isfinite(kl_weight) &&
+                          (kl_weight == 0.0 || (reference.has_value() && reference->defined())),
+                      "clip widths must be non-negative, kl_weight finite and, without reference, zero");
     const Launch launch(logits);
     const Rows shape(logits);
     Tensor loss = f32(logits, {}), kl = f32(logits, {}), log_probs = f32(logits, targets.sizes());
@@ -343,8 +436,9 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_cuda(const Tensor &logits, const 
                                                     const Tensor &advantages, const OptionalTensor &reference,
                                                     const OptionalTensor &valid, double clip_low, double clip_high,
                                                     double kl_weight) {
-    auto [loss, kl, log_probs, kept, gradient] = policy_forward(logits, targets, old, advantages, reference, valid, clip_low,
-                                                                clip_high, kl_weight, false);
+    auto [loss, kl, log_probs, kept, gradient] =
+        policy_forward(readable(logits), targets.contiguous(), old.contiguous(), advantages.contiguous(), dense(reference),
+                       dense(valid), clip_low, clip_high, kl_weight, false);
     return {loss, kl, log_probs};
 }
 
@@ -359,8 +453,11 @@ Route policy_loss_keep_cuda(const Tensor &logits, const Tensor &targets, const T
 
 Tensor policy_loss_backward_cuda(const Tensor &logits, const Tensor &targets, const OptionalTensor &valid,
                                  const Tensor &kept, const Tensor &grad_loss) {
-    const Launch launch(logits);
+    check_policy(logits, targets, valid);
     const Rows shape(logits);
+    require("kept", kept, {2, shape.rows}, at::kFloat, logits);
+    require("grad_loss", grad_loss, {}, at::kFloat, logits);
+    const Launch launch(logits);
     Tensor grad = at::empty(logits.sizes(), logits.options());
     check("koemi_think_policy_loss_backward",
           lib().policy_backward(address<void>(logits), shape.rows, shape.vocab, shape.inner, shape.outer_stride,
@@ -371,6 +468,8 @@ Tensor policy_loss_backward_cuda(const Tensor &logits, const Tensor &targets, co
 }
 
 void policy_loss_scale_cuda(const Tensor &gradient, const Tensor &factor) {
+    TORCH_CHECK_VALUE(one_of_ours(gradient) && gradient.is_contiguous(), "gradient must be contiguous f32, bf16 or f16 on a CUDA device");
+    require("factor", factor, {}, at::kFloat, gradient);
     const Launch launch(gradient);
     check("koemi_think_policy_loss_scale", lib().policy_scale(address<void>(gradient), gradient.numel(), address<float>(factor),
                                                               code_of(gradient), launch.stream));
@@ -407,10 +506,13 @@ struct PolicyLossBackward final : torch::autograd::Node {
     std::string name() const override { return "PolicyLossBackward"; }
 };
 
-std::tuple<Tensor, Tensor, Tensor> policy_loss_autograd(const Tensor &logits, const Tensor &targets, const Tensor &old,
-                                                        const Tensor &advantages, const OptionalTensor &reference,
-                                                        const OptionalTensor &valid, double clip_low, double clip_high,
+std::tuple<Tensor, Tensor, Tensor> policy_loss_autograd(const Tensor &logits_, const Tensor &targets_, const Tensor &old_,
+                                                        const Tensor &advantages_, const OptionalTensor &reference_,
+                                                        const OptionalTensor &valid_, double clip_low, double clip_high,
                                                         double kl_weight) {
+    const Tensor logits = readable(logits_), targets = targets_.contiguous();
+    const Tensor old = old_.contiguous(), advantages = advantages_.contiguous();
+    const OptionalTensor reference = dense(reference_), valid = dense(valid_);
     if (at::GradMode::is_enabled() && differentiates(logits)) {
         auto node = node_of<PolicyLossBackward>(logits);
         Tensor loss, kl, log_probs, kept, gradient;

@@ -27,6 +27,11 @@ def load(device: torch.device) -> None:
     _native.ensure_device(device)
 
 
+def loaded() -> bool:
+    """Whether the ops are registered. They check their arguments and initialise their device themselves."""
+    return _loaded
+
+
 def _register_fakes() -> None:
     f32 = dict(dtype=torch.float32)
 

@@ -48,9 +48,9 @@ def _call(gradients: list, out: list | None, max_norm: float) -> Tensor:
     first = gradients[0] if gradients else None
     if not isinstance(first, Tensor) or not first.is_cuda:
         _explain(lists)
-    if not _training._loaded:
+    if not _training.loaded():
         load_cuda_extension(device=first.device)
-    _training.load(first.device)
+        _training.load(first.device)
     try:
         return _native.binding().koemi_torch_clip_gradients(gradients, out, max_norm)
     except (ValueError, TypeError, RuntimeError):

@@ -35,19 +35,18 @@ def gated_recurrence(projections: Tensor, initial: Tensor | None = None, *, vali
     and the returned final state are fp32. Differentiable to first order in
     ``projections`` and ``initial``; a single token is ``length == 1``.
     """
-    _validate(projections, initial, valid, restart, minimum_retention, maximum_retention)
+    if not _training.loaded():
+        _validate(projections, initial, valid, restart, minimum_retention, maximum_retention)
+        try:
+            _training.load(projections.device)
+        except _native.KoemiNativeUnavailableError as error:
+            raise DenseCudaBuildError(f"failed to load the native dense CUDA library: {error}") from error
     try:
-        _training.load(projections.device)
-    except _native.KoemiNativeUnavailableError as error:
-        raise DenseCudaBuildError(f"failed to load the native dense CUDA library: {error}") from error
-    projections = projections.contiguous()
-    initial, valid, restart = (None if t is None else t.contiguous() for t in (initial, valid, restart))
-    if projections.shape[1] == 0:
-        features = projections.shape[2] // 2
-        start = projections.new_zeros((projections.shape[0], features), dtype=torch.float32) if initial is None else initial.clone()
-        return projections[..., :features].contiguous(), start
-    return torch.ops.koemi_b200.gated_recurrence.default(projections, initial, valid, restart, minimum_retention,
-                                                         maximum_retention)
+        return torch.ops.koemi_b200.gated_recurrence.default(projections, initial, valid, restart, minimum_retention,
+                                                             maximum_retention)
+    except (ValueError, TypeError, RuntimeError):  # what the op refuses is explained here
+        _validate(projections, initial, valid, restart, minimum_retention, maximum_retention)
+        raise
 
 
 def _validate(projections, initial, valid, restart, low, high) -> None:

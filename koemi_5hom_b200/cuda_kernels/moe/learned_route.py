@@ -44,7 +44,24 @@ def route_learned_topk(gate_logits: Tensor, valid_mask: Tensor | None = None, *,
     ids -1, weights and gradient zero. A NaN logit is never preferred and makes
     its row's weights NaN. Differentiable to first order in the logits.
     """
-    from koemi_5hom_b200.cuda_kernels.moe import CudaMoeUnavailableError, CudaMoeValidationError  # the package imports this module
+    if not _training.loaded():
+        _validate(gate_logits, valid_mask, top_k)
+        try:
+            _training.load(gate_logits.device)
+        except _native.KoemiNativeUnavailableError as error:
+            from koemi_5hom_b200.cuda_kernels.moe import CudaMoeUnavailableError  # the package imports this module
+            raise CudaMoeUnavailableError(f"Koemi MoE CUDA library failed to load: {error}") from error
+    try:
+        if type(top_k) is not int:  # the dispatcher takes bools
+            raise TypeError("top_k must be an integer")
+        return LearnedRoute(*torch.ops.koemi_b200.route_learned.default(gate_logits, valid_mask, top_k, bool(renormalize)))
+    except (ValueError, TypeError, RuntimeError):  # what the op refuses is explained here
+        _validate(gate_logits, valid_mask, top_k)
+        raise
+
+
+def _validate(gate_logits, valid_mask, top_k) -> None:
+    from koemi_5hom_b200.cuda_kernels.moe import CudaMoeValidationError  # the package imports this module
 
     def fail(message: str) -> None:
         raise CudaMoeValidationError(message)
@@ -65,9 +82,3 @@ def route_learned_topk(gate_logits: Tensor, valid_mask: Tensor | None = None, *,
         fail("valid_mask must be boolean with shape [tokens]")
     if not gate_logits.is_cuda or (valid_mask is not None and valid_mask.device != gate_logits.device):
         fail("gate_logits and valid_mask must be CUDA tensors on one device")
-    try:
-        _training.load(gate_logits.device)
-    except _native.KoemiNativeUnavailableError as error:
-        raise CudaMoeUnavailableError(f"Koemi MoE CUDA library failed to load: {error}") from error
-    valid = None if valid_mask is None else valid_mask.contiguous()
-    return LearnedRoute(*torch.ops.koemi_b200.route_learned.default(gate_logits.contiguous(), valid, top_k, bool(renormalize)))

@@ -48,16 +48,18 @@ def policy_loss(logits: Tensor, target_ids: Tensor, old_log_probs: Tensor, advan
     Differentiable to first order in ``logits``; while gradients are enabled
     for f32 and bf16 logits the call allocates the logits' gradient.
     """
-    _validate(logits, target_ids, old_log_probs, advantages, reference_log_probs, valid_mask, clip_low, clip_high, kl_weight)
+    arguments = (logits, target_ids, old_log_probs, advantages, reference_log_probs, valid_mask, clip_low, clip_high, kl_weight)
+    if not _training.loaded():
+        _validate(*arguments)
+        try:
+            _training.load(logits.device)
+        except _native.KoemiNativeUnavailableError as error:
+            raise CudaThinkUnavailableError(str(error)) from error
     try:
-        _training.load(logits.device)
-    except _native.KoemiNativeUnavailableError as error:
-        raise CudaThinkUnavailableError(str(error)) from error
-    if logits.shape[-1] > 1 and logits.stride(-1) != 1:
-        logits = logits.contiguous()
-    others = (None if t is None else t.contiguous() for t in
-              (target_ids, old_log_probs, advantages, reference_log_probs, valid_mask))
-    return PolicyLoss(*torch.ops.koemi_b200.policy_loss.default(logits, *others, clip_low, clip_high, kl_weight))
+        return PolicyLoss(*torch.ops.koemi_b200.policy_loss.default(*arguments))
+    except (ValueError, TypeError, RuntimeError):  # what the op refuses is explained here
+        _validate(*arguments)
+        raise
 
 
 def _validate(logits, targets, old, advantages, reference, valid, clip_low, clip_high, kl_weight) -> None:

@@ -14,7 +14,7 @@ import pytest
 import torch
 
 from koemi_5hom_b200.cuda_kernels.core import clip_gradients, gradient_norm
-from koemi_5hom_b200.cuda_kernels.dense import gated_recurrence
+from koemi_5hom_b200.cuda_kernels.dense import DenseCudaValidationError, gated_recurrence
 from koemi_5hom_b200.cuda_kernels.moe import route_learned_topk
 from koemi_5hom_b200.cuda_kernels.think import policy_loss
 from oracle import training as plain
@@ -316,6 +316,58 @@ def test_recurrence_saved_tensors_are_guarded(cuda):
     got, = torch.autograd.grad(states.sum() + final.sum(), y)
     want, = torch.autograd.grad(2 * gated_recurrence(y, h0)[0].sum() + gated_recurrence(y, h0)[1].sum(), y)
     check(got, want.double(), torch.float32, 64 * EPS * 256)
+
+
+def test_recurrence_of_turned_tensors_and_no_positions(cuda):
+    """Strides are taken as they come, and gradients go back through them."""
+    x, h0, *_ = recurrence_case(3, 37, 24, torch.float32, 19, False, cuda)
+    turned, start = x.transpose(0, 1).contiguous().transpose(0, 1), h0.t().contiguous().t()
+    grads = []
+    for p, h in ((x, h0), (turned, start)):
+        p, h = p.detach().requires_grad_(True), h.detach().requires_grad_(True)
+        states, final = gated_recurrence(p, h)
+        grads.append((states, *torch.autograd.grad(states.square().sum() + final.sum(), (p, h))))
+    assert turned.stride() != x.stride() and all(torch.equal(a, b) for a, b in zip(*grads))
+    p, h = x[:, :0].requires_grad_(True), h0.clone().requires_grad_(True)
+    states, final = gated_recurrence(p, h)
+    assert states.shape == (3, 0, 24) and torch.equal(final, h)
+    final.sum().backward()
+    assert torch.equal(h.grad, torch.ones_like(h))
+    with pytest.raises(DenseCudaValidationError, match="initial must be float32"):
+        gated_recurrence(p, h[:2])
+
+
+def test_ops_refuse_what_the_kernels_cannot_take(cuda):
+    """The dispatcher ops check for themselves, whoever calls them."""
+    ops = torch.ops.koemi_b200
+    x = torch.zeros(2, 5, 8, device=cuda)
+    gated_recurrence(x)  # registers them
+    carries, mask = torch.zeros(2, 1, 4, device=cuda), torch.ones(2, 5, dtype=torch.bool, device=cuda)
+    logits, targets = torch.zeros(6, 9, device=cuda), torch.zeros(6, dtype=torch.int64, device=cuda)
+    rows, one = torch.zeros(6, device=cuda), torch.ones((), device=cuda)
+    pairs, ids = torch.zeros(6, 2, device=cuda), torch.zeros(6, 2, dtype=torch.int64, device=cuda)
+    for call in (lambda: ops.gated_recurrence(x, None, mask[:, :4], None, 0.1, 0.9),
+                 lambda: ops.gated_recurrence(x, None, None, mask[:1], 0.1, 0.9),
+                 lambda: ops.gated_recurrence(x, carries[:, 0, :3], None, None, 0.1, 0.9),
+                 lambda: ops.gated_recurrence(x, None, None, None, 0.9, 0.1),
+                 lambda: ops.gated_recurrence(x.cpu(), carries[:, 0], None, None, 0.1, 0.9),
+                 lambda: ops.gated_recurrence_keep(x.transpose(0, 1), None, None, None, 0.1, 0.9),
+                 lambda: ops.gated_recurrence_keep(x[:, :0], None, None, None, 0.1, 0.9),
+                 lambda: ops.gated_recurrence_backward(x, None, None, carries[:, :0], None, None, 0.1, 0.9),
+                 lambda: ops.gated_recurrence_backward(x, None, None, carries, x, None, 0.1, 0.9),
+                 lambda: ops.route_learned(logits, None, 10, False),
+                 lambda: ops.route_learned(logits, mask[0], 1, False),
+                 lambda: ops.route_learned_backward(logits, ids, pairs[:5], rows[:5], None, None, False),
+                 lambda: ops.route_learned_backward(logits, ids, pairs, rows, None, None, False),
+                 lambda: ops.policy_loss(logits, targets[:5], rows, rows, None, None, 0.2, 0.2, 0.0),
+                 lambda: ops.policy_loss(logits, targets, rows[:5], rows, None, None, 0.2, 0.2, 0.0),
+                 lambda: ops.policy_loss(logits, targets, rows, rows, None, None, 0.2, 0.2, 1.0),
+                 lambda: ops.policy_loss(logits, targets, rows, rows, rows.double(), None, 0.2, 0.2, 0.0),
+                 lambda: ops.policy_loss(logits, targets, rows, rows, None, None, -0.2, 0.2, 0.0),
+                 lambda: ops.policy_loss_backward(logits, targets, None, pairs, one),
+                 lambda: ops.policy_loss_scale(logits, rows)):
+        with pytest.raises(ValueError):
+            call()
 
 
 # ------------------------------------------------------------ the learned route
