@@ -85,19 +85,19 @@ __device__ __forceinline__ float rcp_approx(float x) {
     return r;
 }
 
-// a and k of one element. With yp = 1 + e^-p and yc = 1 + e^2c, s = 1 / yp and
+// s and k of one element. With yp = 1 + e^-p and yc = 1 + e^2c, s = 1 / yp and
 // k = 1 - 2 / yc share one reciprocal, of yp yc; the exponents stop at 40,
 // where both have reached their limits in fp32, so that the product stays
 // finite. Both are good to a few 2^-24 of 1. For 16-bit inputs that is far
 // below the inputs' own rounding; fp32 inputs near 0 take tanh's series
 // instead (good to 2^-24 of k up to |c| = 1/4), since k is as small as c there.
 template <typename T>
-__device__ __forceinline__ void gate_of(float p, float c, float lo, float span, float &a, float &k) {
+__device__ __forceinline__ void gate_of(float p, float c, float &s, float &k) {
     constexpr float kLog2e = 1.4426950408889634f;
     const float yp = 1.0f + ex2_approx(min_nan(-kLog2e * p, 40.0f * kLog2e));
     const float yc = 1.0f + ex2_approx(min_nan(2.0f * kLog2e * c, 40.0f * kLog2e));
     const float r = rcp_approx(yp * yc);
-    a = fmaf(span, r * yc, lo);
+    s = r * yc;
     k = fmaf(-2.0f, r * yp, 1.0f);
     if constexpr (sizeof(T) == 4) {
         const float z = c * c;
@@ -126,10 +126,10 @@ __global__ void gated_forward_lane_kernel(GatedShape shape, const T *__restrict_
         const int64_t row = b * shape.length + t;
         if (shape.restart != nullptr && shape.restart[row]) h = 0.0f;
         if (shape.valid == nullptr || shape.valid[row]) {
-            float a, k;
+            float s, k;
             gate_of<T>(to_acc(projections[row * 2 * shape.features + f]),
-                       to_acc(projections[row * 2 * shape.features + shape.features + f]), shape.lo,
-                       shape.hi - shape.lo, a, k);
+                       to_acc(projections[row * 2 * shape.features + shape.features + f]), s, k);
+            const float a = fmaf(shape.hi - shape.lo, s, shape.lo);
             h = fmaf(a, h, fmaf(-a, k, k));
         }
         states[row * shape.features + f] = from_acc<T>(h);
@@ -146,7 +146,7 @@ __global__ void gated_backward_lane_kernel(GatedShape shape, const T *__restrict
     if (lane >= shape.batch * shape.features) return;
     const int64_t b = lane / shape.features, f = lane - b * shape.features;
     const float span = shape.hi - shape.lo;
-    float a[kShortLength], k[kShortLength], before[kShortLength];
+    float s[kShortLength], k[kShortLength], before[kShortLength];
     uint32_t live = 0, cut = 0;
     float h = carries[lane];
 #pragma unroll
@@ -161,8 +161,9 @@ __global__ void gated_backward_lane_kernel(GatedShape shape, const T *__restrict
         if (shape.valid == nullptr || shape.valid[row]) {
             live |= 1u << t;
             gate_of<T>(to_acc(projections[row * 2 * shape.features + f]),
-                       to_acc(projections[row * 2 * shape.features + shape.features + f]), shape.lo, span, a[t], k[t]);
-            h = fmaf(a[t], h, fmaf(-a[t], k[t], k[t]));
+                       to_acc(projections[row * 2 * shape.features + shape.features + f]), s[t], k[t]);
+            const float a = fmaf(span, s[t], shape.lo);
+            h = fmaf(a, h, fmaf(-a, k[t], k[t]));
         }
     }
     float x = grad_final != nullptr ? grad_final[lane] : 0.0f;
@@ -174,9 +175,11 @@ __global__ void gated_backward_lane_kernel(GatedShape shape, const T *__restrict
         float dp = 0.0f, dc = 0.0f;
         x = adjoint;
         if (live >> t & 1u) {
-            dp = adjoint * (before[t] - k[t]) * ((a[t] - shape.lo) * (shape.hi - a[t]) / span);
-            dc = adjoint * (1.0f - a[t]) * fmaf(-k[t], k[t], 1.0f);
-            x = a[t] * adjoint;
+            // the gate's slope from s: read back from a it would lose digits under narrow bounds, and be 0 / 0 under equal ones
+            const float a = fmaf(span, s[t], shape.lo);
+            dp = adjoint * (before[t] - k[t]) * (span * s[t] * (1.0f - s[t]));
+            dc = adjoint * (1.0f - a) * fmaf(-k[t], k[t], 1.0f);
+            x = a * adjoint;
         }
         if (cut >> t & 1u) x = 0.0f;
         grad_projections[row * 2 * shape.features + f] = from_acc<T>(dp);

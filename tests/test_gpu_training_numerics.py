@@ -1,0 +1,114 @@
+"""The training operators' results entry by entry against 64-bit forms, with bounds carried through the formulas.
+
+A result of type T may be off by its own rounding, U[T] relative, plus what the
+fp32 arithmetic in front of it loses. The losses are counted in roundings (EPS =
+2^-24) of the terms that the formula adds up at that very entry, so that a small
+gradient is held to a small error.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from koemi_5hom_b200.cuda_kernels.dense import gated_recurrence
+from koemi_5hom_b200.cuda_kernels.think import policy_loss
+from oracle import training as plain
+
+pytestmark = pytest.mark.gpu
+
+EPS = 2.0 ** -24
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25}  # fp16: half the subnormal spacing
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def check(got, exact, allowed):
+    """|got - exact| <= U |exact| + allowed, elementwise (allowed: a tensor of the results' shape, or a number)."""
+    dtype, got, exact = got.dtype, got.detach().double(), exact.detach().double()
+    over = (got - exact).abs() - (U[dtype] * 1.0001 * exact.abs() + allowed + TINY[dtype])
+    assert got.shape == exact.shape and not got.isnan().any()
+    assert not got.numel() or over.max().item() <= 0, f"off by {over.max().item()} more than allowed"
+
+
+# ------------------------------------------------------- the gated recurrence
+
+def recurrence_with_bounds(x, h0, gs, gf, valid=None, restart=None, low=plain.LOW, high=plain.HIGH):
+    """64-bit (states, final, gradient of x, gradient of h0), and what fp32 may lose of each, position by position.
+
+    a and k: ex2, rcp and four products, at most 16 roundings of s and of 1. A
+    step adds a's and k's losses and three roundings of its terms to a times the
+    loss so far; the walks over tiles round the same terms once more: all
+    counted twice. The adjoint likewise, with |g| in place of g.
+    """
+    x, h0, gs, gf = x.double(), h0.double(), gs.double(), gf.double()
+    features = x.shape[2] // 2
+    p, c = x[..., :features], x[..., features:]
+    span = high - low
+    s, k = torch.sigmoid(p), torch.tanh(c)
+    a = low + span * s
+    live = torch.ones_like(a, dtype=torch.bool) if valid is None else valid[..., None].expand_as(a)
+    cut = torch.zeros_like(live) if restart is None else restart[..., None].expand_as(a)
+    keep = torch.where(live, a, 1.0)
+    a_lost, k_lost = 16 * EPS * span * s + 2 * EPS * a, torch.full_like(k, 16 * EPS)
+    h, lost = h0, torch.zeros_like(h0)
+    states, states_lost, before, before_lost = [], [], [], []
+    for t in range(x.shape[1]):
+        h, lost = torch.where(cut[:, t], 0.0, h), torch.where(cut[:, t], 0.0, lost)
+        before.append(h)
+        before_lost.append(lost)
+        size = h.abs() + k[:, t].abs()
+        step = 2 * (a_lost[:, t] * size + (1 - a[:, t]) * k_lost[:, t] + 5 * EPS * size)
+        lost = torch.where(live[:, t], a[:, t] * lost + step, lost)
+        h = torch.where(live[:, t], a[:, t] * h + (1 - a[:, t]) * k[:, t], h)
+        states.append(h)
+        states_lost.append(lost)
+    back, size, lost = gf, gf.abs(), torch.zeros_like(gf)
+    dx, dx_lost = torch.zeros_like(x), torch.zeros_like(x)
+    for t in range(x.shape[1] - 1, -1, -1):
+        adjoint, size = gs[:, t] + back, gs[:, t].abs() + size
+        lost = lost + 6 * EPS * size
+        gap, gap_lost = before[t] - k[:, t], before_lost[t] + k_lost[:, t] + 2 * EPS * (before[t].abs() + k[:, t].abs())
+        slope = span * s[:, t] * (1 - s[:, t])
+        slope_lost = 20 * EPS * span * s[:, t]
+        dp, dc = adjoint * gap * slope, adjoint * (1 - a[:, t]) * (1 - k[:, t] ** 2)
+        dp_lost = lost * gap.abs() * slope + adjoint.abs() * (gap_lost * slope + gap.abs() * slope_lost)
+        dc_lost = lost * (1 - a[:, t]) + adjoint.abs() * (a_lost[:, t] + 2 * EPS + (1 - a[:, t]) * 2 * (k_lost[:, t] + 2 * EPS))
+        for part, exact, off in ((slice(0, features), dp, dp_lost), (slice(features, None), dc, dc_lost)):
+            dx[:, t, part] = torch.where(live[:, t], exact, 0.0)
+            dx_lost[:, t, part] = torch.where(live[:, t], off + 8 * EPS * exact.abs(), 0.0)
+        lost = torch.where(cut[:, t], 0.0, keep[:, t] * lost + torch.where(live[:, t], 2 * a_lost[:, t] * size, 0.0))
+        back, size = torch.where(cut[:, t], 0.0, keep[:, t] * adjoint), torch.where(cut[:, t], 0.0, keep[:, t] * size)
+    stack = lambda rows: torch.stack(rows, 1)  # noqa: E731
+    return ((stack(states), stack(states_lost)), (h, states_lost[-1]), (dx, dx_lost), (back, lost + 6 * EPS * size))
+
+
+def check_recurrence(x, h0, gs, gf, valid=None, restart=None, low=plain.LOW, high=plain.HIGH):
+    xg, hg = x.clone().requires_grad_(True), h0.clone().requires_grad_(True)
+    states, final = gated_recurrence(xg, hg, valid=valid, restart=restart, minimum_retention=low, maximum_retention=high)
+    got = (states, final, *torch.autograd.grad((states, final), (xg, hg), (gs, gf)))
+    for result, (exact, lost) in zip(got, recurrence_with_bounds(x, h0, gs, gf, valid, restart, low, high)):
+        check(result, exact, lost)
+
+
+def recurrence_case(batch, length, features, dtype, seed, masks, cuda):
+    g = torch.Generator().manual_seed(seed)
+    x = (1.5 * torch.randn(batch, length, 2 * features, generator=g)).to(dtype).to(cuda)
+    h0 = torch.randn(batch, features, generator=g).tanh().to(cuda)
+    gs, gf = torch.randn(batch, length, features, generator=g).to(dtype).to(cuda), torch.randn(batch, features, generator=g).to(cuda)
+    valid = (torch.rand(batch, length, generator=g) < 0.8).to(cuda) if masks else None
+    restart = (torch.rand(batch, length, generator=g) < 0.05).to(cuda) if masks else None
+    return x, h0, gs, gf, valid, restart
+
+
+# exact in fp32, so that the kernel's bounds are the formula's
+RETENTIONS = [(0.5, 0.5), (0.5, 0.5 + 2.0 ** -10), (0.875, 0.9375)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length", [1, 16, 17, 300])
+@pytest.mark.parametrize("low,high", RETENTIONS)
+def test_recurrence_of_equal_and_narrow_retention_bounds(low, high, length, dtype, cuda):
+    """Equal bounds: a is the bound and dp is 0. Narrow ones: the slope (hi - lo) s (1 - s) keeps its digits."""
+    check_recurrence(*recurrence_case(3, length, 72, dtype, length, False, cuda), low=low, high=high)
