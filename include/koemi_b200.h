@@ -775,9 +775,14 @@ KOEMI_API int koemi_moe_route_learned_backward(const void *logits, const int64_t
  *          1 + clip_high) A) + kl_weight (exp(d) - d - 1),
  *   kl = mean of exp(d) - d - 1 (0 with reference_log_probs NULL).
  * log_probs [rows] is 0 on rows that are not valid and NaN where a target is
- * outside [0, vocab). lse and slopes [rows] are kept for the backward.
+ * outside [0, vocab). lse and slopes [rows] are kept for the backward. With
+ * KOEMI_POLICY_SUMS added to dtype, in both calls, lse is [2 * rows]: the rows'
+ * maxima, then their sums of exp(l - maximum), from which the backward's
+ * softmax is as good as the forward's; from the log-sum-exps alone it is off by
+ * their rounding, 2^-24 of the logits' magnitude.
  * grad_logits ([rows, vocab], dtype, contiguous, 16-byte aligned; NULL: not
  * wanted) receives d loss / d logits in the same pass. */
+#define KOEMI_POLICY_SUMS 0x100
 KOEMI_API size_t koemi_think_policy_loss_workspace(void);
 KOEMI_API int koemi_think_policy_loss_forward(const void *logits, int64_t rows, int64_t vocab, int64_t inner_rows,
                                               int64_t outer_stride, int64_t inner_stride, const int64_t *targets,

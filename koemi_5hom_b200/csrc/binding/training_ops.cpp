@@ -403,7 +403,7 @@ void check_policy(const Tensor &logits, const Tensor &targets, const OptionalTen
     require("valid", valid, shape, at::kBool, logits);
 }
 
-// loss, kl, log-probs, (log-sum-exps | slopes), gradient (undefined unless wanted)
+// loss, kl, log-probs, (maxima | sums | slopes), gradient (undefined unless wanted)
 Route policy_forward(const Tensor &logits, const Tensor &targets, const Tensor &old, const Tensor &advantages,
                      const OptionalTensor &reference, const OptionalTensor &valid, double clip_low, double clip_high,
                      double kl_weight, bool with_gradient) {
@@ -417,7 +417,7 @@ Route policy_forward(const Tensor &logits, const Tensor &targets, const Tensor &
     const Launch launch(logits);
     const Rows shape(logits);
     Tensor loss = f32(logits, {}), kl = f32(logits, {}), log_probs = f32(logits, targets.sizes());
-    Tensor kept = f32(logits, {2, shape.rows}), gradient;
+    Tensor kept = f32(logits, {3, shape.rows}), gradient;
     if (with_gradient) gradient = at::empty(logits.sizes(), logits.options());
     const int64_t size = static_cast<int64_t>(lib().policy_workspace());
     Tensor workspace = at::empty({size}, logits.options().dtype(at::kByte));
@@ -426,8 +426,8 @@ Route policy_forward(const Tensor &logits, const Tensor &targets, const Tensor &
                                shape.inner_stride, address<int64_t>(targets), address<float>(old), address<float>(advantages),
                                address<float>(reference), address<uint8_t>(valid), static_cast<float>(clip_low),
                                static_cast<float>(clip_high), static_cast<float>(kl_weight), address<float>(loss),
-                               address<float>(kl), address<float>(log_probs), address<float>(kept), address<float>(kept) + shape.rows,
-                               with_gradient ? address<void>(gradient) : nullptr, code_of(logits), address<void>(workspace), size,
+                               address<float>(kl), address<float>(log_probs), address<float>(kept), address<float>(kept) + 2 * shape.rows,
+                               with_gradient ? address<void>(gradient) : nullptr, code_of(logits) | KOEMI_POLICY_SUMS, address<void>(workspace), size,
                                launch.stream));
     return {loss, kl, log_probs, kept, gradient};
 }
@@ -455,14 +455,15 @@ Tensor policy_loss_backward_cuda(const Tensor &logits, const Tensor &targets, co
                                  const Tensor &kept, const Tensor &grad_loss) {
     check_policy(logits, targets, valid);
     const Rows shape(logits);
-    require("kept", kept, {2, shape.rows}, at::kFloat, logits);
+    require("kept", kept, {3, shape.rows}, at::kFloat, logits);
     require("grad_loss", grad_loss, {}, at::kFloat, logits);
     const Launch launch(logits);
     Tensor grad = at::empty(logits.sizes(), logits.options());
     check("koemi_think_policy_loss_backward",
           lib().policy_backward(address<void>(logits), shape.rows, shape.vocab, shape.inner, shape.outer_stride,
                                 shape.inner_stride, address<int64_t>(targets), address<uint8_t>(valid), address<float>(kept),
-                                address<float>(kept) + shape.rows, address<float>(grad_loss), address<void>(grad), code_of(logits),
+                                address<float>(kept) + 2 * shape.rows, address<float>(grad_loss), address<void>(grad),
+                                code_of(logits) | KOEMI_POLICY_SUMS,
                                 launch.stream));
     return grad;
 }

@@ -150,11 +150,24 @@ __device__ __forceinline__ Partial warp_merge(Partial p) {
 }
 __device__ __forceinline__ float lse_of(Partial p) { return p.max + logf(p.sum); }
 
-// What a forward kernel writes beside the gradient.
+// What a forward kernel writes beside the gradient. For the backward a row
+// leaves its maximum and its sum, which give the same softmax as the forward's;
+// with sums NULL only its log-sum-exp, which rounds at the logits' magnitude:
+// near 1e6 its probabilities are 2% off, and a row of the type's lowest value,
+// which absorbs the logarithm, gets 1 in every entry for 1 / vocab.
 struct PolicyOut {
     const float *inverse;  // NULL: the CTA counts the valid rows
-    float *log_probs, *lse, *slopes;
+    float *log_probs, *lse, *sums, *slopes;  // lse: the maxima where sums is given
     double2 *partials;
+    __device__ __forceinline__ void keep(int64_t index, Partial p, float slope) const {
+        lse[index] = sums != nullptr ? p.max : lse_of(p);
+        if (sums != nullptr) sums[index] = p.sum;
+        slopes[index] = slope;
+    }
+    __device__ __forceinline__ void skip(int64_t index) const {
+        log_probs[index] = 0.0f;
+        keep(index, Partial{0.0f, 1.0f}, 0.0f);
+    }
 };
 
 // A row's scalars, and what follows from its log-sum-exp: every thread takes
@@ -195,12 +208,11 @@ struct RowScalars : RowTerms {
         }
     }
     // the row's results, by one thread
-    __device__ void finish(const PolicyTerms &terms, const PolicyOut &out, int64_t index, float lp, float lse,
+    __device__ void finish(const PolicyTerms &terms, const PolicyOut &out, int64_t index, float lp, Partial p,
                            float scaled_slope, double &loss, double &kl) const {
         add_loss(terms, lp, loss, kl);
         out.log_probs[index] = lp;
-        out.lse[index] = lse;
-        out.slopes[index] = scaled_slope;
+        out.keep(index, p, scaled_slope);
     }
 };
 
@@ -220,7 +232,7 @@ __global__ __launch_bounds__(256) void policy_warp_kernel(PolicyRows shape, Poli
             if (out != nullptr) {
                 for (int v = lane; v < vocab; v += 32) out[v] = from_acc<T>(0.0f);
             }
-            if (lane == 0) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
+            if (lane == 0) result.skip(row);
             continue;
         }
         const T *in = logits + shape.start(row);
@@ -247,8 +259,8 @@ __global__ __launch_bounds__(256) void policy_warp_kernel(PolicyRows shape, Poli
             p.sum += e[j];
         }
         p.sum = warp_sum(p.sum);
-        const float lse = lse_of(p), lp = scalars.log_prob(p), slope = scalars.slope(terms, lp) * scale;
-        if (lane == 0) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
+        const float lp = scalars.log_prob(p), slope = scalars.slope(terms, lp) * scale;
+        if (lane == 0) scalars.finish(terms, result, row, lp, p, slope, loss_sum, kl_sum);
         if (out != nullptr) {
             const float factor = -slope / p.sum;
 #pragma unroll
@@ -490,7 +502,7 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
         T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
         if (!row_terms.valid()) {
             if (out != nullptr) clear_row(out, vocab, first, last_slice ? 0 : slice);
-            if (threadIdx.x == kThreads - 1 && rank == 0) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
+            if (threadIdx.x == kThreads - 1 && rank == 0) result.skip(row);
             continue;
         }
         const T *in = logits + (kExact ? 0 : shape.start(row));
@@ -584,8 +596,8 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
         ++taken;
 
         const RowScalars scalars(row_terms, chosen);
-        const float lse = lse_of(all), lp = scalars.log_prob(all), slope = scalars.slope(terms, lp) * scale;
-        if (threadIdx.x == kThreads - 1 && rank == 0) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
+        const float lp = scalars.log_prob(all), slope = scalars.slope(terms, lp) * scale;
+        if (threadIdx.x == kThreads - 1 && rank == 0) scalars.finish(terms, result, row, lp, all, slope, loss_sum, kl_sum);
         if (out != nullptr) {
             // of an fp32 warp with nothing but -inf: 0
             const float factor = -__fdividef(slope, all.sum) * (sizeof(T) == 4 ? exp_from(p.max, all.max) : 1.0f);
@@ -653,7 +665,7 @@ __global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows sh
         const RowTerms row_terms = load_terms(terms, row, vocab);
         if (!row_terms.valid()) {
             if (out != nullptr) clear_row(out, vocab);
-            if (threadIdx.x == 0) result.log_probs[row] = result.lse[row] = result.slopes[row] = 0.0f;
+            if (threadIdx.x == 0) result.skip(row);
             continue;
         }
         const T *in = logits + shape.start(row);
@@ -693,8 +705,8 @@ __global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows sh
             for (int i = 0; i < kWidth; ++i) p.sum += exp_from(v[i], from);
         });
         const Partial all = block_merge<kWalkThreads>(warp_merge(p), merged, taken++ & 1);
-        const float lse = lse_of(all), lp = scalars.log_prob(all), slope = scalars.slope(terms, lp) * scale;
-        if (threadIdx.x == 0) scalars.finish(terms, result, row, lp, lse, slope, loss_sum, kl_sum);
+        const float lp = scalars.log_prob(all), slope = scalars.slope(terms, lp) * scale;
+        if (threadIdx.x == 0) scalars.finish(terms, result, row, lp, all, slope, loss_sum, kl_sum);
         if (out != nullptr) {
             const float factor = -slope / all.sum;
             const bool fits = packets.fits(out);
@@ -745,14 +757,14 @@ __global__ __launch_bounds__(kFinishThreads) void policy_finish_kernel(const dou
     }
 }
 
-// The gradient from the kept log-sum-exps: a CTA takes a row's packets (or,
+// The gradient from what the forward kept of its rows: a CTA takes a row's packets (or,
 // grid.y > 1, every grid.y-th run of them).
 constexpr int kBackwardThreads = 256;
 template <typename T>
 __global__ __launch_bounds__(kBackwardThreads) void policy_backward_kernel(
     PolicyRows shape, const T *__restrict__ logits, const int64_t *__restrict__ targets,
-    const uint8_t *__restrict__ valid, const float *__restrict__ lse, const float *__restrict__ slopes,
-    const float *__restrict__ grad_loss, T *__restrict__ grad_logits) {
+    const uint8_t *__restrict__ valid, const float *__restrict__ lse, const float *__restrict__ sums,
+    const float *__restrict__ slopes, const float *__restrict__ grad_loss, T *__restrict__ grad_logits) {
     constexpr int kWidth = Pack<T>::kWidth, kPackets = 4;
     const float scale = *grad_loss;
     const int vocab = static_cast<int>(shape.vocab), step = static_cast<int>(gridDim.y) * kBackwardThreads * kPackets;
@@ -765,7 +777,7 @@ __global__ __launch_bounds__(kBackwardThreads) void policy_backward_kernel(
         }
         const Packets<T> packets(in, vocab);
         const bool fits = packets.fits(out);
-        const float slope = slopes[row] * scale, from = lse[row];
+        const float slope = slopes[row] * scale, from = lse[row], factor = sums != nullptr ? -slope / sums[row] : -slope;
         const int64_t target = targets[row];
         const int at = static_cast<int>(target) + packets.skip, packet = target >= 0 && target < vocab ? at / kWidth : -1;
         for (int first = blockIdx.y * kBackwardThreads * kPackets + threadIdx.x; first < packets.count; first += step) {
@@ -786,7 +798,7 @@ __global__ __launch_bounds__(kBackwardThreads) void policy_backward_kernel(
                     packets.load_partly(c, v);
                 }
 #pragma unroll
-                for (int i = 0; i < kWidth; ++i) v[i] = -slope * exp_from(v[i], from);
+                for (int i = 0; i < kWidth; ++i) v[i] = exp_from(v[i], from) * factor;
                 if (packet == c) {
 #pragma unroll
                     for (int i = 0; i < kWidth; ++i) v[i] += at % kWidth == i ? slope : 0.0f;
@@ -816,6 +828,13 @@ __global__ __launch_bounds__(256) void policy_scale_kernel(T *__restrict__ grad,
         T *tail = grad + packets * kWidth + thread;
         *tail = from_acc<T>(to_acc(*tail) * f);
     }
+}
+
+// Takes the flag out of a dtype; the sums behind `lse`, or NULL.
+float *sums_of(int &dtype, float *lse, int64_t rows) {
+    const bool given = (dtype & KOEMI_POLICY_SUMS) != 0;
+    dtype &= ~KOEMI_POLICY_SUMS;
+    return given && lse != nullptr ? lse + rows : nullptr;
 }
 
 PolicyRows rows_of(int64_t rows, int64_t vocab, int64_t inner_rows, int64_t outer_stride, int64_t inner_stride) {
@@ -900,10 +919,10 @@ int launch_warps(const PolicyRows &shape, const PolicyTerms &terms, const T *log
 
 template <typename T>
 int policy_forward(const PolicyRows &shape, const PolicyTerms &terms, const void *logits, float *loss, float *kl,
-                   float *log_probs, float *lse, float *slopes, void *grad_logits, void *workspace,
+                   float *log_probs, float *lse, float *sums, float *slopes, void *grad_logits, void *workspace,
                    cudaStream_t stream) {
     float *inverse = static_cast<float *>(workspace);
-    PolicyOut result{nullptr, log_probs, lse, slopes, reinterpret_cast<double2 *>(static_cast<unsigned char *>(workspace) + 256)};
+    PolicyOut result{nullptr, log_probs, lse, sums, slopes, reinterpret_cast<double2 *>(static_cast<unsigned char *>(workspace) + 256)};
     const T *in = static_cast<const T *>(logits);
     T *grad = static_cast<T *>(grad_logits);
     unsigned blocks = 0;
@@ -946,7 +965,7 @@ int policy_forward(const PolicyRows &shape, const PolicyTerms &terms, const void
 
 template <typename T>
 int policy_backward(const PolicyRows &shape, const void *logits, const int64_t *targets, const uint8_t *valid,
-                    const float *lse, const float *slopes, const float *grad_loss, void *grad_logits,
+                    const float *lse, const float *sums, const float *slopes, const float *grad_loss, void *grad_logits,
                     cudaStream_t stream) {
     // few long rows: several CTAs a row
     const int64_t runs = ceil_div(shape.vocab, kBackwardThreads * 4 * Pack<T>::kWidth), places = 8 * int64_t(sm_count());
@@ -954,7 +973,7 @@ int policy_backward(const PolicyRows &shape, const void *logits, const int64_t *
     int64_t y = ceil_div(places, x);
     if (y > runs) y = runs;
     policy_backward_kernel<T><<<dim3(x, static_cast<unsigned>(y)), kBackwardThreads, 0, stream>>>(
-        shape, static_cast<const T *>(logits), targets, valid, lse, slopes, grad_loss, static_cast<T *>(grad_logits));
+        shape, static_cast<const T *>(logits), targets, valid, lse, sums, slopes, grad_loss, static_cast<T *>(grad_logits));
     KOEMI_LAUNCH_CHECK();
     return KOEMI_OK;
 }
@@ -997,11 +1016,12 @@ extern "C" int koemi_think_policy_loss_forward(const void *logits, int64_t rows,
         return fail(KOEMI_ERR_WORKSPACE, "the policy loss's workspace is smaller than koemi_think_policy_loss_workspace()");
     }
     const PolicyTerms terms{targets, old_log_probs, advantages, reference_log_probs, valid, clip_low, clip_high, kl_weight};
+    float *sums = sums_of(dtype, lse, rows);
     cudaStream_t s = as_stream(stream);
     switch (dtype) {
-        case KOEMI_F32: return policy_forward<float>(shape, terms, logits, loss, kl, log_probs, lse, slopes, grad_logits, workspace, s);
-        case KOEMI_F16: return policy_forward<__half>(shape, terms, logits, loss, kl, log_probs, lse, slopes, grad_logits, workspace, s);
-        case KOEMI_BF16: return policy_forward<__nv_bfloat16>(shape, terms, logits, loss, kl, log_probs, lse, slopes, grad_logits, workspace, s);
+        case KOEMI_F32: return policy_forward<float>(shape, terms, logits, loss, kl, log_probs, lse, sums, slopes, grad_logits, workspace, s);
+        case KOEMI_F16: return policy_forward<__half>(shape, terms, logits, loss, kl, log_probs, lse, sums, slopes, grad_logits, workspace, s);
+        case KOEMI_BF16: return policy_forward<__nv_bfloat16>(shape, terms, logits, loss, kl, log_probs, lse, sums, slopes, grad_logits, workspace, s);
         default: return fail(KOEMI_ERR_INVALID, "unsupported policy loss dtype %d", dtype);
     }
 }
@@ -1020,11 +1040,12 @@ extern "C" int koemi_think_policy_loss_backward(const void *logits, int64_t rows
         return fail(KOEMI_ERR_INVALID, "policy loss backward tensors must be non-NULL");
     }
     if (!aligned(grad_logits, 16)) return fail(KOEMI_ERR_INVALID, "grad_logits must be 16-byte aligned");
+    const float *sums = sums_of(dtype, const_cast<float *>(lse), rows);
     cudaStream_t s = as_stream(stream);
     switch (dtype) {
-        case KOEMI_F32: return policy_backward<float>(shape, logits, targets, valid, lse, slopes, grad_loss, grad_logits, s);
-        case KOEMI_F16: return policy_backward<__half>(shape, logits, targets, valid, lse, slopes, grad_loss, grad_logits, s);
-        case KOEMI_BF16: return policy_backward<__nv_bfloat16>(shape, logits, targets, valid, lse, slopes, grad_loss, grad_logits, s);
+        case KOEMI_F32: return policy_backward<float>(shape, logits, targets, valid, lse, sums, slopes, grad_loss, grad_logits, s);
+        case KOEMI_F16: return policy_backward<__half>(shape, logits, targets, valid, lse, sums, slopes, grad_loss, grad_logits, s);
+        case KOEMI_BF16: return policy_backward<__nv_bfloat16>(shape, logits, targets, valid, lse, sums, slopes, grad_loss, grad_logits, s);
         default: return fail(KOEMI_ERR_INVALID, "unsupported policy loss dtype %d", dtype);
     }
 }

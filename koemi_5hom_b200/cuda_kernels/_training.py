@@ -82,7 +82,7 @@ def _register_fakes() -> None:
     def _(logits, targets, old, advantages, reference, valid, clip_low, clip_high, kl_weight):
         rows = logits.numel() // logits.shape[-1]
         at_once = logits.dtype != torch.float16
-        return (*policy(logits), logits.new_empty((2, rows), **f32), logits.new_empty(logits.shape if at_once else (0,)))
+        return (*policy(logits), logits.new_empty((3, rows), **f32), logits.new_empty(logits.shape if at_once else (0,)))
 
     @fake("policy_loss_backward")
     def _(logits, targets, valid, kept, grad_loss):

@@ -4,7 +4,7 @@
 the clipped surrogate loss, the mean KL estimate and the tokens' log-probs.
 The gradient with respect to the logits is formed in the forward's own pass,
 while a row is on chip (f32, bf16); f16 gradients, which underflow before the
-factor of a scaled loss, are formed in the backward from the kept log-sum-exps.
+factor of a scaled loss, are formed in the backward from the rows' kept maxima and sums.
 """
 from __future__ import annotations
 

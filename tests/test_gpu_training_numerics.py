@@ -12,6 +12,7 @@ import math
 import pytest
 import torch
 
+from koemi_5hom_b200 import _native
 from koemi_5hom_b200.cuda_kernels.dense import gated_recurrence
 from koemi_5hom_b200.cuda_kernels.think import policy_loss
 from oracle import training as plain
@@ -112,3 +113,117 @@ RETENTIONS = [(0.5, 0.5), (0.5, 0.5 + 2.0 ** -10), (0.875, 0.9375)]
 def test_recurrence_of_equal_and_narrow_retention_bounds(low, high, length, dtype, cuda):
     """Equal bounds: a is the bound and dp is 0. Narrow ones: the slope (hi - lo) s (1 - s) keeps its digits."""
     check_recurrence(*recurrence_case(3, length, 72, dtype, length, False, cuda), low=low, high=high)
+
+
+# ------------------------------------------------------------- the policy loss
+
+CLIP_LOW, CLIP_HIGH, BETA = 0.2, 0.3, 0.05
+
+
+def policy_case(rows, vocab, dtype, seed, cuda, offset=0.0):
+    """Ratios away from the clipping's edges, where the gradient jumps; `offset` moves all logits."""
+    g = torch.Generator().manual_seed(seed)
+    logits = (2.5 * torch.randn(rows, vocab, generator=g) + offset).to(dtype)
+    targets = torch.randint(0, vocab, (rows,), generator=g)
+    return finish_case(dict(logits=logits, targets=targets, valid=torch.arange(rows) % 5 != 1), g, cuda)
+
+
+def finish_case(case, g, cuda):
+    rows = case["targets"].numel()
+    lp = torch.log_softmax(case["logits"].double(), -1).gather(-1, case["targets"][:, None])[:, 0]
+    drift = 0.2 * torch.randn(rows, generator=g).double()
+    for edge in (math.log(1 - CLIP_LOW), math.log(1 + CLIP_HIGH)):
+        drift = torch.where((drift - edge).abs() < 1e-2, edge + 2e-2, drift)
+    case.update(old=(lp - drift).float(), advantages=torch.randn(rows, generator=g),
+                reference=(lp + 0.1 * torch.randn(rows, generator=g)).float())
+    return {name: t.to(cuda) for name, t in case.items()}
+
+
+def policy_of(case, logits):
+    return policy_loss(logits, case["targets"], case["old"], case["advantages"], reference_log_probs=case["reference"],
+                       valid_mask=case["valid"], clip_low=CLIP_LOW, clip_high=CLIP_HIGH, kl_weight=BETA)
+
+
+def policy_gradient_with_bounds(case, factor=1.0):
+    """The 64-bit gradient, and what fp32 may lose of each of its entries.
+
+    A log-prob loses the roundings of its exponentials' arguments and of their
+    sum, 136 EPS in all; the ratio and e^d inherit that; an entry's probability
+    loses the same, relative to itself.
+    """
+    x = case["logits"].double()
+    live = case["valid"].double()
+    count = max(1, int(case["valid"].sum()))
+    p = torch.softmax(x, -1)
+    lp = torch.log_softmax(x, -1).gather(-1, case["targets"][:, None])[:, 0]
+    ratio, gap = torch.exp(lp - case["old"].double()), torch.exp(case["reference"].double() - lp)
+    a = case["advantages"].double()
+    free, clipped = ratio * a, ratio.clamp(1 - CLIP_LOW, 1 + CLIP_HIGH) * a
+    slope = (torch.where(free <= clipped, -free, 0.0) + BETA * (1 - gap)) * live * factor / count
+    slope_lost = 144 * EPS * ((ratio * a).abs() + BETA * (1 + gap)) * live * factor / count
+    want = -slope[:, None] * p
+    lost = p * (slope_lost + 144 * EPS * slope.abs())[:, None]
+    at = case["targets"][:, None]
+    return want.scatter_add(1, at, slope[:, None]), lost.scatter_add(1, at, slope_lost[:, None])
+
+
+POLICY_SHAPES = [(64, 257), (17, 1024), (10, 4097), (7, 8200), (5, 32767), (6, 32768), (3, 65000), (2, 131072), (2, 250001), (2, 600001)]
+
+
+def factor_of(dtype):
+    return 64.0 if dtype == torch.float16 else 1.0  # fp16 gradients are there to be scaled
+
+
+def gradient_of(case, logits=None, factor=1.0, **more):
+    logits = case["logits"].clone().requires_grad_(True) if logits is None else logits
+    result = policy_of(case, logits)
+    return torch.autograd.grad(result.loss, logits, torch.tensor(factor, device=logits.device), **more)[0]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [900, 4097, 32768, 131072, 300000])
+def test_policy_gradient_of_low_and_large_logits_in_every_backward(vocab, dtype, cuda):
+    """Rows of the type's lowest value are uniform, and logits of large magnitude differ as they stand: in the first
+    backward, and in another through a retained graph."""
+    g = torch.Generator().manual_seed(vocab)
+    most = torch.finfo(dtype).max
+    logits = 2.5 * torch.randn(6, vocab, generator=g)
+    logits[0] = -most
+    logits[1] = torch.where(torch.arange(vocab) % 2 == 0, -most, most / 2)
+    logits[3] += 3e4 if dtype == torch.float16 else 1e6
+    logits[4] -= 200.0
+    targets = torch.randint(0, vocab, (6,), generator=g) | 1  # odd: the entries of row 1 that are possible
+    case = finish_case(dict(logits=logits.to(dtype), targets=targets.clamp_max(vocab - 1 - vocab % 2), valid=torch.ones(6, dtype=torch.bool)), g, cuda)
+    factor = factor_of(dtype)
+    leaf = case["logits"].clone().requires_grad_(True)
+    result = policy_of(case, leaf)
+    weight = torch.tensor(factor, device=cuda)
+    want, lost = policy_gradient_with_bounds(case, factor)
+    for retain in (True, True, False):
+        got, = torch.autograd.grad(result.loss, leaf, weight, retain_graph=retain)
+        check(got, want, lost)
+
+
+def test_policy_entries_with_log_sum_exps_alone(cuda):
+    """The C entries as a caller has them that keeps one float per row: the softmax is off by the log-sum-exps' rounding."""
+    rows, vocab = 9, 1500
+    case = policy_case(rows, vocab, torch.float32, 41, cuda)
+    lib, stream = _native.library(), torch.cuda.current_stream().cuda_stream
+    policy_of(case, case["logits"])  # initialises the device
+    loss, kl, one = (torch.ones((), device=cuda) for _ in range(3))
+    log_probs, lse, slopes = (torch.full((rows,), math.nan, device=cuda) for _ in range(3))
+    size = lib.koemi_think_policy_loss_workspace()
+    workspace, grad = torch.empty(size, dtype=torch.uint8, device=cuda), torch.full((rows, vocab), math.nan, device=cuda)
+    at = lambda t: t.data_ptr()  # noqa: E731
+    assert lib.koemi_think_policy_loss_forward(
+        at(case["logits"]), rows, vocab, rows, 0, vocab, at(case["targets"]), at(case["old"]), at(case["advantages"]),
+        at(case["reference"]), at(case["valid"]), CLIP_LOW, CLIP_HIGH, BETA, at(loss), at(kl), at(log_probs), at(lse), at(slopes),
+        None, _native.F32, at(workspace), size, stream) == 0
+    assert lib.koemi_think_policy_loss_backward(
+        at(case["logits"]), rows, vocab, rows, 0, vocab, at(case["targets"]), at(case["valid"]), at(lse), at(slopes), at(one),
+        at(grad), _native.F32, stream) == 0
+    exact = torch.where(case["valid"], torch.logsumexp(case["logits"].double(), -1), 0.0)
+    check(lse, exact, 136 * EPS)
+    want, lost = policy_gradient_with_bounds(case)
+    # a log-sum-exp below 32 rounds to 16 EPS once more
+    check(grad, want, lost + 32 * EPS * want.abs())
