@@ -783,6 +783,7 @@ KOEMI_API int koemi_moe_route_learned_backward(const void *logits, const int64_t
  * grad_logits ([rows, vocab], dtype, contiguous, 16-byte aligned; NULL: not
  * wanted) receives d loss / d logits in the same pass. */
 #define KOEMI_POLICY_SUMS 0x100
+#define KOEMI_POLICY_HELD 0x200
 KOEMI_API size_t koemi_think_policy_loss_workspace(void);
 KOEMI_API int koemi_think_policy_loss_forward(const void *logits, int64_t rows, int64_t vocab, int64_t inner_rows,
                                               int64_t outer_stride, int64_t inner_stride, const int64_t *targets,
@@ -793,12 +794,15 @@ KOEMI_API int koemi_think_policy_loss_forward(const void *logits, int64_t rows, 
                                               int dtype, void *workspace, size_t workspace_bytes, void *stream);
 /* d loss / d logits times *grad_loss from the logits, lse and slopes (where
  * the forward did not write it, and for f16, whose gradients underflow before
- * the factor of a scaled loss). */
+ * the factor of a scaled loss). With KOEMI_POLICY_HELD added to dtype,
+ * grad_logits holds the forward's gradient: it stays where *grad_loss is one
+ * and is written anew elsewhere, rounded once. */
 KOEMI_API int koemi_think_policy_loss_backward(const void *logits, int64_t rows, int64_t vocab, int64_t inner_rows,
                                                int64_t outer_stride, int64_t inner_stride, const int64_t *targets,
                                                const uint8_t *valid, const float *lse, const float *slopes,
                                                const float *grad_loss, void *grad_logits, int dtype, void *stream);
-/* grad_logits *= *factor in place; a factor of one reads and writes nothing. */
+/* grad_logits *= *factor in place; a factor of one reads and writes nothing.
+ * In 16 bits the products are a second rounding. */
 KOEMI_API int koemi_think_policy_loss_scale(void *grad_logits, int64_t count, const float *factor, int dtype,
                                             void *stream);
 

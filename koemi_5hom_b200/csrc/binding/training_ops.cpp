@@ -451,21 +451,33 @@ Route policy_loss_keep_cuda(const Tensor &logits, const Tensor &targets, const T
     return out;
 }
 
-Tensor policy_loss_backward_cuda(const Tensor &logits, const Tensor &targets, const OptionalTensor &valid,
-                                 const Tensor &kept, const Tensor &grad_loss) {
-    check_policy(logits, targets, valid);
+// Into `grad`; held: it holds the gradient for a factor of one.
+void policy_backward(const Tensor &logits, const Tensor &targets, const OptionalTensor &valid, const Tensor &kept,
+                     const Tensor &grad_loss, const Tensor &grad, bool held) {
     const Rows shape(logits);
     require("kept", kept, {3, shape.rows}, at::kFloat, logits);
     require("grad_loss", grad_loss, {}, at::kFloat, logits);
     const Launch launch(logits);
-    Tensor grad = at::empty(logits.sizes(), logits.options());
     check("koemi_think_policy_loss_backward",
           lib().policy_backward(address<void>(logits), shape.rows, shape.vocab, shape.inner, shape.outer_stride,
                                 shape.inner_stride, address<int64_t>(targets), address<uint8_t>(valid), address<float>(kept),
                                 address<float>(kept) + 2 * shape.rows, address<float>(grad_loss), address<void>(grad),
-                                code_of(logits) | KOEMI_POLICY_SUMS,
-                                launch.stream));
+                                code_of(logits) | KOEMI_POLICY_SUMS | (held ? KOEMI_POLICY_HELD : 0), launch.stream));
+}
+
+Tensor policy_loss_backward_cuda(const Tensor &logits, const Tensor &targets, const OptionalTensor &valid,
+                                 const Tensor &kept, const Tensor &grad_loss) {
+    check_policy(logits, targets, valid);
+    Tensor grad = at::empty(logits.sizes(), logits.options());
+    policy_backward(logits, targets, valid, kept, grad_loss, grad, false);
     return grad;
+}
+
+void policy_loss_rescale_cuda(const Tensor &gradient, const Tensor &logits, const Tensor &targets, const OptionalTensor &valid,
+                              const Tensor &kept, const Tensor &factor) {
+    check_policy(logits, targets, valid);
+    require("gradient", gradient, logits.sizes(), logits.scalar_type(), logits);
+    policy_backward(logits, targets, valid, kept, factor, gradient, true);
 }
 
 void policy_loss_scale_cuda(const Tensor &gradient, const Tensor &factor) {
@@ -491,8 +503,13 @@ struct PolicyLossBackward final : torch::autograd::Node {
         if (gradient.defined()) {
             result[0] = std::move(gradient);
             gradient = Tensor();
-            KOEMI_OP(policy_loss_scale, decltype(policy_loss_scale_cuda));
-            policy_loss_scale.call(result[0], factor);
+            if (saved.scalar_type() == at::kFloat) {  // a product more costs 2^-24
+                KOEMI_OP(policy_loss_scale, decltype(policy_loss_scale_cuda));
+                policy_loss_scale.call(result[0], factor);
+            } else {
+                KOEMI_OP(policy_loss_rescale, decltype(policy_loss_rescale_cuda));
+                policy_loss_rescale.call(result[0], saved, targets.unpack(), given(valid.unpack()), kept.unpack(), factor);
+            }
         } else {
             KOEMI_OP(policy_loss_backward, decltype(policy_loss_backward_cuda));
             result[0] = policy_loss_backward.call(saved, targets.unpack(), given(valid.unpack()), kept.unpack(), factor);
@@ -661,6 +678,7 @@ TORCH_LIBRARY_FRAGMENT(koemi_b200, m) {
     m.def("policy_loss_keep(Tensor logits, Tensor targets, Tensor old, Tensor advantages, Tensor? reference, Tensor? valid, float clip_low, float clip_high, float kl_weight) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("policy_loss_backward(Tensor logits, Tensor targets, Tensor? valid, Tensor kept, Tensor grad_loss) -> Tensor");
     m.def("policy_loss_scale(Tensor(a!) gradient, Tensor factor) -> ()");
+    m.def("policy_loss_rescale(Tensor(a!) gradient, Tensor logits, Tensor targets, Tensor? valid, Tensor kept, Tensor factor) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(koemi_b200, CUDA, m) {
@@ -674,6 +692,7 @@ TORCH_LIBRARY_IMPL(koemi_b200, CUDA, m) {
     m.impl("policy_loss_keep", policy_loss_keep_cuda);
     m.impl("policy_loss_backward", policy_loss_backward_cuda);
     m.impl("policy_loss_scale", policy_loss_scale_cuda);
+    m.impl("policy_loss_rescale", policy_loss_rescale_cuda);
 }
 
 TORCH_LIBRARY_IMPL(koemi_b200, Autograd, m) {

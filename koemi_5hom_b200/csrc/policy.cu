@@ -328,14 +328,14 @@ struct Packets {
     }
 };
 
-// Zeros into a row of the gradient, by a CTA: from packet `first` on, `count`
-// of them or, the last slice, to the row's end.
-template <typename T>
+// Zeros into a row of the gradient, by kRowThreads neighbouring threads: from
+// packet `first` on, `count` of them or, the last slice, to the row's end.
+template <typename T, int kRowThreads>
 __device__ void clear_row(T *out, int vocab, int first = 0, int count = 0) {
     const Packets<T> packets(out, vocab);
     const float zeros[Packets<T>::kWidth] = {};
     const int end = count > 0 ? first + count : packets.count;
-    for (int c = first + threadIdx.x; c < end; c += blockDim.x) packets.store(out, packets.whole(c), c, zeros);
+    for (int c = first + static_cast<int>(threadIdx.x % kRowThreads); c < end; c += kRowThreads) packets.store(out, packets.whole(c), c, zeros);
 }
 
 // The warps' partials of a row, merged by every warp alike: the row's partial
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
         const RowTerms row_terms = table[index % kTable];
         T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
         if (!row_terms.valid()) {
-            if (out != nullptr) clear_row(out, vocab, first, last_slice ? 0 : slice);
+            if (out != nullptr) clear_row<T, kThreads>(out, vocab, first, last_slice ? 0 : slice);
             if (threadIdx.x == kThreads - 1 && rank == 0) result.skip(row);
             continue;
         }
@@ -664,7 +664,7 @@ __global__ __launch_bounds__(kWalkThreads) void policy_walk_kernel(PolicyRows sh
         T *out = grad_logits == nullptr ? nullptr : grad_logits + row * vocab;
         const RowTerms row_terms = load_terms(terms, row, vocab);
         if (!row_terms.valid()) {
-            if (out != nullptr) clear_row(out, vocab);
+            if (out != nullptr) clear_row<T, kWalkThreads>(out, vocab);
             if (threadIdx.x == 0) result.skip(row);
             continue;
         }
@@ -757,22 +757,29 @@ __global__ __launch_bounds__(kFinishThreads) void policy_finish_kernel(const dou
     }
 }
 
-// The gradient from what the forward kept of its rows: a CTA takes a row's packets (or,
-// grid.y > 1, every grid.y-th run of them).
+// The gradient from what the forward kept of its rows: kRowThreads threads take
+// a row's packets (or, grid.y > 1, every grid.y-th run of them). held: grad_logits holds it for a
+// factor of one, which stays. A 16-bit gradient under another factor is formed
+// again from the logits: as many bytes as scaling it, and one rounding, where a
+// product of the rounded gradient would have two (8192 x 32768 bf16, 75% of the
+// rows valid: 166 us, the product 175; 65536 x 1000 53 and 48).
 constexpr int kBackwardThreads = 256;
-template <typename T>
+template <typename T, int kRowThreads>
 __global__ __launch_bounds__(kBackwardThreads) void policy_backward_kernel(
     PolicyRows shape, const T *__restrict__ logits, const int64_t *__restrict__ targets,
     const uint8_t *__restrict__ valid, const float *__restrict__ lse, const float *__restrict__ sums,
-    const float *__restrict__ slopes, const float *__restrict__ grad_loss, T *__restrict__ grad_logits) {
+    const float *__restrict__ slopes, const float *__restrict__ grad_loss, T *__restrict__ grad_logits, bool held) {
     constexpr int kWidth = Pack<T>::kWidth, kPackets = 4;
     const float scale = *grad_loss;
-    const int vocab = static_cast<int>(shape.vocab), step = static_cast<int>(gridDim.y) * kBackwardThreads * kPackets;
-    for (int64_t row = blockIdx.x; row < shape.rows; row += gridDim.x) {
+    if (held && scale == 1.0f) return;
+    constexpr int kRows = kBackwardThreads / kRowThreads;  // of a CTA at a time
+    const int thread = threadIdx.x % kRowThreads, run = blockIdx.y * kRowThreads * kPackets;
+    const int vocab = static_cast<int>(shape.vocab), step = static_cast<int>(gridDim.y) * kRowThreads * kPackets;
+    for (int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / kRowThreads; row < shape.rows; row += int64_t(gridDim.x) * kRows) {
         const T *in = logits + shape.start(row);
         T *out = grad_logits + row * vocab;
         if (valid != nullptr && valid[row] == 0) {
-            if (blockIdx.y == 0) clear_row(out, vocab);
+            if (blockIdx.y == 0) clear_row<T, kRowThreads>(out, vocab);
             continue;
         }
         const Packets<T> packets(in, vocab);
@@ -780,16 +787,16 @@ __global__ __launch_bounds__(kBackwardThreads) void policy_backward_kernel(
         const float slope = slopes[row] * scale, from = lse[row], factor = sums != nullptr ? -slope / sums[row] : -slope;
         const int64_t target = targets[row];
         const int at = static_cast<int>(target) + packets.skip, packet = target >= 0 && target < vocab ? at / kWidth : -1;
-        for (int first = blockIdx.y * kBackwardThreads * kPackets + threadIdx.x; first < packets.count; first += step) {
+        for (int first = run + thread; first < packets.count; first += step) {
             uint4 raw[kPackets];
 #pragma unroll
             for (int j = 0; j < kPackets; ++j) {
-                const int c = first + j * kBackwardThreads;
+                const int c = first + j * kRowThreads;
                 raw[j] = packets.whole(c) ? load_cached(packets.base + int64_t(c) * kWidth) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int j = 0; j < kPackets; ++j) {
-                const int c = first + j * kBackwardThreads;
+                const int c = first + j * kRowThreads;
                 if (c >= packets.count) continue;
                 float v[kWidth];
                 if (packets.whole(c)) {
@@ -830,11 +837,11 @@ __global__ __launch_bounds__(256) void policy_scale_kernel(T *__restrict__ grad,
     }
 }
 
-// Takes the flag out of a dtype; the sums behind `lse`, or NULL.
-float *sums_of(int &dtype, float *lse, int64_t rows) {
-    const bool given = (dtype & KOEMI_POLICY_SUMS) != 0;
-    dtype &= ~KOEMI_POLICY_SUMS;
-    return given && lse != nullptr ? lse + rows : nullptr;
+// Takes a flag out of a dtype.
+bool take_flag(int &dtype, int flag) {
+    const bool given = (dtype & flag) != 0;
+    dtype &= ~flag;
+    return given;
 }
 
 PolicyRows rows_of(int64_t rows, int64_t vocab, int64_t inner_rows, int64_t outer_stride, int64_t inner_stride) {
@@ -894,6 +901,11 @@ int launch_rows(int64_t bytes, bool exact, const PolicyRows &shape, const Policy
                                        slice, device_status_word()));
     return KOEMI_OK;
 }
+
+// Up to here (packets) eight threads, and a warp, take a row of the backward; a
+// CTA takes longer ones: 65536 x 64 bf16 19 us with eight threads and 33 with a
+// warp, 16384 x 1100 27 us with a warp and 53 with a CTA.
+constexpr int kTinyRow = 32, kShortRow = 1024;
 
 // The row kernel with the fewest threads that hold the row.
 template <typename T>
@@ -966,14 +978,23 @@ int policy_forward(const PolicyRows &shape, const PolicyTerms &terms, const void
 template <typename T>
 int policy_backward(const PolicyRows &shape, const void *logits, const int64_t *targets, const uint8_t *valid,
                     const float *lse, const float *sums, const float *slopes, const float *grad_loss, void *grad_logits,
-                    cudaStream_t stream) {
-    // few long rows: several CTAs a row
-    const int64_t runs = ceil_div(shape.vocab, kBackwardThreads * 4 * Pack<T>::kWidth), places = 8 * int64_t(sm_count());
-    const unsigned x = static_cast<unsigned>(shape.rows < places ? shape.rows : places);
-    int64_t y = ceil_div(places, x);
-    if (y > runs) y = runs;
-    policy_backward_kernel<T><<<dim3(x, static_cast<unsigned>(y)), kBackwardThreads, 0, stream>>>(
-        shape, static_cast<const T *>(logits), targets, valid, lse, sums, slopes, grad_loss, static_cast<T *>(grad_logits));
+                    bool held, cudaStream_t stream) {
+    // threads of a row, rows of a CTA at a time, and for few long rows several CTAs a row
+    const int64_t packets = ceil_div(shape.vocab, Pack<T>::kWidth), most = 8 * int64_t(sm_count());
+    auto go = [&](auto kernel, int row_threads) {
+        const int64_t turns = ceil_div(shape.rows, kBackwardThreads / row_threads), x = turns < most ? turns : most;
+        const int64_t runs = ceil_div(packets, row_threads * 4), wanted = ceil_div(most, x);
+        const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(wanted < runs ? wanted : runs));
+        kernel<<<grid, kBackwardThreads, 0, stream>>>(shape, static_cast<const T *>(logits), targets, valid, lse, sums, slopes,
+                                                      grad_loss, static_cast<T *>(grad_logits), held);
+    };
+    if (packets <= kTinyRow) {
+        go(policy_backward_kernel<T, 8>, 8);
+    } else if (packets <= kShortRow) {
+        go(policy_backward_kernel<T, 32>, 32);
+    } else {
+        go(policy_backward_kernel<T, kBackwardThreads>, kBackwardThreads);
+    }
     KOEMI_LAUNCH_CHECK();
     return KOEMI_OK;
 }
@@ -1016,7 +1037,7 @@ extern "C" int koemi_think_policy_loss_forward(const void *logits, int64_t rows,
         return fail(KOEMI_ERR_WORKSPACE, "the policy loss's workspace is smaller than koemi_think_policy_loss_workspace()");
     }
     const PolicyTerms terms{targets, old_log_probs, advantages, reference_log_probs, valid, clip_low, clip_high, kl_weight};
-    float *sums = sums_of(dtype, lse, rows);
+    float *sums = take_flag(dtype, KOEMI_POLICY_SUMS) && lse != nullptr ? lse + rows : nullptr;
     cudaStream_t s = as_stream(stream);
     switch (dtype) {
         case KOEMI_F32: return policy_forward<float>(shape, terms, logits, loss, kl, log_probs, lse, sums, slopes, grad_logits, workspace, s);
@@ -1040,12 +1061,13 @@ extern "C" int koemi_think_policy_loss_backward(const void *logits, int64_t rows
         return fail(KOEMI_ERR_INVALID, "policy loss backward tensors must be non-NULL");
     }
     if (!aligned(grad_logits, 16)) return fail(KOEMI_ERR_INVALID, "grad_logits must be 16-byte aligned");
-    const float *sums = sums_of(dtype, const_cast<float *>(lse), rows);
+    const float *sums = take_flag(dtype, KOEMI_POLICY_SUMS) ? lse + rows : nullptr;
+    const bool held = take_flag(dtype, KOEMI_POLICY_HELD);
     cudaStream_t s = as_stream(stream);
     switch (dtype) {
-        case KOEMI_F32: return policy_backward<float>(shape, logits, targets, valid, lse, sums, slopes, grad_loss, grad_logits, s);
-        case KOEMI_F16: return policy_backward<__half>(shape, logits, targets, valid, lse, sums, slopes, grad_loss, grad_logits, s);
-        case KOEMI_BF16: return policy_backward<__nv_bfloat16>(shape, logits, targets, valid, lse, sums, slopes, grad_loss, grad_logits, s);
+        case KOEMI_F32: return policy_backward<float>(shape, logits, targets, valid, lse, sums, slopes, grad_loss, grad_logits, held, s);
+        case KOEMI_F16: return policy_backward<__half>(shape, logits, targets, valid, lse, sums, slopes, grad_loss, grad_logits, held, s);
+        case KOEMI_BF16: return policy_backward<__nv_bfloat16>(shape, logits, targets, valid, lse, sums, slopes, grad_loss, grad_logits, held, s);
         default: return fail(KOEMI_ERR_INVALID, "unsupported policy loss dtype %d", dtype);
     }
 }

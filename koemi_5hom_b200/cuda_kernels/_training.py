@@ -91,3 +91,7 @@ def _register_fakes() -> None:
     @fake("policy_loss_scale")
     def _(gradient, factor):
         return None
+
+    @fake("policy_loss_rescale")
+    def _(gradient, logits, targets, valid, kept, factor):
+        return None

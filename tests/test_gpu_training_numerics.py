@@ -204,6 +204,18 @@ def test_policy_gradient_of_low_and_large_logits_in_every_backward(vocab, dtype,
         check(got, want, lost)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [257, 4097, 32768, 131072])
+def test_policy_gradient_is_rounded_once_whatever_the_factor(vocab, dtype, cuda):
+    """A loss divided by the number of accumulated steps: 16-bit gradients are those of the formula, rounded once.
+    An fp32 gradient is a product more, a rounding of 2^-24."""
+    case = policy_case(9, vocab, dtype, vocab + 1, cuda)
+    for factor in (1.0 / 3.0, 0.7):
+        factor = torch.tensor(factor).item() * factor_of(dtype)  # as fp32 holds it
+        want, lost = policy_gradient_with_bounds(case, factor)
+        check(gradient_of(case, factor=factor), want, lost + (EPS * want.abs() if dtype == torch.float32 else 0.0))
+
+
 def test_policy_entries_with_log_sum_exps_alone(cuda):
     """The C entries as a caller has them that keeps one float per row: the softmax is off by the log-sum-exps' rounding."""
     rows, vocab = 9, 1500
@@ -227,3 +239,17 @@ def test_policy_entries_with_log_sum_exps_alone(cuda):
     want, lost = policy_gradient_with_bounds(case)
     # a log-sum-exp below 32 rounds to 16 EPS once more
     check(grad, want, lost + 32 * EPS * want.abs())
+
+
+def test_rescale_refuses_what_the_kernel_cannot_take(cuda):
+    logits, targets = torch.zeros(6, 9, device=cuda, dtype=torch.bfloat16), torch.zeros(6, dtype=torch.int64, device=cuda)
+    rows, one = torch.zeros(6, device=cuda), torch.ones((), device=cuda)
+    policy_loss(logits, targets, rows, rows)  # registers the ops
+    rescale, kept = torch.ops.koemi_b200.policy_loss_rescale, torch.ones(3, 6, device=cuda)
+    for call in (lambda: rescale(logits[:5].clone(), logits, targets, None, kept, one),
+                 lambda: rescale(logits.float(), logits, targets, None, kept, one),
+                 lambda: rescale(logits.clone(), logits, targets[:5], None, kept, one),
+                 lambda: rescale(logits.clone(), logits, targets, None, kept[:2], one),
+                 lambda: rescale(logits.clone(), logits, targets, None, kept, rows)):
+        with pytest.raises(ValueError):
+            call()
