@@ -9,21 +9,30 @@ fronts report CPU tensors before dispatch.
 """
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from koemi_5hom_b200 import _native
 
 SEGMENT = 128  # positions between two carries of the gated recurrence
+_LOCK = threading.Lock()
 _loaded = False
 
 
-def load(device: torch.device) -> None:
-    """Register the ops (once) and initialise ``device``."""
+def register() -> None:
+    """Register the ops and their fake implementations (once, whichever threads call first)."""
     global _loaded
-    if not _loaded:
-        _native.binding()
-        _register_fakes()
-        _loaded = True
+    with _LOCK:
+        if not _loaded:
+            _native.binding()
+            _register_fakes()
+            _loaded = True
+
+
+def load(device: torch.device) -> None:
+    """Register the ops and initialise ``device``."""
+    register()
     _native.ensure_device(device)
 
 
