@@ -224,19 +224,22 @@ std::tuple<Tensor, Tensor> gated_recurrence_backward_cuda(const Tensor &projecti
 #define KOEMI_OP(name, signature) \
     static auto name = c10::Dispatcher::singleton().findSchemaOrThrow("koemi_b200::" #name, "").typed<signature>()
 
+// The nodes unpack what they saved above the autograd keys: under activation
+// checkpointing that runs the forward again, which has to be recorded.
 struct GatedRecurrenceBackward final : torch::autograd::Node {
     SavedVariable projections, valid, restart, carries;
     double low = 0, high = 0;
     variable_list apply(variable_list &&grads) override {
         first_order_only();
         std::lock_guard<std::mutex> lock(mutex_);
-        at::AutoDispatchBelowADInplaceOrView below;
         variable_list result(2);
         if (!grads[0].defined() && !grads[1].defined()) return result;
+        const Tensor projections_ = projections.unpack(), valid_ = valid.unpack(), restart_ = restart.unpack();
+        const Tensor carries_ = carries.unpack();
+        at::AutoDispatchBelowADInplaceOrView below;
         KOEMI_OP(gated_recurrence_backward, decltype(gated_recurrence_backward_cuda));
-        auto [grad_projections, grad_initial] =
-            gated_recurrence_backward.call(projections.unpack(), given(valid.unpack()), given(restart.unpack()),
-                                           carries.unpack(), dense(grads[0]), dense(grads[1]), low, high);
+        auto [grad_projections, grad_initial] = gated_recurrence_backward.call(
+            projections_, given(valid_), given(restart_), carries_, dense(grads[0]), dense(grads[1]), low, high);
         if (task_should_compute_output(0)) result[0] = grad_projections;
         if (task_should_compute_output(1)) result[1] = grad_initial;
         return result;
@@ -335,12 +338,13 @@ struct RouteLearnedBackward final : torch::autograd::Node {
     variable_list apply(variable_list &&grads) override {
         first_order_only();
         std::lock_guard<std::mutex> lock(mutex_);
-        at::AutoDispatchBelowADInplaceOrView below;
         variable_list result(1);
         if (!grads[0].defined() && !grads[1].defined()) return result;
+        const Tensor logits_ = logits.unpack(), ids_ = ids.unpack(), weights_ = weights.unpack(shared_from_this());
+        const Tensor slope_ = slope.unpack();
+        at::AutoDispatchBelowADInplaceOrView below;
         KOEMI_OP(route_learned_backward, decltype(route_learned_backward_cuda));
-        result[0] = route_learned_backward.call(logits.unpack(), ids.unpack(), weights.unpack(shared_from_this()), slope.unpack(),
-                                                dense(grads[0]), dense(grads[1]), renormalize);
+        result[0] = route_learned_backward.call(logits_, ids_, weights_, slope_, dense(grads[0]), dense(grads[1]), renormalize);
         return result;
     }
     void release_variables() override {
@@ -494,25 +498,24 @@ struct PolicyLossBackward final : torch::autograd::Node {
     variable_list apply(variable_list &&grads) override {
         first_order_only();
         std::lock_guard<std::mutex> lock(mutex_);
-        at::AutoDispatchBelowADInplaceOrView below;
         variable_list result(1);
         if (!grads[0].defined()) return result;
+        const Tensor logits_ = logits.unpack(), targets_ = targets.unpack(), valid_ = valid.unpack(), kept_ = kept.unpack();
+        at::AutoDispatchBelowADInplaceOrView below;
         const Tensor factor = grads[0].contiguous();
-        // f16, and another backward through a retained graph, form the gradient from the logits
-        Tensor saved = logits.unpack();
-        if (gradient.defined()) {
-            result[0] = std::move(gradient);
-            gradient = Tensor();
-            if (saved.scalar_type() == at::kFloat) {  // a product more costs 2^-24
-                KOEMI_OP(policy_loss_scale, decltype(policy_loss_scale_cuda));
-                policy_loss_scale.call(result[0], factor);
-            } else {
-                KOEMI_OP(policy_loss_rescale, decltype(policy_loss_rescale_cuda));
-                policy_loss_rescale.call(result[0], saved, targets.unpack(), given(valid.unpack()), kept.unpack(), factor);
-            }
-        } else {
+        if (!gradient.defined()) {  // f16, and another backward through a retained graph: from the logits
             KOEMI_OP(policy_loss_backward, decltype(policy_loss_backward_cuda));
-            result[0] = policy_loss_backward.call(saved, targets.unpack(), given(valid.unpack()), kept.unpack(), factor);
+            result[0] = policy_loss_backward.call(logits_, targets_, given(valid_), kept_, factor);
+            return result;
+        }
+        result[0] = std::move(gradient);
+        gradient = Tensor();
+        if (logits_.scalar_type() == at::kFloat) {  // a product more costs 2^-24
+            KOEMI_OP(policy_loss_scale, decltype(policy_loss_scale_cuda));
+            policy_loss_scale.call(result[0], factor);
+        } else {
+            KOEMI_OP(policy_loss_rescale, decltype(policy_loss_rescale_cuda));
+            policy_loss_rescale.call(result[0], logits_, targets_, given(valid_), kept_, factor);
         }
         return result;
     }

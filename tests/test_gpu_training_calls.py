@@ -1,0 +1,48 @@
+"""The training operators called as training programs call them: recomputed, captured, from several threads."""
+from __future__ import annotations
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from koemi_5hom_b200.cuda_kernels.dense import gated_recurrence
+from koemi_5hom_b200.cuda_kernels.moe import route_learned_topk
+from koemi_5hom_b200.cuda_kernels.think import policy_loss
+
+pytestmark = pytest.mark.gpu
+
+
+def recurrence_value(x):
+    states, final = gated_recurrence(x)
+    return states.float().square().sum() + final.sum()
+
+
+def route_value(x):
+    route = route_learned_topk(x, top_k=2, renormalize=True)
+    return route.weights.square().sum() + route.balance_loss
+
+
+def policy_value(x):
+    rows = torch.arange(x.shape[0], device=x.device)
+    return policy_loss(x, rows, torch.full_like(rows, -8, dtype=torch.float32), 1.0 + rows.float().cos()).loss / 3
+
+
+# the scalar of an operator's differentiable outputs, and an input
+VALUES = {"recurrence": (recurrence_value, (3, 300, 128), torch.bfloat16), "recurrence step": (recurrence_value, (64, 1, 128), torch.float32),
+          "route": (route_value, (300, 64), torch.float32), "policy": (policy_value, (30, 5000), torch.bfloat16),
+          "policy of short rows": (policy_value, (30, 257), torch.float32), "policy of long rows": (policy_value, (30, 70000), torch.float16)}
+
+
+@pytest.fixture(params=VALUES, ids=VALUES)
+def operator(request, cuda):
+    value, shape, dtype = VALUES[request.param]
+    return value, torch.randn(shape, generator=torch.Generator().manual_seed(1)).to(dtype).to(cuda)
+
+
+def test_activation_checkpointing_gives_the_same_bits(operator):
+    value, x = operator
+    grads = []
+    for run in (value, lambda t: checkpoint(value, t, use_reentrant=False)):
+        leaf = x.clone().requires_grad_(True)
+        grads.append(torch.autograd.grad(run(leaf), leaf)[0])
+    assert torch.equal(*grads) and grads[0].any()

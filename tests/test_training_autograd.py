@@ -5,6 +5,12 @@ import subprocess
 import sys
 from pathlib import Path
 
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from koemi_5hom_b200.cuda_kernels import _training
+
 ROOT = Path(__file__).resolve().parent.parent
 
 
@@ -34,3 +40,41 @@ assert _training.loaded()
 """
     result = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert result.returncode == 0, result.stderr
+
+
+def recurrence(x, initial=None):
+    return torch.ops.koemi_b200.gated_recurrence(x, initial, None, None, 0.1, 0.9)
+
+
+def route(logits):
+    return torch.ops.koemi_b200.route_learned(logits, None, 2, False)
+
+
+def policy(logits, old=None, advantages=None, reference=None):
+    rows = torch.zeros(6, device="meta")
+    targets = torch.zeros(6, dtype=torch.int64, device="meta")
+    return torch.ops.koemi_b200.policy_loss(logits, targets, rows if old is None else old, rows if advantages is None else advantages,
+                                            reference, None, 0.2, 0.2, 0.0)
+
+
+# an operator's scalar of its differentiable outputs, and the shape of its input
+SCALARS = {"recurrence": (lambda x: sum(t.sum() for t in recurrence(x)), (2, 40, 16)),
+           "route": (lambda x: route(x)[1].sum() + route(x)[3], (6, 9)),
+           "policy": (lambda x: policy(x)[0], (6, 9))}
+
+
+@pytest.fixture(params=SCALARS, ids=SCALARS)
+def operator(request):
+    _training.register()
+    value, shape = SCALARS[request.param]
+    return value, torch.zeros(shape, device="meta")
+
+
+@pytest.mark.parametrize("before", [False, True])
+def test_activation_checkpointing(operator, before):
+    """The recomputation inside the node's unpacking is recorded, as it is for torch's own operators."""
+    value, x = operator
+    leaf = x.clone().requires_grad_(True)
+    out = checkpoint(lambda t: value(2 * t if before else t), leaf, use_reentrant=False)
+    grad, = torch.autograd.grad(out, leaf)
+    assert grad.shape == x.shape
