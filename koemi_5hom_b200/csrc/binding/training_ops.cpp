@@ -138,6 +138,15 @@ void first_order_only() {
     TORCH_CHECK(!at::GradMode::is_enabled(), "the training operators are differentiable to first order only (create_graph=True)");
 }
 
+// There is no forward-mode derivative: an input that carries a tangent is
+// refused, or the result would pass for a constant.
+bool has_tangent(const Tensor &t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptionalTensor &t) { return t.has_value() && has_tangent(*t); }
+template <typename... Inputs>
+void reverse_mode_only(const Inputs &...inputs) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(inputs) || ...), "the training operators have no forward-mode derivative");
+}
+
 // ----------------------------------------------------- the gated recurrence
 
 constexpr int64_t kSegment = 128;  // positions between two carries
@@ -260,6 +269,7 @@ std::tuple<Tensor, Tensor> gated_recurrence_autograd(const Tensor &projections_,
         check_forward(projections, initial, valid, restart, low, high);
         return no_positions(projections, initial);
     }
+    reverse_mode_only(projections, initial);
     if (at::GradMode::is_enabled() && (differentiates(projections) || differentiates(initial))) {
         auto node = node_of<GatedRecurrenceBackward>(projections, initial);
         Tensor states, final_state, carries;
@@ -358,6 +368,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> route_learned_autograd(const Tensor &
                                                                   int64_t top_k, bool renormalize) {
     const Tensor logits = logits_.contiguous();
     const OptionalTensor valid = dense(valid_);
+    reverse_mode_only(logits);
     if (at::GradMode::is_enabled() && differentiates(logits)) {
         auto node = node_of<RouteLearnedBackward>(logits);
         Tensor ids, weights, counts, balance, slope;
@@ -534,6 +545,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_loss_autograd(const Tensor &logits_, c
     const Tensor logits = readable(logits_), targets = targets_.contiguous();
     const Tensor old = old_.contiguous(), advantages = advantages_.contiguous();
     const OptionalTensor reference = dense(reference_), valid = dense(valid_);
+    reverse_mode_only(logits, old, advantages, reference);
     if (at::GradMode::is_enabled() && differentiates(logits)) {
         auto node = node_of<PolicyLossBackward>(logits);
         Tensor loss, kl, log_probs, kept, gradient;
@@ -581,6 +593,7 @@ struct Table {
             const auto type = t.scalar_type();
             TORCH_CHECK_VALUE(type == at::kFloat || type == at::kHalf || type == at::kBFloat16, name,
                               " must use float32, float16 or bfloat16; found ", type);
+            reverse_mode_only(t);
             tensors.push_back(&t);
             addresses.push_back(reinterpret_cast<uint64_t>(t.data_ptr()));
             elements.push_back(t.numel());

@@ -3,8 +3,10 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
+from koemi_5hom_b200.cuda_kernels.core import clip_gradients
 from koemi_5hom_b200.cuda_kernels.dense import gated_recurrence
 from koemi_5hom_b200.cuda_kernels.moe import route_learned_topk
 from koemi_5hom_b200.cuda_kernels.think import policy_loss
@@ -46,3 +48,11 @@ def test_activation_checkpointing_gives_the_same_bits(operator):
         leaf = x.clone().requires_grad_(True)
         grads.append(torch.autograd.grad(run(leaf), leaf)[0])
     assert torch.equal(*grads) and grads[0].any()
+
+
+def test_forward_mode_is_refused(operator, cuda):
+    value, x = operator
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        value(forward_ad.make_dual(x, torch.ones_like(x)))
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        clip_gradients([forward_ad.make_dual(x, torch.ones_like(x))], 1.0)

@@ -7,6 +7,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 from koemi_5hom_b200.cuda_kernels import _training
@@ -78,3 +79,26 @@ def test_activation_checkpointing(operator, before):
     out = checkpoint(lambda t: value(2 * t if before else t), leaf, use_reentrant=False)
     grad, = torch.autograd.grad(out, leaf)
     assert grad.shape == x.shape
+
+
+def test_forward_mode_is_refused(operator):
+    """A tangent is never dropped without a word."""
+    value, x = operator
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        value(forward_ad.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(value, (x,), (torch.ones_like(x),))
+    with forward_ad.dual_level():  # no tangent of this level: as ever
+        value(x)
+
+
+def test_forward_mode_of_the_other_inputs_is_refused():
+    _training.register()
+    rows, logits = torch.zeros(6, device="meta"), torch.zeros(6, 9, device="meta")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(rows, torch.ones_like(rows))
+        for call in (lambda: policy(logits, old=dual), lambda: policy(logits, advantages=dual), lambda: policy(logits, reference=dual),
+                     lambda: recurrence(torch.zeros(2, 3, 4, device="meta"), forward_ad.make_dual(torch.zeros(2, 2, device="meta"),
+                                                                                                  torch.ones(2, 2, device="meta")))):
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
