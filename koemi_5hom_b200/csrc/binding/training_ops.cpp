@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -134,8 +135,19 @@ void require(const char *name, const OptionalTensor &t, at::IntArrayRef shape, a
 }
 OptionalTensor dense(const OptionalTensor &t) { return t.has_value() && t->defined() ? OptionalTensor(t->contiguous()) : OptionalTensor(); }
 
+// For the ops that a node calls: nothing of them is recorded. torch.func.grad
+// runs every backward with gradients enabled, and what is outside it may record
+// the calls: there they stay visible, and refuse to be differentiated.
+struct BelowAutograd {
+    std::optional<at::AutoDispatchBelowADInplaceOrView> below;
+    static bool transformed() { return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode); }
+    BelowAutograd() {
+        if (!transformed()) below.emplace();
+    }
+};
 void first_order_only() {
-    TORCH_CHECK(!at::GradMode::is_enabled(), "the training operators are differentiable to first order only (create_graph=True)");
+    TORCH_CHECK(!at::GradMode::is_enabled() || BelowAutograd::transformed(),
+                "the training operators are differentiable to first order only (create_graph=True)");
 }
 
 // There is no forward-mode derivative: an input that carries a tangent is
@@ -245,7 +257,7 @@ struct GatedRecurrenceBackward final : torch::autograd::Node {
         if (!grads[0].defined() && !grads[1].defined()) return result;
         const Tensor projections_ = projections.unpack(), valid_ = valid.unpack(), restart_ = restart.unpack();
         const Tensor carries_ = carries.unpack();
-        at::AutoDispatchBelowADInplaceOrView below;
+        const BelowAutograd below;
         KOEMI_OP(gated_recurrence_backward, decltype(gated_recurrence_backward_cuda));
         auto [grad_projections, grad_initial] = gated_recurrence_backward.call(
             projections_, given(valid_), given(restart_), carries_, dense(grads[0]), dense(grads[1]), low, high);
@@ -352,7 +364,7 @@ struct RouteLearnedBackward final : torch::autograd::Node {
         if (!grads[0].defined() && !grads[1].defined()) return result;
         const Tensor logits_ = logits.unpack(), ids_ = ids.unpack(), weights_ = weights.unpack(shared_from_this());
         const Tensor slope_ = slope.unpack();
-        at::AutoDispatchBelowADInplaceOrView below;
+        const BelowAutograd below;
         KOEMI_OP(route_learned_backward, decltype(route_learned_backward_cuda));
         result[0] = route_learned_backward.call(logits_, ids_, weights_, slope_, dense(grads[0]), dense(grads[1]), renormalize);
         return result;
@@ -512,7 +524,7 @@ struct PolicyLossBackward final : torch::autograd::Node {
         variable_list result(1);
         if (!grads[0].defined()) return result;
         const Tensor logits_ = logits.unpack(), targets_ = targets.unpack(), valid_ = valid.unpack(), kept_ = kept.unpack();
-        at::AutoDispatchBelowADInplaceOrView below;
+        const BelowAutograd below;
         const Tensor factor = grads[0].contiguous();
         if (!gradient.defined()) {  // f16, and another backward through a retained graph: from the logits
             KOEMI_OP(policy_loss_backward, decltype(policy_loss_backward_cuda));
@@ -715,4 +727,9 @@ TORCH_LIBRARY_IMPL(koemi_b200, Autograd, m) {
     m.impl("gated_recurrence", gated_recurrence_autograd);
     m.impl("route_learned", route_learned_autograd);
     m.impl("policy_loss", policy_loss_autograd);
+    // reached with gradients to record under torch.func alone, an order or a level further out
+    for (const char *inner : {"gated_recurrence_keep", "gated_recurrence_backward", "route_learned_keep", "route_learned_backward",
+                              "policy_loss_keep", "policy_loss_backward", "policy_loss_scale", "policy_loss_rescale"}) {
+        m.impl(inner, torch::autograd::autogradNotImplementedFallback());
+    }
 }

@@ -56,3 +56,10 @@ def test_forward_mode_is_refused(operator, cuda):
         value(forward_ad.make_dual(x, torch.ones_like(x)))
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         clip_gradients([forward_ad.make_dual(x, torch.ones_like(x))], 1.0)
+
+
+def test_functional_gradients_give_the_same_bits(operator):
+    value, x = operator
+    leaf = x.clone().requires_grad_(True)
+    want, = torch.autograd.grad(value(leaf), leaf)
+    assert torch.equal(torch.func.grad(value)(x), want)

@@ -102,3 +102,23 @@ def test_forward_mode_of_the_other_inputs_is_refused():
                                                                                                   torch.ones(2, 2, device="meta")))):
             with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_functional_gradients_of_first_order(operator):
+    value, x = operator
+    assert torch.func.grad(value)(x).shape == x.shape
+    grad, result = torch.func.grad_and_value(value)(x)
+    assert grad.shape == x.shape and result.shape == ()
+
+
+def test_second_orders_are_refused(operator):
+    """By torch.func inside itself, by autograd around it, and by create_graph."""
+    value, x = operator
+    first = torch.func.grad(value)
+    with pytest.raises(RuntimeError, match="not implemented"):
+        torch.func.grad(lambda t: first(t).sum())(x)
+    leaf = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="not implemented"):
+        torch.autograd.grad(first(leaf).sum(), leaf)
+    with pytest.raises(RuntimeError, match="first order"):
+        torch.autograd.grad(value(leaf), leaf, create_graph=True)
