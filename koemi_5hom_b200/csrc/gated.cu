@@ -889,9 +889,11 @@ int chains_per_cluster(const GatedShape &shape, int64_t chains, int cluster, int
 }
 
 template <typename... KernelArgs, typename... Args>
-int launch_tiles(void (*kernel)(KernelArgs...), int64_t clusters, int cluster, size_t smem, cudaStream_t stream, Args &&...args) {
+int launch_tiles(void (*kernel)(KernelArgs...), int64_t clusters, int cluster, size_t smem, size_t most_smem, cudaStream_t stream,
+                 Args &&...args) {
     if (clusters * cluster >= (int64_t(1) << 31)) return fail(KOEMI_ERR_UNSUPPORTED, "the recurrence has too many lanes");
-    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    // the most that any call wants, not this one's: another thread's launch may stand between the two calls
+    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most_smem)));
     KOEMI_CUDA_TRY(launch_programmatic(false, kernel, dim3(static_cast<unsigned>(clusters * cluster)), dim3(kTileThreads), smem,
                                        stream, dim3(cluster, 1, 1), std::forward<Args>(args)...));
     return KOEMI_OK;
@@ -917,8 +919,8 @@ int gated_forward(const GatedShape &shape, const void *projections, const float 
     int *status = device_status_word();
     CUtensorMap map{};
     auto go = [&](auto kernel, bool tma) {
-        const size_t smem = tma ? TileMemory<T, 2, 2, 2, 1>::bytes(cluster) : TileMemory<T, 2, 0, 2, 1>::bytes(cluster);
-        return launch_tiles(kernel, ceil_div(chains, per), cluster, smem, stream, map, shape,
+        auto bytes = tma ? TileMemory<T, 2, 2, 2, 1>::bytes : TileMemory<T, 2, 0, 2, 1>::bytes;
+        return launch_tiles(kernel, ceil_div(chains, per), cluster, bytes(cluster), bytes(kMaxCluster), stream, map, shape,
                             feature_tiles, cluster, per, in, initial, out, final_state, carries, status);
     };
     if (tma_rows<T>(shape, projections, nullptr, states)) {
@@ -949,8 +951,8 @@ int gated_backward(const GatedShape &shape, const void *projections, const float
     int *status = device_status_word();
     CUtensorMap map{}, grad_map{};
     auto go = [&](auto kernel, bool tma) {
-        const size_t smem = tma ? TileMemory<T, 3, backward_stages<T>(), 3, 2>::bytes(cluster) : TileMemory<T, 3, 0, 3, 2>::bytes(cluster);
-        return launch_tiles(kernel, ceil_div(chains, per), cluster, smem, stream, map, grad_map,
+        auto bytes = tma ? TileMemory<T, 3, backward_stages<T>(), 3, 2>::bytes : TileMemory<T, 3, 0, 3, 2>::bytes;
+        return launch_tiles(kernel, ceil_div(chains, per), cluster, bytes(cluster), bytes(kMaxCluster), stream, map, grad_map,
                             shape, feature_tiles, cluster, per, in, carries, grad, grad_final, out, grad_initial, status);
     };
     if (tma_rows<T>(shape, projections, grad_states, grad_projections)) {

@@ -892,7 +892,8 @@ int launch_rows(int64_t bytes, bool exact, const PolicyRows &shape, const Policy
     auto kernel = exact ? policy_row_kernel<T, kThreads, kThreadBytes, true, kSplit>
                         : policy_row_kernel<T, kThreads, kThreadBytes, false, kSplit>;
     const int shared = buffers * static_cast<int>(buffer_bytes);
-    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
+    // the most that any call wants, not this one's: another thread's launch may stand between the two calls
+    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(room)));
     int64_t places = kSplit ? resident_clusters(kernel, kThreads, shared, cluster) : int64_t(sm_count()) * kPerSm;
     if (places > kPolicyBlocks) places = kPolicyBlocks;  // a partial sum each
     blocks = static_cast<unsigned>(shape.rows < places ? shape.rows : places);

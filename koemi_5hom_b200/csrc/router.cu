@@ -33,6 +33,7 @@ namespace {
 constexpr int kRouteWarps = 16;  // 32 warps per SM: a row is a chain of reductions
 constexpr int kWideWarps = 8;    // each has a row of sums in shared memory
 constexpr int kRouteBlocks = 296;
+constexpr int kMostExperts = 4096;
 
 struct RouteShape {
     int64_t tokens, experts, top_k;
@@ -496,7 +497,7 @@ bool with_layout(int64_t experts, F &&go) {
 
 int check_route(const RouteShape &shape) {
     if (shape.tokens < 0 || shape.tokens > (int64_t(1) << 31)) return fail(KOEMI_ERR_INVALID, "tokens must be in [0, 2^31]");
-    if (shape.experts < 1 || shape.experts > 4096) return fail(KOEMI_ERR_INVALID, "expert_count must be in [1, 4096]");
+    if (shape.experts < 1 || shape.experts > kMostExperts) return fail(KOEMI_ERR_INVALID, "expert_count must be in [1, 4096]");
     if (shape.top_k < 1 || shape.top_k > shape.experts || shape.top_k > 256) {
         return fail(KOEMI_ERR_INVALID, "top_k must be in [1, min(expert_count, 256)]");
     }
@@ -517,9 +518,10 @@ int route_forward(const RouteShape &shape, const void *logits, int64_t *ids, flo
             shape, in, ids, weights, mass, partial_counts, live, RouteTotals{counts, balance, slope});
     });
     if (!narrow) {
-        const size_t smem = (kWideWarps + 1) * shape.experts * sizeof(float);
+        const size_t per_expert = (kWideWarps + 1) * sizeof(float), smem = per_expert * shape.experts;
         auto kernel = route_forward_wide_kernel<T>;
-        KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+        // the most that any call wants, not this one's: another thread's launch may stand between the two calls
+        KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(per_expert * kMostExperts)));
         kernel<<<grid, kWideWarps * 32, smem, stream>>>(shape, in, ids, weights, mass, partial_counts, live);
     }
     KOEMI_LAUNCH_CHECK();

@@ -1,6 +1,8 @@
 """The training operators called as training programs call them: recomputed, captured, from several threads."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -63,3 +65,32 @@ def test_functional_gradients_give_the_same_bits(operator):
     leaf = x.clone().requires_grad_(True)
     want, = torch.autograd.grad(value(leaf), leaf)
     assert torch.equal(torch.func.grad(value)(x), want)
+
+
+# calls of one kernel with different needs of shared memory
+SIZES = {"policy": (policy_value, [(4, v) for v in (32768, 20000, 17000, 30000)], torch.bfloat16),
+         "recurrence": (recurrence_value, [(1, 2100, 64), (40, 300, 512), (1, 600, 64)], torch.bfloat16),
+         "route": (route_value, [(5, e) for e in (4096, 300, 2000)], torch.float32)}
+
+
+@pytest.mark.parametrize("name", SIZES)
+def test_threads_with_different_sizes(name, cuda):
+    """One thread's call never takes from another's launch the shared memory that it needs."""
+    value, shapes, dtype = SIZES[name]
+    errors = []
+
+    def work(shape):
+        try:
+            x = torch.randn(shape, device=cuda).to(dtype)
+            with torch.no_grad():
+                for _ in range(1500):
+                    value(x)
+        except Exception as error:  # noqa: BLE001
+            errors.append(error)
+
+    threads = [threading.Thread(target=work, args=(shape,)) for shape in shapes]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not errors, errors[0]
