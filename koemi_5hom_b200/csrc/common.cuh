@@ -196,23 +196,37 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// kCluster: the phase is completed by stores of other CTAs of the cluster
+// (st.async), which a wait of the default scope, the CTA's, need not make visible.
+template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t phase) {
     uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(phase)
-        : "memory");
+    if constexpr (kCluster) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(smem_addr(bar)), "r"(phase)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(smem_addr(bar)), "r"(phase)
+            : "memory");
+    }
     return done != 0;
 }
 
 // Waits for `phase` of `bar` with a bounded spin. Returns false (after
 // recording KOEMI_ERR_TIMEOUT in *status) when the budget runs out.
+template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t phase, int *status) {
     for (uint32_t spin = 0; spin < kWaitSpinLimit; ++spin) {
-        if (mbar_try_wait(bar, phase)) return true;
+        if (mbar_try_wait<kCluster>(bar, phase)) return true;
     }
     if (status != nullptr) atomicExch(status, KOEMI_ERR_TIMEOUT);
     return false;

@@ -468,7 +468,7 @@ __device__ __forceinline__ float meet(Memory &memory, int item, int cluster, int
     float2 *tiles = memory.tiles + parity * cluster * kTileFeatures + lane;
     if (lane == 0) mbar_arrive_expect_tx(bar, cluster * kTileFeatures * sizeof(float2));
     for (int r = 0; r < cluster; ++r) store_to_rank(tiles + rank * kTileFeatures, bar, r, mine);
-    if (!dead) dead = !mbar_wait_bounded(bar, static_cast<uint32_t>(item >> 1) & 1, status);
+    if (!dead) dead = !mbar_wait_bounded<true>(bar, static_cast<uint32_t>(item >> 1) & 1, status);
     float start = carry;
     for (int i = 0; i < cluster; ++i) {
         const int r = kBackward ? cluster - 1 - i : i;

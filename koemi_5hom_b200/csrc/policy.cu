@@ -584,7 +584,7 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
             uint64_t *bar = &meeting[taken & 1];
             if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, cluster * sizeof(float4));
             if (threadIdx.x < cluster) store_to_rank(parts + rank, bar, threadIdx.x, make_float4(all.max, all.sum, chosen, 0.0f));
-            if (!dead) dead = !mbar_wait_bounded(bar, static_cast<uint32_t>(taken >> 1) & 1, status);
+            if (!dead) dead = !mbar_wait_bounded<true>(bar, static_cast<uint32_t>(taken >> 1) & 1, status);
             const int lane = threadIdx.x & 31;
             all = warp_merge(lane < cluster ? Partial{parts[lane].x, parts[lane].y} : Partial{-INFINITY, 0.0f});
             if (packet >= 0) chosen = parts[packet / slice < cluster ? packet / slice : cluster - 1].z;

@@ -94,3 +94,16 @@ def test_threads_with_different_sizes(name, cuda):
     for thread in threads:
         thread.join()
     assert not errors, errors[0]
+
+
+@pytest.mark.parametrize("value,shape,dtype", [(recurrence_value, (1, 9000, 64), torch.bfloat16), (recurrence_value, (2, 5000, 96), torch.float32),
+                                               (policy_value, (600, 70000), torch.bfloat16), (policy_value, (40, 131072), torch.float32)])
+def test_exchanges_inside_clusters_repeat(value, shape, dtype, cuda):
+    """Long chains and long rows, whose parts CTAs of a cluster store into each other's memory, give equal bits each time."""
+    x = torch.randn(shape, generator=torch.Generator().manual_seed(5)).to(dtype).to(cuda).requires_grad_(True)
+    results = []
+    for _ in range(12):
+        result = value(x)
+        results.append((result.detach(), *torch.autograd.grad(result, x)))
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
