@@ -19,6 +19,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -154,9 +155,12 @@ void first_order_only() {
 // refused, or the result would pass for a constant.
 bool has_tangent(const Tensor &t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
 bool has_tangent(const OptionalTensor &t) { return t.has_value() && has_tangent(*t); }
+// Asked only while there is a level of tangents: a list of hundreds of views
+// costs microseconds.
+bool forward_mode() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 template <typename... Inputs>
 void reverse_mode_only(const Inputs &...inputs) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(inputs) || ...), "the training operators have no forward-mode derivative");
+    TORCH_CHECK_NOT_IMPLEMENTED(!forward_mode() || !(has_tangent(inputs) || ...), "the training operators have no forward-mode derivative");
 }
 
 // ----------------------------------------------------- the gated recurrence
@@ -594,6 +598,7 @@ struct Table {
         TORCH_CHECK_VALUE(count > 0, name, " must not be empty");
         tensors.reserve(count);
         addresses.reserve(count);
+        const bool tangents = forward_mode();
         elements.reserve(count);
         codes.reserve(count);
         for (Py_ssize_t i = 0; i < count; ++i) {
@@ -605,7 +610,7 @@ struct Table {
             const auto type = t.scalar_type();
             TORCH_CHECK_VALUE(type == at::kFloat || type == at::kHalf || type == at::kBFloat16, name,
                               " must use float32, float16 or bfloat16; found ", type);
-            reverse_mode_only(t);
+            if (tangents) reverse_mode_only(t);
             tensors.push_back(&t);
             addresses.push_back(reinterpret_cast<uint64_t>(t.data_ptr()));
             elements.push_back(t.numel());
