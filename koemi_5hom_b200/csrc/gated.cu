@@ -264,6 +264,7 @@ __device__ __forceinline__ float2 load_clamped(const float *at) {
 }
 
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Stores 8 bytes into CTA `rank`'s copy of `local` and counts them on its copy
@@ -423,6 +424,7 @@ struct TileMemory {
     T *stages;
     uint64_t *full;  // [kStages]
     uint64_t *met;   // [2]
+    int *issued;     // items whose loads are on their way or done: the loading thread's
     float *maps;     // [kMaps][kBlocks][32]
     float *starts;   // [kStarts][kBlocks][32]
     float2 *tiles;   // [2][CTAs of the cluster][32]
@@ -430,6 +432,7 @@ struct TileMemory {
         stages = reinterpret_cast<T *>(raw);
         full = reinterpret_cast<uint64_t *>(raw + size_t(kStages) * kStageBytes);
         met = full + 4;
+        issued = reinterpret_cast<int *>(met + 2);
         maps = reinterpret_cast<float *>(met + 4);
         starts = maps + kMaps * kPlane;
         tiles = reinterpret_cast<float2 *>(starts + kStarts * kPlane);
@@ -466,9 +469,10 @@ __device__ __forceinline__ float meet(Memory &memory, int item, int cluster, int
     const int lane = threadIdx.x, parity = item & 1;
     uint64_t *bar = &memory.met[parity];
     float2 *tiles = memory.tiles + parity * cluster * kTileFeatures + lane;
+    if (dead) return carry;  // nor sends any more: the others give up too
     if (lane == 0) mbar_arrive_expect_tx(bar, cluster * kTileFeatures * sizeof(float2));
     for (int r = 0; r < cluster; ++r) store_to_rank(tiles + rank * kTileFeatures, bar, r, mine);
-    if (!dead) dead = !mbar_wait_bounded<true>(bar, static_cast<uint32_t>(item >> 1) & 1, status);
+    dead = !mbar_wait_bounded<true>(bar, static_cast<uint32_t>(item >> 1) & 1, status);
     float start = carry;
     for (int i = 0; i < cluster; ++i) {
         const int r = kBackward ? cluster - 1 - i : i;
@@ -477,6 +481,23 @@ __device__ __forceinline__ float meet(Memory &memory, int item, int cluster, int
         carry = apply<kMasks>(v.x, v.y, carry);
     }
     return start;
+}
+
+// The end of a tile kernel. After a wait that gave up, the loading thread waits
+// (again with a limit) for the copies that it has issued, `*issued` items of
+// them, an item a stage; and no CTA of a cluster ends while another may store
+// into it.
+template <int kStages>
+__device__ __forceinline__ void leave(uint64_t *full, const int *issued, int cluster, bool dead, int *status) {
+    if constexpr (kStages > 0) {
+        if (threadIdx.x == kLoader && dead) {
+            for (int s = 0; s < kStages; ++s) {
+                const int phases = (*issued + kStages - 1 - s) / kStages;
+                if (phases > 0) mbar_wait_bounded(&full[s], static_cast<uint32_t>(phases - 1) & 1, status);
+            }
+        }
+    }
+    if (cluster > 1) cluster_sync();
 }
 
 template <typename T, bool kTma, bool kMasks>
@@ -497,6 +518,7 @@ __global__ __launch_bounds__(kTileThreads, sizeof(T) == 2 ? kForwardResident : 3
     auto issue = [&](int item) {
         const int chain = item / walk.waves, segment = (item - chain * walk.waves) * cluster + rank;
         uint64_t *bar = &memory.full[item & 1];
+        *memory.issued = item + 1;
         if (segment >= segments) {  // no tile in the chain's last wave: an empty phase
             mbar_arrive(bar);
             return;
@@ -630,6 +652,7 @@ __global__ __launch_bounds__(kTileThreads, sizeof(T) == 2 ? kForwardResident : 3
         }
         if (rank == 0 && walks_in) final_state[batch * shape.features + walked] = carry;
     }
+    leave<kStages>(memory.full, memory.issued, cluster, dead, status);
 }
 
 // The waves run from the end. Per row a lane keeps a, k and u = (h' - k)(hi -
@@ -655,6 +678,7 @@ __global__ __launch_bounds__(kTileThreads, kBackwardResident) void gated_backwar
         const int chain = item / walk.waves, segment = (walk.waves - 1 - (item - chain * walk.waves)) * cluster + rank;
         const int stage = item % (kStages > 0 ? kStages : 1);
         uint64_t *bar = &memory.full[stage];
+        *memory.issued = item + 1;
         if (segment >= segments) {  // no tile in the chain's last wave: an empty phase
             mbar_arrive(bar);
             return;
@@ -840,6 +864,7 @@ __global__ __launch_bounds__(kTileThreads, kBackwardResident) void gated_backwar
         }
         if (grad_initial != nullptr && rank == 0 && walks_in) grad_initial[batch * shape.features + walked] = x;
     }
+    leave<kStages>(memory.full, memory.issued, cluster, dead, status);
 }
 
 // A tensor map over [batch, length, width] in boxes of one tile.

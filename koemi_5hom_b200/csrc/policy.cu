@@ -392,6 +392,7 @@ __device__ __forceinline__ float2 exp_from(float2 v, float from) {
 }
 
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Four floats into the same place of CTA `rank` of the cluster, counted on its
@@ -582,8 +583,9 @@ __global__ __launch_bounds__(kThreads, kSmBytes / kThreadBytes / kThreads) void 
         if (kSplit) {
             float4 *parts = met[taken & 1];
             uint64_t *bar = &meeting[taken & 1];
-            if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, cluster * sizeof(float4));
-            if (threadIdx.x < cluster) store_to_rank(parts + rank, bar, threadIdx.x, make_float4(all.max, all.sum, chosen, 0.0f));
+            // a CTA that gave up sends no more: the others give up too
+            if (threadIdx.x == 0 && !dead) mbar_arrive_expect_tx(bar, cluster * sizeof(float4));
+            if (threadIdx.x < cluster && !dead) store_to_rank(parts + rank, bar, threadIdx.x, make_float4(all.max, all.sum, chosen, 0.0f));
             if (!dead) dead = !mbar_wait_bounded<true>(bar, static_cast<uint32_t>(taken >> 1) & 1, status);
             const int lane = threadIdx.x & 31;
             all = warp_merge(lane < cluster ? Partial{parts[lane].x, parts[lane].y} : Partial{-INFINITY, 0.0f});
