@@ -88,9 +88,13 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // s and k of one element. With yp = 1 + e^-p and yc = 1 + e^2c, s = 1 / yp and
 // k = 1 - 2 / yc share one reciprocal, of yp yc; the exponents stop at 40,
 // where both have reached their limits in fp32, so that the product stays
-// finite. Both are good to a few 2^-24 of 1. For 16-bit inputs that is far
-// below the inputs' own rounding; fp32 inputs near 0 take tanh's series
-// instead (good to 2^-24 of k up to |c| = 1/4), since k is as small as c there.
+// finite. Both are good to a few 2^-24 of 1, which near 0 is not good enough
+// for k, as small as c there, and would make something of a c of 0. fp32
+// inputs take tanh's series up to |c| = 1/4 (good to 2^-24 of k); 16-bit inputs
+// below 2^-8 are their own tanh to 2^-17, and above the 2^-24s are 2^-14 of k
+// at most, a part of the inputs' own rounding (8 x 4096 x 1024 bf16 173 to 175
+// us a pass, 1 x 32768 x 2048 312 to 320).
+constexpr float kOwnTanh = 0.00390625f;
 template <typename T>
 __device__ __forceinline__ void gate_of(float p, float c, float &s, float &k) {
     constexpr float kLog2e = 1.4426950408889634f;
@@ -105,6 +109,8 @@ __device__ __forceinline__ void gate_of(float p, float c, float &s, float &k) {
         series = fmaf(z, series, 2.0f / 15.0f);
         series = fmaf(z, series, -1.0f / 3.0f);
         if (z < 0.0625f) k = fmaf(c * z, series, c);
+    } else if (fabsf(c) < kOwnTanh) {
+        k = c;
     }
 }
 
@@ -239,6 +245,9 @@ __device__ __forceinline__ void gates_of(float2 p, float2 c, float2 &s, float2 &
         series = fma2(mul2(c, z), series, c);
         if (z.x < 0.0625f) k.x = series.x;
         if (z.y < 0.0625f) k.y = series.y;
+    } else {
+        if (fabsf(c.x) < kOwnTanh) k.x = c.x;
+        if (fabsf(c.y) < kOwnTanh) k.y = c.y;
     }
 }
 

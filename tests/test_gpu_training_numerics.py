@@ -115,6 +115,34 @@ def test_recurrence_of_equal_and_narrow_retention_bounds(low, high, length, dtyp
     check_recurrence(*recurrence_case(3, length, 72, dtype, length, False, cuda), low=low, high=high)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length", [3, 40])
+def test_recurrence_of_small_candidates(length, dtype, cuda):
+    """A candidate near 0 is as good as one near 1, and one of exactly 0 adds exactly nothing. Bounds of one half make
+    every state half its candidate, each at a restart. 16-bit candidates below 2^-8 are their own tanh to 2^-17; from
+    there on the 16 roundings of k (as above) are 2^-12 of it; fp32 takes the series, a few roundings of k itself."""
+    g = torch.Generator().manual_seed(length)
+    p = 3 * torch.randn(2, length, 64, generator=g)
+    c = torch.randn(2, length, 64, generator=g) * torch.exp2(torch.randint(-23, -2, (2, length, 64), generator=g).float())
+    c[:, :, ::5] = 0.0
+    x = torch.cat((p, c), -1).to(dtype).to(cuda)
+    every = torch.ones(2, length, dtype=torch.bool, device=cuda)
+    states, _ = gated_recurrence(x, restart=every, minimum_retention=0.5, maximum_retention=0.5)
+    exact = 0.5 * torch.tanh(x[..., 64:].double())
+    check(states, exact, (2.0 ** -12 if dtype != torch.float32 else 16 * EPS) * exact.abs())
+    assert not states[:, :, ::5].any()
+
+
+@pytest.mark.parametrize("length", [1, 16, 64, 600])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_recurrence_of_zeros_stays_zero(dtype, length, cuda):
+    """Zero projections leave a zero state at zero, whatever the gates."""
+    x = torch.zeros(2, length, 2 * 64, device=cuda)
+    x[..., :64] = torch.linspace(-6, 6, 64, device=cuda)
+    states, final = gated_recurrence(x.to(dtype))
+    assert not states.any() and not final.any()
+
+
 # ------------------------------------------------------------- the policy loss
 
 CLIP_LOW, CLIP_HIGH, BETA = 0.2, 0.3, 0.05
