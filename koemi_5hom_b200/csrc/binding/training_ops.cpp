@@ -179,7 +179,8 @@ void check_forward(const Tensor &projections, const OptionalTensor &initial, con
                    const OptionalTensor &restart, double low, double high) {
     check_recurrence(projections, valid, restart);
     require("initial", initial, {projections.size(0), projections.size(2) / 2}, at::kFloat, projections);
-    TORCH_CHECK_VALUE(0.0 < low && low <= high && high < 1.0, "retention bounds must satisfy 0 < minimum <= maximum < 1");
+    const float lo = static_cast<float>(low), hi = static_cast<float>(high);  // as the kernels have them
+    TORCH_CHECK_VALUE(0.0f < lo && low <= high && hi < 1.0f, "retention bounds must satisfy 0 < minimum <= maximum < 1 in fp32");
 }
 
 std::tuple<Tensor, Tensor, Tensor> gated_forward(const Tensor &projections, const OptionalTensor &initial,
@@ -442,7 +443,7 @@ Route policy_forward(const Tensor &logits, const Tensor &targets, const Tensor &
     require("old", old, targets.sizes(), at::kFloat, logits);
     require("advantages", advantages, targets.sizes(), at::kFloat, logits);
     require("reference", reference, targets.sizes(), at::kFloat, logits);
-    TORCH_CHECK_VALUE(clip_low >= 0.0 && clip_high >= 0.0 && std::isfinite(kl_weight) &&
+    TORCH_CHECK_VALUE(clip_low >= 0.0 && clip_high >= 0.0 && std::isfinite(static_cast<float>(kl_weight)) &&
                           (kl_weight == 0.0 || (reference.has_value() && reference->defined())),
                       "clip widths must be non-negative, kl_weight finite and, without reference, zero");
     const Launch launch(logits);

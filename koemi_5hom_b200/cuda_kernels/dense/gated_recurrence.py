@@ -8,6 +8,8 @@ backward. There is no CPU fallback.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 from torch import Tensor
 
@@ -66,8 +68,8 @@ def _validate(projections, initial, valid, restart, low, high) -> None:
     for name, mask in (("valid", valid), ("restart", restart)):
         if mask is not None and (mask.shape != (batch, length) or mask.dtype != torch.bool):
             fail(f"{name} must be bool with shape {(batch, length)}, got {mask.dtype} {tuple(mask.shape)}")
-    if not 0.0 < low <= high < 1.0:
-        fail("retention bounds must satisfy 0 < minimum <= maximum < 1")
+    if not (0.0 < ctypes.c_float(low).value and low <= high and ctypes.c_float(high).value < 1.0):
+        fail("retention bounds must satisfy 0 < minimum <= maximum < 1 in fp32")
     if not projections.is_cuda and not native_cuda_available():
         raise DenseCudaUnavailableError("native gated recurrence requires torch CUDA support, a CUDA device, and the built kernel library")
     for value in (projections, initial, valid, restart):

@@ -8,6 +8,7 @@ factor of a scaled loss, are formed in the backward from the rows' kept maxima a
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import NamedTuple
 
@@ -80,8 +81,8 @@ def _validate(logits, targets, old, advantages, reference, valid, clip_low, clip
     for name, value, dtype in named[1:]:
         if value is not None and (value.shape != shape or value.dtype != dtype):
             fail(f"{name} must be {dtype} with shape {tuple(shape)}, got {value.dtype} {tuple(value.shape)}")
-    if not (clip_low >= 0.0 and clip_high >= 0.0 and math.isfinite(kl_weight)):
-        fail("clip widths must be non-negative and kl_weight finite")
+    if not (clip_low >= 0.0 and clip_high >= 0.0 and math.isfinite(ctypes.c_float(kl_weight).value)):
+        fail("clip widths must be non-negative and kl_weight finite in fp32")
     if kl_weight != 0.0 and reference is None:
         fail("kl_weight needs reference_log_probs")
     if not logits.is_cuda and not torch.cuda.is_available():
