@@ -107,3 +107,23 @@ def test_exchanges_inside_clusters_repeat(value, shape, dtype, cuda):
         results.append((result.detach(), *torch.autograd.grad(result, x)))
     for other in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+def test_forward_and_backward_in_a_cuda_graph(operator):
+    value, x = operator
+    x.requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            torch.autograd.grad(value(x), x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        result = value(x)
+        grad, = torch.autograd.grad(result, x)
+    with torch.no_grad():
+        x.copy_(x.flip(0))
+    graph.replay()
+    expected = value(x)
+    assert torch.equal(result, expected) and torch.equal(grad, torch.autograd.grad(expected, x)[0])

@@ -143,6 +143,20 @@ def test_recurrence_of_zeros_stays_zero(dtype, length, cuda):
     assert not states.any() and not final.any()
 
 
+@pytest.mark.parametrize("masks", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(3, 1, 64), (2, 8, 33), (3, 16, 40), (2, 17, 64), (1, 129, 515), (3, 200, 64), (2, 511, 72),
+                                   (1, 1025, 96), (1, 2100, 64), (40, 130, 136)])
+def test_recurrence_entry_by_entry(shape, dtype, masks, cuda):
+    check_recurrence(*recurrence_case(*shape, dtype, 100 + sum(shape), masks, cuda))
+
+
+def test_recurrence_of_clusters_entry_by_entry(cuda):
+    """A few long chains, which clusters of CTAs walk, exchanging their tiles' maps in every wave."""
+    for masks in (False, True):
+        check_recurrence(*recurrence_case(1, 9000, 64, torch.bfloat16, 31, masks, cuda))
+
+
 # ------------------------------------------------------------- the policy loss
 
 CLIP_LOW, CLIP_HIGH, BETA = 0.2, 0.3, 0.05
@@ -281,3 +295,14 @@ def test_rescale_refuses_what_the_kernel_cannot_take(cuda):
                  lambda: rescale(logits.clone(), logits, targets, None, kept, rows)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", POLICY_SHAPES)
+def test_policy_gradient_entry_by_entry(shape, dtype, cuda):
+    case = policy_case(*shape, dtype, 7 + sum(shape), cuda)
+    factor = factor_of(dtype)
+    want, lost = policy_gradient_with_bounds(case, factor)
+    got = gradient_of(case, factor=factor)
+    check(got, want, lost)
+    assert not got[~case["valid"]].any()
