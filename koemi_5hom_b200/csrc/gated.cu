@@ -54,7 +54,15 @@ constexpr int kTileThreads = kWarps * 32;
 constexpr int kBlocks = 2 * kWarps;             // half warps of a CTA
 constexpr int kRows = kSegment / kBlocks;       // rows of a half warp
 constexpr int kMaxCluster = 8;
-constexpr int kForwardResident = 4;  // CTAs per SM (registers, and shared memory of the 16-bit types)
+// CTAs per SM that the kernels are compiled for and the launches planned with:
+// forward four of 64 registers in 16 bits, and in fp32 three, which is what 74
+// KB of shared memory each let in. fp32 planned with two instead took 45 for 43 us at 64 x 128 x 2048 with
+// masks and as long elsewhere; compiled for two, 47 there and 124 for 131 at
+// 64 x 1024 x 1024 without masks.
+template <typename T>
+constexpr int forward_resident() {
+    return sizeof(T) == 2 ? 4 : 3;
+}
 constexpr int kBackwardResident = 2;
 constexpr int kShortLength = 16;  // up to here one thread walks a lane
 
@@ -510,7 +518,7 @@ __device__ __forceinline__ void leave(uint64_t *full, const int *issued, int clu
 }
 
 template <typename T, bool kTma, bool kMasks>
-__global__ __launch_bounds__(kTileThreads, sizeof(T) == 2 ? kForwardResident : 3) void gated_forward_tile_kernel(
+__global__ __launch_bounds__(kTileThreads, forward_resident<T>()) void gated_forward_tile_kernel(
     const __grid_constant__ CUtensorMap map, GatedShape shape, int64_t feature_tiles, int cluster, int per,
     const T *__restrict__ projections, const float *__restrict__ initial, T *__restrict__ states,
     float *__restrict__ final_state, float *__restrict__ carries, int *status) {
@@ -946,9 +954,8 @@ int gated_forward(const GatedShape &shape, const void *projections, const float 
     }
     const int64_t feature_tiles = ceil_div(shape.features, kTileFeatures);
     const int64_t chains = shape.batch * feature_tiles;
-    constexpr int kResident = sizeof(T) == 2 ? kForwardResident : 2;
-    const int cluster = cluster_size(shape, chains, kResident, kMaxCluster);
-    const int per = chains_per_cluster(shape, chains, cluster, kResident);
+    const int cluster = cluster_size(shape, chains, forward_resident<T>(), kMaxCluster);
+    const int per = chains_per_cluster(shape, chains, cluster, forward_resident<T>());
     const bool masks = shape.valid != nullptr || shape.restart != nullptr;
     int *status = device_status_word();
     CUtensorMap map{};
