@@ -4,7 +4,7 @@
 //   out = g min(1, max_norm / (norm + 1e-6))
 //
 // The tensors travel in the kernel's parameters, in a table of 16, 160 or 1000
-// (a launch copies the whole table, 28 KB of the largest), cut into chunks of
+// (a launch copies the whole table, 24 KB of the largest), cut into chunks of
 // kChunkElements; a CTA adds its chunks' sums of squares up into one partial,
 // and every CTA of the second kernel adds all partials in the same fixed
 // order, so equal inputs give equal bits. In place, a factor of one writes

@@ -30,18 +30,18 @@
 // Every byte is read and written once; the time is the arithmetic's and the
 // walk's beside HBM's. Batch x length x features, microseconds forward and
 // backward, and the fraction of the device's copy bandwidth:
-//   16 x 4096 x 1184 bf16   103, 0.69   163, 0.73   (places of the GPU filled)
-//   8 x 4096 x 1024 fp32     70, 0.88   115, 0.89   (half the arithmetic per byte)
-//   8 x 4096 x 1024 bf16     62, 0.49    85, 0.60   (256 chains: 3 or 4 CTAs an SM)
-//   1 x 32768 x 2048 bf16   120, 0.51   189, 0.54   (64 chains, in clusters of 8)
-//   256 x 128 x 2048 bf16   102, 0.61   167, 0.61   (one tile a chain)
-// In the first case the schedulers issue in 0.62 of their cycles and the
-// special-function units are busy for 0.53; the rest is waits at the tile's
+//   16 x 4096 x 1184 bf16   106, 0.67   168, 0.71   (places of the GPU filled)
+//   8 x 4096 x 1024 fp32     69, 0.90   111, 0.92   (half the arithmetic per byte)
+//   8 x 4096 x 1024 bf16     63, 0.49    86, 0.60   (256 chains: 3 or 4 CTAs an SM)
+//   1 x 32768 x 2048 bf16   125, 0.49   189, 0.54   (64 chains, in clusters of 8 and of 4)
+//   256 x 128 x 2048 bf16   108, 0.57   178, 0.58   (one tile a chain)
+// In the first case the schedulers issue in about six tenths of their cycles and
+// the special-function units are busy for half; the rest is waits at the tile's
 // barriers. Tiles of 64 x 64, of four warps with 16 rows each or of 16 with
 // four, three or four stages, and three CTAs per SM backward were slower. With
 // plain remote stores and cluster barriers, whose release waits for global
 // stores, and arithmetic on single floats, 8 x 4096 x 1024 bf16 with masks took
-// 177 us forward; it takes 63.
+// 177 us forward; it takes 66.
 #include "common.cuh"
 
 namespace koemi {

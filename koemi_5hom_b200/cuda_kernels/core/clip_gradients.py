@@ -24,9 +24,10 @@ def clip_gradients(gradients: Iterable[Tensor], max_norm: float, *, out: Sequenc
     """Scale ``gradients`` by ``min(1, max_norm / (norm + 1e-6))`` and return the norm before.
 
     ``norm`` is the 2-norm over all tensors (f32, bf16 and f16 may be mixed; any
-    shapes, contiguous, one device), an fp32 scalar on their device. In place by
-    default: nothing is written when the factor is one. With ``out`` (tensors of the same
-    sizes and dtypes, not overlapping the gradients) the scaled values go there.
+    shapes, contiguous, one device, none overlapping another), an fp32 scalar on their
+    device. In place by default: nothing is written when the factor is one. With ``out``
+    (tensors of the same sizes and dtypes, not overlapping the gradients) the scaled values
+    go there. No derivative passes through it, and dispatch modes do not see it.
     A norm that is not finite gives the formula's result: zeros and NaNs for an
     infinite norm, NaNs for a NaN.
     """
