@@ -818,6 +818,40 @@ KOEMI_API int koemi_core_clip_gradients(const uint64_t *gradients, const uint64_
                                         const int32_t *dtypes, int64_t count, float max_norm, float *norm,
                                         void *workspace, size_t workspace_bytes, void *stream);
 
+/* Layer norm: out = (x - mean) / sqrt(var + eps) * weight + bias over rows of
+ * `width` values (f32, f16, bf16). Row r of the values starts at
+ * (r / inner_rows) * outer_stride + (r % inner_rows) * inner_stride elements,
+ * its entries are contiguous; out is [rows, width]. weight and bias ([width],
+ * bias NULL: none) are both of weight_dtype: the values' dtype or fp32. stats
+ * ([2, rows] fp32, NULL: not wanted) receives the rows' means, then their
+ * 1 / sqrt(var + eps), which the backward needs. Statistics and sums are fp32. */
+KOEMI_API int koemi_core_layer_norm_forward(const void *values, int64_t rows, int64_t width, int64_t inner_rows,
+                                            int64_t outer_stride, int64_t inner_stride, const void *weight,
+                                            const void *bias, int weight_dtype, void *out, float *stats, float eps,
+                                            int dtype, void *stream);
+/* Its gradients from grad_out [rows, width]: grad_values [rows, width] (dtype),
+ * grad_weight and grad_bias [width] (weight_dtype), each NULL where it is not
+ * wanted. Without rows the weights' gradients are zeros. */
+KOEMI_API size_t koemi_core_layer_norm_backward_workspace(int64_t rows, int64_t width);
+KOEMI_API int koemi_core_layer_norm_backward(const void *values, int64_t rows, int64_t width, int64_t inner_rows,
+                                             int64_t outer_stride, int64_t inner_stride, const void *weight,
+                                             int weight_dtype, const float *stats, const void *grad_out,
+                                             void *grad_values, void *grad_weight, void *grad_bias, int dtype,
+                                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* Dropout from counters: out[e] = residual[e] + (lane(e) < dropped ? 0 :
+ * values[e] * 65536 / (65536 - dropped)) over `count` contiguous values (f32,
+ * f16, bf16; residual NULL: none; dropped in [0, 65536], 65536 drops all), with
+ *   key = mix(seed ^ mix(site ^ mix(step))), mix = SplitMix64's finaliser,
+ *   lane(e) = bits [16 (e % 4), 16 (e % 4) + 16) of
+ *             mix(key + (e / 4) * 0x9E3779B97F4A7C15).
+ * step_device (NULL: `step`) is read on the device in place of `step`, so that
+ * a captured graph draws other numbers at every replay. The gradient with
+ * respect to the values is the same call on the gradient of out. */
+KOEMI_API int koemi_core_dropout(const void *values, const void *residual, void *out, int64_t count, int64_t dropped,
+                                 uint64_t seed, uint64_t site, uint64_t step, const int64_t *step_device, int dtype,
+                                 void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -42,6 +42,7 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
+_u64 = ctypes.c_uint64
 
 # name -> (restype, argtypes); mirrors include/koemi_b200.h.
 SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
@@ -144,6 +145,11 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "koemi_think_policy_loss_scale": (_int, (_p, _i64, _p, _int, _p)),
     "koemi_core_clip_gradients_workspace": (_sz, (_p, _i64)),
     "koemi_core_clip_gradients": (_int, (_p, _p, _p, _p, _i64, _f, _p, _p, _sz, _p)),
+    "koemi_core_layer_norm_forward": (_int, (_p, _i64, _i64, _i64, _i64, _i64, _p, _p, _int, _p, _p, _f, _int, _p)),
+    "koemi_core_layer_norm_backward_workspace": (_sz, (_i64, _i64)),
+    "koemi_core_layer_norm_backward": (
+        _int, (_p, _i64, _i64, _i64, _i64, _i64, _p, _int, _p, _p, _p, _p, _p, _int, _p, _sz, _p)),
+    "koemi_core_dropout": (_int, (_p, _p, _p, _i64, _i64, _u64, _u64, _u64, _p, _int, _p)),
 }
 
 

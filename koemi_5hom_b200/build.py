@@ -6,7 +6,7 @@ Every ``csrc/*.cu`` translation unit is compiled by nvcc for
 linked into ``lib/libkoemi_b200.so`` with a static CUDA runtime, so the
 library depends on nothing but the driver. nvcc cross-compiles without a GPU.
 
-``csrc/binding/training_ops.cpp`` is compiled by g++ against the installed torch into
+``csrc/binding/*.cpp`` are compiled by g++ against the installed torch into
 ``lib/libkoemi_b200_torch.so``: the dispatcher ops and autograd formulas of the
 training operators, which open the kernel library at run time.
 
@@ -28,7 +28,7 @@ SOURCE_DIR = PACKAGE_DIR / "csrc"
 INCLUDE_DIR = PACKAGE_DIR.parent / "include"
 BUILD_DIR = PACKAGE_DIR.parent / "_build"
 LIBRARY_PATH = PACKAGE_DIR / "lib" / "libkoemi_b200.so"
-BINDING_SOURCE = SOURCE_DIR / "binding" / "training_ops.cpp"
+BINDING_DIR = SOURCE_DIR / "binding"
 BINDING_PATH = PACKAGE_DIR / "lib" / "libkoemi_b200_torch.so"
 
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
@@ -81,25 +81,40 @@ def build_binding(verbose: bool = False) -> Path:
         raise RuntimeError("g++ was not found; set CXX")
     root = Path(torch.__file__).resolve().parent
     cuda = Path(find_nvcc()).resolve().parent.parent
-    newest_input = max(p.stat().st_mtime for p in
-                       [BINDING_SOURCE, *INCLUDE_DIR.glob("*.h"), Path(__file__), root / "version.py"])
-    if BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= newest_input:
+    newest_header = max(p.stat().st_mtime for p in
+                        [*BINDING_DIR.glob("*.h"), *INCLUDE_DIR.glob("*.h"), Path(__file__), root / "version.py"])
+    sources = sorted(BINDING_DIR.glob("*.cpp"))
+    if BINDING_PATH.exists() and BINDING_PATH.stat().st_mtime >= max(newest_header, *(p.stat().st_mtime for p in sources)):
         return BINDING_PATH
     BINDING_PATH.parent.mkdir(parents=True, exist_ok=True)
+    BUILD_DIR.mkdir(parents=True, exist_ok=True)
+
+    def run(command: list[str], what: str) -> None:
+        if verbose:
+            print(" ".join(command), flush=True)
+        result = subprocess.run(command, capture_output=True, text=True)
+        if result.returncode != 0:
+            raise RuntimeError(f"{what} failed:\n{result.stdout}\n{result.stderr}")
+
+    def compile_one(source: Path) -> Path:
+        target = BUILD_DIR / f"binding_{source.stem}.o"
+        if not target.exists() or target.stat().st_mtime < max(newest_header, source.stat().st_mtime):
+            run([compiler, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                 "-I", str(INCLUDE_DIR), "-isystem", str(root / "include"),
+                 "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+                 "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_path("include"),
+                 "-c", str(source), "-o", str(target)], f"compiling {source.name}")
+        return target
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(sources)) as pool:
+        objects = list(pool.map(compile_one, sources))
     temporary = BINDING_PATH.with_suffix(".so.tmp")
-    command = [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-               "-I", str(INCLUDE_DIR), "-isystem", str(root / "include"),
-               "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
-               "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_path("include"), str(BINDING_SOURCE), "-o", str(temporary),
-               # torch's own C++ library: one linked in statically, as some compilers do by
-               # themselves, crashes where both sides' streams meet
-               "-l:libstdc++.so.6", "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python", "-ldl"]
-    if verbose:
-        print(" ".join(command), flush=True)
-    result = subprocess.run(command, capture_output=True, text=True)
-    if result.returncode != 0:
-        raise RuntimeError(f"compiling {BINDING_SOURCE.name} failed:\n{result.stdout}\n{result.stderr}")
+    run([compiler, "-shared", *map(str, objects), "-o", str(temporary),
+         # torch's own C++ library: one linked in statically, as some compilers do by
+         # themselves, crashes where both sides' streams meet
+         "-l:libstdc++.so.6", "-L", str(root / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python", "-ldl"],
+        "linking the torch binding")
     os.replace(temporary, BINDING_PATH)
     return BINDING_PATH
 

@@ -1,0 +1,147 @@
+// Dropout from a counter-based generator, with an optional residual, for
+// sm_100a: y = residual + (kept ? x * 65536 / (65536 - dropped) : 0).
+//
+// The mask is never stored: value e (row-major) has the 16 bits
+//   lane(e) = (splitmix64(key + (e / 4) * 0x9E3779B97F4A7C15) >> 16 (e % 4)) & 0xFFFF,
+//   key = splitmix64(seed ^ splitmix64(site ^ splitmix64(step))),
+// the sampler's generator (Steele, Lea and Flood's SplitMix finaliser, OOPSLA
+// 2014), and is dropped where lane(e) < dropped. The backward pass is the same
+// kernel on the gradient. With 16 bits a value the drop probability is a
+// multiple of 2^-16 and the scale is exactly its reciprocal's, so the mean is
+// unbiased; a word serves four values, which keeps the generator's 64-bit
+// products under the loads' time (two 32-bit lanes a word would not).
+//
+// Bound by bytes: x (and the residual) in, y out.
+#include <algorithm>
+
+#include "vec.cuh"
+
+namespace koemi {
+namespace {
+
+__device__ __forceinline__ uint64_t splitmix64(uint64_t z) {
+    z += 0x9E3779B97F4A7C15ull;
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    return z ^ (z >> 31);
+}
+
+struct Numbers {
+    uint64_t seed, site, step;
+    const int64_t *step_device;  // taken in place of `step` where it is given
+    uint32_t dropped;            // of 65536
+    float scale;
+};
+
+__device__ __forceinline__ uint64_t key_of(const Numbers &n) {
+    const uint64_t step = n.step_device != nullptr ? static_cast<uint64_t>(*n.step_device) : n.step;
+    return splitmix64(n.seed ^ splitmix64(n.site ^ splitmix64(step)));
+}
+
+__device__ __forceinline__ uint64_t word_of(uint64_t key, int64_t group) {
+    return splitmix64(key + static_cast<uint64_t>(group) * 0x9E3779B97F4A7C15ull);
+}
+
+constexpr int kThreads = 256;
+constexpr int kInFlight = 4;  // packets requested by a thread before the first is used
+
+template <typename T, bool kResidual>
+__global__ __launch_bounds__(kThreads) void dropout_kernel(const T *__restrict__ x, const T *__restrict__ residual, T *__restrict__ y,
+                                                           int64_t packets, int64_t count, const Numbers n) {
+    constexpr int W = Pack<T>::kWidth;
+    const uint64_t key = key_of(n);
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads * kInFlight + threadIdx.x;
+    uint4 vx[kInFlight], vr[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+        const int64_t p = first + u * kThreads;
+        if (p < packets) {
+            vx[u] = load_stream(x + p * W);
+            if (kResidual) vr[u] = load_stream(residual + p * W);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+        const int64_t p = first + u * kThreads;
+        if (p >= packets) break;
+        float v[W], r[W];
+        unpack(vx[u], v, T());
+        if (kResidual) unpack(vr[u], r, T());
+#pragma unroll
+        for (int q = 0; q < W / 4; ++q) {
+            const uint64_t word = word_of(key, p * (W / 4) + q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t lane = static_cast<uint32_t>(word >> (16 * e)) & 0xFFFFu;
+                const float kept = lane < n.dropped ? 0.0f : v[4 * q + e] * n.scale;
+                v[4 * q + e] = kResidual ? r[4 * q + e] + kept : kept;
+            }
+        }
+        store_stream(y + p * W, pack(v, T()));
+    }
+    // the values behind the last whole packet
+    if (blockIdx.x == 0 && threadIdx.x < count - packets * W) {
+        const int64_t i = packets * W + threadIdx.x;
+        const uint32_t lane = static_cast<uint32_t>(word_of(key, i >> 2) >> (16 * (i & 3))) & 0xFFFFu;
+        const float kept = lane < n.dropped ? 0.0f : to_acc(x[i]) * n.scale;
+        y[i] = from_acc<T>(kResidual ? to_acc(residual[i]) + kept : kept);
+    }
+}
+
+// Tensors that start off a 16-byte boundary.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void dropout_element_kernel(const T *__restrict__ x, const T *__restrict__ residual, T *__restrict__ y,
+                                                                   int64_t count, const Numbers n) {
+    const uint64_t key = key_of(n);
+    const int64_t group = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (group * 4 >= count) return;
+    const uint64_t word = word_of(key, group);
+    for (int e = 0; e < 4 && group * 4 + e < count; ++e) {
+        const int64_t i = group * 4 + e;
+        const uint32_t lane = static_cast<uint32_t>(word >> (16 * e)) & 0xFFFFu;
+        const float kept = lane < n.dropped ? 0.0f : to_acc(x[i]) * n.scale;
+        y[i] = from_acc<T>(residual != nullptr ? to_acc(residual[i]) + kept : kept);
+    }
+}
+
+template <typename T>
+int run(const void *x, const void *residual, void *y, int64_t count, const Numbers &n, cudaStream_t stream) {
+    const T *px = static_cast<const T *>(x), *pr = static_cast<const T *>(residual);
+    T *py = static_cast<T *>(y);
+    if (aligned(x, 16) && aligned(residual, 16) && aligned(y, 16)) {
+        const int64_t packets = count / Pack<T>::kWidth;
+        const int64_t blocks = std::max<int64_t>(1, ceil_div(packets, kThreads * kInFlight));
+        if (blocks > INT32_MAX) return fail(KOEMI_ERR_INVALID, "dropout of too many values");
+        if (residual != nullptr) {
+            dropout_kernel<T, true><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(px, pr, py, packets, count, n);
+        } else {
+            dropout_kernel<T, false><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(px, pr, py, packets, count, n);
+        }
+    } else {
+        const int64_t blocks = ceil_div(ceil_div(count, 4), kThreads);
+        if (blocks > INT32_MAX) return fail(KOEMI_ERR_INVALID, "dropout of too many values");
+        dropout_element_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(px, pr, py, count, n);
+    }
+    KOEMI_LAUNCH_CHECK();
+    return KOEMI_OK;
+}
+
+}  // namespace
+}  // namespace koemi
+
+using namespace koemi;
+
+extern "C" int koemi_core_dropout(const void *values, const void *residual, void *out, int64_t count, int64_t dropped, uint64_t seed,
+                                  uint64_t site, uint64_t step, const int64_t *step_device, int dtype, void *stream) {
+    clear_error();
+    if (count < 0) return fail(KOEMI_ERR_INVALID, "dropout of a negative number of values");
+    if (dropped < 0 || dropped > 65536) return fail(KOEMI_ERR_INVALID, "dropped must be in [0, 65536]");
+    if (dtype != KOEMI_F32 && dtype != KOEMI_F16 && dtype != KOEMI_BF16) return fail(KOEMI_ERR_INVALID, "unsupported dropout dtype %d", dtype);
+    if (count == 0) return KOEMI_OK;
+    if (values == nullptr || out == nullptr) return fail(KOEMI_ERR_INVALID, "values and out must be non-NULL");
+    const Numbers n{seed, site, step, step_device, static_cast<uint32_t>(dropped),
+                    dropped == 65536 ? 0.0f : static_cast<float>(65536.0 / (65536.0 - static_cast<double>(dropped)))};
+    if (dtype == KOEMI_F32) return run<float>(values, residual, out, count, n, as_stream(stream));
+    if (dtype == KOEMI_F16) return run<__half>(values, residual, out, count, n, as_stream(stream));
+    return run<__nv_bfloat16>(values, residual, out, count, n, as_stream(stream));
+}

@@ -1,7 +1,7 @@
 """The training operators' dispatcher ops: loading them, and their fake implementations.
 
 The ops (schemas, CUDA implementations, autograd formulas) live in C++, in
-``lib/libkoemi_b200_torch.so`` (csrc/binding/training_ops.cpp), so that neither a
+``lib/libkoemi_b200_torch.so`` (csrc/binding/), so that neither a
 call nor a backward pass on autograd's thread runs Python; their outputs and
 workspaces come from torch's caching allocator and their kernels run on the
 current stream, as those of ``_ops.py``. There is no CPU implementation: the
@@ -104,3 +104,20 @@ def _register_fakes() -> None:
     @fake("policy_loss_rescale")
     def _(gradient, logits, targets, valid, kept, factor):
         return None
+
+    @fake("layer_norm")
+    def _(values, weight, bias, eps):
+        return values.new_empty(values.shape)
+
+    @fake("layer_norm_keep")
+    def _(values, weight, bias, eps):
+        return values.new_empty(values.shape), values.new_empty((2, values.numel() // values.shape[-1]), **f32)
+
+    @fake("layer_norm_backward")
+    def _(values, weight, stats, grad, wanted):
+        return (values.new_empty(values.shape if wanted[0] else (0,)), weight.new_empty(weight.shape if wanted[1] else (0,)),
+                weight.new_empty(weight.shape if wanted[2] else (0,)))
+
+    @fake("dropout")
+    def _(values, residual, step, dropped, seed, site, step_number):
+        return values.new_empty(values.shape)
