@@ -852,6 +852,40 @@ KOEMI_API int koemi_core_dropout(const void *values, const void *residual, void 
                                  uint64_t seed, uint64_t site, uint64_t step, const int64_t *step_device, int dtype,
                                  void *stream);
 
+/* The gated feed-forward block over rows of values (f32, f16, bf16):
+ *   out = (silu(x Wg^T + bg) * (x Wv^T + bv)) Wo^T + bo,
+ * Wg and Wv [hidden_width, width], Wo [out_width, hidden_width], biases NULL or
+ * [hidden_width], [hidden_width], [out_width], all of dtype and contiguous; row
+ * r of the values starts at r * value_stride elements. kept (NULL: for
+ * inference) receives what the backward needs, of
+ * koemi_dense_gated_feed_forward_kept bytes. Products run on tensor cores with
+ * fp32 sums; fp32 operands as three bf16 parts each, to fp32's precision (an
+ * infinite fp32 operand gives NaN). 16-bit hidden values are rounded to the type,
+ * so an fp16 one past 65504 is infinite. workspace and kept start at multiples
+ * of 256 bytes. */
+KOEMI_API size_t koemi_dense_gated_feed_forward_kept(int64_t rows, int64_t hidden_width, int dtype);
+KOEMI_API size_t koemi_dense_gated_feed_forward_workspace(int64_t rows, int64_t width, int64_t hidden_width,
+                                                          int64_t out_width, int dtype, int backward);
+KOEMI_API int koemi_dense_gated_feed_forward_forward(const void *values, int64_t value_stride, const void *gate_weight,
+                                                     const void *value_weight, const void *output_weight,
+                                                     const void *gate_bias, const void *value_bias,
+                                                     const void *output_bias, void *out, void *kept, size_t kept_bytes,
+                                                     int64_t rows, int64_t width, int64_t hidden_width,
+                                                     int64_t out_width, int dtype, void *workspace,
+                                                     size_t workspace_bytes, void *stream);
+/* Its gradients from grad_out [rows, out_width]; each result is contiguous, of
+ * dtype, and NULL where it is not wanted. Without rows the weights' and biases'
+ * gradients are zeros. */
+KOEMI_API int koemi_dense_gated_feed_forward_backward(const void *values, int64_t value_stride, const void *gate_weight,
+                                                      const void *value_weight, const void *output_weight,
+                                                      const void *kept, size_t kept_bytes, const void *grad_out,
+                                                      void *grad_values, void *grad_gate_weight,
+                                                      void *grad_value_weight, void *grad_output_weight,
+                                                      void *grad_gate_bias, void *grad_value_bias,
+                                                      void *grad_output_bias, int64_t rows, int64_t width,
+                                                      int64_t hidden_width, int64_t out_width, int dtype,
+                                                      void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

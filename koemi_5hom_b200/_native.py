@@ -149,6 +149,12 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "koemi_core_layer_norm_backward_workspace": (_sz, (_i64, _i64)),
     "koemi_core_layer_norm_backward": (
         _int, (_p, _i64, _i64, _i64, _i64, _i64, _p, _int, _p, _p, _p, _p, _p, _int, _p, _sz, _p)),
+    "koemi_dense_gated_feed_forward_kept": (_sz, (_i64, _i64, _int)),
+    "koemi_dense_gated_feed_forward_workspace": (_sz, (_i64, _i64, _i64, _i64, _int, _int)),
+    "koemi_dense_gated_feed_forward_forward": (
+        _int, (_p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64, _int, _p, _sz, _p)),
+    "koemi_dense_gated_feed_forward_backward": (
+        _int, (_p, _i64, _p, _p, _p, _p, _sz, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _int, _p, _sz, _p)),
     "koemi_core_dropout": (_int, (_p, _p, _p, _i64, _i64, _u64, _u64, _u64, _p, _int, _p)),
 }
 

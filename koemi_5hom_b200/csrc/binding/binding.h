@@ -52,6 +52,10 @@ struct Library {
     decltype(&koemi_core_layer_norm_backward_workspace) norm_workspace;
     decltype(&koemi_core_layer_norm_backward) norm_backward;
     decltype(&koemi_core_dropout) dropout;
+    decltype(&koemi_dense_gated_feed_forward_kept) block_kept;
+    decltype(&koemi_dense_gated_feed_forward_workspace) block_workspace;
+    decltype(&koemi_dense_gated_feed_forward_forward) block_forward;
+    decltype(&koemi_dense_gated_feed_forward_backward) block_backward;
 };
 
 const Library &lib();  // refuses until koemi_torch_open has run

@@ -1,6 +1,9 @@
 // PyTorch operators of a feed-forward sub-layer over the C ABI of
-// libkoemi_b200.so: layer norm and dropout, with their autograd nodes (see
-// training_ops.cpp for why they are C++).
+// libkoemi_b200.so: layer norm, dropout and the gated block, with their autograd
+// nodes (see training_ops.cpp for why they are C++).
+#include <algorithm>
+#include <array>
+
 #include "binding.h"
 
 using namespace koemi_torch;
@@ -189,6 +192,169 @@ Tensor dropout_autograd(const Tensor &values, const OptionalTensor &residual, co
     return out;
 }
 
+// ------------------------------------------------------------ the gated block
+
+// The weights and biases of a call, in the order of its gradients after the values'.
+struct BlockShape {
+    int64_t rows, width, hidden, out, stride;
+    BlockShape(const Tensor &values, const Tensor &gate_weight, const Tensor &value_weight, const Tensor &output_weight,
+               const OptionalTensor &gate_bias, const OptionalTensor &value_bias, const OptionalTensor &output_bias) {
+        TORCH_CHECK_VALUE(one_of_ours(values) && values.dim() == 2 && values.size(1) > 0 && readable_rows(values),
+                          "values must be [rows, width] in f32, bf16 or f16 on a CUDA device");
+        TORCH_CHECK_VALUE(gate_weight.dim() == 2 && gate_weight.size(0) > 0 && output_weight.dim() == 2 && output_weight.size(0) > 0,
+                          "weights must be matrices with rows");
+        rows = values.size(0);
+        width = values.size(1);
+        hidden = gate_weight.size(0);
+        out = output_weight.size(0);
+        stride = rows > 1 ? values.stride(0) : width;
+        const auto type = values.scalar_type();
+        require("gate_weight", gate_weight, {hidden, width}, type, values);
+        require("value_weight", value_weight, {hidden, width}, type, values);
+        require("output_weight", output_weight, {out, hidden}, type, values);
+        require("gate_bias", gate_bias, {hidden}, type, values);
+        require("value_bias", value_bias, {hidden}, type, values);
+        require("output_bias", output_bias, {out}, type, values);
+    }
+    // Rows that do not overlap, their entries contiguous.
+    static bool readable_rows(const Tensor &values) {
+        return (values.size(1) == 1 || values.stride(1) == 1) && (values.size(0) <= 1 || values.stride(0) >= values.size(1));
+    }
+};
+
+Tensor rows_of(const Tensor &values) { return BlockShape::readable_rows(values) ? values : values.contiguous(); }
+
+Tensor bytes_of(const Tensor &like, size_t size) {
+    return at::empty({static_cast<int64_t>(std::max<size_t>(size, 256))}, like.options().dtype(at::kByte));
+}
+
+Tensor block_forward(const Tensor &values, const Tensor &gate_weight, const Tensor &value_weight, const Tensor &output_weight,
+                     const OptionalTensor &gate_bias, const OptionalTensor &value_bias, const OptionalTensor &output_bias, Tensor *kept) {
+    const BlockShape s(values, gate_weight, value_weight, output_weight, gate_bias, value_bias, output_bias);
+    const Launch launch(values);
+    const int code = code_of(values);
+    Tensor out = at::empty({s.rows, s.out}, values.options());
+    if (kept != nullptr) *kept = bytes_of(values, lib().block_kept(s.rows, s.hidden, code));
+    Tensor workspace = bytes_of(values, lib().block_workspace(s.rows, s.width, s.hidden, s.out, code, 0));
+    check("koemi_dense_gated_feed_forward_forward",
+          lib().block_forward(address<void>(values), s.stride, address<void>(gate_weight), address<void>(value_weight),
+                              address<void>(output_weight), address<void>(gate_bias), address<void>(value_bias),
+                              address<void>(output_bias), address<void>(out), kept != nullptr ? address<void>(*kept) : nullptr,
+                              kept != nullptr ? kept->numel() : 0, s.rows, s.width, s.hidden, s.out, code, address<void>(workspace),
+                              workspace.numel(), launch.stream));
+    return out;
+}
+
+Tensor gated_feed_forward_cuda(const Tensor &values_, const Tensor &gate_weight, const Tensor &value_weight, const Tensor &output_weight,
+                               const OptionalTensor &gate_bias, const OptionalTensor &value_bias, const OptionalTensor &output_bias) {
+    TORCH_CHECK_VALUE(values_.dim() > 0 && output_weight.dim() == 2 && values_.size(-1) > 0, "values must be [..., width], weights matrices");
+    const Tensor values = values_.dim() == 2 ? values_ : values_.reshape({values_.numel() / values_.size(-1), values_.size(-1)});
+    Tensor out = block_forward(rows_of(values), gate_weight.contiguous(), value_weight.contiguous(), output_weight.contiguous(),
+                               dense(gate_bias), dense(value_bias), dense(output_bias), nullptr);
+    if (values_.dim() == 2) return out;
+    auto sizes = values_.sizes().vec();
+    sizes.back() = out.size(1);
+    return out.view(sizes);
+}
+
+std::tuple<Tensor, Tensor> gated_feed_forward_keep_cuda(const Tensor &values, const Tensor &gate_weight, const Tensor &value_weight,
+                                                        const Tensor &output_weight, const OptionalTensor &gate_bias,
+                                                        const OptionalTensor &value_bias, const OptionalTensor &output_bias) {
+    Tensor kept;
+    Tensor out = block_forward(values, gate_weight, value_weight, output_weight, gate_bias, value_bias, output_bias, &kept);
+    return {out, kept};
+}
+
+// Gradients of values, gate_weight, value_weight, output_weight and the three
+// biases, bit k of `wanted` for the k-th; one that is not wanted is empty.
+std::vector<Tensor> gated_feed_forward_backward_cuda(const Tensor &values, const Tensor &gate_weight, const Tensor &value_weight,
+                                                     const Tensor &output_weight, const Tensor &kept, const Tensor &grad, int64_t wanted) {
+    const OptionalTensor none;
+    const BlockShape s(values, gate_weight, value_weight, output_weight, none, none, none);
+    const Launch launch(values);
+    const int code = code_of(values);
+    require("grad", grad, {s.rows, s.out}, values.scalar_type(), values);
+    TORCH_CHECK_VALUE(kept.scalar_type() == at::kByte && kept.is_contiguous() && kept.device() == values.device() &&
+                          kept.numel() >= static_cast<int64_t>(lib().block_kept(s.rows, s.hidden, code)),
+                      "kept is not what the forward of these values returned");
+    const std::vector<int64_t> sizes[] = {{s.rows, s.width}, {s.hidden, s.width}, {s.hidden, s.width}, {s.out, s.hidden}, {s.hidden}, {s.hidden}, {s.out}};
+    std::vector<Tensor> grads;
+    void *p[7];
+    for (int k = 0; k < 7; ++k) {
+        const bool want = wanted >> k & 1;
+        grads.push_back(want ? at::empty(sizes[k], values.options()) : at::empty({0}, values.options()));
+        p[k] = want ? address<void>(grads.back()) : nullptr;
+    }
+    Tensor workspace = bytes_of(values, lib().block_workspace(s.rows, s.width, s.hidden, s.out, code, 1));
+    check("koemi_dense_gated_feed_forward_backward",
+          lib().block_backward(address<void>(values), s.stride, address<void>(gate_weight), address<void>(value_weight),
+                               address<void>(output_weight), address<void>(kept), kept.numel(), address<void>(grad), p[0], p[1], p[2],
+                               p[3], p[4], p[5], p[6], s.rows, s.width, s.hidden, s.out, code, address<void>(workspace),
+                               workspace.numel(), launch.stream));
+    return grads;
+}
+
+struct GatedFeedForwardBackward final : torch::autograd::Node {
+    SavedVariable values, gate_weight, value_weight, output_weight, kept;
+    variable_list apply(variable_list &&grads) override {
+        first_order_only();
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list result(7);
+        if (!grads[0].defined()) return result;
+        const Tensor values_ = values.unpack(), gate = gate_weight.unpack(), value = value_weight.unpack(), output = output_weight.unpack();
+        const Tensor kept_ = kept.unpack();
+        const BelowAutograd below;
+        int64_t wanted = 0;
+        for (int k = 0; k < 7; ++k) wanted |= static_cast<int64_t>(task_should_compute_output(k)) << k;
+        KOEMI_OP(gated_feed_forward_backward, decltype(gated_feed_forward_backward_cuda));
+        auto found = gated_feed_forward_backward.call(values_, gate, value, output, kept_, grads[0].contiguous(), wanted);
+        for (int k = 0; k < 7; ++k) {
+            if (wanted >> k & 1) result[k] = found[k];
+        }
+        return result;
+    }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *saved : {&values, &gate_weight, &value_weight, &output_weight, &kept}) saved->reset_data();
+    }
+    std::string name() const override { return "GatedFeedForwardBackward"; }
+};
+
+Tensor gated_feed_forward_autograd(const Tensor &values_, const Tensor &gate_weight_, const Tensor &value_weight_, const Tensor &output_weight_,
+                                   const OptionalTensor &gate_bias_, const OptionalTensor &value_bias_, const OptionalTensor &output_bias_) {
+    reverse_mode_only(values_, gate_weight_, value_weight_, output_weight_, gate_bias_, value_bias_, output_bias_);
+    if (!(at::GradMode::is_enabled() && (differentiates(values_) || differentiates(gate_weight_) || differentiates(value_weight_) ||
+                                         differentiates(output_weight_) || differentiates(gate_bias_) || differentiates(value_bias_) ||
+                                         differentiates(output_bias_)))) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        KOEMI_OP(gated_feed_forward, decltype(gated_feed_forward_cuda));
+        return gated_feed_forward.call(values_, gate_weight_, value_weight_, output_weight_, gate_bias_, value_bias_, output_bias_);
+    }
+    TORCH_CHECK_VALUE(values_.dim() > 0 && output_weight_.dim() == 2 && values_.size(-1) > 0, "values must be [..., width], weights matrices");
+    // differentiably
+    const Tensor values = rows_of(values_.dim() == 2 ? values_ : values_.reshape({values_.numel() / values_.size(-1), values_.size(-1)}));
+    const Tensor gate_weight = gate_weight_.contiguous(), value_weight = value_weight_.contiguous(), output_weight = output_weight_.contiguous();
+    const OptionalTensor gate_bias = dense(gate_bias_), value_bias = dense(value_bias_), output_bias = dense(output_bias_);
+    auto node = node_of<GatedFeedForwardBackward>(values, gate_weight, value_weight, output_weight, gate_bias.value_or(Tensor()),
+                                                  value_bias.value_or(Tensor()), output_bias.value_or(Tensor()));
+    Tensor out, kept;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        KOEMI_OP(gated_feed_forward_keep, decltype(gated_feed_forward_keep_cuda));
+        std::tie(out, kept) = gated_feed_forward_keep.call(values, gate_weight, value_weight, output_weight, gate_bias, value_bias, output_bias);
+    }
+    node->values = SavedVariable(values, false);
+    node->gate_weight = SavedVariable(gate_weight, false);
+    node->value_weight = SavedVariable(value_weight, false);
+    node->output_weight = SavedVariable(output_weight, false);
+    node->kept = SavedVariable(kept, false);
+    torch::autograd::set_history(out, node);
+    if (values_.dim() == 2) return out;
+    auto sizes = values_.sizes().vec();
+    sizes.back() = out.size(1);
+    return out.view(sizes);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(koemi_b200, m) {
@@ -196,6 +362,9 @@ TORCH_LIBRARY_FRAGMENT(koemi_b200, m) {
     m.def("layer_norm_keep(Tensor values, Tensor weight, Tensor? bias, float eps) -> (Tensor, Tensor)");
     m.def("layer_norm_backward(Tensor values, Tensor weight, Tensor stats, Tensor grad, bool[3] wanted) -> (Tensor, Tensor, Tensor)");
     m.def("dropout(Tensor values, Tensor? residual, Tensor? step, int dropped, int seed, int site, int step_number) -> Tensor");
+    m.def("gated_feed_forward(Tensor values, Tensor gate_weight, Tensor value_weight, Tensor output_weight, Tensor? gate_bias, Tensor? value_bias, Tensor? output_bias) -> Tensor");
+    m.def("gated_feed_forward_keep(Tensor values, Tensor gate_weight, Tensor value_weight, Tensor output_weight, Tensor? gate_bias, Tensor? value_bias, Tensor? output_bias) -> (Tensor, Tensor)");
+    m.def("gated_feed_forward_backward(Tensor values, Tensor gate_weight, Tensor value_weight, Tensor output_weight, Tensor kept, Tensor grad, int wanted) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(koemi_b200, CUDA, m) {
@@ -203,10 +372,16 @@ TORCH_LIBRARY_IMPL(koemi_b200, CUDA, m) {
     m.impl("layer_norm_keep", layer_norm_keep_cuda);
     m.impl("layer_norm_backward", layer_norm_backward_cuda);
     m.impl("dropout", dropout_cuda);
+    m.impl("gated_feed_forward", gated_feed_forward_cuda);
+    m.impl("gated_feed_forward_keep", gated_feed_forward_keep_cuda);
+    m.impl("gated_feed_forward_backward", gated_feed_forward_backward_cuda);
 }
 
 TORCH_LIBRARY_IMPL(koemi_b200, Autograd, m) {
     m.impl("layer_norm", layer_norm_autograd);
     m.impl("dropout", dropout_autograd);
-    for (const char *inner : {"layer_norm_keep", "layer_norm_backward"}) m.impl(inner, torch::autograd::autogradNotImplementedFallback());
+    m.impl("gated_feed_forward", gated_feed_forward_autograd);
+    for (const char *inner : {"layer_norm_keep", "layer_norm_backward", "gated_feed_forward_keep", "gated_feed_forward_backward"}) {
+        m.impl(inner, torch::autograd::autogradNotImplementedFallback());
+    }
 }

@@ -524,6 +524,10 @@ extern "C" __attribute__((visibility("default"))) const char *koemi_torch_open(c
     take(library.norm_workspace, "koemi_core_layer_norm_backward_workspace");
     take(library.norm_backward, "koemi_core_layer_norm_backward");
     take(library.dropout, "koemi_core_dropout");
+    take(library.block_kept, "koemi_dense_gated_feed_forward_kept");
+    take(library.block_workspace, "koemi_dense_gated_feed_forward_workspace");
+    take(library.block_forward, "koemi_dense_gated_feed_forward_forward");
+    take(library.block_backward, "koemi_dense_gated_feed_forward_backward");
     opened = message.empty();
     return opened ? nullptr : message.c_str();
 }

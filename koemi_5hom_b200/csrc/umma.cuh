@@ -17,6 +17,19 @@ __device__ __forceinline__ uint64_t sw128_kmajor_desc(uint32_t smem_address) {
     return desc;
 }
 
+// A tile whose rows are K (128 bytes of M or N each, 64 K rows a tile, tiles of
+// 64 M or N entries one after the other): repeats along M or N every 8192
+// bytes, along K every 8 rows.
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_address) {
+    uint64_t desc = 0;
+    desc |= static_cast<uint64_t>((smem_address & 0x3FFFF) >> 4);
+    desc |= static_cast<uint64_t>(8192 >> 4) << 16;  // LBO: the next 64 entries of M or N
+    desc |= static_cast<uint64_t>(1024 >> 4) << 32;  // SBO: the next 8 rows of K
+    desc |= static_cast<uint64_t>(1) << 46;
+    desc |= static_cast<uint64_t>(2) << 61;
+    return desc;
+}
+
 __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t accumulate) {
     asm volatile(

@@ -121,3 +121,18 @@ def _register_fakes() -> None:
     @fake("dropout")
     def _(values, residual, step, dropped, seed, site, step_number):
         return values.new_empty(values.shape)
+
+    @fake("gated_feed_forward")
+    def _(values, gate_weight, value_weight, output_weight, gate_bias, value_bias, output_bias):
+        return values.new_empty((*values.shape[:-1], output_weight.shape[0]))
+
+    @fake("gated_feed_forward_keep")
+    def _(values, gate_weight, value_weight, output_weight, gate_bias, value_bias, output_bias):
+        kept = _native.library().koemi_dense_gated_feed_forward_kept(values.shape[0], gate_weight.shape[0], _native.dtype_code(values.dtype))
+        return values.new_empty((values.shape[0], output_weight.shape[0])), values.new_empty((max(kept, 256),), dtype=torch.uint8)
+
+    @fake("gated_feed_forward_backward")
+    def _(values, gate_weight, value_weight, output_weight, kept, grad, wanted):
+        hidden, out = gate_weight.shape[:1], output_weight.shape[:1]
+        shapes = (values.shape, gate_weight.shape, gate_weight.shape, output_weight.shape, hidden, hidden, out)
+        return [values.new_empty(shape if wanted >> k & 1 else (0,)) for k, shape in enumerate(shapes)]

@@ -9,7 +9,7 @@ from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 from koemi_5hom_b200 import _native
-from koemi_5hom_b200.cuda_kernels import _training, core
+from koemi_5hom_b200.cuda_kernels import _training, core, dense
 from koemi_5hom_b200.cuda_kernels.loader import CudaExtensionUnavailableError, CudaExtensionValidationError
 
 cpu_only = pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-CUDA contract")
@@ -61,6 +61,34 @@ def test_dropout_refusals():
             call()
 
 
+def test_block_refusals():
+    x, g, v, o = torch.rand(2, 3, 8), torch.rand(16, 8), torch.rand(16, 8), torch.rand(4, 16)
+    block = dense.gated_feed_forward
+    refused(((lambda: block(torch.tensor(1.0), g, v, o), "shape"),
+             (lambda: block(torch.rand(2, 0), torch.rand(4, 0), torch.rand(4, 0), torch.rand(2, 4)), "positive width"),
+             (lambda: block(x.double(), g, v, o), "unsupported CUDA dtype"),
+             (lambda: block(x, g[0], v, o), "gate_weight must have shape"),
+             (lambda: block(x, g[:, :7], v[:, :7], o), "gate_weight must have shape"),
+             (lambda: block(x, g[:0], v[:0], o[:, :0]), "gate_weight must have shape"),
+             (lambda: block(x, g, v[:15], o), "value_weight must have shape"),
+             (lambda: block(x, g, v, o[:, :15]), "output_weight must have shape"),
+             (lambda: block(x, g, v, o[:0]), "output_weight must have shape"),
+             (lambda: block(x, g, v, o, gate_bias=torch.rand(15)), "gate_bias must have shape"),
+             (lambda: block(x, g, v, o, output_bias=torch.rand(1, 4)), "output_bias must have shape"),
+             (lambda: block(x, g, v.half(), o), "value_weight must use"),
+             (lambda: block(x.half(), g.half(), v.half(), o.half(), value_bias=torch.rand(16)), "value_bias must use")),
+            dense.DenseCudaValidationError)
+    for call in (lambda: block([1.0], g, v, o), lambda: block(x, None, v, o), lambda: block(x, g, v, o, value_bias=1.0)):
+        with pytest.raises(TypeError):
+            call()
+
+
+@cpu_only
+def test_block_reports_unavailable_without_cuda():
+    with pytest.raises(dense.DenseCudaUnavailableError):
+        dense.gated_feed_forward(torch.rand(2, 8), torch.rand(16, 8), torch.rand(16, 8), torch.rand(4, 16))
+
+
 @cpu_only
 def test_cpu_tensors_are_refused():
     x, w = torch.rand(2, 8), torch.rand(8)
@@ -76,6 +104,10 @@ def test_tensors_of_another_device_are_refused(cuda):
              (lambda: core.layer_norm(x, w, w.cpu()), "one CUDA device"), (lambda: core.dropout(x.cpu(), 0.1, seed=1), "one CUDA device"),
              (lambda: core.dropout(x, 0.1, seed=1, residual=x.cpu()), "one CUDA device"),
              (lambda: core.dropout(x, 0.1, seed=1, step=torch.tensor(1)), "one CUDA device")), CudaExtensionValidationError)
+    g, o = torch.rand(16, 8, device=cuda), torch.rand(4, 16, device=cuda)
+    refused(((lambda: dense.gated_feed_forward(x, g, g.cpu(), o), "one CUDA device"),
+             (lambda: dense.gated_feed_forward(x.cpu(), g, g, o), "one CUDA device"),
+             (lambda: dense.gated_feed_forward(x, g, g, o, output_bias=torch.rand(4)), "one CUDA device")), dense.DenseCudaValidationError)
 
 
 def test_entries_refuse_bad_arguments_before_touching_the_device():
@@ -106,6 +138,31 @@ def test_entries_refuse_bad_arguments_before_touching_the_device():
     def drop(count=4, dropped=100, dtype=_native.F32, values=one):
         return lib.koemi_core_dropout(values, None, one, count, dropped, 1, 2, 3, None, dtype, None)
 
+    kept = lib.koemi_dense_gated_feed_forward_kept(10, 20, _native.BF16)
+    assert kept == 3 * 512 and lib.koemi_dense_gated_feed_forward_kept(-1, 20, _native.BF16) == 0  # 10 x 24 values thrice
+    assert lib.koemi_dense_gated_feed_forward_kept(10, 20, _native.F32) == 1536 + 2 * 1024  # three bf16 parts, two fp32 matrices
+    rooms = [lib.koemi_dense_gated_feed_forward_workspace(10, 16, 20, 8, _native.BF16, backward) for backward in (0, 1)]
+    assert min(rooms) > 0 and lib.koemi_dense_gated_feed_forward_workspace(10, 16, 20, 8, 99, 0) == 0
+    page = ctypes.c_void_p(256)
+
+    def block(rows=10, width=16, hidden=20, out=8, stride=16, dtype=_native.BF16, values=page, keep=page, keep_bytes=kept, room=rooms[0], ws=page):
+        return lib.koemi_dense_gated_feed_forward_forward(values, stride, page, page, page, None, None, None, page, keep, keep_bytes, rows,
+                                                          width, hidden, out, dtype, ws, room, None)
+
+    assert block(rows=-1) == invalid and block(width=0) == invalid and block(hidden=0) == invalid and block(out=0) == invalid
+    assert block(rows=1 << 31) == invalid and block(hidden=1 << 25) == invalid and block(stride=15) == invalid
+    assert block(dtype=_native.I32) == invalid and block(values=None) == invalid and block(rows=0) == 0
+    assert block(keep_bytes=kept - 1) == workspace and block(keep=one) == workspace
+    assert block(room=rooms[0] - 1) == workspace and block(ws=None) == workspace and block(ws=one) == workspace
+
+    def block_backward(rows=10, stride=16, dtype=_native.BF16, keep=page, grad=page, room=rooms[1]):
+        return lib.koemi_dense_gated_feed_forward_backward(page, stride, page, page, page, keep, kept, grad, page, page, page, page, page, page,
+                                                           page, rows, 16, 20, 8, dtype, page, room, None)
+
+    assert block_backward(rows=-1) == invalid and block_backward(stride=3) == invalid and block_backward(dtype=99) == invalid
+    assert block_backward(keep=None) == invalid and block_backward(grad=None) == invalid and block_backward(keep=one) == workspace
+    assert block_backward(room=rooms[1] - 1) == workspace
+
     assert drop(count=-1) == invalid and drop(dropped=-1) == invalid and drop(dropped=65537) == invalid
     assert drop(dtype=_native.BOOL) == invalid and drop(values=None) == invalid and drop(count=0) == 0
 
@@ -120,7 +177,11 @@ def dropout_value(x):
     return torch.ops.koemi_b200.dropout(x, 2 * x, None, 6554, 1, 2, 3).sum()
 
 
-SCALARS = {"norm": norm_value, "dropout": dropout_value}
+def block_value(x):
+    return torch.ops.koemi_b200.gated_feed_forward(x.view(2, 3, 16), x[0].expand(8, 16), x[1:2].expand(8, 16), x[:4, :8], x[0, :8], None, x[1, :4]).sum()
+
+
+SCALARS = {"norm": norm_value, "dropout": dropout_value, "block": block_value}
 
 
 @pytest.fixture(params=SCALARS, ids=SCALARS)
@@ -142,14 +203,15 @@ def test_forward_mode_is_refused(operator):
         value(forward_ad.make_dual(x, torch.ones_like(x)))
 
 
-def test_second_orders_of_the_norm_are_refused():
+@pytest.mark.parametrize("value", [norm_value, block_value])
+def test_second_orders_are_refused(value):
     _training.register()
     x = torch.zeros(6, 16, device="meta")
     with pytest.raises(RuntimeError, match="not implemented"):
-        torch.func.grad(lambda t: torch.func.grad(norm_value)(t).sum())(x)
+        torch.func.grad(lambda t: torch.func.grad(value)(t).sum())(x)
     leaf = x.requires_grad_(True)
     with pytest.raises(RuntimeError, match="first order"):
-        torch.autograd.grad(norm_value(leaf), leaf, create_graph=True)
+        torch.autograd.grad(value(leaf), leaf, create_graph=True)
 
 
 def test_dropout_has_every_order():
