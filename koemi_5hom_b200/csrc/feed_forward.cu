@@ -757,24 +757,26 @@ struct Cut {
     int tile_n, ctas, splits;
 };
 
-// The cheapest of the cuts by clocks: a K block costs a CTA 512 clocks of
-// tensor pipe per 256 columns, and no less than its bytes at about 64 a clock
-// from L2 (128 x 256 tiles load 48 KB: 768; a pair's CTAs 32 KB each); a tile
-// adds about 1500 for its first loads and its last epilogue; parts of K add a
-// kernel and their accumulators' way through L2.
+// The cheapest of the cuts by clocks: an SM takes about 52 bytes a clock from
+// L2 (measured with all SMs loading: 128 x 256 tiles 51, 128 x 128 tiles 53),
+// which is what a K block of every shape but a pair's 256 x 256 waits for; a
+// launch adds about 6500 for its first loads and its last epilogue; parts of K
+// add a kernel and their accumulators' way through L2.
 Cut cut_of(int64_t m, int64_t n, int total_k, bool gate, int parts, int sms) {
     Cut best{128, 1, 1};
     double least = 1e30;
-    const struct { int tile_n, ctas; double clocks; } shapes[] = {{256, 1, 768}, {128, 1, 512}, {64, 1, 384}};
+    const struct { int tile_n, ctas; } shapes[] = {{256, 2}, {128, 2}, {256, 1}, {128, 1}, {64, 1}};
     for (const auto &shape : shapes) {
         if (parts > 1 && shape.tile_n > 128) continue;  // the sums of the passes have to fit registers
+        if (shape.ctas == 2 && m <= kBM) continue;
+        const double clocks = std::max(shape.tile_n * 2.0, (kBM + shape.tile_n / shape.ctas) * kBK * 2 / 52.0);
         const int64_t units = gate ? shape.tile_n / 2 : shape.tile_n;
         const int64_t tiles = ceil_div(m, kBM * shape.ctas) * ceil_div(n, units), places = std::max(1, sms / shape.ctas);
         for (int splits = 1; splits <= 64 && splits <= total_k; splits += splits < 8 ? 1 : splits / 4) {
             const int per = static_cast<int>(ceil_div(total_k, splits));
             if (ceil_div(total_k, per) != splits) continue;  // every part has blocks
             const double waves = static_cast<double>(ceil_div(tiles * splits, places));
-            double cost = waves * per * shape.clocks + 1500;
+            double cost = waves * per * clocks + 6500;
             if (splits > 1) cost += 6000 + (gate ? 2.0 : 1.0) * static_cast<double>(m) * static_cast<double>(n) * (splits + 1) * 4 / 2500;
             if (cost < least) least = cost, best = Cut{shape.tile_n, shape.ctas, splits};
         }
@@ -846,9 +848,9 @@ int multiply(const Product &p, GemmArgs args, float *partials, cudaStream_t stre
     if (cut.tile_n == 64) {
         rc = launch_shape<T, kEpilogue, 64, 1>(args, stream);
     } else if (cut.tile_n == 128) {
-        rc = launch_shape<T, kEpilogue, 128, 1>(args, stream);
+        rc = cut.ctas == 2 ? launch_shape<T, kEpilogue, 128, 2>(args, stream) : launch_shape<T, kEpilogue, 128, 1>(args, stream);
     } else if constexpr (sizeof(T) == 2) {
-        rc = launch_shape<T, kEpilogue, 256, 1>(args, stream);
+        rc = cut.ctas == 2 ? launch_shape<T, kEpilogue, 256, 2>(args, stream) : launch_shape<T, kEpilogue, 256, 1>(args, stream);
     }
     if (rc != KOEMI_OK) return rc;
     if (cut.splits > 1) {
