@@ -17,11 +17,12 @@
 //
 // fp32 values are split into three bf16 parts (8 bits each, together the 24 of
 // fp32), x = x0 + x1 + x2 with |x1| <= 2^-9 |x0|, |x2| <= 2^-18 |x0|, and a
-// product is the six part products that matter, added up smallest first in the
-// same fp32 accumulator: x0 y2, x2 y0, x1 y1, x0 y1, x1 y0, x0 y0. What is left
-// out is below 2^-26 of |x y|. Six bf16 products run several times faster than
-// fp32 FMAs. 16-bit operands whose rows TMA cannot describe (a width that is no
-// multiple of 8, a start off 16 bytes) are copied to padded rows first.
+// product is the six part products that matter, x0 y0, x0 y1, x1 y0, x1 y1, x0 y2
+// and x2 y0: x0 y0 in one accumulator, the others, 2^-9 of it and less, in a
+// second one, where they are not cut off at the first one's last place. What is
+// left out is below 2^-26 of |x y|. Six bf16 products run several times faster than fp32 FMAs. 16-bit operands whose rows TMA
+// cannot describe (a width that is no multiple of 8, a start off 16 bytes) are
+// copied to padded rows first.
 //
 // In 16 bits h, p, q, dp and dq are rounded to the type between two products
 // (h, dp and dq because the tensor cores take no wider operand, p and q because
@@ -41,13 +42,18 @@ constexpr int kThreads = (2 + kEpilogueWarps) * 32;
 constexpr uint32_t kABytes = kBM * kBK * 2;
 constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr int kMaxStages = 8;
+constexpr int kMaxJobs = 4;
+// An epilogue warp's staging area: 32 rows of 64 bytes, 16 apart so that rows written 16
+// bytes a lane fall into different banks.
+constexpr int kStagedRow = 64 + 16;
+constexpr uint32_t kStagedBytes = 32 * kStagedRow;
 // The tensor cores cut off what an fp32 accumulator cannot hold, which 256
 // instructions in a row turn into 2e-6 of the result. Where that is too much,
 // for fp32 values, the accumulators are added up in registers, rounded to
-// nearest, every kPass K blocks (32 instructions).
+// nearest, every kPass K blocks (32 instructions on x0 y0).
 constexpr int kPass = 8;
 constexpr uint32_t kTmemColumns = 512;
-constexpr size_t kSmemBytes = 1024 + kRingBytes + 256;
+constexpr size_t kSmemBytes = 1024 + kRingBytes + kEpilogueWarps * kStagedBytes + 256;
 static_assert((2 * kMaxStages + 4) * 8 + 8 <= 256, "barrier area");
 
 enum Epilogue : int { kGate = 0, kInner = 1, kOut = 2 };
@@ -70,15 +76,15 @@ struct Parts {
     int64_t ld, part_stride;  // elements
 };
 
-struct GemmArgs {
+// One product, D = A B, or A B + A' B' (two segments of K).
+struct Job {
     CUtensorMap a[2], b[2];  // a segment's operands; kGate: b[0] and b[1] are the gate's and the value's weights
-    int segments;            // D = sum over segments of A B
-    int k_blocks[2];         // K blocks of a segment
-    int pairs;               // part products: 1 or 6
+    int first_blocks;        // K blocks of the first segment
+    int total_k, splits, k_per_split;
     int a_mn, b_mn;          // MN-major operands
+    uint32_t idesc;
     int64_t m, n;            // rows and columns of the result (kGate: hidden units)
-    int m_tiles, n_tiles, splits, band;
-    int total_k, k_per_split;
+    int m_tiles, n_tiles, tiles, band;
     const void *bias0, *bias1;
     void *out;               // kOut
     int64_t ld_out;
@@ -87,8 +93,16 @@ struct GemmArgs {
     int64_t ld_pq;
     float *partials;         // splits > 1: raw accumulators [split][gate | value][m][ld_partial]
     int64_t ld_partial;
+};
+
+// Independent products in one launch, in two classes of equal K: the tiles of
+// the longer class go round the places first, `ahead` places get one more, the
+// others catch up on `catch_up` tiles of the second class, and the rest go round.
+struct GemmArgs {
+    Job jobs[kMaxJobs];
+    int job_count, first_jobs;
+    int first_tiles, second_tiles, ahead, catch_up, places;
     int *status;
-    uint32_t idesc;
 };
 
 // ------------------------------------------------------------------- PTX
@@ -176,7 +190,7 @@ struct Tile {
 
 // Bands of `band` row tiles, columns walked inside a band: the tiles that run
 // together share their operands' tiles in L2.
-__device__ __forceinline__ Tile tile_at(const GemmArgs &a, int t) {
+__device__ __forceinline__ Tile tile_at(const Job &a, int t) {
     Tile tile;
     const int per_split = a.m_tiles * a.n_tiles;
     tile.split = t / per_split;
@@ -191,22 +205,35 @@ __device__ __forceinline__ Tile tile_at(const GemmArgs &a, int t) {
     return tile;
 }
 
-// K block `kb` of all: its segment, the parts of A and B, and its block there.
-struct Block {
-    int segment, a_part, b_part, k;
+// The tiles of one place (a CTA or a pair), the same for all its roles.
+struct Walk {
+    int place, phase = 0, round = 0;
+    __device__ explicit Walk(int p) : place(p) {}
+    __device__ __forceinline__ bool next(const GemmArgs &a, int &job, Tile &tile) {
+        int t = -1;
+        if (phase == 0) {
+            t = place + round * a.places;
+            job = 0;
+            if (t >= a.first_tiles) t = -1, phase = 1, round = 0;
+        }
+        if (phase == 1) {
+            const int behind = a.places - a.ahead;
+            t = place - a.ahead + round * behind;
+            job = a.first_jobs;
+            if (round >= a.catch_up || place < a.ahead || t >= a.second_tiles) t = -1, phase = 2, round = 0;
+        }
+        if (phase == 2) {
+            const int turn = place >= a.ahead ? place - a.ahead : place - a.ahead + a.places;
+            t = a.catch_up * (a.places - a.ahead) + turn + round * a.places;
+            job = a.first_jobs;
+            if (t >= a.second_tiles) return false;
+        }
+        ++round;
+        while (t >= a.jobs[job].tiles) t -= a.jobs[job++].tiles;
+        tile = tile_at(a.jobs[job], t);
+        return true;
+    }
 };
-__device__ __forceinline__ Block block_at(const GemmArgs &a, int kb) {
-    Block b;
-    const int first = a.pairs * a.k_blocks[0];
-    b.segment = kb >= first;
-    if (b.segment) kb -= first;
-    const int pair = kb / a.k_blocks[b.segment];
-    b.k = kb - pair * a.k_blocks[b.segment];
-    // the six pairs of parts, smallest products first: (0 2) (2 0) (1 1) (0 1) (1 0) (0 0)
-    b.a_part = a.pairs == 1 ? 0 : (0x021010 >> (4 * (5 - pair))) & 3;
-    b.b_part = a.pairs == 1 ? 0 : (0x201100 >> (4 * (5 - pair))) & 3;
-    return b;
-}
 
 // ---------------------------------------------------------------- epilogues
 
@@ -247,27 +274,88 @@ __device__ __forceinline__ void store_values(T *dst, int64_t left, const float (
     }
 }
 
-// The three bf16 parts of a value.
-__device__ __forceinline__ void split(float v, float &a, float &b, float &c) {
-    a = __bfloat162float(__float2bfloat16_rn(v));
-    const float rest = v - a;
-    b = __bfloat162float(__float2bfloat16_rn(rest));
-    c = rest - b;
-}
+// Where 32 (or, in join_kernel, 8) columns of a result go. Direct: a thread
+// stores its row's columns itself.
+struct DirectStore {
+    int64_t row, column, left;
+    bool live;
+    template <int kWide, typename E>
+    __device__ __forceinline__ void operator()(E *base, int64_t ld, const float (&in)[kWide]) const {
+        if (live && left > 0) store_values<kWide>(base + row * ld + column, left, in);
+    }
+};
 
-template <int kWide, typename T>
-__device__ __forceinline__ void store_parts(const Parts &to, int64_t row, int64_t column, int64_t left, const float (&in)[kWide]) {
-    using E = typename Operand16<T>::type;
-    E *dst = static_cast<E *>(to.base) + row * to.ld + column;
-    if constexpr (Operand16<T>::kParts == 1) {
-        store_values<kWide>(dst, left, in);
-    } else {
-        float a[kWide], b[kWide], c[kWide];
+// Staged: lane r of a warp holds row r; the rows pass through shared memory, so
+// that a warp stores 64 contiguous bytes of 8 rows at a time, or 32 entries of a
+// row that is off 16 bytes. 2-byte stores down 32 rows took 6 us of a tile.
+struct StagedStore {
+    uint8_t *area;
+    int64_t row0, column, left;  // the warp's first row
+    int rows;                    // its rows inside the result
+    int lane;
+    template <typename E>
+    __device__ __forceinline__ void operator()(E *base, int64_t ld, const float (&in)[32]) const {
+        constexpr int W = Pack<E>::kWidth, kColumns = 4 * W;  // 64 bytes a row
 #pragma unroll
-        for (int j = 0; j < kWide; ++j) split(in[j], a[j], b[j], c[j]);
-        store_values<kWide>(dst, left, a);
-        store_values<kWide>(dst + to.part_stride, left, b);
-        store_values<kWide>(dst + 2 * to.part_stride, left, c);
+        for (int half = 0; half < 32 / kColumns; ++half) {
+            if (half * kColumns >= left) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float part[W];
+#pragma unroll
+                for (int e = 0; e < W; ++e) part[e] = in[half * kColumns + j * W + e];
+                *reinterpret_cast<uint4 *>(area + lane * kStagedRow + 16 * j) = pack(part, E());
+            }
+            __syncwarp();
+            E *dst = base + row0 * ld + column + half * kColumns;
+            const int columns = static_cast<int>(min(left - half * kColumns, static_cast<int64_t>(kColumns)));
+            if (((reinterpret_cast<uintptr_t>(dst) | static_cast<uintptr_t>(ld * sizeof(E))) & 15) == 0) {
+                const int piece = lane & 3;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = i * 8 + (lane >> 2);
+                    if (r >= rows) continue;
+                    const uint4 v = *reinterpret_cast<const uint4 *>(area + r * kStagedRow + 16 * piece);
+                    E *to = dst + r * ld + piece * W;
+                    if (piece * W + W <= columns) {
+                        store_stream(to, v);
+                    } else {
+                        const E *from = reinterpret_cast<const E *>(area + r * kStagedRow) + piece * W;
+                        for (int e = 0; e < columns - piece * W; ++e) to[e] = from[e];
+                    }
+                }
+            } else {
+                const int c = lane % kColumns;
+                constexpr int kRows = 32 / kColumns;
+                if (c < columns) {
+#pragma unroll 4
+                    for (int r = lane / kColumns; r < rows; r += kRows) {
+                        dst[r * ld + c] = reinterpret_cast<const E *>(area + r * kStagedRow)[c];
+                    }
+                }
+            }
+            __syncwarp();
+        }
+    }
+};
+
+template <int kWide, typename T, typename Store>
+__device__ __forceinline__ void store_parts(const Store &store, const Parts &to, const float (&in)[kWide]) {
+    using E = typename Operand16<T>::type;
+    E *dst = static_cast<E *>(to.base);
+    if constexpr (Operand16<T>::kParts == 1) {
+        store(dst, to.ld, in);
+    } else {
+        float rest[kWide], part[kWide];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+#pragma unroll
+            for (int j = 0; j < kWide; ++j) {
+                rest[j] = k == 0 ? in[j] : rest[j] - part[j];
+                part[j] = __bfloat162float(__float2bfloat16_rn(rest[j]));
+            }
+            store(dst + k * to.part_stride, to.ld, part);
+        }
     }
 }
 
@@ -281,61 +369,103 @@ __device__ __forceinline__ float sigmoid_of(float p) {
     }
 }
 
-// kGate on kWide hidden units of one row: p and q without their biases.
 template <int kWide, typename T>
-__device__ __forceinline__ void finish_gate(const GemmArgs &a, int64_t row, int64_t column, bool live, float (&p)[kWide], float (&q)[kWide]) {
-    const int64_t left = a.n - column;
-    if (!live || left <= 0) return;
-    if (a.bias0 != nullptr) {
-        float b[kWide];
-        load_values<kWide>(static_cast<const T *>(a.bias0) + column, left, b);
+__device__ __forceinline__ void add_bias(const void *bias, int64_t column, int64_t left, float (&v)[kWide]) {
+    if (bias == nullptr) return;
+    float b[kWide];
+    load_values<kWide>(static_cast<const T *>(bias) + column, left, b);
 #pragma unroll
-        for (int j = 0; j < kWide; ++j) p[j] += b[j];
-    }
-    if (a.bias1 != nullptr) {
-        float b[kWide];
-        load_values<kWide>(static_cast<const T *>(a.bias1) + column, left, b);
-#pragma unroll
-        for (int j = 0; j < kWide; ++j) q[j] += b[j];
-    }
+    for (int j = 0; j < kWide; ++j) v[j] += b[j];
+}
+
+// kGate on kWide hidden units of one row: p and q without their biases.
+template <int kWide, typename T, typename Store>
+__device__ __forceinline__ void finish_gate(const Job &a, const Store &store, float (&p)[kWide], float (&q)[kWide]) {
+    add_bias<kWide, T>(a.bias0, store.column, store.left, p);
+    add_bias<kWide, T>(a.bias1, store.column, store.left, q);
     if (a.p != nullptr) {
-        store_values<kWide>(static_cast<T *>(a.p) + row * a.ld_pq + column, left, p);
-        store_values<kWide>(static_cast<T *>(a.q) + row * a.ld_pq + column, left, q);
+        store(static_cast<T *>(a.p), a.ld_pq, p);
+        store(static_cast<T *>(a.q), a.ld_pq, q);
     }
 #pragma unroll
     for (int j = 0; j < kWide; ++j) q[j] *= p[j] * sigmoid_of<T>(p[j]);
-    store_parts<kWide, T>(a.first, row, column, left, q);
+    store_parts<kWide, T>(store, a.first, q);
 }
 
-// kInner on kWide hidden units of one row of dh.
+// kWide kept values of a row as they lie in memory (rows start at 16 bytes and are padded to them).
 template <int kWide, typename T>
-__device__ __forceinline__ void finish_inner(const GemmArgs &a, int64_t row, int64_t column, bool live, float (&dh)[kWide]) {
-    const int64_t left = a.n - column;
-    if (!live || left <= 0) return;
+struct KeptRow {
+    uint4 raw[kWide / Pack<T>::kWidth];
+    __device__ __forceinline__ void load(const void *base, int64_t ld, int64_t row, int64_t column, bool live) {
+        const T *src = static_cast<const T *>(base) + row * ld + column;
+#pragma unroll
+        for (int i = 0; i < kWide / Pack<T>::kWidth; ++i) {
+            raw[i] = live && column + i * Pack<T>::kWidth < ld ? load_cached(src + i * Pack<T>::kWidth) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void values(float (&out)[kWide]) const {
+        constexpr int W = Pack<T>::kWidth;
+#pragma unroll
+        for (int i = 0; i < kWide / W; ++i) {
+            float part[W];
+            unpack(raw[i], part, T());
+#pragma unroll
+            for (int e = 0; e < W; ++e) out[i * W + e] = part[e];
+        }
+    }
+};
+
+__device__ __forceinline__ float dp_of(float dh, float p, float q, float s) { return q * (dh * (s * fmaf(p, 1.0f - s, 1.0f))); }
+__device__ __forceinline__ float dq_of(float dh, float p, float s) { return p * (s * dh); }
+
+// kInner on kWide hidden units of one row of dh.
+template <int kWide, typename T, typename Store>
+__device__ __forceinline__ void finish_inner(const Job &a, const Store &store, const KeptRow<kWide, T> &kept_p, const KeptRow<kWide, T> &kept_q,
+                                             float (&dh)[kWide]) {
     float p[kWide], q[kWide];
-    load_values<kWide>(static_cast<const T *>(a.p) + row * a.ld_pq + column, left, p);
-    load_values<kWide>(static_cast<const T *>(a.q) + row * a.ld_pq + column, left, q);
+    kept_p.values(p);
+    kept_q.values(q);
 #pragma unroll
     for (int j = 0; j < kWide; ++j) {
         const float s = sigmoid_of<T>(p[j]);
-        q[j] *= dh[j] * (s * fmaf(p[j], 1.0f - s, 1.0f));
-        p[j] *= s * dh[j];
+        q[j] = dp_of(dh[j], p[j], q[j], s);
+        p[j] = dq_of(dh[j], p[j], s);
     }
-    store_parts<kWide, T>(a.first, row, column, left, q);
-    store_parts<kWide, T>(a.second, row, column, left, p);
+    store_parts<kWide, T>(store, a.first, q);
+    store_parts<kWide, T>(store, a.second, p);
 }
 
-template <int kWide, typename T>
-__device__ __forceinline__ void finish_out(const GemmArgs &a, int64_t row, int64_t column, bool live, float (&y)[kWide]) {
-    const int64_t left = a.n - column;
-    if (!live || left <= 0) return;
-    if (a.bias0 != nullptr) {
-        float b[kWide];
-        load_values<kWide>(static_cast<const T *>(a.bias0) + column, left, b);
+// The same where p and q do not fit the registers beside the sums (fp32): 8
+// columns of them at a time, once for dp and once for dq.
+template <typename T, typename Store>
+__device__ __forceinline__ void finish_inner_slowly(const Job &a, const Store &store, int64_t row, bool live, float (&dh)[32]) {
+    float out[32];
 #pragma unroll
-        for (int j = 0; j < kWide; ++j) y[j] += b[j];
+    for (int side = 0; side < 2; ++side) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            KeptRow<8, T> kept;
+            float p[8], q[8];
+            kept.load(a.p, a.ld_pq, row, store.column + 8 * i, live);
+            kept.values(p);
+            if (side == 0) {
+                kept.load(a.q, a.ld_pq, row, store.column + 8 * i, live);
+                kept.values(q);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float s = sigmoid_of<T>(p[e]);
+                out[8 * i + e] = side == 0 ? dp_of(dh[8 * i + e], p[e], q[e], s) : dq_of(dh[8 * i + e], p[e], s);
+            }
+        }
+        store_parts<32, T>(store, side == 0 ? a.first : a.second, out);
     }
-    store_values<kWide>(static_cast<T *>(a.out) + row * a.ld_out + column, left, y);
+}
+
+template <int kWide, typename T, typename Store>
+__device__ __forceinline__ void finish_out(const Job &a, const Store &store, float (&y)[kWide]) {
+    add_bias<kWide, T>(a.bias0, store.column, store.left, y);
+    store(static_cast<T *>(a.out), a.ld_out, y);
 }
 
 // ------------------------------------------------------------------- kernel
@@ -345,19 +475,25 @@ __device__ __forceinline__ void finish_out(const GemmArgs &a, int64_t row, int64
 // tile is finished while the next is multiplied. kCtas = 2: a pair of CTAs
 // computes 256 rows with one instruction; each loads its 128 rows of A and half
 // of B's columns, so an SM reads a third fewer bytes per product than with a
-// 128 x 256 tile of its own. Every wait is bounded; one that gives up raises the
-// CTA's abort flag and the status word, and all roles leave.
+// 128 x 256 tile of its own (32768 rows of 2048 -> 4096 -> 2048: 856 us for 923
+// of the gate's product). fp32: a K block is three stages, one a part, each
+// loaded once for all the products of its parts. Every wait is bounded; one that
+// gives up raises the CTA's abort flag and the status word, and all roles leave.
 template <typename T, int kEpilogue, int kTileN, int kCtas>
 __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant__ GemmArgs args) {
     constexpr uint32_t kBBytes = static_cast<uint32_t>(kTileN / kCtas) * kBK * 2;
     constexpr uint32_t kStage = kABytes + kBBytes;
     constexpr int kStages = kRingBytes / kStage < kMaxStages ? kRingBytes / kStage : kMaxStages;
     constexpr int kUnits = kEpilogue == kGate ? kTileN / 2 : kTileN;  // result columns of a tile
-    constexpr bool kPasses = sizeof(T) == 4;
-    static_assert(!kPasses || kTileN <= 128, "an epilogue thread holds 64 sums");
+    constexpr int kParts = Operand16<T>::kParts;
+    constexpr bool kPasses = kParts > 1;
+    constexpr int kAccumulator = kPasses ? 2 * kTileN : kTileN;  // TMEM columns
+    static_assert(2 * kAccumulator <= static_cast<int>(kTmemColumns), "two accumulators");
+    static_assert(kStages >= kParts + 2, "a K block's parts stay while the next is loaded");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-    uint64_t *full = reinterpret_cast<uint64_t *>(ring + kRingBytes);
+    uint8_t *staged = ring + kRingBytes;
+    uint64_t *full = reinterpret_cast<uint64_t *>(staged + kEpilogueWarps * kStagedBytes);
     uint64_t *empty = full + kMaxStages;
     uint64_t *acc_full = empty + kMaxStages;
     uint64_t *acc_empty = acc_full + 2;
@@ -392,58 +528,58 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
     if constexpr (kCtas == 2) cluster_sync();  // the pair's barriers are set up
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int tiles = args.m_tiles * args.n_tiles * args.splits;
-    const int first_tile = blockIdx.x / kCtas, step = gridDim.x / kCtas;
+    Walk walk(blockIdx.x / kCtas);
+    int job;
+    Tile tile;
 
     if (warp == 0) {
         if (lane == 0) {
-            for (int s = 0; s < args.segments; ++s) {
-                prefetch_tensor_map(&args.a[s]);
-                prefetch_tensor_map(&args.b[s]);
-            }
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int t = first_tile; t < tiles && ok; t += step) {
-                const Tile tile = tile_at(args, t);
+            while (ok && walk.next(args, job, tile)) {
+                const Job &j = args.jobs[job];
                 const int32_t row = (tile.m * kCtas + rank) * kBM;
-                for (int kb = tile.k_begin; kb < tile.k_end; ++kb) {
-                    ok = wait<kCtas == 2>(&empty[stage], phase ^ 1, abort, args.status);
-                    if (!ok) break;
-                    const Block block = block_at(args, kb);
-                    const CUtensorMap *ma = &args.a[block.segment], *mb = &args.b[block.segment];
-                    uint8_t *to_a = ring + stage * kStage, *to_b = to_a + kABytes;
-                    const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
-                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], kStage * kCtas);
-                    const int32_t k = block.k * kBK;
-                    if (args.a_mn) {
-                        load_box<kCtas>(to_a, ma, bar, row, k, block.a_part);
-                        load_box<kCtas>(to_a + kABytes / 2, ma, bar, row + 64, k, block.a_part);
-                    } else {
-                        load_box<kCtas>(to_a, ma, bar, k, row, block.a_part);
-                    }
-                    if constexpr (kEpilogue == kGate) {  // K-major: the units' gate rows, then their value rows
-                        const int32_t unit = tile.n * kUnits;
-                        if constexpr (kCtas == 1) {
-                            load_box<1>(to_b, &args.b[0], bar, k, unit, block.b_part);
-                            load_box<1>(to_b + kBBytes / 2, &args.b[1], bar, k, unit, block.b_part);
+                for (int kb = tile.k_begin; kb < tile.k_end && ok; ++kb) {
+                    const int segment = kEpilogue != kGate && kb >= j.first_blocks;
+                    const CUtensorMap *ma = &j.a[segment], *mb = &j.b[segment];
+                    const int32_t k = (segment ? kb - j.first_blocks : kb) * kBK;
+#pragma unroll 1
+                    for (int part = 0; part < kParts; ++part) {
+                        ok = wait<kCtas == 2>(&empty[stage], phase ^ 1, abort, args.status);
+                        if (!ok) break;
+                        uint8_t *to_a = ring + stage * kStage, *to_b = to_a + kABytes;
+                        const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
+                        if (rank == 0) mbar_arrive_expect_tx(&full[stage], kStage * kCtas);
+                        if (j.a_mn) {
+                            load_box<kCtas>(to_a, ma, bar, row, k, part);
+                            load_box<kCtas>(to_a + kABytes / 2, ma, bar, row + 64, k, part);
                         } else {
-                            load_box<2>(to_b, &args.b[rank], bar, k, unit, block.b_part);
+                            load_box<kCtas>(to_a, ma, bar, k, row, part);
                         }
-                    } else {
-                        const int32_t column = tile.n * kTileN + rank * (kTileN / kCtas);
-                        if (args.b_mn) {
-#pragma unroll
-                            for (int c = 0; c < kTileN / kCtas / 64; ++c) {
-                                load_box<kCtas>(to_b + c * 8192, mb, bar, column + 64 * c, k, block.b_part);
+                        if constexpr (kEpilogue == kGate) {  // K-major: the units' gate rows, then their value rows
+                            const int32_t unit = tile.n * kUnits;
+                            if constexpr (kCtas == 1) {
+                                load_box<1>(to_b, &j.b[0], bar, k, unit, part);
+                                load_box<1>(to_b + kBBytes / 2, &j.b[1], bar, k, unit, part);
+                            } else {
+                                load_box<2>(to_b, &j.b[rank], bar, k, unit, part);
                             }
                         } else {
-                            load_box<kCtas>(to_b, mb, bar, k, column, block.b_part);
+                            const int32_t column = tile.n * kTileN + rank * (kTileN / kCtas);
+                            if (j.b_mn) {
+#pragma unroll
+                                for (int c = 0; c < kTileN / kCtas / 64; ++c) {
+                                    load_box<kCtas>(to_b + c * 8192, mb, bar, column + 64 * c, k, part);
+                                }
+                            } else {
+                                load_box<kCtas>(to_b, mb, bar, k, column, part);
+                            }
                         }
-                    }
-                    if (++stage == kStages) {
-                        stage = 0;
-                        phase ^= 1;
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
                     }
                 }
             }
@@ -466,34 +602,53 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                     acc_phase ^= 1;
                 }
             };
-            for (int t = first_tile; t < tiles && ok; t += step) {
-                const Tile tile = tile_at(args, t);
+            while (ok && walk.next(args, job, tile)) {
+                const int a_mn = args.jobs[job].a_mn, b_mn = args.jobs[job].b_mn;
+                const uint32_t idesc = args.jobs[job].idesc;
+                // 16 of K: 16 rows of 128 bytes, or 32 bytes of every row (addresses count 16 bytes)
+                const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
                 uint32_t d = 0;
-                for (int kb = tile.k_begin; kb < tile.k_end; ++kb) {
+                auto multiply_parts = [&](uint32_t to, int at_stage_a, int at_stage_b, bool fresh) {
+                    const uint32_t at_a = smem_addr(ring + at_stage_a * kStage), at_b = smem_addr(ring + at_stage_b * kStage) + kABytes;
+                    const uint64_t da = a_mn ? sw128_mnmajor_desc(at_a) : sw128_kmajor_desc(at_a);
+                    const uint64_t db = b_mn ? sw128_mnmajor_desc(at_b) : sw128_kmajor_desc(at_b);
+#pragma unroll
+                    for (int k = 0; k < kBK / 16; ++k) mma<kCtas>(to, da + k * step_a, db + k * step_b, idesc, !fresh || k > 0);
+                };
+                for (int kb = tile.k_begin; kb < tile.k_end && ok; ++kb) {
                     const bool fresh = kb == tile.k_begin || (kPasses && (kb - tile.k_begin) % kPass == 0);
                     if (fresh) {
                         if (kb > tile.k_begin) full_accumulator();
                         ok = wait<kCtas == 2>(&acc_empty[acc], acc_phase ^ 1, abort, args.status);
                         if (!ok) break;
                         tc_fence_after();
-                        d = tmem + static_cast<uint32_t>(acc * kTileN);
+                        d = tmem + static_cast<uint32_t>(acc * kAccumulator);
                     }
-                    ok = wait<kCtas == 2>(&full[stage], phase, abort, args.status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t at_a = smem_addr(ring + stage * kStage), at_b = at_a + kABytes;
-                    const uint64_t da = args.a_mn ? sw128_mnmajor_desc(at_a) : sw128_kmajor_desc(at_a);
-                    const uint64_t db = args.b_mn ? sw128_mnmajor_desc(at_b) : sw128_kmajor_desc(at_b);
-                    // 16 of K: 16 rows of 128 bytes, or 32 bytes of every row (addresses count 16 bytes)
-                    const uint64_t step_a = args.a_mn ? 2048 >> 4 : 32 >> 4, step_b = args.b_mn ? 2048 >> 4 : 32 >> 4;
+                    int at[kParts];
 #pragma unroll
-                    for (int k = 0; k < kBK / 16; ++k) {
-                        mma<kCtas>(d, da + k * step_a, db + k * step_b, args.idesc, !fresh || k > 0);
-                    }
-                    commit<kCtas>(&empty[stage]);
-                    if (++stage == kStages) {
-                        stage = 0;
-                        phase ^= 1;
+                    for (int part = 0; part < kParts; ++part) {
+                        ok = wait<kCtas == 2>(&full[stage], phase, abort, args.status);
+                        if (!ok) break;
+                        tc_fence_after();
+                        at[part] = stage;
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1;
+                        }
+                        if (part == 0) {
+                            multiply_parts(d, at[0], at[0], fresh);
+                            if (kParts == 1) commit<kCtas>(&empty[at[0]]);
+                        } else if (part == 1) {
+                            multiply_parts(d + kTileN, at[0], at[part], fresh);
+                            multiply_parts(d + kTileN, at[part], at[0], false);
+                            multiply_parts(d + kTileN, at[part], at[part], false);
+                            commit<kCtas>(&empty[at[part]]);
+                        } else {
+                            multiply_parts(d + kTileN, at[0], at[part], false);
+                            multiply_parts(d + kTileN, at[part], at[0], false);
+                            commit<kCtas>(&empty[at[0]]);
+                            commit<kCtas>(&empty[at[part]]);
+                        }
                     }
                 }
                 if (ok) full_accumulator();
@@ -503,6 +658,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
     } else {
         const int quarter = warp & 3, part = (warp - 2) >> 2;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        constexpr int kChunks = kUnits / 32, kSides = kEpilogue == kGate ? 2 : 1;
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -521,28 +677,42 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                 acc_phase ^= 1;
             }
         };
-        for (int t = first_tile; t < tiles && ok; t += step) {
-            const Tile tile = tile_at(args, t);
-            const int64_t row = static_cast<int64_t>(tile.m * kCtas + rank) * kBM + quarter * 32 + lane;
-            const bool live = row < args.m;
+        StagedStore store{staged + (warp - 2) * kStagedBytes, 0, 0, 0, 0, lane};
+        while (ok && walk.next(args, job, tile)) {
+            const Job &j = args.jobs[job];
+            store.row0 = static_cast<int64_t>(tile.m * kCtas + rank) * kBM + quarter * 32;
+            store.rows = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(32), j.m - store.row0)));
             const int64_t first_column = static_cast<int64_t>(tile.n) * kUnits;
-            constexpr int kChunks = kUnits / 32, kSides = kEpilogue == kGate ? 2 : 1;
-            // 32 columns of one row (kGate: of p and of q)
-            auto finish = [&](int c, float (&v)[kSides][32]) {
-                const int64_t column = first_column + c * 32;
-                if (args.splits > 1) {
-                    if (!live || column >= args.n) return;
-                    float *dst = args.partials + (kSides * tile.split * args.m + row) * args.ld_partial + column;
-#pragma unroll
-                    for (int k = 0; k < kSides; ++k) store_values<32>(dst + k * args.m * args.ld_partial, args.n - column, v[k]);
-                } else if constexpr (kEpilogue == kGate) {
-                    finish_gate<32, T>(args, row, column, live, v[0], v[1]);
-                } else if constexpr (kEpilogue == kInner) {
-                    finish_inner<32, T>(args, row, column, live, v[0]);
-                } else {
-                    finish_out<32, T>(args, row, column, live, v[0]);
+            KeptRow<32, T> kept_p, kept_q;  // kInner: of the chunk to come
+            auto request = [&](int c) {
+                if constexpr (kEpilogue == kInner && !kPasses) {
+                    if (j.splits > 1 || c >= kChunks) return;
+                    kept_p.load(j.p, j.ld_pq, store.row0 + lane, first_column + c * 32, lane < store.rows);
+                    kept_q.load(j.q, j.ld_pq, store.row0 + lane, first_column + c * 32, lane < store.rows);
                 }
             };
+            // 32 columns of the warp's rows (kGate: of p and of q)
+            auto finish = [&](int c, float (&v)[kSides][32]) {
+                store.column = first_column + c * 32;
+                store.left = j.n - store.column;
+                if (store.left <= 0) return;
+                if (j.splits > 1) {
+                    float *base = j.partials + kSides * tile.split * j.m * j.ld_partial;
+#pragma unroll
+                    for (int k = 0; k < kSides; ++k) store(base + k * j.m * j.ld_partial, j.ld_partial, v[k]);
+                } else if constexpr (kEpilogue == kGate) {
+                    finish_gate<32, T>(j, store, v[0], v[1]);
+                } else if constexpr (kEpilogue == kInner && kPasses) {
+                    finish_inner_slowly<T>(j, store, store.row0 + lane, lane < store.rows, v[0]);
+                } else if constexpr (kEpilogue == kInner) {
+                    const KeptRow<32, T> p = kept_p, q = kept_q;
+                    request(c + 2);
+                    finish_inner<32, T>(j, store, p, q, v[0]);
+                } else {
+                    finish_out<32, T>(j, store, v[0]);
+                }
+            };
+            request(part);
             if constexpr (kPasses) {
                 constexpr int kMine = (kChunks + 1) / 2;
                 float sum[kMine][kSides][32];
@@ -551,25 +721,28 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
 #pragma unroll
                     for (int k = 0; k < kSides; ++k) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) sum[i][k][j] = 0.0f;
+                        for (int e = 0; e < 32; ++e) sum[i][k][e] = 0.0f;
                     }
                 }
                 for (int kb = tile.k_begin; kb < tile.k_end; kb += kPass) {
                     ok = wait<kCtas == 2>(&acc_full[acc], acc_phase, abort, args.status);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t from = tmem + lanes + static_cast<uint32_t>(acc * kTileN);
+                    const uint32_t from = tmem + lanes + static_cast<uint32_t>(acc * kAccumulator);
 #pragma unroll
                     for (int i = 0; i < kMine; ++i) {
                         const int c = part + 2 * i;
                         if (c >= kChunks) continue;
 #pragma unroll
                         for (int k = 0; k < kSides; ++k) {
-                            uint32_t raw[32];
-                            KOEMI_TMEM_LD32(from + k * kUnits + c * 32, raw);
-                            tmem_wait_ld();
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) sum[i][k][j] += __uint_as_float(raw[j]);
+                            for (int part = 0; part < 2; ++part) {  // x0 y0, and the rest
+                                uint32_t raw[32];
+                                KOEMI_TMEM_LD32(from + part * kTileN + k * kUnits + c * 32, raw);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) sum[i][k][e] += __uint_as_float(raw[e]);
+                            }
                         }
                     }
                     release();
@@ -583,7 +756,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                 ok = wait<kCtas == 2>(&acc_full[acc], acc_phase, abort, args.status);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t from = tmem + lanes + static_cast<uint32_t>(acc * kTileN);
+                const uint32_t from = tmem + lanes + static_cast<uint32_t>(acc * kAccumulator);
 #pragma unroll 1
                 for (int c = part; c < kChunks; c += 2) {
                     uint32_t raw[kSides][32];
@@ -594,7 +767,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
 #pragma unroll
                     for (int k = 0; k < kSides; ++k) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[k][j] = __uint_as_float(raw[k][j]);
+                        for (int e = 0; e < 32; ++e) v[k][e] = __uint_as_float(raw[k][e]);
                     }
                     finish(c, v);
                 }
@@ -615,32 +788,40 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
     }
 }
 
-// The splits' accumulators added in order, then the epilogue: 8 columns a thread.
+// The splits' accumulators added in order, then the epilogue: 8 columns a thread. grid.y: the job.
 template <typename T, int kEpilogue>
 __global__ __launch_bounds__(256) void join_kernel(const __grid_constant__ GemmArgs args) {
-    const int64_t groups = (args.n + 7) / 8;
+    const Job &j = args.jobs[blockIdx.y];
+    const int64_t groups = (j.n + 7) / 8;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= groups * args.m) return;
+    if (j.splits == 1 || i >= groups * j.m) return;
     const int64_t row = i / groups, column = (i - row * groups) * 8;
     constexpr int kSides = kEpilogue == kGate ? 2 : 1;
-    const int64_t side = args.m * args.ld_partial;
-    const float *src = args.partials + row * args.ld_partial + column;
+    const int64_t side = j.m * j.ld_partial;
+    const float *src = j.partials + row * j.ld_partial + column;
+    KeptRow<8, T> kept_p, kept_q;
+    if constexpr (kEpilogue == kInner) {
+        kept_p.load(j.p, j.ld_pq, row, column, true);
+        kept_q.load(j.q, j.ld_pq, row, column, true);
+    }
     float sum[kSides][8] = {};
-    for (int s = 0; s < args.splits; ++s, src += kSides * side) {
+#pragma unroll 4
+    for (int s = 0; s < j.splits; ++s) {
 #pragma unroll
         for (int k = 0; k < kSides; ++k) {
             float v[8];
-            load_values<8>(src + k * side, 8, v);  // ld_partial is a multiple of 8
+            load_values<8>(src + (kSides * s + k) * side, 8, v);  // ld_partial is a multiple of 8
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[k][e] += v[e];
         }
     }
+    const DirectStore store{row, column, j.n - column, true};
     if constexpr (kEpilogue == kGate) {
-        finish_gate<8, T>(args, row, column, true, sum[0], sum[1]);
+        finish_gate<8, T>(j, store, sum[0], sum[1]);
     } else if constexpr (kEpilogue == kInner) {
-        finish_inner<8, T>(args, row, column, true, sum[0]);
+        finish_inner<8, T>(j, store, kept_p, kept_q, sum[0]);
     } else {
-        finish_out<8, T>(args, row, column, true, sum[0]);
+        finish_out<8, T>(j, store, sum[0]);
     }
 }
 
@@ -651,9 +832,9 @@ struct PackJob {
     int64_t rows, columns, ld;
     Parts to;
 };
-constexpr int kMaxJobs = 5;
+constexpr int kMaxPacks = 5;
 struct PackArgs {
-    PackJob jobs[kMaxJobs];
+    PackJob jobs[kMaxPacks];
 };
 
 // Row-major matrices copied (fp32: split) to rows of a multiple of 8 columns, zeros behind the last. grid.y: the matrix.
@@ -665,7 +846,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const __grid_constant__ PackA
         const int64_t row = i / groups, column = (i - row * groups) * 8;
         float v[8];
         load_values<8>(static_cast<const T *>(job.src) + row * job.ld + column, job.columns - column, v);
-        store_parts<8, T>(job.to, row, column, 8, v);
+        store_parts<8, T>(DirectStore{row, column, 8, true}, job.to, v);
     }
 }
 
@@ -752,54 +933,7 @@ int encode(CUtensorMap *map, const Matrix &matrix, bool half, bool mn_major, int
     return encode_tensor_map(map, type, 3, matrix.base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// How a product is cut: tile columns, CTAs a tile, parts of K.
-struct Cut {
-    int tile_n, ctas, splits;
-};
-
-// The cheapest of the cuts by clocks: an SM takes about 52 bytes a clock from
-// L2 (measured with all SMs loading: 128 x 256 tiles 51, 128 x 128 tiles 53),
-// which is what a K block of every shape but a pair's 256 x 256 waits for; a
-// launch adds about 6500 for its first loads and its last epilogue; parts of K
-// add a kernel and their accumulators' way through L2.
-Cut cut_of(int64_t m, int64_t n, int total_k, bool gate, int parts, int sms) {
-    Cut best{128, 1, 1};
-    double least = 1e30;
-    const struct { int tile_n, ctas; } shapes[] = {{256, 2}, {128, 2}, {256, 1}, {128, 1}, {64, 1}};
-    for (const auto &shape : shapes) {
-        if (parts > 1 && shape.tile_n > 128) continue;  // the sums of the passes have to fit registers
-        if (shape.ctas == 2 && m <= kBM) continue;
-        const double clocks = std::max(shape.tile_n * 2.0, (kBM + shape.tile_n / shape.ctas) * kBK * 2 / 52.0);
-        const int64_t units = gate ? shape.tile_n / 2 : shape.tile_n;
-        const int64_t tiles = ceil_div(m, kBM * shape.ctas) * ceil_div(n, units), places = std::max(1, sms / shape.ctas);
-        for (int splits = 1; splits <= 64 && splits <= total_k; splits += splits < 8 ? 1 : splits / 4) {
-            const int per = static_cast<int>(ceil_div(total_k, splits));
-            if (ceil_div(total_k, per) != splits) continue;  // every part has blocks
-            const double waves = static_cast<double>(ceil_div(tiles * splits, places));
-            double cost = waves * per * clocks + 6500;
-            if (splits > 1) cost += 6000 + (gate ? 2.0 : 1.0) * static_cast<double>(m) * static_cast<double>(n) * (splits + 1) * 4 / 2500;
-            if (cost < least) least = cost, best = Cut{shape.tile_n, shape.ctas, splits};
-        }
-    }
-    return best;
-}
-
-size_t partial_bytes(const Cut &cut, int64_t m, int64_t n, bool gate) {
-    return cut.splits == 1 ? 0 : static_cast<size_t>(cut.splits) * (gate ? 2 : 1) * m * round8(n) * sizeof(float);
-}
-
-template <typename T, int kEpilogue, int kTileN, int kCtas>
-int launch_shape(const GemmArgs &args, cudaStream_t stream) {
-    auto kernel = gemm_kernel<T, kEpilogue, kTileN, kCtas>;
-    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes)));
-    const int64_t tiles = static_cast<int64_t>(args.m_tiles) * args.n_tiles * args.splits;
-    if (tiles > INT32_MAX) return fail(KOEMI_ERR_INVALID, "feed-forward sizes are too large");
-    const int64_t grid = std::min<int64_t>(tiles, sm_count() / kCtas) * kCtas;
-    KOEMI_CUDA_TRY(launch_programmatic(false, kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), kSmemBytes, stream, dim3(kCtas, 1, 1), args));
-    return KOEMI_OK;
-}
-
-// One product: A and B of up to two segments (kGate: one A, B the two weights).
+// One product as the host sees it. kGate: one A, B the two weights, n hidden units.
 struct Product {
     Matrix a[2], b[2];
     int segments;
@@ -807,43 +941,144 @@ struct Product {
     int64_t m, n;
 };
 
-int total_k_of(const Product &p, bool gate) {
-    const int pairs = p.a[0].parts == 3 ? 6 : 1;
-    int64_t blocks = 0;
-    for (int s = 0; s < (gate ? 1 : p.segments); ++s) blocks += ceil_div(p.a_mn ? p.a[s].rows : p.a[s].columns, kBK);
-    return static_cast<int>(blocks * pairs);
+int blocks_of(const Product &p, int segment) {
+    return static_cast<int>(ceil_div(p.a_mn ? p.a[segment].rows : p.a[segment].columns, kBK));
+}
+int total_k_of(const Product &p, bool gate) { return blocks_of(p, 0) + (!gate && p.segments > 1 ? blocks_of(p, 1) : 0); }
+
+// How a launch is cut: its tiles' columns, CTAs a tile, and each product's parts of K.
+struct Cut {
+    int tile_n, ctas, splits[kMaxJobs];
+};
+
+int64_t tiles_of(const Product &p, bool gate, int tile_n, int ctas) {
+    return ceil_div(p.m, kBM * ctas) * ceil_div(p.n, gate ? tile_n / 2 : tile_n);
 }
 
+// The cheapest cut by clocks. An SM takes about 52 bytes a clock from L2
+// (measured with all SMs loading: 128 x 256 tiles 51, 128 x 128 tiles 53), which
+// is what a K block of every shape but a pair's 256 x 256 waits for; its
+// products take the tensor cores 2 clocks a column (six products a block of
+// fp32). A product is parted along K where a whole tile of it would outlast an
+// even share of the work. A launch adds about 6500 clocks for its first loads
+// and its last epilogue; parts of K add a kernel and their accumulators' way
+// through L2. Products of one group are in at most two classes of equal K, the
+// longer first.
+Cut cut_of(const Product *const *products, int count, bool gate, int sms) {
+    const int parts = products[0]->a[0].parts;
+    Cut best{128, 1, {1, 1, 1, 1}};
+    double least = 1e300;
+    const struct { int tile_n, ctas; } shapes[] = {{256, 2}, {128, 2}, {256, 1}, {128, 1}, {64, 1}};
+    int64_t rows = 0;
+    for (int i = 0; i < count; ++i) rows = std::max(rows, products[i]->m);
+    for (const auto &shape : shapes) {
+        if (parts > 1 && shape.tile_n > 128) continue;  // two accumulators of two parts, and their sums in registers
+        if (shape.ctas == 2 && rows <= kBM) continue;
+        const double clocks = std::max(shape.tile_n * (parts > 1 ? 12.0 : 2.0), parts * (kBM + shape.tile_n / shape.ctas) * kBK * 2 / 52.0);
+        const double places = std::max(1, sms / shape.ctas);
+        double work = 0;
+        for (int i = 0; i < count; ++i) work += static_cast<double>(tiles_of(*products[i], gate, shape.tile_n, shape.ctas)) * total_k_of(*products[i], gate) * clocks;
+        for (int eager = 0; eager < 2; ++eager) {  // parts of K as long as an even share, or shorter ones
+            Cut cut{shape.tile_n, shape.ctas, {1, 1, 1, 1}};
+            const double share = std::max(work / places / (1 + eager), 3000.0);
+            double load = 0, longest = 0, joined = 0;
+            for (int i = 0; i < count; ++i) {
+                const int total = total_k_of(*products[i], gate);
+                int splits = static_cast<int>(std::min(64.0, total * clocks / share + (eager ? 0.999 : 0.3)));
+                splits = std::max(1, std::min(splits, total));
+                const int per = static_cast<int>(ceil_div(total, splits));
+                splits = static_cast<int>(ceil_div(total, per));  // every part has blocks
+                cut.splits[i] = splits;
+                const double tiles = static_cast<double>(tiles_of(*products[i], gate, shape.tile_n, shape.ctas)) * splits;
+                longest = std::max(longest, per * clocks);
+                load += tiles * per * clocks;
+                if (splits > 1) joined += (gate ? 2.0 : 1.0) * static_cast<double>(products[i]->m) * static_cast<double>(products[i]->n) * (splits + 1) * 4;
+            }
+            // an even share, rounded up to whole tiles of the shortest product
+            const Product &last = *products[count - 1];
+            const double shortest = ceil_div(total_k_of(last, gate), cut.splits[count - 1]) * clocks;
+            double cost = std::max(longest, std::ceil(load / places / shortest - 1e-9) * shortest) + 6500;
+            if (joined > 0) cost += 6000 + joined / 2500;
+            if (cost < least) least = cost, best = cut;
+        }
+    }
+    return best;
+}
+
+size_t partial_bytes(const Cut &cut, int i, const Product &p, bool gate) {
+    return cut.splits[i] == 1 ? 0 : round256(static_cast<size_t>(cut.splits[i]) * (gate ? 2 : 1) * p.m * round8(p.n) * sizeof(float));
+}
+
+// What the products of one launch, cut alike, need for their partial sums.
+size_t partial_bytes(const Product *const *products, int count, bool gate) {
+    const Cut cut = cut_of(products, count, gate, sm_count());
+    size_t bytes = 0;
+    for (int i = 0; i < count; ++i) bytes += partial_bytes(cut, i, *products[i], gate);
+    return bytes;
+}
+
+template <typename T, int kEpilogue, int kTileN, int kCtas>
+int launch_shape(GemmArgs &args, cudaStream_t stream) {
+    auto kernel = gemm_kernel<T, kEpilogue, kTileN, kCtas>;
+    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes)));
+    args.places = std::min(args.first_tiles + args.second_tiles, sm_count() / kCtas);
+    const int first = args.jobs[0].k_per_split, second = args.jobs[args.job_count - 1].k_per_split;
+    args.ahead = args.first_tiles % args.places;
+    args.catch_up = args.ahead > 0 && args.second_tiles > 0 ? first / second : 0;
+    if (args.ahead == 0) args.catch_up = 0;
+    KOEMI_CUDA_TRY(launch_programmatic(false, kernel, dim3(static_cast<unsigned>(args.places * kCtas)), dim3(kThreads), kSmemBytes, stream,
+                                       dim3(kCtas, 1, 1), args));
+    return KOEMI_OK;
+}
+
+// Independent products in one launch, those of the longer K first; jobs: their
+// epilogues' fields. The cut is that of all of them, wanted or not, so that the
+// workspace does not depend on which are.
 template <typename T, int kEpilogue>
-int multiply(const Product &p, GemmArgs args, float *partials, cudaStream_t stream) {
+int multiply(const Product *const *products, const Job *jobs, int count, char *partials, cudaStream_t stream) {
     constexpr bool gate = kEpilogue == kGate;
     const bool half = std::is_same<typename Operand16<T>::type, __half>::value;
-    const int total_k = total_k_of(p, gate);
-    const Cut cut = cut_of(p.m, p.n, total_k, gate, p.a[0].parts, sm_count());
-    args.segments = gate ? 2 : p.segments;
-    args.pairs = p.a[0].parts == 3 ? 6 : 1;
-    args.a_mn = p.a_mn;
-    args.b_mn = p.b_mn;
-    args.m = p.m;
-    args.n = p.n;
-    args.m_tiles = static_cast<int>(ceil_div(p.m, kBM * cut.ctas));
-    args.n_tiles = static_cast<int>(ceil_div(p.n, gate ? cut.tile_n / 2 : cut.tile_n));
-    args.splits = cut.splits;
-    args.band = std::max(1, 16 / cut.ctas);
-    args.total_k = total_k;
-    args.k_per_split = static_cast<int>(ceil_div(total_k, cut.splits));
-    args.partials = partials;
-    args.ld_partial = round8(p.n);
+    const Cut cut = cut_of(products, count, gate, sm_count());
+    GemmArgs args{};
     args.status = device_status_word();
-    args.idesc = 1u << 4 | (half ? 0u : 1u << 7 | 1u << 10) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u) |
-                 static_cast<uint32_t>(cut.tile_n >> 3) << 17 | static_cast<uint32_t>(kBM * cut.ctas >> 4) << 24;
-    for (int s = 0; s < 2; ++s) {
-        const Matrix &a = p.a[gate || s >= p.segments ? 0 : s], &b = p.b[gate || s < p.segments ? s : 0];
-        args.k_blocks[s] = static_cast<int>(ceil_div(p.a_mn ? a.rows : a.columns, kBK));
-        int rc = encode(&args.a[s], a, half, p.a_mn, kBM);
-        if (rc == KOEMI_OK) rc = encode(&args.b[s], b, half, p.b_mn, gate ? cut.tile_n / 2 : cut.tile_n / cut.ctas);
-        if (rc != KOEMI_OK) return rc;
+    int64_t tiles[2] = {0, 0}, most = 0;
+    for (int i = 0; i < count; ++i) {
+        const Product &p = *products[i];
+        if (kEpilogue == kOut && jobs[i].out == nullptr) continue;  // not wanted: the others are cut as beside it
+        const int at = args.job_count++;
+        Job &j = args.jobs[at] = jobs[i];
+        j.total_k = total_k_of(p, gate);
+        j.first_blocks = blocks_of(p, 0);
+        j.splits = cut.splits[i];
+        j.k_per_split = static_cast<int>(ceil_div(j.total_k, j.splits));
+        j.a_mn = p.a_mn;
+        j.b_mn = p.b_mn;
+        j.m = p.m;
+        j.n = p.n;
+        j.m_tiles = static_cast<int>(ceil_div(p.m, kBM * cut.ctas));
+        j.n_tiles = static_cast<int>(ceil_div(p.n, gate ? cut.tile_n / 2 : cut.tile_n));
+        j.band = std::max(1, 16 / cut.ctas);
+        j.partials = reinterpret_cast<float *>(partials);
+        j.ld_partial = round8(p.n);
+        partials += partial_bytes(cut, i, p, gate);
+        j.idesc = 1u << 4 | (half ? 0u : 1u << 7 | 1u << 10) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u) |
+                  static_cast<uint32_t>(cut.tile_n >> 3) << 17 | static_cast<uint32_t>(kBM * cut.ctas >> 4) << 24;
+        for (int s = 0; s < (gate ? 2 : p.segments); ++s) {
+            int rc = s > 0 && gate ? KOEMI_OK : encode(&j.a[s], p.a[s], half, p.a_mn, kBM);
+            if (rc == KOEMI_OK) rc = encode(&j.b[s], p.b[s], half, p.b_mn, gate ? cut.tile_n / 2 : cut.tile_n / cut.ctas);
+            if (rc != KOEMI_OK) return rc;
+        }
+        const int64_t own = static_cast<int64_t>(j.m_tiles) * j.n_tiles * j.splits;
+        const bool first = args.jobs[0].k_per_split == j.k_per_split && args.first_jobs == at;
+        tiles[first ? 0 : 1] += own;
+        if (first) ++args.first_jobs;
+        if (tiles[0] + tiles[1] > INT32_MAX / 2) return fail(KOEMI_ERR_INVALID, "feed-forward sizes are too large");
+        j.tiles = static_cast<int>(own);
+        if (j.splits > 1) most = std::max(most, ceil_div(p.n, 8) * p.m);
     }
+    if (args.job_count == 0) return KOEMI_OK;
+    args.first_tiles = static_cast<int>(tiles[0]);
+    args.second_tiles = static_cast<int>(tiles[1]);
     int rc = KOEMI_OK;
     if (cut.tile_n == 64) {
         rc = launch_shape<T, kEpilogue, 64, 1>(args, stream);
@@ -853,9 +1088,8 @@ int multiply(const Product &p, GemmArgs args, float *partials, cudaStream_t stre
         rc = cut.ctas == 2 ? launch_shape<T, kEpilogue, 256, 2>(args, stream) : launch_shape<T, kEpilogue, 256, 1>(args, stream);
     }
     if (rc != KOEMI_OK) return rc;
-    if (cut.splits > 1) {
-        const int64_t threads = (args.n + 7) / 8 * args.m;
-        join_kernel<T, kEpilogue><<<static_cast<unsigned>(ceil_div(threads, 256)), 256, 0, stream>>>(args);
+    if (most > 0) {
+        join_kernel<T, kEpilogue><<<dim3(static_cast<unsigned>(ceil_div(most, 256)), static_cast<unsigned>(args.job_count)), 256, 0, stream>>>(args);
         KOEMI_LAUNCH_CHECK();
     }
     return KOEMI_OK;
@@ -930,7 +1164,7 @@ struct ForwardPlan {
     PackArgs jobs;
     int job_count;
     Product gate, out;
-    float *partials;
+    char *partials;
 };
 
 // pool: the workspace; kept_base: the buffer that the backward will read, or NULL.
@@ -944,10 +1178,8 @@ void plan_forward(ForwardPlan &plan, const Problem &q, Pool &pool, char *kept_ba
     plan.kept = keep ? kept_of(kept_pool, q.rows, q.hidden, q.dtype, true) : kept_of(pool, q.rows, q.hidden, q.dtype, false);
     plan.gate = Product{{plan.x, {}}, {plan.wg, plan.wv}, 1, false, false, q.rows, q.hidden};
     plan.out = Product{{matrix_of(plan.kept.h, q.rows, q.hidden, q.dtype), {}}, {plan.wo, {}}, 1, false, false, q.rows, q.out_width};
-    const int sms = sm_count();
-    const size_t first = partial_bytes(cut_of(q.rows, q.hidden, total_k_of(plan.gate, true), true, parts_of(q.dtype), sms), q.rows, q.hidden, true);
-    const size_t second = partial_bytes(cut_of(q.rows, q.out_width, total_k_of(plan.out, false), false, parts_of(q.dtype), sms), q.rows, q.out_width, false);
-    plan.partials = static_cast<float *>(pool.take(std::max(first, second)));
+    const Product *gate = &plan.gate, *out = &plan.out;
+    plan.partials = static_cast<char *>(pool.take(std::max(partial_bytes(&gate, 1, true), partial_bytes(&out, 1, false))));
 }
 
 template <typename T>
@@ -957,20 +1189,21 @@ int forward(const Problem &q, void *y, void *kept, void *workspace, cudaStream_t
     plan_forward(plan, q, pool, static_cast<char *>(kept), kept != nullptr);
     int rc = pack_all<T>(plan.jobs, plan.job_count, stream);
     if (rc != KOEMI_OK) return rc;
-    GemmArgs gate{};
+    const Product *first = &plan.gate, *second = &plan.out;
+    Job gate{};
     gate.bias0 = q.bg;
     gate.bias1 = q.bv;
     gate.first = plan.kept.h;
     gate.p = plan.kept.p;
     gate.q = plan.kept.q;
     gate.ld_pq = plan.kept.ld;
-    rc = multiply<T, kGate>(plan.gate, gate, plan.partials, stream);
+    rc = multiply<T, kGate>(&first, &gate, 1, plan.partials, stream);
     if (rc != KOEMI_OK) return rc;
-    GemmArgs out{};
+    Job out{};
     out.bias0 = q.bo;
     out.out = y;
     out.ld_out = q.out_width;
-    return multiply<T, kOut>(plan.out, out, plan.partials, stream);
+    return multiply<T, kOut>(&second, &out, 1, plan.partials, stream);
 }
 
 struct Gradients {
@@ -985,8 +1218,10 @@ struct BackwardPlan {
     PackArgs jobs;
     int job_count;
     Product inner, values, gate_weight, value_weight, output_weight;
+    const Product *last[kMaxJobs];  // the products behind inner, the longer first, and where they go
+    void *results[kMaxJobs];
     SumArgs sums;
-    float *partials;
+    char *partials;
 };
 
 void plan_backward(BackwardPlan &plan, const Problem &q, const Gradients &g, Pool &pool, char *kept_base) {
@@ -1008,12 +1243,18 @@ void plan_backward(BackwardPlan &plan, const Problem &q, const Gradients &g, Poo
     plan.gate_weight = Product{{dp, {}}, {plan.x, {}}, 1, true, true, q.hidden, q.width};
     plan.value_weight = Product{{dq, {}}, {plan.x, {}}, 1, true, true, q.hidden, q.width};
     plan.output_weight = Product{{plan.dy, {}}, {matrix_of(plan.kept.h, q.rows, q.hidden, q.dtype), {}}, 1, true, true, q.out_width, q.hidden};
-    const int sms = sm_count();
-    size_t most = 0;
-    for (const Product *p : {&plan.inner, &plan.values, &plan.gate_weight, &plan.value_weight, &plan.output_weight}) {
-        most = std::max(most, partial_bytes(cut_of(p->m, p->n, total_k_of(*p, false), false, parts_of(q.dtype), sms), p->m, p->n, false));
+    const Product *candidates[] = {&plan.gate_weight, &plan.value_weight, &plan.output_weight, &plan.values};
+    void *results[] = {g.dwg, g.dwv, g.dwo, g.dx};
+    const bool values_first = total_k_of(plan.values, false) > total_k_of(plan.gate_weight, false);
+    for (int i = 0; i < kMaxJobs; ++i) {
+        const int at = values_first ? (i + 3) % 4 : i;
+        plan.last[i] = candidates[at];
+        plan.results[i] = results[at];
     }
-    plan.partials = static_cast<float *>(pool.take(most));
+    const Product *inner = &plan.inner;
+    const size_t most = std::max(partial_bytes(&inner, 1, false), partial_bytes(plan.last, kMaxJobs, false));
+    plan.partials = static_cast<char *>(pool.take(most));
+    const int sms = sm_count();
     const int64_t columns = std::max(q.hidden, q.out_width);
     plan.sums.rows = q.rows;
     plan.sums.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(q.rows, 64), 16 * sms / ceil_div(columns, 32))));
@@ -1033,26 +1274,24 @@ int backward(const Problem &q, const Gradients &g, const void *kept, void *works
     plan_backward(plan, q, g, pool, static_cast<char *>(const_cast<void *>(kept)));
     int rc = pack_all<T>(plan.jobs, plan.job_count, stream);
     if (rc != KOEMI_OK) return rc;
-    auto plain = [&](const Product &product, void *out) -> int {
-        if (out == nullptr) return KOEMI_OK;
-        GemmArgs args{};
-        args.out = out;
-        args.ld_out = product.n;
-        return multiply<T, kOut>(product, args, plan.partials, stream);
-    };
     if (g.dx != nullptr || g.dwg != nullptr || g.dwv != nullptr || g.dbg != nullptr || g.dbv != nullptr) {
-        GemmArgs inner{};
+        const Product *product = &plan.inner;
+        Job inner{};
         inner.first = plan.dp;
         inner.second = plan.dq;
         inner.p = plan.kept.p;
         inner.q = plan.kept.q;
         inner.ld_pq = plan.kept.ld;
-        rc = multiply<T, kInner>(plan.inner, inner, plan.partials, stream);
+        rc = multiply<T, kInner>(&product, &inner, 1, plan.partials, stream);
     }
-    if (rc == KOEMI_OK) rc = plain(plan.values, g.dx);
-    if (rc == KOEMI_OK) rc = plain(plan.gate_weight, g.dwg);
-    if (rc == KOEMI_OK) rc = plain(plan.value_weight, g.dwv);
-    if (rc == KOEMI_OK) rc = plain(plan.output_weight, g.dwo);
+    if (rc == KOEMI_OK) {
+        Job jobs[kMaxJobs]{};
+        for (int i = 0; i < kMaxJobs; ++i) {
+            jobs[i].out = plan.results[i];
+            jobs[i].ld_out = plan.last[i]->n;
+        }
+        rc = multiply<T, kOut>(plan.last, jobs, kMaxJobs, plan.partials, stream);
+    }
     if (rc != KOEMI_OK) return rc;
     if (g.dbg != nullptr || g.dbv != nullptr || g.dbo != nullptr) {
         const unsigned columns = static_cast<unsigned>(plan.sums.ld);
