@@ -171,6 +171,27 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
     }
 }
 
+// One lane of a converged warp. What its instructions take has to be the same
+// in all lanes and computed by all of them: matrix and copy instructions read
+// uniform registers, and filling those from a single lane's cost 675 clocks a K block.
+__device__ __forceinline__ bool elect() {
+    uint32_t chosen;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
+    return chosen != 0;
+}
+
+// By all lanes of a warp.
+template <bool kCluster>
+__device__ __forceinline__ bool wait_together(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
+    for (uint32_t spin = 0; spin < kWaitSpinLimit; ++spin) {
+        if (__all_sync(0xffffffffu, mbar_try_wait<kCluster>(bar, parity))) return true;
+        if ((spin & 255) == 255 && __any_sync(0xffffffffu, *abort)) return false;
+    }
+    *abort = 1;
+    if (status != nullptr) atomicExch(status, KOEMI_ERR_TIMEOUT);
+    return false;
+}
+
 template <bool kCluster>
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
     for (uint32_t spin = 0; spin < kWaitSpinLimit; ++spin) {
@@ -533,70 +554,66 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
     Tile tile;
 
     if (warp == 0) {
-        if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            while (ok && walk.next(args, job, tile)) {
-                const Job &j = args.jobs[job];
-                const int32_t row = (tile.m * kCtas + rank) * kBM;
-                for (int kb = tile.k_begin; kb < tile.k_end && ok; ++kb) {
-                    const int segment = kEpilogue != kGate && kb >= j.first_blocks;
-                    const CUtensorMap *ma = &j.a[segment], *mb = &j.b[segment];
-                    const int32_t k = (segment ? kb - j.first_blocks : kb) * kBK;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        while (ok && walk.next(args, job, tile)) {
+            const Job &j = args.jobs[job];
+            const int32_t row = (tile.m * kCtas + rank) * kBM;
+            const int32_t column = kEpilogue == kGate ? tile.n * kUnits : tile.n * kTileN + rank * (kTileN / kCtas);
+            const bool a_mn = j.a_mn, b_mn = j.b_mn;
+            const int first_blocks = kEpilogue == kGate ? tile.k_end : j.first_blocks;
+            for (int kb = tile.k_begin; kb < tile.k_end && ok; ++kb) {
+                const int segment = kb >= first_blocks;
+                const CUtensorMap *ma = &j.a[segment], *mb = kEpilogue == kGate && kCtas == 2 ? &j.b[rank] : &j.b[segment];
+                const int32_t k = (segment ? kb - first_blocks : kb) * kBK;
 #pragma unroll 1
-                    for (int part = 0; part < kParts; ++part) {
-                        ok = wait<kCtas == 2>(&empty[stage], phase ^ 1, abort, args.status);
-                        if (!ok) break;
-                        uint8_t *to_a = ring + stage * kStage, *to_b = to_a + kABytes;
-                        const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
+                for (int part = 0; part < kParts; ++part) {
+                    ok = wait_together<kCtas == 2>(&empty[stage], phase ^ 1, abort, args.status);
+                    if (!ok) break;
+                    uint8_t *to_a = ring + stage * kStage, *to_b = to_a + kABytes;
+                    const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
+                    if (elect()) {
                         if (rank == 0) mbar_arrive_expect_tx(&full[stage], kStage * kCtas);
-                        if (j.a_mn) {
+                        if (a_mn) {
                             load_box<kCtas>(to_a, ma, bar, row, k, part);
                             load_box<kCtas>(to_a + kABytes / 2, ma, bar, row + 64, k, part);
                         } else {
                             load_box<kCtas>(to_a, ma, bar, k, row, part);
                         }
                         if constexpr (kEpilogue == kGate) {  // K-major: the units' gate rows, then their value rows
-                            const int32_t unit = tile.n * kUnits;
-                            if constexpr (kCtas == 1) {
-                                load_box<1>(to_b, &j.b[0], bar, k, unit, part);
-                                load_box<1>(to_b + kBBytes / 2, &j.b[1], bar, k, unit, part);
-                            } else {
-                                load_box<2>(to_b, &j.b[rank], bar, k, unit, part);
-                            }
-                        } else {
-                            const int32_t column = tile.n * kTileN + rank * (kTileN / kCtas);
-                            if (j.b_mn) {
+                            load_box<kCtas>(to_b, mb, bar, k, column, part);
+                            if (kCtas == 1) load_box<1>(to_b + kBBytes / 2, &j.b[1], bar, k, column, part);
+                        } else if (b_mn) {
 #pragma unroll
-                                for (int c = 0; c < kTileN / kCtas / 64; ++c) {
-                                    load_box<kCtas>(to_b + c * 8192, mb, bar, column + 64 * c, k, part);
-                                }
-                            } else {
-                                load_box<kCtas>(to_b, mb, bar, k, column, part);
-                            }
-                        }
-                        if (++stage == kStages) {
-                            stage = 0;
-                            phase ^= 1;
+                            for (int c = 0; c < kTileN / kCtas / 64; ++c) load_box<kCtas>(to_b + c * 8192, mb, bar, column + 64 * c, k, part);
+                        } else {
+                            load_box<kCtas>(to_b, mb, bar, k, column, part);
                         }
                     }
-                }
-            }
-            if (*abort && rank == 0) {  // copies still under way land before the CTA ends
-                for (int s = 0; s < kStages; ++s) {
-                    for (uint32_t spin = 0; spin < (1u << 16) && !mbar_try_wait<kCtas == 2>(&full[s], s < stage ? phase : phase ^ 1); ++spin) {
+                    __syncwarp();
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1;
                     }
                 }
             }
         }
+        if (*abort && rank == 0 && lane == 0) {  // copies still under way land before the CTA ends
+            for (int s = 0; s < kStages; ++s) {
+                for (uint32_t spin = 0; spin < (1u << 16) && !mbar_try_wait<kCtas == 2>(&full[s], s < stage ? phase : phase ^ 1); ++spin) {
+                }
+            }
+        }
+        __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
             auto full_accumulator = [&] {
-                commit<kCtas>(&acc_full[acc]);
+                if (elect()) commit<kCtas>(&acc_full[acc]);
+                __syncwarp();
                 if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1;
@@ -607,19 +624,23 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                 const uint32_t idesc = args.jobs[job].idesc;
                 // 16 of K: 16 rows of 128 bytes, or 32 bytes of every row (addresses count 16 bytes)
                 const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
+                const uint64_t kind_a = a_mn ? sw128_mnmajor_desc(0) : sw128_kmajor_desc(0);
+                const uint64_t kind_b = b_mn ? sw128_mnmajor_desc(0) : sw128_kmajor_desc(0);
+                const uint32_t base = smem_addr(ring);
                 uint32_t d = 0;
-                auto multiply_parts = [&](uint32_t to, int at_stage_a, int at_stage_b, bool fresh) {
-                    const uint32_t at_a = smem_addr(ring + at_stage_a * kStage), at_b = smem_addr(ring + at_stage_b * kStage) + kABytes;
-                    const uint64_t da = a_mn ? sw128_mnmajor_desc(at_a) : sw128_kmajor_desc(at_a);
-                    const uint64_t db = b_mn ? sw128_mnmajor_desc(at_b) : sw128_kmajor_desc(at_b);
+                // the K block in `chosen`'s lane: A's part from one stage, B's from another
+                auto multiply_parts = [&](bool chosen, uint32_t to, int stage_a, int stage_b, bool fresh) {
+                    const uint64_t da = kind_a | (base + stage_a * kStage) >> 4, db = kind_b | (base + stage_b * kStage + kABytes) >> 4;
+                    if (chosen) {
 #pragma unroll
-                    for (int k = 0; k < kBK / 16; ++k) mma<kCtas>(to, da + k * step_a, db + k * step_b, idesc, !fresh || k > 0);
+                        for (int k = 0; k < kBK / 16; ++k) mma<kCtas>(to, da + k * step_a, db + k * step_b, idesc, !fresh || k > 0);
+                    }
                 };
                 for (int kb = tile.k_begin; kb < tile.k_end && ok; ++kb) {
                     const bool fresh = kb == tile.k_begin || (kPasses && (kb - tile.k_begin) % kPass == 0);
                     if (fresh) {
                         if (kb > tile.k_begin) full_accumulator();
-                        ok = wait<kCtas == 2>(&acc_empty[acc], acc_phase ^ 1, abort, args.status);
+                        ok = wait_together<kCtas == 2>(&acc_empty[acc], acc_phase ^ 1, abort, args.status);
                         if (!ok) break;
                         tc_fence_after();
                         d = tmem + static_cast<uint32_t>(acc * kAccumulator);
@@ -627,7 +648,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                     int at[kParts];
 #pragma unroll
                     for (int part = 0; part < kParts; ++part) {
-                        ok = wait<kCtas == 2>(&full[stage], phase, abort, args.status);
+                        ok = wait_together<kCtas == 2>(&full[stage], phase, abort, args.status);
                         if (!ok) break;
                         tc_fence_after();
                         at[part] = stage;
@@ -635,20 +656,24 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                             stage = 0;
                             phase ^= 1;
                         }
+                        const bool chosen = elect();
                         if (part == 0) {
-                            multiply_parts(d, at[0], at[0], fresh);
-                            if (kParts == 1) commit<kCtas>(&empty[at[0]]);
+                            multiply_parts(chosen, d, at[0], at[0], fresh);
+                            if (kParts == 1 && chosen) commit<kCtas>(&empty[at[0]]);
                         } else if (part == 1) {
-                            multiply_parts(d + kTileN, at[0], at[part], fresh);
-                            multiply_parts(d + kTileN, at[part], at[0], false);
-                            multiply_parts(d + kTileN, at[part], at[part], false);
-                            commit<kCtas>(&empty[at[part]]);
+                            multiply_parts(chosen, d + kTileN, at[0], at[part], fresh);
+                            multiply_parts(chosen, d + kTileN, at[part], at[0], false);
+                            multiply_parts(chosen, d + kTileN, at[part], at[part], false);
+                            if (chosen) commit<kCtas>(&empty[at[part]]);
                         } else {
-                            multiply_parts(d + kTileN, at[0], at[part], false);
-                            multiply_parts(d + kTileN, at[part], at[0], false);
-                            commit<kCtas>(&empty[at[0]]);
-                            commit<kCtas>(&empty[at[part]]);
+                            multiply_parts(chosen, d + kTileN, at[0], at[part], false);
+                            multiply_parts(chosen, d + kTileN, at[part], at[0], false);
+                            if (chosen) {
+                                commit<kCtas>(&empty[at[0]]);
+                                commit<kCtas>(&empty[at[part]]);
+                            }
                         }
+                        __syncwarp();
                     }
                 }
                 if (ok) full_accumulator();
@@ -974,7 +999,8 @@ Cut cut_of(const Product *const *products, int count, bool gate, int sms) {
     for (const auto &shape : shapes) {
         if (parts > 1 && shape.tile_n > 128) continue;  // two accumulators of two parts, and their sums in registers
         if (shape.ctas == 2 && rows <= kBM) continue;
-        const double clocks = std::max(shape.tile_n * (parts > 1 ? 12.0 : 2.0), parts * (kBM + shape.tile_n / shape.ctas) * kBK * 2 / 52.0);
+        const double loaded = static_cast<double>(std::min<int64_t>(rows, kBM)) + shape.tile_n / shape.ctas;
+        const double clocks = std::max(shape.tile_n * (parts > 1 ? 12.0 : 2.0), parts * loaded * kBK * 2 / 52.0);
         const double places = std::max(1, sms / shape.ctas);
         double work = 0;
         for (int i = 0; i < count; ++i) work += static_cast<double>(tiles_of(*products[i], gate, shape.tile_n, shape.ctas)) * total_k_of(*products[i], gate) * clocks;
@@ -998,7 +1024,7 @@ Cut cut_of(const Product *const *products, int count, bool gate, int sms) {
             const Product &last = *products[count - 1];
             const double shortest = ceil_div(total_k_of(last, gate), cut.splits[count - 1]) * clocks;
             double cost = std::max(longest, std::ceil(load / places / shortest - 1e-9) * shortest) + 6500;
-            if (joined > 0) cost += 6000 + joined / 2500;
+            if (joined > 0) cost += 9000 + joined / 2500;
             if (cost < least) least = cost, best = cut;
         }
     }
