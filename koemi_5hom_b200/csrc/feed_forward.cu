@@ -43,8 +43,8 @@ constexpr uint32_t kABytes = kBM * kBK * 2;
 constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr int kMaxStages = 8;
 constexpr int kMaxJobs = 4;
-// An epilogue warp's staging area: 32 rows of 64 bytes, 16 apart so that rows written 16
-// bytes a lane fall into different banks.
+// An epilogue warp's staging area: 32 rows of up to 64 bytes, 16 apart so that
+// rows written 16 bytes a lane fall into different banks.
 constexpr int kStagedRow = 64 + 16;
 constexpr uint32_t kStagedBytes = 32 * kStagedRow;
 // The tensor cores cut off what an fp32 accumulator cannot hold, which 256
@@ -76,15 +76,24 @@ struct Parts {
     int64_t ld, part_stride;  // elements
 };
 
-// One product, D = A B, or A B + A' B' (two segments of K).
+// Division by a number that the host knows, of values below 2^31.
+struct Divisor {
+    uint32_t magic, shift;
+    __device__ __forceinline__ int of(int n) const {
+        return magic == 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), magic) >> shift);
+    }
+};
+
+// One product, D = A B, or A B + A' B' (two segments of K). What every role
+// reads first comes first: parameters are fetched from memory a line at a time.
 struct Job {
-    CUtensorMap a[2], b[2];  // a segment's operands; kGate: b[0] and b[1] are the gate's and the value's weights
+    int tiles, m_tiles, band, total_k, k_per_split, splits;
     int first_blocks;        // K blocks of the first segment
-    int total_k, splits, k_per_split;
+    int per_split, per_band; // tiles of a part of K, and of a band of rows in it
+    Divisor by_split, by_band, by_rows, by_last_rows;  // rows of a band, and of the last one
     int a_mn, b_mn;          // MN-major operands
     uint32_t idesc;
     int64_t m, n;            // rows and columns of the result (kGate: hidden units)
-    int m_tiles, n_tiles, tiles, band;
     const void *bias0, *bias1;
     void *out;               // kOut
     int64_t ld_out;
@@ -93,16 +102,17 @@ struct Job {
     int64_t ld_pq;
     float *partials;         // splits > 1: raw accumulators [split][gate | value][m][ld_partial]
     int64_t ld_partial;
+    CUtensorMap a[2], b[2];  // a segment's operands; kGate: b[0] and b[1] are the gate's and the value's weights
 };
 
 // Independent products in one launch, in two classes of equal K: the tiles of
 // the longer class go round the places first, `ahead` places get one more, the
 // others catch up on `catch_up` tiles of the second class, and the rest go round.
 struct GemmArgs {
-    Job jobs[kMaxJobs];
     int job_count, first_jobs;
     int first_tiles, second_tiles, ahead, catch_up, places;
     int *status;
+    Job jobs[kMaxJobs];
 };
 
 // ------------------------------------------------------------------- PTX
@@ -213,13 +223,12 @@ struct Tile {
 // together share their operands' tiles in L2.
 __device__ __forceinline__ Tile tile_at(const Job &a, int t) {
     Tile tile;
-    const int per_split = a.m_tiles * a.n_tiles;
-    tile.split = t / per_split;
-    t -= tile.split * per_split;
-    const int per_band = a.band * a.n_tiles;
-    const int band = t / per_band, inside = t - band * per_band;
-    const int rows = min(a.band, a.m_tiles - band * a.band);
-    tile.n = inside / rows;
+    tile.split = a.by_split.of(t);
+    t -= tile.split * a.per_split;
+    const int band = a.by_band.of(t), inside = t - band * a.per_band;
+    const bool last = (band + 1) * a.band > a.m_tiles;
+    const int rows = last ? a.m_tiles - band * a.band : a.band;
+    tile.n = last ? a.by_last_rows.of(inside) : a.by_rows.of(inside);
     tile.m = band * a.band + (inside - tile.n * rows);
     tile.k_begin = tile.split * a.k_per_split;
     tile.k_end = min(a.total_k, tile.k_begin + a.k_per_split);
@@ -295,7 +304,7 @@ __device__ __forceinline__ void store_values(T *dst, int64_t left, const float (
     }
 }
 
-// Where 32 (or, in join_kernel, 8) columns of a result go. Direct: a thread
+// Where columns of a result go, as the epilogues see it. Direct: a thread
 // stores its row's columns itself.
 struct DirectStore {
     int64_t row, column, left;
@@ -306,57 +315,49 @@ struct DirectStore {
     }
 };
 
-// Staged: lane r of a warp holds row r; the rows pass through shared memory, so
-// that a warp stores 64 contiguous bytes of 8 rows at a time, or 32 entries of a
-// row that is off 16 bytes. 2-byte stores down 32 rows took 6 us of a tile.
-struct StagedStore {
+// 32 bytes at a multiple of 32: a whole sector with one instruction.
+__device__ __forceinline__ void store_sector(void *p, const uint4 &a, const uint4 &b) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+                 "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+
+// 16 columns of a warp's 32 rows, lane r holding row r: whole sectors where the
+// rows allow it, else through shared memory, so that a warp stores contiguous
+// entries of a row (2-byte stores down 32 rows took 6 us of a tile).
+struct TileStore {
     uint8_t *area;
-    int64_t row0, column, left;  // the warp's first row
+    int64_t row0, column, left;  // the warp's first row; columns from here to the result's last
     int rows;                    // its rows inside the result
     int lane;
     template <typename E>
-    __device__ __forceinline__ void operator()(E *base, int64_t ld, const float (&in)[32]) const {
-        constexpr int W = Pack<E>::kWidth, kColumns = 4 * W;  // 64 bytes a row
+    __device__ __forceinline__ void operator()(E *base, int64_t ld, const float (&in)[16]) const {
+        constexpr int W = Pack<E>::kWidth, kPieces = 16 / W;
+        uint4 pieces[kPieces];
 #pragma unroll
-        for (int half = 0; half < 32 / kColumns; ++half) {
-            if (half * kColumns >= left) break;
+        for (int i = 0; i < kPieces; ++i) {
+            float part[W];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float part[W];
-#pragma unroll
-                for (int e = 0; e < W; ++e) part[e] = in[half * kColumns + j * W + e];
-                *reinterpret_cast<uint4 *>(area + lane * kStagedRow + 16 * j) = pack(part, E());
-            }
-            __syncwarp();
-            E *dst = base + row0 * ld + column + half * kColumns;
-            const int columns = static_cast<int>(min(left - half * kColumns, static_cast<int64_t>(kColumns)));
-            if (((reinterpret_cast<uintptr_t>(dst) | static_cast<uintptr_t>(ld * sizeof(E))) & 15) == 0) {
-                const int piece = lane & 3;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = i * 8 + (lane >> 2);
-                    if (r >= rows) continue;
-                    const uint4 v = *reinterpret_cast<const uint4 *>(area + r * kStagedRow + 16 * piece);
-                    E *to = dst + r * ld + piece * W;
-                    if (piece * W + W <= columns) {
-                        store_stream(to, v);
-                    } else {
-                        const E *from = reinterpret_cast<const E *>(area + r * kStagedRow) + piece * W;
-                        for (int e = 0; e < columns - piece * W; ++e) to[e] = from[e];
-                    }
-                }
-            } else {
-                const int c = lane % kColumns;
-                constexpr int kRows = 32 / kColumns;
-                if (c < columns) {
-#pragma unroll 4
-                    for (int r = lane / kColumns; r < rows; r += kRows) {
-                        dst[r * ld + c] = reinterpret_cast<const E *>(area + r * kStagedRow)[c];
-                    }
-                }
-            }
-            __syncwarp();
+            for (int e = 0; e < W; ++e) part[e] = in[i * W + e];
+            pieces[i] = pack(part, E());
         }
+        E *dst = base + row0 * ld + column;
+        if (left >= 16 && ((reinterpret_cast<uintptr_t>(dst) | static_cast<uintptr_t>(ld * sizeof(E))) & 31) == 0) {
+            if (lane < rows) {
+#pragma unroll
+                for (int i = 0; i < kPieces; i += 2) store_sector(dst + lane * ld + i * W, pieces[i], pieces[i + 1]);
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) *reinterpret_cast<uint4 *>(area + lane * kStagedRow + 16 * i) = pieces[i];
+        __syncwarp();
+        const int c = lane & 15;
+        if (c < left) {
+#pragma unroll 1
+            for (int r = lane >> 4; r < rows; r += 2) dst[r * ld + c] = reinterpret_cast<const E *>(area + r * kStagedRow)[c];
+        }
+        __syncwarp();
     }
 };
 
@@ -413,19 +414,19 @@ __device__ __forceinline__ void finish_gate(const Job &a, const Store &store, fl
     store_parts<kWide, T>(store, a.first, q);
 }
 
-// kWide kept values of a row as they lie in memory (rows start at 16 bytes and are padded to them).
+// kWide kept values of a row as they lie in memory (rows start at 32 bytes and are padded to them).
 template <int kWide, typename T>
 struct KeptRow {
-    uint4 raw[kWide / Pack<T>::kWidth];
+    static constexpr int W = Pack<T>::kWidth;
+    uint4 raw[kWide / W];
     __device__ __forceinline__ void load(const void *base, int64_t ld, int64_t row, int64_t column, bool live) {
         const T *src = static_cast<const T *>(base) + row * ld + column;
 #pragma unroll
-        for (int i = 0; i < kWide / Pack<T>::kWidth; ++i) {
-            raw[i] = live && column + i * Pack<T>::kWidth < ld ? load_cached(src + i * Pack<T>::kWidth) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kWide / W; ++i) {
+            raw[i] = live && column + i * W < ld ? load_cached(src + i * W) : make_uint4(0, 0, 0, 0);
         }
     }
     __device__ __forceinline__ void values(float (&out)[kWide]) const {
-        constexpr int W = Pack<T>::kWidth;
 #pragma unroll
         for (int i = 0; i < kWide / W; ++i) {
             float part[W];
@@ -454,33 +455,6 @@ __device__ __forceinline__ void finish_inner(const Job &a, const Store &store, c
     }
     store_parts<kWide, T>(store, a.first, q);
     store_parts<kWide, T>(store, a.second, p);
-}
-
-// The same where p and q do not fit the registers beside the sums (fp32): 8
-// columns of them at a time, once for dp and once for dq.
-template <typename T, typename Store>
-__device__ __forceinline__ void finish_inner_slowly(const Job &a, const Store &store, int64_t row, bool live, float (&dh)[32]) {
-    float out[32];
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            KeptRow<8, T> kept;
-            float p[8], q[8];
-            kept.load(a.p, a.ld_pq, row, store.column + 8 * i, live);
-            kept.values(p);
-            if (side == 0) {
-                kept.load(a.q, a.ld_pq, row, store.column + 8 * i, live);
-                kept.values(q);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float s = sigmoid_of<T>(p[e]);
-                out[8 * i + e] = side == 0 ? dp_of(dh[8 * i + e], p[e], q[e], s) : dq_of(dh[8 * i + e], p[e], s);
-            }
-        }
-        store_parts<32, T>(store, side == 0 ? a.first : a.second, out);
-    }
 }
 
 template <int kWide, typename T, typename Store>
@@ -681,9 +655,12 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
         }
         __syncwarp();
     } else {
+        // Groups of 16 columns, alternately for the two warps of a quarter, in a
+        // loop that is not unrolled: a tile's epilogue runs once or twice a
+        // launch of a small problem, at the speed that its code is fetched.
         const int quarter = warp & 3, part = (warp - 2) >> 2;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        constexpr int kChunks = kUnits / 32, kSides = kEpilogue == kGate ? 2 : 1;
+        constexpr int kGroups = kUnits / 16, kSides = kEpilogue == kGate ? 2 : 1;
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -702,23 +679,23 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                 acc_phase ^= 1;
             }
         };
-        StagedStore store{staged + (warp - 2) * kStagedBytes, 0, 0, 0, 0, lane};
+        TileStore store{staged + (warp - 2) * kStagedBytes, 0, 0, 0, 0, lane};
         while (ok && walk.next(args, job, tile)) {
             const Job &j = args.jobs[job];
             store.row0 = static_cast<int64_t>(tile.m * kCtas + rank) * kBM + quarter * 32;
             store.rows = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(32), j.m - store.row0)));
             const int64_t first_column = static_cast<int64_t>(tile.n) * kUnits;
-            KeptRow<32, T> kept_p, kept_q;  // kInner: of the chunk to come
-            auto request = [&](int c) {
-                if constexpr (kEpilogue == kInner && !kPasses) {
-                    if (j.splits > 1 || c >= kChunks) return;
-                    kept_p.load(j.p, j.ld_pq, store.row0 + lane, first_column + c * 32, lane < store.rows);
-                    kept_q.load(j.q, j.ld_pq, store.row0 + lane, first_column + c * 32, lane < store.rows);
+            KeptRow<16, T> kept_p, kept_q;  // kInner: of the group to come
+            auto request = [&](int g) {
+                if constexpr (kEpilogue == kInner) {
+                    if (j.splits > 1 || g >= kGroups) return;
+                    kept_p.load(j.p, j.ld_pq, store.row0 + lane, first_column + g * 16, lane < store.rows);
+                    kept_q.load(j.q, j.ld_pq, store.row0 + lane, first_column + g * 16, lane < store.rows);
                 }
             };
-            // 32 columns of the warp's rows (kGate: of p and of q)
-            auto finish = [&](int c, float (&v)[kSides][32]) {
-                store.column = first_column + c * 32;
+            // 16 columns of the warp's rows (kGate: of p and of q)
+            auto finish = [&](int g, float (&v)[kSides][16]) {
+                store.column = first_column + g * 16;
                 store.left = j.n - store.column;
                 if (store.left <= 0) return;
                 if (j.splits > 1) {
@@ -726,47 +703,43 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
 #pragma unroll
                     for (int k = 0; k < kSides; ++k) store(base + k * j.m * j.ld_partial, j.ld_partial, v[k]);
                 } else if constexpr (kEpilogue == kGate) {
-                    finish_gate<32, T>(j, store, v[0], v[1]);
-                } else if constexpr (kEpilogue == kInner && kPasses) {
-                    finish_inner_slowly<T>(j, store, store.row0 + lane, lane < store.rows, v[0]);
+                    finish_gate<16, T>(j, store, v[0], v[1]);
                 } else if constexpr (kEpilogue == kInner) {
-                    const KeptRow<32, T> p = kept_p, q = kept_q;
-                    request(c + 2);
-                    finish_inner<32, T>(j, store, p, q, v[0]);
+                    const KeptRow<16, T> p = kept_p, q = kept_q;
+                    request(g + 2);
+                    finish_inner<16, T>(j, store, p, q, v[0]);
                 } else {
-                    finish_out<32, T>(j, store, v[0]);
+                    finish_out<16, T>(j, store, v[0]);
                 }
             };
             request(part);
             if constexpr (kPasses) {
-                constexpr int kMine = (kChunks + 1) / 2;
-                float sum[kMine][kSides][32];
+                constexpr int kMine = kGroups / 2;
+                float sum[kMine][kSides][16];
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
 #pragma unroll
                     for (int k = 0; k < kSides; ++k) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) sum[i][k][e] = 0.0f;
+                        for (int e = 0; e < 16; ++e) sum[i][k][e] = 0.0f;
                     }
                 }
                 for (int kb = tile.k_begin; kb < tile.k_end; kb += kPass) {
                     ok = wait<kCtas == 2>(&acc_full[acc], acc_phase, abort, args.status);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t from = tmem + lanes + static_cast<uint32_t>(acc * kAccumulator);
+                    const uint32_t from = tmem + lanes + static_cast<uint32_t>(acc * kAccumulator + part * 16);
 #pragma unroll
                     for (int i = 0; i < kMine; ++i) {
-                        const int c = part + 2 * i;
-                        if (c >= kChunks) continue;
 #pragma unroll
                         for (int k = 0; k < kSides; ++k) {
 #pragma unroll
-                            for (int part = 0; part < 2; ++part) {  // x0 y0, and the rest
-                                uint32_t raw[32];
-                                KOEMI_TMEM_LD32(from + part * kTileN + k * kUnits + c * 32, raw);
+                            for (int which = 0; which < 2; ++which) {  // x0 y0, and the rest
+                                uint32_t raw[16];
+                                KOEMI_TMEM_LD16(from + which * kTileN + k * kUnits + i * 32, raw);
                                 tmem_wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) sum[i][k][e] += __uint_as_float(raw[e]);
+                                for (int e = 0; e < 16; ++e) sum[i][k][e] += __uint_as_float(raw[e]);
                             }
                         }
                     }
@@ -774,27 +747,25 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                 }
                 if (!ok) break;
 #pragma unroll
-                for (int i = 0; i < kMine; ++i) {
-                    if (part + 2 * i < kChunks) finish(part + 2 * i, sum[i]);
-                }
+                for (int i = 0; i < kMine; ++i) finish(part + 2 * i, sum[i]);
             } else {
                 ok = wait<kCtas == 2>(&acc_full[acc], acc_phase, abort, args.status);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t from = tmem + lanes + static_cast<uint32_t>(acc * kAccumulator);
 #pragma unroll 1
-                for (int c = part; c < kChunks; c += 2) {
-                    uint32_t raw[kSides][32];
-                    float v[kSides][32];
+                for (int g = part; g < kGroups; g += 2) {
+                    uint32_t raw[kSides][16];
+                    float v[kSides][16];
 #pragma unroll
-                    for (int k = 0; k < kSides; ++k) KOEMI_TMEM_LD32(from + k * kUnits + c * 32, raw[k]);
+                    for (int k = 0; k < kSides; ++k) KOEMI_TMEM_LD16(from + k * kUnits + g * 16, raw[k]);
                     tmem_wait_ld();
 #pragma unroll
                     for (int k = 0; k < kSides; ++k) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) v[k][e] = __uint_as_float(raw[k][e]);
+                        for (int e = 0; e < 16; ++e) v[k][e] = __uint_as_float(raw[k][e]);
                     }
-                    finish(c, v);
+                    finish(g, v);
                 }
                 release();
             }
@@ -835,7 +806,7 @@ __global__ __launch_bounds__(256) void join_kernel(const __grid_constant__ GemmA
 #pragma unroll
         for (int k = 0; k < kSides; ++k) {
             float v[8];
-            load_values<8>(src + (kSides * s + k) * side, 8, v);  // ld_partial is a multiple of 8
+            load_values<8>(src + (kSides * s + k) * side, 8, v);  // ld_partial is a multiple of 16
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[k][e] += v[e];
         }
@@ -862,7 +833,7 @@ struct PackArgs {
     PackJob jobs[kMaxPacks];
 };
 
-// Row-major matrices copied (fp32: split) to rows of a multiple of 8 columns, zeros behind the last. grid.y: the matrix.
+// Row-major matrices copied (fp32: split) to rows of a multiple of 16 columns, zeros behind the last. grid.y: the matrix.
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(const __grid_constant__ PackArgs args) {
     const PackJob &job = args.jobs[blockIdx.y];
@@ -946,7 +917,7 @@ struct Matrix {
     int parts;
 };
 
-int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
+int64_t round16(int64_t v) { return (v + 15) / 16 * 16; }  // whole sectors of 16-bit values
 size_t round256(size_t v) { return (v + 255) & ~size_t(255); }
 
 int encode(CUtensorMap *map, const Matrix &matrix, bool half, bool mn_major, int box_rows) {
@@ -1032,7 +1003,7 @@ Cut cut_of(const Product *const *products, int count, bool gate, int sms) {
 }
 
 size_t partial_bytes(const Cut &cut, int i, const Product &p, bool gate) {
-    return cut.splits[i] == 1 ? 0 : round256(static_cast<size_t>(cut.splits[i]) * (gate ? 2 : 1) * p.m * round8(p.n) * sizeof(float));
+    return cut.splits[i] == 1 ? 0 : round256(static_cast<size_t>(cut.splits[i]) * (gate ? 2 : 1) * p.m * round16(p.n) * sizeof(float));
 }
 
 // What the products of one launch, cut alike, need for their partial sums.
@@ -1055,6 +1026,15 @@ int launch_shape(GemmArgs &args, cudaStream_t stream) {
     KOEMI_CUDA_TRY(launch_programmatic(false, kernel, dim3(static_cast<unsigned>(args.places * kCtas)), dim3(kThreads), kSmemBytes, stream,
                                        dim3(kCtas, 1, 1), args));
     return KOEMI_OK;
+}
+
+// n / d == umulhi(n, magic) >> shift for 0 <= n < 2^31: magic = ceil(2^(32 + shift) / d) exceeds 2^(32 + shift) / d
+// by less than 1, so the quotient by less than n / 2^(32 + shift) < 1 / d with 2^shift >= d / 2.
+Divisor divisor(int d) {
+    if (d == 1) return Divisor{0, 0};
+    uint32_t shift = 0;
+    while ((int64_t(2) << shift) < d) ++shift;
+    return Divisor{static_cast<uint32_t>(((uint64_t(1) << (32 + shift)) + d - 1) / d), shift};
 }
 
 // Independent products in one launch, those of the longer K first; jobs: their
@@ -1082,10 +1062,19 @@ int multiply(const Product *const *products, const Job *jobs, int count, char *p
         j.m = p.m;
         j.n = p.n;
         j.m_tiles = static_cast<int>(ceil_div(p.m, kBM * cut.ctas));
-        j.n_tiles = static_cast<int>(ceil_div(p.n, gate ? cut.tile_n / 2 : cut.tile_n));
-        j.band = std::max(1, 16 / cut.ctas);
+        const int64_t n_tiles = ceil_div(p.n, gate ? cut.tile_n / 2 : cut.tile_n);
+        const int64_t own = j.m_tiles * n_tiles * j.splits;
+        if (own > INT32_MAX / 2) return fail(KOEMI_ERR_INVALID, "feed-forward sizes are too large");
+        j.tiles = static_cast<int>(own);
+        j.band = std::min(j.m_tiles, 16 / cut.ctas);
+        j.per_split = static_cast<int>(j.m_tiles * n_tiles);
+        j.per_band = static_cast<int>(j.band * n_tiles);
+        j.by_split = divisor(j.per_split);
+        j.by_band = divisor(j.per_band);
+        j.by_rows = divisor(j.band);
+        j.by_last_rows = divisor(j.m_tiles % j.band == 0 ? j.band : j.m_tiles % j.band);
         j.partials = reinterpret_cast<float *>(partials);
-        j.ld_partial = round8(p.n);
+        j.ld_partial = round16(p.n);
         partials += partial_bytes(cut, i, p, gate);
         j.idesc = 1u << 4 | (half ? 0u : 1u << 7 | 1u << 10) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u) |
                   static_cast<uint32_t>(cut.tile_n >> 3) << 17 | static_cast<uint32_t>(kBM * cut.ctas >> 4) << 24;
@@ -1094,12 +1083,10 @@ int multiply(const Product *const *products, const Job *jobs, int count, char *p
             if (rc == KOEMI_OK) rc = encode(&j.b[s], p.b[s], half, p.b_mn, gate ? cut.tile_n / 2 : cut.tile_n / cut.ctas);
             if (rc != KOEMI_OK) return rc;
         }
-        const int64_t own = static_cast<int64_t>(j.m_tiles) * j.n_tiles * j.splits;
         const bool first = args.jobs[0].k_per_split == j.k_per_split && args.first_jobs == at;
         tiles[first ? 0 : 1] += own;
         if (first) ++args.first_jobs;
         if (tiles[0] + tiles[1] > INT32_MAX / 2) return fail(KOEMI_ERR_INVALID, "feed-forward sizes are too large");
-        j.tiles = static_cast<int>(own);
         if (j.splits > 1) most = std::max(most, ceil_div(p.n, 8) * p.m);
     }
     if (args.job_count == 0) return KOEMI_OK;
@@ -1149,7 +1136,7 @@ struct Kept {
 
 Kept kept_of(Pool &pool, int64_t rows, int64_t hidden, int dtype, bool with_pq) {
     Kept kept{};
-    kept.ld = round8(hidden);
+    kept.ld = round16(hidden);
     const size_t count = static_cast<size_t>(rows) * kept.ld;
     kept.h = Parts{pool.take(count * 2 * parts_of(dtype)), kept.ld, rows * kept.ld};
     if (with_pq) {
@@ -1163,7 +1150,7 @@ Kept kept_of(Pool &pool, int64_t rows, int64_t hidden, int dtype, bool with_pq) 
 // base is unknown: it asks for room as if the copy were made.
 Matrix operand(Pool &pool, const void *src, int64_t rows, int64_t columns, int64_t ld, int dtype, PackArgs &jobs, int &count) {
     if (dtype != KOEMI_F32 && pool.base != nullptr && ld % 8 == 0 && aligned(src, 16)) return Matrix{src, rows, columns, ld, 0, 1};
-    const int64_t padded = round8(columns);
+    const int64_t padded = round16(columns);
     const Parts to{pool.take(static_cast<size_t>(rows) * padded * 2 * parts_of(dtype)), padded, rows * padded};
     jobs.jobs[count++] = PackJob{src, rows, columns, ld, to};
     return Matrix{to.base, rows, columns, padded, to.part_stride, parts_of(dtype)};
@@ -1259,7 +1246,7 @@ void plan_backward(BackwardPlan &plan, const Problem &q, const Gradients &g, Poo
     plan.wg = operand(pool, q.wg, q.hidden, q.width, q.width, q.dtype, plan.jobs, plan.job_count);
     plan.wv = operand(pool, q.wv, q.hidden, q.width, q.width, q.dtype, plan.jobs, plan.job_count);
     plan.wo = operand(pool, q.wo, q.out_width, q.hidden, q.hidden, q.dtype, plan.jobs, plan.job_count);
-    const int64_t ld = round8(q.hidden);
+    const int64_t ld = round16(q.hidden);
     const size_t bytes = static_cast<size_t>(q.rows) * ld * 2 * parts_of(q.dtype);
     plan.dp = Parts{pool.take(bytes), ld, q.rows * ld};
     plan.dq = Parts{pool.take(bytes), ld, q.rows * ld};

@@ -58,6 +58,15 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
           "=r"(v[29]), "=r"(v[30]), "=r"(v[31])                                                                \
         : "r"(taddr))
 
+#define KOEMI_TMEM_LD16(taddr, v)                                                                              \
+    asm volatile(                                                                                              \
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, " \
+        "%14, %15}, [%16];"                                                                                    \
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),     \
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),             \
+          "=r"(v[15])                                                                                          \
+        : "r"(taddr))
+
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Bounded wait that also watches the CTA abort flag.

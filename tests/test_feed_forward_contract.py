@@ -139,8 +139,8 @@ def test_entries_refuse_bad_arguments_before_touching_the_device():
         return lib.koemi_core_dropout(values, None, one, count, dropped, 1, 2, 3, None, dtype, None)
 
     kept = lib.koemi_dense_gated_feed_forward_kept(10, 20, _native.BF16)
-    assert kept == 3 * 512 and lib.koemi_dense_gated_feed_forward_kept(-1, 20, _native.BF16) == 0  # 10 x 24 values thrice
-    assert lib.koemi_dense_gated_feed_forward_kept(10, 20, _native.F32) == 1536 + 2 * 1024  # three bf16 parts, two fp32 matrices
+    assert kept == 3 * 768 and lib.koemi_dense_gated_feed_forward_kept(-1, 20, _native.BF16) == 0  # 10 x 32 values thrice
+    assert lib.koemi_dense_gated_feed_forward_kept(10, 20, _native.F32) == 2048 + 2 * 1280  # three bf16 parts, two fp32 matrices
     rooms = [lib.koemi_dense_gated_feed_forward_workspace(10, 16, 20, 8, _native.BF16, backward) for backward in (0, 1)]
     assert min(rooms) > 0 and lib.koemi_dense_gated_feed_forward_workspace(10, 16, 20, 8, 99, 0) == 0
     page = ctypes.c_void_p(256)
