@@ -38,7 +38,8 @@ namespace {
 constexpr int kBM = 128;  // accumulator rows of a CTA
 constexpr int kBK = 64;   // K of a stage: 128 bytes of 16-bit values, the swizzle's span
 constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = (2 + kEpilogueWarps) * 32;
+constexpr int kLoaders = 2;  // warps that load, every other stage each
+constexpr int kThreads = (kLoaders + 1 + kEpilogueWarps) * 32;
 constexpr uint32_t kABytes = kBM * kBK * 2;
 constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr int kMaxStages = 8;
@@ -52,8 +53,9 @@ constexpr uint32_t kStagedBytes = 32 * kStagedRow;
 // for fp32 values, the accumulators are added up in registers, rounded to
 // nearest, every kPass K blocks (32 instructions on x0 y0).
 constexpr int kPass = 8;
+constexpr uint32_t kBiasBytes = 128 * sizeof(float);  // an epilogue warp's columns' biases
 constexpr uint32_t kTmemColumns = 512;
-constexpr size_t kSmemBytes = 1024 + kRingBytes + kEpilogueWarps * kStagedBytes + 256;
+constexpr size_t kSmemBytes = 1024 + kRingBytes + kEpilogueWarps * (kStagedBytes + kBiasBytes) + 256;
 static_assert((2 * kMaxStages + 4) * 8 + 8 <= 256, "barrier area");
 
 enum Epilogue : int { kGate = 0, kInner = 1, kOut = 2 };
@@ -111,6 +113,7 @@ struct Job {
 struct GemmArgs {
     int job_count, first_jobs;
     int first_tiles, second_tiles, ahead, catch_up, places;
+    int early;               // the kernel before writes no B: the first stages' are loaded while it ends
     int *status;
     Job jobs[kMaxJobs];
 };
@@ -400,11 +403,18 @@ __device__ __forceinline__ void add_bias(const void *bias, int64_t column, int64
     for (int j = 0; j < kWide; ++j) v[j] += b[j];
 }
 
-// kGate on kWide hidden units of one row: p and q without their biases.
+template <int kWide>
+__device__ __forceinline__ void add_staged(const float *bias, float (&v)[kWide]) {
+#pragma unroll
+    for (int j = 0; j < kWide / 4; ++j) {
+        const float4 b = reinterpret_cast<const float4 *>(bias)[j];
+        v[4 * j] += b.x, v[4 * j + 1] += b.y, v[4 * j + 2] += b.z, v[4 * j + 3] += b.w;
+    }
+}
+
+// kGate on kWide hidden units of one row.
 template <int kWide, typename T, typename Store>
 __device__ __forceinline__ void finish_gate(const Job &a, const Store &store, float (&p)[kWide], float (&q)[kWide]) {
-    add_bias<kWide, T>(a.bias0, store.column, store.left, p);
-    add_bias<kWide, T>(a.bias1, store.column, store.left, q);
     if (a.p != nullptr) {
         store(static_cast<T *>(a.p), a.ld_pq, p);
         store(static_cast<T *>(a.q), a.ld_pq, q);
@@ -459,14 +469,14 @@ __device__ __forceinline__ void finish_inner(const Job &a, const Store &store, c
 
 template <int kWide, typename T, typename Store>
 __device__ __forceinline__ void finish_out(const Job &a, const Store &store, float (&y)[kWide]) {
-    add_bias<kWide, T>(a.bias0, store.column, store.left, y);
     store(static_cast<T *>(a.out), a.ld_out, y);
 }
 
 // ------------------------------------------------------------------- kernel
 //
-// Warp 0 loads, warp 1 multiplies, eight warps finish tiles: two per quarter of
-// the accumulator's lanes, each on half of its columns. Two accumulators, so a
+// Two warps load, every other stage each (one loader spends 430 clocks a stage
+// on its wait and its copies, whatever their size), one multiplies, eight
+// finish tiles: two per quarter of the accumulator's lanes, each on half of its columns. Two accumulators, so a
 // tile is finished while the next is multiplied. kCtas = 2: a pair of CTAs
 // computes 256 rows with one instruction; each loads its 128 rows of A and half
 // of B's columns, so an SM reads a third fewer bytes per product than with a
@@ -488,7 +498,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     uint8_t *staged = ring + kRingBytes;
-    uint64_t *full = reinterpret_cast<uint64_t *>(staged + kEpilogueWarps * kStagedBytes);
+    uint64_t *full = reinterpret_cast<uint64_t *>(staged + kEpilogueWarps * (kStagedBytes + kBiasBytes));
     uint64_t *empty = full + kMaxStages;
     uint64_t *acc_full = empty + kMaxStages;
     uint64_t *acc_empty = acc_full + 2;
@@ -509,7 +519,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
         *abort = 0;
         fence_barrier_init();
     }
-    if (warp == 1) {
+    if (warp == kLoaders) {
         if constexpr (kCtas == 1) {
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kTmemColumns));
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -524,63 +534,96 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     Walk walk(blockIdx.x / kCtas);
-    int job;
-    Tile tile;
+    int job = 0;
+    Tile tile{};
 
-    if (warp == 0) {
-        int stage = 0;
+    pdl_trigger();
+    if (warp < kLoaders) {
+        int stage = 0, turn = 0;
         uint32_t phase = 0;
         bool ok = true;
+        auto advance = [&] {
+            turn ^= 1;
+            if (++stage == kStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        };
+        // B's part of K block kb, and the stage's bytes announced; A's part
+        auto load_b = [&](const Job &j, int kb, int part) {
+            const int segment = kEpilogue != kGate && kb >= j.first_blocks;
+            const CUtensorMap *mb = kEpilogue == kGate && kCtas == 2 ? &j.b[rank] : &j.b[segment];
+            const int32_t k = (segment ? kb - j.first_blocks : kb) * kBK;
+            const int32_t column = kEpilogue == kGate ? tile.n * kUnits : tile.n * kTileN + rank * (kTileN / kCtas);
+            uint8_t *to = ring + stage * kStage + kABytes;
+            const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
+            const bool mn = j.b_mn;
+            if (elect()) {
+                if (rank == 0) mbar_arrive_expect_tx(&full[stage], kStage * kCtas);
+                if constexpr (kEpilogue == kGate) {  // K-major: the units' gate rows, then their value rows
+                    load_box<kCtas>(to, mb, bar, k, column, part);
+                    if (kCtas == 1) load_box<1>(to + kBBytes / 2, &j.b[1], bar, k, column, part);
+                } else if (mn) {
+#pragma unroll
+                    for (int c = 0; c < kTileN / kCtas / 64; ++c) load_box<kCtas>(to + c * 8192, mb, bar, column + 64 * c, k, part);
+                } else {
+                    load_box<kCtas>(to, mb, bar, k, column, part);
+                }
+            }
+        };
+        auto load_a = [&](const Job &j, int kb, int part) {
+            const int segment = kEpilogue != kGate && kb >= j.first_blocks;
+            const CUtensorMap *ma = &j.a[segment];
+            const int32_t k = (segment ? kb - j.first_blocks : kb) * kBK, row = (tile.m * kCtas + rank) * kBM;
+            uint8_t *to = ring + stage * kStage;
+            const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
+            const bool mn = j.a_mn;
+            if (elect()) {
+                if (mn) {
+                    load_box<kCtas>(to, ma, bar, row, k, part);
+                    load_box<kCtas>(to + kABytes / 2, ma, bar, row + 64, k, part);
+                } else {
+                    load_box<kCtas>(to, ma, bar, k, row, part);
+                }
+            }
+        };
+        bool first = true;
         while (ok && walk.next(args, job, tile)) {
             const Job &j = args.jobs[job];
-            const int32_t row = (tile.m * kCtas + rank) * kBM;
-            const int32_t column = kEpilogue == kGate ? tile.n * kUnits : tile.n * kTileN + rank * (kTileN / kCtas);
-            const bool a_mn = j.a_mn, b_mn = j.b_mn;
-            const int first_blocks = kEpilogue == kGate ? tile.k_end : j.first_blocks;
+            int ready = 0;  // stages of this tile whose B is under way
+            if (first && args.early) {
+                ready = min(kStages, (tile.k_end - tile.k_begin) * kParts);
+                for (int i = 0; i < ready; ++i, advance()) {
+                    if (turn == warp) load_b(j, tile.k_begin + i / kParts, i % kParts);
+                }
+                stage = turn = 0;
+                phase = 0;
+            }
+            if (first) pdl_wait();
+            first = false;
             for (int kb = tile.k_begin; kb < tile.k_end && ok; ++kb) {
-                const int segment = kb >= first_blocks;
-                const CUtensorMap *ma = &j.a[segment], *mb = kEpilogue == kGate && kCtas == 2 ? &j.b[rank] : &j.b[segment];
-                const int32_t k = (segment ? kb - first_blocks : kb) * kBK;
 #pragma unroll 1
-                for (int part = 0; part < kParts; ++part) {
-                    ok = wait_together<kCtas == 2>(&empty[stage], phase ^ 1, abort, args.status);
-                    if (!ok) break;
-                    uint8_t *to_a = ring + stage * kStage, *to_b = to_a + kABytes;
-                    const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
-                    if (elect()) {
-                        if (rank == 0) mbar_arrive_expect_tx(&full[stage], kStage * kCtas);
-                        if (a_mn) {
-                            load_box<kCtas>(to_a, ma, bar, row, k, part);
-                            load_box<kCtas>(to_a + kABytes / 2, ma, bar, row + 64, k, part);
-                        } else {
-                            load_box<kCtas>(to_a, ma, bar, k, row, part);
-                        }
-                        if constexpr (kEpilogue == kGate) {  // K-major: the units' gate rows, then their value rows
-                            load_box<kCtas>(to_b, mb, bar, k, column, part);
-                            if (kCtas == 1) load_box<1>(to_b + kBBytes / 2, &j.b[1], bar, k, column, part);
-                        } else if (b_mn) {
-#pragma unroll
-                            for (int c = 0; c < kTileN / kCtas / 64; ++c) load_box<kCtas>(to_b + c * 8192, mb, bar, column + 64 * c, k, part);
-                        } else {
-                            load_box<kCtas>(to_b, mb, bar, k, column, part);
-                        }
+                for (int part = 0; part < kParts; ++part, --ready, advance()) {
+                    if (turn != warp) continue;
+                    if (ready <= 0) {
+                        ok = wait_together<kCtas == 2>(&empty[stage], phase ^ 1, abort, args.status);
+                        if (!ok) break;
+                        load_b(j, kb, part);
                     }
+                    load_a(j, kb, part);
                     __syncwarp();
-                    if (++stage == kStages) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
                 }
             }
         }
-        if (*abort && rank == 0 && lane == 0) {  // copies still under way land before the CTA ends
+        if (first) pdl_wait();
+        if (*abort && warp == 0 && rank == 0 && lane == 0) {  // copies still under way land before the CTA ends
             for (int s = 0; s < kStages; ++s) {
                 for (uint32_t spin = 0; spin < (1u << 16) && !mbar_try_wait<kCtas == 2>(&full[s], s < stage ? phase : phase ^ 1); ++spin) {
                 }
             }
         }
         __syncwarp();
-    } else if (warp == 1) {
+    } else if (warp == kLoaders) {
         if (rank == 0) {
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
@@ -658,7 +701,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
         // Groups of 16 columns, alternately for the two warps of a quarter, in a
         // loop that is not unrolled: a tile's epilogue runs once or twice a
         // launch of a small problem, at the speed that its code is fetched.
-        const int quarter = warp & 3, part = (warp - 2) >> 2;
+        const int quarter = warp & 3, part = (warp - kLoaders - 1) >> 2;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         constexpr int kGroups = kUnits / 16, kSides = kEpilogue == kGate ? 2 : 1;
         int acc = 0;
@@ -679,7 +722,9 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                 acc_phase ^= 1;
             }
         };
-        TileStore store{staged + (warp - 2) * kStagedBytes, 0, 0, 0, 0, lane};
+        TileStore store{staged + (warp - kLoaders - 1) * kStagedBytes, 0, 0, 0, 0, lane};
+        float *const biases = reinterpret_cast<float *>(staged + kEpilogueWarps * kStagedBytes + (warp - kLoaders - 1) * kBiasBytes);
+        bool first = true;
         while (ok && walk.next(args, job, tile)) {
             const Job &j = args.jobs[job];
             store.row0 = static_cast<int64_t>(tile.m * kCtas + rank) * kBM + quarter * 32;
@@ -703,16 +748,34 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
 #pragma unroll
                     for (int k = 0; k < kSides; ++k) store(base + k * j.m * j.ld_partial, j.ld_partial, v[k]);
                 } else if constexpr (kEpilogue == kGate) {
+                    add_staged<16>(biases + g / 2 * 16, v[0]);
+                    add_staged<16>(biases + kUnits / 2 + g / 2 * 16, v[1]);
                     finish_gate<16, T>(j, store, v[0], v[1]);
                 } else if constexpr (kEpilogue == kInner) {
                     const KeptRow<16, T> p = kept_p, q = kept_q;
                     request(g + 2);
                     finish_inner<16, T>(j, store, p, q, v[0]);
                 } else {
+                    add_staged<16>(biases + g / 2 * 16, v[0]);
                     finish_out<16, T>(j, store, v[0]);
                 }
             };
+            if (first) pdl_wait();  // before p and q of the kernel before are read, and anything is written
+            first = false;
             request(part);
+            if constexpr (kEpilogue != kInner) {  // the biases of the warp's columns, while the tile is multiplied
+                if (j.splits == 1) {
+                    __syncwarp();
+#pragma unroll 1
+                    for (int i = lane; i < kSides * kUnits / 2; i += 32) {
+                        const int side = i / (kUnits / 2), c = i % (kUnits / 2);
+                        const int64_t column = first_column + (part + 2 * (c / 16)) * 16 + c % 16;
+                        const T *bias = static_cast<const T *>(side == 0 ? j.bias0 : j.bias1);
+                        biases[i] = bias != nullptr && column < j.n ? to_acc(bias[column]) : 0.0f;
+                    }
+                    __syncwarp();
+                }
+            }
             if constexpr (kPasses) {
                 constexpr int kMine = kGroups / 2;
                 float sum[kMine][kSides][16];
@@ -774,7 +837,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
     tc_fence_before();
     __syncthreads();
     if constexpr (kCtas == 2) cluster_sync();  // no arrival reaches a CTA that has ended
-    if (warp == 1) {
+    if (warp == kLoaders) {
         tc_fence_after();
         if constexpr (kCtas == 1) {
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
@@ -813,10 +876,13 @@ __global__ __launch_bounds__(256) void join_kernel(const __grid_constant__ GemmA
     }
     const DirectStore store{row, column, j.n - column, true};
     if constexpr (kEpilogue == kGate) {
+        add_bias<8, T>(j.bias0, column, store.left, sum[0]);
+        add_bias<8, T>(j.bias1, column, store.left, sum[1]);
         finish_gate<8, T>(j, store, sum[0], sum[1]);
     } else if constexpr (kEpilogue == kInner) {
         finish_inner<8, T>(j, store, kept_p, kept_q, sum[0]);
     } else {
+        add_bias<8, T>(j.bias0, column, store.left, sum[0]);
         finish_out<8, T>(j, store, sum[0]);
     }
 }
@@ -1015,7 +1081,7 @@ size_t partial_bytes(const Product *const *products, int count, bool gate) {
 }
 
 template <typename T, int kEpilogue, int kTileN, int kCtas>
-int launch_shape(GemmArgs &args, cudaStream_t stream) {
+int launch_shape(GemmArgs &args, bool dependent, cudaStream_t stream) {
     auto kernel = gemm_kernel<T, kEpilogue, kTileN, kCtas>;
     KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes)));
     args.places = std::min(args.first_tiles + args.second_tiles, sm_count() / kCtas);
@@ -1023,7 +1089,8 @@ int launch_shape(GemmArgs &args, cudaStream_t stream) {
     args.ahead = args.first_tiles % args.places;
     args.catch_up = args.ahead > 0 && args.second_tiles > 0 ? first / second : 0;
     if (args.ahead == 0) args.catch_up = 0;
-    KOEMI_CUDA_TRY(launch_programmatic(false, kernel, dim3(static_cast<unsigned>(args.places * kCtas)), dim3(kThreads), kSmemBytes, stream,
+    args.early = dependent;
+    KOEMI_CUDA_TRY(launch_programmatic(dependent, kernel, dim3(static_cast<unsigned>(args.places * kCtas)), dim3(kThreads), kSmemBytes, stream,
                                        dim3(kCtas, 1, 1), args));
     return KOEMI_OK;
 }
@@ -1038,10 +1105,12 @@ Divisor divisor(int d) {
 }
 
 // Independent products in one launch, those of the longer K first; jobs: their
-// epilogues' fields. The cut is that of all of them, wanted or not, so that the
+// epilogues' fields. dependent: the stream's last kernel, which writes none of
+// the products' B, may still be running when this one starts; all before it has
+// ended, because no launch that comes first in a call is a dependent one. The cut is that of all of them, wanted or not, so that the
 // workspace does not depend on which are.
 template <typename T, int kEpilogue>
-int multiply(const Product *const *products, const Job *jobs, int count, char *partials, cudaStream_t stream) {
+int multiply(const Product *const *products, const Job *jobs, int count, char *partials, bool dependent, cudaStream_t stream) {
     constexpr bool gate = kEpilogue == kGate;
     const bool half = std::is_same<typename Operand16<T>::type, __half>::value;
     const Cut cut = cut_of(products, count, gate, sm_count());
@@ -1094,11 +1163,11 @@ int multiply(const Product *const *products, const Job *jobs, int count, char *p
     args.second_tiles = static_cast<int>(tiles[1]);
     int rc = KOEMI_OK;
     if (cut.tile_n == 64) {
-        rc = launch_shape<T, kEpilogue, 64, 1>(args, stream);
+        rc = launch_shape<T, kEpilogue, 64, 1>(args, dependent, stream);
     } else if (cut.tile_n == 128) {
-        rc = cut.ctas == 2 ? launch_shape<T, kEpilogue, 128, 2>(args, stream) : launch_shape<T, kEpilogue, 128, 1>(args, stream);
+        rc = cut.ctas == 2 ? launch_shape<T, kEpilogue, 128, 2>(args, dependent, stream) : launch_shape<T, kEpilogue, 128, 1>(args, dependent, stream);
     } else if constexpr (sizeof(T) == 2) {
-        rc = cut.ctas == 2 ? launch_shape<T, kEpilogue, 256, 2>(args, stream) : launch_shape<T, kEpilogue, 256, 1>(args, stream);
+        rc = cut.ctas == 2 ? launch_shape<T, kEpilogue, 256, 2>(args, dependent, stream) : launch_shape<T, kEpilogue, 256, 1>(args, dependent, stream);
     }
     if (rc != KOEMI_OK) return rc;
     if (most > 0) {
@@ -1210,13 +1279,13 @@ int forward(const Problem &q, void *y, void *kept, void *workspace, cudaStream_t
     gate.p = plan.kept.p;
     gate.q = plan.kept.q;
     gate.ld_pq = plan.kept.ld;
-    rc = multiply<T, kGate>(&first, &gate, 1, plan.partials, stream);
+    rc = multiply<T, kGate>(&first, &gate, 1, plan.partials, false, stream);
     if (rc != KOEMI_OK) return rc;
     Job out{};
     out.bias0 = q.bo;
     out.out = y;
     out.ld_out = q.out_width;
-    return multiply<T, kOut>(&second, &out, 1, plan.partials, stream);
+    return multiply<T, kOut>(&second, &out, 1, plan.partials, true, stream);
 }
 
 struct Gradients {
@@ -1287,6 +1356,7 @@ int backward(const Problem &q, const Gradients &g, const void *kept, void *works
     plan_backward(plan, q, g, pool, static_cast<char *>(const_cast<void *>(kept)));
     int rc = pack_all<T>(plan.jobs, plan.job_count, stream);
     if (rc != KOEMI_OK) return rc;
+    bool dependent = false;
     if (g.dx != nullptr || g.dwg != nullptr || g.dwv != nullptr || g.dbg != nullptr || g.dbv != nullptr) {
         const Product *product = &plan.inner;
         Job inner{};
@@ -1295,7 +1365,8 @@ int backward(const Problem &q, const Gradients &g, const void *kept, void *works
         inner.p = plan.kept.p;
         inner.q = plan.kept.q;
         inner.ld_pq = plan.kept.ld;
-        rc = multiply<T, kInner>(&product, &inner, 1, plan.partials, stream);
+        rc = multiply<T, kInner>(&product, &inner, 1, plan.partials, false, stream);
+        dependent = true;
     }
     if (rc == KOEMI_OK) {
         Job jobs[kMaxJobs]{};
@@ -1303,7 +1374,7 @@ int backward(const Problem &q, const Gradients &g, const void *kept, void *works
             jobs[i].out = plan.results[i];
             jobs[i].ld_out = plan.last[i]->n;
         }
-        rc = multiply<T, kOut>(plan.last, jobs, kMaxJobs, plan.partials, stream);
+        rc = multiply<T, kOut>(plan.last, jobs, kMaxJobs, plan.partials, dependent, stream);
     }
     if (rc != KOEMI_OK) return rc;
     if (g.dbg != nullptr || g.dbv != nullptr || g.dbo != nullptr) {
