@@ -90,6 +90,7 @@ struct Divisor {
 // reads first comes first: parameters are fetched from memory a line at a time.
 struct Job {
     int tiles, m_tiles, band, total_k, k_per_split, splits;
+    int a_rows;              // rows of A that a CTA loads of a tile
     int first_blocks;        // K blocks of the first segment
     int per_split, per_band; // tiles of a part of K, and of a band of rows in it
     Divisor by_split, by_band, by_rows, by_last_rows;  // rows of a band, and of the last one
@@ -126,8 +127,12 @@ __device__ __forceinline__ uint32_t cta_rank() {
     return r;
 }
 
+// All threads of the pair. Orders no memory but barriers set up before
+// fence_barrier_init: a release would wait for every store under way, 1700
+// clocks at a tile's end. What one CTA sends to the other's barriers is waited
+// for there before the last of these.
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // The address that `local` has in the first CTA of the pair.
@@ -184,25 +189,31 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
     }
 }
 
-// One lane of a converged warp. What its instructions take has to be the same
-// in all lanes and computed by all of them: matrix and copy instructions read
-// uniform registers, and filling those from a single lane's cost 675 clocks a K block.
+// One lane of a converged warp. The loaders' and the multiplier's whole loops
+// run in such a lane: a warp that parts and meets again for every K block waits
+// each time until its copies or matrix instructions have left (150 to 250 clocks).
 __device__ __forceinline__ bool elect() {
     uint32_t chosen;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
     return chosen != 0;
 }
 
-// By all lanes of a warp.
+// Whether the phase is complete, without waiting. A wait behind copies or matrix
+// instructions comes back late, ready or not, so the next stage is asked for
+// between those of this one.
 template <bool kCluster>
-__device__ __forceinline__ bool wait_together(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
-    for (uint32_t spin = 0; spin < kWaitSpinLimit; ++spin) {
-        if (__all_sync(0xffffffffu, mbar_try_wait<kCluster>(bar, parity))) return true;
-        if ((spin & 255) == 255 && __any_sync(0xffffffffu, *abort)) return false;
+__device__ __forceinline__ bool test(uint64_t *bar, uint32_t parity) {
+    uint32_t done;
+    if constexpr (kCluster) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
     }
-    *abort = 1;
-    if (status != nullptr) atomicExch(status, KOEMI_ERR_TIMEOUT);
-    return false;
+    return done != 0;
 }
 
 template <bool kCluster>
@@ -474,8 +485,7 @@ __device__ __forceinline__ void finish_out(const Job &a, const Store &store, flo
 
 // ------------------------------------------------------------------- kernel
 //
-// Two warps load, every other stage each (one loader spends 430 clocks a stage
-// on its wait and its copies, whatever their size), one multiplies, eight
+// Two warps load, every other stage each, one multiplies, eight
 // finish tiles: two per quarter of the accumulator's lanes, each on half of its columns. Two accumulators, so a
 // tile is finished while the next is multiplied. kCtas = 2: a pair of CTAs
 // computes 256 rows with one instruction; each loads its 128 rows of A and half
@@ -507,6 +517,11 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = kCtas == 1 ? 0 : static_cast<int>(cta_rank());
+    pdl_trigger();
+    Walk walk(blockIdx.x / kCtas);
+    int job = 0;
+    Tile tile{};
+    bool more = walk.next(args, job, tile);  // the parameters come in while barriers and TMEM are set up
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&full[s], 1);
@@ -518,6 +533,10 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
         }
         *abort = 0;
         fence_barrier_init();
+    }
+    if (threadIdx.x == 32) {
+        prefetch_tensor_map(&args.jobs[job].a[0]);
+        prefetch_tensor_map(&args.jobs[job].b[kEpilogue == kGate && kCtas == 2 ? rank : 0]);
     }
     if (warp == kLoaders) {
         if constexpr (kCtas == 1) {
@@ -533,110 +552,104 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
     if constexpr (kCtas == 2) cluster_sync();  // the pair's barriers are set up
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    Walk walk(blockIdx.x / kCtas);
-    int job = 0;
-    Tile tile{};
 
-    pdl_trigger();
     if (warp < kLoaders) {
-        int stage = 0, turn = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        auto advance = [&] {
-            turn ^= 1;
-            if (++stage == kStages) {
-                stage = 0;
-                phase ^= 1;
-            }
-        };
-        // B's part of K block kb, and the stage's bytes announced; A's part
-        auto load_b = [&](const Job &j, int kb, int part) {
-            const int segment = kEpilogue != kGate && kb >= j.first_blocks;
-            const CUtensorMap *mb = kEpilogue == kGate && kCtas == 2 ? &j.b[rank] : &j.b[segment];
-            const int32_t k = (segment ? kb - j.first_blocks : kb) * kBK;
-            const int32_t column = kEpilogue == kGate ? tile.n * kUnits : tile.n * kTileN + rank * (kTileN / kCtas);
-            uint8_t *to = ring + stage * kStage + kABytes;
-            const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
-            const bool mn = j.b_mn;
-            if (elect()) {
-                if (rank == 0) mbar_arrive_expect_tx(&full[stage], kStage * kCtas);
+        if (elect()) {
+            int stage = 0, turn = 0;
+            uint32_t phase = 0;
+            bool ok = true, first = true, next_empty = false;
+            auto advance = [&] {
+                turn ^= 1;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            };
+            // B's part of K block kb, and the stage's bytes announced; A's part
+            auto load_b = [&](const Job &j, int kb, int part) {
+                const int segment = kEpilogue != kGate && kb >= j.first_blocks;
+                const CUtensorMap *mb = kEpilogue == kGate && kCtas == 2 ? &j.b[rank] : &j.b[segment];
+                const int32_t k = (segment ? kb - j.first_blocks : kb) * kBK;
+                const int32_t column = kEpilogue == kGate ? tile.n * kUnits : tile.n * kTileN + rank * (kTileN / kCtas);
+                uint8_t *to = ring + stage * kStage + kABytes;
+                const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
+                if (rank == 0) mbar_arrive_expect_tx(&full[stage], (kBBytes + j.a_rows * (kBK * 2)) * kCtas);
                 if constexpr (kEpilogue == kGate) {  // K-major: the units' gate rows, then their value rows
                     load_box<kCtas>(to, mb, bar, k, column, part);
                     if (kCtas == 1) load_box<1>(to + kBBytes / 2, &j.b[1], bar, k, column, part);
-                } else if (mn) {
+                } else if (j.b_mn) {
 #pragma unroll
                     for (int c = 0; c < kTileN / kCtas / 64; ++c) load_box<kCtas>(to + c * 8192, mb, bar, column + 64 * c, k, part);
                 } else {
                     load_box<kCtas>(to, mb, bar, k, column, part);
                 }
-            }
-        };
-        auto load_a = [&](const Job &j, int kb, int part) {
-            const int segment = kEpilogue != kGate && kb >= j.first_blocks;
-            const CUtensorMap *ma = &j.a[segment];
-            const int32_t k = (segment ? kb - j.first_blocks : kb) * kBK, row = (tile.m * kCtas + rank) * kBM;
-            uint8_t *to = ring + stage * kStage;
-            const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
-            const bool mn = j.a_mn;
-            if (elect()) {
-                if (mn) {
+            };
+            auto load_a = [&](const Job &j, int kb, int part) {
+                const int segment = kEpilogue != kGate && kb >= j.first_blocks;
+                const CUtensorMap *ma = &j.a[segment];
+                const int32_t k = (segment ? kb - j.first_blocks : kb) * kBK, row = (tile.m * kCtas + rank) * kBM;
+                uint8_t *to = ring + stage * kStage;
+                const uint32_t bar = kCtas == 1 ? smem_addr(&full[stage]) : in_leader(smem_addr(&full[stage]));
+                if (j.a_mn) {
                     load_box<kCtas>(to, ma, bar, row, k, part);
                     load_box<kCtas>(to + kABytes / 2, ma, bar, row + 64, k, part);
                 } else {
                     load_box<kCtas>(to, ma, bar, k, row, part);
                 }
-            }
-        };
-        bool first = true;
-        while (ok && walk.next(args, job, tile)) {
-            const Job &j = args.jobs[job];
-            int ready = 0;  // stages of this tile whose B is under way
-            if (first && args.early) {
-                ready = min(kStages, (tile.k_end - tile.k_begin) * kParts);
-                for (int i = 0; i < ready; ++i, advance()) {
-                    if (turn == warp) load_b(j, tile.k_begin + i / kParts, i % kParts);
+            };
+            for (; more && ok; more = walk.next(args, job, tile)) {
+                const Job &j = args.jobs[job];
+                int ready = 0;  // stages of this tile whose B is under way
+                if (first && args.early) {
+                    ready = min(kStages, (tile.k_end - tile.k_begin) * kParts);
+                    for (int i = 0; i < ready; ++i, advance()) {
+                        if (turn == warp) load_b(j, tile.k_begin + i / kParts, i % kParts);
+                    }
+                    stage = turn = 0;
+                    phase = 0;
                 }
-                stage = turn = 0;
-                phase = 0;
+                if (first) pdl_wait();
+                first = false;
+                for (int kb = tile.k_begin; kb < tile.k_end && ok; ++kb) {
+#pragma unroll 1
+                    for (int part = 0; part < kParts; ++part, --ready, advance()) {
+                        if (turn != warp) continue;
+                        if (ready <= 0) {
+                            ok = next_empty || wait<kCtas == 2>(&empty[stage], phase ^ 1, abort, args.status);
+                            if (!ok) break;
+                            const int s = stage + kLoaders < kStages ? stage + kLoaders : stage + kLoaders - kStages;
+                            next_empty = test<kCtas == 2>(&empty[s], s > stage ? phase ^ 1 : phase);
+                            load_b(j, kb, part);
+                        }
+                        load_a(j, kb, part);
+                    }
+                }
             }
             if (first) pdl_wait();
-            first = false;
-            for (int kb = tile.k_begin; kb < tile.k_end && ok; ++kb) {
-#pragma unroll 1
-                for (int part = 0; part < kParts; ++part, --ready, advance()) {
-                    if (turn != warp) continue;
-                    if (ready <= 0) {
-                        ok = wait_together<kCtas == 2>(&empty[stage], phase ^ 1, abort, args.status);
-                        if (!ok) break;
-                        load_b(j, kb, part);
-                    }
-                    load_a(j, kb, part);
-                    __syncwarp();
-                }
+            // the last stages' releases, which the pair's leader sends, have come before the CTA ends
+            for (int i = 0; i < kStages && ok; ++i, advance()) {
+                if (turn == warp) ok = wait<kCtas == 2>(&empty[stage], phase ^ 1, abort, args.status);
             }
-        }
-        if (first) pdl_wait();
-        if (*abort && warp == 0 && rank == 0 && lane == 0) {  // copies still under way land before the CTA ends
-            for (int s = 0; s < kStages; ++s) {
-                for (uint32_t spin = 0; spin < (1u << 16) && !mbar_try_wait<kCtas == 2>(&full[s], s < stage ? phase : phase ^ 1); ++spin) {
+            if (*abort && warp == 0 && rank == 0) {  // copies still under way land before the CTA ends
+                for (int s = 0; s < kStages; ++s) {
+                    for (uint32_t spin = 0; spin < (1u << 16) && !mbar_try_wait<kCtas == 2>(&full[s], s < stage ? phase : phase ^ 1); ++spin) {
+                    }
                 }
             }
         }
         __syncwarp();
     } else if (warp == kLoaders) {
-        if (rank == 0) {
+        if (rank == 0 && elect()) {
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
-            bool ok = true;
-            auto full_accumulator = [&] {
-                if (elect()) commit<kCtas>(&acc_full[acc]);
-                __syncwarp();
+            bool ok = true, next_full = false;
+            auto next_accumulator = [&] {
                 if (++acc == 2) {
                     acc = 0;
                     acc_phase ^= 1;
                 }
             };
-            while (ok && walk.next(args, job, tile)) {
+            for (; more && ok; more = walk.next(args, job, tile)) {
                 const int a_mn = args.jobs[job].a_mn, b_mn = args.jobs[job].b_mn;
                 const uint32_t idesc = args.jobs[job].idesc;
                 // 16 of K: 16 rows of 128 bytes, or 32 bytes of every row (addresses count 16 bytes)
@@ -645,19 +658,23 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                 const uint64_t kind_b = b_mn ? sw128_mnmajor_desc(0) : sw128_kmajor_desc(0);
                 const uint32_t base = smem_addr(ring);
                 uint32_t d = 0;
-                // the K block in `chosen`'s lane: A's part from one stage, B's from another
-                auto multiply_parts = [&](bool chosen, uint32_t to, int stage_a, int stage_b, bool fresh) {
+                // A's part from one stage, B's from another; on the way, whether the stage behind has come
+                auto multiply_parts = [&](uint32_t to, int stage_a, int stage_b, bool fresh, bool ask) {
                     const uint64_t da = kind_a | (base + stage_a * kStage) >> 4, db = kind_b | (base + stage_b * kStage + kABytes) >> 4;
-                    if (chosen) {
 #pragma unroll
-                        for (int k = 0; k < kBK / 16; ++k) mma<kCtas>(to, da + k * step_a, db + k * step_b, idesc, !fresh || k > 0);
+                    for (int k = 0; k < kBK / 16; ++k) {
+                        mma<kCtas>(to, da + k * step_a, db + k * step_b, idesc, !fresh || k > 0);
+                        if (k == 1 && ask) next_full = test<kCtas == 2>(&full[stage], phase);
                     }
                 };
                 for (int kb = tile.k_begin; kb < tile.k_end && ok; ++kb) {
                     const bool fresh = kb == tile.k_begin || (kPasses && (kb - tile.k_begin) % kPass == 0);
                     if (fresh) {
-                        if (kb > tile.k_begin) full_accumulator();
-                        ok = wait_together<kCtas == 2>(&acc_empty[acc], acc_phase ^ 1, abort, args.status);
+                        if (kb > tile.k_begin) {
+                            commit<kCtas>(&acc_full[acc]);
+                            next_accumulator();
+                        }
+                        ok = wait<kCtas == 2>(&acc_empty[acc], acc_phase ^ 1, abort, args.status);
                         if (!ok) break;
                         tc_fence_after();
                         d = tmem + static_cast<uint32_t>(acc * kAccumulator);
@@ -665,7 +682,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                     int at[kParts];
 #pragma unroll
                     for (int part = 0; part < kParts; ++part) {
-                        ok = wait_together<kCtas == 2>(&full[stage], phase, abort, args.status);
+                        ok = next_full || wait<kCtas == 2>(&full[stage], phase, abort, args.status);
                         if (!ok) break;
                         tc_fence_after();
                         at[part] = stage;
@@ -673,27 +690,30 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                             stage = 0;
                             phase ^= 1;
                         }
-                        const bool chosen = elect();
                         if (part == 0) {
-                            multiply_parts(chosen, d, at[0], at[0], fresh);
-                            if (kParts == 1 && chosen) commit<kCtas>(&empty[at[0]]);
+                            multiply_parts(d, at[0], at[0], fresh, true);
+                            if (kParts == 1) commit<kCtas>(&empty[at[0]]);
                         } else if (part == 1) {
-                            multiply_parts(chosen, d + kTileN, at[0], at[part], fresh);
-                            multiply_parts(chosen, d + kTileN, at[part], at[0], false);
-                            multiply_parts(chosen, d + kTileN, at[part], at[part], false);
-                            if (chosen) commit<kCtas>(&empty[at[part]]);
+                            multiply_parts(d + kTileN, at[0], at[part], fresh, false);
+                            multiply_parts(d + kTileN, at[part], at[0], false, false);
+                            multiply_parts(d + kTileN, at[part], at[part], false, true);
+                            commit<kCtas>(&empty[at[part]]);
                         } else {
-                            multiply_parts(chosen, d + kTileN, at[0], at[part], false);
-                            multiply_parts(chosen, d + kTileN, at[part], at[0], false);
-                            if (chosen) {
-                                commit<kCtas>(&empty[at[0]]);
-                                commit<kCtas>(&empty[at[part]]);
-                            }
+                            multiply_parts(d + kTileN, at[0], at[part], false, false);
+                            multiply_parts(d + kTileN, at[part], at[0], false, true);
+                            commit<kCtas>(&empty[at[0]]);
+                            commit<kCtas>(&empty[at[part]]);
                         }
-                        __syncwarp();
                     }
                 }
-                if (ok) full_accumulator();
+                if (ok) {
+                    commit<kCtas>(&acc_full[acc]);
+                    next_accumulator();
+                }
+            }
+            for (int b = 0; b < 2 && ok; ++b) {  // the other CTA's releases of the accumulators have come, too
+                ok = wait<kCtas == 2>(&acc_empty[acc], acc_phase ^ 1, abort, args.status);
+                next_accumulator();
             }
         }
         __syncwarp();
@@ -725,7 +745,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
         TileStore store{staged + (warp - kLoaders - 1) * kStagedBytes, 0, 0, 0, 0, lane};
         float *const biases = reinterpret_cast<float *>(staged + kEpilogueWarps * kStagedBytes + (warp - kLoaders - 1) * kBiasBytes);
         bool first = true;
-        while (ok && walk.next(args, job, tile)) {
+        for (; more && ok; more = walk.next(args, job, tile)) {
             const Job &j = args.jobs[job];
             store.row0 = static_cast<int64_t>(tile.m * kCtas + rank) * kBM + quarter * 32;
             store.rows = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(32), j.m - store.row0)));
@@ -836,7 +856,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
     }
     tc_fence_before();
     __syncthreads();
-    if constexpr (kCtas == 2) cluster_sync();  // no arrival reaches a CTA that has ended
+    if constexpr (kCtas == 2) cluster_sync();  // the pair ends together
     if (warp == kLoaders) {
         tc_fence_after();
         if constexpr (kCtas == 1) {
@@ -1128,6 +1148,8 @@ int multiply(const Product *const *products, const Job *jobs, int count, char *p
         j.k_per_split = static_cast<int>(ceil_div(j.total_k, j.splits));
         j.a_mn = p.a_mn;
         j.b_mn = p.b_mn;
+        // few rows: the others of the accumulator hold whatever the stage held, and are not stored
+        j.a_rows = !p.a_mn && p.m < kBM ? static_cast<int>(ceil_div(p.m, 8) * 8) : kBM;
         j.m = p.m;
         j.n = p.n;
         j.m_tiles = static_cast<int>(ceil_div(p.m, kBM * cut.ctas));
@@ -1148,7 +1170,7 @@ int multiply(const Product *const *products, const Job *jobs, int count, char *p
         j.idesc = 1u << 4 | (half ? 0u : 1u << 7 | 1u << 10) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u) |
                   static_cast<uint32_t>(cut.tile_n >> 3) << 17 | static_cast<uint32_t>(kBM * cut.ctas >> 4) << 24;
         for (int s = 0; s < (gate ? 2 : p.segments); ++s) {
-            int rc = s > 0 && gate ? KOEMI_OK : encode(&j.a[s], p.a[s], half, p.a_mn, kBM);
+            int rc = s > 0 && gate ? KOEMI_OK : encode(&j.a[s], p.a[s], half, p.a_mn, j.a_rows);
             if (rc == KOEMI_OK) rc = encode(&j.b[s], p.b[s], half, p.b_mn, gate ? cut.tile_n / 2 : cut.tile_n / cut.ctas);
             if (rc != KOEMI_OK) return rc;
         }
