@@ -336,6 +336,12 @@ __device__ __forceinline__ void store_sector(void *p, const uint4 &a, const uint
                  : "memory");
 }
 
+__device__ __forceinline__ void load_sector(const void *p, uint4 &a, uint4 &b) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                 : "l"(p));
+}
+
 // 16 columns of a warp's 32 rows, lane r holding row r: whole sectors where the
 // rows allow it, else through shared memory, so that a warp stores contiguous
 // entries of a row (2-byte stores down 32 rows took 6 us of a tile).
@@ -442,9 +448,20 @@ struct KeptRow {
     uint4 raw[kWide / W];
     __device__ __forceinline__ void load(const void *base, int64_t ld, int64_t row, int64_t column, bool live) {
         const T *src = static_cast<const T *>(base) + row * ld + column;
+        if constexpr (kWide * sizeof(T) % 32 == 0) {  // whole sectors
 #pragma unroll
-        for (int i = 0; i < kWide / W; ++i) {
-            raw[i] = live && column + i * W < ld ? load_cached(src + i * W) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < kWide / W; i += 2) {
+                if (live && column + i * W < ld) {
+                    load_sector(src + i * W, raw[i], raw[i + 1]);
+                } else {
+                    raw[i] = raw[i + 1] = make_uint4(0, 0, 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWide / W; ++i) {
+                raw[i] = live && column + i * W < ld ? load_cached(src + i * W) : make_uint4(0, 0, 0, 0);
+            }
         }
     }
     __device__ __forceinline__ void values(float (&out)[kWide]) const {
