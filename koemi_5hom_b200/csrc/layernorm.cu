@@ -72,6 +72,26 @@ struct Packet {
     }
 };
 
+// A thread's packets of a row; p: the row, or NULL behind the last. The next
+// row is asked for as soon as this one's values are taken. (Rings of three and
+// four rows in shared memory by cp.async were slower: 32768 x 2048 bf16 67 for
+// 64 us forward, 115 for 95 backward.)
+template <typename T, bool kVec, int K>
+struct RowPackets {
+    Packet<T, kVec> packets[K];
+    __device__ __forceinline__ void request(const T *p, int team, int t, int width) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * team + t) * Packet<T, kVec>::kWide;
+            if (p != nullptr && c < width) {
+                packets[k].load(p + c);
+            } else {
+                packets[k].zero();
+            }
+        }
+    }
+};
+
 // kWide weights from column c, fp32 or of type T.
 template <typename T, int kWide>
 __device__ __forceinline__ void load_weights(const void *w, bool wide, int c, float (&out)[kWide]) {
@@ -100,101 +120,127 @@ struct Moments {
     float mean, square;  // square: the sum of squared distances from the mean
 };
 
+// The sum over lanes that differ in the bits below `span` (a power of two).
+__device__ __forceinline__ float span_sum(float v, int span) {
+    for (int offset = span >> 1; offset > 0; offset >>= 1) v += __shfl_xor_sync(0xffffffffu, v, offset);
+    return v;
+}
+
 // Mean and rsqrt(variance + eps) from one (mean, square) a warp; counts[w]
-// is the number of elements that warp w holds.
-__device__ __forceinline__ void join(const Moments *parts, const float *counts, int warps, int width, float eps, float &mean,
-                                     float &inverse) {
-    const int lane = threadIdx.x & 31;
-    const float n = lane < warps ? counts[lane] : 0.0f;
-    const Moments part = lane < warps ? parts[lane] : Moments{0.0f, 0.0f};
-    const float inv_width = 1.0f / static_cast<float>(width);
-    mean = warp_sum(n * part.mean) * inv_width;
+// is the number of elements that warp w holds, zero behind the last up to `span`.
+__device__ __forceinline__ void join(const Moments *parts, const float *counts, int warps, int span, float inv_width, float eps,
+                                     float &mean, float &inverse) {
+    const int w = threadIdx.x & (span - 1);
+    const float n = counts[w];
+    const Moments part = w < warps ? parts[w] : Moments{0.0f, 0.0f};
+    mean = span_sum(n * part.mean, span) * inv_width;
     const float gap = part.mean - mean;
-    inverse = rsqrtf(warp_sum(fmaf(n * gap, gap, part.square)) * inv_width + eps);
+    inverse = rsqrtf(span_sum(fmaf(n * gap, gap, part.square), span) * inv_width + eps);
 }
 
-// The longest rows of the forward pass take 1024 threads of the most packets, all others up to 512.
-template <typename T, bool kVec, int K>
-constexpr int most_threads() {
-    return K == (kVec ? 4 : 16) ? 1024 : 512;
+// Two sums over a warp for little more than one: the halves of the warp take
+// one each. a's is in lanes 0 to 15, b's in the others.
+__device__ __forceinline__ float half_sums(float a, float b) {
+    const bool upper = threadIdx.x & 16;
+    float mine = upper ? b : a;
+    mine += __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+    return span_sum(mine, 16);
 }
 
-// kWarp: a warp a row, 8 rows a CTA; else a CTA a row. K packets a thread.
+__host__ __device__ __forceinline__ int span_of(int warps) {
+    int span = 1;
+    while (span < warps) span *= 2;
+    return span;
+}
+
+// kWarp: a warp a row, 8 teams a CTA; else a CTA a row. K packets a thread.
 template <typename T, bool kVec, int K, bool kWarp>
-__global__ __launch_bounds__(kWarp ? 256 : most_threads<T, kVec, K>()) void norm_forward_kernel(const NormRows a, const void *__restrict__ weight, const void *__restrict__ bias, bool wide,
-                                    T *__restrict__ y, float *__restrict__ stats, float eps) {
+__global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const NormRows a, const void *__restrict__ weight,
+                                                                                             const void *__restrict__ bias, bool wide,
+                                                                                             T *__restrict__ y, float *__restrict__ stats, float eps) {
     using P = Packet<T, kVec>;
     constexpr int W = P::kWide;
+    __shared__ Moments parts[kWarp ? 1 : 2][32];
+    __shared__ float counts[32];
     const int team = kWarp ? 32 : blockDim.x;
     const int t = kWarp ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t row = kWarp ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
-    if (kWarp && row >= a.rows) return;
-    const T *x = static_cast<const T *>(a.x) + row_start(a, row);
-    P packets[K];
-    int held = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
+    const int warps = blockDim.x / 32;
+    const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * warps : gridDim.x;
+    int64_t row = kWarp ? static_cast<int64_t>(blockIdx.x) * warps + threadIdx.x / 32 : blockIdx.x;
+    RowPackets<T, kVec, K> next;
+    auto request = [&](int64_t at) {
+        next.request(at < a.rows ? static_cast<const T *>(a.x) + row_start(a, at) : nullptr, team, t, a.width);
+    };
+    request(row);
+    constexpr bool kHeld = K * W <= (kVec ? 16 : 8);  // the weights' columns stay in registers, too
+    float w[kHeld ? K : 1][W], b[kHeld ? K : 1][W], count = static_cast<float>(a.width);
+    auto weights_of = [&](int k, float (&wk)[W], float (&bk)[W]) {
         const int c = (k * team + t) * W;
+#pragma unroll
+        for (int e = 0; e < W; ++e) wk[e] = bk[e] = 0.0f;
         if (c < a.width) {
-            packets[k].load(x + c);
-            held += W;
-        } else {
-            packets[k].zero();
+            load_weights<T>(weight, wide, c, wk);
+            if (bias != nullptr) load_weights<T>(bias, wide, c, bk);
         }
+    };
+    if constexpr (kHeld) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) weights_of(k, w[k], b[k]);
     }
-    float v[K][W], sum = 0.0f;
+    if constexpr (!kWarp) {
+        int held = 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        packets[k].values(v[k]);
-#pragma unroll
-        for (int e = 0; e < W; ++e) sum += v[k][e];
+        for (int k = 0; k < K; ++k) held += (k * team + t) * W < a.width ? W : 0;
+        count = warp_sum(static_cast<float>(held));
+        if (t < 32) counts[t] = 0.0f;
+        __syncthreads();
+        if ((t & 31) == 0) counts[t >> 5] = count;
     }
-    const float count = kWarp ? static_cast<float>(a.width) : warp_sum(static_cast<float>(held));
-    float mean = warp_sum(sum) / fmaxf(count, 1.0f), square = 0.0f;
+    const int span = span_of(warps);
+    const float inv_count = 1.0f / fmaxf(count, 1.0f), inv_width = 1.0f / static_cast<float>(a.width);
+    for (int round = 0; row < a.rows; row += step, round ^= 1) {
+        float v[K][W], mean = 0.0f, inverse = 0.0f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        if ((k * team + t) * W < a.width) {
+        for (int k = 0; k < K; ++k) {
+            next.packets[k].values(v[k]);
 #pragma unroll
-            for (int e = 0; e < W; ++e) {
-                const float gap = v[k][e] - mean;
-                square = fmaf(gap, gap, square);
+            for (int e = 0; e < W; ++e) mean += v[k][e];
+        }
+        if (row + step < a.rows) request(row + step);
+        mean = warp_sum(mean) * inv_count;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if ((k * team + t) * W < a.width) {
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    const float gap = v[k][e] - mean;
+                    inverse = fmaf(gap, gap, inverse);
+                }
             }
         }
-    }
-    square = warp_sum(square);
-    float inverse;
-    if constexpr (kWarp) {
-        inverse = rsqrtf(square / count + eps);
-    } else {
-        __shared__ Moments parts[32];
-        __shared__ float counts[32];
-        if ((t & 31) == 0) {
-            parts[t >> 5] = Moments{mean, square};
-            counts[t >> 5] = count;
-        }
-        __syncthreads();
-        join(parts, counts, (blockDim.x + 31) / 32, a.width, eps, mean, inverse);
-    }
-    if (stats != nullptr && t == 0) {
-        stats[row] = mean;
-        stats[a.rows + row] = inverse;
-    }
-    T *out = y + row * a.width;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int c = (k * team + t) * W;
-        if (c >= a.width) continue;
-        float w[W], b[W];
-        load_weights<T>(weight, wide, c, w);
-        if (bias != nullptr) {
-            load_weights<T>(bias, wide, c, b);
+        inverse = warp_sum(inverse);
+        if constexpr (kWarp) {
+            inverse = rsqrtf(inverse * inv_width + eps);
         } else {
-#pragma unroll
-            for (int e = 0; e < W; ++e) b[e] = 0.0f;
+            // the other round's slots are free: all have passed this round's barrier only after reading them
+            if ((t & 31) == 0) parts[round][t >> 5] = Moments{mean, inverse};
+            __syncthreads();
+            join(parts[round], counts, warps, span, inv_width, eps, mean, inverse);
         }
+        if (stats != nullptr && t == 0) {
+            stats[row] = mean;
+            stats[a.rows + row] = inverse;
+        }
+        T *out = y + row * a.width;
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[k][e] = fmaf((v[k][e] - mean) * inverse, w[e], b[e]);
-        P::store(out + c, v[k]);
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * team + t) * W;
+            if (c >= a.width) continue;
+            if constexpr (!kHeld) weights_of(k, w[0], b[0]);
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[k][e] = fmaf((v[k][e] - mean) * inverse, w[kHeld ? k : 0][e], b[kHeld ? k : 0][e]);
+            P::store(out + c, v[k]);
+        }
     }
 }
 
@@ -238,18 +284,30 @@ __global__ __launch_bounds__(1024) void norm_forward_long_kernel(const NormRows 
 
 // partials: [grid][2][width], NULL where neither dw nor db is wanted; dx may be NULL.
 template <typename T, bool kVec, int K, bool kWarp>
-__global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const NormRows a, const void *__restrict__ weight, bool wide, const float *__restrict__ stats,
-                                     const T *__restrict__ g, T *__restrict__ dx, float *__restrict__ partials) {
+__global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const NormRows a, const void *__restrict__ weight, bool wide,
+                                                                          const float *__restrict__ stats, const T *__restrict__ g,
+                                                                          T *__restrict__ dx, float *__restrict__ partials) {
     using P = Packet<T, kVec>;
     constexpr int W = P::kWide;
-    extern __shared__ float pool[];  // kWarp: [2][width]; else two rounds of two sums a warp
+    extern __shared__ float pool[];  // kWarp: [2][width]
+    __shared__ float slots[kWarp ? 1 : 2][32];  // a round's first sums, then its second
     const int team = kWarp ? 32 : blockDim.x;
     const int t = kWarp ? threadIdx.x & 31 : threadIdx.x;
     const int warps = (blockDim.x + 31) / 32;
     const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * warps : gridDim.x;
     int64_t row = kWarp ? static_cast<int64_t>(blockIdx.x) * warps + threadIdx.x / 32 : blockIdx.x;
     const float inv_width = 1.0f / static_cast<float>(a.width);
+    const int span = span_of(warps);
 
+    RowPackets<T, kVec, K> next_x, next_g;
+    float next_mean = 0.0f, next_inverse = 0.0f;
+    auto request = [&](int64_t at) {
+        const bool live = at < a.rows;
+        next_x.request(live ? static_cast<const T *>(a.x) + row_start(a, at) : nullptr, team, t, a.width);
+        next_g.request(live ? g + at * a.width : nullptr, team, t, a.width);
+        if (live) next_mean = stats[at], next_inverse = stats[a.rows + at];
+    };
+    request(row);
     float w[K][W], dw[K][W], db[K][W];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -258,33 +316,14 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
         for (int e = 0; e < W; ++e) w[k][e] = dw[k][e] = db[k][e] = 0.0f;
         if (c < a.width) load_weights<T>(weight, wide, c, w[k]);
     }
-    P px[K], pg[K];
-    auto request = [&](int64_t r) {
-        const T *x = static_cast<const T *>(a.x) + row_start(a, r), *gr = g + r * a.width;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (k * team + t) * W;
-            if (c < a.width) {
-                px[k].load(x + c);
-                pg[k].load(gr + c);
-            } else {
-                px[k].zero();
-                pg[k].zero();
-            }
-        }
-    };
-    float mean = 0.0f, inverse = 0.0f;
-    if (row < a.rows) {
-        request(row);
-        mean = stats[row], inverse = stats[a.rows + row];
-    }
     for (int round = 0; row < a.rows; row += step, round ^= 1) {
         float u[K][W], q[K][W], first = 0.0f, second = 0.0f;
+        const float mean = next_mean, inverse = next_inverse;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const bool live = (k * team + t) * W < a.width;
-            px[k].values(u[k]);
-            pg[k].values(q[k]);
+            next_x.packets[k].values(u[k]);
+            next_g.packets[k].values(q[k]);
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 u[k][e] = live ? (u[k][e] - mean) * inverse : 0.0f;
@@ -295,34 +334,28 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
                 second = fmaf(q[k][e], u[k][e], second);
             }
         }
-        const float scale = inverse;
-        const int64_t current = row;
-        if (row + step < a.rows) {
-            request(row + step);
-            mean = stats[row + step], inverse = stats[a.rows + row + step];
-        }
+        if (row + step < a.rows) request(row + step);
         if (dx == nullptr) continue;
-        first = warp_sum(first);
-        second = warp_sum(second);
+        float sums = half_sums(first, second);
         if constexpr (!kWarp) {
             // the slots of the other round are free: all have passed this round's
             // barrier only after reading them
-            float2 *slots = reinterpret_cast<float2 *>(pool) + round * 32;
-            if ((t & 31) == 0) slots[t >> 5] = make_float2(first, second);
+            if ((t & 15) == 0) slots[round][(t & 16) + (t >> 5)] = sums;
             __syncthreads();
-            const float2 part = (t & 31) < warps ? slots[t & 31] : make_float2(0.0f, 0.0f);
-            first = warp_sum(part.x);
-            second = warp_sum(part.y);
+            const int w = t & (span - 1);  // at most 16 warps
+            sums = span_sum(w < warps ? slots[round][(t & 16) + w] : 0.0f, span);
         }
+        first = __shfl_sync(0xffffffffu, sums, 0);
+        second = __shfl_sync(0xffffffffu, sums, 16);
         first *= inv_width;
         second *= inv_width;
-        T *out = dx + current * a.width;
+        T *out = dx + row * a.width;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * team + t) * W;
             if (c >= a.width) continue;
 #pragma unroll
-            for (int e = 0; e < W; ++e) q[k][e] = scale * (q[k][e] - first - u[k][e] * second);
+            for (int e = 0; e < W; ++e) q[k][e] = inverse * (q[k][e] - first - u[k][e] * second);
             P::store(out + c, q[k]);
         }
     }
@@ -357,6 +390,96 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
             }
         }
     }
+}
+
+// Wide rows: 1024 threads, one CTA an SM, dw and db of all columns in its
+// shared memory (a register each would be 64 a thread). A row is asked into L2
+// while the one before it is worked on.
+template <typename T, int K>
+__global__ __launch_bounds__(1024) void norm_backward_wide_kernel(const NormRows a, const void *__restrict__ weight, bool wide,
+                                                                  const float *__restrict__ stats, const T *__restrict__ g,
+                                                                  T *__restrict__ dx, float *__restrict__ partials) {
+    constexpr int W = Pack<T>::kWidth;
+    extern __shared__ float4 sums[];  // [dw | db][width / 4]
+    __shared__ float2 slots[2][32];
+    const int t = threadIdx.x, quads = a.width / 4;
+    const float inv_width = 1.0f / static_cast<float>(a.width);
+    if (partials != nullptr) {
+        for (int i = t; i < 2 * quads; i += 1024) sums[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        __syncthreads();
+    }
+    for (int64_t row = blockIdx.x, round = 0; row < a.rows; row += gridDim.x, round ^= 1) {
+        const T *x = static_cast<const T *>(a.x) + row_start(a, row), *gr = g + row * a.width;
+        const float mean = stats[row], inverse = stats[a.rows + row];
+        uint4 px[K], pg[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * 1024 + t) * W;
+            px[k] = pg[k] = make_uint4(0, 0, 0, 0);
+            if (c < a.width) px[k] = load_stream(x + c), pg[k] = load_stream(gr + c);
+        }
+        if (row + gridDim.x < a.rows) {
+            const T *nx = static_cast<const T *>(a.x) + row_start(a, row + gridDim.x), *ng = gr + static_cast<int64_t>(gridDim.x) * a.width;
+            constexpr int kLine = 128 / sizeof(T);
+            for (int c = t * kLine; c < a.width; c += 1024 * kLine) {
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(nx + c));
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(ng + c));
+            }
+        }
+        float first = 0.0f, second = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * 1024 + t) * W;
+            if (c >= a.width) continue;
+            float u[W], q[W], w[W];
+            unpack(px[k], u, T());
+            unpack(pg[k], q, T());
+            load_weights<T>(weight, wide, c, w);
+#pragma unroll
+            for (int e = 0; e < W; ++e) u[e] = (u[e] - mean) * inverse;
+            if (partials != nullptr) {
+#pragma unroll
+                for (int e = 0; e < W; e += 4) {
+                    float4 dw = sums[(c + e) / 4], db = sums[quads + (c + e) / 4];
+                    dw.x = fmaf(q[e], u[e], dw.x), dw.y = fmaf(q[e + 1], u[e + 1], dw.y);
+                    dw.z = fmaf(q[e + 2], u[e + 2], dw.z), dw.w = fmaf(q[e + 3], u[e + 3], dw.w);
+                    db.x += q[e], db.y += q[e + 1], db.z += q[e + 2], db.w += q[e + 3];
+                    sums[(c + e) / 4] = dw;
+                    sums[quads + (c + e) / 4] = db;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                first = fmaf(q[e], w[e], first);
+                second = fmaf(q[e] * w[e], u[e], second);
+            }
+        }
+        if (dx == nullptr) continue;
+        first = warp_sum(first);
+        second = warp_sum(second);
+        if ((t & 31) == 0) slots[round][t >> 5] = make_float2(first, second);
+        __syncthreads();
+        const float2 part = slots[round][t & 31];
+        first = warp_sum(part.x) * inv_width;
+        second = warp_sum(part.y) * inv_width;
+        T *out = dx + row * a.width;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * 1024 + t) * W;
+            if (c >= a.width) continue;
+            float u[W], q[W], w[W];
+            unpack(px[k], u, T());
+            unpack(pg[k], q, T());
+            load_weights<T>(weight, wide, c, w);
+#pragma unroll
+            for (int e = 0; e < W; ++e) q[e] = inverse * (q[e] * w[e] - first - (u[e] - mean) * inverse * second);
+            store_stream(out + c, pack(q, T()));
+        }
+    }
+    if (partials == nullptr) return;
+    __syncthreads();
+    float4 *mine = reinterpret_cast<float4 *>(partials + static_cast<int64_t>(blockIdx.x) * 2 * a.width);
+    for (int i = t; i < 2 * quads; i += 1024) mine[i] = sums[i];
 }
 
 // dx of rows that no team holds in registers: two walks.
@@ -439,6 +562,7 @@ __global__ __launch_bounds__(32 * kFinishWarps) void norm_finish_kernel(const fl
 
 constexpr int kWarpRows = 8;       // rows (warps) a CTA of the warp-a-row kernels
 constexpr int kMostPartials = 1024;  // partial rows of dw and db
+constexpr size_t kMostShared = 224 * 1024;
 
 // How a row is held: packets of `wide` elements, `per_thread` of them a thread.
 struct Plan {
@@ -446,18 +570,24 @@ struct Plan {
     int threads, per_thread;
 };
 
-Plan plan_of(bool vector, int wide, int64_t width, int most_per_thread, int most_threads) {
+// Many rows are bound by instructions, of which a row's sums are a warp's worth
+// whatever it holds, so they get few threads with many elements each: a warp
+// that holds up to `warp_most` packets a lane, else `good` packets a thread and
+// more only where 512 threads need them (32768 x 2048 bf16 forward: 52 us with
+// two packets and their weights in registers, 64 with one, 66 with two and the
+// weights from L1, 68 with eight in a warp). Few rows are bound by latency and
+// get a packet a thread.
+Plan plan_of(bool vector, int wide, int64_t rows, int64_t width, int warp_most, int good, int most, int most_threads) {
     Plan plan{vector, false, true, 0, 0};
     const int64_t packets = ceil_div(width, wide);
-    const int warp_most = std::min(vector ? 4 : 16, most_per_thread);
-    if (packets <= 32 * warp_most) {
+    const bool few = rows < 8 * sm_count();
+    if (packets <= 32 * (few && vector ? 1 : warp_most)) {
         plan.warp = true;
         plan.threads = 32 * kWarpRows;
         plan.per_thread = static_cast<int>(ceil_div(packets, 32));
     } else {
-        // as few packets a thread as 512 threads hold, then up to the limits
-        int per = 1;
-        while (per < most_per_thread && ceil_div(packets, per) > 512) per *= 2;
+        int per = few && vector ? 1 : good;
+        while (per < most && ceil_div(packets, per) > 512) per *= 2;
         const int64_t threads = ceil_div(ceil_div(packets, per), 32) * 32;
         plan.fits = threads <= most_threads;
         plan.threads = static_cast<int>(std::min<int64_t>(threads, most_threads));
@@ -472,48 +602,81 @@ bool rows_fit_vectors(const NormRows &a) {
     return aligned(a.x, 16) && a.width % wide == 0 && a.inner_stride % wide == 0 && (a.inner >= a.rows || a.outer_stride % wide == 0);
 }
 
+// CTAs of `kernel` that the GPU holds at once.
+template <typename Kernel>
+int64_t resident_of(Kernel kernel, int threads, size_t shared) {
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, shared) != cudaSuccess) cudaGetLastError();
+    return static_cast<int64_t>(sm_count()) * std::max(per_sm, 1);
+}
+
+template <typename T, bool kVec, int K, bool kWarp>
+int launch_forward(const Plan &plan, const NormRows &a, const void *weight, const void *bias, bool wide, void *y, float *stats,
+                   float eps, cudaStream_t stream) {
+    auto kernel = norm_forward_kernel<T, kVec, K, kWarp>;
+    const int64_t teams = kWarp ? ceil_div(a.rows, kWarpRows) : a.rows;
+    const int64_t grid = std::min(teams, resident_of(kernel, plan.threads, 0));
+    kernel<<<static_cast<unsigned>(grid), plan.threads, 0, stream>>>(a, weight, bias, wide, static_cast<T *>(y), stats, eps);
+    return KOEMI_OK;
+}
+
 template <typename T, bool kVec, int K>
-void launch_forward(const Plan &plan, const NormRows &a, const void *weight, const void *bias, bool wide, void *y, float *stats,
-                    float eps, cudaStream_t stream) {
-    if (plan.warp) {
-        norm_forward_kernel<T, kVec, K, true><<<static_cast<unsigned>(ceil_div(a.rows, kWarpRows)), plan.threads, 0, stream>>>(
-            a, weight, bias, wide, static_cast<T *>(y), stats, eps);
-    } else {
-        norm_forward_kernel<T, kVec, K, false><<<static_cast<unsigned>(a.rows), plan.threads, 0, stream>>>(
-            a, weight, bias, wide, static_cast<T *>(y), stats, eps);
-    }
+int forward_of(const Plan &plan, const NormRows &a, const void *weight, const void *bias, bool wide, void *y, float *stats, float eps,
+               cudaStream_t stream) {
+    return plan.warp ? launch_forward<T, kVec, K, true>(plan, a, weight, bias, wide, y, stats, eps, stream)
+                     : launch_forward<T, kVec, K, false>(plan, a, weight, bias, wide, y, stats, eps, stream);
 }
 
 template <typename T>
 int forward(const NormRows &a, const void *weight, const void *bias, bool wide, void *y, float *stats, float eps, cudaStream_t stream) {
     const bool vector = rows_fit_vectors<T>(a) && aligned(y, 16) && aligned(weight, 16) && aligned(bias, 16);
-    const Plan plan = plan_of(vector, vector ? Pack<T>::kWidth : 1, a.width, vector ? 4 : 16, 1024);
+    constexpr int kGood = 16 / Pack<T>::kWidth;  // with their weights: 48 registers
+    const Plan plan = plan_of(vector, vector ? Pack<T>::kWidth : 1, a.rows, a.width, vector ? kGood : 16, vector ? kGood : 16, vector ? 8 : 16, 512);
+    int rc = KOEMI_OK;
     if (!plan.fits) {
         norm_forward_long_kernel<T><<<static_cast<unsigned>(a.rows), 1024, 0, stream>>>(a, weight, bias, wide, static_cast<T *>(y), stats, eps);
     } else if (vector) {
-        if (plan.per_thread <= 1) launch_forward<T, true, 1>(plan, a, weight, bias, wide, y, stats, eps, stream);
-        else if (plan.per_thread <= 2) launch_forward<T, true, 2>(plan, a, weight, bias, wide, y, stats, eps, stream);
-        else launch_forward<T, true, 4>(plan, a, weight, bias, wide, y, stats, eps, stream);
+        if (plan.per_thread <= 1) rc = forward_of<T, true, 1>(plan, a, weight, bias, wide, y, stats, eps, stream);
+        else if (plan.per_thread <= 2) rc = forward_of<T, true, 2>(plan, a, weight, bias, wide, y, stats, eps, stream);
+        else if (plan.per_thread <= 4) rc = forward_of<T, true, 4>(plan, a, weight, bias, wide, y, stats, eps, stream);
+        else rc = launch_forward<T, true, 8, false>(plan, a, weight, bias, wide, y, stats, eps, stream);
     } else {
-        if (plan.per_thread <= 4) launch_forward<T, false, 4>(plan, a, weight, bias, wide, y, stats, eps, stream);
-        else launch_forward<T, false, 16>(plan, a, weight, bias, wide, y, stats, eps, stream);
+        if (plan.per_thread <= 4) rc = forward_of<T, false, 4>(plan, a, weight, bias, wide, y, stats, eps, stream);
+        else rc = forward_of<T, false, 16>(plan, a, weight, bias, wide, y, stats, eps, stream);
     }
+    if (rc != KOEMI_OK) return rc;
     KOEMI_LAUNCH_CHECK();
     return KOEMI_OK;
 }
 
-template <typename T, bool kVec, int K>
+template <typename T, bool kVec, int K, bool kWarp>
 int launch_backward(const Plan &plan, const NormRows &a, const void *weight, bool wide, const float *stats, const void *g, void *dx,
-                    float *partials, int64_t *grid_out, cudaStream_t stream) {
-    auto kernel = plan.warp ? norm_backward_kernel<T, kVec, K, true> : norm_backward_kernel<T, kVec, K, false>;
-    const size_t shared = plan.warp ? sizeof(float) * 2 * a.width : sizeof(float2) * 2 * 32;
-    int resident = 0;
-    KOEMI_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, plan.threads, shared));
-    const int64_t teams = plan.warp ? ceil_div(a.rows, kWarpRows) : a.rows;
-    const int64_t grid = std::min<int64_t>({teams, static_cast<int64_t>(sm_count()) * std::max(resident, 1), kMostPartials});
-    kernel<<<static_cast<unsigned>(grid), plan.threads, shared, stream>>>(a, weight, wide, stats, static_cast<const T *>(g),
-                                                                          static_cast<T *>(dx), partials);
-    *grid_out = grid;
+                    float *partials, int64_t *grid, cudaStream_t stream) {
+    auto kernel = norm_backward_kernel<T, kVec, K, kWarp>;
+    const size_t shared = kWarp ? sizeof(float) * 2 * a.width : 0;
+    const int64_t teams = kWarp ? ceil_div(a.rows, kWarpRows) : a.rows;
+    *grid = std::min<int64_t>({teams, resident_of(kernel, plan.threads, shared), kMostPartials});
+    kernel<<<static_cast<unsigned>(*grid), plan.threads, shared, stream>>>(a, weight, wide, stats, static_cast<const T *>(g),
+                                                                           static_cast<T *>(dx), partials);
+    return KOEMI_OK;
+}
+
+// *grid: the number of partial rows.
+template <typename T, bool kVec, int K>
+int backward_of(const Plan &plan, const NormRows &a, const void *weight, bool wide, const float *stats, const void *g, void *dx,
+                float *partials, int64_t *grid, cudaStream_t stream) {
+    return plan.warp ? launch_backward<T, kVec, K, true>(plan, a, weight, wide, stats, g, dx, partials, grid, stream)
+                     : launch_backward<T, kVec, K, false>(plan, a, weight, wide, stats, g, dx, partials, grid, stream);
+}
+
+template <typename T, int K>
+int backward_wide(const NormRows &a, const void *weight, bool wide, const float *stats, const void *g, void *dx, float *partials,
+                  int64_t *grid, cudaStream_t stream) {
+    auto kernel = norm_backward_wide_kernel<T, K>;
+    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostShared)));
+    *grid = std::min<int64_t>(a.rows, sm_count());
+    kernel<<<static_cast<unsigned>(*grid), 1024, partials != nullptr ? sizeof(float) * 2 * a.width : 0, stream>>>(
+        a, weight, wide, stats, static_cast<const T *>(g), static_cast<T *>(dx), partials);
     return KOEMI_OK;
 }
 
@@ -521,11 +684,16 @@ template <typename T>
 int backward(const NormRows &a, const void *weight, bool wide, const float *stats, const void *g, void *dx, void *dw, void *db,
              float *partials, cudaStream_t stream) {
     const bool vector = rows_fit_vectors<T>(a) && aligned(g, 16) && aligned(dx, 16) && aligned(weight, 16);
-    const Plan plan = plan_of(vector, vector ? Pack<T>::kWidth : 1, a.width, vector ? 16 / Pack<T>::kWidth : 16, 512);
+    constexpr int kMost = 16 / Pack<T>::kWidth;  // 16 elements a thread: dw and db take a register each for every one
+    const Plan plan = plan_of(vector, vector ? Pack<T>::kWidth : 1, a.rows, a.width, vector ? kMost : 16, vector ? kMost : 16, vector ? kMost : 16, 512);
     if (dw == nullptr && db == nullptr) partials = nullptr;
     int64_t grid = 0;
     int rc = KOEMI_OK;
-    if (!plan.fits) {
+    const int64_t packets = ceil_div(a.width, Pack<T>::kWidth);
+    if (!plan.fits && vector && packets <= 4096 && sizeof(float) * 2 * a.width <= kMostShared) {
+        rc = packets <= 2048 ? backward_wide<T, 2>(a, weight, wide, stats, g, dx, partials, &grid, stream)
+                             : backward_wide<T, 4>(a, weight, wide, stats, g, dx, partials, &grid, stream);
+    } else if (!plan.fits) {
         if (dx != nullptr) {
             norm_backward_long_kernel<T><<<static_cast<unsigned>(a.rows), 1024, 0, stream>>>(a, weight, wide, stats, static_cast<const T *>(g), static_cast<T *>(dx));
         }
@@ -536,13 +704,12 @@ int backward(const NormRows &a, const void *weight, bool wide, const float *stat
                 a, stats, static_cast<const T *>(g), partials);
         }
     } else if (vector) {
-        // 16 elements a thread at most: dw and db take a register each for every one of them
-        if (plan.per_thread <= 1) rc = launch_backward<T, true, 1>(plan, a, weight, wide, stats, g, dx, partials, &grid, stream);
-        else if (plan.per_thread <= 2) rc = launch_backward<T, true, 2>(plan, a, weight, wide, stats, g, dx, partials, &grid, stream);
-        else if constexpr (sizeof(T) == 4) rc = launch_backward<T, true, 4>(plan, a, weight, wide, stats, g, dx, partials, &grid, stream);
+        if (plan.per_thread <= 1) rc = backward_of<T, true, 1>(plan, a, weight, wide, stats, g, dx, partials, &grid, stream);
+        else if (plan.per_thread <= 2) rc = backward_of<T, true, 2>(plan, a, weight, wide, stats, g, dx, partials, &grid, stream);
+        else if constexpr (sizeof(T) == 4) rc = backward_of<T, true, 4>(plan, a, weight, wide, stats, g, dx, partials, &grid, stream);
     } else {
-        if (plan.per_thread <= 4) rc = launch_backward<T, false, 4>(plan, a, weight, wide, stats, g, dx, partials, &grid, stream);
-        else rc = launch_backward<T, false, 16>(plan, a, weight, wide, stats, g, dx, partials, &grid, stream);
+        if (plan.per_thread <= 4) rc = backward_of<T, false, 4>(plan, a, weight, wide, stats, g, dx, partials, &grid, stream);
+        else rc = backward_of<T, false, 16>(plan, a, weight, wide, stats, g, dx, partials, &grid, stream);
     }
     if (rc != KOEMI_OK) return rc;
     KOEMI_LAUNCH_CHECK();
