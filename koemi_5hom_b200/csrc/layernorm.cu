@@ -116,6 +116,44 @@ __device__ __forceinline__ void load_weights(const void *w, bool wide, int c, fl
     }
 }
 
+// Two fp32 operations an instruction: these kernels are bound by issue slots
+// before they are bound by bytes.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)),
+        "l"(reinterpret_cast<uint64_t &>(c)));
+    return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// A thread's K packets of W elements as pairs.
+template <int W, int N>
+__device__ __forceinline__ void to_pairs(const float (&in)[W], int k, float2 (&out)[N]) {
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+        const int i = k * W + e;
+        if (i % 2 == 0) out[i / 2].x = in[e]; else out[i / 2].y = in[e];
+    }
+}
+template <int W, int N>
+__device__ __forceinline__ void from_pairs(const float2 (&in)[N], int k, float (&out)[W]) {
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+        const int i = k * W + e;
+        out[e] = i % 2 == 0 ? in[i / 2].x : in[i / 2].y;
+    }
+}
+
 struct Moments {
     float mean, square;  // square: the sum of squared distances from the mean
 };
@@ -173,9 +211,10 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const N
     };
     request(row);
     constexpr bool kHeld = K * W <= (kVec ? 16 : 8);  // the weights' columns stay in registers, too
-    float w[kHeld ? K : 1][W], b[kHeld ? K : 1][W], count = static_cast<float>(a.width);
-    auto weights_of = [&](int k, float (&wk)[W], float (&bk)[W]) {
-        const int c = (k * team + t) * W;
+    constexpr int N = K * W / 2;
+    float2 w[kHeld ? N : 1], b[kHeld ? N : 1];
+    float count = static_cast<float>(a.width);
+    auto weights_of = [&](int c, float (&wk)[W], float (&bk)[W]) {
 #pragma unroll
         for (int e = 0; e < W; ++e) wk[e] = bk[e] = 0.0f;
         if (c < a.width) {
@@ -185,7 +224,12 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const N
     };
     if constexpr (kHeld) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) weights_of(k, w[k], b[k]);
+        for (int k = 0; k < K; ++k) {
+            float wk[W], bk[W];
+            weights_of((k * team + t) * W, wk, bk);
+            to_pairs(wk, k, w);
+            to_pairs(bk, k, b);
+        }
     }
     if constexpr (!kWarp) {
         int held = 0;
@@ -199,26 +243,25 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const N
     const int span = span_of(warps);
     const float inv_count = 1.0f / fmaxf(count, 1.0f), inv_width = 1.0f / static_cast<float>(a.width);
     for (int round = 0; row < a.rows; row += step, round ^= 1) {
-        float v[K][W], mean = 0.0f, inverse = 0.0f;
+        float2 v[N], sum = both(0.0f), square = both(0.0f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            next.packets[k].values(v[k]);
-#pragma unroll
-            for (int e = 0; e < W; ++e) mean += v[k][e];
+            float x[W];
+            next.packets[k].values(x);
+            to_pairs(x, k, v);
         }
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum = add2(sum, v[i]);
         if (row + step < a.rows) request(row + step);
-        mean = warp_sum(mean) * inv_count;
+        float mean = warp_sum(sum.x + sum.y) * inv_count;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            if ((k * team + t) * W < a.width) {
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    const float gap = v[k][e] - mean;
-                    inverse = fmaf(gap, gap, inverse);
-                }
-            }
+        for (int i = 0; i < N; ++i) {
+            float2 gap = add2(v[i], both(-mean));
+            if (((2 * i / W) * team + t) * W >= a.width) gap.x = 0.0f;
+            if (((2 * i + 1) / W * team + t) * W >= a.width) gap.y = 0.0f;
+            square = fma2(gap, gap, square);
         }
-        inverse = warp_sum(inverse);
+        float inverse = warp_sum(square.x + square.y);
         if constexpr (kWarp) {
             inverse = rsqrtf(inverse * inv_width + eps);
         } else {
@@ -233,13 +276,24 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const N
         }
         T *out = y + row * a.width;
 #pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = mul2(add2(v[i], both(-mean)), both(inverse));
+        if constexpr (kHeld) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = fma2(v[i], w[i], b[i]);
+        }
+#pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * team + t) * W;
             if (c >= a.width) continue;
-            if constexpr (!kHeld) weights_of(k, w[0], b[0]);
+            float o[W];
+            from_pairs(v, k, o);
+            if constexpr (!kHeld) {
+                float wk[W], bk[W];
+                weights_of(c, wk, bk);
 #pragma unroll
-            for (int e = 0; e < W; ++e) v[k][e] = fmaf((v[k][e] - mean) * inverse, w[kHeld ? k : 0][e], b[kHeld ? k : 0][e]);
-            P::store(out + c, v[k]);
+                for (int e = 0; e < W; ++e) o[e] = fmaf(o[e], wk[e], bk[e]);
+            }
+            P::store(out + c, o);
         }
     }
 }
@@ -308,32 +362,41 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
         if (live) next_mean = stats[at], next_inverse = stats[a.rows + at];
     };
     request(row);
-    float w[K][W], dw[K][W], db[K][W];
+    constexpr int N = K * W / 2;
+    float2 w[N], dw[N], db[N];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = (k * team + t) * W;
+        float wk[W];
 #pragma unroll
-        for (int e = 0; e < W; ++e) w[k][e] = dw[k][e] = db[k][e] = 0.0f;
-        if (c < a.width) load_weights<T>(weight, wide, c, w[k]);
+        for (int e = 0; e < W; ++e) wk[e] = 0.0f;
+        if (c < a.width) load_weights<T>(weight, wide, c, wk);
+        to_pairs(wk, k, w);
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) dw[i] = db[i] = both(0.0f);
     for (int round = 0; row < a.rows; row += step, round ^= 1) {
-        float u[K][W], q[K][W], first = 0.0f, second = 0.0f;
+        float2 u[N], q[N], firsts = both(0.0f), seconds = both(0.0f);
         const float mean = next_mean, inverse = next_inverse;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const bool live = (k * team + t) * W < a.width;
-            next_x.packets[k].values(u[k]);
-            next_g.packets[k].values(q[k]);
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                u[k][e] = live ? (u[k][e] - mean) * inverse : 0.0f;
-                dw[k][e] = fmaf(q[k][e], u[k][e], dw[k][e]);
-                db[k][e] += q[k][e];
-                q[k][e] *= w[k][e];
-                first += q[k][e];
-                second = fmaf(q[k][e], u[k][e], second);
-            }
+            float x[W], y[W];
+            next_x.packets[k].values(x);
+            next_g.packets[k].values(y);
+            to_pairs(x, k, u);
+            to_pairs(y, k, q);
         }
+        // columns behind the last have g = 0 and w = 0: whatever u is there, nothing of it counts
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            u[i] = mul2(add2(u[i], both(-mean)), both(inverse));
+            dw[i] = fma2(q[i], u[i], dw[i]);
+            db[i] = add2(db[i], q[i]);
+            q[i] = mul2(q[i], w[i]);
+            firsts = add2(firsts, q[i]);
+            seconds = fma2(q[i], u[i], seconds);
+        }
+        float first = firsts.x + firsts.y, second = seconds.x + seconds.y;
         if (row + step < a.rows) request(row + step);
         if (dx == nullptr) continue;
         float sums = half_sums(first, second);
@@ -351,44 +414,39 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
         second *= inv_width;
         T *out = dx + row * a.width;
 #pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = mul2(both(inverse), fma2(u[i], both(-second), add2(q[i], both(-first))));
+#pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * team + t) * W;
             if (c >= a.width) continue;
-#pragma unroll
-            for (int e = 0; e < W; ++e) q[k][e] = inverse * (q[k][e] - first - u[k][e] * second);
-            P::store(out + c, q[k]);
+            float o[W];
+            from_pairs(q, k, o);
+            P::store(out + c, o);
         }
     }
     if (partials == nullptr) return;
     float *mine = partials + static_cast<int64_t>(blockIdx.x) * 2 * a.width;
-    if constexpr (kWarp) {  // the CTA's warps add their parts in order
-        for (int turn = 0; turn < warps; ++turn) {
-            if (turn == static_cast<int>(threadIdx.x / 32)) {
+    float *const to = kWarp ? pool : mine;
+    for (int turn = 0; turn < (kWarp ? warps : 1); ++turn) {  // kWarp: the CTA's warps add their parts in order
+        if (!kWarp || turn == static_cast<int>(threadIdx.x / 32)) {
 #pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    const int c = (k * team + t) * W;
-                    if (c >= a.width) continue;
+            for (int k = 0; k < K; ++k) {
+                const int c = (k * team + t) * W;
+                if (c >= a.width) continue;
+                float one[W], other[W];
+                from_pairs(dw, k, one);
+                from_pairs(db, k, other);
 #pragma unroll
-                    for (int e = 0; e < W; ++e) {
-                        pool[c + e] = turn == 0 ? dw[k][e] : pool[c + e] + dw[k][e];
-                        pool[a.width + c + e] = turn == 0 ? db[k][e] : pool[a.width + c + e] + db[k][e];
-                    }
+                for (int e = 0; e < W; ++e) {
+                    to[c + e] = turn == 0 ? one[e] : to[c + e] + one[e];
+                    to[a.width + c + e] = turn == 0 ? other[e] : to[a.width + c + e] + other[e];
                 }
             }
-            __syncthreads();
         }
+        if (kWarp) __syncthreads();
+    }
+    if constexpr (kWarp) {
         for (int i = threadIdx.x; i < 2 * a.width; i += blockDim.x) mine[i] = pool[i];
-    } else {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (k * team + t) * W;
-            if (c >= a.width) continue;
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                mine[c + e] = dw[k][e];
-                mine[a.width + c + e] = db[k][e];
-            }
-        }
     }
 }
 
