@@ -28,6 +28,7 @@ struct NormRows {
     int64_t rows, inner;  // row r starts at (r / inner) * outer_stride + (r % inner) * inner_stride elements
     int64_t outer_stride, inner_stride;
     int width;
+    int lanes;  // of a warp that share a row, where no CTA does (a power of two)
 };
 
 __device__ __forceinline__ int64_t row_start(const NormRows &a, int64_t r) {
@@ -191,7 +192,7 @@ __host__ __device__ __forceinline__ int span_of(int warps) {
     return span;
 }
 
-// kWarp: a warp a row, 8 teams a CTA; else a CTA a row. K packets a thread.
+// kWarp: 8 warps a CTA, a row for every `lanes` lanes; else a CTA a row. K packets a thread.
 template <typename T, bool kVec, int K, bool kWarp>
 __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const NormRows a, const void *__restrict__ weight,
                                                                                              const void *__restrict__ bias, bool wide,
@@ -200,11 +201,13 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const N
     constexpr int W = P::kWide;
     __shared__ Moments parts[kWarp ? 1 : 2][32];
     __shared__ float counts[32];
-    const int team = kWarp ? 32 : blockDim.x;
-    const int t = kWarp ? threadIdx.x & 31 : threadIdx.x;
-    const int warps = blockDim.x / 32;
-    const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * warps : gridDim.x;
-    int64_t row = kWarp ? static_cast<int64_t>(blockIdx.x) * warps + threadIdx.x / 32 : blockIdx.x;
+    const int team = kWarp ? a.lanes : blockDim.x;
+    const int t = kWarp ? threadIdx.x & (team - 1) : threadIdx.x;
+    const int warps = blockDim.x / 32, teams = kWarp ? blockDim.x / team : 1;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
+    // the team's row, and that of its warp's first team: a warp's lanes leave the loop together
+    int64_t row = static_cast<int64_t>(blockIdx.x) * teams + (kWarp ? threadIdx.x / team : 0);
+    int64_t lead = static_cast<int64_t>(blockIdx.x) * teams + (kWarp ? (threadIdx.x & ~31) / team : 0);
     RowPackets<T, kVec, K> next;
     auto request = [&](int64_t at) {
         next.request(at < a.rows ? static_cast<const T *>(a.x) + row_start(a, at) : nullptr, team, t, a.width);
@@ -242,7 +245,7 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const N
     }
     const int span = span_of(warps);
     const float inv_count = 1.0f / fmaxf(count, 1.0f), inv_width = 1.0f / static_cast<float>(a.width);
-    for (int round = 0; row < a.rows; row += step, round ^= 1) {
+    for (int round = 0; lead < a.rows; lead += step, row += step, round ^= 1) {
         float2 v[N], sum = both(0.0f), square = both(0.0f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -252,8 +255,8 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const N
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) sum = add2(sum, v[i]);
-        if (row + step < a.rows) request(row + step);
-        float mean = warp_sum(sum.x + sum.y) * inv_count;
+        if (lead + step < a.rows) request(row + step);
+        float mean = (kWarp ? span_sum(sum.x + sum.y, team) : warp_sum(sum.x + sum.y)) * inv_count;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float2 gap = add2(v[i], both(-mean));
@@ -261,7 +264,7 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const N
             if (((2 * i + 1) / W * team + t) * W >= a.width) gap.y = 0.0f;
             square = fma2(gap, gap, square);
         }
-        float inverse = warp_sum(square.x + square.y);
+        float inverse = kWarp ? span_sum(square.x + square.y, team) : warp_sum(square.x + square.y);
         if constexpr (kWarp) {
             inverse = rsqrtf(inverse * inv_width + eps);
         } else {
@@ -270,6 +273,7 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_forward_kernel(const N
             __syncthreads();
             join(parts[round], counts, warps, span, inv_width, eps, mean, inverse);
         }
+        if (kWarp && row >= a.rows) continue;
         if (stats != nullptr && t == 0) {
             stats[row] = mean;
             stats[a.rows + row] = inverse;
@@ -345,11 +349,12 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
     constexpr int W = P::kWide;
     extern __shared__ float pool[];  // kWarp: [2][width]
     __shared__ float slots[kWarp ? 1 : 2][32];  // a round's first sums, then its second
-    const int team = kWarp ? 32 : blockDim.x;
-    const int t = kWarp ? threadIdx.x & 31 : threadIdx.x;
-    const int warps = (blockDim.x + 31) / 32;
-    const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * warps : gridDim.x;
-    int64_t row = kWarp ? static_cast<int64_t>(blockIdx.x) * warps + threadIdx.x / 32 : blockIdx.x;
+    const int team = kWarp ? a.lanes : blockDim.x;
+    const int t = kWarp ? threadIdx.x & (team - 1) : threadIdx.x;
+    const int warps = blockDim.x / 32, teams = kWarp ? blockDim.x / team : 1;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * teams + (kWarp ? threadIdx.x / team : 0);
+    int64_t lead = static_cast<int64_t>(blockIdx.x) * teams + (kWarp ? (threadIdx.x & ~31) / team : 0);
     const float inv_width = 1.0f / static_cast<float>(a.width);
     const int span = span_of(warps);
 
@@ -359,7 +364,8 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
         const bool live = at < a.rows;
         next_x.request(live ? static_cast<const T *>(a.x) + row_start(a, at) : nullptr, team, t, a.width);
         next_g.request(live ? g + at * a.width : nullptr, team, t, a.width);
-        if (live) next_mean = stats[at], next_inverse = stats[a.rows + at];
+        next_mean = live ? stats[at] : 0.0f;
+        next_inverse = live ? stats[a.rows + at] : 0.0f;
     };
     request(row);
     constexpr int N = K * W / 2;
@@ -375,7 +381,7 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) dw[i] = db[i] = both(0.0f);
-    for (int round = 0; row < a.rows; row += step, round ^= 1) {
+    for (int round = 0; lead < a.rows; lead += step, row += step, round ^= 1) {
         float2 u[N], q[N], firsts = both(0.0f), seconds = both(0.0f);
         const float mean = next_mean, inverse = next_inverse;
 #pragma unroll
@@ -386,7 +392,7 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
             to_pairs(x, k, u);
             to_pairs(y, k, q);
         }
-        // columns behind the last have g = 0 and w = 0: whatever u is there, nothing of it counts
+        // columns and rows behind the last have g = 0 and w = 0: whatever u is there, nothing of it counts
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             u[i] = mul2(add2(u[i], both(-mean)), both(inverse));
@@ -397,19 +403,25 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
             seconds = fma2(q[i], u[i], seconds);
         }
         float first = firsts.x + firsts.y, second = seconds.x + seconds.y;
-        if (row + step < a.rows) request(row + step);
+        if (lead + step < a.rows) request(row + step);
         if (dx == nullptr) continue;
-        float sums = half_sums(first, second);
-        if constexpr (!kWarp) {
-            // the slots of the other round are free: all have passed this round's
-            // barrier only after reading them
-            if ((t & 15) == 0) slots[round][(t & 16) + (t >> 5)] = sums;
-            __syncthreads();
-            const int w = t & (span - 1);  // at most 16 warps
-            sums = span_sum(w < warps ? slots[round][(t & 16) + w] : 0.0f, span);
+        if (kWarp && team < 32) {
+            first = span_sum(first, team);
+            second = span_sum(second, team);
+        } else {
+            float sums = half_sums(first, second);
+            if constexpr (!kWarp) {
+                // the slots of the other round are free: all have passed this
+                // round's barrier only after reading them
+                if ((t & 15) == 0) slots[round][(t & 16) + (t >> 5)] = sums;
+                __syncthreads();
+                const int w = t & (span - 1);  // at most 16 warps
+                sums = span_sum(w < warps ? slots[round][(t & 16) + w] : 0.0f, span);
+            }
+            first = __shfl_sync(0xffffffffu, sums, 0);
+            second = __shfl_sync(0xffffffffu, sums, 16);
         }
-        first = __shfl_sync(0xffffffffu, sums, 0);
-        second = __shfl_sync(0xffffffffu, sums, 16);
+        if (kWarp && row >= a.rows) continue;
         first *= inv_width;
         second *= inv_width;
         T *out = dx + row * a.width;
@@ -427,8 +439,8 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
     if (partials == nullptr) return;
     float *mine = partials + static_cast<int64_t>(blockIdx.x) * 2 * a.width;
     float *const to = kWarp ? pool : mine;
-    for (int turn = 0; turn < (kWarp ? warps : 1); ++turn) {  // kWarp: the CTA's warps add their parts in order
-        if (!kWarp || turn == static_cast<int>(threadIdx.x / 32)) {
+    for (int turn = 0; turn < teams; ++turn) {  // kWarp: the CTA's teams add their parts in order
+        if (!kWarp || turn == static_cast<int>(threadIdx.x / team)) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int c = (k * team + t) * W;
@@ -618,39 +630,42 @@ __global__ __launch_bounds__(32 * kFinishWarps) void norm_finish_kernel(const fl
 
 // -------------------------------------------------------------------- plan
 
-constexpr int kWarpRows = 8;       // rows (warps) a CTA of the warp-a-row kernels
+constexpr int kTeamThreads = 256;  // a CTA of the kernels whose rows are shared by lanes
 constexpr int kMostPartials = 1024;  // partial rows of dw and db
 constexpr size_t kMostShared = 224 * 1024;
 
 // How a row is held: packets of `wide` elements, `per_thread` of them a thread.
 struct Plan {
-    bool vector, warp, fits;
-    int threads, per_thread;
+    bool warp, fits;
+    int threads, per_thread, lanes;
+    int64_t teams_of(int64_t rows) const { return warp ? ceil_div(rows, kTeamThreads / lanes) : rows; }  // CTAs of one row a team
 };
 
 // Many rows are bound by instructions, of which a row's sums are a warp's worth
-// whatever it holds, so they get few threads with many elements each: a warp
-// that holds up to `warp_most` packets a lane, else `good` packets a thread and
-// more only where 512 threads need them (32768 x 2048 bf16 forward: 52 us with
-// two packets and their weights in registers, 64 with one, 66 with two and the
-// weights from L1, 68 with eight in a warp). Few rows are bound by latency and
-// get a packet a thread.
-Plan plan_of(bool vector, int wide, int64_t rows, int64_t width, int warp_most, int good, int most, int most_threads) {
-    Plan plan{vector, false, true, 0, 0};
+// whatever it holds, so they get few threads with many elements each: `good`
+// packets a thread, up to 32 lanes a row and else CTAs, and more only where 512 threads need
+// them (32768 x 2048 bf16 forward: 52 us with two packets and their weights in
+// registers, 64 with one, 66 with two and the weights from L1, 68 with eight in
+// a warp; 524288 x 128: 88 with a warp a row). Few rows are bound by latency and get a packet a thread.
+Plan plan_of(bool vector, int wide, int64_t rows, int64_t width, int warp_good, int good, int most) {
+    Plan plan{false, true, 0, 0, 32};
     const int64_t packets = ceil_div(width, wide);
-    const bool few = rows < 8 * sm_count();
-    if (packets <= 32 * (few && vector ? 1 : warp_most)) {
+    const bool few = vector && rows < 8 * sm_count();
+    if (!vector && packets <= 128) warp_good = 4;
+    if (few) warp_good = good = 1;
+    if (packets <= 32 * warp_good) {
         plan.warp = true;
-        plan.threads = 32 * kWarpRows;
-        plan.per_thread = static_cast<int>(ceil_div(packets, 32));
-    } else {
-        int per = few && vector ? 1 : good;
-        while (per < most && ceil_div(packets, per) > 512) per *= 2;
-        const int64_t threads = ceil_div(ceil_div(packets, per), 32) * 32;
-        plan.fits = threads <= most_threads;
-        plan.threads = static_cast<int>(std::min<int64_t>(threads, most_threads));
-        plan.per_thread = per;
+        plan.threads = kTeamThreads;
+        plan.per_thread = warp_good;
+        plan.lanes = span_of(static_cast<int>(ceil_div(packets, warp_good)));
+        return plan;
     }
+    int per = good;
+    while (per < most && ceil_div(packets, per) > 512) per *= 2;
+    const int64_t threads = ceil_div(ceil_div(packets, per), 32) * 32;
+    plan.fits = threads <= 512;
+    plan.threads = static_cast<int>(std::min<int64_t>(threads, 512));
+    plan.per_thread = per;
     return plan;
 }
 
@@ -669,10 +684,11 @@ int64_t resident_of(Kernel kernel, int threads, size_t shared) {
 }
 
 template <typename T, bool kVec, int K, bool kWarp>
-int launch_forward(const Plan &plan, const NormRows &a, const void *weight, const void *bias, bool wide, void *y, float *stats,
+int launch_forward(const Plan &plan, NormRows a, const void *weight, const void *bias, bool wide, void *y, float *stats,
                    float eps, cudaStream_t stream) {
     auto kernel = norm_forward_kernel<T, kVec, K, kWarp>;
-    const int64_t teams = kWarp ? ceil_div(a.rows, kWarpRows) : a.rows;
+    a.lanes = plan.lanes;
+    const int64_t teams = plan.teams_of(a.rows);
     const int64_t grid = std::min(teams, resident_of(kernel, plan.threads, 0));
     kernel<<<static_cast<unsigned>(grid), plan.threads, 0, stream>>>(a, weight, bias, wide, static_cast<T *>(y), stats, eps);
     return KOEMI_OK;
@@ -689,7 +705,7 @@ template <typename T>
 int forward(const NormRows &a, const void *weight, const void *bias, bool wide, void *y, float *stats, float eps, cudaStream_t stream) {
     const bool vector = rows_fit_vectors<T>(a) && aligned(y, 16) && aligned(weight, 16) && aligned(bias, 16);
     constexpr int kGood = 16 / Pack<T>::kWidth;  // with their weights: 48 registers
-    const Plan plan = plan_of(vector, vector ? Pack<T>::kWidth : 1, a.rows, a.width, vector ? kGood : 16, vector ? kGood : 16, vector ? 8 : 16, 512);
+    const Plan plan = plan_of(vector, vector ? Pack<T>::kWidth : 1, a.rows, a.width, vector ? kGood : 16, vector ? kGood : 16, vector ? 8 : 16);
     int rc = KOEMI_OK;
     if (!plan.fits) {
         norm_forward_long_kernel<T><<<static_cast<unsigned>(a.rows), 1024, 0, stream>>>(a, weight, bias, wide, static_cast<T *>(y), stats, eps);
@@ -708,11 +724,12 @@ int forward(const NormRows &a, const void *weight, const void *bias, bool wide, 
 }
 
 template <typename T, bool kVec, int K, bool kWarp>
-int launch_backward(const Plan &plan, const NormRows &a, const void *weight, bool wide, const float *stats, const void *g, void *dx,
+int launch_backward(const Plan &plan, NormRows a, const void *weight, bool wide, const float *stats, const void *g, void *dx,
                     float *partials, int64_t *grid, cudaStream_t stream) {
     auto kernel = norm_backward_kernel<T, kVec, K, kWarp>;
+    a.lanes = plan.lanes;
     const size_t shared = kWarp ? sizeof(float) * 2 * a.width : 0;
-    const int64_t teams = kWarp ? ceil_div(a.rows, kWarpRows) : a.rows;
+    const int64_t teams = plan.teams_of(a.rows);
     *grid = std::min<int64_t>({teams, resident_of(kernel, plan.threads, shared), kMostPartials});
     kernel<<<static_cast<unsigned>(*grid), plan.threads, shared, stream>>>(a, weight, wide, stats, static_cast<const T *>(g),
                                                                            static_cast<T *>(dx), partials);
@@ -743,7 +760,7 @@ int backward(const NormRows &a, const void *weight, bool wide, const float *stat
              float *partials, cudaStream_t stream) {
     const bool vector = rows_fit_vectors<T>(a) && aligned(g, 16) && aligned(dx, 16) && aligned(weight, 16);
     constexpr int kMost = 16 / Pack<T>::kWidth;  // 16 elements a thread: dw and db take a register each for every one
-    const Plan plan = plan_of(vector, vector ? Pack<T>::kWidth : 1, a.rows, a.width, vector ? kMost : 16, vector ? kMost : 16, vector ? kMost : 16, 512);
+    const Plan plan = plan_of(vector, vector ? Pack<T>::kWidth : 1, a.rows, a.width, vector ? 2 : 16, vector ? kMost : 16, vector ? kMost : 16);
     if (dw == nullptr && db == nullptr) partials = nullptr;
     int64_t grid = 0;
     int rc = KOEMI_OK;
@@ -803,7 +820,7 @@ extern "C" int koemi_core_layer_norm_forward(const void *values, int64_t rows, i
     if (!(eps >= 0.0f) || eps > 3.0e38f) return fail(KOEMI_ERR_INVALID, "eps must be finite and non-negative");
     if (rows == 0) return KOEMI_OK;
     if (values == nullptr || weight == nullptr || out == nullptr) return fail(KOEMI_ERR_INVALID, "values, weight and out must be non-NULL");
-    const NormRows a{values, rows, inner_rows, outer_stride, inner_stride, static_cast<int>(width)};
+    const NormRows a{values, rows, inner_rows, outer_stride, inner_stride, static_cast<int>(width), 32};
     const bool wide = weight_dtype == KOEMI_F32;
     if (dtype == KOEMI_F32) return forward<float>(a, weight, bias, wide, out, stats, eps, as_stream(stream));
     if (dtype == KOEMI_F16) return forward<__half>(a, weight, bias, wide, out, stats, eps, as_stream(stream));
@@ -835,7 +852,7 @@ extern "C" int koemi_core_layer_norm_backward(const void *values, int64_t rows, 
     if (sums && (workspace == nullptr || workspace_bytes < koemi_core_layer_norm_backward_workspace(rows, width))) {
         return fail(KOEMI_ERR_WORKSPACE, "layer norm backward needs %zu workspace bytes", koemi_core_layer_norm_backward_workspace(rows, width));
     }
-    const NormRows a{values, rows, inner_rows, outer_stride, inner_stride, static_cast<int>(width)};
+    const NormRows a{values, rows, inner_rows, outer_stride, inner_stride, static_cast<int>(width), 32};
     const bool wide = weight_dtype == KOEMI_F32;
     float *partials = static_cast<float *>(workspace);
     if (dtype == KOEMI_F32) return backward<float>(a, weight, wide, stats, grad_out, grad_values, grad_weight, grad_bias, partials, as_stream(stream));
