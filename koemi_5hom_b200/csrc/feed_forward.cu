@@ -1,15 +1,15 @@
 // The gated feed-forward block, forward and backward, on tcgen05 tensor cores:
 //
 //   p = x Wg^T + bg, q = x Wv^T + bv, h = silu(p) q, y = h Wo^T + bo;
-//   dh = dy Wo, dq = dh silu(p), dp = dh q s (1 + p (1 - s)), s = sigmoid(p),
+//   dh = dy Wo, dq = dh a, dp = dh b with a = silu(p), b = q s (1 + p (1 - s)), s = sigmoid(p),
 //   dx = dp Wg + dq Wv, dWg = dp^T x, dWv = dq^T x, dWo = dy^T h, and the
 //   biases' gradients are the column sums of dp, dq and dy.
 //
 // One matrix product kernel with three epilogues:
 //   kGate   p and q of the same hidden units side by side in one accumulator,
-//           h from both (and p, q for the backward): both projections, the
+//           h from both (and a, b for the backward): both projections, the
 //           activation and the product in one pass over x;
-//   kInner  dh, and from it, p and q, dp and dq (dh is never stored);
+//   kInner  dh, and from it dp and dq (dh is never stored);
 //   kOut    the plain product, with a bias or without.
 // Its operands are row-major matrices of 16-bit values read by TMA, each with K
 // along its rows (K-major) or down its columns (MN-major): the transposed
@@ -24,10 +24,11 @@
 // cannot describe (a width that is no multiple of 8, a start off 16 bytes) are
 // copied to padded rows first.
 //
-// In 16 bits h, p, q, dp and dq are rounded to the type between two products
-// (h, dp and dq because the tensor cores take no wider operand, p and q because
-// their 32 bits would cost the backward twice the bytes); all sums are fp32.
+// In 16 bits h, dp and dq are rounded to the type between two products, because
+// the tensor cores take no wider operand. a and b stay fp32: in 16 bits they
+// would cost the gradients two roundings more (bf16 3.1e-3 for 2.4e-3 of a gradient's norm). All sums are fp32.
 #include <algorithm>
+#include <atomic>
 
 #include "umma.cuh"
 #include "vec.cuh"
@@ -101,8 +102,8 @@ struct Job {
     void *out;               // kOut
     int64_t ld_out;
     Parts first, second;     // kGate: first = h; kInner: first = dp, second = dq
-    void *p, *q;             // kGate: written (NULL: not wanted); kInner: read
-    int64_t ld_pq;
+    float *a_kept, *b_kept;  // kGate: a and b written (NULL: not wanted); kInner: read. In blocks, see kept_at
+    int64_t kept_blocks;     // of 16 columns
     float *partials;         // splits > 1: raw accumulators [split][gate | value][m][ld_partial]
     int64_t ld_partial;
     CUtensorMap a[2], b[2];  // a segment's operands; kGate: b[0] and b[1] are the gate's and the value's weights
@@ -325,6 +326,8 @@ __device__ __forceinline__ void store_values(T *dst, int64_t left, const float (
 struct DirectStore {
     int64_t row, column, left;
     bool live;
+    __device__ __forceinline__ bool inside() const { return live; }
+    __device__ __forceinline__ int64_t own_row() const { return row; }
     template <int kWide, typename E>
     __device__ __forceinline__ void operator()(E *base, int64_t ld, const float (&in)[kWide]) const {
         if (live && left > 0) store_values<kWide>(base + row * ld + column, left, in);
@@ -352,6 +355,8 @@ struct TileStore {
     int64_t row0, column, left;  // the warp's first row; columns from here to the result's last
     int rows;                    // its rows inside the result
     int lane;
+    __device__ __forceinline__ bool inside() const { return lane < rows; }
+    __device__ __forceinline__ int64_t own_row() const { return row0 + lane; }
     template <typename E>
     __device__ __forceinline__ void operator()(E *base, int64_t ld, const float (&in)[16]) const {
         constexpr int W = Pack<E>::kWidth, kPieces = 16 / W;
@@ -431,70 +436,82 @@ __device__ __forceinline__ void add_staged(const float *bias, float (&v)[kWide])
     }
 }
 
-// kGate on kWide hidden units of one row.
-template <int kWide, typename T, typename Store>
-__device__ __forceinline__ void finish_gate(const Job &a, const Store &store, float (&p)[kWide], float (&q)[kWide]) {
-    if (a.p != nullptr) {
-        store(static_cast<T *>(a.p), a.ld_pq, p);
-        store(static_cast<T *>(a.q), a.ld_pq, q);
-    }
-#pragma unroll
-    for (int j = 0; j < kWide; ++j) q[j] *= p[j] * sigmoid_of<T>(p[j]);
-    store_parts<kWide, T>(store, a.first, q);
+// Where a and b of a row's 8 columns lie: blocks of 32 rows and 16 columns, two
+// halves of 8 columns each, the rows side by side. The writer's and the reader's
+// lane r both hold row r, so that a warp moves a kilobyte at a stretch (row by
+// row, 32 sectors each: the reading kernel took 540 us for 32768 x 4096).
+__device__ __forceinline__ float *kept_at(float *base, int64_t blocks, int64_t row, int64_t column) {
+    return base + ((row >> 5) * blocks + (column >> 4)) * 512 + (column & 8) * 32 + (row & 31) * 8;
 }
 
-// kWide kept values of a row as they lie in memory (rows start at 32 bytes and are padded to them).
-template <int kWide, typename T>
+// kWide kept values of a row.
+template <int kWide>
 struct KeptRow {
-    static constexpr int W = Pack<T>::kWidth;
-    uint4 raw[kWide / W];
-    __device__ __forceinline__ void load(const void *base, int64_t ld, int64_t row, int64_t column, bool live) {
-        const T *src = static_cast<const T *>(base) + row * ld + column;
-        if constexpr (kWide * sizeof(T) % 32 == 0) {  // whole sectors
+    uint4 raw[kWide / 4];
+    __device__ __forceinline__ void load(float *base, int64_t blocks, int64_t row, int64_t column, bool live) {
 #pragma unroll
-            for (int i = 0; i < kWide / W; i += 2) {
-                if (live && column + i * W < ld) {
-                    load_sector(src + i * W, raw[i], raw[i + 1]);
-                } else {
-                    raw[i] = raw[i + 1] = make_uint4(0, 0, 0, 0);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kWide / W; ++i) {
-                raw[i] = live && column + i * W < ld ? load_cached(src + i * W) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kWide / 4; i += 2) {
+            if (live) {
+                load_sector(kept_at(base, blocks, row, column + 4 * i), raw[i], raw[i + 1]);
+            } else {
+                raw[i] = raw[i + 1] = make_uint4(0, 0, 0, 0);
             }
         }
     }
-    __device__ __forceinline__ void values(float (&out)[kWide]) const {
+    static __device__ __forceinline__ void store(float *base, int64_t blocks, int64_t row, int64_t column, const float (&in)[kWide]) {
 #pragma unroll
-        for (int i = 0; i < kWide / W; ++i) {
-            float part[W];
-            unpack(raw[i], part, T());
+        for (int i = 0; i < kWide; i += 8) {
+            uint4 v[2];
 #pragma unroll
-            for (int e = 0; e < W; ++e) out[i * W + e] = part[e];
+            for (int k = 0; k < 2; ++k) {
+                v[k] = make_uint4(__float_as_uint(in[i + 4 * k]), __float_as_uint(in[i + 4 * k + 1]), __float_as_uint(in[i + 4 * k + 2]),
+                                  __float_as_uint(in[i + 4 * k + 3]));
+            }
+            store_sector(kept_at(base, blocks, row, column + i), v[0], v[1]);
+        }
+    }
+    __device__ __forceinline__ void times(const float (&in)[kWide], float (&out)[kWide]) const {
+#pragma unroll
+        for (int i = 0; i < kWide / 4; ++i) {
+            out[4 * i] = in[4 * i] * __uint_as_float(raw[i].x);
+            out[4 * i + 1] = in[4 * i + 1] * __uint_as_float(raw[i].y);
+            out[4 * i + 2] = in[4 * i + 2] * __uint_as_float(raw[i].z);
+            out[4 * i + 3] = in[4 * i + 3] * __uint_as_float(raw[i].w);
         }
     }
 };
 
-__device__ __forceinline__ float dp_of(float dh, float p, float q, float s) { return q * (dh * (s * fmaf(p, 1.0f - s, 1.0f))); }
-__device__ __forceinline__ float dq_of(float dh, float p, float s) { return p * (s * dh); }
+// kGate on kWide hidden units of one row.
+template <int kWide, typename T, typename Store>
+__device__ __forceinline__ void finish_gate(const Job &a, const Store &store, float (&p)[kWide], float (&q)[kWide]) {
+    if (a.a_kept == nullptr) {
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) q[j] *= p[j] * sigmoid_of<T>(p[j]);
+    } else {
+        float slope[kWide];
+#pragma unroll
+        for (int j = 0; j < kWide; ++j) {
+            const float s = sigmoid_of<T>(p[j]);
+            slope[j] = q[j] * (s * fmaf(p[j], 1.0f - s, 1.0f));
+            p[j] *= s;
+            q[j] *= p[j];
+        }
+        if (store.inside()) {
+            KeptRow<kWide>::store(a.a_kept, a.kept_blocks, store.own_row(), store.column, p);
+            KeptRow<kWide>::store(a.b_kept, a.kept_blocks, store.own_row(), store.column, slope);
+        }
+    }
+    store_parts<kWide, T>(store, a.first, q);
+}
 
 // kInner on kWide hidden units of one row of dh.
 template <int kWide, typename T, typename Store>
-__device__ __forceinline__ void finish_inner(const Job &a, const Store &store, const KeptRow<kWide, T> &kept_p, const KeptRow<kWide, T> &kept_q,
-                                             float (&dh)[kWide]) {
-    float p[kWide], q[kWide];
-    kept_p.values(p);
-    kept_q.values(q);
-#pragma unroll
-    for (int j = 0; j < kWide; ++j) {
-        const float s = sigmoid_of<T>(p[j]);
-        q[j] = dp_of(dh[j], p[j], q[j], s);
-        p[j] = dq_of(dh[j], p[j], s);
-    }
-    store_parts<kWide, T>(store, a.first, q);
-    store_parts<kWide, T>(store, a.second, p);
+__device__ __forceinline__ void finish_inner(const Job &j, const Store &store, const KeptRow<kWide> &a, const KeptRow<kWide> &b, const float (&dh)[kWide]) {
+    float out[kWide];
+    b.times(dh, out);
+    store_parts<kWide, T>(store, j.first, out);
+    a.times(dh, out);
+    store_parts<kWide, T>(store, j.second, out);
 }
 
 template <int kWide, typename T, typename Store>
@@ -764,17 +781,18 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
         TileStore store{staged + (warp - kLoaders - 1) * kStagedBytes, 0, 0, 0, 0, lane};
         float *const biases = reinterpret_cast<float *>(staged + kEpilogueWarps * kStagedBytes + (warp - kLoaders - 1) * kBiasBytes);
         bool first = true;
-        for (; more && ok; more = walk.next(args, job, tile)) {
+        // a warp that has given up still meets the others at every tile
+        for (; more; more = walk.next(args, job, tile)) {
             const Job &j = args.jobs[job];
             store.row0 = static_cast<int64_t>(tile.m * kCtas + rank) * kBM + quarter * 32;
             store.rows = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(32), j.m - store.row0)));
             const int64_t first_column = static_cast<int64_t>(tile.n) * kUnits;
-            KeptRow<16, T> kept_p, kept_q;  // kInner: of the group to come
+            KeptRow<16> kept_a, kept_b;  // kInner: of the group to come
             auto request = [&](int g) {
                 if constexpr (kEpilogue == kInner) {
                     if (j.splits > 1 || g >= kGroups) return;
-                    kept_p.load(j.p, j.ld_pq, store.row0 + lane, first_column + g * 16, lane < store.rows);
-                    kept_q.load(j.q, j.ld_pq, store.row0 + lane, first_column + g * 16, lane < store.rows);
+                    kept_a.load(j.a_kept, j.kept_blocks, store.row0 + lane, first_column + g * 16, lane < store.rows && first_column + g * 16 < j.n);
+                    kept_b.load(j.b_kept, j.kept_blocks, store.row0 + lane, first_column + g * 16, lane < store.rows && first_column + g * 16 < j.n);
                 }
             };
             // 16 columns of the warp's rows (kGate: of p and of q)
@@ -782,7 +800,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                 store.column = first_column + g * 16;
                 store.left = j.n - store.column;
                 if (store.left <= 0) return;
-                if (j.splits > 1) {
+                if (j.splits > 1) {  // parts of the sums are parked
                     float *base = j.partials + kSides * tile.split * j.m * j.ld_partial;
 #pragma unroll
                     for (int k = 0; k < kSides; ++k) store(base + k * j.m * j.ld_partial, j.ld_partial, v[k]);
@@ -791,15 +809,15 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                     add_staged<16>(biases + kUnits / 2 + g / 2 * 16, v[1]);
                     finish_gate<16, T>(j, store, v[0], v[1]);
                 } else if constexpr (kEpilogue == kInner) {
-                    const KeptRow<16, T> p = kept_p, q = kept_q;
+                    const KeptRow<16> a = kept_a, b = kept_b;
                     request(g + 2);
-                    finish_inner<16, T>(j, store, p, q, v[0]);
+                    finish_inner<16, T>(j, store, a, b, v[0]);
                 } else {
                     add_staged<16>(biases + g / 2 * 16, v[0]);
                     finish_out<16, T>(j, store, v[0]);
                 }
             };
-            if (first) pdl_wait();  // before p and q of the kernel before are read, and anything is written
+            if (first) pdl_wait();  // before anything of the kernel before is read, and anything written
             first = false;
             request(part);
             if constexpr (kEpilogue != kInner) {  // the biases of the warp's columns, while the tile is multiplied
@@ -826,7 +844,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                         for (int e = 0; e < 16; ++e) sum[i][k][e] = 0.0f;
                     }
                 }
-                for (int kb = tile.k_begin; kb < tile.k_end; kb += kPass) {
+                for (int kb = tile.k_begin; kb < tile.k_end && ok; kb += kPass) {
                     ok = wait<kCtas == 2>(&acc_full[acc], acc_phase, abort, args.status);
                     if (!ok) break;
                     tc_fence_after();
@@ -847,16 +865,16 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
                     }
                     release();
                 }
-                if (!ok) break;
 #pragma unroll
-                for (int i = 0; i < kMine; ++i) finish(part + 2 * i, sum[i]);
+                for (int i = 0; i < kMine; ++i) {
+                    if (ok) finish(part + 2 * i, sum[i]);
+                }
             } else {
-                ok = wait<kCtas == 2>(&acc_full[acc], acc_phase, abort, args.status);
-                if (!ok) break;
+                ok = ok && wait<kCtas == 2>(&acc_full[acc], acc_phase, abort, args.status);
                 tc_fence_after();
                 const uint32_t from = tmem + lanes + static_cast<uint32_t>(acc * kAccumulator);
 #pragma unroll 1
-                for (int g = part; g < kGroups; g += 2) {
+                for (int g = part; g < kGroups && ok; g += 2) {
                     uint32_t raw[kSides][16];
                     float v[kSides][16];
 #pragma unroll
@@ -886,7 +904,9 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
     }
 }
 
-// The splits' accumulators added in order, then the epilogue: 8 columns a thread. grid.y: the job.
+// The splits' accumulators added in order, then the epilogue: 8 columns a
+// thread. grid.y: the job. (Joined by the last CTA of a tile to come, through a
+// counter, the same took 3 to 6 times as long: one CTA reads what here the whole GPU does.)
 template <typename T, int kEpilogue>
 __global__ __launch_bounds__(256) void join_kernel(const __grid_constant__ GemmArgs args) {
     const Job &j = args.jobs[blockIdx.y];
@@ -897,10 +917,10 @@ __global__ __launch_bounds__(256) void join_kernel(const __grid_constant__ GemmA
     constexpr int kSides = kEpilogue == kGate ? 2 : 1;
     const int64_t side = j.m * j.ld_partial;
     const float *src = j.partials + row * j.ld_partial + column;
-    KeptRow<8, T> kept_p, kept_q;
+    KeptRow<8> kept_a, kept_b;
     if constexpr (kEpilogue == kInner) {
-        kept_p.load(j.p, j.ld_pq, row, column, true);
-        kept_q.load(j.q, j.ld_pq, row, column, true);
+        kept_a.load(j.a_kept, j.kept_blocks, row, column, true);
+        kept_b.load(j.b_kept, j.kept_blocks, row, column, true);
     }
     float sum[kSides][8] = {};
 #pragma unroll 4
@@ -919,7 +939,7 @@ __global__ __launch_bounds__(256) void join_kernel(const __grid_constant__ GemmA
         add_bias<8, T>(j.bias1, column, store.left, sum[1]);
         finish_gate<8, T>(j, store, sum[0], sum[1]);
     } else if constexpr (kEpilogue == kInner) {
-        finish_inner<8, T>(j, store, kept_p, kept_q, sum[0]);
+        finish_inner<8, T>(j, store, kept_a, kept_b, sum[0]);
     } else {
         add_bias<8, T>(j.bias0, column, store.left, sum[0]);
         finish_out<8, T>(j, store, sum[0]);
@@ -1112,17 +1132,22 @@ size_t partial_bytes(const Cut &cut, int i, const Product &p, bool gate) {
 }
 
 // What the products of one launch, cut alike, need for their partial sums.
-size_t partial_bytes(const Product *const *products, int count, bool gate) {
-    const Cut cut = cut_of(products, count, gate, sm_count());
+size_t partial_bytes(const Cut &cut, const Product *const *products, int count, bool gate) {
     size_t bytes = 0;
     for (int i = 0; i < count; ++i) bytes += partial_bytes(cut, i, *products[i], gate);
     return bytes;
 }
-
 template <typename T, int kEpilogue, int kTileN, int kCtas>
 int launch_shape(GemmArgs &args, bool dependent, cudaStream_t stream) {
     auto kernel = gemm_kernel<T, kEpilogue, kTileN, kCtas>;
-    KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes)));
+    // once a device: the most that any launch takes
+    static std::atomic<bool> allowed[64];
+    int device = 0;
+    KOEMI_CUDA_TRY(cudaGetDevice(&device));
+    if (device >= 64 || !allowed[device].load(std::memory_order_acquire)) {
+        KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes)));
+        if (device < 64) allowed[device].store(true, std::memory_order_release);
+    }
     args.places = std::min(args.first_tiles + args.second_tiles, sm_count() / kCtas);
     const int first = args.jobs[0].k_per_split, second = args.jobs[args.job_count - 1].k_per_split;
     args.ahead = args.first_tiles % args.places;
@@ -1149,16 +1174,19 @@ Divisor divisor(int d) {
 // ended, because no launch that comes first in a call is a dependent one. The cut is that of all of them, wanted or not, so that the
 // workspace does not depend on which are.
 template <typename T, int kEpilogue>
-int multiply(const Product *const *products, const Job *jobs, int count, char *partials, bool dependent, cudaStream_t stream) {
+int multiply(const Product *const *products, const Job *jobs, int count, const Cut &cut, char *partials, bool dependent,
+              cudaStream_t stream) {
     constexpr bool gate = kEpilogue == kGate;
     const bool half = std::is_same<typename Operand16<T>::type, __half>::value;
-    const Cut cut = cut_of(products, count, gate, sm_count());
     GemmArgs args{};
     args.status = device_status_word();
     int64_t tiles[2] = {0, 0}, most = 0;
     for (int i = 0; i < count; ++i) {
         const Product &p = *products[i];
-        if (kEpilogue == kOut && jobs[i].out == nullptr) continue;  // not wanted: the others are cut as beside it
+        if (kEpilogue == kOut && jobs[i].out == nullptr) {  // not wanted: the others are cut as beside it
+            partials += partial_bytes(cut, i, p, gate);
+            continue;
+        }
         const int at = args.job_count++;
         Job &j = args.jobs[at] = jobs[i];
         j.total_k = total_k_of(p, gate);
@@ -1237,21 +1265,22 @@ struct Problem {
 
 int parts_of(int dtype) { return dtype == KOEMI_F32 ? 3 : 1; }
 
-// What the backward needs of the forward: h (in parts), p and q.
+// What the backward needs of the forward: h (in parts), a and b.
 struct Kept {
     Parts h;
-    void *p, *q;
+    float *a, *b;
     int64_t ld;
 };
 
-Kept kept_of(Pool &pool, int64_t rows, int64_t hidden, int dtype, bool with_pq) {
+Kept kept_of(Pool &pool, int64_t rows, int64_t hidden, int dtype, bool with_slopes) {
     Kept kept{};
     kept.ld = round16(hidden);
     const size_t count = static_cast<size_t>(rows) * kept.ld;
     kept.h = Parts{pool.take(count * 2 * parts_of(dtype)), kept.ld, rows * kept.ld};
-    if (with_pq) {
-        kept.p = pool.take(count * dtype_size(dtype));
-        kept.q = pool.take(count * dtype_size(dtype));
+    if (with_slopes) {
+        const size_t blocks = static_cast<size_t>(ceil_div(rows, 32)) * kept.ld / 16;
+        kept.a = static_cast<float *>(pool.take(blocks * 512 * sizeof(float)));
+        kept.b = static_cast<float *>(pool.take(blocks * 512 * sizeof(float)));
     }
     return kept;
 }
@@ -1287,6 +1316,7 @@ struct ForwardPlan {
     PackArgs jobs;
     int job_count;
     Product gate, out;
+    Cut gate_cut, out_cut;
     char *partials;
 };
 
@@ -1302,14 +1332,22 @@ void plan_forward(ForwardPlan &plan, const Problem &q, Pool &pool, char *kept_ba
     plan.gate = Product{{plan.x, {}}, {plan.wg, plan.wv}, 1, false, false, q.rows, q.hidden};
     plan.out = Product{{matrix_of(plan.kept.h, q.rows, q.hidden, q.dtype), {}}, {plan.wo, {}}, 1, false, false, q.rows, q.out_width};
     const Product *gate = &plan.gate, *out = &plan.out;
-    plan.partials = static_cast<char *>(pool.take(std::max(partial_bytes(&gate, 1, true), partial_bytes(&out, 1, false))));
+    const int sms = sm_count();
+    plan.gate_cut = cut_of(&gate, 1, true, sms);
+    plan.out_cut = cut_of(&out, 1, false, sms);
+    plan.partials = static_cast<char *>(pool.take(std::max(partial_bytes(plan.gate_cut, &gate, 1, true), partial_bytes(plan.out_cut, &out, 1, false))));
+}
+
+int too_small(size_t need) {
+    return fail(KOEMI_ERR_WORKSPACE, "the feed-forward block needs %zu workspace bytes from a multiple of 256 here", need);
 }
 
 template <typename T>
-int forward(const Problem &q, void *y, void *kept, void *workspace, cudaStream_t stream) {
+int forward(const Problem &q, void *y, void *kept, void *workspace, size_t room, cudaStream_t stream) {
     ForwardPlan plan{};
     Pool pool{static_cast<char *>(workspace)};
     plan_forward(plan, q, pool, static_cast<char *>(kept), kept != nullptr);
+    if (pool.used > room) return too_small(pool.used);
     int rc = pack_all<T>(plan.jobs, plan.job_count, stream);
     if (rc != KOEMI_OK) return rc;
     const Product *first = &plan.gate, *second = &plan.out;
@@ -1317,16 +1355,16 @@ int forward(const Problem &q, void *y, void *kept, void *workspace, cudaStream_t
     gate.bias0 = q.bg;
     gate.bias1 = q.bv;
     gate.first = plan.kept.h;
-    gate.p = plan.kept.p;
-    gate.q = plan.kept.q;
-    gate.ld_pq = plan.kept.ld;
-    rc = multiply<T, kGate>(&first, &gate, 1, plan.partials, false, stream);
+    gate.a_kept = plan.kept.a;
+    gate.b_kept = plan.kept.b;
+    gate.kept_blocks = plan.kept.ld / 16;
+    rc = multiply<T, kGate>(&first, &gate, 1, plan.gate_cut, plan.partials, false, stream);
     if (rc != KOEMI_OK) return rc;
     Job out{};
     out.bias0 = q.bo;
     out.out = y;
     out.ld_out = q.out_width;
-    return multiply<T, kOut>(&second, &out, 1, plan.partials, true, stream);
+    return multiply<T, kOut>(&second, &out, 1, plan.out_cut, plan.partials, true, stream);
 }
 
 struct Gradients {
@@ -1344,6 +1382,7 @@ struct BackwardPlan {
     const Product *last[kMaxJobs];  // the products behind inner, the longer first, and where they go
     void *results[kMaxJobs];
     SumArgs sums;
+    Cut inner_cut, last_cut;
     char *partials;
 };
 
@@ -1375,9 +1414,10 @@ void plan_backward(BackwardPlan &plan, const Problem &q, const Gradients &g, Poo
         plan.results[i] = results[at];
     }
     const Product *inner = &plan.inner;
-    const size_t most = std::max(partial_bytes(&inner, 1, false), partial_bytes(plan.last, kMaxJobs, false));
-    plan.partials = static_cast<char *>(pool.take(most));
     const int sms = sm_count();
+    plan.inner_cut = cut_of(&inner, 1, false, sms);
+    plan.last_cut = cut_of(plan.last, kMaxJobs, false, sms);
+    plan.partials = static_cast<char *>(pool.take(std::max(partial_bytes(plan.inner_cut, &inner, 1, false), partial_bytes(plan.last_cut, plan.last, kMaxJobs, false))));
     const int64_t columns = std::max(q.hidden, q.out_width);
     plan.sums.rows = q.rows;
     plan.sums.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(q.rows, 64), 16 * sms / ceil_div(columns, 32))));
@@ -1391,10 +1431,11 @@ void plan_backward(BackwardPlan &plan, const Problem &q, const Gradients &g, Poo
 }
 
 template <typename T>
-int backward(const Problem &q, const Gradients &g, const void *kept, void *workspace, cudaStream_t stream) {
+int backward(const Problem &q, const Gradients &g, const void *kept, void *workspace, size_t room, cudaStream_t stream) {
     BackwardPlan plan{};
     Pool pool{static_cast<char *>(workspace)};
     plan_backward(plan, q, g, pool, static_cast<char *>(const_cast<void *>(kept)));
+    if (pool.used > room) return too_small(pool.used);
     int rc = pack_all<T>(plan.jobs, plan.job_count, stream);
     if (rc != KOEMI_OK) return rc;
     bool dependent = false;
@@ -1403,10 +1444,10 @@ int backward(const Problem &q, const Gradients &g, const void *kept, void *works
         Job inner{};
         inner.first = plan.dp;
         inner.second = plan.dq;
-        inner.p = plan.kept.p;
-        inner.q = plan.kept.q;
-        inner.ld_pq = plan.kept.ld;
-        rc = multiply<T, kInner>(&product, &inner, 1, plan.partials, false, stream);
+        inner.a_kept = plan.kept.a;
+        inner.b_kept = plan.kept.b;
+        inner.kept_blocks = plan.kept.ld / 16;
+        rc = multiply<T, kInner>(&product, &inner, 1, plan.inner_cut, plan.partials, false, stream);
         dependent = true;
     }
     if (rc == KOEMI_OK) {
@@ -1415,7 +1456,7 @@ int backward(const Problem &q, const Gradients &g, const void *kept, void *works
             jobs[i].out = plan.results[i];
             jobs[i].ld_out = plan.last[i]->n;
         }
-        rc = multiply<T, kOut>(plan.last, jobs, kMaxJobs, plan.partials, dependent, stream);
+        rc = multiply<T, kOut>(plan.last, jobs, kMaxJobs, plan.last_cut, plan.partials, dependent, stream);
     }
     if (rc != KOEMI_OK) return rc;
     if (g.dbg != nullptr || g.dbv != nullptr || g.dbo != nullptr) {
@@ -1479,14 +1520,11 @@ extern "C" int koemi_dense_gated_feed_forward_forward(const void *values, int64_
     if (kept != nullptr && (kept_bytes < koemi_dense_gated_feed_forward_kept(rows, hidden_width, dtype) || !aligned(kept, 256))) {
         return fail(KOEMI_ERR_WORKSPACE, "kept must hold %zu bytes from a multiple of 256", koemi_dense_gated_feed_forward_kept(rows, hidden_width, dtype));
     }
-    const size_t need = koemi_dense_gated_feed_forward_workspace(rows, width, hidden_width, out_width, dtype, 0);
-    if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)) {
-        return fail(KOEMI_ERR_WORKSPACE, "the feed-forward block needs %zu workspace bytes from a multiple of 256", need);
-    }
+    if (workspace == nullptr || !aligned(workspace, 256)) return fail(KOEMI_ERR_WORKSPACE, "the workspace must start at a multiple of 256");
     const Problem q{values, gate_weight, value_weight, output_weight, gate_bias, value_bias, output_bias, rows, width, hidden_width, out_width, value_stride, dtype};
-    if (dtype == KOEMI_F32) return forward<float>(q, out, kept, workspace, as_stream(stream));
-    if (dtype == KOEMI_F16) return forward<__half>(q, out, kept, workspace, as_stream(stream));
-    return forward<__nv_bfloat16>(q, out, kept, workspace, as_stream(stream));
+    if (dtype == KOEMI_F32) return forward<float>(q, out, kept, workspace, workspace_bytes, as_stream(stream));
+    if (dtype == KOEMI_F16) return forward<__half>(q, out, kept, workspace, workspace_bytes, as_stream(stream));
+    return forward<__nv_bfloat16>(q, out, kept, workspace, workspace_bytes, as_stream(stream));
 }
 
 extern "C" int koemi_dense_gated_feed_forward_backward(const void *values, int64_t value_stride, const void *gate_weight,
@@ -1516,13 +1554,10 @@ extern "C" int koemi_dense_gated_feed_forward_backward(const void *values, int64
     if (kept_bytes < koemi_dense_gated_feed_forward_kept(rows, hidden_width, dtype) || !aligned(kept, 256)) {
         return fail(KOEMI_ERR_WORKSPACE, "kept must hold %zu bytes from a multiple of 256", koemi_dense_gated_feed_forward_kept(rows, hidden_width, dtype));
     }
-    const size_t need = koemi_dense_gated_feed_forward_workspace(rows, width, hidden_width, out_width, dtype, 1);
-    if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256)) {
-        return fail(KOEMI_ERR_WORKSPACE, "the feed-forward block's backward needs %zu workspace bytes from a multiple of 256", need);
-    }
+    if (workspace == nullptr || !aligned(workspace, 256)) return fail(KOEMI_ERR_WORKSPACE, "the workspace must start at a multiple of 256");
     const Problem q{values, gate_weight, value_weight, output_weight, nullptr, nullptr, nullptr, rows, width, hidden_width, out_width, value_stride, dtype};
     const Gradients g{grad_out, grad_values, grad_gate_weight, grad_value_weight, grad_output_weight, grad_gate_bias, grad_value_bias, grad_output_bias};
-    if (dtype == KOEMI_F32) return backward<float>(q, g, kept, workspace, as_stream(stream));
-    if (dtype == KOEMI_F16) return backward<__half>(q, g, kept, workspace, as_stream(stream));
-    return backward<__nv_bfloat16>(q, g, kept, workspace, as_stream(stream));
+    if (dtype == KOEMI_F32) return backward<float>(q, g, kept, workspace, workspace_bytes, as_stream(stream));
+    if (dtype == KOEMI_F16) return backward<__half>(q, g, kept, workspace, workspace_bytes, as_stream(stream));
+    return backward<__nv_bfloat16>(q, g, kept, workspace, workspace_bytes, as_stream(stream));
 }

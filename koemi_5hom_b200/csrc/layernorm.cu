@@ -439,8 +439,19 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
     if (partials == nullptr) return;
     float *mine = partials + static_cast<int64_t>(blockIdx.x) * 2 * a.width;
     float *const to = kWarp ? pool : mine;
-    for (int turn = 0; turn < teams; ++turn) {  // kWarp: the CTA's teams add their parts in order
-        if (!kWarp || turn == static_cast<int>(threadIdx.x / team)) {
+    if (kWarp) {  // the teams of a warp first
+        for (int offset = team; offset < 32; offset <<= 1) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                dw[i].x += __shfl_xor_sync(0xffffffffu, dw[i].x, offset);
+                dw[i].y += __shfl_xor_sync(0xffffffffu, dw[i].y, offset);
+                db[i].x += __shfl_xor_sync(0xffffffffu, db[i].x, offset);
+                db[i].y += __shfl_xor_sync(0xffffffffu, db[i].y, offset);
+            }
+        }
+    }
+    for (int turn = 0; turn < (kWarp ? warps : 1); ++turn) {  // then the CTA's warps, in order
+        if (!kWarp || (turn == static_cast<int>(threadIdx.x / 32) && (threadIdx.x & 31) < team)) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int c = (k * team + t) * W;

@@ -139,8 +139,8 @@ def test_entries_refuse_bad_arguments_before_touching_the_device():
         return lib.koemi_core_dropout(values, None, one, count, dropped, 1, 2, 3, None, dtype, None)
 
     kept = lib.koemi_dense_gated_feed_forward_kept(10, 20, _native.BF16)
-    assert kept == 3 * 768 and lib.koemi_dense_gated_feed_forward_kept(-1, 20, _native.BF16) == 0  # 10 x 32 values thrice
-    assert lib.koemi_dense_gated_feed_forward_kept(10, 20, _native.F32) == 2048 + 2 * 1280  # three bf16 parts, two fp32 matrices
+    assert kept == 768 + 2 * 4096 and lib.koemi_dense_gated_feed_forward_kept(-1, 20, _native.BF16) == 0  # 10 x 32 values, twice 32 x 32 in fp32
+    assert lib.koemi_dense_gated_feed_forward_kept(10, 20, _native.F32) == 2048 + 2 * 4096  # three bf16 parts
     rooms = [lib.koemi_dense_gated_feed_forward_workspace(10, 16, 20, 8, _native.BF16, backward) for backward in (0, 1)]
     assert min(rooms) > 0 and lib.koemi_dense_gated_feed_forward_workspace(10, 16, 20, 8, 99, 0) == 0
     page = ctypes.c_void_p(256)
@@ -153,7 +153,7 @@ def test_entries_refuse_bad_arguments_before_touching_the_device():
     assert block(rows=1 << 31) == invalid and block(hidden=1 << 25) == invalid and block(stride=15) == invalid
     assert block(dtype=_native.I32) == invalid and block(values=None) == invalid and block(rows=0) == 0
     assert block(keep_bytes=kept - 1) == workspace and block(keep=one) == workspace
-    assert block(room=rooms[0] - 1) == workspace and block(ws=None) == workspace and block(ws=one) == workspace
+    assert block(room=8) == workspace and block(ws=None) == workspace and block(ws=one) == workspace
 
     def block_backward(rows=10, stride=16, dtype=_native.BF16, keep=page, grad=page, room=rooms[1]):
         return lib.koemi_dense_gated_feed_forward_backward(page, stride, page, page, page, keep, kept, grad, page, page, page, page, page, page,
@@ -161,7 +161,7 @@ def test_entries_refuse_bad_arguments_before_touching_the_device():
 
     assert block_backward(rows=-1) == invalid and block_backward(stride=3) == invalid and block_backward(dtype=99) == invalid
     assert block_backward(keep=None) == invalid and block_backward(grad=None) == invalid and block_backward(keep=one) == workspace
-    assert block_backward(room=rooms[1] - 1) == workspace
+    assert block_backward(room=8) == workspace
 
     assert drop(count=-1) == invalid and drop(dropped=-1) == invalid and drop(dropped=65537) == invalid
     assert drop(dtype=_native.BOOL) == invalid and drop(values=None) == invalid and drop(count=0) == 0
