@@ -408,14 +408,31 @@ __device__ __forceinline__ void store_parts(const Store &store, const Parts &to,
     }
 }
 
-// 16-bit results leave room for the fast exponential and quotient (relative error about 1e-6).
+// 16-bit results leave room for the approximate exponential and reciprocal
+// (relative error about 1e-6; exp(-p) of 2^128 and more gives 0).
 template <typename T>
 __device__ __forceinline__ float sigmoid_of(float p) {
     if constexpr (sizeof(T) == 4) {
         return 1.0f / (1.0f + expf(-p));
     } else {
-        return __fdividef(1.0f, 1.0f + __expf(-p));
+        float e, s;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(p * -1.4426950408889634f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + e));
+        return s;
     }
+}
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)),
+        "l"(reinterpret_cast<uint64_t &>(c)));
+    return r;
 }
 
 template <int kWide, typename T>
@@ -490,11 +507,14 @@ __device__ __forceinline__ void finish_gate(const Job &a, const Store &store, fl
     } else {
         float slope[kWide];
 #pragma unroll
-        for (int j = 0; j < kWide; ++j) {
-            const float s = sigmoid_of<T>(p[j]);
-            slope[j] = q[j] * (s * fmaf(p[j], 1.0f - s, 1.0f));
-            p[j] *= s;
-            q[j] *= p[j];
+        for (int j = 0; j < kWide; j += 2) {
+            const float2 s = make_float2(sigmoid_of<T>(p[j]), sigmoid_of<T>(p[j + 1])), x = make_float2(p[j], p[j + 1]), y = make_float2(q[j], q[j + 1]);
+            const float2 one = make_float2(1.0f, 1.0f);
+            const float2 rest = fma2(s, make_float2(-1.0f, -1.0f), one);  // 1 - s
+            const float2 b = mul2(y, mul2(s, fma2(x, rest, one))), a = mul2(x, s), h = mul2(y, a);
+            slope[j] = b.x, slope[j + 1] = b.y;
+            p[j] = a.x, p[j + 1] = a.y;
+            q[j] = h.x, q[j + 1] = h.y;
         }
         if (store.inside()) {
             KeptRow<kWide>::store(a.a_kept, a.kept_blocks, store.own_row(), store.column, p);
@@ -805,15 +825,15 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
 #pragma unroll
                     for (int k = 0; k < kSides; ++k) store(base + k * j.m * j.ld_partial, j.ld_partial, v[k]);
                 } else if constexpr (kEpilogue == kGate) {
-                    add_staged<16>(biases + g / 2 * 16, v[0]);
-                    add_staged<16>(biases + kUnits / 2 + g / 2 * 16, v[1]);
+                    if (j.bias0 != nullptr) add_staged<16>(biases + g / 2 * 16, v[0]);
+                    if (j.bias1 != nullptr) add_staged<16>(biases + kUnits / 2 + g / 2 * 16, v[1]);
                     finish_gate<16, T>(j, store, v[0], v[1]);
                 } else if constexpr (kEpilogue == kInner) {
                     const KeptRow<16> a = kept_a, b = kept_b;
                     request(g + 2);
                     finish_inner<16, T>(j, store, a, b, v[0]);
                 } else {
-                    add_staged<16>(biases + g / 2 * 16, v[0]);
+                    if (j.bias0 != nullptr) add_staged<16>(biases + g / 2 * 16, v[0]);
                     finish_out<16, T>(j, store, v[0]);
                 }
             };
@@ -821,7 +841,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
             first = false;
             request(part);
             if constexpr (kEpilogue != kInner) {  // the biases of the warp's columns, while the tile is multiplied
-                if (j.splits == 1) {
+                if (j.splits == 1 && (j.bias0 != nullptr || j.bias1 != nullptr)) {
                     __syncwarp();
 #pragma unroll 1
                     for (int i = lane; i < kSides * kUnits / 2; i += 32) {
