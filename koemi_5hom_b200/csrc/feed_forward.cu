@@ -305,7 +305,7 @@ __device__ __forceinline__ void load_values(const T *src, int64_t left, float (&
 template <int kWide, typename T>
 __device__ __forceinline__ void store_values(T *dst, int64_t left, const float (&in)[kWide]) {
     constexpr int W = Pack<T>::kWidth;
-    if (left >= kWide && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+    if (kWide % W == 0 && left >= kWide && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
 #pragma unroll
         for (int q = 0; q < kWide / W; ++q) {
             float part[W];
@@ -966,6 +966,168 @@ __global__ __launch_bounds__(256) void join_kernel(const __grid_constant__ GemmA
     }
 }
 
+// ------------------------------------------------------------------ few rows
+//
+// A few rows (tokens at decode) are bound by the weights' bytes: a warp takes the
+// dot products of kFewUnits units with every row on the FMA units, straight from
+// the weights as they lie (fp32 too: no parts), 16 bytes a lane at a time. The
+// tensor cores' tiles are 128 rows high and their sums parted along K. Measured,
+// here and there, 2048 -> 4096 -> 2048: 1 row 19 and 25 us in bf16, 22 and 99 in
+// fp32; 4 rows 27 and 26 (1024 -> 2048 -> 1024: 13 and 17); 8 rows 49 and 26, in
+// fp32 51 and 99; rows that no 16-byte load fits (3229 -> 2690 -> 3229 bf16) 2
+// rows 39 and 50, 4 rows 99 and 50. Hence the limit:
+int64_t few_limit(int64_t width, int64_t hidden, int dtype) {
+    return dtype == KOEMI_F32 ? 8 : width % 8 == 0 && hidden % 8 == 0 ? 4 : 2;
+}
+constexpr int kFewUnits = 2;
+
+struct FewArgs {
+    const void *x, *w0, *w1;   // kGate: the gate's and the value's weights; kOut: w0
+    const void *bias0, *bias1;
+    int64_t ld_x, width, units;
+    int rows;
+    void *out;                 // kOut: [rows, units]; kGate: h as the second product reads it
+    int64_t ld_out;
+    Parts parts;               // kGate: h for the backward (base NULL: not wanted)
+    float *a_kept, *b_kept;
+    int64_t kept_blocks;
+};
+
+// 16 bytes of a row of weights, or one value, as they lie.
+template <typename T, bool kVec>
+struct Piece {
+    uint4 raw;
+    T one;
+    __device__ __forceinline__ void load(const T *p, bool live) {
+        if constexpr (kVec) {
+            raw = live ? load_stream(p) : make_uint4(0, 0, 0, 0);
+        } else {
+            one = live ? __ldg(p) : from_acc<T>(0.0f);
+        }
+    }
+    template <int W>
+    __device__ __forceinline__ void values(float (&out)[W]) const {
+        if constexpr (kVec) {
+            unpack(raw, out, T());
+        } else {
+            out[0] = to_acc(one);
+        }
+    }
+};
+
+template <typename T, int kEpilogue, int R, bool kVec>
+__global__ __launch_bounds__(256) void few_rows_kernel(const __grid_constant__ FewArgs args) {
+    constexpr int W = kVec ? Pack<T>::kWidth : 1, kSides = kEpilogue == kGate ? 2 : 1, N = kFewUnits * kSides;
+    constexpr int kAsked = (kVec ? 16 : 32) / N;  // steps of 32 lanes whose weights are asked for together
+    const int lane = threadIdx.x & 31;
+    const int64_t unit0 = (static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32) * kFewUnits;
+    if (unit0 >= args.units) {
+        pdl_wait();
+        return;
+    }
+    pdl_trigger();
+    const T *w[N];
+#pragma unroll
+    for (int u = 0; u < kFewUnits; ++u) {
+        const int64_t unit = min(unit0 + u, args.units - 1);  // a unit behind the last is the last once more, and not stored
+#pragma unroll
+        for (int k = 0; k < kSides; ++k) w[u * kSides + k] = static_cast<const T *>(k == 0 ? args.w0 : args.w1) + unit * args.width;
+    }
+    const T *x = static_cast<const T *>(args.x);
+    float sum[N][R];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) sum[n][r] = 0.0f;
+    }
+    bool waited = false;
+    for (int64_t base = 0; base < args.width; base += kAsked * 32 * W) {
+        Piece<T, kVec> pieces[kAsked][N];
+#pragma unroll
+        for (int i = 0; i < kAsked; ++i) {
+            const int64_t c = base + (i * 32 + lane) * W;
+#pragma unroll
+            for (int n = 0; n < N; ++n) pieces[i][n].load(w[n] + c, c < args.width);
+        }
+        if (!waited) {  // the first weights are under way while the kernel before ends
+            pdl_wait();
+            waited = true;
+        }
+#pragma unroll
+        for (int i = 0; i < kAsked; ++i) {
+            const int64_t c = base + (i * 32 + lane) * W;
+            if (c >= args.width) continue;
+            float wv[N][W];
+#pragma unroll
+            for (int n = 0; n < N; ++n) pieces[i][n].values(wv[n]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                // a row behind the last is the last once more; not through the read-only path: the kernel before may have written it
+                const T *from = x + min(r, args.rows - 1) * args.ld_x + c;
+                float xv[W];
+                if constexpr (kVec) {
+                    unpack(*reinterpret_cast<const uint4 *>(from), xv, T());
+                } else {
+                    xv[0] = to_acc(*from);
+                }
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) sum[n][r] = fmaf(wv[n][e], xv[e], sum[n][r]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) sum[n][r] = warp_sum(sum[n][r]);
+    }
+    // lane r finishes row r
+#pragma unroll
+    for (int u = 0; u < kFewUnits; ++u) {
+        const int64_t unit = unit0 + u;
+        if (unit >= args.units || lane >= args.rows) continue;
+        float v[kSides];
+#pragma unroll
+        for (int k = 0; k < kSides; ++k) {
+            v[k] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < R; ++r) v[k] = lane == r ? sum[u * kSides + k][r] : v[k];
+            const T *bias = static_cast<const T *>(k == 0 ? args.bias0 : args.bias1);
+            if (bias != nullptr) v[k] += to_acc(bias[unit]);
+        }
+        T *out = static_cast<T *>(args.out) + lane * args.ld_out + unit;
+        if constexpr (kEpilogue == kGate) {
+            const float s = sigmoid_of<T>(v[0]), a = v[0] * s;
+            if (args.parts.base != nullptr) {
+                *(kept_at(args.a_kept, args.kept_blocks, lane, unit & ~7) + (unit & 7)) = a;
+                *(kept_at(args.b_kept, args.kept_blocks, lane, unit & ~7) + (unit & 7)) = v[1] * (s * fmaf(v[0], 1.0f - s, 1.0f));
+                const float h[1] = {a * v[1]};
+                store_parts<1, T>(DirectStore{lane, unit, 1, true}, args.parts, h);
+            }
+            *out = from_acc<T>(a * v[1]);
+        } else {
+            *out = from_acc<T>(v[0]);
+        }
+    }
+}
+
+template <typename T, int kEpilogue>
+int few_rows(const FewArgs &args, bool dependent, cudaStream_t stream) {
+    constexpr int W = Pack<T>::kWidth;
+    const bool vector = args.width % W == 0 && args.ld_x % W == 0 && aligned(args.x, 16) && aligned(args.w0, 16) && aligned(args.w1, 16);
+    auto kernel = vector ? few_rows_kernel<T, kEpilogue, 1, true> : few_rows_kernel<T, kEpilogue, 1, false>;
+    if (args.rows > 1) kernel = vector ? few_rows_kernel<T, kEpilogue, 2, true> : few_rows_kernel<T, kEpilogue, 2, false>;
+    if (args.rows > 2) kernel = vector ? few_rows_kernel<T, kEpilogue, 4, true> : few_rows_kernel<T, kEpilogue, 4, false>;
+    if constexpr (sizeof(T) == 4) {
+        if (args.rows > 4) kernel = vector ? few_rows_kernel<T, kEpilogue, 8, true> : few_rows_kernel<T, kEpilogue, 8, false>;
+    }
+    const int64_t blocks = ceil_div(args.units, 8 * kFewUnits);
+    KOEMI_CUDA_TRY(launch_programmatic(dependent, kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, dim3(1, 1, 1), args));
+    return KOEMI_OK;
+}
+
 // ------------------------------------------------------------ packed operands
 
 struct PackJob {
@@ -1358,12 +1520,31 @@ void plan_forward(ForwardPlan &plan, const Problem &q, Pool &pool, char *kept_ba
     plan.partials = static_cast<char *>(pool.take(std::max(partial_bytes(plan.gate_cut, &gate, 1, true), partial_bytes(plan.out_cut, &out, 1, false))));
 }
 
+// h of few rows, as the second product reads it.
+size_t few_bytes(int64_t rows, int64_t hidden, int dtype) { return static_cast<size_t>(rows) * round16(hidden) * dtype_size(dtype); }
+
 int too_small(size_t need) {
     return fail(KOEMI_ERR_WORKSPACE, "the feed-forward block needs %zu workspace bytes from a multiple of 256 here", need);
 }
 
 template <typename T>
+int forward_few(const Problem &q, void *y, void *kept_base, void *workspace, size_t room, cudaStream_t stream) {
+    Pool pool{static_cast<char *>(workspace)}, kept_pool{static_cast<char *>(kept_base)};
+    void *h = pool.take(few_bytes(q.rows, q.hidden, q.dtype));
+    if (pool.used > room) return too_small(pool.used);
+    const Kept kept = kept_of(kept_pool, q.rows, q.hidden, q.dtype, true);
+    const int rows = static_cast<int>(q.rows);
+    FewArgs gate{q.x, q.wg, q.wv, q.bg, q.bv, q.ld_x, q.width, q.hidden, rows, h, round16(q.hidden), kept.h, kept.a, kept.b, kept.ld / 16};
+    if (kept_base == nullptr) gate.parts.base = nullptr;
+    const int rc = few_rows<T, kGate>(gate, false, stream);
+    if (rc != KOEMI_OK) return rc;
+    const FewArgs out{h, q.wo, nullptr, q.bo, nullptr, round16(q.hidden), q.hidden, q.out_width, rows, y, q.out_width, Parts{}, nullptr, nullptr, 0};
+    return few_rows<T, kOut>(out, true, stream);
+}
+
+template <typename T>
 int forward(const Problem &q, void *y, void *kept, void *workspace, size_t room, cudaStream_t stream) {
+    if (q.rows <= few_limit(q.width, q.hidden, q.dtype)) return forward_few<T>(q, y, kept, workspace, room, stream);
     ForwardPlan plan{};
     Pool pool{static_cast<char *>(workspace)};
     plan_forward(plan, q, pool, static_cast<char *>(kept), kept != nullptr);
@@ -1516,6 +1697,8 @@ extern "C" size_t koemi_dense_gated_feed_forward_workspace(int64_t rows, int64_t
     if (backward) {
         BackwardPlan plan{};
         plan_backward(plan, q, Gradients{}, pool, nullptr);
+    } else if (rows <= few_limit(width, hidden_width, dtype)) {
+        pool.take(few_bytes(rows, hidden_width, dtype));
     } else {
         ForwardPlan plan{};
         plan_forward(plan, q, pool, nullptr, false);

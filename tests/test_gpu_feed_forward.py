@@ -22,7 +22,8 @@ DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 NAMES = ("y", "dx", "dwg", "dwv", "dwo", "dbg", "dbv", "dbo")
 
 # rows, width, hidden, out
-SHAPES = [(1, 1, 1, 1), (1, 8, 8, 8), (2, 15, 30, 7), (7, 64, 64, 64), (3, 65, 127, 33), (127, 200, 129, 72), (128, 128, 256, 128),
+SHAPES = [(1, 1, 1, 1), (1, 8, 8, 8), (2, 15, 30, 7), (7, 64, 64, 64), (3, 65, 127, 33), (4, 512, 264, 100), (8, 300, 1040, 56),
+          (9, 72, 40, 64), (5, 1000, 2000, 1000), (2, 4100, 260, 4100), (127, 200, 129, 72), (128, 128, 256, 128),
           (129, 72, 520, 515), (300, 515, 1030, 515), (1000, 96, 40, 264), (1, 2048, 4096, 2048), (64, 1000, 2000, 1000),
           (256, 2048, 4096, 2048), (5000, 64, 136, 40), (777, 1024, 384, 1032)]
 
