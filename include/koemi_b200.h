@@ -860,8 +860,9 @@ KOEMI_API int koemi_core_dropout(const void *values, const void *residual, void 
  * inference) receives what the backward needs, of
  * koemi_dense_gated_feed_forward_kept bytes. Products run on tensor cores with
  * fp32 sums; fp32 operands as three bf16 parts each, to fp32's precision (an
- * infinite fp32 operand gives NaN). 16-bit hidden values are rounded to the type,
- * so an fp16 one past 65504 is infinite. A call needs at most
+ * fp32 operand past 3.38e38 may give NaN). The forward of up to 8 rows in fp32
+ * and 2 to 4 in 16 bits takes its products on the FMA units. 16-bit hidden values
+ * are rounded to the type, so an fp16 one past 65504 is infinite. A call needs at most
  * koemi_dense_gated_feed_forward_workspace bytes; workspace and kept start at
  * multiples of 256 bytes. */
 KOEMI_API size_t koemi_dense_gated_feed_forward_kept(int64_t rows, int64_t hidden_width, int dtype);

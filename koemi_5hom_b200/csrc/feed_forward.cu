@@ -969,23 +969,28 @@ __global__ __launch_bounds__(256) void join_kernel(const __grid_constant__ GemmA
 // ------------------------------------------------------------------ few rows
 //
 // A few rows (tokens at decode) are bound by the weights' bytes: a warp takes the
-// dot products of kFewUnits units with every row on the FMA units, straight from
+// dot products of few_units units with every row on the FMA units, straight from
 // the weights as they lie (fp32 too: no parts), 16 bytes a lane at a time. The
 // tensor cores' tiles are 128 rows high and their sums parted along K. Measured,
-// here and there, 2048 -> 4096 -> 2048: 1 row 19 and 25 us in bf16, 22 and 99 in
-// fp32; 4 rows 27 and 26 (1024 -> 2048 -> 1024: 13 and 17); 8 rows 49 and 26, in
-// fp32 51 and 99; rows that no 16-byte load fits (3229 -> 2690 -> 3229 bf16) 2
-// rows 39 and 50, 4 rows 99 and 50. Hence the limit:
+// here and there, 2048 -> 4096 -> 2048: 1 row 16 and 25 us in bf16, 22 and 99 in
+// fp32; 4 rows 23 and 25 (1024 -> 2048 -> 1024: 14 and 17); 8 rows in fp32 43 and
+// 99; with rows that no 16-byte load fits (3229 -> 2690 -> 3229) 2 rows of bf16 39
+// and 50, 8 of fp32 86 and 110. Hence the limit, next to which the two meet:
 int64_t few_limit(int64_t width, int64_t hidden, int dtype) {
     return dtype == KOEMI_F32 ? 8 : width % 8 == 0 && hidden % 8 == 0 ? 4 : 2;
 }
-constexpr int kFewUnits = 2;
+// Units of a warp. Loads by element want more of them to an x: 1 row of 3229 ->
+// 2690 -> 3229 bf16 30 us with 2, 23 with 4 (2048 -> 4096 -> 2048, 16 bytes a load: 17 and 19).
+constexpr int few_units(bool vector) { return vector ? 2 : 4; }
+// Steps of 32 lanes whose weights a warp asks for together.
+constexpr int few_asked(bool vector, int dots) { return (vector ? 16 : 32) / dots; }
 
 struct FewArgs {
     const void *x, *w0, *w1;   // kGate: the gate's and the value's weights; kOut: w0
     const void *bias0, *bias1;
     int64_t ld_x, width, units;
     int rows;
+    int share;                 // warps that part the width of one's units (a power of two up to 8)
     void *out;                 // kOut: [rows, units]; kGate: h as the second product reads it
     int64_t ld_out;
     Parts parts;               // kGate: h for the backward (base NULL: not wanted)
@@ -1017,19 +1022,17 @@ struct Piece {
 
 template <typename T, int kEpilogue, int R, bool kVec>
 __global__ __launch_bounds__(256) void few_rows_kernel(const __grid_constant__ FewArgs args) {
-    constexpr int W = kVec ? Pack<T>::kWidth : 1, kSides = kEpilogue == kGate ? 2 : 1, N = kFewUnits * kSides;
-    constexpr int kAsked = (kVec ? 16 : 32) / N;  // steps of 32 lanes whose weights are asked for together
-    const int lane = threadIdx.x & 31;
-    const int64_t unit0 = (static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32) * kFewUnits;
-    if (unit0 >= args.units) {
-        pdl_wait();
-        return;
-    }
+    constexpr int W = kVec ? Pack<T>::kWidth : 1, kSides = kEpilogue == kGate ? 2 : 1;
+    constexpr int kFewUnits = few_units(kVec), N = kFewUnits * kSides, kAsked = few_asked(kVec, N);
+    __shared__ float sums[8][N * R];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, part = warp & (args.share - 1);
+    // units behind the last are the last once more, and not stored
+    const int64_t unit0 = (static_cast<int64_t>(blockIdx.x) * 8 + warp) / args.share * kFewUnits;
     pdl_trigger();
     const T *w[N];
 #pragma unroll
     for (int u = 0; u < kFewUnits; ++u) {
-        const int64_t unit = min(unit0 + u, args.units - 1);  // a unit behind the last is the last once more, and not stored
+        const int64_t unit = min(unit0 + u, args.units - 1);
 #pragma unroll
         for (int k = 0; k < kSides; ++k) w[u * kSides + k] = static_cast<const T *>(k == 0 ? args.w0 : args.w1) + unit * args.width;
     }
@@ -1041,7 +1044,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const __grid_constant__ F
         for (int r = 0; r < R; ++r) sum[n][r] = 0.0f;
     }
     bool waited = false;
-    for (int64_t base = 0; base < args.width; base += kAsked * 32 * W) {
+    for (int64_t base = part * (kAsked * 32 * W); base < args.width; base += args.share * (kAsked * 32 * W)) {
         Piece<T, kVec> pieces[kAsked][N];
 #pragma unroll
         for (int i = 0; i < kAsked; ++i) {
@@ -1081,19 +1084,24 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const __grid_constant__ F
 #pragma unroll
     for (int n = 0; n < N; ++n) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) sum[n][r] = warp_sum(sum[n][r]);
+        for (int r = 0; r < R; ++r) {
+            sum[n][r] = warp_sum(sum[n][r]);
+            if (lane == 0) sums[warp][n * R + r] = sum[n][r];
+        }
     }
-    // lane r finishes row r
+    if (!waited) pdl_wait();  // a part behind the width
+    __syncthreads();
+    if (part != 0 || lane >= args.rows) return;
+    // lane r of the first part's warp adds and finishes row r
 #pragma unroll
     for (int u = 0; u < kFewUnits; ++u) {
         const int64_t unit = unit0 + u;
-        if (unit >= args.units || lane >= args.rows) continue;
+        if (unit >= args.units) continue;
         float v[kSides];
 #pragma unroll
         for (int k = 0; k < kSides; ++k) {
             v[k] = 0.0f;
-#pragma unroll
-            for (int r = 0; r < R; ++r) v[k] = lane == r ? sum[u * kSides + k][r] : v[k];
+            for (int i = 0; i < args.share; ++i) v[k] += sums[warp + i][(u * kSides + k) * R + lane];
             const T *bias = static_cast<const T *>(k == 0 ? args.bias0 : args.bias1);
             if (bias != nullptr) v[k] += to_acc(bias[unit]);
         }
@@ -1114,7 +1122,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const __grid_constant__ F
 }
 
 template <typename T, int kEpilogue>
-int few_rows(const FewArgs &args, bool dependent, cudaStream_t stream) {
+int few_rows(FewArgs args, bool dependent, cudaStream_t stream) {
     constexpr int W = Pack<T>::kWidth;
     const bool vector = args.width % W == 0 && args.ld_x % W == 0 && aligned(args.x, 16) && aligned(args.w0, 16) && aligned(args.w1, 16);
     auto kernel = vector ? few_rows_kernel<T, kEpilogue, 1, true> : few_rows_kernel<T, kEpilogue, 1, false>;
@@ -1123,7 +1131,14 @@ int few_rows(const FewArgs &args, bool dependent, cudaStream_t stream) {
     if constexpr (sizeof(T) == 4) {
         if (args.rows > 4) kernel = vector ? few_rows_kernel<T, kEpilogue, 8, true> : few_rows_kernel<T, kEpilogue, 8, false>;
     }
-    const int64_t blocks = ceil_div(args.units, 8 * kFewUnits);
+    // warps share units until 8 an SM (16 with loads by element) have work, and while each has a step of its
+    // own: 1 row of 2048 -> 4096 -> 2048 bf16 19 us without, 16 with, 18 where steps are not full
+    const int units = few_units(vector);
+    const int64_t groups = ceil_div(args.units, units), want = (vector ? 8 : 16) * sm_count();
+    const int64_t step = few_asked(vector, units * (kEpilogue == kGate ? 2 : 1)) * 32 * (vector ? W : 1);
+    args.share = 1;
+    while (args.share < 8 && groups * args.share < want && 2 * args.share * step <= args.width) args.share *= 2;
+    const int64_t blocks = ceil_div(groups * args.share, 8);
     KOEMI_CUDA_TRY(launch_programmatic(dependent, kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, dim3(1, 1, 1), args));
     return KOEMI_OK;
 }
@@ -1534,11 +1549,11 @@ int forward_few(const Problem &q, void *y, void *kept_base, void *workspace, siz
     if (pool.used > room) return too_small(pool.used);
     const Kept kept = kept_of(kept_pool, q.rows, q.hidden, q.dtype, true);
     const int rows = static_cast<int>(q.rows);
-    FewArgs gate{q.x, q.wg, q.wv, q.bg, q.bv, q.ld_x, q.width, q.hidden, rows, h, round16(q.hidden), kept.h, kept.a, kept.b, kept.ld / 16};
+    FewArgs gate{q.x, q.wg, q.wv, q.bg, q.bv, q.ld_x, q.width, q.hidden, rows, 1, h, round16(q.hidden), kept.h, kept.a, kept.b, kept.ld / 16};
     if (kept_base == nullptr) gate.parts.base = nullptr;
     const int rc = few_rows<T, kGate>(gate, false, stream);
     if (rc != KOEMI_OK) return rc;
-    const FewArgs out{h, q.wo, nullptr, q.bo, nullptr, round16(q.hidden), q.hidden, q.out_width, rows, y, q.out_width, Parts{}, nullptr, nullptr, 0};
+    const FewArgs out{h, q.wo, nullptr, q.bo, nullptr, round16(q.hidden), q.hidden, q.out_width, rows, 1, y, q.out_width, Parts{}, nullptr, nullptr, 0};
     return few_rows<T, kOut>(out, true, stream);
 }
 

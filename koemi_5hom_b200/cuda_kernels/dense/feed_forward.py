@@ -29,9 +29,10 @@ def gated_feed_forward(values: Tensor, gate_weight: Tensor, value_weight: Tensor
     are ``[hidden]``, ``[hidden]``, ``[out]`` (zeros when omitted), all of one
     dtype: f32, bf16 or f16. Sums are fp32. In 16 bits the hidden values are
     rounded to the type between the products, so an fp16 one past 65504 is
-    infinite; fp32 products have fp32's precision, and an infinite operand gives
-    NaN. Differentiable to first order in everything; a call that may be
-    differentiated keeps the two projections and the hidden values.
+    infinite; fp32 products have fp32's precision, and an operand past 3.38e38 may
+    give NaN. Differentiable to first order in everything; a call that may be
+    differentiated keeps the hidden values, silu of the gate and the slope that the
+    gate's gradient takes, 10 bytes a hidden value in 16 bits and 14 in fp32.
     """
     arguments = (values, gate_weight, value_weight, output_weight, gate_bias, value_bias, output_bias)
     if not _training.loaded():
