@@ -253,3 +253,35 @@ def test_large_and_small_fp32_values(cuda):
         arguments[0] = arguments[0] * scale
         arguments[1], arguments[2] = arguments[1] / scale, arguments[2] / scale
         check_ordinary(arguments, grad)
+
+
+@pytest.mark.parametrize("rows", [2, 3, 4, 8, 9])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_rows_are_independent_of_what_is_beside_them(rows, dtype, cuda):
+    for width in (64, 33):
+        arguments, _ = ordinary(rows, width, 40, 24, dtype, cuda, True)
+        weights, biases = arguments[1:4], dict(gate_bias=arguments[4], value_bias=arguments[5], output_bias=arguments[6])
+        clean = gated_feed_forward(arguments[0], *weights, **biases)
+        arguments[0][rows - 1, width - 1] = float("nan")
+        dirty = gated_feed_forward(arguments[0], *weights, **biases)
+        assert torch.equal(dirty[:-1], clean[:-1]) and dirty[-1].isnan().all()
+
+
+def test_rows_past_32_bits(cuda):
+    """x, dx, y and dy of 4.3 thousand million entries. Two results of the same rows are each within three
+    roundings of the formula, so they differ by no more than six, 6 U of the norm."""
+    rows, limit = (1 << 26) + 777, 6 * U[torch.bfloat16]
+    g = torch.Generator(device=cuda).manual_seed(3)
+    x = torch.empty(rows, 64, dtype=torch.bfloat16, device=cuda).normal_(generator=g)
+    weights = [(torch.randn(a, b, generator=g, device=cuda) / 8).bfloat16() for a, b in ((16, 64), (16, 64), (64, 16))]
+    y = gated_feed_forward(x.requires_grad_(True), *weights)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    y, x = y.detach(), x.detach()
+    for first in (0, (1 << 25) - 100, rows - 3000):
+        part = x[first:first + 3000].clone().requires_grad_(True)
+        want = gated_feed_forward(part, *weights)
+        grad, = torch.autograd.grad(want, part, part.detach())
+        for got, w in ((y[first:first + 3000], want), (dx[first:first + 3000], grad)):
+            assert (got.double() - w.double()).norm() <= limit * w.double().norm()
+    del x, y, dx
+    torch.cuda.empty_cache()

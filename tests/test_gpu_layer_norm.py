@@ -259,3 +259,23 @@ def test_dropout_is_linear_to_every_order(cuda):
     grad, = torch.autograd.grad(dropout(x, 0.3, seed=1), x, g, create_graph=True)
     again, = torch.autograd.grad(grad, g, torch.ones_like(g))
     assert torch.equal(again, dropout(torch.ones(100, device=cuda), 0.3, seed=1))
+
+
+def test_layer_norm_rows_past_32_bits(cuda):
+    """4.3 thousand million entries. Two results of the same rows are each within a rounding and fp32's
+    errors of the formula, so they differ by no more than three roundings, 3 * 2^-8 of the norm."""
+    rows = (1 << 26) + 777
+    g = torch.Generator(device=cuda).manual_seed(4)
+    x = torch.empty(rows, 64, dtype=torch.bfloat16, device=cuda).normal_(generator=g)
+    weight, bias = torch.randn(2, 64, generator=g, device=cuda)
+    y = layer_norm(x.requires_grad_(True), weight, bias)
+    dx, = torch.autograd.grad(y, x, y.detach())
+    y, x = y.detach(), x.detach()
+    for first in (0, (1 << 25) - 100, rows - 3000):
+        part = x[first:first + 3000].clone().requires_grad_(True)
+        want = layer_norm(part, weight, bias)
+        grad, = torch.autograd.grad(want, part, y[first:first + 3000].clone())
+        for got, w in ((y[first:first + 3000], want), (dx[first:first + 3000], grad)):
+            assert (got.double() - w.double()).norm() <= 3 * 2.0 ** -8 * w.double().norm()
+    del x, y, dx
+    torch.cuda.empty_cache()
