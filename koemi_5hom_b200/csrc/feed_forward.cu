@@ -936,6 +936,7 @@ __global__ __launch_bounds__(kThreads, 1) void gemm_kernel(const __grid_constant
 template <typename T, int kEpilogue>
 __global__ __launch_bounds__(256) void join_kernel(const __grid_constant__ GemmArgs args) {
     const Job &j = args.jobs[blockIdx.y];
+    pdl_wait();
     const int64_t groups = (j.n + 7) / 8;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (j.splits == 1 || i >= groups * j.m) return;
@@ -953,10 +954,13 @@ __global__ __launch_bounds__(256) void join_kernel(const __grid_constant__ GemmA
     for (int s = 0; s < j.splits; ++s) {
 #pragma unroll
         for (int k = 0; k < kSides; ++k) {
-            float v[8];
-            load_values<8>(src + (kSides * s + k) * side, 8, v);  // ld_partial is a multiple of 16
+            // ld_partial is a multiple of 16; not through the read-only path: the kernel before wrote them
+            const float4 *from = reinterpret_cast<const float4 *>(src + (kSides * s + k) * side);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum[k][e] += v[e];
+            for (int i = 0; i < 2; ++i) {
+                const float4 v = from[i];
+                sum[k][4 * i] += v.x, sum[k][4 * i + 1] += v.y, sum[k][4 * i + 2] += v.z, sum[k][4 * i + 3] += v.w;
+            }
         }
     }
     const DirectStore store{row, column, j.n - column, true};
@@ -1197,6 +1201,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void column_sums_kernel(const __grid_constant__ SumArgs args) {
     using E = typename Operand16<T>::type;
     __shared__ float parts[8][33];
+    pdl_trigger();
     const SumJob &job = args.jobs[blockIdx.z];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t column = static_cast<int64_t>(blockIdx.x) * 32 + lane;
@@ -1231,6 +1236,7 @@ __global__ __launch_bounds__(128) void column_totals_kernel(const __grid_constan
     const SumJob &job = args.jobs[blockIdx.y];
     const int64_t column = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
     if (job.out == nullptr || column >= job.columns) return;
+    pdl_wait();
     const float *src = args.partials + blockIdx.y * args.chunks * args.ld + column;
     float sum = 0.0f;
 #pragma unroll 8
@@ -1445,8 +1451,8 @@ int multiply(const Product *const *products, const Job *jobs, int count, const C
     }
     if (rc != KOEMI_OK) return rc;
     if (most > 0) {
-        join_kernel<T, kEpilogue><<<dim3(static_cast<unsigned>(ceil_div(most, 256)), static_cast<unsigned>(args.job_count)), 256, 0, stream>>>(args);
-        KOEMI_LAUNCH_CHECK();
+        KOEMI_CUDA_TRY(launch_programmatic(true, join_kernel<T, kEpilogue>, dim3(static_cast<unsigned>(ceil_div(most, 256)), static_cast<unsigned>(args.job_count)),
+                                           dim3(256), 0, stream, dim3(1, 1, 1), args));
     }
     return KOEMI_OK;
 }
@@ -1686,8 +1692,8 @@ int backward(const Problem &q, const Gradients &g, const void *kept, void *works
     if (g.dbg != nullptr || g.dbv != nullptr || g.dbo != nullptr) {
         const unsigned columns = static_cast<unsigned>(plan.sums.ld);
         column_sums_kernel<T><<<dim3((columns + 31) / 32, plan.sums.chunks, 3), 256, 0, stream>>>(plan.sums);
-        column_totals_kernel<T><<<dim3((columns + 127) / 128, 3), 128, 0, stream>>>(plan.sums);
         KOEMI_LAUNCH_CHECK();
+        KOEMI_CUDA_TRY(launch_programmatic(true, column_totals_kernel<T>, dim3((columns + 127) / 128, 3), dim3(128), 0, stream, dim3(1, 1, 1), plan.sums));
     }
     return KOEMI_OK;
 }

@@ -361,6 +361,7 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
     int64_t lead = static_cast<int64_t>(blockIdx.x) * teams + (kWarp ? (threadIdx.x & ~31) / team : 0);
     const float inv_width = 1.0f / static_cast<float>(a.width);
     const int span = span_of(warps);
+    pdl_trigger();
 
     RowPackets<T, kVec, K> next_x, next_g;
     float next_mean = 0.0f, next_inverse = 0.0f;
@@ -487,6 +488,7 @@ __global__ __launch_bounds__(1024) void norm_backward_wide_kernel(const NormRows
     constexpr int W = Pack<T>::kWidth;
     extern __shared__ float4 sums[];  // [dw | db][width / 4]
     __shared__ float2 slots[2][32];
+    pdl_trigger();
     const int t = threadIdx.x, quads = a.width / 4;
     const float inv_width = 1.0f / static_cast<float>(a.width);
     if (partials != nullptr) {
@@ -617,12 +619,13 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(const NormRows a, con
 // dw (grid.y 0) and db (1): the partial rows added in order, 32 columns a
 // CTA, 16 of its warps' strided parts joined in order.
 constexpr int kFinishWarps = 16;
-__global__ __launch_bounds__(32 * kFinishWarps) void norm_finish_kernel(const float *__restrict__ partials, int64_t rows, int width,
+__global__ __launch_bounds__(32 * kFinishWarps) void norm_finish_kernel(const float *partials, int64_t rows, int width,
                                                                          void *dw, void *db, int dtype) {
     __shared__ float parts[kFinishWarps][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     void *out = blockIdx.y == 0 ? dw : db;
     if (out == nullptr) return;
+    pdl_wait();
     float sum = 0.0f;
     if (c < width) {
         const float *p = partials + static_cast<int64_t>(blockIdx.y) * width + c;
@@ -805,9 +808,8 @@ int backward(const NormRows &a, const void *weight, bool wide, const float *stat
     KOEMI_LAUNCH_CHECK();
     if (partials != nullptr) {
         const int dtype = wide ? KOEMI_F32 : sizeof(T) == 4 ? KOEMI_F32 : std::is_same<T, __half>::value ? KOEMI_F16 : KOEMI_BF16;
-        norm_finish_kernel<<<dim3(static_cast<unsigned>(ceil_div(a.width, 32)), 2), 32 * kFinishWarps, 0, stream>>>(
-            partials, grid, a.width, dw, db, dtype);
-        KOEMI_LAUNCH_CHECK();
+        KOEMI_CUDA_TRY(launch_programmatic(true, norm_finish_kernel, dim3(static_cast<unsigned>(ceil_div(a.width, 32)), 2), dim3(32 * kFinishWarps), 0,
+                                           stream, dim3(1, 1, 1), partials, grid, a.width, dw, db, dtype));
     }
     return KOEMI_OK;
 }
