@@ -397,7 +397,7 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
             to_pairs(x, k, u);
             to_pairs(y, k, q);
         }
-        // columns and rows behind the last have g = 0 and w = 0: whatever u is there, nothing of it counts
+        // columns and rows behind the last have g = 0 and w = 0: whatever finite u is there, nothing of it counts
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             u[i] = mul2(add2(u[i], both(-mean)), both(inverse));
@@ -406,6 +406,16 @@ __global__ __launch_bounds__(kWarp ? 256 : 512) void norm_backward_kernel(const 
             q[i] = mul2(q[i], w[i]);
             firsts = add2(firsts, q[i]);
             seconds = fma2(q[i], u[i], seconds);
+        }
+        // A large constant row's mean over sqrt(eps) is infinite, and 0 times it NaN: the sum over its own columns only.
+        // (Their mean taken as 0 in every row cost rows by element 96 bytes of spills.)
+        if (isinf(mean * inverse)) {
+            seconds = both(0.0f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (((2 * i / W) * team + t) * W < a.width) seconds.x = fmaf(q[i].x, u[i].x, seconds.x);
+                if (((2 * i + 1) / W * team + t) * W < a.width) seconds.y = fmaf(q[i].y, u[i].y, seconds.y);
+            }
         }
         float first = firsts.x + firsts.y, second = seconds.x + seconds.y;
         if (lead + step < a.rows) request(row + step);

@@ -1,0 +1,45 @@
+"""Corners of the feed-forward sub-layer's operators on the GPU: values at the ends of their range, every plan of the
+norm's kernels, buffers of exactly the size that the C entries ask for, calls on several streams at once."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from koemi_5hom_b200.cuda_kernels.core import layer_norm
+
+pytestmark = pytest.mark.gpu
+
+EPS = 2.0 ** -24
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def normal(cuda, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return lambda *shape, scale=1.0, dtype=torch.float32: (scale * torch.randn(*shape, generator=g)).to(dtype).to(cuda)
+
+
+# ---------------------------------------------------------------- layer norm
+
+@pytest.mark.parametrize("rows", [5, 1500])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width,exponent,eps", [(33, 120, 1e-5), (96, 120, 1e-5), (40, 120, 1e-5), (1021, 110, 1e-12), (1032, 110, 1e-12),
+                                                (2312, 110, 1e-12), (16384, 110, 1e-12), (33000, 110, 1e-12)])
+def test_norm_of_large_constant_rows(width, exponent, eps, dtype, rows, cuda):
+    """The mean is exact (a power of two, at widths n with fl(fl(1 / n) n) = 1), so u is 0, y is b and dw is 0 to the bit,
+    and dx = (a - mean(a)) / sqrt(eps). Mean times 1 / sqrt(eps) is past fp32's range: nothing may form it."""
+    new = normal(cuda, width)
+    x = torch.full((rows, width), 2.0 ** exponent, dtype=dtype, device=cuda, requires_grad=True)
+    w, b = (new(width).requires_grad_(True) for _ in range(2))
+    g = new(rows, width, dtype=dtype)
+    y = layer_norm(x, w, b, eps=eps)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    assert torch.equal(y, b.to(dtype).expand_as(y)) and not dw.any()
+    # a sum over a row is at most width / 1024 + 40 additions deep, over rows rows / 148 + 100; the rest: 12 roundings
+    deep, down = (width / 1024 + 40) * EPS, (rows / 148 + 100) * EPS
+    a = g.double() * w.detach().double()
+    mean, inverse = a.mean(-1, keepdim=True), eps ** -0.5
+    want = inverse * (a - mean)
+    allowed = inverse * (2 * deep * a.abs().mean(-1, keepdim=True) + (deep + 12 * EPS) * (a.abs() + mean.abs()))
+    assert ((dx.double() - want).abs() <= U[dtype] * 1.0001 * want.abs() + allowed).all()
+    assert ((db.double() - g.double().sum(0)).abs() <= EPS * db.double().abs() + 2 * down * g.double().abs().sum(0)).all()
