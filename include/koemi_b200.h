@@ -15,7 +15,8 @@
  *     first call that uses a device).
  *   - The return value is KOEMI_OK (0) or a negative KOEMI_ERR_* code; the
  *     message for the calling thread is read with koemi_last_error().
- *   - `dtype` arguments take a koemi_dtype value.
+ *   - `dtype` arguments take a koemi_dtype value. Pointers are aligned to
+ *     the type that they point to.
  *
  * Reference interfaces named below are paths inside the Koemi-5HOM project.
  */
@@ -831,7 +832,8 @@ KOEMI_API int koemi_core_layer_norm_forward(const void *values, int64_t rows, in
                                             int dtype, void *stream);
 /* Its gradients from grad_out [rows, width]: grad_values [rows, width] (dtype),
  * grad_weight and grad_bias [width] (weight_dtype), each NULL where it is not
- * wanted. Without rows the weights' gradients are zeros. */
+ * wanted. Without rows the weights' gradients are zeros. The workspace, which
+ * those two take, starts at a multiple of 16 bytes. */
 KOEMI_API size_t koemi_core_layer_norm_backward_workspace(int64_t rows, int64_t width);
 KOEMI_API int koemi_core_layer_norm_backward(const void *values, int64_t rows, int64_t width, int64_t inner_rows,
                                              int64_t outer_stride, int64_t inner_stride, const void *weight,

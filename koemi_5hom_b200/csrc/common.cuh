@@ -10,6 +10,7 @@
 #include <cstdarg>
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 #include <utility>
 
 #include "../../include/koemi_b200.h"
@@ -50,6 +51,14 @@ inline size_t dtype_size(int dtype) {
 
 inline bool aligned(const void *pointer, size_t bytes) {
     return (reinterpret_cast<uintptr_t>(pointer) % bytes) == 0;
+}
+
+// NULL counts as aligned.
+inline bool aligned(std::initializer_list<const void *> pointers, size_t bytes) {
+    for (const void *pointer : pointers) {
+        if (!aligned(pointer, bytes)) return false;
+    }
+    return true;
 }
 
 inline cudaStream_t as_stream(void *stream) { return reinterpret_cast<cudaStream_t>(stream); }

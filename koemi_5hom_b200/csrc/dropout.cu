@@ -140,6 +140,9 @@ extern "C" int koemi_core_dropout(const void *values, const void *residual, void
     if (dtype != KOEMI_F32 && dtype != KOEMI_F16 && dtype != KOEMI_BF16) return fail(KOEMI_ERR_INVALID, "unsupported dropout dtype %d", dtype);
     if (count == 0) return KOEMI_OK;
     if (values == nullptr || out == nullptr) return fail(KOEMI_ERR_INVALID, "values and out must be non-NULL");
+    if (!aligned({values, residual, out}, dtype_size(dtype)) || !aligned(step_device, 8)) {
+        return fail(KOEMI_ERR_INVALID, "dropout's pointers must be aligned to their types");
+    }
     const Numbers n{seed, site, step, step_device, static_cast<uint32_t>(dropped),
                     dropped == 65536 ? 0.0f : static_cast<float>(65536.0 / (65536.0 - static_cast<double>(dropped)))};
     if (dtype == KOEMI_F32) return run<float>(values, residual, out, count, n, as_stream(stream));

@@ -1706,6 +1706,8 @@ int check(int64_t rows, int64_t width, int64_t hidden, int64_t out_width, int dt
     return KOEMI_OK;
 }
 
+int misaligned() { return fail(KOEMI_ERR_INVALID, "feed-forward pointers must be aligned to their type"); }
+
 }  // namespace
 }  // namespace koemi
 
@@ -1749,6 +1751,7 @@ extern "C" int koemi_dense_gated_feed_forward_forward(const void *values, int64_
     if (values == nullptr || gate_weight == nullptr || value_weight == nullptr || output_weight == nullptr || out == nullptr) {
         return fail(KOEMI_ERR_INVALID, "values, weights and out must be non-NULL");
     }
+    if (!aligned({values, gate_weight, value_weight, output_weight, gate_bias, value_bias, output_bias, out}, dtype_size(dtype))) return misaligned();
     if (kept != nullptr && (kept_bytes < koemi_dense_gated_feed_forward_kept(rows, hidden_width, dtype) || !aligned(kept, 256))) {
         return fail(KOEMI_ERR_WORKSPACE, "kept must hold %zu bytes from a multiple of 256", koemi_dense_gated_feed_forward_kept(rows, hidden_width, dtype));
     }
@@ -1770,6 +1773,10 @@ extern "C" int koemi_dense_gated_feed_forward_backward(const void *values, int64
     const int rc = check(rows, width, hidden_width, out_width, dtype);
     if (rc != KOEMI_OK) return rc;
     if (value_stride < width) return fail(KOEMI_ERR_INVALID, "value_stride must be at least the width");
+    if (!aligned({values, gate_weight, value_weight, output_weight, grad_out, grad_values, grad_gate_weight, grad_value_weight, grad_output_weight,
+                  grad_gate_bias, grad_value_bias, grad_output_bias}, dtype_size(dtype))) {
+        return misaligned();
+    }
     if (rows == 0) {  // sums of no rows
         const size_t size = dtype_size(dtype);
         const struct { void *p; int64_t count; } sums[] = {{grad_gate_weight, hidden_width * width}, {grad_value_weight, hidden_width * width},

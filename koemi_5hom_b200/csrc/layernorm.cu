@@ -833,6 +833,8 @@ int check(const void *x, int64_t rows, int64_t width, int64_t inner, int64_t out
     return KOEMI_OK;
 }
 
+int misaligned() { return fail(KOEMI_ERR_INVALID, "layer norm's pointers must be aligned to their types"); }
+
 }  // namespace
 }  // namespace koemi
 
@@ -847,6 +849,7 @@ extern "C" int koemi_core_layer_norm_forward(const void *values, int64_t rows, i
     if (!(eps >= 0.0f) || eps > 3.0e38f) return fail(KOEMI_ERR_INVALID, "eps must be finite and non-negative");
     if (rows == 0) return KOEMI_OK;
     if (values == nullptr || weight == nullptr || out == nullptr) return fail(KOEMI_ERR_INVALID, "values, weight and out must be non-NULL");
+    if (!aligned(out, dtype_size(dtype)) || !aligned({weight, bias}, dtype_size(weight_dtype)) || !aligned(stats, 4)) return misaligned();
     const NormRows a{values, rows, inner_rows, outer_stride, inner_stride, static_cast<int>(width), 32};
     const bool wide = weight_dtype == KOEMI_F32;
     if (dtype == KOEMI_F32) return forward<float>(a, weight, bias, wide, out, stats, eps, as_stream(stream));
@@ -867,6 +870,10 @@ extern "C" int koemi_core_layer_norm_backward(const void *values, int64_t rows, 
     const int rc = check(values, rows, width, inner_rows, outer_stride, inner_stride, dtype, weight_dtype);
     if (rc != KOEMI_OK) return rc;
     const bool sums = grad_weight != nullptr || grad_bias != nullptr;
+    if (!aligned({grad_out, grad_values}, dtype_size(dtype)) || !aligned({weight, grad_weight, grad_bias}, dtype_size(weight_dtype)) ||
+        !aligned(stats, 4)) {
+        return misaligned();
+    }
     if (rows == 0) {  // the sum of no rows
         const size_t bytes = dtype_size(weight_dtype) * static_cast<size_t>(width);
         if (grad_weight != nullptr) KOEMI_CUDA_TRY(cudaMemsetAsync(grad_weight, 0, bytes, as_stream(stream)));
@@ -876,8 +883,9 @@ extern "C" int koemi_core_layer_norm_backward(const void *values, int64_t rows, 
     if (values == nullptr || weight == nullptr || stats == nullptr || grad_out == nullptr) {
         return fail(KOEMI_ERR_INVALID, "values, weight, stats and grad_out must be non-NULL");
     }
-    if (sums && (workspace == nullptr || workspace_bytes < koemi_core_layer_norm_backward_workspace(rows, width))) {
-        return fail(KOEMI_ERR_WORKSPACE, "layer norm backward needs %zu workspace bytes", koemi_core_layer_norm_backward_workspace(rows, width));
+    if (sums && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < koemi_core_layer_norm_backward_workspace(rows, width))) {
+        return fail(KOEMI_ERR_WORKSPACE, "layer norm backward needs %zu workspace bytes from a multiple of 16",
+                    koemi_core_layer_norm_backward_workspace(rows, width));
     }
     const NormRows a{values, rows, inner_rows, outer_stride, inner_stride, static_cast<int>(width), 32};
     const bool wide = weight_dtype == KOEMI_F32;

@@ -1,0 +1,47 @@
+"""Corners of the feed-forward sub-layer's operators that need no GPU: what their C entries refuse."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from koemi_5hom_b200 import _native
+
+PAGE = 256  # an address that nothing reads
+
+
+def pointers(names, odd, by):
+    """PAGE for every name, `by` bytes behind it for `odd`."""
+    return {name: ctypes.c_void_p(PAGE + (by if name == odd else 0)) for name in names}
+
+
+@pytest.mark.parametrize("dtype", [_native.F32, _native.BF16])
+def test_entries_refuse_pointers_off_their_type(dtype):
+    """Before anything is launched: on the device such an access would end the context."""
+    lib, invalid = _native.library(), _native.KOEMI_ERR_INVALID
+    half = 2 if dtype == _native.F32 else 1
+    names = ("values", "weight", "bias", "out", "stats")
+    for odd in names:
+        p = pointers(names, odd, 2 if odd == "stats" else half)
+        assert lib.koemi_core_layer_norm_forward(p["values"], 4, 8, 4, 0, 8, p["weight"], p["bias"], dtype, p["out"], p["stats"], 1e-5, dtype,
+                                                 None) == invalid, odd
+    names = ("values", "weight", "stats", "grad", "dx", "dw", "db", "workspace")
+    for odd in names:
+        p = pointers(names, odd, {"stats": 2, "workspace": 8}.get(odd, half))
+        assert lib.koemi_core_layer_norm_backward(p["values"], 4, 8, 4, 0, 8, p["weight"], dtype, p["stats"], p["grad"], p["dx"], p["dw"], p["db"],
+                                                  dtype, p["workspace"], 1 << 20, None) == (_native.KOEMI_ERR_WORKSPACE if odd == "workspace" else invalid), odd
+    names = ("values", "residual", "out", "step")
+    for odd in names:
+        p = pointers(names, odd, 4 if odd == "step" else half)
+        assert lib.koemi_core_dropout(p["values"], p["residual"], p["out"], 9, 100, 1, 2, 3, p["step"], dtype, None) == invalid, odd
+    names = ("values", "wg", "wv", "wo", "bg", "bv", "bo", "out")
+    for odd in names:
+        p = pointers(names, odd, half)
+        assert lib.koemi_dense_gated_feed_forward_forward(p["values"], 16, *(p[n] for n in names[1:]), None, 0, 10, 16, 20, 8, dtype,
+                                                          ctypes.c_void_p(PAGE), 1 << 24, None) == invalid, odd
+    names = ("values", "wg", "wv", "wo", "grad", "dx", "dwg", "dwv", "dwo", "dbg", "dbv", "dbo")
+    for odd in names:
+        p = pointers(names, odd, half)
+        assert lib.koemi_dense_gated_feed_forward_backward(p["values"], 16, p["wg"], p["wv"], p["wo"], ctypes.c_void_p(PAGE), 1 << 20,
+                                                           *(p[n] for n in names[4:]), 10, 16, 20, 8, dtype, ctypes.c_void_p(PAGE), 1 << 24,
+                                                           None) == invalid, odd
