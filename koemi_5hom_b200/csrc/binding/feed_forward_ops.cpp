@@ -192,6 +192,11 @@ Tensor dropout_autograd(const Tensor &values, const OptionalTensor &residual, co
     return out;
 }
 
+// vmap would call the operator once a sample, each time with the same positions and so the same mask.
+Tensor dropout_batched(const Tensor &, const OptionalTensor &, const OptionalTensor &, int64_t, int64_t, int64_t, int64_t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(false, "dropout has no vmap rule: every sample would get the same mask; call it on the whole batch");
+}
+
 // ------------------------------------------------------------ the gated block
 
 // The weights and biases of a call, in the order of its gradients after the values'.
@@ -376,6 +381,8 @@ TORCH_LIBRARY_IMPL(koemi_b200, CUDA, m) {
     m.impl("gated_feed_forward_keep", gated_feed_forward_keep_cuda);
     m.impl("gated_feed_forward_backward", gated_feed_forward_backward_cuda);
 }
+
+TORCH_LIBRARY_IMPL(koemi_b200, FuncTorchBatched, m) { m.impl("dropout", dropout_batched); }
 
 TORCH_LIBRARY_IMPL(koemi_b200, Autograd, m) {
     m.impl("layer_norm", layer_norm_autograd);

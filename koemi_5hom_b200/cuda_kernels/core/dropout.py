@@ -31,6 +31,8 @@ def dropout(values: Tensor, probability: float, *, seed: int, site: int = 0, ste
     is read by the kernel, so that a captured graph draws new numbers when the
     program advances it; it must not change between a pass's forward and backward. A dropped
     value may be anything, infinities and NaN too. Differentiable in reverse mode.
+    ``torch.vmap`` over it is refused: a position names its bits, so every sample
+    would get the same mask.
     """
     if isinstance(probability, bool) or not isinstance(probability, (int, float)) or not 0.0 <= probability <= 1.0:
         raise CudaExtensionValidationError("probability must be in [0, 1]")

@@ -1,11 +1,14 @@
-"""Corners of the feed-forward sub-layer's operators that need no GPU: what their C entries refuse."""
+"""Corners of the feed-forward sub-layer's operators that need no GPU: what their C entries and torch's transforms are
+refused, what they ask for, and the arithmetic of fp32 values in bf16 parts."""
 from __future__ import annotations
 
 import ctypes
 
 import pytest
+import torch
 
 from koemi_5hom_b200 import _native
+from koemi_5hom_b200.cuda_kernels import _training
 
 PAGE = 256  # an address that nothing reads
 
@@ -45,3 +48,15 @@ def test_entries_refuse_pointers_off_their_type(dtype):
         assert lib.koemi_dense_gated_feed_forward_backward(p["values"], 16, p["wg"], p["wv"], p["wo"], ctypes.c_void_p(PAGE), 1 << 20,
                                                            *(p[n] for n in names[4:]), 10, 16, 20, 8, dtype, ctypes.c_void_p(PAGE), 1 << 24,
                                                            None) == invalid, odd
+
+
+@pytest.mark.parametrize("batched", ["values", "residual"])
+def test_dropout_is_refused_under_vmap(batched):
+    """Called once a sample it would name the same positions' bits, the same mask, for every one of them."""
+    _training.register()
+    x, r = torch.zeros(5, 6, 16, device="meta"), torch.zeros(6, 16, device="meta")
+    drop = lambda t: torch.ops.koemi_b200.dropout(*((t, r) if batched == "values" else (r, t)), None, 6554, 1, 2, 3)  # noqa: E731
+    assert drop(x[0]).shape == r.shape
+    for call in (drop, torch.func.grad(lambda t: drop(t).sum())):
+        with pytest.raises(NotImplementedError, match="vmap"):
+            torch.vmap(call)(x)

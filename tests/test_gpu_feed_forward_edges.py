@@ -5,7 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from koemi_5hom_b200.cuda_kernels.core import layer_norm
+from koemi_5hom_b200.cuda_kernels.core import dropout, layer_norm
+from koemi_5hom_b200.cuda_kernels.dense import gated_feed_forward
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +44,17 @@ def test_norm_of_large_constant_rows(width, exponent, eps, dtype, rows, cuda):
     allowed = inverse * (2 * deep * a.abs().mean(-1, keepdim=True) + (deep + 12 * EPS) * (a.abs() + mean.abs()))
     assert ((dx.double() - want).abs() <= U[dtype] * 1.0001 * want.abs() + allowed).all()
     assert ((db.double() - g.double().sum(0)).abs() <= EPS * db.double().abs() + 2 * down * g.double().abs().sum(0)).all()
+
+
+# -------------------------------------------------------- torch's transforms
+
+def test_vmap(cuda):
+    """Refused where samples would share a mask; else the samples' own results."""
+    new = normal(cuda)
+    x, w, b = new(5, 40, 64), new(64), new(64)
+    wg, wv, wo = new(48, 64), new(48, 64), new(64, 48)
+    assert torch.equal(torch.vmap(lambda t: layer_norm(t, w, b))(x), torch.stack([layer_norm(t, w, b) for t in x]))
+    assert torch.equal(torch.vmap(lambda t: gated_feed_forward(t, wg, wv, wo))(x), torch.stack([gated_feed_forward(t, wg, wv, wo) for t in x]))
+    for call in (lambda t: dropout(t, 0.1, seed=1), lambda t: dropout(x[0], 0.1, seed=1, residual=t)):
+        with pytest.raises(NotImplementedError, match="vmap"):
+            torch.vmap(call)(x)
