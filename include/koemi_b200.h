@@ -865,11 +865,18 @@ KOEMI_API int koemi_core_dropout(const void *values, const void *residual, void 
  * fp32 operand past 3.38e38 may give NaN). The forward of up to 8 rows in fp32
  * and 2 to 4 in 16 bits takes its products on the FMA units. 16-bit hidden values
  * are rounded to the type, so an fp16 one past 65504 is infinite. A call needs at most
- * koemi_dense_gated_feed_forward_workspace bytes; workspace and kept start at
- * multiples of 256 bytes. */
+ * koemi_dense_gated_feed_forward_workspace bytes, on the device that is current
+ * when they are asked for; workspace and kept start at multiples of 256 bytes.
+ * pass: 0 the forward, or a sum of these. Without ALIGNED it counts copies of
+ * operands that the kernels may not be able to read as they lie. */
+enum koemi_feed_forward_pass {
+    KOEMI_FEED_FORWARD_BACKWARD = 1, /* the backward */
+    KOEMI_FEED_FORWARD_KEEPS = 2,    /* the forward with kept */
+    KOEMI_FEED_FORWARD_ALIGNED = 4   /* values, weights and grad_out start at multiples of 16 bytes, and value_stride is a multiple of 8 */
+};
 KOEMI_API size_t koemi_dense_gated_feed_forward_kept(int64_t rows, int64_t hidden_width, int dtype);
 KOEMI_API size_t koemi_dense_gated_feed_forward_workspace(int64_t rows, int64_t width, int64_t hidden_width,
-                                                          int64_t out_width, int dtype, int backward);
+                                                          int64_t out_width, int dtype, int pass);
 KOEMI_API int koemi_dense_gated_feed_forward_forward(const void *values, int64_t value_stride, const void *gate_weight,
                                                      const void *value_weight, const void *output_weight,
                                                      const void *gate_bias, const void *value_bias,

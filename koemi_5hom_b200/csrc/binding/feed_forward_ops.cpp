@@ -233,6 +233,13 @@ Tensor bytes_of(const Tensor &like, size_t size) {
     return at::empty({static_cast<int64_t>(std::max<size_t>(size, 256))}, like.options().dtype(at::kByte));
 }
 
+// Whether the kernels read these as they lie, as far as starts and the values' stride go.
+int aligned_pass(int64_t stride, std::initializer_list<const Tensor *> operands) {
+    bool aligned = stride % 8 == 0;
+    for (const Tensor *t : operands) aligned = aligned && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
+    return aligned ? KOEMI_FEED_FORWARD_ALIGNED : 0;
+}
+
 Tensor block_forward(const Tensor &values, const Tensor &gate_weight, const Tensor &value_weight, const Tensor &output_weight,
                      const OptionalTensor &gate_bias, const OptionalTensor &value_bias, const OptionalTensor &output_bias, Tensor *kept) {
     const BlockShape s(values, gate_weight, value_weight, output_weight, gate_bias, value_bias, output_bias);
@@ -240,7 +247,8 @@ Tensor block_forward(const Tensor &values, const Tensor &gate_weight, const Tens
     const int code = code_of(values);
     Tensor out = at::empty({s.rows, s.out}, values.options());
     if (kept != nullptr) *kept = bytes_of(values, lib().block_kept(s.rows, s.hidden, code));
-    Tensor workspace = bytes_of(values, lib().block_workspace(s.rows, s.width, s.hidden, s.out, code, 0));
+    const int pass = aligned_pass(s.stride, {&values, &gate_weight, &value_weight, &output_weight}) | (kept != nullptr ? KOEMI_FEED_FORWARD_KEEPS : 0);
+    Tensor workspace = bytes_of(values, lib().block_workspace(s.rows, s.width, s.hidden, s.out, code, pass));
     check("koemi_dense_gated_feed_forward_forward",
           lib().block_forward(address<void>(values), s.stride, address<void>(gate_weight), address<void>(value_weight),
                               address<void>(output_weight), address<void>(gate_bias), address<void>(value_bias),
@@ -290,7 +298,8 @@ std::vector<Tensor> gated_feed_forward_backward_cuda(const Tensor &values, const
         grads.push_back(want ? at::empty(sizes[k], values.options()) : at::empty({0}, values.options()));
         p[k] = want ? address<void>(grads.back()) : nullptr;
     }
-    Tensor workspace = bytes_of(values, lib().block_workspace(s.rows, s.width, s.hidden, s.out, code, 1));
+    const int pass = aligned_pass(s.stride, {&values, &gate_weight, &value_weight, &output_weight, &grad}) | KOEMI_FEED_FORWARD_BACKWARD;
+    Tensor workspace = bytes_of(values, lib().block_workspace(s.rows, s.width, s.hidden, s.out, code, pass));
     check("koemi_dense_gated_feed_forward_backward",
           lib().block_backward(address<void>(values), s.stride, address<void>(gate_weight), address<void>(value_weight),
                                address<void>(output_weight), address<void>(kept), kept.numel(), address<void>(grad), p[0], p[1], p[2],

@@ -1457,10 +1457,12 @@ int multiply(const Product *const *products, const Job *jobs, int count, const C
     return KOEMI_OK;
 }
 
-// Hands out 256-byte aligned parts of a workspace; without one it only counts.
+// Hands out 256-byte aligned parts of a workspace; without one it only counts,
+// for operands that TMA reads as they lie (direct) or for any.
 struct Pool {
     char *base;
     size_t used = 0;
+    bool direct = false;
     void *take(size_t bytes) {
         void *p = base == nullptr ? nullptr : base + used;
         used += round256(bytes);
@@ -1496,10 +1498,10 @@ Kept kept_of(Pool &pool, int64_t rows, int64_t hidden, int dtype, bool with_slop
     return kept;
 }
 
-// `src` as an operand: itself where TMA reads it, else a packed copy, noted in `jobs`. With counting, the
-// base is unknown: it asks for room as if the copy were made.
+// `src` as an operand: itself where TMA reads it, else a packed copy, noted in `jobs`.
 Matrix operand(Pool &pool, const void *src, int64_t rows, int64_t columns, int64_t ld, int dtype, PackArgs &jobs, int &count) {
-    if (dtype != KOEMI_F32 && pool.base != nullptr && ld % 8 == 0 && aligned(src, 16)) return Matrix{src, rows, columns, ld, 0, 1};
+    const bool direct = pool.base == nullptr ? pool.direct : aligned(src, 16);
+    if (dtype != KOEMI_F32 && direct && ld % 8 == 0) return Matrix{src, rows, columns, ld, 0, 1};
     const int64_t padded = round16(columns);
     const Parts to{pool.take(static_cast<size_t>(rows) * padded * 2 * parts_of(dtype)), padded, rows * padded};
     jobs.jobs[count++] = PackJob{src, rows, columns, ld, to};
@@ -1721,20 +1723,20 @@ extern "C" size_t koemi_dense_gated_feed_forward_kept(int64_t rows, int64_t hidd
 }
 
 extern "C" size_t koemi_dense_gated_feed_forward_workspace(int64_t rows, int64_t width, int64_t hidden_width, int64_t out_width,
-                                                           int dtype, int backward) {
+                                                           int dtype, int pass) {
     if (rows < 1 || check(rows, width, hidden_width, out_width, dtype) != KOEMI_OK) return 0;
     const Problem q{nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, rows, width, hidden_width, out_width, width, dtype};
-    Pool pool{nullptr};
-    if (backward) {
+    Pool pool{nullptr, 0, (pass & KOEMI_FEED_FORWARD_ALIGNED) != 0};
+    if (pass & KOEMI_FEED_FORWARD_BACKWARD) {
         BackwardPlan plan{};
         plan_backward(plan, q, Gradients{}, pool, nullptr);
     } else if (rows <= few_limit(width, hidden_width, dtype)) {
         pool.take(few_bytes(rows, hidden_width, dtype));
     } else {
         ForwardPlan plan{};
-        plan_forward(plan, q, pool, nullptr, false);
+        plan_forward(plan, q, pool, nullptr, (pass & KOEMI_FEED_FORWARD_KEEPS) != 0);
     }
-    return pool.used;
+    return std::max<size_t>(pool.used, 256);
 }
 
 extern "C" int koemi_dense_gated_feed_forward_forward(const void *values, int64_t value_stride, const void *gate_weight,

@@ -60,3 +60,21 @@ def test_dropout_is_refused_under_vmap(batched):
     for call in (drop, torch.func.grad(lambda t: drop(t).sum())):
         with pytest.raises(NotImplementedError, match="vmap"):
             torch.vmap(call)(x)
+
+
+def test_block_workspace_is_what_the_pass_uses():
+    """Bits of the query's last argument: 1 the backward, 2 the forward writes kept, 4 every operand starts at a
+    multiple of 16 bytes with rows of a multiple of 8 values. 0 and 1 ask for enough for any operands."""
+    ask = _native.library().koemi_dense_gated_feed_forward_workspace
+    sizes, rows, hidden = (32768, 2048, 4096, 2048), 32768, 4096
+    operands = 2 * (rows * 2048 + 3 * 4096 * 2048)  # x and the weights in padded rows
+    assert ask(*sizes, _native.BF16, 0) >= 2 * rows * hidden + operands
+    assert 2 * rows * hidden <= ask(*sizes, _native.BF16, 4) < 2 * rows * hidden + 2 ** 20  # h
+    assert 0 < ask(*sizes, _native.BF16, 2 | 4) < 2 ** 20
+    assert operands <= ask(*sizes, _native.BF16, 2) < operands + 2 ** 20
+    both = 4 * rows * hidden  # dp and dq
+    assert both <= ask(*sizes, _native.BF16, 1 | 4) < both + 2 ** 21 and ask(*sizes, _native.BF16, 1) >= both + operands + 2 * rows * 2048
+    for dtype in (_native.F32, _native.BF16):  # fp32 operands are always split, odd rows always copied
+        for odd in ((300, 515, 1030, 515), (3, 515, 77, 33)):
+            assert ask(*odd, dtype, 0) == ask(*odd, dtype, 4) and ask(*odd, dtype, 1) == ask(*odd, dtype, 1 | 4)
+            assert 0 < ask(*odd, dtype, 2) <= ask(*odd, dtype, 0)

@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from koemi_5hom_b200 import _native
 from koemi_5hom_b200.cuda_kernels.core import dropout, layer_norm
 from koemi_5hom_b200.cuda_kernels.dense import gated_feed_forward
 
@@ -58,3 +59,28 @@ def test_vmap(cuda):
     for call in (lambda t: dropout(t, 0.1, seed=1), lambda t: dropout(x[0], 0.1, seed=1, residual=t)):
         with pytest.raises(NotImplementedError, match="vmap"):
             torch.vmap(call)(x)
+
+
+# ---------------------------------------------------------------- memory
+
+def test_block_takes_no_memory_that_it_does_not_use(cuda):
+    """A training pass of aligned bf16: the forward leaves y and what the backward needs (h in 2 bytes a hidden value,
+    two slopes in 4), the backward takes what the query asks for operands that are read as they lie; a megabyte for the allocator."""
+    rows, width, hidden = 16384, 512, 1024
+    new = normal(cuda)
+    leaves = [new(*shape, dtype=torch.bfloat16).requires_grad_(True) for shape in ((rows, width), (hidden, width), (hidden, width), (width, hidden))]
+    grad = new(rows, width, dtype=torch.bfloat16)
+
+    def peak(call):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        result = call()
+        torch.cuda.synchronize()
+        return result, torch.cuda.max_memory_allocated() - before
+
+    y, forward = peak(lambda: gated_feed_forward(*leaves))
+    assert forward <= 2 * rows * width + 10 * rows * hidden + 2 ** 20
+    results, backward = peak(lambda: torch.autograd.grad(y, leaves, grad))
+    ask = lambda bits: _native.library().koemi_dense_gated_feed_forward_workspace(rows, width, hidden, width, _native.BF16, bits)  # noqa: E731
+    assert backward <= sum(2 * t.numel() for t in leaves) + ask(1 | 4) + 2 ** 20 and ask(1 | 4) <= ask(1) - 4 * rows * width
