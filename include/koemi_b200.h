@@ -833,7 +833,8 @@ KOEMI_API int koemi_core_layer_norm_forward(const void *values, int64_t rows, in
 /* Its gradients from grad_out [rows, width]: grad_values [rows, width] (dtype),
  * grad_weight and grad_bias [width] (weight_dtype), each NULL where it is not
  * wanted. Without rows the weights' gradients are zeros. The workspace, which
- * those two take, starts at a multiple of 16 bytes. */
+ * those two take, starts at a multiple of 16 bytes; its size is that for the
+ * device that is current when it is asked for. */
 KOEMI_API size_t koemi_core_layer_norm_backward_workspace(int64_t rows, int64_t width);
 KOEMI_API int koemi_core_layer_norm_backward(const void *values, int64_t rows, int64_t width, int64_t inner_rows,
                                              int64_t outer_stride, int64_t inner_stride, const void *weight,

@@ -662,6 +662,12 @@ constexpr int kTeamThreads = 256;  // a CTA of the kernels whose rows are shared
 constexpr int kMostPartials = 1024;  // partial rows of dw and db
 constexpr size_t kMostShared = 224 * 1024;
 
+// CTAs of a backward launch, each of which leaves a partial row. A thread holds at most 16 columns in 64 registers and
+// more, so an SM holds no more than 1024 threads' worth of rows.
+int64_t most_partials(int64_t rows, int64_t width) {
+    return std::min<int64_t>({rows, kMostPartials, sm_count() * std::max<int64_t>(1, 16 * 1024 / width)});
+}
+
 // How a row is held: packets of `wide` elements, `per_thread` of them a thread.
 struct Plan {
     bool warp, fits;
@@ -758,7 +764,7 @@ int launch_backward(const Plan &plan, NormRows a, const void *weight, bool wide,
     a.lanes = plan.lanes;
     const size_t shared = kWarp ? sizeof(float) * 2 * a.width : 0;
     const int64_t teams = plan.teams_of(a.rows);
-    *grid = std::min<int64_t>({teams, resident_of(kernel, plan.threads, shared), kMostPartials});
+    *grid = std::min<int64_t>({teams, resident_of(kernel, plan.threads, shared), most_partials(a.rows, a.width)});
     kernel<<<static_cast<unsigned>(*grid), plan.threads, shared, stream>>>(a, weight, wide, stats, static_cast<const T *>(g),
                                                                            static_cast<T *>(dx), partials);
     return KOEMI_OK;
@@ -777,7 +783,7 @@ int backward_wide(const NormRows &a, const void *weight, bool wide, const float 
                   int64_t *grid, cudaStream_t stream) {
     auto kernel = norm_backward_wide_kernel<T, K>;
     KOEMI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostShared)));
-    *grid = std::min<int64_t>(a.rows, sm_count());
+    *grid = std::min<int64_t>(sm_count(), most_partials(a.rows, a.width));
     kernel<<<static_cast<unsigned>(*grid), 1024, partials != nullptr ? sizeof(float) * 2 * a.width : 0, stream>>>(
         a, weight, wide, stats, static_cast<const T *>(g), static_cast<T *>(dx), partials);
     return KOEMI_OK;
@@ -802,7 +808,7 @@ int backward(const NormRows &a, const void *weight, bool wide, const float *stat
         }
         if (partials != nullptr) {
             const int64_t columns = ceil_div(a.width, 256);
-            grid = std::min<int64_t>({a.rows, std::max<int64_t>(1, 8 * sm_count() / columns), kMostPartials});
+            grid = std::min<int64_t>(std::max<int64_t>(1, 8 * sm_count() / columns), most_partials(a.rows, a.width));
             norm_columns_kernel<T><<<dim3(static_cast<unsigned>(columns), static_cast<unsigned>(grid)), 256, 0, stream>>>(
                 a, stats, static_cast<const T *>(g), partials);
         }
@@ -859,7 +865,7 @@ extern "C" int koemi_core_layer_norm_forward(const void *values, int64_t rows, i
 
 extern "C" size_t koemi_core_layer_norm_backward_workspace(int64_t rows, int64_t width) {
     if (rows < 1 || width < 1) return 0;
-    return static_cast<size_t>(std::min<int64_t>(rows, kMostPartials)) * 2 * width * sizeof(float);
+    return static_cast<size_t>(most_partials(rows, width)) * 2 * width * sizeof(float);
 }
 
 extern "C" int koemi_core_layer_norm_backward(const void *values, int64_t rows, int64_t width, int64_t inner_rows, int64_t outer_stride,

@@ -78,3 +78,16 @@ def test_block_workspace_is_what_the_pass_uses():
         for odd in ((300, 515, 1030, 515), (3, 515, 77, 33)):
             assert ask(*odd, dtype, 0) == ask(*odd, dtype, 4) and ask(*odd, dtype, 1) == ask(*odd, dtype, 1 | 4)
             assert 0 < ask(*odd, dtype, 2) <= ask(*odd, dtype, 0)
+
+
+def test_norm_workspace_holds_the_partial_rows_that_there_are():
+    """A wide row takes many threads, so an SM holds few CTAs, each with one partial row of dw and db: 8 an SM of 2048
+    columns, 1 an SM from 16384 on; never more than rows."""
+    ask = _native.library().koemi_core_layer_norm_backward_workspace
+    for width in (1, 128, 2000):
+        assert ask(1 << 20, width) == 1024 * 2 * width * 4
+    sms = ask(1 << 20, 1 << 20) // (2 * 4 << 20)
+    assert 1 <= sms <= 512
+    for width, each in ((4096, 4), (5000, 3), (8192, 2), (12000, 1), (16384, 1), (33000, 1)):
+        assert ask(1 << 20, width) == min(1024, each * sms) * 2 * width * 4
+        assert ask(7, width) == 7 * 2 * width * 4
