@@ -16,13 +16,14 @@
 // products of the backward need no transposed copy.
 //
 // fp32 values are split into three bf16 parts (8 bits each, together the 24 of
-// fp32), x = x0 + x1 + x2 with |x1| <= 2^-9 |x0|, |x2| <= 2^-18 |x0|, and a
+// fp32), x = x0 + x1 + x2 with |x1| <= 2^-8 |x0|, |x2| <= 2^-17 |x0|, and a
 // product is the six part products that matter, x0 y0, x0 y1, x1 y0, x1 y1, x0 y2
-// and x2 y0: x0 y0 in one accumulator, the others, 2^-9 of it and less, in a
+// and x2 y0: x0 y0 in one accumulator, the others, 2^-8 of it and less, in a
 // second one, where they are not cut off at the first one's last place. What is
-// left out is below 2^-26 of |x y|. Six bf16 products run several times faster
-// than fp32 FMAs. 16-bit operands whose rows TMA cannot describe (a width that is
-// no multiple of 8, a start off 16 bytes) are copied to padded rows first.
+// left out is about 2^-24 of |x y|, one rounding of fp32. Six bf16 products run
+// several times faster than fp32 FMAs. 16-bit operands whose rows TMA cannot
+// describe (a width that is no multiple of 8, a start off 16 bytes) are copied to
+// padded rows first.
 //
 // In 16 bits h, dp and dq are rounded to the type between two products, because
 // the tensor cores take no wider operand. a and b stay fp32: in 16 bits they

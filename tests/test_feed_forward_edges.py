@@ -91,3 +91,20 @@ def test_norm_workspace_holds_the_partial_rows_that_there_are():
     for width, each in ((4096, 4), (5000, 3), (8192, 2), (12000, 1), (16384, 1), (33000, 1)):
         assert ask(1 << 20, width) == min(1024, each * sms) * 2 * width * 4
         assert ask(7, width) == 7 * 2 * width * 4
+
+
+def test_three_bf16_parts_hold_an_fp32_value():
+    """Every fp32 value of a binade: the parts add up to it exactly, and the products of parts that the block leaves out,
+    x1 y2, x2 y1 and x2 y2, are one fp32 rounding of x y at most (the parts' bounds make it 2^-24 + 2^-34 of x0 y0)."""
+    x = torch.arange(1 << 23, dtype=torch.int32).add_(0x3F800000).view(torch.float32)
+    parts, rest = [], x
+    for _ in range(3):
+        parts.append(rest.bfloat16().float())
+        rest = rest - parts[-1]
+    assert not rest.any()
+    x0, x1, x2 = (t.double() for t in parts)
+    assert (x1 / x0).abs().max().item() == 2.0 ** -8 and (x2 / x0).abs().max().item() <= 2.0 ** -17
+    for order in (torch.arange(1 << 23), torch.randperm(1 << 23, generator=torch.Generator().manual_seed(0))):
+        y0, y1, y2 = x0[order], x1[order], x2[order]
+        left_out = ((x1 * y2 + x2 * y1 + x2 * y2) / (x.double() * x.double()[order])).abs().max().item()
+        assert left_out <= 1.01 * 2.0 ** -24
