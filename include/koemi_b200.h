@@ -865,7 +865,8 @@ KOEMI_API int koemi_core_dropout(const void *values, const void *residual, void 
  * fp32 sums; fp32 operands as three bf16 parts each, to fp32's precision (an
  * fp32 operand past 3.38e38 may give NaN). The forward of up to 8 rows in fp32
  * and 2 to 4 in 16 bits takes its products on the FMA units. 16-bit hidden values
- * are rounded to the type, so an fp16 one past 65504 is infinite. A call needs at most
+ * and their gradients are rounded to the type between the products: an fp16 value
+ * past 65504 is infinite, a gradient of one under 2^-25 is lost. A call needs at most
  * koemi_dense_gated_feed_forward_workspace bytes, on the device that is current
  * when they are asked for; workspace and kept start at multiples of 256 bytes.
  * pass: 0 the forward, or a sum of these. Without ALIGNED it counts copies of

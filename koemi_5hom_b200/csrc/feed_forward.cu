@@ -26,9 +26,14 @@
 // padded rows first.
 //
 // In 16 bits h, dp and dq are rounded to the type between two products, because
-// the tensor cores take no wider operand. a and b stay fp32: in 16 bits they
-// would cost the gradients two roundings more (bf16 3.1e-3 for 2.4e-3 of a
-// gradient's norm). All sums are fp32.
+// the tensor cores take no wider operand; an fp16 entry of dp or dq under 2^-14
+// loses digits by that and one under 2^-25 all of them. A result's error is that
+// of two roundings, 1.4 times that of one. The few rows' kernel, which could keep
+// h wider, rounds it alike, so that a row's result has the same roundings in
+// every batch and the backward, which reads that h, belongs to the y returned. The
+// biases' gradients sum the dp and dq whose products the weights' gradients are. a
+// and b stay fp32: in 16 bits they would cost the gradients two roundings more
+// (bf16 3.1e-3 for 2.4e-3 of a gradient's norm). All sums are fp32.
 //
 // Many rows are bound by the tensor cores: 32768 rows of 2048 -> 4096 -> 2048 in
 // bf16 take 805 us for the gate's products, 369 for y, 469 for dh with dp and dq,
@@ -553,8 +558,8 @@ __device__ __forceinline__ void finish_out(const Job &a, const Store &store, flo
 // accumulators, so a tile is finished while the next is multiplied. kCtas = 2: a pair of CTAs
 // computes 256 rows with one instruction; each loads its 128 rows of A and half
 // of B's columns, so an SM reads a third fewer bytes per product than with a
-// 128 x 256 tile of its own (32768 rows of 2048 -> 4096 -> 2048: 856 us for 923
-// of the gate's product). fp32: a K block is three stages, one a part, each
+// 128 x 256 tile of its own (32768 rows of 2048 -> 4096 -> 2048: 923 to 856 us of
+// the gate's product when pairs came in, 805 now). fp32: a K block is three stages, one a part, each
 // loaded once for all the products of its parts. Every wait is bounded; one that
 // gives up raises the CTA's abort flag and the status word, and all roles leave.
 template <typename T, int kEpilogue, int kTileN, int kCtas>
@@ -1117,7 +1122,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const __grid_constant__ F
             if (bias != nullptr) v[k] += to_acc(bias[unit]);
         }
         T *out = static_cast<T *>(args.out) + lane * args.ld_out + unit;
-        if constexpr (kEpilogue == kGate) {
+        if constexpr (kEpilogue == kGate) {  // h in the type, as the tensor cores' path rounds it
             const float s = sigmoid_of<T>(v[0]), a = v[0] * s;
             if (args.parts.base != nullptr) {
                 *(kept_at(args.a_kept, args.kept_blocks, lane, unit & ~7) + (unit & 7)) = a;

@@ -24,9 +24,11 @@ def layer_norm(values: Tensor, weight: Tensor, bias: Tensor | None = None, eps: 
 
     ``values`` is ``[..., width]`` (f32, bf16 or f16; rows of any stride);
     ``weight`` and ``bias`` are ``[width]``, both in the values' dtype or both
-    in fp32. Statistics and sums are fp32, the result has the values' dtype and
-    is rounded once. Differentiable to first order in all three; the gradients
-    of ``weight`` and ``bias`` are sums over all rows in a fixed order.
+    in fp32. Statistics and sums are fp32: a row whose sum, or whose sum of
+    squared distances from the mean, leaves fp32's range is not what the formula
+    gives. The result has the values' dtype and is rounded once. Differentiable
+    to first order in all three; the gradients of ``weight`` and ``bias`` are sums
+    over all rows in a fixed order.
     """
     if not _training.loaded():
         _validate(values, weight, bias, eps)

@@ -27,10 +27,11 @@ def gated_feed_forward(values: Tensor, gate_weight: Tensor, value_weight: Tensor
     ``values`` is ``[..., width]``, ``gate_weight`` and ``value_weight`` are
     ``[hidden, width]``, ``output_weight`` is ``[out, hidden]`` and the biases
     are ``[hidden]``, ``[hidden]``, ``[out]`` (zeros when omitted), all of one
-    dtype: f32, bf16 or f16. Sums are fp32. In 16 bits the hidden values are
-    rounded to the type between the products, so an fp16 one past 65504 is
-    infinite; fp32 products have fp32's precision, and an operand past 3.38e38 may
-    give NaN. Differentiable to first order in everything; a call that may be
+    dtype: f32, bf16 or f16. Sums are fp32. In 16 bits the hidden values and
+    their gradients are rounded to the type between the products: an fp16 hidden
+    value past 65504 is infinite, and what a gradient of one has under 2^-14 loses
+    digits, under 2^-25 everything, so scale an fp16 loss. fp32 products have fp32's
+    precision, and an operand past 3.38e38 may give NaN. Differentiable to first order in everything; a call that may be
     differentiated keeps the hidden values, silu of the gate and the slope that the
     gate's gradient takes, 10 bytes a hidden value in 16 bits and 14 in fp32.
     """
