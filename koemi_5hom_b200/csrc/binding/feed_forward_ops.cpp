@@ -144,6 +144,12 @@ Tensor dropout_cuda(const Tensor &values_, const OptionalTensor &residual_, cons
     return out;
 }
 
+// The operator without a residual, under a name of its own: a batch of gradients
+// of one call has that call's mask, so vmap may call this once for each.
+Tensor dropout_gradient_cuda(const Tensor &grad, const OptionalTensor &step, int64_t dropped, int64_t seed, int64_t site, int64_t step_number) {
+    return dropout_cuda(grad, OptionalTensor(), step, dropped, seed, site, step_number);
+}
+
 // Linear in both inputs: the gradient is the operator on the gradient, which
 // is recorded where a further order is asked for.
 struct DropoutBackward final : torch::autograd::Node {
@@ -154,10 +160,10 @@ struct DropoutBackward final : torch::autograd::Node {
         std::lock_guard<std::mutex> lock(mutex_);
         variable_list result(2);
         if (!grads[0].defined()) return result;
-        KOEMI_OP(dropout, decltype(dropout_cuda));
+        KOEMI_OP(dropout_gradient, decltype(dropout_gradient_cuda));
         if (task_should_compute_output(0)) {
             const OptionalTensor step_ = has_step ? OptionalTensor(step.unpack()) : OptionalTensor();
-            result[0] = dropout.call(grads[0], OptionalTensor(), step_, dropped, seed, site, step_number);
+            result[0] = dropout_gradient.call(grads[0], step_, dropped, seed, site, step_number);
         }
         if (task_should_compute_output(1)) result[1] = grads[0];
         return result;
@@ -169,27 +175,42 @@ struct DropoutBackward final : torch::autograd::Node {
     std::string name() const override { return "DropoutBackward"; }
 };
 
+// `out` recorded as dropout of `values` onto `residual`, where one of them is differentiated.
+Tensor dropped_out(Tensor out, const Tensor &values, const OptionalTensor &residual, const OptionalTensor &step, int64_t dropped, int64_t seed,
+                   int64_t site, int64_t step_number) {
+    if (!at::GradMode::is_enabled() || !(differentiates(values) || differentiates(residual))) return out;
+    auto node = node_of<DropoutBackward>(values, residual.value_or(Tensor()));
+    node->has_step = step.has_value() && step->defined();
+    if (node->has_step) node->step = SavedVariable(*step, false);
+    node->dropped = dropped;
+    node->seed = seed;
+    node->site = site;
+    node->step_number = step_number;
+    torch::autograd::set_history(out, node);
+    return out;
+}
+
 Tensor dropout_autograd(const Tensor &values, const OptionalTensor &residual, const OptionalTensor &step, int64_t dropped, int64_t seed,
                         int64_t site, int64_t step_number) {
     reverse_mode_only(values, residual);
-    const bool record = at::GradMode::is_enabled() && (differentiates(values) || differentiates(residual));
     Tensor out;
     {
         at::AutoDispatchBelowADInplaceOrView below;
         KOEMI_OP(dropout, decltype(dropout_cuda));
         out = dropout.call(values, residual, step, dropped, seed, site, step_number);
     }
-    if (record) {
-        auto node = node_of<DropoutBackward>(values, residual.value_or(Tensor()));
-        node->has_step = step.has_value() && step->defined();
-        if (node->has_step) node->step = SavedVariable(*step, false);
-        node->dropped = dropped;
-        node->seed = seed;
-        node->site = site;
-        node->step_number = step_number;
-        torch::autograd::set_history(out, node);
+    return dropped_out(out, values, residual, step, dropped, seed, site, step_number);
+}
+
+Tensor dropout_gradient_autograd(const Tensor &grad, const OptionalTensor &step, int64_t dropped, int64_t seed, int64_t site, int64_t step_number) {
+    reverse_mode_only(grad);
+    Tensor out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        KOEMI_OP(dropout_gradient, decltype(dropout_gradient_cuda));
+        out = dropout_gradient.call(grad, step, dropped, seed, site, step_number);
     }
-    return out;
+    return dropped_out(out, grad, OptionalTensor(), step, dropped, seed, site, step_number);
 }
 
 // vmap would call the operator once a sample, each time with the same positions and so the same mask.
@@ -376,6 +397,7 @@ TORCH_LIBRARY_FRAGMENT(koemi_b200, m) {
     m.def("layer_norm_keep(Tensor values, Tensor weight, Tensor? bias, float eps) -> (Tensor, Tensor)");
     m.def("layer_norm_backward(Tensor values, Tensor weight, Tensor stats, Tensor grad, bool[3] wanted) -> (Tensor, Tensor, Tensor)");
     m.def("dropout(Tensor values, Tensor? residual, Tensor? step, int dropped, int seed, int site, int step_number) -> Tensor");
+    m.def("dropout_gradient(Tensor grad, Tensor? step, int dropped, int seed, int site, int step_number) -> Tensor");
     m.def("gated_feed_forward(Tensor values, Tensor gate_weight, Tensor value_weight, Tensor output_weight, Tensor? gate_bias, Tensor? value_bias, Tensor? output_bias) -> Tensor");
     m.def("gated_feed_forward_keep(Tensor values, Tensor gate_weight, Tensor value_weight, Tensor output_weight, Tensor? gate_bias, Tensor? value_bias, Tensor? output_bias) -> (Tensor, Tensor)");
     m.def("gated_feed_forward_backward(Tensor values, Tensor gate_weight, Tensor value_weight, Tensor output_weight, Tensor kept, Tensor grad, int wanted) -> Tensor[]");
@@ -386,6 +408,7 @@ TORCH_LIBRARY_IMPL(koemi_b200, CUDA, m) {
     m.impl("layer_norm_keep", layer_norm_keep_cuda);
     m.impl("layer_norm_backward", layer_norm_backward_cuda);
     m.impl("dropout", dropout_cuda);
+    m.impl("dropout_gradient", dropout_gradient_cuda);
     m.impl("gated_feed_forward", gated_feed_forward_cuda);
     m.impl("gated_feed_forward_keep", gated_feed_forward_keep_cuda);
     m.impl("gated_feed_forward_backward", gated_feed_forward_backward_cuda);
@@ -396,6 +419,7 @@ TORCH_LIBRARY_IMPL(koemi_b200, FuncTorchBatched, m) { m.impl("dropout", dropout_
 TORCH_LIBRARY_IMPL(koemi_b200, Autograd, m) {
     m.impl("layer_norm", layer_norm_autograd);
     m.impl("dropout", dropout_autograd);
+    m.impl("dropout_gradient", dropout_gradient_autograd);
     m.impl("gated_feed_forward", gated_feed_forward_autograd);
     for (const char *inner : {"layer_norm_keep", "layer_norm_backward", "gated_feed_forward_keep", "gated_feed_forward_backward"}) {
         m.impl(inner, torch::autograd::autogradNotImplementedFallback());

@@ -122,6 +122,10 @@ def _register_fakes() -> None:
     def _(values, residual, step, dropped, seed, site, step_number):
         return values.new_empty(values.shape)
 
+    @fake("dropout_gradient")
+    def _(grad, step, dropped, seed, site, step_number):
+        return grad.new_empty(grad.shape)
+
     @fake("gated_feed_forward")
     def _(values, gate_weight, value_weight, output_weight, gate_bias, value_bias, output_bias):
         return values.new_empty((*values.shape[:-1], output_weight.shape[0]))

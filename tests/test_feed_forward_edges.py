@@ -108,3 +108,14 @@ def test_three_bf16_parts_hold_an_fp32_value():
         y0, y1, y2 = x0[order], x1[order], x2[order]
         left_out = ((x1 * y2 + x2 * y1 + x2 * y2) / (x.double() * x.double()[order])).abs().max().item()
         assert left_out <= 1.01 * 2.0 ** -24
+
+
+def test_dropout_has_batched_gradients():
+    """Rows of a Jacobian share the forward's mask: there vmap calls the gradient's operator, not dropout."""
+    _training.register()
+    x = torch.zeros(6, 16, device="meta", requires_grad=True)
+    drop = lambda t: torch.ops.koemi_b200.dropout(t, 2 * t, None, 6554, 1, 2, 3)  # noqa: E731
+    grad, = torch.autograd.grad(drop(x), x, torch.zeros(5, 6, 16, device="meta"), is_grads_batched=True)
+    assert grad.shape == (5, 6, 16)
+    assert torch.func.jacrev(drop)(x.detach()).shape == (6, 16, 6, 16)
+    assert torch.func.jacrev(torch.func.jacrev(lambda t: drop(t * t).sum()))(x.detach()[:1]).shape == (1, 16, 1, 16)

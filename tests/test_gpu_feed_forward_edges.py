@@ -292,3 +292,12 @@ def test_block_takes_no_memory_that_it_does_not_use(cuda):
     results, backward = peak(lambda: torch.autograd.grad(y, leaves, grad))
     ask = lambda bits: _native.library().koemi_dense_gated_feed_forward_workspace(rows, width, hidden, width, _native.BF16, bits)  # noqa: E731
     assert backward <= sum(2 * t.numel() for t in leaves) + ask(1 | 4) + 2 ** 20 and ask(1 | 4) <= ask(1) - 4 * rows * width
+
+
+def test_batched_gradients_of_dropout(cuda):
+    """A batch of gradients of one call: each has the call's mask."""
+    new = normal(cuda)
+    x, r, grads = new(40, 33).requires_grad_(True), new(40, 33).requires_grad_(True), new(5, 40, 33)
+    y = dropout(x, 0.4, seed=2, site=1, step=torch.tensor(9, device=cuda), residual=r)
+    dx, dr = torch.autograd.grad(y, (x, r), grads, is_grads_batched=True)
+    assert torch.equal(dx, torch.stack([dropout(g, 0.4, seed=2, site=1, step=9) for g in grads])) and torch.equal(dr, grads)
