@@ -300,8 +300,10 @@ std::tuple<Tensor, Tensor> gated_feed_forward_keep_cuda(const Tensor &values, co
 }
 
 // Gradients of values, gate_weight, value_weight, output_weight and the three
-// biases, bit k of `wanted` for the k-th; one that is not wanted is empty.
-std::vector<Tensor> gated_feed_forward_backward_cuda(const Tensor &values, const Tensor &gate_weight, const Tensor &value_weight,
+// biases, bit k of `wanted` for the k-th; one that is not wanted is empty. A
+// tuple: vmap, which calls this once a sample, takes no list.
+using BlockGradients = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
+BlockGradients gated_feed_forward_backward_cuda(const Tensor &values, const Tensor &gate_weight, const Tensor &value_weight,
                                                      const Tensor &output_weight, const Tensor &kept, const Tensor &grad, int64_t wanted) {
     const OptionalTensor none;
     const BlockShape s(values, gate_weight, value_weight, output_weight, none, none, none);
@@ -312,12 +314,12 @@ std::vector<Tensor> gated_feed_forward_backward_cuda(const Tensor &values, const
                           kept.numel() >= static_cast<int64_t>(lib().block_kept(s.rows, s.hidden, code)),
                       "kept is not what the forward of these values returned");
     const std::vector<int64_t> sizes[] = {{s.rows, s.width}, {s.hidden, s.width}, {s.hidden, s.width}, {s.out, s.hidden}, {s.hidden}, {s.hidden}, {s.out}};
-    std::vector<Tensor> grads;
+    std::array<Tensor, 7> grads;
     void *p[7];
     for (int k = 0; k < 7; ++k) {
         const bool want = wanted >> k & 1;
-        grads.push_back(want ? at::empty(sizes[k], values.options()) : at::empty({0}, values.options()));
-        p[k] = want ? address<void>(grads.back()) : nullptr;
+        grads[k] = want ? at::empty(sizes[k], values.options()) : at::empty({0}, values.options());
+        p[k] = want ? address<void>(grads[k]) : nullptr;
     }
     const int pass = aligned_pass(s.stride, {&values, &gate_weight, &value_weight, &output_weight, &grad}) | KOEMI_FEED_FORWARD_BACKWARD;
     Tensor workspace = bytes_of(values, lib().block_workspace(s.rows, s.width, s.hidden, s.out, code, pass));
@@ -326,7 +328,7 @@ std::vector<Tensor> gated_feed_forward_backward_cuda(const Tensor &values, const
                                address<void>(output_weight), address<void>(kept), kept.numel(), address<void>(grad), p[0], p[1], p[2],
                                p[3], p[4], p[5], p[6], s.rows, s.width, s.hidden, s.out, code, address<void>(workspace),
                                workspace.numel(), launch.stream));
-    return grads;
+    return std::tuple_cat(grads);
 }
 
 struct GatedFeedForwardBackward final : torch::autograd::Node {
@@ -342,7 +344,9 @@ struct GatedFeedForwardBackward final : torch::autograd::Node {
         int64_t wanted = 0;
         for (int k = 0; k < 7; ++k) wanted |= static_cast<int64_t>(task_should_compute_output(k)) << k;
         KOEMI_OP(gated_feed_forward_backward, decltype(gated_feed_forward_backward_cuda));
-        auto found = gated_feed_forward_backward.call(values_, gate, value, output, kept_, grads[0].contiguous(), wanted);
+        std::array<Tensor, 7> found;
+        std::tie(found[0], found[1], found[2], found[3], found[4], found[5], found[6]) =
+            gated_feed_forward_backward.call(values_, gate, value, output, kept_, grads[0].contiguous(), wanted);
         for (int k = 0; k < 7; ++k) {
             if (wanted >> k & 1) result[k] = found[k];
         }
@@ -400,7 +404,7 @@ TORCH_LIBRARY_FRAGMENT(koemi_b200, m) {
     m.def("dropout_gradient(Tensor grad, Tensor? step, int dropped, int seed, int site, int step_number) -> Tensor");
     m.def("gated_feed_forward(Tensor values, Tensor gate_weight, Tensor value_weight, Tensor output_weight, Tensor? gate_bias, Tensor? value_bias, Tensor? output_bias) -> Tensor");
     m.def("gated_feed_forward_keep(Tensor values, Tensor gate_weight, Tensor value_weight, Tensor output_weight, Tensor? gate_bias, Tensor? value_bias, Tensor? output_bias) -> (Tensor, Tensor)");
-    m.def("gated_feed_forward_backward(Tensor values, Tensor gate_weight, Tensor value_weight, Tensor output_weight, Tensor kept, Tensor grad, int wanted) -> Tensor[]");
+    m.def("gated_feed_forward_backward(Tensor values, Tensor gate_weight, Tensor value_weight, Tensor output_weight, Tensor kept, Tensor grad, int wanted) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(koemi_b200, CUDA, m) {

@@ -139,4 +139,4 @@ def _register_fakes() -> None:
     def _(values, gate_weight, value_weight, output_weight, kept, grad, wanted):
         hidden, out = gate_weight.shape[:1], output_weight.shape[:1]
         shapes = (values.shape, gate_weight.shape, gate_weight.shape, output_weight.shape, hidden, hidden, out)
-        return [values.new_empty(shape if wanted >> k & 1 else (0,)) for k, shape in enumerate(shapes)]
+        return tuple(values.new_empty(shape if wanted >> k & 1 else (0,)) for k, shape in enumerate(shapes))

@@ -119,3 +119,13 @@ def test_dropout_has_batched_gradients():
     assert grad.shape == (5, 6, 16)
     assert torch.func.jacrev(drop)(x.detach()).shape == (6, 16, 6, 16)
     assert torch.func.jacrev(torch.func.jacrev(lambda t: drop(t * t).sum()))(x.detach()[:1]).shape == (1, 16, 1, 16)
+
+
+@pytest.mark.parametrize("call", [lambda x: torch.ops.koemi_b200.layer_norm(x, x[0].detach() + 1, x[0], 1e-5),
+                                  lambda x: torch.ops.koemi_b200.gated_feed_forward(x, x[:1].expand(8, 16), x[1:2].expand(8, 16), x[:4, :8], None, None, x[1, :4])])
+def test_norm_and_block_have_batched_gradients(call):
+    _training.register()
+    x = torch.zeros(6, 16, device="meta", requires_grad=True)
+    y = call(x)
+    grad, = torch.autograd.grad(y, x, torch.zeros(5, *y.shape, device="meta"), is_grads_batched=True)
+    assert grad.shape == (5, 6, 16) and torch.func.jacrev(call)(x.detach()).shape == (*y.shape, 6, 16)

@@ -301,3 +301,16 @@ def test_batched_gradients_of_dropout(cuda):
     y = dropout(x, 0.4, seed=2, site=1, step=torch.tensor(9, device=cuda), residual=r)
     dx, dr = torch.autograd.grad(y, (x, r), grads, is_grads_batched=True)
     assert torch.equal(dx, torch.stack([dropout(g, 0.4, seed=2, site=1, step=9) for g in grads])) and torch.equal(dr, grads)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_of_each_sample(dtype, cuda):
+    """vmap of the norm's and the block's gradients: those of calls alone."""
+    new = normal(cuda)
+    x, nw = new(5, 40, 64, dtype=dtype), new(64, dtype=dtype)
+    wg, wv, wo = new(48, 64, dtype=dtype), new(48, 64, dtype=dtype), new(64, 48, dtype=dtype)
+    value = lambda t, nw, wg, wo: gated_feed_forward(layer_norm(t, nw), wg, wv, wo).float().square().sum()  # noqa: E731
+    each = torch.func.grad(value, argnums=(0, 1, 2, 3))
+    got = torch.vmap(each, in_dims=(0, None, None, None))(x, nw, wg, wo)
+    for a, b in zip(got, zip(*(each(t, nw, wg, wo) for t in x))):
+        assert torch.equal(a, torch.stack(b))
