@@ -175,6 +175,14 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+// The finaliser of Steele, Lea and Flood's SplitMix (OOPSLA 2014): the sampler's and dropout's generator.
+__host__ __device__ __forceinline__ uint64_t splitmix64(uint64_t z) {
+    z += 0x9E3779B97F4A7C15ull;
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    return z ^ (z >> 31);
+}
+
 // Spin budget of every bounded wait: about a second or more at B200 clocks
 // before the waiting thread records KOEMI_ERR_TIMEOUT and gives up.
 constexpr uint32_t kWaitSpinLimit = 1u << 24;

@@ -20,13 +20,6 @@
 namespace koemi {
 namespace {
 
-__device__ __forceinline__ uint64_t splitmix64(uint64_t z) {
-    z += 0x9E3779B97F4A7C15ull;
-    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-    return z ^ (z >> 31);
-}
-
 struct Numbers {
     uint64_t seed, site, step;
     const int64_t *step_device;  // taken in place of `step` where it is given

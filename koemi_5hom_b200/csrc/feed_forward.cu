@@ -434,19 +434,6 @@ __device__ __forceinline__ float sigmoid_of(float p) {
     }
 }
 
-// Two fp32 operations an instruction.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)),
-        "l"(reinterpret_cast<uint64_t &>(c)));
-    return r;
-}
-
 template <int kWide, typename T>
 __device__ __forceinline__ void add_bias(const void *bias, int64_t column, int64_t left, float (&v)[kWide]) {
     if (bias == nullptr) return;

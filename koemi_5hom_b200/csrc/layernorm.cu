@@ -121,24 +121,8 @@ __device__ __forceinline__ void load_weights(const void *w, bool wide, int c, fl
     }
 }
 
-// Two fp32 operations an instruction: these kernels are bound by issue slots
-// before they are bound by bytes.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)),
-        "l"(reinterpret_cast<uint64_t &>(c)));
-    return r;
-}
+// Pairs of fp32 values (vec.cuh): these kernels are bound by issue slots before
+// they are bound by bytes.
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // A thread's K packets of W elements as pairs.

@@ -92,13 +92,6 @@ __global__ __launch_bounds__(kSamplerThreads) void greedy_kernel(const float *__
 // The PAD column, NaN logits and (with `thresholds`) logits below the row's
 // threshold are never chosen; ties go to the lower index.
 
-__host__ __device__ __forceinline__ uint64_t splitmix64(uint64_t z) {
-    z += 0x9E3779B97F4A7C15ull;
-    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-    return z ^ (z >> 31);
-}
-
 __device__ __forceinline__ void take_sample(Best &best, float logit, int64_t i, int64_t pad, float inv_t,
                                             float threshold, uint64_t key) {
     if (i == pad || isnan(logit) || logit < threshold) return;

@@ -73,4 +73,22 @@ __device__ __forceinline__ uint4 load_cached(const void *p) {
 // load-after-store of a loop into one L2 round trip per iteration.
 __device__ __forceinline__ void store_stream(void *p, const uint4 &v) { *reinterpret_cast<uint4 *>(p) = v; }
 
+// Two fp32 operations an instruction, rounded as the single ones.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t &>(r)) : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)),
+        "l"(reinterpret_cast<uint64_t &>(c)));
+    return r;
+}
+
 }  // namespace koemi
